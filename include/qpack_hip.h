@@ -28,7 +28,7 @@ typedef struct qph_model qph_model;
 
 /* tensor kinds (the QPACK2 kinds the Llama path reads, /root/reference/QPACK2.md table; the kinds LlamaCuda uploads,
  * src/model_llama_cuda.cu:549-556) */
-enum { QPH_F32 = 0, QPH_Q8 = 1, QPH_Q4 = 2, QPH_Q1 = 3 };
+enum { QPH_F32 = 0, QPH_Q8 = 1, QPH_Q4 = 2, QPH_Q1 = 3, QPH_F16 = 4, QPH_BF16 = 5 };   /* F16, BF16: rows of the kv entry points only */
 
 /* Model config: the config.json keys read by the reference (/root/reference/src/model_llama.cpp:21-27). */
 typedef struct {
@@ -177,6 +177,52 @@ int qph_kernel_rans_decode(const uint8_t *blob, int64_t len, uint8_t *out, int64
  * f16 / f32 blob rANS-coded (16 MiB chunks above 32 MiB) where that makes it smaller; *coded = blobs coded.  Host only
  * (the writer of the coded files the loader decodes on the GPU). */
 int qph_pack(const char *src, const char *dst, int threads, int *coded);
+
+/* ---- key / value caches of several sequences (no counterpart in the reference, whose models hold one fp16 cache each).
+ * For servers that keep their own caches and batch sequences.  Every pointer is a device pointer, every call is enqueued on
+ * `stream` (a hipStream_t of the current device; NULL = the null stream) and not waited for, allocates nothing and keeps
+ * nothing between calls, so calls can be captured into a graph (which then reads pos and lens anew at every replay).
+ *
+ * QPH_F16: k and v point to fp16 rows; sequence b, position p, head h at b * seq + p * row + h * head_dim elements (0 for
+ * seq or row: [nseq][ctx][kv_heads][head_dim] without gaps); 16-byte aligned, strides multiples of 8.
+ * QPH_Q4: k points to qph_kv_bytes bytes (16-byte aligned), v, seq and row unused: per sequence, kv head and 8 positions one record of 9
+ * head_dim bytes.  32 dims of one position share a scale: a = max |x| of them, s = fp16(bf16(min(a, 65504) / 7)), code =
+ * clamp(rint(x / s), -7, 7) + 8 (8 when s is 0), value = (code - 8) * s, which fp16 holds exactly; a group with a NaN or
+ * an infinity has a NaN scale.  In a record:
+ *   K codes  position i at bytes i head_dim / 2; its 32-bit word w holds dims 8 w .. 8 w + 7, dim 8 w + 2 e + o at bits 16 o + 4 e
+ *   V codes  at 4 head_dim: dim d in word (d % 16) (head_dim / 16) + d / 16, position 2 e + o at bits 16 o + 4 e
+ *   K scales at 8 head_dim: fp16 [8 positions][head_dim / 32];  V scales at 8.5 head_dim: fp16 [head_dim / 32][8 positions]
+ * Memory that was never written may hold anything: no position that a token does not see changes its result. */
+typedef struct {
+  int kind;                            /* QPH_F16 or QPH_Q4 */
+  int nseq, kv_heads, head_dim;        /* head_dim 64 or 128; nseq <= 65535, kv_heads <= 4096 */
+  int64_t ctx;                         /* positions of a sequence, <= 2^30 */
+  void *k, *v;
+  int64_t seq, row;
+} qph_kv;
+/* rows of tokens: sequence b, token t, head h at p + b * seq + t * tok + h * head elements of type (QPH_F32, QPH_F16 or
+ * QPH_BF16), head_dim consecutive ones.  Any alignment of the type; 16-byte aligned pointers and strides are faster */
+typedef struct {
+  void *p;
+  int type;
+  int64_t seq, tok, head;
+} qph_rows;
+/* bytes of a QPH_Q4 cache, or of K and V together of a QPH_F16 one without gaps */
+int qph_kv_bytes(int kind, int nseq, int kv_heads, int head_dim, int64_t ctx, int64_t *bytes);
+/* Token t of sequence b, t < min(n, lens[b]) (lens NULL: t < n), is position pos[b] + t; sequences with pos[b] < 0 and
+ * positions at or past ctx take no part: nothing of them is read or written.  n <= 2^20.
+ * qph_kv_write rounds k and v (one type) into the cache; what else the cache holds stays.  qph_kv_read returns what it holds, rounded to the
+ * rows' type (fp16 and fp32: exact). */
+int qph_kv_write(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, const int *pos, const int *lens, void *stream);
+int qph_kv_read(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, const int *pos, const int *lens, void *stream);
+/* out = softmax(scale * q K^T) V for the tokens at pos[b] + t, whose rows are in the cache: position P sees p <= P and, with window > 0,
+ * of those only p > P - window and p < sinks.  heads a multiple of kv_heads (head h reads kv head h / (heads / kv_heads)), n * heads <=
+ * 2^28; scale 0: 1 / sqrt(head_dim), else > 0.  out has q's type and may be q.  work: qph_kv_attention_work bytes of scratch
+ * (16-byte aligned; NULL if 0) that no other call uses meanwhile - two graphs that may run at once need one each.  fp32 queries are computed to
+ * about 22 bits, fp16 and bf16 ones to the 11 of an fp16 operand, all sums in fp32. */
+int qph_kv_attention_work(const qph_kv *c, int type, int heads, int n, int window, int sinks, int64_t *bytes);
+int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, int heads, int n, const int *pos, const int *lens,
+                     int window, int sinks, float scale, void *work, int64_t work_bytes, void *stream);
 
 /* ---- synthetic models (no reference counterpart: the reference's files come from convert_llama.py / qpack-quantize).
  * Writes a seeded random-init Llama-family QPACK2 file; see qpack_amd/csrc/host/synth.cpp for the exact rules. */

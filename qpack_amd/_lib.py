@@ -9,7 +9,7 @@ import os
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "libqpack_hip.so")
 
-QPH_F32, QPH_Q8, QPH_Q4, QPH_Q1 = 0, 1, 2, 3
+QPH_F32, QPH_Q8, QPH_Q4, QPH_Q1, QPH_F16, QPH_BF16 = 0, 1, 2, 3, 4, 5
 
 
 class QphError(RuntimeError):
@@ -38,6 +38,15 @@ class SynthSpecC(C.Structure):
                 ("q4", C.c_int), ("q4m_alt", C.c_int), ("rms_eps", C.c_float), ("rope_theta", C.c_double), ("std", C.c_float),
                 ("seed", C.c_uint64), ("model_type", C.c_char * 32), ("more_bits", C.c_int), ("q4_head", C.c_int),
                 ("mlp_q1", C.c_int)]
+
+
+class KvC(C.Structure):
+    _fields_ = [("kind", C.c_int), ("nseq", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("ctx", C.c_int64),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("seq", C.c_int64), ("row", C.c_int64)]
+
+
+class RowsC(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("type", C.c_int), ("seq", C.c_int64), ("tok", C.c_int64), ("head", C.c_int64)]
 
 
 _P = C.c_void_p
@@ -81,6 +90,11 @@ SIGNATURES = {
     "qph_topk_noalloc": (_I, [_P, _I, _I, _P, _P, _P]),
     "qph_synth_write": (_I, [C.POINTER(SynthSpecC), C.c_char_p, _I]),
     "qph_load_stats_of": (_I, [C.c_void_p, C.POINTER(LoadStatsC)]),
+    "qph_kv_bytes": (_I, [_I, _I, _I, _I, C.c_int64, C.POINTER(C.c_int64)]),
+    "qph_kv_write": (_I, [_P, _P, _P, _I, _P, _P, _P]),
+    "qph_kv_read": (_I, [_P, _P, _P, _I, _P, _P, _P]),
+    "qph_kv_attention_work": (_I, [_P, _I, _I, _I, _I, _I, C.POINTER(C.c_int64)]),
+    "qph_kv_attention": (_I, [_P, _P, _P, _I, _I, _P, _P, _I, _I, C.c_float, _P, C.c_int64, _P]),
     "qph_kernel_rans_decode": (_I, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.POINTER(C.c_int64), _FP]),
     "qph_pack": (_I, [C.c_char_p, C.c_char_p, _I, _IP]),
 }

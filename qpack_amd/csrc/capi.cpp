@@ -2,6 +2,7 @@
 // and turns it into status -1 plus a thread-local message, so no exception crosses the C boundary.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <stdexcept>
@@ -35,6 +36,62 @@ static thread_local std::string g_err;
 
 static void need(const void *p, const char *what) {
   if (!p) throw std::invalid_argument(std::string(what) + " is NULL");
+}
+// ---- the kv entry points' arguments
+static int kv_kind(const qph_kv *c) { return c->kind == QPH_Q4 ? qph::MK_Q4 : qph::MK_F32; }
+static void kv_check(int kind, int nseq, int kv_heads, int head_dim, int64_t ctx) {
+  if (kind != QPH_F16 && kind != QPH_Q4) throw std::invalid_argument("kv: kind must be QPH_F16 or QPH_Q4");
+  if (nseq < 1 || nseq > 65535 || kv_heads < 1 || kv_heads > 4096) throw std::invalid_argument("kv: nseq must be in [1, 65535] and kv_heads in [1, 4096]");
+  if (head_dim != 64 && head_dim != 128) throw std::invalid_argument("kv: head_dim must be 64 or 128");
+  if (ctx < 1 || ctx > (int64_t)1 << 30) throw std::invalid_argument("kv: ctx must be in [1, 2^30]");
+}
+// the cache's strides
+static void kv_cache(const qph_kv *c, int64_t *seq, int64_t *row) {
+  need(c, "cache");
+  kv_check(c->kind, c->nseq, c->kv_heads, c->head_dim, c->ctx);
+  need(c->k, "cache k");
+  *seq = *row = 0;
+  if ((uintptr_t)c->k % 16) throw std::invalid_argument("kv: the cache must be 16-byte aligned");
+  if (c->kind == QPH_Q4) return;
+  need(c->v, "cache v");
+  const int64_t d = (int64_t)c->kv_heads * c->head_dim;
+  *row = c->row ? c->row : d;
+  *seq = c->seq ? c->seq : c->ctx * *row;
+  if ((uintptr_t)c->v % 16 || *row % 8 || *seq % 8) throw std::invalid_argument("kv: an fp16 cache must be 16-byte aligned and its strides multiples of 8");
+  if (*row < d || (c->nseq > 1 && *seq < (c->ctx - 1) * *row + d)) throw std::invalid_argument("kv: the cache's rows or sequences overlap");
+}
+static qph::KvRows kv_rows(const qph_rows *r, const char *what, bool out, int nseq, int n, int heads, int hd) {
+  need(r, what); need(r->p, what);
+  if (r->type != QPH_F32 && r->type != QPH_F16 && r->type != QPH_BF16) throw std::invalid_argument(std::string("kv: the type of ") + what + " must be QPH_F32, QPH_F16 or QPH_BF16");
+  if ((uintptr_t)r->p % (r->type == QPH_F32 ? 4 : 2)) throw std::invalid_argument(std::string("kv: ") + what + " is not aligned to its type");
+  if (r->seq < 0 || r->tok < 0 || r->head < 0) throw std::invalid_argument(std::string("kv: negative strides of ") + what);
+  if (out && ((nseq > 1 && r->seq < hd) || (n > 1 && r->tok < hd) || (heads > 1 && r->head < hd))) throw std::invalid_argument(std::string("kv: the rows of ") + what + " overlap");
+  return {r->p, r->type == QPH_F32 ? qph::RT_F32 : r->type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16, r->seq, r->tok, r->head};
+}
+static bool kv_vec(const qph::KvRows &r) {
+  const int e = r.type == qph::RT_F32 ? 4 : 8;
+  return (uintptr_t)r.p % 16 == 0 && r.seq % e == 0 && r.tok % e == 0 && r.head % e == 0;
+}
+static qph::KvIoArgs kv_io(const qph_kv *c, const qph_rows *k, const qph_rows *v, bool out, int n, const int *pos, const int *lens) {
+  qph::KvIoArgs a{};
+  kv_cache(c, &a.cseq, &a.crow);
+  if (n < 0 || n > 1 << 20) throw std::invalid_argument("kv: n must be in [0, 2^20]");
+  need(pos, "pos");
+  a.cache = c->k; a.cache_v = c->v; a.ctx = c->ctx; a.nrec = qph::kv4_records(c->ctx);
+  a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.n = n; a.pos = pos; a.lens = lens;
+  a.k = kv_rows(k, "k", out, c->nseq, n, c->kv_heads, c->head_dim); a.v = kv_rows(v, "v", out, c->nseq, n, c->kv_heads, c->head_dim);
+  if (a.k.type != a.v.type) throw std::invalid_argument("kv: k and v must have the same type");
+  a.vec = kv_vec(a.k) && kv_vec(a.v);
+  return a;
+}
+static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sinks, qph::KvAttnArgs &a) {
+  kv_cache(c, &a.cseq, &a.crow);
+  if (heads < 1 || heads % c->kv_heads) throw std::invalid_argument("kv: heads must be a positive multiple of kv_heads");
+  if (n < 0 || n > 1 << 20 || (int64_t)n * heads > 1 << 28 || heads > 65535) throw std::invalid_argument("kv: n must be in [0, 2^20], heads <= 65535 and n * heads <= 2^28");
+  if (window < 0 || sinks < 0) throw std::invalid_argument("kv: window and sinks must not be negative");
+  a.cache = c->k; a.cache_v = c->v; a.ctx = c->ctx; a.nrec = qph::kv4_records(c->ctx);
+  a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.heads = heads; a.rep = heads / c->kv_heads; a.n = n;
+  a.window = window; a.sinks = sinks;
 }
 static void hck(hipError_t e, const char *what) {
   if (e != hipSuccess) throw std::runtime_error(std::string("hip: ") + hipGetErrorString(e) + " (" + what + ")");
@@ -338,6 +395,56 @@ int qph_kernel_matmul_ref(int kind, const void *q, const void *scale, int rows, 
       hck(hipMemcpy(Y, dy, 4ull * B * rows, hipMemcpyDeviceToHost), "download Y");
     } catch (...) { for (void *p : bufs) (void)hipFree(p); throw; }
     for (void *p : bufs) (void)hipFree(p);
+  });
+}
+
+int qph_kv_bytes(int kind, int nseq, int kv_heads, int head_dim, int64_t ctx, int64_t *bytes) {
+  QPH_API_TRY({
+    need(bytes, "bytes");
+    kv_check(kind, nseq, kv_heads, head_dim, ctx);
+    *bytes = kind == QPH_Q4 ? qph::kv4_bytes(nseq, kv_heads, head_dim, ctx) : 4 * nseq * ctx * kv_heads * head_dim;
+  });
+}
+int qph_kv_write(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, const int *pos, const int *lens, void *stream) {
+  QPH_API_TRY({
+    const qph::KvIoArgs a = kv_io(c, k, v, false, n, pos, lens);
+    if (n) hck(qph::launch_kv_write(kv_kind(c), a, (hipStream_t)stream), "kv write");
+  });
+}
+int qph_kv_read(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, const int *pos, const int *lens, void *stream) {
+  QPH_API_TRY({
+    const qph::KvIoArgs a = kv_io(c, k, v, true, n, pos, lens);
+    if (n) hck(qph::launch_kv_read(kv_kind(c), a, (hipStream_t)stream), "kv read");
+  });
+}
+int qph_kv_attention_work(const qph_kv *c, int type, int heads, int n, int window, int sinks, int64_t *bytes) {
+  QPH_API_TRY({
+    need(bytes, "bytes");
+    if (type != QPH_F32 && type != QPH_F16 && type != QPH_BF16) throw std::invalid_argument("kv: the type of q must be QPH_F32, QPH_F16 or QPH_BF16");
+    qph::KvAttnArgs a{};
+    kv_attn_args(c, heads, n, window, sinks, a);
+    a.q.type = type == QPH_F32 ? qph::RT_F32 : type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16;
+    *bytes = n ? (int64_t)qph::kv_attn_plan(a) : 0;
+  });
+}
+int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, int heads, int n, const int *pos, const int *lens,
+                     int window, int sinks, float scale, void *work, int64_t work_bytes, void *stream) {
+  QPH_API_TRY({
+    qph::KvAttnArgs a{};
+    kv_attn_args(c, heads, n, window, sinks, a);
+    need(pos, "pos");
+    a.q = kv_rows(q, "q", false, c->nseq, n, heads, c->head_dim); a.out = kv_rows(out, "out", true, c->nseq, n, heads, c->head_dim);
+    if (a.q.type != a.out.type) throw std::invalid_argument("kv: q and out must have the same type");
+    if (!(scale >= 0.f) || std::isinf(scale)) throw std::invalid_argument("kv: scale must be finite and not negative (0: 1 / sqrt(head_dim))");
+    a.vec_q = kv_vec(a.q); a.vec_o = kv_vec(a.out);
+    a.pos = pos; a.lens = lens;
+    a.scale2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim));
+    if (n) {
+      const int64_t bytes = (int64_t)qph::kv_attn_plan(a);
+      if (bytes && (!work || work_bytes < bytes || (uintptr_t)work % 16)) throw std::invalid_argument("kv: work must have the " + std::to_string(bytes) + " bytes that qph_kv_attention_work gives, 16-byte aligned");
+      a.part = (float *)work;
+      hck(qph::launch_kv_attn(kv_kind(c), a, (hipStream_t)stream), "kv attention");
+    }
   });
 }
 

@@ -1,0 +1,972 @@
+// Key / value caches of several sequences, in fp16 or in 4 bits: writing rows, reading them back, and the attention of new
+// tokens over them, all positions or a sliding window with a few first positions that stay visible.
+//
+// The 4-bit cache.  Each 32 dims of one position's K (V) row share an fp16 scale s: a = max |x|, s = fp16(bf16(min(a, 65504)
+// / 7)), code = clamp(rint(x / s), -7, 7) + 8.  s has 8 significant bits and code - 8 three, so every value (code - 8) s is an
+// fp16 number: the matrix cores' operands, the rows read back and an fp16 snapshot are exact, and a row read back and
+// written again gives the same values.  Rounding s to 8 bits costs at most 2^-9 of it, the codes' step is 2^-3.  A
+// group that holds a NaN or an infinity has a NaN scale and reads back as NaN.
+//
+// One record of 9 HD bytes holds 8 positions of one (sequence, kv head); records follow each other in position order:
+//   [0, 4 HD)         K codes: position i at i HD / 2, a row's 32-bit word w = dims 8 w ..: dim 8 w + 2 e + o at bits 16 o + 4 e
+//   [4 HD, 8 HD)      V codes: dim d's word (d % 16) (HD / 16) + d / 16: position 2 e + o at bits 16 o + 4 e
+//   [8 HD, 8.5 HD)    K scales [8 positions][HD / 32]
+//   [8.5 HD, 9 HD)    V scales [HD / 32][8 positions]
+// K words run along the dims and V words along the positions because the matrix cores sum K q over dims and P V over
+// positions: a lane's word is its fragment, four (mask, or, subtract, multiply) pairs away, with no transposition and no LDS
+// on the decode path.  A single stream of records per head keeps a tile of 32 positions in 4.5 KiB of consecutive bytes.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "launch.hpp"
+
+namespace qph {
+
+namespace {
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+constexpr int kRec = 8;   // positions of a record
+
+__device__ __forceinline__ float bf16_to_f(uint16_t h) { return __builtin_bit_cast(float, (uint32_t)h << 16); }
+// round to nearest even; NaN stays NaN
+__device__ __forceinline__ uint16_t f_to_bf16(float f) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)(u >> 16 | 0x40);
+  return (uint16_t)((u + 0x7fff + (u >> 16 & 1)) >> 16);
+}
+
+// N (a multiple of 4) consecutive elements from element offset `at` of rows of a type; vec: 16-byte loads (the pointer and
+// the strides are multiples of 16 bytes, and so is every offset that the kernels ask for)
+template <int N>
+__device__ __forceinline__ void load_elems(const KvRows &r, int64_t at, bool vec, float *x) {
+  if (r.type == RT_F32) {
+    const float *p = (const float *)r.p + at;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) { const f32x4 v = *(const f32x4 *)(p + i); x[i] = v[0]; x[i + 1] = v[1]; x[i + 2] = v[2]; x[i + 3] = v[3]; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = p[i];
+    }
+    return;
+  }
+  const uint16_t *p = (const uint16_t *)r.p + at;
+  uint16_t h[N];
+  if (vec && N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+      const u32x4 v = *(const u32x4 *)(p + i);
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[i + j] = (uint16_t)(v[j / 2] >> 16 * (j & 1));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) x[i] = r.type == RT_F16 ? half_bits_to_float(h[i]) : bf16_to_f(h[i]);
+}
+__device__ __forceinline__ uint16_t to_elem16(int type, float f) { return type == RT_F16 ? float_to_half_bits(f) : f_to_bf16(f); }
+template <int N>
+__device__ __forceinline__ void store_elems(const KvRows &r, int64_t at, bool vec, const float *x) {
+  if (r.type == RT_F32) {
+    float *p = (float *)r.p + at;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *(f32x4 *)(p + i) = (f32x4){x[i], x[i + 1], x[i + 2], x[i + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) p[i] = x[i];
+    }
+    return;
+  }
+  uint16_t *p = (uint16_t *)r.p + at;
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint32_t a = to_elem16(r.type, x[i]) | (uint32_t)to_elem16(r.type, x[i + 1]) << 16;
+      const uint32_t b = to_elem16(r.type, x[i + 2]) | (uint32_t)to_elem16(r.type, x[i + 3]) << 16;
+      *(u32x2 *)(p + i) = (u32x2){a, b};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = to_elem16(r.type, x[i]);
+  }
+}
+
+// bit position of element i (0 .. 7) of a word of codes
+__host__ __device__ constexpr int nib(int i) { return 16 * (i & 1) + 4 * (i >> 1); }
+
+// a word's 8 values in element order.  Codes 0 .. 15 in the low mantissa bits of fp16 1024 (or, four bits higher, 16 times
+// them, brought back by an exact fma): c - 8 exact, times the elements' scales exact
+__device__ __forceinline__ h2 code_pair(uint32_t w, int e) {
+  const h2 k1032 = {(_Float16)1032.f, (_Float16)1032.f}, k16 = {(_Float16)0.0625f, (_Float16)0.0625f}, k72 = {(_Float16)-72.f, (_Float16)-72.f};
+  if (e & 1) {
+    const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x00f000f0u) | 0x64006400u);
+    return __builtin_elementwise_fma(x, k16, k72);
+  }
+  const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x000f000fu) | 0x64006400u);
+  return x - k1032;
+}
+// scales of the four element pairs: one for all (K: a group of dims), or the positions' own (V)
+__device__ __forceinline__ h8 values(uint32_t w, h2 s0, h2 s1, h2 s2, h2 s3) {
+  const h2 a = code_pair(w, 0) * s0, b = code_pair(w, 1) * s1, c = code_pair(w, 2) * s2, d = code_pair(w, 3) * s3;
+  return (h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ h8 values(uint32_t w, uint16_t s) {
+  const h2 x = __builtin_bit_cast(h2, (uint32_t)s * 0x10001u);
+  return values(w, x, x, x, x);
+}
+__device__ __forceinline__ h8 values(uint32_t w, u32x4 s) {
+  const uint32_t s0 = s[0], s1 = s[1], s2 = s[2], s3 = s[3];   // (a bit cast of a vector's element takes the first one)
+  return values(w, __builtin_bit_cast(h2, s0), __builtin_bit_cast(h2, s1), __builtin_bit_cast(h2, s2), __builtin_bit_cast(h2, s3));
+}
+
+__device__ __forceinline__ int tokens_of(const int *lens, int b, int n) { return lens ? min(max(lens[b], 0), n) : n; }
+
+// ------------------------------------------------------------------ writing and reading
+// the scale of a group from the bits of its largest magnitude
+__device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 0x7e00;
+  const float a = fminf(__builtin_bit_cast(float, amax_bits), 65504.f);
+  return float_to_half_bits(bf16_to_f(f_to_bf16(a / 7.f)));
+}
+// clamp(rint(x / s), -7, 7) + 8, ties to even, of the real quotient: the product with 1 / s is off by one step at most, and
+// only next to a border; e = x - r s is exact (r s has 11 bits, e is a multiple of x's last place below 2^24 of them)
+__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
+  const float y = fminf(fmaxf(x, -7.f * s), 7.f * s);
+  float r = __builtin_rintf(y * inv);
+  const float e = 2.f * __builtin_fmaf(-r, s, y);
+  const bool odd = ((int)r & 1) != 0;
+  if (e > s || (e == s && odd)) r += 1.f;
+  else if (e < -s || (e == -s && odd)) r -= 1.f;
+  return (uint32_t)((int)r + 8);
+}
+
+// One wave per record's K, one per its V: lane = position lane / 8 of the record, dims EL (lane % 8) ..  Positions outside the
+// call's keep their codes and scales: their K rows and scales are not stored, and the V words, which hold all 8
+// positions, are read and merged where the call covers a part only (no other workgroup of the launch has the record).
+// Bound by memory for prompts and by latency for single tokens.
+template <int HD>
+__global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
+  constexpr int EL = HD / 8, GL = 32 / EL;   // elements of a lane; lanes of a group
+  __shared__ __align__(16) uint8_t codes[kRec][HD];
+  const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 63, vside = threadIdx.x >> 6;
+  const int P0 = a.pos[b], cnt = tokens_of(a.lens, b, a.n);
+  if (P0 < 0 || cnt <= 0) return;
+  const int64_t rec = P0 / kRec + (int64_t)blockIdx.x;
+  const int64_t last = min((int64_t)P0 + cnt, a.ctx);   // one past the last position written
+  if (rec * kRec >= last) return;
+  const int row = lane >> 3, part = lane & 7;
+  const int64_t p = rec * kRec + row;
+  const bool mine = p >= P0 && p < last;
+  const KvRows &r = vside ? a.v : a.k;
+  float x[EL];
+  uint32_t mx = 0;
+  if (mine) {
+    load_elems<EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, a.vec, x);
+#pragma unroll
+    for (int i = 0; i < EL; i++) mx = max(mx, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+  }
+  mx = max(mx, (uint32_t)dpp_i<kDppQuadXor1>((int)mx));
+  if (GL == 4) mx = max(mx, (uint32_t)dpp_i<kDppQuadXor2>((int)mx));
+  const uint16_t sb = group_scale(mx);
+  const float s = half_bits_to_float(sb);
+  uint32_t c[EL];
+  if (s > 0.f) {
+    const float inv = 1.f / s;
+#pragma unroll
+    for (int i = 0; i < EL; i++) c[i] = mine ? code_of(x[i], s, inv) : 8;
+  } else {
+#pragma unroll
+    for (int i = 0; i < EL; i++) c[i] = 8;
+  }
+  uint8_t *o = (uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD);
+  if (!vside) {
+    if (!mine) return;
+    uint32_t w[EL / 8];
+#pragma unroll
+    for (int i = 0; i < EL / 8; i++) {
+      w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) w[i] |= c[8 * i + j] << nib(j);
+      *(uint32_t *)(o + row * (HD / 2) + part * (EL / 2) + 4 * i) = w[i];
+    }
+    if (part % GL == 0) *(uint16_t *)(o + 8 * HD + 2 * (row * (HD / 32) + part / GL)) = sb;
+    return;
+  }
+  if (mine && part % GL == 0) *(uint16_t *)(o + 8 * HD + HD / 2 + 2 * (part / GL * kRec + row)) = sb;
+#pragma unroll
+  for (int i = 0; i < EL; i += 4) *(uint32_t *)&codes[row][EL * part + i] = c[i] | c[i + 1] << 8 | c[i + 2] << 16 | c[i + 3] << 24;
+  // the V wave alone reads what it wrote
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  uint32_t keep = 0;   // bits of the positions that the call does not write
+#pragma unroll
+  for (int i = 0; i < kRec; i++)
+    if (!(rec * kRec + i >= P0 && rec * kRec + i < last)) keep |= 15u << nib(i);
+#pragma unroll
+  for (int k = 0; k < HD / 64; k++) {
+    const int idx = lane * (HD / 64) + k, d = idx % (HD / 16) * 16 + idx / (HD / 16);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < kRec; i++) w |= (uint32_t)codes[i][d] << nib(i);
+    uint32_t *dst = (uint32_t *)(o + 4 * HD) + idx;
+    if (keep) w = (w & ~keep) | (*dst & keep);
+    *dst = w;
+  }
+}
+
+template <int HD>
+__global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
+  constexpr int EL = HD / 8, GL = 32 / EL;
+  const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 63, vside = threadIdx.x >> 6;
+  const int P0 = a.pos[b], cnt = tokens_of(a.lens, b, a.n);
+  if (P0 < 0 || cnt <= 0) return;
+  const int64_t rec = P0 / kRec + (int64_t)blockIdx.x;
+  const int row = lane >> 3, part = lane & 7;
+  const int64_t p = rec * kRec + row;
+  if (p < P0 || p >= min((int64_t)P0 + cnt, a.ctx)) return;
+  const uint8_t *o = (const uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD);
+  float x[EL];
+  if (!vside) {
+    const uint16_t s = *(const uint16_t *)(o + 8 * HD + 2 * (row * (HD / 32) + part / GL));
+#pragma unroll
+    for (int i = 0; i < EL / 8; i++) {
+      const h8 v = values(*(const uint32_t *)(o + row * (HD / 2) + part * (EL / 2) + 4 * i), s);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[8 * i + j] = (float)v[j];
+    }
+  } else {
+    const float s = half_bits_to_float(*(const uint16_t *)(o + 8 * HD + HD / 2 + 2 * (part / GL * kRec + row)));
+#pragma unroll
+    for (int i = 0; i < EL; i++) {
+      const int d = EL * part + i;
+      const uint32_t w = ((const uint32_t *)(o + 4 * HD))[d % 16 * (HD / 16) + d / 16];
+      x[i] = ((int)(w >> (16 * (row & 1) + 4 * (row >> 1)) & 15) - 8) * s;
+    }
+  }
+  const KvRows &r = vside ? a.v : a.k;
+  store_elems<EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, a.vec, x);
+}
+
+// the fp16 cache's: a copy with a conversion, 8 dims of one position's K and V a thread
+template <bool WRITE>
+__global__ __launch_bounds__(256) void k_kv16_io(KvIoArgs a) {
+  const int b = blockIdx.z, per = a.nkv * a.hd / 8;
+  const int P0 = a.pos[b], cnt = tokens_of(a.lens, b, a.n);
+  if (P0 < 0) return;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / per, p = P0 + t;
+  if (t >= cnt || p >= a.ctx) return;
+  const int g = (int)(i % per) / (a.hd / 8), d = 8 * ((int)(i % per) % (a.hd / 8));
+  const KvRows &r = blockIdx.y ? a.v : a.k;
+  uint16_t *c = (uint16_t *)(blockIdx.y ? a.cache_v : a.cache) + b * a.cseq + p * a.crow + g * a.hd + d;
+  const int64_t at = b * r.seq + t * r.tok + g * r.head + d;
+  float x[8];
+  u32x4 w;
+  if (WRITE) {
+    load_elems<8>(r, at, a.vec, x);
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = float_to_half_bits(x[2 * j]) | (uint32_t)float_to_half_bits(x[2 * j + 1]) << 16;
+    *(u32x4 *)c = w;
+  } else {
+    w = *(const u32x4 *)c;
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = half_bits_to_float((uint16_t)(w[j / 2] >> 16 * (j & 1)));
+    store_elems<8>(r, at, a.vec, x);
+  }
+}
+
+// ------------------------------------------------------------------ what a workgroup of the attention reads
+// Columns: a kv head's (token, query head) pairs, the head fastest; a workgroup has a.cols of them, c0 .. of sequence b.  The
+// records any of its columns may see: the SR first ones (positions below sinks), then from the window's first on; virtual
+// record v is v, or v + skip from SR on.
+struct Span {
+  int P0, cnt;      // the sequence's first new position and its tokens that count
+  int PA, PB;       // positions of the workgroup's first and last token
+  int ws;           // first position of PA's window
+  int SR, skip, NR; // virtual records
+  int nt, S;        // tiles of a.tile positions, splits in use
+  bool any;
+};
+__device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int c0) {
+  Span s;
+  s.P0 = a.pos[b]; s.cnt = tokens_of(a.lens, b, a.n);
+  const int ta = c0 / a.rep;
+  s.any = s.P0 >= 0 && ta < s.cnt && (int64_t)s.P0 + ta < a.ctx;
+  s.PA = s.P0 + ta;
+  s.PB = (int)min((int64_t)s.P0 + min((c0 + a.cols - 1) / a.rep, s.cnt - 1), a.ctx - 1);
+  s.ws = a.window > 0 ? max(0, s.PA - a.window + 1) : 0;
+  const int r0 = s.ws / kRec;
+  s.SR = min((int)(((int64_t)a.sinks + kRec - 1) / kRec), r0);
+  s.skip = r0 - s.SR;
+  s.NR = s.PB / kRec + 1 - s.skip;
+  const int rt = a.tile / kRec;
+  s.nt = (s.NR + rt - 1) / rt;
+  s.S = max(1, min(a.nsplit, (s.nt + a.min_tiles - 1) / a.min_tiles));
+  return s;
+}
+__device__ __forceinline__ int record(const Span &s, int v) { return v < s.SR ? v : v + s.skip; }
+// whether the token at P sees position p
+__device__ __forceinline__ bool sees(const KvAttnArgs &a, int P, int p) {
+  return p <= P && (a.window <= 0 || p > P - a.window || p < a.sinks);
+}
+
+// Queries enter as fp16, each row scaled by the power of two that brings its largest magnitude into [1, 2): fp16 and bf16
+// values keep every bit that is not 2^-25 below that (fp32 ones go in two halves, hi + lo, and keep 22 bits).  The power
+// returns with the softmax scale, in fp32.
+__device__ __forceinline__ float row_power(float mx) {   // 2^-e; 1 for rows that are zero or not finite
+  const uint32_t e = __builtin_bit_cast(uint32_t, mx) >> 23;
+  return e == 0 || e >= 254 ? 1.f : __builtin_bit_cast(float, (254u - e) << 23);
+}
+
+// probabilities are held as 2^(x - m + 14): in fp16 what lies 2^-38 below the largest is still there, and the sum
+// they are divided by is scaled alike
+constexpr float kPBias = 14.f;
+
+// ------------------------------------------------------------------ few tokens
+// Grid (split, kv head and column chunk, sequence), 8 waves, each streaming its own tiles of 32 positions (4 records) with
+// the next tile's loads in flight.
+//   scores  S^T[p][c] = K[p] . q[c] on v_mfma_f32_16x16x32_f16, A = K rows, B = q^T with 16 columns.  Row r of tile half mt is
+//           position 8 (r / 4) + 4 mt + r % 4, so the C layout leaves lane group lg = lane / 16 the 8 positions of record lg.
+//   values  O^T[d][c] += V^T[d][p] P^T[p][c]: those 8 probabilities are the lane's B fragment as they are, and the A
+//           fragment is dim 16 t + lane % 16 of record lg: one word of V codes.
+// TWO (fp32 queries): 8 columns, with the queries' hi halves in columns 0 .. 7 and their lo halves in 8 .. 15 of the same
+// product, and P's likewise: 22 bits for the price of 11 where no more than 8 columns are needed.
+constexpr int kFewWaves = 8, kFewTile = 32;
+
+template <int HD>
+struct Tile4 {   // a tile of a 4-bit cache
+  static constexpr int KW = HD / 32, VW = HD / 16;   // words of a lane: K row piece, V dims
+  uint32_t k[2][KW], v[VW];
+  uint16_t ks[2];
+  u32x4 vs[HD / 32];
+};
+template <int HD>
+__device__ __forceinline__ void load_tile4(const uint8_t *head, const Span &s, int tile, int lane, Tile4<HD> &t) {
+  const int lr = lane & 15, lg = lane >> 4;
+  {
+    const uint8_t *r = head + (int64_t)record(s, min(4 * tile + (lr >> 2), s.NR - 1)) * (9 * HD);
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) {
+      const int row = 4 * mt + (lr & 3);
+      const uint8_t *kp = r + row * (HD / 2) + lg * (HD / 8);
+      if constexpr (HD == 128) { const u32x4 x = *(const u32x4 *)kp; t.k[mt][0] = x[0]; t.k[mt][1] = x[1]; t.k[mt][2] = x[2]; t.k[mt][3] = x[3]; }
+      else { const u32x2 x = *(const u32x2 *)kp; t.k[mt][0] = x[0]; t.k[mt][1] = x[1]; }
+      t.ks[mt] = *(const uint16_t *)(r + 8 * HD + 2 * (row * (HD / 32) + lg * HD / 128));
+    }
+  }
+  const uint8_t *r = head + (int64_t)record(s, min(4 * tile + lg, s.NR - 1)) * (9 * HD);
+#pragma unroll
+  for (int i = 0; i < HD / 64; i++) {
+    const u32x4 x = *(const u32x4 *)(r + 4 * HD + lr * (HD / 4) + 16 * i);
+#pragma unroll
+    for (int j = 0; j < 4; j++) t.v[4 * i + j] = x[j];
+  }
+#pragma unroll
+  for (int i = 0; i < HD / 32; i++) t.vs[i] = *(const u32x4 *)(r + 8 * HD + HD / 2 + 16 * i);
+}
+template <int HD>
+struct Tile16 { u32x4 k[2][HD / 32]; };   // K of a tile of an fp16 cache; its V goes to LDS
+// 16-byte segment c of V row x sits at c ^ vsw(x): the 8 rows that the 32 lanes of a transpose read address (0 .. 3 or 4 .. 7 of two
+// records) cover all banks
+template <int HD>
+__device__ __forceinline__ int vsw(int x) { return HD == 128 ? 2 * ((x & 3) | (x >> 1 & 4)) : 2 * ((x >> 1 & 1) | (x >> 2 & 2)); }
+template <int HD>
+__device__ __forceinline__ void load_tile16(const KvAttnArgs &a, const uint16_t *kh, const uint16_t *vh, const Span &s, int tile, int lane,
+                                            Tile16<HD> &t, uint16_t *buf) {
+  const int lr = lane & 15, lg = lane >> 4;
+  constexpr int SEG = HD / 8, RPI = 64 / SEG;   // 16-byte segments of a row, rows of a 1 KiB load
+#pragma unroll
+  for (int q = 0; q < kFewTile / RPI; q++) {
+    const int x = q * RPI + lane / SEG, seg = lane % SEG;
+    const int64_t p = min((int64_t)kRec * record(s, min(4 * tile + x / kRec, s.NR - 1)) + x % kRec, a.ctx - 1);
+    dma16(vh + p * a.crow + 8 * (seg ^ vsw<HD>(x)), buf + q * RPI * HD);
+  }
+#pragma unroll
+  for (int mt = 0; mt < 2; mt++) {
+    const int64_t p = min((int64_t)kRec * record(s, min(4 * tile + (lr >> 2), s.NR - 1)) + 4 * mt + (lr & 3), a.ctx - 1);
+#pragma unroll
+    for (int k = 0; k < HD / 32; k++) t.k[mt][k] = *(const u32x4 *)(kh + p * a.crow + 32 * k + 8 * lg);
+  }
+}
+
+__device__ __forceinline__ bool not_finite(h8 v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) bad |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+  return bad;
+}
+// v with the elements of clear bits of `on` zeroed
+__device__ __forceinline__ h8 only(h8 v, uint32_t on) {
+  u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[i] &= (on >> 2 * i & 1 ? 0xffffu : 0u) | (on >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
+  return __builtin_bit_cast(h8, w);
+}
+
+template <int HD, int KIND, bool TWO>
+__global__ __launch_bounds__(kFewWaves * 64) void k_kv_few(KvAttnArgs a) {
+  constexpr int NW = kFewWaves, KS = HD / 32, DT = HD / 16, NC = TWO ? 8 : 16, QS = HD + 4;
+  constexpr int kTileBytes = KIND == MK_Q4 ? 0 : NW * kFewTile * HD * 2, kOutBytes = NW * NC * QS * 4;
+  __shared__ __align__(16) uint8_t sm[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
+  __shared__ float wm[NW][NC], wl[NW][NC];
+  const int b = blockIdx.z, g = blockIdx.y / a.nchunk, c0 = blockIdx.y % a.nchunk * NC, split = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const Span s = span_of(a, b, c0);
+  if (!s.any || split >= s.S) return;
+  const int col = c0 + (TWO ? lr & 7 : lr), tok = col / a.rep;
+  const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
+  const int P = live ? s.P0 + tok : -1;
+  const int t0 = (int)((int64_t)split * s.nt / s.S), t1 = (int)((int64_t)(split + 1) * s.nt / s.S);
+  const uint8_t *head4 = nullptr;
+  const uint16_t *kh = nullptr, *vh = nullptr;
+  uint16_t *vbuf = (uint16_t *)sm + wave * kFewTile * HD;
+  if constexpr (KIND == MK_Q4) head4 = (const uint8_t *)a.cache + ((int64_t)b * a.nkv + g) * a.nrec * (9 * HD);
+  else { kh = (const uint16_t *)a.cache + b * a.cseq + g * HD; vh = (const uint16_t *)a.cache_v + b * a.cseq + g * HD; }
+  using Tile = typename std::conditional<KIND == MK_Q4, Tile4<HD>, Tile16<HD>>::type;
+  Tile ta, tb;
+  auto load = [&](int tile, Tile &t) {
+    if constexpr (KIND == MK_Q4) load_tile4<HD>(head4, s, tile, lane, t);
+    else load_tile16<HD>(a, kh, vh, s, tile, lane, t, vbuf);
+  };
+  if (t0 + wave < t1) load(t0 + wave, ta);
+  // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j
+  h8 q[KS];
+  float f;   // softmax scale in base 2, times the row's power
+  {
+    float x[KS][8], mx = 0.f;
+    const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)(g * a.rep + col % a.rep) * a.q.head;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      if (live) load_elems<8>(a.q, at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg), a.vec_q, x[k]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) { if (!live) x[k][j] = 0.f; mx = fmaxf(mx, fabsf(x[k][j])); }
+    }
+    mx = pair_max32(pair_max16(mx));
+    const float p2 = row_power(mx);
+    f = a.scale2 / p2;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float y = x[k][j] * p2;
+        const _Float16 h = (_Float16)y;
+        q[k][j] = TWO && lr >= 8 ? (_Float16)(y - (float)h) : h;
+      }
+  }
+  f32x4 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  auto step = [&](Tile &cur, Tile &nxt, int tile) {
+    const int v = 4 * tile + lg, p0 = kRec * record(s, min(v, s.NR - 1));
+    const bool in = v < s.NR;
+    // positions of the tile that some column does not see: its first and last record bound the others
+    const int pf = kRec * record(s, 4 * tile), pl = kRec * record(s, min(4 * tile + 3, s.NR - 1)) + kRec - 1;
+    const bool edge = 4 * tile + 4 > s.NR || pl > s.PA || (a.window > 0 && pf <= s.PB - a.window && pl >= a.sinks);
+    h8 vf[DT];
+    if constexpr (KIND != MK_Q4) {
+      // K's registers were asked for after V's tile: once they are here, it is
+#pragma unroll
+      for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+        for (int k = 0; k < KS; k++) asm volatile("" ::"v"(cur.k[mt][k]));
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      // ds_read_b64_tr_b16 hands lane i of 16 the element i % 4 of what lanes 4 j + i / 4 address, as its element j
+      const int x = 8 * lg + (lr >> 2), dq = 4 * (lr & 3);
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const int seg = (16 * d + dq) >> 3, in8 = dq & 4;
+        const s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + x * HD + 8 * (seg ^ vsw<HD>(x)) + in8));
+        const s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + (x + 4) * HD + 8 * (seg ^ vsw<HD>(x + 4)) + in8));
+        vf[d] = __builtin_bit_cast(h8, (s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile is read before the next one's loads write it
+    }
+    if (tile + NW < t1) load(tile + NW, nxt);
+    f32x4 sc[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) {
+      sc[mt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        h8 kf;
+        if constexpr (KIND == MK_Q4) kf = values(cur.k[mt][k], cur.ks[mt]);
+        else kf = __builtin_bit_cast(h8, cur.k[mt][k]);
+        sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[k], sc[mt], 0, 0, 0);
+      }
+    }
+    float x[8], bm = -INFINITY;
+    uint32_t some = 0;   // positions that a column of the workgroup may see
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float y = sc[j >> 2][j & 3];
+      if (TWO) y += xchg8_f(y);
+      y *= f;
+      if (edge) {
+        const int p = p0 + j;
+        if (!(in && sees(a, P, p))) y = -INFINITY;
+        some |= in && p <= s.PB && (p >= s.ws || p < a.sinks) ? 1u << j : 0u;
+      }
+      x[j] = y; bm = fmaxf(bm, y);
+    }
+    bm = pair_max32(pair_max16(bm));
+    const float mn = fmaxf(m, bm), mz = mn == -INFINITY ? 0.f : mn;
+    const float corr = __builtin_amdgcn_exp2f(m - mz);
+    float rs = 0.f;
+    h8 ph;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float pv = __builtin_amdgcn_exp2f(x[j] - mz + kPBias);
+      rs += pv;
+      const _Float16 h = (_Float16)pv;
+      ph[j] = TWO && lr >= 8 ? (_Float16)(pv - (float)h) : h;
+    }
+    rs = pair_sum32(pair_sum16(rs));
+    l = l * corr + rs;
+    m = mn;
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      o[d] *= corr;
+      if constexpr (KIND == MK_Q4) vf[d] = values(cur.v[d], cur.vs[d / 2]);
+    }
+    if (edge) {
+      // what no column sees may hold anything: zeroed, since 0 x NaN is not 0.  What some columns see and others don't, the
+      // tokens one at a time, and only where it matters
+      bool bad = false;
+#pragma unroll
+      for (int d = 0; d < DT; d++) { vf[d] = only(vf[d], some); bad |= not_finite(vf[d]); }
+      if (s.PA != s.PB && __any(bad)) {
+        for (int Pt = s.PA; Pt <= s.PB; Pt++) {
+          uint32_t on = 0;
+#pragma unroll
+          for (int j = 0; j < 8; j++) on |= in && sees(a, Pt, p0 + j) ? 1u << j : 0u;
+#pragma unroll
+          for (int d = 0; d < DT; d++) {
+            const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(only(vf[d], on), ph, o[d], 0, 0, 0);
+            if (P == Pt) o[d] = y;
+          }
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph, o[d], 0, 0, 0);
+  };
+  for (int t = t0 + wave; t < t1; t += 2 * NW) {
+    step(ta, tb, t);
+    if (t + NW >= t1) break;
+    step(tb, ta, t + NW);
+  }
+  // the waves' sums meet in LDS
+  if (KIND != MK_Q4) __syncthreads();   // no wave's V tile is in use
+  float *ored = (float *)sm;
+#pragma unroll
+  for (int d = 0; d < DT; d++) {
+    f32x4 y = o[d];
+    if (TWO) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] += xchg8_f(y[i]);
+    }
+    if (lr < NC) *(f32x4 *)(ored + (wave * NC + lr) * QS + 16 * d + 4 * lg) = y;
+  }
+  if (lg == 0 && lr < NC) { wm[wave][lr] = m; wl[wave][lr] = l; }
+  __syncthreads();
+  const int e = threadIdx.x, c = e / (HD / 4), d = 4 * (e % (HD / 4));
+  if (c >= NC) return;
+  const int cc = c0 + c, tk = cc / a.rep;
+  if (tk >= s.cnt || (int64_t)s.P0 + tk >= a.ctx) return;
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][c]);
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  const float Mz = M == -INFINITY ? 0.f : M;
+#pragma unroll
+  for (int w = 0; w < NW; w++) {
+    const float k = __builtin_amdgcn_exp2f(wm[w][c] - Mz);
+    L += wl[w][c] * k;
+    y += *(const f32x4 *)(ored + (w * NC + c) * QS + d) * k;
+  }
+  const int head = g * a.rep + cc % a.rep;
+  if (s.S == 1) {
+    const float inv = 1.f / L;   // a visible position's score is -inf only where the plain softmax gives NaN too: 0 x inf
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = y[i] * inv;
+    store_elems<4>(a.out, b * a.out.seq + (int64_t)tk * a.out.tok + (int64_t)head * a.out.head + d, a.vec_o, r);
+    return;
+  }
+  const int64_t row = ((int64_t)b * a.n + tk) * a.heads + head, at = row * a.nsplit + split;
+  *(f32x4 *)(a.part + at * HD + d) = y;
+  if (d == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.nsplit * HD + 2 * at) = make_float2(M, L);
+}
+
+// The splits' sums of one row a workgroup: 256 threads, HD / 4 of them side by side over the dims, the others over the
+// splits.  M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L
+template <int HD>
+__global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
+  constexpr int CT = HD / 4, SL = 256 / CT;
+  __shared__ f32x4 oo[SL][CT];
+  const int head = blockIdx.x, tok = blockIdx.y, b = blockIdx.z, g = head / a.rep;
+  const int col = tok * a.rep + head - g * a.rep;
+  const Span s = span_of(a, b, col / a.cols * a.cols);
+  if (!s.any || s.S == 1 || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
+  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.nsplit * HD) + row * a.nsplit;
+  const float *po = a.part + row * a.nsplit * HD;
+  const int ct = threadIdx.x % CT, sl = threadIdx.x / CT, lane = threadIdx.x & 63;
+  // every wave forms M and L itself: one split a lane (at most 64)
+  const float2 x = lane < s.S ? ml[lane] : make_float2(-INFINITY, 0.f);
+  const float M = wave_max(x.x), Mz = M == -INFINITY ? 0.f : M;
+  const float L = wave_sum(x.y * __builtin_amdgcn_exp2f(x.x - Mz));
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = sl; i < s.S; i += SL) y += *(const f32x4 *)(po + (int64_t)i * HD + 4 * ct) * __builtin_amdgcn_exp2f(ml[i].x - Mz);
+  oo[sl][ct] = y;
+  __syncthreads();
+  if (sl) return;
+#pragma unroll
+  for (int i = 1; i < SL; i++) y += oo[i][ct];
+  const float inv = 1.f / L;
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) r[i] = y[i] * inv;
+  store_elems<4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, a.vec_o, r);
+}
+
+// ------------------------------------------------------------------ many tokens
+// 8 waves of 32 columns; the workgroup's 256 columns share blocks of 64 positions (8 records) in LDS, two buffers: the next
+// block's codes are on their way to registers and the one after the present one is expanded into LDS while the
+// present one is computed.
+//   scores  S^T[p][c] on v_mfma_f32_32x32x16_f16, A = K rows from LDS.  Row r of a 32-position tile is position 16 (r / 16) +
+//           8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4: the C layout then leaves lane half h = lane / 32 the 8 positions of records
+//           2 u + h, u = 0, 1, in order, which is the B fragment of the value product's 16-position step u.
+//   values  O^T[d][c] += V^T[d][p] P^T[p][c]: 4-bit: V^T lies in LDS as the words expand, 8 positions of a dim together, one
+//           16-byte read a fragment; fp16: V lies as stored and two transpose reads fetch one.
+// TWO (fp32 queries): hi and lo halves of the queries and probabilities as products of their own.
+constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
+
+template <int HD, int KIND, bool TWO>
+__global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
+  constexpr int NT = kManyWaves * 64, KQ = HD / 16, OT = HD / 32, BR = kManyBlk / kRec;
+  constexpr int KST = HD + 8;                                   // halves of a K row in LDS: an odd number of 16-byte columns
+  constexpr int VST = KIND == MK_Q4 ? kManyBlk + 8 : HD + 32;   // of a V^T row (dims), or a V row (positions): 4 rows of 64 bytes apart
+  constexpr int VN = KIND == MK_Q4 ? HD * VST : kManyBlk * VST;
+  __shared__ __align__(16) uint16_t ks[2][kManyBlk * KST];
+  __shared__ __align__(16) uint16_t vs[2][VN];
+  __shared__ int badf[3];   // block kb's at (kb - kb0) % 3: set while kb - 1 is computed, read with kb, cleared with kb + 1
+  const int b = blockIdx.y, g = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv, split = rest % a.nsplit;
+  const int c0 = (a.nchunk - 1 - rest / a.nsplit) * kManyCols;   // the last columns, with the most to read, first
+  const Span s = span_of(a, b, c0);
+  if (!s.any || split >= s.S) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, ln = lane & 31, hf = lane >> 5;
+  const int col = c0 + 32 * wave + ln, tok = col / a.rep, head = g * a.rep + col % a.rep;
+  const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
+  const int P = live ? s.P0 + tok : -1;
+  // the wave's own first and last token
+  const int wa = (c0 + 32 * wave) / a.rep;
+  const bool wlive = wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
+  const int PA = s.P0 + wa, PB = (int)min((int64_t)s.P0 + min((c0 + 32 * wave + 31) / a.rep, s.cnt - 1), a.ctx - 1);
+  const int kb0 = (int)((int64_t)split * s.nt / s.S), kb1 = (int)((int64_t)(split + 1) * s.nt / s.S);
+  const uint8_t *head4 = (const uint8_t *)a.cache + ((int64_t)b * a.nkv + g) * a.nrec * (9 * HD);
+  const uint16_t *kh = (const uint16_t *)a.cache + b * a.cseq + g * HD, *vh = (const uint16_t *)a.cache_v + b * a.cseq + g * HD;
+
+  // ---- a block's codes (or fp16 pieces): memory -> registers -> LDS
+  constexpr int NP = KIND == MK_Q4 ? 1 : kManyBlk * HD / 8 / NT;
+  constexpr bool kAll = KIND != MK_Q4 || HD * 4 == NT;   // every thread has a share
+  u32x2 kq, vq;
+  uint16_t ksc;
+  u32x4 vsc, kp[NP], vp[NP];
+  auto fetch = [&](int kb) {
+    if constexpr (KIND == MK_Q4) {
+      if (!kAll && tid >= HD * 4) return;
+      const int row = tid / (HD / 16), wp = tid % (HD / 16);
+      const uint8_t *r = head4 + (int64_t)record(s, min(BR * kb + row / kRec, s.NR - 1)) * (9 * HD);
+      kq = *(const u32x2 *)(r + row % kRec * (HD / 2) + 8 * wp);
+      ksc = *(const uint16_t *)(r + 8 * HD + 2 * (row % kRec * (HD / 32) + wp / 2));
+      const int rl = tid / (HD / 2), w = 2 * (tid % (HD / 2));
+      const uint8_t *q = head4 + (int64_t)record(s, min(BR * kb + rl, s.NR - 1)) * (9 * HD);
+      vq = *(const u32x2 *)(q + 4 * HD + 4 * w);
+      vsc = *(const u32x4 *)(q + 8 * HD + HD / 2 + 16 * (w % (HD / 16) / 2));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
+        const int64_t p = min((int64_t)kRec * record(s, min(BR * kb + x / kRec, s.NR - 1)) + x % kRec, a.ctx - 1);
+        kp[i] = *(const u32x4 *)(kh + p * a.crow + 8 * sg);
+        vp[i] = *(const u32x4 *)(vh + p * a.crow + 8 * sg);
+      }
+    }
+  };
+  // first and last position of a block, and whether some columns of tokens A .. B do not see all of it
+  auto first = [&](int kb) { return kRec * record(s, BR * kb); };
+  auto last = [&](int kb) { return kRec * record(s, min(BR * kb + BR - 1, s.NR - 1)) + kRec - 1; };
+  auto partial = [&](int kb, int A, int B) {
+    const int pf = first(kb), pl = last(kb);
+    return BR * kb + BR > s.NR || pl > A || (a.window > 0 && pf <= B - a.window && pl >= a.sinks);
+  };
+  auto any_sees = [&](int v, int p) { return v < s.NR && p <= s.PB && (p >= s.ws || p < a.sinks); };
+  auto expand = [&](int kb, int buf) {
+    const bool edge = partial(kb, s.PA, s.PB);
+    if constexpr (KIND == MK_Q4) {
+      if (!kAll && tid >= HD * 4) return;
+      const int row = tid / (HD / 16), wp = tid % (HD / 16);
+#pragma unroll
+      for (int i = 0; i < 2; i++) *(h8 *)(ks[buf] + row * KST + 16 * wp + 8 * i) = values(kq[i], ksc);
+      const int rl = tid / (HD / 2), w = 2 * (tid % (HD / 2)), d = w % (HD / 16) * 16 + w / (HD / 16);
+      uint32_t on = 255;
+      if (edge) {
+        on = 0;
+        const int v = BR * kb + rl, p0 = kRec * record(s, min(v, s.NR - 1));
+#pragma unroll
+        for (int j = 0; j < kRec; j++) on |= any_sees(v, p0 + j) ? 1u << j : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        h8 x = values(vq[i], vsc);
+        if (edge) { x = only(x, on); if (not_finite(x)) badf[(kb - kb0) % 3] = 1; }
+        *(h8 *)(vs[buf] + (d + 16 * i) * VST + kRec * rl) = x;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
+        *(u32x4 *)(ks[buf] + x * KST + 8 * sg) = kp[i];
+        u32x4 w = vp[i];
+        if (edge) {
+          const int v = BR * kb + x / kRec;
+          if (!any_sees(v, kRec * record(s, min(v, s.NR - 1)) + x % kRec)) w = (u32x4){0u, 0u, 0u, 0u};
+          if (not_finite(__builtin_bit_cast(h8, w))) badf[(kb - kb0) % 3] = 1;
+        }
+        *(u32x4 *)(vs[buf] + x * VST + 8 * sg) = w;
+      }
+    }
+  };
+  if (tid < 3) badf[tid] = 0;
+  fetch(kb0);
+  // ---- queries
+  h8 q[KQ], ql[TWO ? KQ : 1];
+  float f;
+  {
+    float x[KQ][8], mx = 0.f;
+    const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)head * a.q.head;
+#pragma unroll
+    for (int k = 0; k < KQ; k++) {
+      if (live) load_elems<8>(a.q, at + 16 * k + 8 * hf, a.vec_q, x[k]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) { if (!live) x[k][j] = 0.f; mx = fmaxf(mx, fabsf(x[k][j])); }
+    }
+    mx = pair_max32(mx);
+    const float p2 = row_power(mx);
+    f = a.scale2 / p2;
+#pragma unroll
+    for (int k = 0; k < KQ; k++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float y = x[k][j] * p2;
+        const _Float16 h = (_Float16)y;
+        q[k][j] = h;
+        if constexpr (TWO) ql[k][j] = (_Float16)(y - (float)h);
+      }
+  }
+  f32x16 o[OT];
+#pragma unroll
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[t][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  // LDS row of the lane's K row
+  const int kr = (ln & 16) | (ln & 4) << 1 | (ln & 8) >> 1 | (ln & 3);
+  auto vfrag = [&](const uint16_t *v, int t, int u) {
+    if constexpr (KIND == MK_Q4) return *(const h8 *)(v + (32 * t + ln) * VST + 16 * u + 8 * hf);
+    else {
+      const int r = lane & 15, x = 16 * u + 8 * hf + (r >> 2), d = 32 * t + (ln & 16) + 4 * (r & 3);
+      const s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v + x * VST + d));
+      const s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v + (x + 4) * VST + d));
+      return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+  auto block = [&](int kb, int buf) {
+    const uint16_t *kl = ks[buf], *vl = vs[buf];
+    const bool edge = partial(kb, PA, PB);
+    f32x16 sc[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) sc[mt][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KQ; k++) {
+        const h8 kf = *(const h8 *)(kl + (32 * mt + kr) * KST + 16 * k + 8 * hf);
+        sc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[k], sc[mt], 0, 0, 0);
+        if constexpr (TWO) sc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc[mt], 0, 0, 0);
+      }
+    }
+    float bm = -INFINITY;
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1));
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (!(v < s.NR && sees(a, P, p0 + j))) sc[u >> 1][8 * (u & 1) + j] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[mt][i]);
+    bm = pair_max32(bm) * f;   // f > 0
+    const float mn = fmaxf(m, bm), mz = mn == -INFINITY ? 0.f : mn;
+    const float corr = __builtin_amdgcn_exp2f(m - mz);
+    const float sub = kPBias - mz;
+    float rs = 0.f;
+    h8 ph[4], pl[TWO ? 4 : 1];
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][8 * (u & 1) + j], f, sub));
+        rs += pv;
+        const _Float16 h = (_Float16)pv;
+        ph[u][j] = h;
+        if constexpr (TWO) pl[u][j] = (_Float16)(pv - (float)h);
+      }
+    rs = pair_sum32(rs);
+    l = l * corr + rs;
+    if (__any(mn != m)) {
+#pragma unroll
+      for (int t = 0; t < OT; t++) o[t] *= corr;
+    }
+    m = mn;
+    if (edge && badf[(kb - kb0) % 3]) {
+      for (int Pt = PA; Pt <= PB; Pt++) {   // see k_kv_few
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          asm volatile("" ::: "memory");   // the fragments are read again for each token, not kept in registers
+          const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1));
+          uint32_t on = 0;
+#pragma unroll
+          for (int j = 0; j < 8; j++) on |= v < s.NR && sees(a, Pt, p0 + j) ? 1u << j : 0u;
+#pragma unroll
+          for (int t = 0; t < OT; t++) {
+            const h8 x = only(vfrag(vl, t, u), on);
+            f32x16 y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[u], o[t], 0, 0, 0);
+            if constexpr (TWO) y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[u], y, 0, 0, 0);
+            if (P == Pt) o[t] = y;
+          }
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int t = 0; t < OT; t++)
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const h8 x = vfrag(vl, t, u);
+        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[u], o[t], 0, 0, 0);
+        if constexpr (TWO) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[u], o[t], 0, 0, 0);
+      }
+  };
+  __syncthreads();   // badf
+  expand(kb0, 0);
+  if (kb0 + 1 < kb1) fetch(kb0 + 1);
+  __syncthreads();
+  for (int kb = kb0; kb < kb1; kb++) {
+    const int buf = (kb - kb0) & 1;
+    if (kb + 1 < kb1) expand(kb + 1, buf ^ 1);
+    if (kb + 2 < kb1) fetch(kb + 2);
+    const int pf = first(kb), pl = last(kb);
+    if (wlive && pf <= PB && !(a.window > 0 && pl <= PA - a.window && pf >= a.sinks)) block(kb, buf);
+    if (tid == 0) badf[(kb - kb0 + 2) % 3] = 0;
+    __syncthreads();
+  }
+  if (!live) return;
+  if (s.S == 1) {
+    const float inv = 1.f / l;
+    const int64_t at = b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head;
+#pragma unroll
+    for (int t = 0; t < OT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float r[4] = {o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv};
+        store_elems<4>(a.out, at + 32 * t + 8 * i + 4 * hf, a.vec_o, r);
+      }
+    return;
+  }
+  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head, at = row * a.nsplit + split;
+#pragma unroll
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      *(f32x4 *)(a.part + at * HD + 32 * t + 8 * i + 4 * hf) = (f32x4){o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+  if (hf == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.nsplit * HD + 2 * at) = make_float2(m, l);
+}
+
+// ------------------------------------------------------------------ launches
+#define QPH_HD(KERNEL, hd, grid, threads, a)                                                    \
+  do {                                                                                          \
+    if ((hd) == 128) hipLaunchKernelGGL((KERNEL<128>), grid, dim3(threads), 0, st, a);          \
+    else hipLaunchKernelGGL((KERNEL<64>), grid, dim3(threads), 0, st, a);                       \
+  } while (0)
+}  // namespace
+
+hipError_t launch_kv_write(int kind, const KvIoArgs &a, hipStream_t st) {
+  if (kind == MK_Q4) QPH_HD(k_kv4_write, a.hd, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
+  else hipLaunchKernelGGL(k_kv16_io<true>, dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+hipError_t launch_kv_read(int kind, const KvIoArgs &a, hipStream_t st) {
+  if (kind == MK_Q4) QPH_HD(k_kv4_read, a.hd, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
+  else hipLaunchKernelGGL(k_kv16_io<false>, dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+size_t kv_attn_plan(KvAttnArgs &a) {
+  const int cus = 256;
+  const bool two = a.q.type == RT_F32;
+  const int64_t cols = (int64_t)a.n * a.rep;
+  a.many = cols > 64;
+  a.cols = a.many ? kManyCols : two ? 8 : 16;
+  a.tile = a.many ? kManyBlk : kFewTile;
+  a.min_tiles = a.many ? 4 : kFewWaves;
+  a.nchunk = (int)((cols + a.cols - 1) / a.cols);
+  // positions that a workgroup can have to read, at most
+  const int64_t reach = a.window > 0 ? std::min<int64_t>(a.ctx, (int64_t)a.window + a.sinks + (a.cols + a.rep - 1) / a.rep + 3 * kRec) : a.ctx;
+  const int64_t tiles = (reach + a.tile - 1) / a.tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
+  const int64_t want = (a.many ? 2 : 4) * (int64_t)cus / std::max<int64_t>(groups, 1);
+  a.nsplit = (int)std::max<int64_t>(1, std::min({want, (tiles + a.min_tiles - 1) / a.min_tiles, (int64_t)64}));
+  if (a.n > 65535) a.nsplit = 1;
+  return a.nsplit > 1 ? (size_t)a.nseq * a.n * a.heads * a.nsplit * (a.hd + 2) * 4 : 0;
+}
+
+template <int HD, int KIND, bool TWO>
+static void launch_one(const KvAttnArgs &a, hipStream_t st) {
+  if (a.many) hipLaunchKernelGGL((k_kv_many<HD, KIND, TWO>), dim3((unsigned)(a.nkv * a.nchunk * a.nsplit), a.nseq), dim3(kManyWaves * 64), 0, st, a);
+  else hipLaunchKernelGGL((k_kv_few<HD, KIND, TWO>), dim3(a.nsplit, a.nkv * a.nchunk, a.nseq), dim3(kFewWaves * 64), 0, st, a);
+}
+hipError_t launch_kv_attn(int kind, const KvAttnArgs &a, hipStream_t st) {
+  const bool two = a.q.type == RT_F32;
+#define QPH_KVA(HD, KIND) (two ? launch_one<HD, KIND, true>(a, st) : launch_one<HD, KIND, false>(a, st))
+  if (kind == MK_Q4) { if (a.hd == 128) QPH_KVA(128, MK_Q4); else QPH_KVA(64, MK_Q4); }
+  else { if (a.hd == 128) QPH_KVA(128, MK_F32); else QPH_KVA(64, MK_F32); }
+#undef QPH_KVA
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.nsplit == 1) return e;
+  QPH_HD(k_kv_merge, a.hd, dim3(a.heads, a.n, a.nseq), 256, a);
+  return hipGetLastError();
+}
+
+}  // namespace qph

@@ -291,6 +291,43 @@ struct PfAttnArgs {
 };
 hipError_t launch_pf_attn(const PfAttnArgs &a, hipStream_t st);
 
+// ---- caches of several sequences, fp16 or 4-bit (kvcache.hip).  kind: MK_Q4, or MK_F32 for fp16
+enum RowType : int { RT_F32 = 0, RT_F16 = 1, RT_BF16 = 2 };
+struct KvRows { void *p; int type; int64_t seq, tok, head; };   // strides in elements; a head's dims are consecutive
+// bytes of a sequence's records of one kv head
+inline int64_t kv4_records(int64_t ctx) { return (ctx + 7) / 8; }
+inline int64_t kv4_bytes(int nseq, int nkv, int hd, int64_t ctx) { return (int64_t)nseq * nkv * kv4_records(ctx) * 9 * hd; }
+// rows k / v of tokens 0 .. lens[b] - 1 (n without lens) of sequence b <-> positions pos[b] .. below ctx; pos[b] < 0: none
+struct KvIoArgs {
+  void *cache, *cache_v;        // 4-bit: the records; fp16: K and V
+  int64_t cseq, crow;           // fp16: elements between sequences, positions
+  int64_t ctx, nrec;            // positions; 4-bit: records of a head
+  int nseq, nkv, hd, n;
+  KvRows k, v;
+  bool vec;                     // k and v: pointers and strides in multiples of 16 bytes
+  const int *pos, *lens;        // device
+};
+hipError_t launch_kv_write(int kind, const KvIoArgs &a, hipStream_t st);
+hipError_t launch_kv_read(int kind, const KvIoArgs &a, hipStream_t st);
+// tokens 0 .. of sequence b at positions pos[b] .., whose rows are in the cache, over positions p <= P with p > P - window
+// (window > 0) or p < sinks
+struct KvAttnArgs {
+  const void *cache, *cache_v;
+  int64_t cseq, crow, ctx, nrec;
+  int nseq, nkv, hd, heads, rep, n;
+  KvRows q, out;
+  bool vec_q, vec_o;
+  const int *pos, *lens;
+  int window, sinks;
+  float scale2;                 // softmax scale times log2(e), > 0
+  float *part;                  // nsplit > 1: partial sums, then (max, sum) pairs, kv_attn_plan's bytes
+  // set by kv_attn_plan
+  int many, cols, nchunk, tile, min_tiles, nsplit;
+};
+// how the call is laid out; the bytes of part
+size_t kv_attn_plan(KvAttnArgs &a);
+hipError_t launch_kv_attn(int kind, const KvAttnArgs &a, hipStream_t st);
+
 // ---- reference-order mode (exact.hip): the reference CPU path's float orders, bit-identical results
 // RMSNorm of `rows` vectors [ldx] with the sequential sum of squares, out [ldo]
 hipError_t launch_ex_rmsnorm(const float *x, int ldx, const float *w, int n, float eps, float *out, int ldo, int rows,
