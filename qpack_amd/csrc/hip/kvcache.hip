@@ -344,20 +344,37 @@ constexpr float kPBias = 14.f;
 //           fragment is dim 16 t + lane % 16 of record lg: one word of V codes.
 // TWO (fp32 queries): 8 columns, with the queries' hi halves in columns 0 .. 7 and their lo halves in 8 .. 15 of the same
 // product, and P's likewise: 22 bits for the price of 11 where no more than 8 columns are needed.
-constexpr int kFewWaves = 8, kFewTile = 32;
+constexpr int kFewWaves = 8, kFewTile = 32, kFewOcc = 4;   // waves of a workgroup, positions of a tile, waves of a SIMD
 
+template <int HD, int KIND>
+struct Tile;
 template <int HD>
-struct Tile4 {   // a tile of a 4-bit cache
-  static constexpr int KW = HD / 32, VW = HD / 16;   // words of a lane: K row piece, V dims
+struct Tile<HD, MK_Q4> {   // a lane's words of a tile: two K row pieces, its V dims of one record
+  static constexpr int KW = HD / 32, VW = HD / 16;
   uint32_t k[2][KW], v[VW];
   uint16_t ks[2];
   u32x4 vs[HD / 32];
 };
 template <int HD>
-__device__ __forceinline__ void load_tile4(const uint8_t *head, const Span &s, int tile, int lane, Tile4<HD> &t) {
+struct Tile<HD, MK_F32> { u32x4 k[2][HD / 32]; };   // an fp16 cache's K; its V goes to LDS
+// a workgroup's part of the cache: its kv head's records, or its rows
+struct Head { const uint8_t *rec; const uint16_t *k, *v; };
+template <int HD, int KIND>
+__device__ __forceinline__ Head head_of(const KvAttnArgs &a, int b, int g) {
+  Head h{};
+  if constexpr (KIND == MK_Q4) h.rec = (const uint8_t *)a.cache + ((int64_t)b * a.nkv + g) * a.nrec * (9 * HD);
+  else { h.k = (const uint16_t *)a.cache + b * a.cseq + g * HD; h.v = (const uint16_t *)a.cache_v + b * a.cseq + g * HD; }
+  return h;
+}
+// records and positions past the span's are the last one's (masked, and in the allocation)
+__device__ __forceinline__ int64_t row_of(const KvAttnArgs &a, const Span &s, int v, int j) {
+  return min((int64_t)kRec * record(s, min(v, s.NR - 1)) + j, a.ctx - 1) * a.crow;
+}
+template <int HD, int KIND>
+__device__ __forceinline__ void load_k(const KvAttnArgs &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t) {
   const int lr = lane & 15, lg = lane >> 4;
-  {
-    const uint8_t *r = head + (int64_t)record(s, min(4 * tile + (lr >> 2), s.NR - 1)) * (9 * HD);
+  if constexpr (KIND == MK_Q4) {
+    const uint8_t *r = h.rec + (int64_t)record(s, min(4 * tile + (lr >> 2), s.NR - 1)) * (9 * HD);
 #pragma unroll
     for (int mt = 0; mt < 2; mt++) {
       const int row = 4 * mt + (lr & 3);
@@ -366,47 +383,47 @@ __device__ __forceinline__ void load_tile4(const uint8_t *head, const Span &s, i
       else { const u32x2 x = *(const u32x2 *)kp; t.k[mt][0] = x[0]; t.k[mt][1] = x[1]; }
       t.ks[mt] = *(const uint16_t *)(r + 8 * HD + 2 * (row * (HD / 32) + lg * HD / 128));
     }
+  } else {
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) {
+      const uint16_t *r = h.k + row_of(a, s, 4 * tile + (lr >> 2), 4 * mt + (lr & 3)) + 8 * lg;
+#pragma unroll
+      for (int k = 0; k < HD / 32; k++) t.k[mt][k] = *(const u32x4 *)(r + 32 * k);
+    }
   }
-  const uint8_t *r = head + (int64_t)record(s, min(4 * tile + lg, s.NR - 1)) * (9 * HD);
-#pragma unroll
-  for (int i = 0; i < HD / 64; i++) {
-    const u32x4 x = *(const u32x4 *)(r + 4 * HD + lr * (HD / 4) + 16 * i);
-#pragma unroll
-    for (int j = 0; j < 4; j++) t.v[4 * i + j] = x[j];
-  }
-#pragma unroll
-  for (int i = 0; i < HD / 32; i++) t.vs[i] = *(const u32x4 *)(r + 8 * HD + HD / 2 + 16 * i);
 }
-template <int HD>
-struct Tile16 { u32x4 k[2][HD / 32]; };   // K of a tile of an fp16 cache; its V goes to LDS
 // 16-byte segment c of V row x sits at c ^ vsw(x): the 8 rows that the 32 lanes of a transpose read address (0 .. 3 or 4 .. 7 of two
 // records) cover all banks
 template <int HD>
 __device__ __forceinline__ int vsw(int x) { return HD == 128 ? 2 * ((x & 3) | (x >> 1 & 4)) : 2 * ((x >> 1 & 1) | (x >> 2 & 2)); }
-template <int HD>
-__device__ __forceinline__ void load_tile16(const KvAttnArgs &a, const uint16_t *kh, const uint16_t *vh, const Span &s, int tile, int lane,
-                                            Tile16<HD> &t, uint16_t *buf) {
+template <int HD, int KIND>
+__device__ __forceinline__ void load_v(const KvAttnArgs &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t, uint16_t *buf) {
   const int lr = lane & 15, lg = lane >> 4;
-  constexpr int SEG = HD / 8, RPI = 64 / SEG;   // 16-byte segments of a row, rows of a 1 KiB load
+  if constexpr (KIND == MK_Q4) {
+    const uint8_t *r = h.rec + (int64_t)record(s, min(4 * tile + lg, s.NR - 1)) * (9 * HD);
 #pragma unroll
-  for (int q = 0; q < kFewTile / RPI; q++) {
-    const int x = q * RPI + lane / SEG, seg = lane % SEG;
-    const int64_t p = min((int64_t)kRec * record(s, min(4 * tile + x / kRec, s.NR - 1)) + x % kRec, a.ctx - 1);
-    dma16(vh + p * a.crow + 8 * (seg ^ vsw<HD>(x)), buf + q * RPI * HD);
-  }
+    for (int i = 0; i < HD / 64; i++) {
+      const u32x4 x = *(const u32x4 *)(r + 4 * HD + lr * (HD / 4) + 16 * i);
 #pragma unroll
-  for (int mt = 0; mt < 2; mt++) {
-    const int64_t p = min((int64_t)kRec * record(s, min(4 * tile + (lr >> 2), s.NR - 1)) + 4 * mt + (lr & 3), a.ctx - 1);
+      for (int j = 0; j < 4; j++) t.v[4 * i + j] = x[j];
+    }
 #pragma unroll
-    for (int k = 0; k < HD / 32; k++) t.k[mt][k] = *(const u32x4 *)(kh + p * a.crow + 32 * k + 8 * lg);
+    for (int i = 0; i < HD / 32; i++) t.vs[i] = *(const u32x4 *)(r + 8 * HD + HD / 2 + 16 * i);
+  } else {
+    constexpr int SEG = HD / 8, RPI = 64 / SEG;   // 16-byte segments of a row, rows of a 1 KiB load
+#pragma unroll
+    for (int q = 0; q < kFewTile / RPI; q++) {
+      const int x = q * RPI + lane / SEG;
+      dma16(h.v + row_of(a, s, 4 * tile + x / kRec, x % kRec) + 8 * (lane % SEG ^ vsw<HD>(x)), buf + q * RPI * HD);
+    }
   }
 }
 
-__device__ __forceinline__ bool not_finite(h8 v) {
-  const u32x4 w = __builtin_bit_cast(u32x4, v);
-  bool bad = false;
+// bits of the elements of v that are NaN or infinite
+__device__ __forceinline__ uint32_t not_finite(u32x4 w) {
+  uint32_t bad = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) bad |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+  for (int i = 0; i < 4; i++) bad |= ((w[i] & 0x7c00u) == 0x7c00u ? 1u << 2 * i : 0u) | ((w[i] & 0x7c000000u) == 0x7c000000u ? 2u << 2 * i : 0u);
   return bad;
 }
 // v with the elements of clear bits of `on` zeroed
@@ -416,45 +433,66 @@ __device__ __forceinline__ h8 only(h8 v, uint32_t on) {
   for (int i = 0; i < 4; i++) w[i] &= (on >> 2 * i & 1 ? 0xffffu : 0u) | (on >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
   return __builtin_bit_cast(h8, w);
 }
+// Where some columns see a position and others don't, its V enters the product without its NaN and infinite values, which
+// would reach every column through 0 x NaN.  They are then added to the columns that see the position, read again from
+// memory: o's dims d .. d + 3 (4-bit: a group's scale is what can be NaN)
+template <int HD, int KIND, typename V>
+__device__ __forceinline__ void add_bad(const uint8_t *rec, const uint16_t *row, int p, int d, bool sees, V &o, int i0) {
+  if constexpr (KIND == MK_Q4) {
+    const uint16_t s = *(const uint16_t *)(rec + 8 * HD + HD / 2 + 16 * (d / 32) + 2 * (p % kRec));
+    if (sees && (s & 0x7c00) == 0x7c00) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i0 + i] += __builtin_nanf("");
+    }
+  } else {
+    const u32x2 w = *(const u32x2 *)(row + d);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint16_t h = (uint16_t)(w[i / 2] >> 16 * (i & 1));
+      if (sees && (h & 0x7c00) == 0x7c00) o[i0 + i] += half_bits_to_float(h);
+    }
+  }
+}
 
 template <int HD, int KIND, bool TWO>
-__global__ __launch_bounds__(kFewWaves * 64) void k_kv_few(KvAttnArgs a) {
+__global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a) {
   constexpr int NW = kFewWaves, KS = HD / 32, DT = HD / 16, NC = TWO ? 8 : 16, QS = HD + 4;
   constexpr int kTileBytes = KIND == MK_Q4 ? 0 : NW * kFewTile * HD * 2, kOutBytes = NW * NC * QS * 4;
   __shared__ __align__(16) uint8_t sm[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
   __shared__ float wm[NW][NC], wl[NW][NC];
   const int b = blockIdx.z, g = blockIdx.y / a.nchunk, c0 = blockIdx.y % a.nchunk * NC, split = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int col = c0 + (TWO ? lr & 7 : lr), tok = col / a.rep;
+  // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j.  Asked for before
+  // the sequence's position is known
+  float x[KS][8];
+  {
+    const bool there = tok < a.n;
+    const int64_t at = b * a.q.seq + (int64_t)(there ? tok : 0) * a.q.tok + (int64_t)(g * a.rep + col % a.rep) * a.q.head;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      load_elems<8>(a.q, at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg), a.vec_q, x[k]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[k][j] = there ? x[k][j] : 0.f;
+    }
+  }
   const Span s = span_of(a, b, c0);
   if (!s.any || split >= s.S) return;
-  const int col = c0 + (TWO ? lr & 7 : lr), tok = col / a.rep;
   const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
   const int t0 = (int)((int64_t)split * s.nt / s.S), t1 = (int)((int64_t)(split + 1) * s.nt / s.S);
-  const uint8_t *head4 = nullptr;
-  const uint16_t *kh = nullptr, *vh = nullptr;
+  const Head h = head_of<HD, KIND>(a, b, g);
   uint16_t *vbuf = (uint16_t *)sm + wave * kFewTile * HD;
-  if constexpr (KIND == MK_Q4) head4 = (const uint8_t *)a.cache + ((int64_t)b * a.nkv + g) * a.nrec * (9 * HD);
-  else { kh = (const uint16_t *)a.cache + b * a.cseq + g * HD; vh = (const uint16_t *)a.cache_v + b * a.cseq + g * HD; }
-  using Tile = typename std::conditional<KIND == MK_Q4, Tile4<HD>, Tile16<HD>>::type;
-  Tile ta, tb;
-  auto load = [&](int tile, Tile &t) {
-    if constexpr (KIND == MK_Q4) load_tile4<HD>(head4, s, tile, lane, t);
-    else load_tile16<HD>(a, kh, vh, s, tile, lane, t, vbuf);
-  };
-  if (t0 + wave < t1) load(t0 + wave, ta);
-  // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j
+  Tile<HD, KIND> cur;
+  if (t0 + wave < t1) { load_v<HD, KIND>(a, h, s, t0 + wave, lane, cur, vbuf); load_k<HD, KIND>(a, h, s, t0 + wave, lane, cur); }
   h8 q[KS];
   float f;   // softmax scale in base 2, times the row's power
   {
-    float x[KS][8], mx = 0.f;
-    const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)(g * a.rep + col % a.rep) * a.q.head;
+    float mx = 0.f;
 #pragma unroll
-    for (int k = 0; k < KS; k++) {
-      if (live) load_elems<8>(a.q, at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg), a.vec_q, x[k]);
+    for (int k = 0; k < KS; k++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) { if (!live) x[k][j] = 0.f; mx = fmaxf(mx, fabsf(x[k][j])); }
-    }
+      for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
     mx = pair_max32(pair_max16(mx));
     const float p2 = row_power(mx);
     f = a.scale2 / p2;
@@ -463,40 +501,21 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_kv_few(KvAttnArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const float y = x[k][j] * p2;
-        const _Float16 h = (_Float16)y;
-        q[k][j] = TWO && lr >= 8 ? (_Float16)(y - (float)h) : h;
+        const _Float16 hi = (_Float16)y;
+        q[k][j] = TWO && lr >= 8 ? (_Float16)(y - (float)hi) : hi;
       }
   }
   f32x4 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; d++) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  auto step = [&](Tile &cur, Tile &nxt, int tile) {
+  // the next tile's K is asked for once this one's is used, its V likewise: either is on its way during the other's product
+  for (int tile = t0 + wave; tile < t1; tile += NW) {
     const int v = 4 * tile + lg, p0 = kRec * record(s, min(v, s.NR - 1));
     const bool in = v < s.NR;
-    // positions of the tile that some column does not see: its first and last record bound the others
+    // whether some column does not see all of the tile: its first and last position bound the others
     const int pf = kRec * record(s, 4 * tile), pl = kRec * record(s, min(4 * tile + 3, s.NR - 1)) + kRec - 1;
     const bool edge = 4 * tile + 4 > s.NR || pl > s.PA || (a.window > 0 && pf <= s.PB - a.window && pl >= a.sinks);
-    h8 vf[DT];
-    if constexpr (KIND != MK_Q4) {
-      // K's registers were asked for after V's tile: once they are here, it is
-#pragma unroll
-      for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-        for (int k = 0; k < KS; k++) asm volatile("" ::"v"(cur.k[mt][k]));
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      // ds_read_b64_tr_b16 hands lane i of 16 the element i % 4 of what lanes 4 j + i / 4 address, as its element j
-      const int x = 8 * lg + (lr >> 2), dq = 4 * (lr & 3);
-#pragma unroll
-      for (int d = 0; d < DT; d++) {
-        const int seg = (16 * d + dq) >> 3, in8 = dq & 4;
-        const s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + x * HD + 8 * (seg ^ vsw<HD>(x)) + in8));
-        const s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + (x + 4) * HD + 8 * (seg ^ vsw<HD>(x + 4)) + in8));
-        vf[d] = __builtin_bit_cast(h8, (s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile is read before the next one's loads write it
-    }
-    if (tile + NW < t1) load(tile + NW, nxt);
     f32x4 sc[2];
 #pragma unroll
     for (int mt = 0; mt < 2; mt++) {
@@ -509,20 +528,26 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_kv_few(KvAttnArgs a) {
         sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[k], sc[mt], 0, 0, 0);
       }
     }
-    float x[8], bm = -INFINITY;
-    uint32_t some = 0;   // positions that a column of the workgroup may see
+    if constexpr (KIND == MK_Q4) { if (tile + NW < t1) load_k<HD, KIND>(a, h, s, tile + NW, lane, cur); }
+    float y[8], bm = -INFINITY;
+    uint32_t on = 255;   // positions that a column of the workgroup sees
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      float y = sc[j >> 2][j & 3];
-      if (TWO) y += xchg8_f(y);
-      y *= f;
-      if (edge) {
-        const int p = p0 + j;
-        if (!(in && sees(a, P, p))) y = -INFINITY;
-        some |= in && p <= s.PB && (p >= s.ws || p < a.sinks) ? 1u << j : 0u;
-      }
-      x[j] = y; bm = fmaxf(bm, y);
+      y[j] = sc[j >> 2][j & 3];
+      if (TWO) y[j] += xchg8_f(y[j]);
+      y[j] *= f;
     }
+    if (edge) {
+      on = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int p = p0 + j;
+        if (!(in && sees(a, P, p))) y[j] = -INFINITY;
+        on |= in && p <= s.PB && (p >= s.ws || p < a.sinks) ? 1u << j : 0u;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) bm = fmaxf(bm, y[j]);
     bm = pair_max32(pair_max16(bm));
     const float mn = fmaxf(m, bm), mz = mn == -INFINITY ? 0.f : mn;
     const float corr = __builtin_amdgcn_exp2f(m - mz);
@@ -530,46 +555,61 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_kv_few(KvAttnArgs a) {
     h8 ph;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const float pv = __builtin_amdgcn_exp2f(x[j] - mz + kPBias);
+      const float pv = __builtin_amdgcn_exp2f(y[j] - mz + kPBias);
       rs += pv;
-      const _Float16 h = (_Float16)pv;
-      ph[j] = TWO && lr >= 8 ? (_Float16)(pv - (float)h) : h;
+      const _Float16 hi = (_Float16)pv;
+      ph[j] = TWO && lr >= 8 ? (_Float16)(pv - (float)hi) : hi;
     }
     rs = pair_sum32(pair_sum16(rs));
     l = l * corr + rs;
-    m = mn;
+    if (__any(mn != m)) {
 #pragma unroll
-    for (int d = 0; d < DT; d++) {
-      o[d] *= corr;
-      if constexpr (KIND == MK_Q4) vf[d] = values(cur.v[d], cur.vs[d / 2]);
+      for (int d = 0; d < DT; d++) o[d] *= corr;
     }
-    if (edge) {
-      // what no column sees may hold anything: zeroed, since 0 x NaN is not 0.  What some columns see and others don't, the
-      // tokens one at a time, and only where it matters
-      bool bad = false;
+    m = mn;
+    // what no column sees may hold anything: zeroed (4-bit: its scales), since 0 x NaN is not 0; what only some see, without its
+    // NaN and infinite values
+    uint32_t bad = 0;
+    auto clean = [&](u32x4 w) {
+      uint32_t keep = on;
+      if (s.PA != s.PB) { const uint32_t n = not_finite(w) & on; bad |= n; keep &= ~n; }
+      return __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, w), keep));
+    };
+    if constexpr (KIND == MK_Q4) {
+      if (edge) {
 #pragma unroll
-      for (int d = 0; d < DT; d++) { vf[d] = only(vf[d], some); bad |= not_finite(vf[d]); }
-      if (s.PA != s.PB && __any(bad)) {
-        for (int Pt = s.PA; Pt <= s.PB; Pt++) {
-          uint32_t on = 0;
+        for (int i = 0; i < HD / 32; i++) cur.vs[i] = clean(cur.vs[i]);
+      }
 #pragma unroll
-          for (int j = 0; j < 8; j++) on |= in && sees(a, Pt, p0 + j) ? 1u << j : 0u;
+      for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values(cur.v[d], cur.vs[d / 2]), ph, o[d], 0, 0, 0);
+    } else {
+      // V's tile in LDS (a wait written out, since the compiler does not see what the loads write)
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (tile + NW < t1) load_k<HD, KIND>(a, h, s, tile + NW, lane, cur);
+      // ds_read_b64_tr_b16 hands lane i of 16 the element i % 4 of what lanes 4 j + i / 4 address, as its element j
+      const int xr = 8 * lg + (lr >> 2), dq = 4 * (lr & 3);
 #pragma unroll
-          for (int d = 0; d < DT; d++) {
-            const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(only(vf[d], on), ph, o[d], 0, 0, 0);
-            if (P == Pt) o[d] = y;
-          }
-        }
-        return;
+      for (int d = 0; d < DT; d++) {
+        const int seg = (16 * d + dq) >> 3, in8 = dq & 4;
+        const s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + xr * HD + 8 * (seg ^ vsw<HD>(xr)) + in8));
+        const s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + (xr + 4) * HD + 8 * (seg ^ vsw<HD>(xr + 4)) + in8));
+        u32x4 w = __builtin_bit_cast(u32x4, (s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+        if (edge) w = clean(w);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, w), ph, o[d], 0, 0, 0);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile is read before the next one's loads write it
+    }
+    if (tile + NW < t1) load_v<HD, KIND>(a, h, s, tile + NW, lane, cur, vbuf);
+    if (__any(bad != 0)) {
+#pragma unroll 1
+      for (int i = 0; i < kFewTile; i++) {   // record i / 8 is lane group i / 8's
+        if (!(__ballot(bad >> (i % kRec) & 1) >> 16 * (i / kRec) & 0xffff)) continue;
+        const int r = record(s, 4 * tile + i / kRec), p = kRec * r + i % kRec;
+        const bool sp = sees(a, P, p) && (!TWO || lr < 8);
+#pragma unroll
+        for (int d = 0; d < DT; d++) add_bad<HD, KIND>(h.rec + (int64_t)r * (9 * HD), h.v + (int64_t)p * a.crow, p, 16 * d + 4 * lg, sp, o[d], 0);
       }
     }
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph, o[d], 0, 0, 0);
-  };
-  for (int t = t0 + wave; t < t1; t += 2 * NW) {
-    step(ta, tb, t);
-    if (t + NW >= t1) break;
-    step(tb, ta, t + NW);
   }
   // the waves' sums meet in LDS
   if (KIND != MK_Q4) __syncthreads();   // no wave's V tile is in use
@@ -667,7 +707,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   constexpr int VN = KIND == MK_Q4 ? HD * VST : kManyBlk * VST;
   __shared__ __align__(16) uint16_t ks[2][kManyBlk * KST];
   __shared__ __align__(16) uint16_t vs[2][VN];
-  __shared__ int badf[3];   // block kb's at (kb - kb0) % 3: set while kb - 1 is computed, read with kb, cleared with kb + 1
+  __shared__ uint32_t badp[3][2];   // positions of block kb left to add_bad, at (kb - kb0) % 3: set while kb - 1 is computed, read with kb, cleared with kb + 1
   const int b = blockIdx.y, g = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv, split = rest % a.nsplit;
   const int c0 = (a.nchunk - 1 - rest / a.nsplit) * kManyCols;   // the last columns, with the most to read, first
   const Span s = span_of(a, b, c0);
@@ -681,8 +721,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   const bool wlive = wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
   const int PA = s.P0 + wa, PB = (int)min((int64_t)s.P0 + min((c0 + 32 * wave + 31) / a.rep, s.cnt - 1), a.ctx - 1);
   const int kb0 = (int)((int64_t)split * s.nt / s.S), kb1 = (int)((int64_t)(split + 1) * s.nt / s.S);
-  const uint8_t *head4 = (const uint8_t *)a.cache + ((int64_t)b * a.nkv + g) * a.nrec * (9 * HD);
-  const uint16_t *kh = (const uint16_t *)a.cache + b * a.cseq + g * HD, *vh = (const uint16_t *)a.cache_v + b * a.cseq + g * HD;
+  const Head hd = head_of<HD, KIND>(a, b, g);
 
   // ---- a block's codes (or fp16 pieces): memory -> registers -> LDS
   constexpr int NP = KIND == MK_Q4 ? 1 : kManyBlk * HD / 8 / NT;
@@ -694,20 +733,20 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if constexpr (KIND == MK_Q4) {
       if (!kAll && tid >= HD * 4) return;
       const int row = tid / (HD / 16), wp = tid % (HD / 16);
-      const uint8_t *r = head4 + (int64_t)record(s, min(BR * kb + row / kRec, s.NR - 1)) * (9 * HD);
+      const uint8_t *r = hd.rec + (int64_t)record(s, min(BR * kb + row / kRec, s.NR - 1)) * (9 * HD);
       kq = *(const u32x2 *)(r + row % kRec * (HD / 2) + 8 * wp);
       ksc = *(const uint16_t *)(r + 8 * HD + 2 * (row % kRec * (HD / 32) + wp / 2));
       const int rl = tid / (HD / 2), w = 2 * (tid % (HD / 2));
-      const uint8_t *q = head4 + (int64_t)record(s, min(BR * kb + rl, s.NR - 1)) * (9 * HD);
+      const uint8_t *q = hd.rec + (int64_t)record(s, min(BR * kb + rl, s.NR - 1)) * (9 * HD);
       vq = *(const u32x2 *)(q + 4 * HD + 4 * w);
       vsc = *(const u32x4 *)(q + 8 * HD + HD / 2 + 16 * (w % (HD / 16) / 2));
     } else {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        const int64_t p = min((int64_t)kRec * record(s, min(BR * kb + x / kRec, s.NR - 1)) + x % kRec, a.ctx - 1);
-        kp[i] = *(const u32x4 *)(kh + p * a.crow + 8 * sg);
-        vp[i] = *(const u32x4 *)(vh + p * a.crow + 8 * sg);
+        const int64_t at = row_of(a, s, BR * kb + x / kRec, x % kRec) + 8 * sg;
+        kp[i] = *(const u32x4 *)(hd.k + at);
+        vp[i] = *(const u32x4 *)(hd.v + at);
       }
     }
   };
@@ -733,11 +772,14 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
         const int v = BR * kb + rl, p0 = kRec * record(s, min(v, s.NR - 1));
 #pragma unroll
         for (int j = 0; j < kRec; j++) on |= any_sees(v, p0 + j) ? 1u << j : 0u;
+        const uint32_t bad = on & not_finite(vsc);
+        if (bad) atomicOr(&badp[(kb - kb0) % 3][rl / 4], bad << 8 * (rl % 4));
+        on &= ~bad;
       }
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         h8 x = values(vq[i], vsc);
-        if (edge) { x = only(x, on); if (not_finite(x)) badf[(kb - kb0) % 3] = 1; }
+        if (edge) x = only(x, on);
         *(h8 *)(vs[buf] + (d + 16 * i) * VST + kRec * rl) = x;
       }
     } else {
@@ -749,13 +791,16 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
         if (edge) {
           const int v = BR * kb + x / kRec;
           if (!any_sees(v, kRec * record(s, min(v, s.NR - 1)) + x % kRec)) w = (u32x4){0u, 0u, 0u, 0u};
-          if (not_finite(__builtin_bit_cast(h8, w))) badf[(kb - kb0) % 3] = 1;
+          if (const uint32_t bad = not_finite(w)) {
+            atomicOr(&badp[(kb - kb0) % 3][x / 32], 1u << x % 32);
+            w = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, w), ~bad));
+          }
         }
         *(u32x4 *)(vs[buf] + x * VST + 8 * sg) = w;
       }
     }
   };
-  if (tid < 3) badf[tid] = 0;
+  if (tid < 6) badp[tid / 2][tid % 2] = 0;
   fetch(kb0);
   // ---- queries
   h8 q[KQ], ql[TWO ? KQ : 1];
@@ -851,26 +896,6 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       for (int t = 0; t < OT; t++) o[t] *= corr;
     }
     m = mn;
-    if (edge && badf[(kb - kb0) % 3]) {
-      for (int Pt = PA; Pt <= PB; Pt++) {   // see k_kv_few
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          asm volatile("" ::: "memory");   // the fragments are read again for each token, not kept in registers
-          const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1));
-          uint32_t on = 0;
-#pragma unroll
-          for (int j = 0; j < 8; j++) on |= v < s.NR && sees(a, Pt, p0 + j) ? 1u << j : 0u;
-#pragma unroll
-          for (int t = 0; t < OT; t++) {
-            const h8 x = only(vfrag(vl, t, u), on);
-            f32x16 y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[u], o[t], 0, 0, 0);
-            if constexpr (TWO) y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[u], y, 0, 0, 0);
-            if (P == Pt) o[t] = y;
-          }
-        }
-      }
-      return;
-    }
 #pragma unroll
     for (int t = 0; t < OT; t++)
 #pragma unroll
@@ -879,8 +904,23 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[u], o[t], 0, 0, 0);
         if constexpr (TWO) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[u], o[t], 0, 0, 0);
       }
+    if (partial(kb, s.PA, s.PB)) {   // (some other wave's columns may be the ones that don't see all of it)
+#pragma unroll 1
+      for (int w = 0; w < 2; w++) {
+        uint32_t bad = __builtin_amdgcn_readfirstlane(badp[(kb - kb0) % 3][w]);
+        while (bad) {
+          const int x = 32 * w + __builtin_ctz(bad), r = record(s, BR * kb + x / kRec), p = kRec * r + x % kRec;
+          const bool sp = sees(a, P, p);
+          bad &= bad - 1;
+#pragma unroll
+          for (int t = 0; t < OT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) add_bad<HD, KIND>(hd.rec + (int64_t)r * (9 * HD), hd.v + (int64_t)p * a.crow, p, 32 * t + 8 * i + 4 * hf, sp, o[t], 4 * i);
+        }
+      }
+    }
   };
-  __syncthreads();   // badf
+  __syncthreads();   // badp
   expand(kb0, 0);
   if (kb0 + 1 < kb1) fetch(kb0 + 1);
   __syncthreads();
@@ -890,7 +930,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (kb + 2 < kb1) fetch(kb + 2);
     const int pf = first(kb), pl = last(kb);
     if (wlive && pf <= PB && !(a.window > 0 && pl <= PA - a.window && pf >= a.sinks)) block(kb, buf);
-    if (tid == 0) badf[(kb - kb0 + 2) % 3] = 0;
+    if (tid < 2) badp[(kb - kb0 + 2) % 3][tid] = 0;
     __syncthreads();
   }
   if (!live) return;
@@ -946,7 +986,7 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   // positions that a workgroup can have to read, at most
   const int64_t reach = a.window > 0 ? std::min<int64_t>(a.ctx, (int64_t)a.window + a.sinks + (a.cols + a.rep - 1) / a.rep + 3 * kRec) : a.ctx;
   const int64_t tiles = (reach + a.tile - 1) / a.tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
-  const int64_t want = (a.many ? 2 : 4) * (int64_t)cus / std::max<int64_t>(groups, 1);
+  const int64_t want = (a.many ? 1 : 2) * (int64_t)cus / std::max<int64_t>(groups, 1);
   a.nsplit = (int)std::max<int64_t>(1, std::min({want, (tiles + a.min_tiles - 1) / a.min_tiles, (int64_t)64}));
   if (a.n > 65535) a.nsplit = 1;
   return a.nsplit > 1 ? (size_t)a.nseq * a.n * a.heads * a.nsplit * (a.hd + 2) * 4 : 0;
