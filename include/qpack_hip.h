@@ -201,7 +201,7 @@ typedef struct {
   int64_t seq, row;
 } qph_kv;
 /* rows of tokens: sequence b, token t, head h at p + b * seq + t * tok + h * head elements of type (QPH_F32, QPH_F16 or
- * QPH_BF16), head_dim consecutive ones.  Any alignment of the type; 16-byte aligned pointers and strides are faster */
+ * QPH_BF16), head_dim consecutive ones, at any alignment of the type */
 typedef struct {
   void *p;
   int type;

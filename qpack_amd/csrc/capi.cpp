@@ -68,10 +68,6 @@ static qph::KvRows kv_rows(const qph_rows *r, const char *what, bool out, int ns
   if (out && ((nseq > 1 && r->seq < hd) || (n > 1 && r->tok < hd) || (heads > 1 && r->head < hd))) throw std::invalid_argument(std::string("kv: the rows of ") + what + " overlap");
   return {r->p, r->type == QPH_F32 ? qph::RT_F32 : r->type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16, r->seq, r->tok, r->head};
 }
-static bool kv_vec(const qph::KvRows &r) {
-  const int e = r.type == qph::RT_F32 ? 4 : 8;
-  return (uintptr_t)r.p % 16 == 0 && r.seq % e == 0 && r.tok % e == 0 && r.head % e == 0;
-}
 static qph::KvIoArgs kv_io(const qph_kv *c, const qph_rows *k, const qph_rows *v, bool out, int n, const int *pos, const int *lens) {
   qph::KvIoArgs a{};
   kv_cache(c, &a.cseq, &a.crow);
@@ -81,7 +77,6 @@ static qph::KvIoArgs kv_io(const qph_kv *c, const qph_rows *k, const qph_rows *v
   a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.n = n; a.pos = pos; a.lens = lens;
   a.k = kv_rows(k, "k", out, c->nseq, n, c->kv_heads, c->head_dim); a.v = kv_rows(v, "v", out, c->nseq, n, c->kv_heads, c->head_dim);
   if (a.k.type != a.v.type) throw std::invalid_argument("kv: k and v must have the same type");
-  a.vec = kv_vec(a.k) && kv_vec(a.v);
   return a;
 }
 static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sinks, qph::KvAttnArgs &a) {
@@ -436,7 +431,6 @@ int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, in
     a.q = kv_rows(q, "q", false, c->nseq, n, heads, c->head_dim); a.out = kv_rows(out, "out", true, c->nseq, n, heads, c->head_dim);
     if (a.q.type != a.out.type) throw std::invalid_argument("kv: q and out must have the same type");
     if (!(scale >= 0.f) || std::isinf(scale)) throw std::invalid_argument("kv: scale must be finite and not negative (0: 1 / sqrt(head_dim))");
-    a.vec_q = kv_vec(a.q); a.vec_o = kv_vec(a.out);
     a.pos = pos; a.lens = lens;
     a.scale2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim));
     if (n) {

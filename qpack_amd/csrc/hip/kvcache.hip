@@ -45,62 +45,44 @@ __device__ __forceinline__ uint16_t f_to_bf16(float f) {
   return (uint16_t)((u + 0x7fff + (u >> 16 & 1)) >> 16);
 }
 
-// N (a multiple of 4) consecutive elements from element offset `at` of rows of a type; vec: 16-byte loads (the pointer and
-// the strides are multiples of 16 bytes, and so is every offset that the kernels ask for)
-template <int N>
-__device__ __forceinline__ void load_elems(const KvRows &r, int64_t at, bool vec, float *x) {
-  if (r.type == RT_F32) {
-    const float *p = (const float *)r.p + at;
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < N; i += 4) { const f32x4 v = *(const f32x4 *)(p + i); x[i] = v[0]; x[i + 1] = v[1]; x[i + 2] = v[2]; x[i + 3] = v[3]; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; i++) x[i] = p[i];
-    }
-    return;
-  }
-  const uint16_t *p = (const uint16_t *)r.p + at;
-  uint16_t h[N];
-  if (vec && N % 8 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 8) {
-      const u32x4 v = *(const u32x4 *)(p + i);
-#pragma unroll
-      for (int j = 0; j < 8; j++) h[i + j] = (uint16_t)(v[j / 2] >> 16 * (j & 1));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) h[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < N; i++) x[i] = r.type == RT_F16 ? half_bits_to_float(h[i]) : bf16_to_f(h[i]);
-}
-__device__ __forceinline__ uint16_t to_elem16(int type, float f) { return type == RT_F16 ? float_to_half_bits(f) : f_to_bf16(f); }
-template <int N>
-__device__ __forceinline__ void store_elems(const KvRows &r, int64_t at, bool vec, const float *x) {
-  if (r.type == RT_F32) {
-    float *p = (float *)r.p + at;
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < N; i += 4) *(f32x4 *)(p + i) = (f32x4){x[i], x[i + 1], x[i + 2], x[i + 3]};
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; i++) p[i] = x[i];
-    }
-    return;
-  }
-  uint16_t *p = (uint16_t *)r.p + at;
-  if (vec) {
+// N (a multiple of 8) consecutive elements of type T (RowType) from element `at` of rows.  The loads and stores are 16 (8) bytes at any alignment of
+// the type, which the memory pipeline takes as they are: a second, element by element, path made the kernels twice as
+// long, and their first pass through the instruction cache is what a short call waits for
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+template <int T, int N>
+__device__ __forceinline__ void load_elems(const KvRows &r, int64_t at, float *x) {
+  if constexpr (T == RT_F32) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const uint32_t a = to_elem16(r.type, x[i]) | (uint32_t)to_elem16(r.type, x[i + 1]) << 16;
-      const uint32_t b = to_elem16(r.type, x[i + 2]) | (uint32_t)to_elem16(r.type, x[i + 3]) << 16;
-      *(u32x2 *)(p + i) = (u32x2){a, b};
+      const u32x4 v = *(const u32x4_any *)((const float *)r.p + at + i);
+#pragma unroll
+      for (int j = 0; j < 4; j++) { const uint32_t w = v[j]; x[i + j] = __builtin_bit_cast(float, w); }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) p[i] = to_elem16(r.type, x[i]);
+    for (int i = 0; i < N; i += 8) {
+      const u32x4 v = *(const u32x4_any *)((const uint16_t *)r.p + at + i);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const uint16_t h = (uint16_t)(v[j / 2] >> 16 * (j & 1));
+        x[i + j] = T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h);
+      }
+    }
+  }
+}
+// N a multiple of 4
+template <int T, int N>
+__device__ __forceinline__ void store_elems(const KvRows &r, int64_t at, const float *x) {
+  auto e = [](float f) { return (uint32_t)(T == RT_F16 ? float_to_half_bits(f) : f_to_bf16(f)); };
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    if constexpr (T == RT_F32) {
+      *(u32x4_any *)((float *)r.p + at + i) = (u32x4){__builtin_bit_cast(uint32_t, x[i]), __builtin_bit_cast(uint32_t, x[i + 1]), __builtin_bit_cast(uint32_t, x[i + 2]),
+                                                      __builtin_bit_cast(uint32_t, x[i + 3])};
+    } else {
+      *(u32x2_any *)((uint16_t *)r.p + at + i) = (u32x2){e(x[i]) | e(x[i + 1]) << 16, e(x[i + 2]) | e(x[i + 3]) << 16};
+    }
   }
 }
 
@@ -157,7 +139,7 @@ __device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
 // call's keep their codes and scales: their K rows and scales are not stored, and the V words, which hold all 8
 // positions, are read and merged where the call covers a part only (no other workgroup of the launch has the record).
 // Bound by memory for prompts and by latency for single tokens.
-template <int HD>
+template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   constexpr int EL = HD / 8, GL = 32 / EL;   // elements of a lane; lanes of a group
   __shared__ __align__(16) uint8_t codes[kRec][HD];
@@ -174,7 +156,7 @@ __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   float x[EL];
   uint32_t mx = 0;
   if (mine) {
-    load_elems<EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, a.vec, x);
+    load_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x);
 #pragma unroll
     for (int i = 0; i < EL; i++) mx = max(mx, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
   }
@@ -228,7 +210,7 @@ __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   }
 }
 
-template <int HD>
+template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
   constexpr int EL = HD / 8, GL = 32 / EL;
   const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 63, vside = threadIdx.x >> 6;
@@ -258,11 +240,11 @@ __global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
     }
   }
   const KvRows &r = vside ? a.v : a.k;
-  store_elems<EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, a.vec, x);
+  store_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x);
 }
 
 // the fp16 cache's: a copy with a conversion, 8 dims of one position's K and V a thread
-template <bool WRITE>
+template <bool WRITE, int T>
 __global__ __launch_bounds__(256) void k_kv16_io(KvIoArgs a) {
   const int b = blockIdx.z, per = a.nkv * a.hd / 8;
   const int P0 = a.pos[b], cnt = tokens_of(a.lens, b, a.n);
@@ -276,7 +258,7 @@ __global__ __launch_bounds__(256) void k_kv16_io(KvIoArgs a) {
   float x[8];
   u32x4 w;
   if (WRITE) {
-    load_elems<8>(r, at, a.vec, x);
+    load_elems<T, 8>(r, at, x);
 #pragma unroll
     for (int j = 0; j < 4; j++) w[j] = float_to_half_bits(x[2 * j]) | (uint32_t)float_to_half_bits(x[2 * j + 1]) << 16;
     *(u32x4 *)c = w;
@@ -284,7 +266,7 @@ __global__ __launch_bounds__(256) void k_kv16_io(KvIoArgs a) {
     w = *(const u32x4 *)c;
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = half_bits_to_float((uint16_t)(w[j / 2] >> 16 * (j & 1)));
-    store_elems<8>(r, at, a.vec, x);
+    store_elems<T, 8>(r, at, x);
   }
 }
 
@@ -318,9 +300,15 @@ __device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int c0) {
   return s;
 }
 __device__ __forceinline__ int record(const Span &s, int v) { return v < s.SR ? v : v + s.skip; }
-// whether the token at P sees position p
-__device__ __forceinline__ bool sees(const KvAttnArgs &a, int P, int p) {
-  return p <= P && (a.window <= 0 || p > P - a.window || p < a.sinks);
+// whether the token at P, whose window starts behind lo, sees position p (no short cuts: these are lanes' values)
+__device__ __forceinline__ int behind(const KvAttnArgs &a, int P) { return a.window > 0 ? P - a.window : -1; }
+__device__ __forceinline__ bool sees(const KvAttnArgs &a, int P, int lo, int p) { return (p <= P) & ((p > lo) | (p < a.sinks)); }
+// bits of the positions p0 + j, j < 8, that some token of the workgroup sees
+__device__ __forceinline__ uint32_t seen_bits(const KvAttnArgs &a, const Span &s, int v, int p0) {
+  uint32_t on = 0;
+#pragma unroll
+  for (int j = 0; j < kRec; j++) on |= (uint32_t)((p0 + j <= s.PB) & ((p0 + j >= s.ws) | (p0 + j < a.sinks))) << j;
+  return v < s.NR ? on : 0;
 }
 
 // Queries enter as fp16, each row scaled by the power of two that brings its largest magnitude into [1, 2): fp16 and bf16
@@ -331,9 +319,10 @@ __device__ __forceinline__ float row_power(float mx) {   // 2^-e; 1 for rows tha
   return e == 0 || e >= 254 ? 1.f : __builtin_bit_cast(float, (254u - e) << 23);
 }
 
-// probabilities are held as 2^(x - m + 14): in fp16 what lies 2^-38 below the largest is still there, and the sum
-// they are divided by is scaled alike
-constexpr float kPBias = 14.f;
+// Probabilities are held as 2^(x - m + kPBias) where m follows the running maximum of a column only when that is more than kLag
+// above it: o is rescaled in few tiles rather than in most.  They stay below 2^(kPBias + kLag), fp16's range, and what lies 2^-32
+// below m is still there; the sum they are divided by is scaled alike.
+constexpr float kPBias = 8.f, kLag = 7.f;
 
 // ------------------------------------------------------------------ few tokens
 // Grid (split, kv head and column chunk, sequence), 8 waves, each streaming its own tiles of 32 positions (4 records) with
@@ -454,8 +443,9 @@ __device__ __forceinline__ void add_bad(const uint8_t *rec, const uint16_t *row,
   }
 }
 
-template <int HD, int KIND, bool TWO>
+template <int HD, int KIND, int T>
 __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a) {
+  constexpr bool TWO = T == RT_F32;
   constexpr int NW = kFewWaves, KS = HD / 32, DT = HD / 16, NC = TWO ? 8 : 16, QS = HD + 4;
   constexpr int kTileBytes = KIND == MK_Q4 ? 0 : NW * kFewTile * HD * 2, kOutBytes = NW * NC * QS * 4;
   __shared__ __align__(16) uint8_t sm[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
@@ -471,7 +461,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
     const int64_t at = b * a.q.seq + (int64_t)(there ? tok : 0) * a.q.tok + (int64_t)(g * a.rep + col % a.rep) * a.q.head;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
-      load_elems<8>(a.q, at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg), a.vec_q, x[k]);
+      load_elems<T, 8>(a.q, at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg), x[k]);
 #pragma unroll
       for (int j = 0; j < 8; j++) x[k][j] = there ? x[k][j] : 0.f;
     }
@@ -480,6 +470,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   if (!s.any || split >= s.S) return;
   const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
+  const int lo = behind(a, P);
   const int t0 = (int)((int64_t)split * s.nt / s.S), t1 = (int)((int64_t)(split + 1) * s.nt / s.S);
   const Head h = head_of<HD, KIND>(a, b, g);
   uint16_t *vbuf = (uint16_t *)sm + wave * kFewTile * HD;
@@ -511,8 +502,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   float m = -INFINITY, l = 0.f;
   // the next tile's K is asked for once this one's is used, its V likewise: either is on its way during the other's product
   for (int tile = t0 + wave; tile < t1; tile += NW) {
-    const int v = 4 * tile + lg, p0 = kRec * record(s, min(v, s.NR - 1));
-    const bool in = v < s.NR;
+    const int v = 4 * tile + lg, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
     // whether some column does not see all of the tile: its first and last position bound the others
     const int pf = kRec * record(s, 4 * tile), pl = kRec * record(s, min(4 * tile + 3, s.NR - 1)) + kRec - 1;
     const bool edge = 4 * tile + 4 > s.NR || pl > s.PA || (a.window > 0 && pf <= s.PB - a.window && pl >= a.sinks);
@@ -538,35 +528,36 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       y[j] *= f;
     }
     if (edge) {
-      on = 0;
+      on = seen_bits(a, s, v, p0);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int p = p0 + j;
-        if (!(in && sees(a, P, p))) y[j] = -INFINITY;
-        on |= in && p <= s.PB && (p >= s.ws || p < a.sinks) ? 1u << j : 0u;
-      }
+      for (int j = 0; j < 8; j++) y[j] = sees(a, Pin, lo, p0 + j) ? y[j] : -INFINITY;
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) bm = fmaxf(bm, y[j]);
     bm = pair_max32(pair_max16(bm));
-    const float mn = fmaxf(m, bm), mz = mn == -INFINITY ? 0.f : mn;
-    const float corr = __builtin_amdgcn_exp2f(m - mz);
+    float corr = 1.f;
+    const bool up = __any(bm > m + kLag);
+    if (up) {
+      const float mn = fmaxf(m, bm);
+      corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+    }
+    const float sub = kPBias - (m == -INFINITY ? 0.f : m);
     float rs = 0.f;
     h8 ph;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const float pv = __builtin_amdgcn_exp2f(y[j] - mz + kPBias);
+      const float pv = __builtin_amdgcn_exp2f(y[j] + sub);
       rs += pv;
       const _Float16 hi = (_Float16)pv;
       ph[j] = TWO && lr >= 8 ? (_Float16)(pv - (float)hi) : hi;
     }
     rs = pair_sum32(pair_sum16(rs));
     l = l * corr + rs;
-    if (__any(mn != m)) {
+    if (up) {
 #pragma unroll
       for (int d = 0; d < DT; d++) o[d] *= corr;
     }
-    m = mn;
     // what no column sees may hold anything: zeroed (4-bit: its scales), since 0 x NaN is not 0; what only some see, without its
     // NaN and infinite values
     uint32_t bad = 0;
@@ -605,7 +596,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       for (int i = 0; i < kFewTile; i++) {   // record i / 8 is lane group i / 8's
         if (!(__ballot(bad >> (i % kRec) & 1) >> 16 * (i / kRec) & 0xffff)) continue;
         const int r = record(s, 4 * tile + i / kRec), p = kRec * r + i % kRec;
-        const bool sp = sees(a, P, p) && (!TWO || lr < 8);
+        const bool sp = sees(a, P, lo, p) & (!TWO | (lr < 8));
 #pragma unroll
         for (int d = 0; d < DT; d++) add_bad<HD, KIND>(h.rec + (int64_t)r * (9 * HD), h.v + (int64_t)p * a.crow, p, 16 * d + 4 * lg, sp, o[d], 0);
       }
@@ -646,7 +637,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
     float r[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) r[i] = y[i] * inv;
-    store_elems<4>(a.out, b * a.out.seq + (int64_t)tk * a.out.tok + (int64_t)head * a.out.head + d, a.vec_o, r);
+    store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tk * a.out.tok + (int64_t)head * a.out.head + d, r);
     return;
   }
   const int64_t row = ((int64_t)b * a.n + tk) * a.heads + head, at = row * a.nsplit + split;
@@ -656,7 +647,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
 
 // The splits' sums of one row a workgroup: 256 threads, HD / 4 of them side by side over the dims, the others over the
 // splits.  M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L
-template <int HD>
+template <int HD, int T>
 __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
   constexpr int CT = HD / 4, SL = 256 / CT;
   __shared__ f32x4 oo[SL][CT];
@@ -684,7 +675,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
   float r[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) r[i] = y[i] * inv;
-  store_elems<4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, a.vec_o, r);
+  store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, r);
 }
 
 // ------------------------------------------------------------------ many tokens
@@ -699,15 +690,16 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 // TWO (fp32 queries): hi and lo halves of the queries and probabilities as products of their own.
 constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
 
-template <int HD, int KIND, bool TWO>
+template <int HD, int KIND, int T>
 __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
+  constexpr bool TWO = T == RT_F32;
   constexpr int NT = kManyWaves * 64, KQ = HD / 16, OT = HD / 32, BR = kManyBlk / kRec;
   constexpr int KST = HD + 8;                                   // halves of a K row in LDS: an odd number of 16-byte columns
   constexpr int VST = KIND == MK_Q4 ? kManyBlk + 8 : HD + 32;   // of a V^T row (dims), or a V row (positions): 4 rows of 64 bytes apart
   constexpr int VN = KIND == MK_Q4 ? HD * VST : kManyBlk * VST;
   __shared__ __align__(16) uint16_t ks[2][kManyBlk * KST];
-  __shared__ __align__(16) uint16_t vs[2][VN];
-  __shared__ uint32_t badp[3][2];   // positions of block kb left to add_bad, at (kb - kb0) % 3: set while kb - 1 is computed, read with kb, cleared with kb + 1
+  __shared__ __align__(16) uint16_t vs[3][VN];
+  __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 1, read in kb and kb + 1, cleared in kb + 2
   const int b = blockIdx.y, g = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv, split = rest % a.nsplit;
   const int c0 = (a.nchunk - 1 - rest / a.nsplit) * kManyCols;   // the last columns, with the most to read, first
   const Span s = span_of(a, b, c0);
@@ -716,6 +708,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   const int col = c0 + 32 * wave + ln, tok = col / a.rep, head = g * a.rep + col % a.rep;
   const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
+  const int lo = behind(a, P);
   // the wave's own first and last token
   const int wa = (c0 + 32 * wave) / a.rep;
   const bool wlive = wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
@@ -729,22 +722,31 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   u32x2 kq, vq;
   uint16_t ksc;
   u32x4 vsc, kp[NP], vp[NP];
+  // the thread's offsets from a block's first record (position); blocks whose records follow each other and are all there
+  // take them as they are
+  const int krow = tid / (HD / 16), kwp = tid % (HD / 16), vrl = tid / (HD / 2), vw = 2 * (tid % (HD / 2));
+  const int ko = krow / kRec * (9 * HD) + krow % kRec * (HD / 2) + 8 * kwp, kso = krow / kRec * (9 * HD) + 8 * HD + 2 * (krow % kRec * (HD / 32) + kwp / 2);
+  const int vo = vrl * (9 * HD) + 4 * HD + 4 * vw, vso = vrl * (9 * HD) + 8 * HD + HD / 2 + 16 * (vw % (HD / 16) / 2);
   auto fetch = [&](int kb) {
+    const int v0 = BR * kb;
+    const bool plain = v0 + BR <= s.NR && (s.skip == 0 || v0 >= s.SR || v0 + BR <= s.SR);
     if constexpr (KIND == MK_Q4) {
       if (!kAll && tid >= HD * 4) return;
-      const int row = tid / (HD / 16), wp = tid % (HD / 16);
-      const uint8_t *r = hd.rec + (int64_t)record(s, min(BR * kb + row / kRec, s.NR - 1)) * (9 * HD);
-      kq = *(const u32x2 *)(r + row % kRec * (HD / 2) + 8 * wp);
-      ksc = *(const uint16_t *)(r + 8 * HD + 2 * (row % kRec * (HD / 32) + wp / 2));
-      const int rl = tid / (HD / 2), w = 2 * (tid % (HD / 2));
-      const uint8_t *q = hd.rec + (int64_t)record(s, min(BR * kb + rl, s.NR - 1)) * (9 * HD);
-      vq = *(const u32x2 *)(q + 4 * HD + 4 * w);
-      vsc = *(const u32x4 *)(q + 8 * HD + HD / 2 + 16 * (w % (HD / 16) / 2));
+      const uint8_t *r = hd.rec + (int64_t)record(s, v0) * (9 * HD), *rv = r;
+      if (!plain) {
+        r = hd.rec + ((int64_t)record(s, min(v0 + krow / kRec, s.NR - 1)) - krow / kRec) * (9 * HD);
+        rv = hd.rec + ((int64_t)record(s, min(v0 + vrl, s.NR - 1)) - vrl) * (9 * HD);
+        kq = *(const u32x2 *)(r + ko); ksc = *(const uint16_t *)(r + kso);
+        vq = *(const u32x2 *)(rv + vo); vsc = *(const u32x4 *)(rv + vso);
+        return;
+      }
+      kq = *(const u32x2 *)(r + ko); ksc = *(const uint16_t *)(r + kso);
+      vq = *(const u32x2 *)(rv + vo); vsc = *(const u32x4 *)(rv + vso);
     } else {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        const int64_t at = row_of(a, s, BR * kb + x / kRec, x % kRec) + 8 * sg;
+        const int64_t at = row_of(a, s, v0 + x / kRec, x % kRec) + 8 * sg;
         kp[i] = *(const u32x4 *)(hd.k + at);
         vp[i] = *(const u32x4 *)(hd.v + at);
       }
@@ -757,50 +759,49 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     const int pf = first(kb), pl = last(kb);
     return BR * kb + BR > s.NR || pl > A || (a.window > 0 && pf <= B - a.window && pl >= a.sinks);
   };
-  auto any_sees = [&](int v, int p) { return v < s.NR && p <= s.PB && (p >= s.ws || p < a.sinks); };
-  auto expand = [&](int kb, int buf) {
+  auto expand = [&](int kb) {
+    uint16_t *vt = vs[kb % 3];
     const bool edge = partial(kb, s.PA, s.PB);
     if constexpr (KIND == MK_Q4) {
       if (!kAll && tid >= HD * 4) return;
-      const int row = tid / (HD / 16), wp = tid % (HD / 16);
 #pragma unroll
-      for (int i = 0; i < 2; i++) *(h8 *)(ks[buf] + row * KST + 16 * wp + 8 * i) = values(kq[i], ksc);
-      const int rl = tid / (HD / 2), w = 2 * (tid % (HD / 2)), d = w % (HD / 16) * 16 + w / (HD / 16);
+      for (int i = 0; i < 2; i++) *(h8 *)(ks[kb & 1] + krow * KST + 16 * kwp + 8 * i) = values(kq[i], ksc);
+      const int rl = vrl, d = vw % (HD / 16) * 16 + vw / (HD / 16);
       uint32_t on = 255;
       if (edge) {
-        on = 0;
-        const int v = BR * kb + rl, p0 = kRec * record(s, min(v, s.NR - 1));
-#pragma unroll
-        for (int j = 0; j < kRec; j++) on |= any_sees(v, p0 + j) ? 1u << j : 0u;
+        const int v = BR * kb + rl;
+        on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1)));
         const uint32_t bad = on & not_finite(vsc);
-        if (bad) atomicOr(&badp[(kb - kb0) % 3][rl / 4], bad << 8 * (rl % 4));
+        if (bad) atomicOr(&badp[(kb - kb0) % 4][rl / 4], bad << 8 * (rl % 4));
         on &= ~bad;
       }
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         h8 x = values(vq[i], vsc);
         if (edge) x = only(x, on);
-        *(h8 *)(vs[buf] + (d + 16 * i) * VST + kRec * rl) = x;
+        *(h8 *)(vt + (d + 16 * i) * VST + kRec * rl) = x;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        *(u32x4 *)(ks[buf] + x * KST + 8 * sg) = kp[i];
+        *(u32x4 *)(ks[kb & 1] + x * KST + 8 * sg) = kp[i];
         u32x4 w = vp[i];
         if (edge) {
           const int v = BR * kb + x / kRec;
-          if (!any_sees(v, kRec * record(s, min(v, s.NR - 1)) + x % kRec)) w = (u32x4){0u, 0u, 0u, 0u};
+          const bool on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))) >> x % kRec & 1;
+#pragma unroll
+          for (int j = 0; j < 4; j++) w[j] = on ? w[j] : 0u;
           if (const uint32_t bad = not_finite(w)) {
-            atomicOr(&badp[(kb - kb0) % 3][x / 32], 1u << x % 32);
+            atomicOr(&badp[(kb - kb0) % 4][x / 32], 1u << x % 32);
             w = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, w), ~bad));
           }
         }
-        *(u32x4 *)(vs[buf] + x * VST + 8 * sg) = w;
+        *(u32x4 *)(vt + x * VST + 8 * sg) = w;
       }
     }
   };
-  if (tid < 6) badp[tid / 2][tid % 2] = 0;
+  if (tid < 8) badp[tid / 2][tid % 2] = 0;
   fetch(kb0);
   // ---- queries
   h8 q[KQ], ql[TWO ? KQ : 1];
@@ -810,7 +811,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)head * a.q.head;
 #pragma unroll
     for (int k = 0; k < KQ; k++) {
-      if (live) load_elems<8>(a.q, at + 16 * k + 8 * hf, a.vec_q, x[k]);
+      if (live) load_elems<T, 8>(a.q, at + 16 * k + 8 * hf, x[k]);
 #pragma unroll
       for (int j = 0; j < 8; j++) { if (!live) x[k][j] = 0.f; mx = fmaxf(mx, fabsf(x[k][j])); }
     }
@@ -844,8 +845,9 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   };
-  auto block = [&](int kb, int buf) {
-    const uint16_t *kl = ks[buf], *vl = vs[buf];
+  h8 ph[4], pl[TWO ? 4 : 1];
+  auto scores = [&](int kb) {   // -> ph, pl; o and l brought to the new maximum
+    const uint16_t *kl = ks[kb & 1];
     const bool edge = partial(kb, PA, PB);
     f32x16 sc[2];
 #pragma unroll
@@ -863,10 +865,9 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (edge) {
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1));
+        const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (!(v < s.NR && sees(a, P, p0 + j))) sc[u >> 1][8 * (u & 1) + j] = -INFINITY;
+        for (int j = 0; j < 8; j++) sc[u >> 1][8 * (u & 1) + j] = sees(a, Pin, lo, p0 + j) ? sc[u >> 1][8 * (u & 1) + j] : -INFINITY;
       }
     }
 #pragma unroll
@@ -874,28 +875,35 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[mt][i]);
     bm = pair_max32(bm) * f;   // f > 0
-    const float mn = fmaxf(m, bm), mz = mn == -INFINITY ? 0.f : mn;
-    const float corr = __builtin_amdgcn_exp2f(m - mz);
-    const float sub = kPBias - mz;
-    float rs = 0.f;
-    h8 ph[4], pl[TWO ? 4 : 1];
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][8 * (u & 1) + j], f, sub));
-        rs += pv;
-        const _Float16 h = (_Float16)pv;
-        ph[u][j] = h;
-        if constexpr (TWO) pl[u][j] = (_Float16)(pv - (float)h);
-      }
-    rs = pair_sum32(rs);
-    l = l * corr + rs;
-    if (__any(mn != m)) {
+    if (__any(bm > m + kLag)) {
+      const float mn = fmaxf(m, bm), corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= corr;
 #pragma unroll
       for (int t = 0; t < OT; t++) o[t] *= corr;
     }
-    m = mn;
+    const float sub = kPBias - (m == -INFINITY ? 0.f : m);
+    float rs = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][8 * (u & 1) + j], f, sub));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][8 * (u & 1) + j + 1], f, sub));
+        const h2 h = {(_Float16)p0, (_Float16)p1};
+        ph[u][j] = h[0]; ph[u][j + 1] = h[1];
+        if constexpr (TWO) {
+          rs += p0; rs += p1;
+          pl[u][j] = (_Float16)(p0 - (float)h[0]); pl[u][j + 1] = (_Float16)(p1 - (float)h[1]);
+        } else {
+          rs = __builtin_amdgcn_fdot2(h, (h2){(_Float16)1.f, (_Float16)1.f}, rs, false);   // the sum of what the product takes
+        }
+      }
+    rs = pair_sum32(rs);
+    l += rs;
+  };
+  auto product = [&](int kb) {
+    const uint16_t *vl = vs[kb % 3];
 #pragma unroll
     for (int t = 0; t < OT; t++)
 #pragma unroll
@@ -907,10 +915,10 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (partial(kb, s.PA, s.PB)) {   // (some other wave's columns may be the ones that don't see all of it)
 #pragma unroll 1
       for (int w = 0; w < 2; w++) {
-        uint32_t bad = __builtin_amdgcn_readfirstlane(badp[(kb - kb0) % 3][w]);
+        uint32_t bad = __builtin_amdgcn_readfirstlane(badp[(kb - kb0) % 4][w]);
         while (bad) {
           const int x = 32 * w + __builtin_ctz(bad), r = record(s, BR * kb + x / kRec), p = kRec * r + x % kRec;
-          const bool sp = sees(a, P, p);
+          const bool sp = sees(a, P, lo, p);
           bad &= bad - 1;
 #pragma unroll
           for (int t = 0; t < OT; t++)
@@ -921,16 +929,24 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     }
   };
   __syncthreads();   // badp
-  expand(kb0, 0);
+  expand(kb0);
   if (kb0 + 1 < kb1) fetch(kb0 + 1);
   __syncthreads();
-  for (int kb = kb0; kb < kb1; kb++) {
-    const int buf = (kb - kb0) & 1;
-    if (kb + 1 < kb1) expand(kb + 1, buf ^ 1);
+  // Step kb: block kb + 1 expanded, kb + 2 asked for, kb computed.  Waves w and w + 4 share a SIMD; the upper four run their value
+  // product a step late, first thing, so that of the two one feeds the matrix cores (P V, then K q) while the other one works
+  // on codes and exponentials.
+  const bool late = wave >= kManyWaves / 2;
+  bool mine = false;
+  for (int kb = kb0; kb <= kb1; kb++) {
+    if (late && mine) product(kb - 1);
+    if (kb == kb1) break;
+    if (kb + 1 < kb1) expand(kb + 1);
     if (kb + 2 < kb1) fetch(kb + 2);
-    const int pf = first(kb), pl = last(kb);
-    if (wlive && pf <= PB && !(a.window > 0 && pl <= PA - a.window && pf >= a.sinks)) block(kb, buf);
-    if (tid < 2) badp[(kb - kb0 + 2) % 3][tid] = 0;
+    const int pf = first(kb), pe = last(kb);
+    mine = wlive && pf <= PB && !(a.window > 0 && pe <= PA - a.window && pf >= a.sinks);
+    if (mine) scores(kb);
+    if (!late && mine) product(kb);
+    if (tid < 2) badp[(kb - kb0 + 2) % 4][tid] = 0;
     __syncthreads();
   }
   if (!live) return;
@@ -942,7 +958,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float r[4] = {o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv};
-        store_elems<4>(a.out, at + 32 * t + 8 * i + 4 * hf, a.vec_o, r);
+        store_elems<T, 4>(a.out, at + 32 * t + 8 * i + 4 * hf, r);
       }
     return;
   }
@@ -956,21 +972,37 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
 }
 
 // ------------------------------------------------------------------ launches
-#define QPH_HD(KERNEL, hd, grid, threads, a)                                                    \
-  do {                                                                                          \
-    if ((hd) == 128) hipLaunchKernelGGL((KERNEL<128>), grid, dim3(threads), 0, st, a);          \
-    else hipLaunchKernelGGL((KERNEL<64>), grid, dim3(threads), 0, st, a);                       \
+// KERNEL<HD, T> by head dim and rows' type
+#define QPH_KV(KERNEL, hd, type, grid, threads, a)                                                                      \
+  do {                                                                                                                  \
+    const dim3 g_ = (grid), t_(threads);                                                                                \
+    if ((hd) == 128) {                                                                                                  \
+      if ((type) == RT_F32) hipLaunchKernelGGL((KERNEL<128, RT_F32>), g_, t_, 0, st, a);                                \
+      else if ((type) == RT_F16) hipLaunchKernelGGL((KERNEL<128, RT_F16>), g_, t_, 0, st, a);                           \
+      else hipLaunchKernelGGL((KERNEL<128, RT_BF16>), g_, t_, 0, st, a);                                                \
+    } else {                                                                                                            \
+      if ((type) == RT_F32) hipLaunchKernelGGL((KERNEL<64, RT_F32>), g_, t_, 0, st, a);                                 \
+      else if ((type) == RT_F16) hipLaunchKernelGGL((KERNEL<64, RT_F16>), g_, t_, 0, st, a);                            \
+      else hipLaunchKernelGGL((KERNEL<64, RT_BF16>), g_, t_, 0, st, a);                                                 \
+    }                                                                                                                   \
   } while (0)
+template <bool WRITE>
+void launch_io16(const KvIoArgs &a, hipStream_t st) {
+  const dim3 grid((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), thr(256);
+  if (a.k.type == RT_F32) hipLaunchKernelGGL((k_kv16_io<WRITE, RT_F32>), grid, thr, 0, st, a);
+  else if (a.k.type == RT_F16) hipLaunchKernelGGL((k_kv16_io<WRITE, RT_F16>), grid, thr, 0, st, a);
+  else hipLaunchKernelGGL((k_kv16_io<WRITE, RT_BF16>), grid, thr, 0, st, a);
+}
 }  // namespace
 
 hipError_t launch_kv_write(int kind, const KvIoArgs &a, hipStream_t st) {
-  if (kind == MK_Q4) QPH_HD(k_kv4_write, a.hd, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
-  else hipLaunchKernelGGL(k_kv16_io<true>, dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
+  if (kind == MK_Q4) QPH_KV(k_kv4_write, a.hd, a.k.type, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
+  else launch_io16<true>(a, st);
   return hipGetLastError();
 }
 hipError_t launch_kv_read(int kind, const KvIoArgs &a, hipStream_t st) {
-  if (kind == MK_Q4) QPH_HD(k_kv4_read, a.hd, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
-  else hipLaunchKernelGGL(k_kv16_io<false>, dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
+  if (kind == MK_Q4) QPH_KV(k_kv4_read, a.hd, a.k.type, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
+  else launch_io16<false>(a, st);
   return hipGetLastError();
 }
 
@@ -992,20 +1024,23 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   return a.nsplit > 1 ? (size_t)a.nseq * a.n * a.heads * a.nsplit * (a.hd + 2) * 4 : 0;
 }
 
-template <int HD, int KIND, bool TWO>
-static void launch_one(const KvAttnArgs &a, hipStream_t st) {
-  if (a.many) hipLaunchKernelGGL((k_kv_many<HD, KIND, TWO>), dim3((unsigned)(a.nkv * a.nchunk * a.nsplit), a.nseq), dim3(kManyWaves * 64), 0, st, a);
-  else hipLaunchKernelGGL((k_kv_few<HD, KIND, TWO>), dim3(a.nsplit, a.nkv * a.nchunk, a.nseq), dim3(kFewWaves * 64), 0, st, a);
-}
+template <int HD, int T> static constexpr auto k_few4 = k_kv_few<HD, MK_Q4, T>;
+template <int HD, int T> static constexpr auto k_few16 = k_kv_few<HD, MK_F32, T>;
+template <int HD, int T> static constexpr auto k_many4 = k_kv_many<HD, MK_Q4, T>;
+template <int HD, int T> static constexpr auto k_many16 = k_kv_many<HD, MK_F32, T>;
 hipError_t launch_kv_attn(int kind, const KvAttnArgs &a, hipStream_t st) {
-  const bool two = a.q.type == RT_F32;
-#define QPH_KVA(HD, KIND) (two ? launch_one<HD, KIND, true>(a, st) : launch_one<HD, KIND, false>(a, st))
-  if (kind == MK_Q4) { if (a.hd == 128) QPH_KVA(128, MK_Q4); else QPH_KVA(64, MK_Q4); }
-  else { if (a.hd == 128) QPH_KVA(128, MK_F32); else QPH_KVA(64, MK_F32); }
-#undef QPH_KVA
+  if (a.many) {
+    const dim3 grid((unsigned)(a.nkv * a.nchunk * a.nsplit), a.nseq);
+    if (kind == MK_Q4) QPH_KV(k_many4, a.hd, a.q.type, grid, kManyWaves * 64, a);
+    else QPH_KV(k_many16, a.hd, a.q.type, grid, kManyWaves * 64, a);
+  } else {
+    const dim3 grid(a.nsplit, a.nkv * a.nchunk, a.nseq);
+    if (kind == MK_Q4) QPH_KV(k_few4, a.hd, a.q.type, grid, kFewWaves * 64, a);
+    else QPH_KV(k_few16, a.hd, a.q.type, grid, kFewWaves * 64, a);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nsplit == 1) return e;
-  QPH_HD(k_kv_merge, a.hd, dim3(a.heads, a.n, a.nseq), 256, a);
+  QPH_KV(k_kv_merge, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a);
   return hipGetLastError();
 }
 

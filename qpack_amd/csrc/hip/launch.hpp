@@ -304,7 +304,6 @@ struct KvIoArgs {
   int64_t ctx, nrec;            // positions; 4-bit: records of a head
   int nseq, nkv, hd, n;
   KvRows k, v;
-  bool vec;                     // k and v: pointers and strides in multiples of 16 bytes
   const int *pos, *lens;        // device
 };
 hipError_t launch_kv_write(int kind, const KvIoArgs &a, hipStream_t st);
@@ -316,7 +315,6 @@ struct KvAttnArgs {
   int64_t cseq, crow, ctx, nrec;
   int nseq, nkv, hd, heads, rep, n;
   KvRows q, out;
-  bool vec_q, vec_o;
   const int *pos, *lens;
   int window, sinks;
   float scale2;                 // softmax scale times log2(e), > 0
