@@ -91,13 +91,14 @@ __host__ __device__ constexpr int nib(int i) { return 16 * (i & 1) + 4 * (i >> 1
 
 // a word's 8 values in element order.  Codes 0 .. 15 in the low mantissa bits of fp16 1024 (or, four bits higher, 16 times
 // them, brought back by an exact fma): c - 8 exact, times the elements' scales exact
+__device__ __forceinline__ uint32_t vreg(uint32_t c) { asm("" : "+v"(c)); return c; }   // an instruction reads one scalar: v_and_or_b32 wants the other constant in a vector register
 __device__ __forceinline__ h2 code_pair(uint32_t w, int e) {
   const h2 k1032 = {(_Float16)1032.f, (_Float16)1032.f}, k16 = {(_Float16)0.0625f, (_Float16)0.0625f}, k72 = {(_Float16)-72.f, (_Float16)-72.f};
   if (e & 1) {
-    const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x00f000f0u) | 0x64006400u);
+    const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x00f000f0u) | vreg(0x64006400u));
     return __builtin_elementwise_fma(x, k16, k72);
   }
-  const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x000f000fu) | 0x64006400u);
+  const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x000f000fu) | vreg(0x64006400u));
   return x - k1032;
 }
 // scales of the four element pairs: one for all (K: a group of dims), or the positions' own (V)
@@ -282,13 +283,26 @@ struct Span {
   int nt, S;        // tiles of a.tile positions, splits in use
   bool any;
 };
-__device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int c0) {
+// The columns of a chunk: a.cols from chunk * a.cols on, or, paired (many tokens, no window), half of them from the front and half from
+// the back.  A causal workgroup's time goes with its last position: paired, all take about as long (see k_kv_many)
+__device__ __forceinline__ int chunk_half(const KvAttnArgs &a, int chunk, int h) {   // the first column of half h
+  return (a.paired ? (h ? 2 * a.nchunk - 1 - chunk : chunk) : 2 * chunk + h) * (a.cols / 2);
+}
+__device__ __forceinline__ int chunk_of(const KvAttnArgs &a, int col) {
+  const int u = col / (a.cols / 2);
+  return a.paired ? min(u, 2 * a.nchunk - 1 - u) : u / 2;
+}
+__device__ __forceinline__ int last_token(const KvAttnArgs &a, int first) { return (first + a.cols / 2 - 1) / a.rep; }   // of a half
+__device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int chunk) {
   Span s;
   s.P0 = a.pos[b]; s.cnt = tokens_of(a.lens, b, a.n);
-  const int ta = c0 / a.rep;
+  const int ta = chunk_half(a, chunk, 0) / a.rep, tb = last_token(a, chunk_half(a, chunk, 1));
   s.any = s.P0 >= 0 && ta < s.cnt && (int64_t)s.P0 + ta < a.ctx;
   s.PA = s.P0 + ta;
-  s.PB = (int)min((int64_t)s.P0 + min((c0 + a.cols - 1) / a.rep, s.cnt - 1), a.ctx - 1);
+  // paired, the back half may lie behind the sequence's tokens while the front half does not reach them
+  int te = min(tb, s.cnt - 1);
+  if (a.paired && chunk_half(a, chunk, 1) / a.rep >= s.cnt) te = min(last_token(a, chunk_half(a, chunk, 0)), s.cnt - 1);
+  s.PB = (int)min((int64_t)s.P0 + te, a.ctx - 1);
   s.ws = a.window > 0 ? max(0, s.PA - a.window + 1) : 0;
   const int r0 = s.ws / kRec;
   s.SR = min((int)(((int64_t)a.sinks + kRec - 1) / kRec), r0);
@@ -322,7 +336,7 @@ __device__ __forceinline__ float row_power(float mx) {   // 2^-e; 1 for rows tha
 // Probabilities are held as 2^(x - m + kPBias) where m follows the running maximum of a column only when that is more than kLag
 // above it: o is rescaled in few tiles rather than in most.  They stay below 2^(kPBias + kLag), fp16's range, and what lies 2^-32
 // below m is still there; the sum they are divided by is scaled alike.
-constexpr float kPBias = 8.f, kLag = 7.f;
+constexpr float kPBias = 8.f, kLag = 7.f, kRoom = 32768.f;   // kRoom: what a sum of weights may reach before the maximum is looked for
 
 // ------------------------------------------------------------------ few tokens
 // Grid (split, kv head and column chunk, sequence), 8 waves, each streaming its own tiles of 32 positions (4 records) with
@@ -450,7 +464,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   constexpr int kTileBytes = KIND == MK_Q4 ? 0 : NW * kFewTile * HD * 2, kOutBytes = NW * NC * QS * 4;
   __shared__ __align__(16) uint8_t sm[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
   __shared__ float wm[NW][NC], wl[NW][NC];
-  const int b = blockIdx.z, g = blockIdx.y / a.nchunk, c0 = blockIdx.y % a.nchunk * NC, split = blockIdx.x;
+  const int b = blockIdx.z, g = blockIdx.y / a.nchunk, chunk = blockIdx.y % a.nchunk, c0 = chunk * NC, split = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int col = c0 + (TWO ? lr & 7 : lr), tok = col / a.rep;
   // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j.  Asked for before
@@ -466,7 +480,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       for (int j = 0; j < 8; j++) x[k][j] = there ? x[k][j] : 0.f;
     }
   }
-  const Span s = span_of(a, b, c0);
+  const Span s = span_of(a, b, chunk);
   if (!s.any || split >= s.S) return;
   const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
@@ -653,7 +667,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
   __shared__ f32x4 oo[SL][CT];
   const int head = blockIdx.x, tok = blockIdx.y, b = blockIdx.z, g = head / a.rep;
   const int col = tok * a.rep + head - g * a.rep;
-  const Span s = span_of(a, b, col / a.cols * a.cols);
+  const Span s = span_of(a, b, chunk_of(a, col));
   if (!s.any || s.S == 1 || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
   const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
   const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.nsplit * HD) + row * a.nsplit;
@@ -694,54 +708,58 @@ template <int HD, int KIND, int T>
 __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   constexpr bool TWO = T == RT_F32;
   constexpr int NT = kManyWaves * 64, KQ = HD / 16, OT = HD / 32, BR = kManyBlk / kRec;
+  constexpr bool kAhead = !TWO || HD == 64;
   constexpr int KST = HD + 8;                                   // halves of a K row in LDS: an odd number of 16-byte columns
   constexpr int VST = KIND == MK_Q4 ? kManyBlk + 8 : HD + 32;   // of a V^T row (dims), or a V row (positions): 4 rows of 64 bytes apart
   constexpr int VN = KIND == MK_Q4 ? HD * VST : kManyBlk * VST;
-  __shared__ __align__(16) uint16_t ks[2][kManyBlk * KST];
+  constexpr int KR = kAhead ? 2 : 3;   // K blocks in LDS: block kb is read in step kb - 1 (without kAhead in step kb), kb + 2 written in step kb
+  __shared__ __align__(16) uint16_t ks[KR][kManyBlk * KST];
   __shared__ __align__(16) uint16_t vs[3][VN];
-  __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 1, read in kb and kb + 1, cleared in kb + 2
+  __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
   const int b = blockIdx.y, g = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv, split = rest % a.nsplit;
-  const int c0 = (a.nchunk - 1 - rest / a.nsplit) * kManyCols;   // the last columns, with the most to read, first
-  const Span s = span_of(a, b, c0);
+  const int chunk = a.nchunk - 1 - rest / a.nsplit;   // without pairs: the last columns, with the most to read, first
+  const Span s = span_of(a, b, chunk);
   if (!s.any || split >= s.S) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, ln = lane & 31, hf = lane >> 5;
-  const int col = c0 + 32 * wave + ln, tok = col / a.rep, head = g * a.rep + col % a.rep;
+  // waves w and w + 4 share a SIMD: one of the front half, one of the back half
+  const int cw = chunk_half(a, chunk, wave / (kManyWaves / 2)) + 32 * (wave % (kManyWaves / 2));
+  const int col = cw + ln, tok = col / a.rep, head = g * a.rep + col % a.rep;
   const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
   const int lo = behind(a, P);
-  // the wave's own first and last token
-  const int wa = (c0 + 32 * wave) / a.rep;
+  // first and last position of the wave's own columns, and of the halves'
+  const int wa = cw / a.rep;
   const bool wlive = wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
-  const int PA = s.P0 + wa, PB = (int)min((int64_t)s.P0 + min((c0 + 32 * wave + 31) / a.rep, s.cnt - 1), a.ctx - 1);
+  auto position = [&](int t) { return (int)min((int64_t)s.P0 + min(t, s.cnt - 1), a.ctx - 1); };
+  const int PA = s.P0 + wa, PB = position((cw + 31) / a.rep);
+  const int A0 = s.PA, B0 = position(last_token(a, chunk_half(a, chunk, 0))), A1 = s.P0 + chunk_half(a, chunk, 1) / a.rep, B1 = s.PB;
   const int kb0 = (int)((int64_t)split * s.nt / s.S), kb1 = (int)((int64_t)(split + 1) * s.nt / s.S);
   const Head hd = head_of<HD, KIND>(a, b, g);
 
   // ---- a block's codes (or fp16 pieces): memory -> registers -> LDS
-  constexpr int NP = KIND == MK_Q4 ? 1 : kManyBlk * HD / 8 / NT;
-  constexpr bool kAll = KIND != MK_Q4 || HD * 4 == NT;   // every thread has a share
-  u32x2 kq, vq;
+  // 4-bit: a thread has W words of a K row, and W of a record's V: dims 16 (W vt + i) + vr of record vl, so that the 16 lanes of a
+  // group write V^T rows next to each other.  fp16: pieces tid + NT i
+  constexpr int W = HD / 64, NP = KIND == MK_Q4 ? 1 : kManyBlk * HD / 8 / NT;
+  typedef uint32_t words __attribute__((ext_vector_type(W)));
+  words kq, vq;
   uint16_t ksc;
   u32x4 vsc, kp[NP], vp[NP];
-  // the thread's offsets from a block's first record (position); blocks whose records follow each other and are all there
-  // take them as they are
-  const int krow = tid / (HD / 16), kwp = tid % (HD / 16), vrl = tid / (HD / 2), vw = 2 * (tid % (HD / 2));
-  const int ko = krow / kRec * (9 * HD) + krow % kRec * (HD / 2) + 8 * kwp, kso = krow / kRec * (9 * HD) + 8 * HD + 2 * (krow % kRec * (HD / 32) + kwp / 2);
-  const int vo = vrl * (9 * HD) + 4 * HD + 4 * vw, vso = vrl * (9 * HD) + 8 * HD + HD / 2 + 16 * (vw % (HD / 16) / 2);
+  const int krow = tid >> 3, kw = tid & 7, vl = tid >> 6, vr = tid & 15, vt = tid >> 4 & 3;
+  const uint32_t ko = krow / kRec * (9 * HD) + krow % kRec * (HD / 2) + 4 * W * kw, kso = krow / kRec * (9 * HD) + 8 * HD + 2 * (krow % kRec * (HD / 32) + W * kw / 4);
+  const uint32_t vo = vl * (9 * HD) + 4 * HD + vr * (HD / 4) + 4 * W * vt, vso = vl * (9 * HD) + 8 * HD + HD / 2 + 16 * (W * vt / 2);
   auto fetch = [&](int kb) {
     const int v0 = BR * kb;
-    const bool plain = v0 + BR <= s.NR && (s.skip == 0 || v0 >= s.SR || v0 + BR <= s.SR);
     if constexpr (KIND == MK_Q4) {
-      if (!kAll && tid >= HD * 4) return;
-      const uint8_t *r = hd.rec + (int64_t)record(s, v0) * (9 * HD), *rv = r;
-      if (!plain) {
-        r = hd.rec + ((int64_t)record(s, min(v0 + krow / kRec, s.NR - 1)) - krow / kRec) * (9 * HD);
-        rv = hd.rec + ((int64_t)record(s, min(v0 + vrl, s.NR - 1)) - vrl) * (9 * HD);
-        kq = *(const u32x2 *)(r + ko); ksc = *(const uint16_t *)(r + kso);
-        vq = *(const u32x2 *)(rv + vo); vsc = *(const u32x4 *)(rv + vso);
-        return;
+      if (v0 + BR <= s.NR && (s.skip == 0 || v0 >= s.SR || v0 + BR <= s.SR)) {   // records that follow each other
+        const uint8_t *r = hd.rec + (int64_t)record(s, v0) * (9 * HD);
+        kq = *(const words *)(r + ko); ksc = *(const uint16_t *)(r + kso);
+        vq = *(const words *)(r + vo); vsc = *(const u32x4 *)(r + vso);
+      } else {
+        const uint8_t *r = hd.rec + ((int64_t)record(s, min(v0 + krow / kRec, s.NR - 1)) - krow / kRec) * (9 * HD);
+        const uint8_t *rv = hd.rec + ((int64_t)record(s, min(v0 + vl, s.NR - 1)) - vl) * (9 * HD);
+        kq = *(const words *)(r + ko); ksc = *(const uint16_t *)(r + kso);
+        vq = *(const words *)(rv + vo); vsc = *(const u32x4 *)(rv + vso);
       }
-      kq = *(const u32x2 *)(r + ko); ksc = *(const uint16_t *)(r + kso);
-      vq = *(const u32x2 *)(rv + vo); vsc = *(const u32x4 *)(rv + vso);
     } else {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
@@ -759,45 +777,42 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     const int pf = first(kb), pl = last(kb);
     return BR * kb + BR > s.NR || pl > A || (a.window > 0 && pf <= B - a.window && pl >= a.sinks);
   };
-  auto expand = [&](int kb) {
-    uint16_t *vt = vs[kb % 3];
-    const bool edge = partial(kb, s.PA, s.PB);
+  // the same of the waves that take the block: a wave does not take a block behind its last position
+  auto partial_any = [&](int kb) {
+    const int pf = first(kb);
+    return BR * kb + BR > s.NR || (pf <= B0 && partial(kb, A0, B0)) || (pf <= B1 && partial(kb, A1, B1));
+  };
+  // what no column sees zeroed, and what only some see without its NaN and infinite values (4-bit: by the scales)
+  auto clean = [&](int kb) {
     if constexpr (KIND == MK_Q4) {
-      if (!kAll && tid >= HD * 4) return;
+      const int v = BR * kb + vl;
+      const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))), bad = on & not_finite(vsc);
+      if (bad) atomicOr(&badp[(kb - kb0) % 4][vl / 4], bad << 8 * (vl % 4));
+      vsc = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, vsc), on & ~bad));
+    } else {
 #pragma unroll
-      for (int i = 0; i < 2; i++) *(h8 *)(ks[kb & 1] + krow * KST + 16 * kwp + 8 * i) = values(kq[i], ksc);
-      const int rl = vrl, d = vw % (HD / 16) * 16 + vw / (HD / 16);
-      uint32_t on = 255;
-      if (edge) {
-        const int v = BR * kb + rl;
-        on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1)));
-        const uint32_t bad = on & not_finite(vsc);
-        if (bad) atomicOr(&badp[(kb - kb0) % 4][rl / 4], bad << 8 * (rl % 4));
-        on &= ~bad;
+      for (int i = 0; i < NP; i++) {
+        const int x = (tid + NT * i) / (HD / 8), v = BR * kb + x / kRec;
+        const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))) >> x % kRec & 1 ? 255u : 0u, bad = on & not_finite(vp[i]);
+        if (bad) atomicOr(&badp[(kb - kb0) % 4][x / 32], 1u << x % 32);
+        vp[i] = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, vp[i]), on & ~bad));
       }
+    }
+  };
+  auto expand = [&](int kb) {
+    uint16_t *kd = ks[kb % KR], *vd = vs[kb % 3];
+    if constexpr (KIND == MK_Q4) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        h8 x = values(vq[i], vsc);
-        if (edge) x = only(x, on);
-        *(h8 *)(vt + (d + 16 * i) * VST + kRec * rl) = x;
+      for (int i = 0; i < W; i++) {
+        *(h8 *)(kd + krow * KST + 8 * (W * kw + i)) = values(kq[i], ksc);
+        *(h8 *)(vd + (16 * (W * vt + i) + vr) * VST + kRec * vl) = values(vq[i], vsc);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        *(u32x4 *)(ks[kb & 1] + x * KST + 8 * sg) = kp[i];
-        u32x4 w = vp[i];
-        if (edge) {
-          const int v = BR * kb + x / kRec;
-          const bool on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))) >> x % kRec & 1;
-#pragma unroll
-          for (int j = 0; j < 4; j++) w[j] = on ? w[j] : 0u;
-          if (const uint32_t bad = not_finite(w)) {
-            atomicOr(&badp[(kb - kb0) % 4][x / 32], 1u << x % 32);
-            w = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, w), ~bad));
-          }
-        }
-        *(u32x4 *)(vt + x * VST + 8 * sg) = w;
+        *(u32x4 *)(kd + x * KST + 8 * sg) = kp[i];
+        *(u32x4 *)(vd + x * VST + 8 * sg) = vp[i];
       }
     }
   };
@@ -846,43 +861,23 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     }
   };
   h8 ph[4], pl[TWO ? 4 : 1];
-  auto scores = [&](int kb) {   // -> ph, pl; o and l brought to the new maximum
-    const uint16_t *kl = ks[kb & 1];
-    const bool edge = partial(kb, PA, PB);
-    f32x16 sc[2];
+  f32x16 sa[2], sb[2];
+  auto dots = [&](int kb, f32x16 *x) {   // K q of a block
+    const uint16_t *kl = ks[kb % KR];
 #pragma unroll
     for (int mt = 0; mt < 2; mt++) {
 #pragma unroll
-      for (int i = 0; i < 16; i++) sc[mt][i] = 0.f;
+      for (int i = 0; i < 16; i++) x[mt][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < KQ; k++) {
         const h8 kf = *(const h8 *)(kl + (32 * mt + kr) * KST + 16 * k + 8 * hf);
-        sc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[k], sc[mt], 0, 0, 0);
-        if constexpr (TWO) sc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc[mt], 0, 0, 0);
+        x[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[k], x[mt], 0, 0, 0);
+        if constexpr (TWO) x[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], x[mt], 0, 0, 0);
       }
     }
-    float bm = -INFINITY;
-    if (edge) {
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
-#pragma unroll
-        for (int j = 0; j < 8; j++) sc[u >> 1][8 * (u & 1) + j] = sees(a, Pin, lo, p0 + j) ? sc[u >> 1][8 * (u & 1) + j] : -INFINITY;
-      }
-    }
-#pragma unroll
-    for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[mt][i]);
-    bm = pair_max32(bm) * f;   // f > 0
-    if (__any(bm > m + kLag)) {
-      const float mn = fmaxf(m, bm), corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= corr;
-#pragma unroll
-      for (int t = 0; t < OT; t++) o[t] *= corr;
-    }
-    const float sub = kPBias - (m == -INFINITY ? 0.f : m);
+  };
+  float sub = kPBias;
+  auto weights = [&](const f32x16 *sc) {   // -> ph, pl and their sum over the lane's positions
     float rs = 0.f;
 #pragma unroll
     for (int u = 0; u < 4; u++)
@@ -899,20 +894,20 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
           rs = __builtin_amdgcn_fdot2(h, (h2){(_Float16)1.f, (_Float16)1.f}, rs, false);   // the sum of what the product takes
         }
       }
-    rs = pair_sum32(rs);
-    l += rs;
+    return rs;
   };
   auto product = [&](int kb) {
-    const uint16_t *vl = vs[kb % 3];
+    const uint16_t *vb = vs[kb % 3];
 #pragma unroll
-    for (int t = 0; t < OT; t++)
+    for (int u = 0; u < 4; u++)
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const h8 x = vfrag(vl, t, u);
+      for (int t = 0; t < OT; t++) {
+        const h8 x = vfrag(vb, t, u);
         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[u], o[t], 0, 0, 0);
         if constexpr (TWO) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[u], o[t], 0, 0, 0);
       }
-    if (partial(kb, s.PA, s.PB)) {   // (some other wave's columns may be the ones that don't see all of it)
+  };
+  auto fix = [&](int kb) {
 #pragma unroll 1
       for (int w = 0; w < 2; w++) {
         uint32_t bad = __builtin_amdgcn_readfirstlane(badp[(kb - kb0) % 4][w]);
@@ -926,29 +921,76 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
             for (int i = 0; i < 4; i++) add_bad<HD, KIND>(hd.rec + (int64_t)r * (9 * HD), hd.v + (int64_t)p * a.crow, p, 32 * t + 8 * i + 4 * hf, sp, o[t], 4 * i);
         }
       }
-    }
+  };
+  auto wanted = [&](int kb) {
+    if (!wlive || kb >= kb1) return false;
+    const int pf = first(kb), pe = last(kb);
+    return pf <= PB && !(a.window > 0 && pe <= PA - a.window && pf >= a.sinks);
   };
   __syncthreads();   // badp
+  if (partial_any(kb0)) clean(kb0);
   expand(kb0);
   if (kb0 + 1 < kb1) fetch(kb0 + 1);
   __syncthreads();
-  // Step kb: block kb + 1 expanded, kb + 2 asked for, kb computed.  Waves w and w + 4 share a SIMD; the upper four run their value
-  // product a step late, first thing, so that of the two one feeds the matrix cores (P V, then K q) while the other one works
-  // on codes and exponentials.
-  const bool late = wave >= kManyWaves / 2;
-  bool mine = false;
-  for (int kb = kb0; kb <= kb1; kb++) {
-    if (late && mine) product(kb - 1);
-    if (kb == kb1) break;
-    if (kb + 1 < kb1) expand(kb + 1);
-    if (kb + 2 < kb1) fetch(kb + 2);
-    const int pf = first(kb), pe = last(kb);
-    mine = wlive && pf <= PB && !(a.window > 0 && pe <= PA - a.window && pf >= a.sinks);
-    if (mine) scores(kb);
-    if (!late && mine) product(kb);
-    if (tid < 2) badp[(kb - kb0 + 2) % 4][tid] = 0;
-    __syncthreads();
+  bool cur = wanted(kb0);
+  if (kAhead && cur) dots(kb0, sa);
+  if (kb0 + 1 < kb1) {
+    if (partial_any(kb0 + 1)) clean(kb0 + 1);
+    expand(kb0 + 1);
   }
+  if (kb0 + 2 < kb1) fetch(kb0 + 2);
+  __syncthreads();
+  // Step kb: the products K q of block kb + 1 (kAhead: where the registers allow it; else of block kb, before them) run beside the exponentials of block kb, then P V of block kb beside the expansion of
+  // block kb + 2; kb + 3 is asked for.
+  auto step = [&](int kb, f32x16 *sc, f32x16 *nx) {
+    const bool next = wanted(kb + 1), fresh = kb + 2 < kb1;
+    if (fresh && partial_any(kb + 2)) clean(kb + 2);
+    if (cur) {
+      if constexpr (!kAhead) dots(kb, sc);
+      if (partial(kb, PA, PB)) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
+#pragma unroll
+          for (int j = 0; j < 8; j++) sc[u >> 1][8 * (u & 1) + j] = sees(a, Pin, lo, p0 + j) ? sc[u >> 1][8 * (u & 1) + j] : -INFINITY;
+        }
+      }
+      if constexpr (kAhead) dots(kb + 1, nx);   // (past the last block: of whatever the buffer holds, and not used)
+      float rs = weights(sc);
+      // The maximum is looked for only where the weights say that it has outgrown m, or where there is none yet
+      if (__any(!(rs <= kRoom) | (m == -INFINITY))) {
+        float bm = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[mt][i]);
+        bm = pair_max32(bm) * f;   // f > 0
+        const float mn = fmaxf(m, bm), corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= corr;
+#pragma unroll
+        for (int t = 0; t < OT; t++) o[t] *= corr;
+        sub = kPBias - (m == -INFINITY ? 0.f : m);
+        rs = weights(sc);
+      }
+      l += rs;
+      product(kb);
+      expand(kb + 2);   // (past the last block: what the registers hold, to a place that is not read again)
+      if (partial_any(kb)) fix(kb);   // (also for the columns of a wave that see all of it)
+    } else {
+      if (kAhead && next) dots(kb + 1, nx);
+      expand(kb + 2);
+    }
+    if (kb + 3 < kb1) fetch(kb + 3);
+    cur = next;
+    if (tid < 2) badp[(kb - kb0 + 3) % 4][tid] = 0;
+    __syncthreads();
+  };
+  for (int kb = kb0; kb < kb1; kb += 2) {
+    step(kb, sa, sb);
+    if (kb + 1 < kb1) step(kb + 1, sb, sa);
+  }
+  l = pair_sum32(l);
   if (!live) return;
   if (s.S == 1) {
     const float inv = 1.f / l;
@@ -1015,6 +1057,7 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   a.tile = a.many ? kManyBlk : kFewTile;
   a.min_tiles = a.many ? 4 : kFewWaves;
   a.nchunk = (int)((cols + a.cols - 1) / a.cols);
+  a.paired = a.many && a.window == 0;
   // positions that a workgroup can have to read, at most
   const int64_t reach = a.window > 0 ? std::min<int64_t>(a.ctx, (int64_t)a.window + a.sinks + (a.cols + a.rep - 1) / a.rep + 3 * kRec) : a.ctx;
   const int64_t tiles = (reach + a.tile - 1) / a.tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
