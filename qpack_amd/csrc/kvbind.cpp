@@ -1,0 +1,216 @@
+// The Python side of the kv entry points (qpack_amd._kvbind, used by qpack_amd/kvcache.py): reads tensors through their Python
+// attributes, checks them and calls the C ABI.  A step's kernels take 3 to 8 us each; the same checks through ctypes took 10 us a call
+// (15 with scratch), this takes about 3.  CPython's API alone: no torch headers, no torch library.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <cstdint>
+#include <cstring>
+#include <initializer_list>
+
+#include "../../include/qpack_hip.h"
+
+namespace {
+PyObject *g_error, *g_f32, *g_f16, *g_bf16, *g_i32, *g_stream, *g_device, *g_guard, *g_empty;   // QphError, dtypes, functions
+PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_is_contiguous;
+
+struct Ref {   // owned reference
+  PyObject *p;
+  explicit Ref(PyObject *q) : p(q) {}
+  ~Ref() { Py_XDECREF(p); }
+  Ref(const Ref &) = delete;
+  Ref &operator=(const Ref &) = delete;
+  operator PyObject *() const { return p; }
+};
+
+struct Cache {
+  PyObject_HEAD
+  qph_kv c;
+  int64_t device;
+};
+
+bool fail(const char *fmt, const char *a, const char *b = "") {
+  PyErr_Format(g_error, fmt, a, b);
+  return false;
+}
+bool ints(PyObject *t, int64_t *out, int n) {   // a tuple of n integers
+  if (!t || !PyTuple_Check(t) || PyTuple_GET_SIZE(t) != n) return false;
+  for (int i = 0; i < n; i++) out[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(t, i));
+  return !PyErr_Occurred();
+}
+bool address(PyObject *x, void **p) {
+  Ref v(PyObject_CallMethodNoArgs(x, s_data_ptr));
+  if (!v.p) return false;
+  *p = PyLong_AsVoidPtr(v);
+  return !PyErr_Occurred();
+}
+bool device_of(PyObject *x, int64_t *d) {
+  Ref v(PyObject_CallMethodNoArgs(x, s_get_device));
+  if (!v.p) return false;
+  *d = PyLong_AsLongLong(v);
+  return !PyErr_Occurred();
+}
+bool on_device(const Cache *c, PyObject *x, const char *name) {
+  int64_t d;
+  if (!device_of(x, &d)) return false;
+  return d == c->device || fail("kv: %s is not on the cache's device%s", name);
+}
+// a tensor [nseq, n, heads, head_dim] with consecutive dims
+bool rows(const Cache *c, PyObject *x, const char *name, qph_rows *r, int64_t *n, int64_t *heads) {
+  Ref t(PyObject_GetAttr(x, s_dtype));
+  if (!t.p) return false;
+  if (t.p == g_f32) r->type = QPH_F32;
+  else if (t.p == g_f16) r->type = QPH_F16;
+  else if (t.p == g_bf16) r->type = QPH_BF16;
+  else return fail("kv: %s must be float32, float16 or bfloat16%s", name);
+  if (!on_device(c, x, name)) return false;
+  int64_t s[4], st[4];
+  Ref shape(PyObject_GetAttr(x, s_shape)), stride(PyObject_CallMethodNoArgs(x, s_stride));
+  if (!shape.p || !stride.p) return false;
+  if (!ints(shape, s, 4) || !ints(stride, st, 4) || s[0] != c->c.nseq || s[3] != c->c.head_dim) {
+    PyErr_Clear();
+    PyErr_Format(g_error, "kv: %s must be [%d, n, heads, %d]", name, c->c.nseq, c->c.head_dim);
+    return false;
+  }
+  if (st[3] != 1) return fail("kv: the last dimension of %s must be contiguous%s", name);
+  *n = s[1]; *heads = s[2];
+  r->seq = st[0]; r->tok = st[1]; r->head = st[2];
+  if (!address(x, &r->p)) return false;
+  if (*n == 0 && !r->p) r->p = (void *)16;   // a tensor without elements may have no memory: nothing of it is read
+  return true;
+}
+bool index(const Cache *c, PyObject *x, const char *name, const int **p) {   // int32 [nseq]; None: NULL
+  if (x == Py_None && !strcmp(name, "lens")) { *p = nullptr; return true; }
+  Ref t(PyObject_GetAttr(x, s_dtype)), shape(PyObject_GetAttr(x, s_shape)), con(PyObject_CallMethodNoArgs(x, s_is_contiguous));
+  if (!t.p || !shape.p || !con.p) return false;
+  int64_t s[1];
+  if (t.p != g_i32 || !ints(shape, s, 1) || s[0] != c->c.nseq || con.p != Py_True) {
+    PyErr_Clear();
+    PyErr_Format(g_error, "kv: %s must be a contiguous int32 tensor [%d]", name, c->c.nseq);
+    return false;
+  }
+  void *q;
+  if (!on_device(c, x, name) || !address(x, &q)) return false;
+  *p = (const int *)q;
+  return true;
+}
+bool stream_of(const Cache *c, void **st) {
+  Ref d(PyLong_FromLongLong(c->device));
+  Ref v(PyObject_CallOneArg(g_stream, d));
+  if (!v.p) return false;
+  *st = PyLong_AsVoidPtr(v);
+  return !PyErr_Occurred();
+}
+// runs f on the cache's device; a switch only where another one is current
+template <typename F>
+bool launch(const Cache *c, const F &f) {
+  void *st = nullptr;
+  Ref now(PyObject_CallNoArgs(g_device));
+  if (!now.p || !stream_of(c, &st)) return false;
+  int rc;
+  if (PyLong_AsLongLong(now) == c->device) rc = f(st);
+  else {
+    Ref d(PyLong_FromLongLong(c->device));
+    Ref guard(PyObject_CallOneArg(g_guard, d));
+    Ref in(guard.p ? PyObject_CallMethod(guard, "__enter__", nullptr) : nullptr);
+    if (!in.p) return false;
+    rc = f(st);
+    Ref out(PyObject_CallMethod(guard, "__exit__", "OOO", Py_None, Py_None, Py_None));
+    if (!out.p) return false;
+  }
+  return rc == 0 || fail("%s%s", qph_last_error());
+}
+bool integer(PyObject *x, const char *name, int *v) {
+  const long long y = PyLong_AsLongLong(x);
+  if (PyErr_Occurred()) return false;
+  if (y < INT32_MIN || y > INT32_MAX) return fail("kv: %s is out of range%s", name);
+  *v = (int)y;
+  return true;
+}
+bool nargs(Py_ssize_t n, Py_ssize_t want) {
+  if (n != want) PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
+  return n == want;
+}
+
+// write / read (k, v, pos, lens)
+template <bool WRITE>
+PyObject *io(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
+  const Cache *c = (const Cache *)self;
+  qph_rows k, v;
+  int64_t nk, nv, hk, hv;
+  const int *pos, *lens;
+  if (!nargs(na, 4) || !rows(c, arg[0], "k", &k, &nk, &hk) || !rows(c, arg[1], "v", &v, &nv, &hv) || !index(c, arg[2], "pos", &pos) || !index(c, arg[3], "lens", &lens))
+    return nullptr;
+  if (nk != nv) { fail("kv: k and v have different numbers of tokens%s%s", ""); return nullptr; }
+  if (hk != c->c.kv_heads || hv != c->c.kv_heads) { PyErr_Format(g_error, "kv: k and v must have %d heads", c->c.kv_heads); return nullptr; }
+  if (nk > INT32_MAX) { fail("kv: too many tokens%s%s", ""); return nullptr; }
+  if (!launch(c, [&](void *st) { return (WRITE ? qph_kv_write : qph_kv_read)(&c->c, &k, &v, (int)nk, pos, lens, st); })) return nullptr;
+  Py_RETURN_NONE;
+}
+// attention(q, out, pos, lens, window, sinks, scale)
+PyObject *attention(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
+  const Cache *c = (const Cache *)self;
+  qph_rows q, o;
+  int64_t n, n2, h, h2, bytes = 0;
+  const int *pos, *lens;
+  int window, sinks;
+  if (!nargs(na, 7) || !rows(c, arg[0], "q", &q, &n, &h) || !rows(c, arg[1], "out", &o, &n2, &h2) || !index(c, arg[2], "pos", &pos) || !index(c, arg[3], "lens", &lens) ||
+      !integer(arg[4], "window", &window) || !integer(arg[5], "sinks", &sinks))
+    return nullptr;
+  const double scale = PyFloat_AsDouble(arg[6]);
+  if (PyErr_Occurred()) return nullptr;
+  if (n != n2 || h != h2) { fail("kv: out must have q's shape%s%s", ""); return nullptr; }
+  if (n > INT32_MAX || h > INT32_MAX) { fail("kv: q is too large%s%s", ""); return nullptr; }
+  if (qph_kv_attention_work(&c->c, q.type, (int)h, (int)n, window, sinks, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
+  // scratch of this call alone: the allocator gives it to the stream's later work, or to the graph that is being captured
+  Ref work(bytes ? PyObject_CallFunction(g_empty, "LL", (long long)bytes, (long long)c->device) : nullptr);
+  void *w = nullptr;
+  if (bytes && (!work.p || !address(work, &w))) return nullptr;
+  if (!launch(c, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, (float)scale, w, bytes, st); })) return nullptr;
+  Py_RETURN_NONE;
+}
+
+int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_heads, head_dim, ctx, k, v, seq, row, device)
+  Cache *c = (Cache *)self;
+  long long ctx, k, v, seq, row, device;
+  if (!PyArg_ParseTuple(args, "iiiiLLLLLL", &c->c.kind, &c->c.nseq, &c->c.kv_heads, &c->c.head_dim, &ctx, &k, &v, &seq, &row, &device)) return -1;
+  c->c.ctx = ctx; c->c.k = (void *)k; c->c.v = (void *)v; c->c.seq = seq; c->c.row = row; c->device = device;
+  return 0;
+}
+PyObject *pointer(PyObject *self, PyObject *) { return PyLong_FromVoidPtr(&((Cache *)self)->c); }
+
+PyMethodDef cache_methods[] = {
+    {"write", (PyCFunction)(void (*)(void))io<true>, METH_FASTCALL, "write(k, v, pos, lens)"},
+    {"read", (PyCFunction)(void (*)(void))io<false>, METH_FASTCALL, "read(k, v, pos, lens)"},
+    {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "attention(q, out, pos, lens, window, sinks, scale)"},
+    {"pointer", pointer, METH_NOARGS, "address of the qph_kv"},
+    {nullptr, nullptr, 0, nullptr}};
+PyTypeObject cache_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+
+// setup(QphError, float32, float16, bfloat16, int32, raw stream of a device, current device, device guard, scratch(bytes, device))
+PyObject *setup(PyObject *, PyObject *args) {
+  if (!PyArg_ParseTuple(args, "OOOOOOOOO", &g_error, &g_f32, &g_f16, &g_bf16, &g_i32, &g_stream, &g_device, &g_guard, &g_empty)) return nullptr;
+  for (PyObject *p : {g_error, g_f32, g_f16, g_bf16, g_i32, g_stream, g_device, g_guard, g_empty}) Py_INCREF(p);
+  Py_RETURN_NONE;
+}
+PyMethodDef module_methods[] = {{"setup", setup, METH_VARARGS, "the names that the module uses of Python's side"}, {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvbind", nullptr, -1, module_methods};
+}  // namespace
+
+PyMODINIT_FUNC PyInit__kvbind(void) {
+  s_dtype = PyUnicode_InternFromString("dtype"); s_shape = PyUnicode_InternFromString("shape"); s_stride = PyUnicode_InternFromString("stride");
+  s_data_ptr = PyUnicode_InternFromString("data_ptr"); s_get_device = PyUnicode_InternFromString("get_device");
+  s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+  cache_type.tp_name = "qpack_amd._kvbind.Cache";
+  cache_type.tp_basicsize = sizeof(Cache);
+  cache_type.tp_flags = Py_TPFLAGS_DEFAULT;
+  cache_type.tp_new = PyType_GenericNew;
+  cache_type.tp_init = init;
+  cache_type.tp_methods = cache_methods;
+  if (PyType_Ready(&cache_type) < 0) return nullptr;
+  PyObject *m = PyModule_Create(&module);
+  if (!m) return nullptr;
+  Py_INCREF(&cache_type);
+  PyModule_AddObject(m, "Cache", (PyObject *)&cache_type);
+  return m;
+}

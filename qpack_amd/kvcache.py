@@ -4,17 +4,23 @@ Calls go to the current stream of the tensors' device and are not waited for; th
 reads pos and lens anew at every replay."""
 import ctypes as C
 
-from ._lib import QPH_BF16, QPH_F16, QPH_F32, QPH_Q4, KvC, QphError, RowsC, check, lib
+from ._lib import QPH_F16, QPH_Q4, QphError, check, lib
 
 _KINDS = {"f16": QPH_F16, "q4": QPH_Q4, QPH_F16: QPH_F16, QPH_Q4: QPH_Q4}
-_TYPES = {}
+_bind = None
 
 
-def _types():
-    if not _TYPES:
+def _binding():
+    """the compiled half of this file (csrc/kvbind.cpp), told what it uses of torch"""
+    global _bind
+    if _bind is None:
         import torch
-        _TYPES.update({torch.float32: QPH_F32, torch.float16: QPH_F16, torch.bfloat16: QPH_BF16})
-    return _TYPES
+        lib()   # the library, with its message where it has not been built
+        from . import _kvbind
+        _kvbind.setup(QphError, torch.float32, torch.float16, torch.bfloat16, torch.int32, torch._C._cuda_getCurrentRawStream, torch.cuda.current_device,
+                      torch.cuda.device, lambda n, d: torch.empty(n, dtype=torch.uint8, device=d))
+        _bind = _kvbind
+    return _bind
 
 
 class KvCache:
@@ -35,15 +41,13 @@ class KvCache:
         b = C.c_int64()
         check(lib().qph_kv_bytes(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx, C.byref(b)))
         self.nbytes = b.value
-        c = KvC(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx)
         if self.kind == QPH_Q4:
             shape = (self.nseq, self.kv_heads, (self.ctx + 7) // 8, 9 * self.head_dim)
             if data is None:
                 data = torch.zeros(shape, dtype=torch.uint8, device=device)
             if data.dtype != torch.uint8 or tuple(data.shape) != shape or not data.is_contiguous():
                 raise QphError(f"kv: a q4 cache's data must be a contiguous uint8 tensor {list(shape)}")
-            first = data
-            c.k = data.data_ptr()
+            first, at = data, (data.data_ptr(), 0, 0, 0)
         else:
             shape = (self.nseq, self.ctx, self.kv_heads, self.head_dim)
             if data is None:
@@ -54,48 +58,15 @@ class KvCache:
                     raise QphError(f"kv: an f16 cache's data must be two fp16 tensors {list(shape)} of equal strides with contiguous rows")
             if v.device != k.device:
                 raise QphError("kv: K and V on different devices")
-            first = k
-            c.k, c.v, c.seq, c.row = k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)
+            first, at = k, (k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1))
         if first.device.type != "cuda":
             raise QphError("kv: the cache must be on a GPU")
-        self.data, self.device, self._c = data, first.device, c
-        self._ref = C.byref(c)
-        self._work = {}
-
-    def _rows(self, x, name, heads=None):
-        t = _types().get(x.dtype)
-        if t is None:
-            raise QphError(f"kv: {name} must be float32, float16 or bfloat16, not {x.dtype}")
-        if x.device != self.device:
-            raise QphError(f"kv: {name} is on {x.device}, the cache on {self.device}")
-        s, st = x.shape, x.stride()
-        if len(s) != 4 or s[0] != self.nseq or s[3] != self.head_dim or (heads is not None and s[2] != heads):
-            raise QphError(f"kv: {name} must be [{self.nseq}, n, {heads or 'heads'}, {self.head_dim}], not {list(s)}")
-        if st[3] != 1:
-            raise QphError(f"kv: the last dimension of {name} must be contiguous")
-        return RowsC(x.data_ptr(), t, st[0], st[1], st[2])
-
-    def _index(self, x, name):
-        import torch
-        if x is None and name == "lens":
-            return None
-        if x.dtype != torch.int32 or x.device != self.device or tuple(x.shape) != (self.nseq,) or not x.is_contiguous():
-            raise QphError(f"kv: {name} must be a contiguous int32 tensor [{self.nseq}] on {self.device}")
-        return x.data_ptr()
-
-    def _run(self, f, *args):
-        import torch
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
-                return check(f(*args, torch.cuda.current_stream().cuda_stream))
-        check(f(*args, torch.cuda.current_stream().cuda_stream))
+        self.data, self.device = data, first.device
+        self._c = _binding().Cache(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx, *at, self.device.index)
 
     def write(self, k, v, pos, lens=None):
         """round the rows k and v [nseq, n, kv_heads, head_dim] into the cache"""
-        rk, rv = self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
-        if k.shape[1] != v.shape[1]:
-            raise QphError("kv: k and v have different numbers of tokens")
-        self._run(lib().qph_kv_write, self._ref, C.byref(rk), C.byref(rv), k.shape[1], self._index(pos, "pos"), self._index(lens, "lens"))
+        self._c.write(k, v, pos, lens)
 
     def read(self, pos, n, dtype=None, lens=None, out=None):
         """(k, v) [nseq, n, kv_heads, head_dim]: what the cache holds, in dtype (float16 when None); into out = (k, v) where given.  Rows
@@ -105,30 +76,17 @@ class KvCache:
             shape = (self.nseq, int(n), self.kv_heads, self.head_dim)
             out = tuple(torch.zeros(shape, dtype=dtype or torch.float16, device=self.device) for _ in range(2))
         k, v = out
-        rk, rv = self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
-        if k.shape[1] != n or v.shape[1] != n:
+        if k.shape[1] != n:
             raise QphError("kv: out must have n tokens")
-        self._run(lib().qph_kv_read, self._ref, C.byref(rk), C.byref(rv), int(n), self._index(pos, "pos"), self._index(lens, "lens"))
+        self._c.read(k, v, pos, lens)
         return out
 
     def attention(self, q, pos, lens=None, window=0, sinks=0, scale=0.0, out=None):
         """softmax(scale q K^T) V of the tokens q [nseq, n, heads, head_dim] at pos[b] + t, whose rows are in the cache; scale 0: 1 /
         sqrt(head_dim).  Position P sees p <= P and, with window > 0, of those p > P - window and p < sinks only.  out may be q; rows that
         take no part stay as they are in out, and are zero without it"""
-        import torch
         if out is None:
+            import torch
             out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-        rq, ro = self._rows(q, "q"), self._rows(out, "out")
-        n, heads = q.shape[1], q.shape[2]
-        if out.shape != q.shape:
-            raise QphError("kv: out must have q's shape")
-        key = (rq.type, heads, n, window, sinks)
-        size = self._work.get(key)   # sizes alone are kept: the scratch is each call's own
-        if size is None:
-            b = C.c_int64()
-            check(lib().qph_kv_attention_work(self._ref, rq.type, heads, n, window, sinks, C.byref(b)))
-            size = self._work[key] = b.value
-        work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-        self._run(lib().qph_kv_attention, self._ref, C.byref(rq), C.byref(ro), heads, n, self._index(pos, "pos"), self._index(lens, "lens"),
-                  window, sinks, scale, work.data_ptr() if size else None, size)
+        self._c.attention(q, out, pos, lens, window, sinks, scale)
         return out

@@ -13,7 +13,7 @@ import numpy as np
 import pytest
 
 import qpack_amd as qa
-from qpack_amd._lib import lib
+from qpack_amd._lib import KvC, RowsC, lib
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -371,14 +371,15 @@ def test_scratch_is_not_read_before_it_is_written_and_results_repeat():
     for n, rep in ((1, 4), (40, 4)):
         q = torch.randn(1, n, rep, 128, generator=gen).half().cuda()
         b = C.c_int64()
-        rows = c._rows(q, "q")
-        qa._lib.check(lib().qph_kv_attention_work(c._ref, rows.type, rep, n, 0, 0, C.byref(b)))
+        kv = KvC(qa.QPH_Q4, 1, 1, 128, 3000, c.data.data_ptr())
+        rows = lambda x: RowsC(x.data_ptr(), qa.QPH_F16, x.stride(0), x.stride(1), x.stride(2))   # noqa: E731
+        qa._lib.check(lib().qph_kv_attention_work(C.byref(kv), qa.QPH_F16, rep, n, 0, 0, C.byref(b)))
         assert b.value > 0
         outs, pos = [], i32([3000 - n])
         for fill in (255, 0, 127):
             work = torch.full((b.value + 64,), fill, dtype=torch.uint8, device="cuda")
             o = torch.empty_like(q)
-            qa._lib.check(lib().qph_kv_attention(c._ref, C.byref(rows), C.byref(c._rows(o, "out")), rep, n, pos.data_ptr(), None, 0, 0, 0.0,
+            qa._lib.check(lib().qph_kv_attention(C.byref(kv), C.byref(rows(q)), C.byref(rows(o)), rep, n, pos.data_ptr(), None, 0, 0, 0.0,
                                                  work.data_ptr(), b.value, torch.cuda.current_stream().cuda_stream))
             torch.cuda.synchronize()
             assert bool((work[b.value:] == fill).all())
@@ -425,3 +426,50 @@ def test_conversation(kind):
                 check_rows(out[b, :m], q[b, :m], K[b], V[b], at[b], window=window, sinks=sinks)
             assert not out[b, m:].any()
             at[b] += m
+
+
+def test_python_refusals():
+    c = qa.KvCache("q4", 2, 2, 64, 40)
+    f = qa.KvCache("f16", 2, 2, 64, 40)
+    k = torch.zeros(2, 3, 2, 64, device="cuda", dtype=F16)
+    q, pos = torch.zeros(2, 3, 4, 64, device="cuda", dtype=F16), i32([0, 1])
+    for cache in (c, f):
+        for bad, words in ((k.cpu(), "device"), (k.double(), "float32, float16 or bfloat16"), (k[:1], "must be"), (k[0], "must be"), (k[..., :32], "must be"),
+                           (torch.zeros(2, 3, 2, 128, device="cuda", dtype=F16)[..., ::2], "contiguous"), (k[:, :, :1], "heads")):
+            with pytest.raises(qa.QphError, match=words):
+                cache.write(bad, k, pos)
+            with pytest.raises(qa.QphError, match=words):
+                cache.write(k, bad, pos)
+            with pytest.raises(qa.QphError):
+                cache.read(pos, 3, out=(k, bad))
+            if words != "heads":
+                with pytest.raises(qa.QphError, match=words):
+                    cache.attention(bad, pos, out=q)
+        for bad in (pos.long(), pos[:1], pos.cpu(), i32([0, 0, 1, 1])[::2]):
+            with pytest.raises(qa.QphError, match="pos|device"):
+                cache.attention(q, bad)
+            with pytest.raises(qa.QphError, match="lens|device"):
+                cache.attention(q, pos, lens=bad)
+        with pytest.raises(qa.QphError, match="numbers of tokens"):
+            cache.write(k, k[:, :2], pos)
+        with pytest.raises(qa.QphError, match="q's shape"):
+            cache.attention(q, pos, out=q[:, :2])
+        with pytest.raises(qa.QphError, match="same type"):
+            cache.attention(q, pos, out=q.float())
+        with pytest.raises(qa.QphError, match="multiple of kv_heads"):
+            cache.attention(q[:, :, :3], pos)
+        with pytest.raises(qa.QphError, match="negative"):
+            cache.attention(q, pos, window=-1)
+        with pytest.raises(qa.QphError, match="overlap"):
+            cache.attention(q, pos, out=torch.zeros(1, 3, 4, 64, device="cuda", dtype=F16).expand(2, 3, 4, 64))
+        cache.write(k[:, :0], k[:, :0], pos)
+        assert cache.attention(q[:, :0], pos).shape == (2, 0, 4, 64)
+    for bad in (torch.zeros(2, 2, 5, 575, device="cuda", dtype=torch.uint8), torch.zeros(2, 2, 5, 576, device="cuda")):
+        with pytest.raises(qa.QphError, match="uint8"):
+            qa.KvCache("q4", 2, 2, 64, 40, data=bad)
+    with pytest.raises(qa.QphError, match="fp16"):
+        qa.KvCache("f16", 2, 2, 64, 40, data=(k, k))
+    with pytest.raises(qa.QphError, match="head_dim"):
+        qa.KvCache("q4", 2, 2, 80, 40)
+    with pytest.raises(qa.QphError, match="kind"):
+        qa.KvCache("q8", 2, 2, 64, 40)
