@@ -210,7 +210,7 @@ typedef struct {
 /* bytes of a QPH_Q4 cache, or of K and V together of a QPH_F16 one without gaps */
 int qph_kv_bytes(int kind, int nseq, int kv_heads, int head_dim, int64_t ctx, int64_t *bytes);
 /* Token t of sequence b, t < min(n, lens[b]) (lens NULL: t < n), is position pos[b] + t; sequences with pos[b] < 0 and
- * positions at or past ctx take no part: nothing of them is read or written.  n <= 2^20.
+ * positions at or past ctx take no part: nothing of them is written, and what their rows hold does not matter.  n <= 2^20.
  * qph_kv_write rounds k and v (one type) into the cache; what else the cache holds stays.  qph_kv_read returns what it holds, rounded to the
  * rows' type (fp16 and fp32: exact). */
 int qph_kv_write(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, const int *pos, const int *lens, void *stream);

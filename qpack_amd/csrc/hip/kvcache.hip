@@ -86,6 +86,12 @@ __device__ __forceinline__ void store_elems(const KvRows &r, int64_t at, const f
   }
 }
 
+// 8 fp16 elements as the matrix cores take them
+__device__ __forceinline__ h8 load_halves(const KvRows &r, int64_t at) {
+  const u32x4 v = *(const u32x4_any *)((const uint16_t *)r.p + at);
+  return __builtin_bit_cast(h8, v);
+}
+
 // bit position of element i (0 .. 7) of a word of codes
 __host__ __device__ constexpr int nib(int i) { return 16 * (i & 1) + 4 * (i >> 1); }
 
@@ -211,6 +217,68 @@ __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   }
 }
 
+// One token a sequence: a wave has one row of K or V, HD / 64 dims a lane.  Lanes of a K word meet by DPP; a V word is read (as soon as
+// the position is known, beside the row) and its one code replaced.  In k_kv4_write such a row would keep 8 lanes of 64 busy: 4.9 us
+// against 3.4 for 8 heads of 128 dims, of which 2.4 are the launch
+template <int HD, int T>
+__global__ __launch_bounds__(128) void k_kv4_write1(KvIoArgs a) {
+  constexpr int EL = HD / 64;
+  const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 63, vside = threadIdx.x >> 6;
+  const KvRows &r = vside ? a.v : a.k;
+  const int64_t at = b * r.seq + g * r.head + EL * lane;
+  float x[EL];
+#pragma unroll
+  for (int i = 0; i < EL; i++) {
+    if constexpr (T == RT_F32) x[i] = ((const float *)r.p)[at + i];
+    else { const uint16_t h = ((const uint16_t *)r.p)[at + i]; x[i] = T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h); }
+  }
+  const int p = a.pos[b];
+  if (p < 0 || p >= a.ctx || tokens_of(a.lens, b, a.n) <= 0) return;
+  uint8_t *o = (uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + p / kRec) * (9 * HD);
+  const int row = p % kRec;
+  uint32_t *vw[EL], old[EL];
+  if (vside) {
+#pragma unroll
+    for (int i = 0; i < EL; i++) {
+      const int d = EL * lane + i;
+      vw[i] = (uint32_t *)(o + 4 * HD) + d % 16 * (HD / 16) + d / 16;
+      old[i] = *vw[i];
+    }
+  }
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < EL; i++) mx = max(mx, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+  mx = max(mx, (uint32_t)dpp_i<kDppQuadXor1>((int)mx));
+  mx = max(mx, (uint32_t)dpp_i<kDppQuadXor2>((int)mx));
+  mx = max(mx, (uint32_t)dpp_i<kDppHalfMirror>((int)mx));
+  mx = max(mx, (uint32_t)dpp_i<kDppMirror>((int)mx));
+  if (EL == 1) {   // 32 dims are 32 lanes (a maximum of the bits: NaN's are the largest)
+    float u, v;
+    swap16(__builtin_bit_cast(float, mx), u, v);
+    mx = max(__builtin_bit_cast(uint32_t, u), __builtin_bit_cast(uint32_t, v));
+  }
+  const uint16_t sb = group_scale(mx);
+  const float s = half_bits_to_float(sb), inv = 1.f / s;
+  uint32_t c[EL];
+#pragma unroll
+  for (int i = 0; i < EL; i++) c[i] = s > 0.f ? code_of(x[i], s, inv) : 8;
+  if (vside) {
+    const int sh = 16 * (row & 1) + 4 * (row >> 1);
+#pragma unroll
+    for (int i = 0; i < EL; i++) *vw[i] = (old[i] & ~(15u << sh)) | c[i] << sh;
+    if (lane % (32 / EL) == 0) *(uint16_t *)(o + 8 * HD + HD / 2 + 2 * (lane / (32 / EL) * kRec + row)) = sb;
+    return;
+  }
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < EL; i++) { const int j = (EL * lane + i) & 7; w |= c[i] << (16 * (j & 1) + 4 * (j >> 1)); }
+  w |= (uint32_t)dpp_i<kDppQuadXor1>((int)w);
+  w |= (uint32_t)dpp_i<kDppQuadXor2>((int)w);
+  if (EL == 1) w |= (uint32_t)dpp_i<kDppHalfMirror>((int)w);
+  if (lane % (8 / EL) == 0) *(uint32_t *)(o + row * (HD / 2) + EL * lane / 2) = w;
+  if (lane % (32 / EL) == 0) *(uint16_t *)(o + 8 * HD + 2 * (row * (HD / 32) + lane / (32 / EL))) = sb;
+}
+
 template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
   constexpr int EL = HD / 8, GL = 32 / EL;
@@ -310,7 +378,7 @@ __device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int chunk) {
   s.NR = s.PB / kRec + 1 - s.skip;
   const int rt = a.tile / kRec;
   s.nt = (s.NR + rt - 1) / rt;
-  s.S = max(1, min(a.nsplit, (s.nt + a.min_tiles - 1) / a.min_tiles));
+  s.S = s.nt <= a.one_tiles ? 1 : min(a.nsplit, (s.nt + a.min_tiles - 1) / a.min_tiles);
   return s;
 }
 __device__ __forceinline__ int record(const Span &s, int v) { return v < s.SR ? v : v + s.skip; }
@@ -325,7 +393,7 @@ __device__ __forceinline__ uint32_t seen_bits(const KvAttnArgs &a, const Span &s
   return v < s.NR ? on : 0;
 }
 
-// Queries enter as fp16, each row scaled by the power of two that brings its largest magnitude into [1, 2): fp16 and bf16
+// fp16 queries are the matrix cores' operands as they are.  Others enter as fp16, each row scaled by the power of two that brings its largest magnitude into [1, 2): bf16
 // values keep every bit that is not 2^-25 below that (fp32 ones go in two halves, hi + lo, and keep 22 bits).  The power
 // returns with the softmax scale, in fp32.
 __device__ __forceinline__ float row_power(float mx) {   // 2^-e; 1 for rows that are zero or not finite
@@ -469,15 +537,16 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   const int col = c0 + (TWO ? lr & 7 : lr), tok = col / a.rep;
   // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j.  Asked for before
   // the sequence's position is known
+  h8 q[KS];
   float x[KS][8];
   {
     const bool there = tok < a.n;
     const int64_t at = b * a.q.seq + (int64_t)(there ? tok : 0) * a.q.tok + (int64_t)(g * a.rep + col % a.rep) * a.q.head;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
-      load_elems<T, 8>(a.q, at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg), x[k]);
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[k][j] = there ? x[k][j] : 0.f;
+      const int64_t d = at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg);
+      if constexpr (T == RT_F16) q[k] = load_halves(a.q, d);
+      else load_elems<T, 8>(a.q, d, x[k]);
     }
   }
   const Span s = span_of(a, b, chunk);
@@ -490,9 +559,8 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   uint16_t *vbuf = (uint16_t *)sm + wave * kFewTile * HD;
   Tile<HD, KIND> cur;
   if (t0 + wave < t1) { load_v<HD, KIND>(a, h, s, t0 + wave, lane, cur, vbuf); load_k<HD, KIND>(a, h, s, t0 + wave, lane, cur); }
-  h8 q[KS];
-  float f;   // softmax scale in base 2, times the row's power
-  {
+  float f = a.scale2;   // softmax scale in base 2, times the row's power.  (Columns past the last are some row's: nothing of them is stored)
+  if constexpr (T != RT_F16) {
     float mx = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; k++)
@@ -500,7 +568,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
     mx = pair_max32(pair_max16(mx));
     const float p2 = row_power(mx);
-    f = a.scale2 / p2;
+    f /= p2;
 #pragma unroll
     for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -817,28 +885,34 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   fetch(kb0);
   // ---- queries
   h8 q[KQ], ql[TWO ? KQ : 1];
-  float f;
+  float f = a.scale2;
   {
+    // (columns past the last token are some row's: nothing of them is stored)
+    const int64_t at = b * a.q.seq + (int64_t)min(tok, a.n - 1) * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
     float x[KQ][8], mx = 0.f;
-    const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)head * a.q.head;
 #pragma unroll
     for (int k = 0; k < KQ; k++) {
-      if (live) load_elems<T, 8>(a.q, at + 16 * k + 8 * hf, x[k]);
+      if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
+      else {
+        load_elems<T, 8>(a.q, at + 16 * k, x[k]);
 #pragma unroll
-      for (int j = 0; j < 8; j++) { if (!live) x[k][j] = 0.f; mx = fmaxf(mx, fabsf(x[k][j])); }
-    }
-    mx = pair_max32(mx);
-    const float p2 = row_power(mx);
-    f = a.scale2 / p2;
-#pragma unroll
-    for (int k = 0; k < KQ; k++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float y = x[k][j] * p2;
-        const _Float16 h = (_Float16)y;
-        q[k][j] = h;
-        if constexpr (TWO) ql[k][j] = (_Float16)(y - (float)h);
+        for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
       }
+    }
+    if constexpr (T != RT_F16) {
+      mx = pair_max32(mx);
+      const float p2 = row_power(mx);
+      f /= p2;
+#pragma unroll
+      for (int k = 0; k < KQ; k++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float y = x[k][j] * p2;
+          const _Float16 h = (_Float16)y;
+          q[k][j] = h;
+          if constexpr (TWO) ql[k][j] = (_Float16)(y - (float)h);
+        }
+    }
   }
   f32x16 o[OT];
 #pragma unroll
@@ -1024,7 +1098,8 @@ void launch_io16(const KvIoArgs &a, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_kv_write(int kind, const KvIoArgs &a, hipStream_t st) {
-  if (kind == MK_Q4) QPH_KV(k_kv4_write, a.hd, a.k.type, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
+  if (kind == MK_Q4 && a.n == 1) QPH_KV(k_kv4_write1, a.hd, a.k.type, dim3(1, a.nkv, a.nseq), 128, a);
+  else if (kind == MK_Q4) QPH_KV(k_kv4_write, a.hd, a.k.type, dim3((unsigned)(((int64_t)a.n + 7) / 8 + 1), a.nkv, a.nseq), 128, a);
   else launch_io16<true>(a, st);
   return hipGetLastError();
 }
@@ -1042,13 +1117,14 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   a.cols = a.many ? kManyCols : two ? 8 : 16;
   a.tile = a.many ? kManyBlk : kFewTile;
   a.min_tiles = a.many ? 4 : kFewWaves;
+  a.one_tiles = a.many ? 4 : 4 * kFewWaves;
   a.nchunk = (int)((cols + a.cols - 1) / a.cols);
   a.paired = a.many && a.window == 0;
   // positions that a workgroup can have to read, at most
   const int64_t reach = a.window > 0 ? std::min<int64_t>(a.ctx, (int64_t)a.window + a.sinks + (a.cols + a.rep - 1) / a.rep + 3 * kRec) : a.ctx;
   const int64_t tiles = (reach + a.tile - 1) / a.tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
   const int64_t want = (a.many ? 1 : 2) * (int64_t)cus / std::max<int64_t>(groups, 1);
-  a.nsplit = (int)std::max<int64_t>(1, std::min({want, (tiles + a.min_tiles - 1) / a.min_tiles, (int64_t)64}));
+  a.nsplit = tiles <= a.one_tiles ? 1 : (int)std::max<int64_t>(1, std::min({want, (tiles + a.min_tiles - 1) / a.min_tiles, (int64_t)64}));
   if (a.n > 65535) a.nsplit = 1;
   return a.nsplit > 1 ? (size_t)a.nseq * a.n * a.heads * a.nsplit * (a.hd + 2) * 4 : 0;
 }

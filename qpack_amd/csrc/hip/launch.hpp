@@ -320,7 +320,7 @@ struct KvAttnArgs {
   float scale2;                 // softmax scale times log2(e), > 0
   float *part;                  // nsplit > 1: partial sums, then (max, sum) pairs, kv_attn_plan's bytes
   // set by kv_attn_plan
-  int many, paired, cols, nchunk, tile, min_tiles, nsplit;
+  int many, paired, cols, nchunk, tile, min_tiles, one_tiles, nsplit;
 };
 // how the call is laid out; the bytes of part
 size_t kv_attn_plan(KvAttnArgs &a);

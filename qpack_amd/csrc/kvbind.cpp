@@ -11,8 +11,8 @@
 #include "../../include/qpack_hip.h"
 
 namespace {
-PyObject *g_error, *g_f32, *g_f16, *g_bf16, *g_i32, *g_stream, *g_device, *g_guard, *g_empty;   // QphError, dtypes, functions
-PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_is_contiguous;
+PyObject *g_error, *g_f32, *g_f16, *g_bf16, *g_i32, *g_stream, *g_device, *g_guard;   // QphError, dtypes, functions
+PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_is_contiguous, *s_new_empty;
 
 struct Ref {   // owned reference
   PyObject *p;
@@ -26,7 +26,8 @@ struct Ref {   // owned reference
 struct Cache {
   PyObject_HEAD
   qph_kv c;
-  int64_t device;
+  int64_t device, item;
+  PyObject *data;   // a tensor of the cache's memory, item bytes an element: scratch is a new one like it
 };
 
 bool fail(const char *fmt, const char *a, const char *b = "") {
@@ -102,13 +103,16 @@ bool stream_of(const Cache *c, void **st) {
   return !PyErr_Occurred();
 }
 // runs f on the cache's device; a switch only where another one is current
-template <typename F>
-bool launch(const Cache *c, const F &f) {
-  void *st = nullptr;
+bool current(const Cache *c, bool *yes) {
   Ref now(PyObject_CallNoArgs(g_device));
-  if (!now.p || !stream_of(c, &st)) return false;
+  if (!now.p) return false;
+  *yes = PyLong_AsLongLong(now) == c->device;
+  return !PyErr_Occurred();
+}
+template <typename F>
+bool launch(const Cache *c, bool here, void *st, const F &f) {
   int rc;
-  if (PyLong_AsLongLong(now) == c->device) rc = f(st);
+  if (here) rc = f(st);
   else {
     Ref d(PyLong_FromLongLong(c->device));
     Ref guard(PyObject_CallOneArg(g_guard, d));
@@ -144,7 +148,10 @@ PyObject *io(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   if (nk != nv) { fail("kv: k and v have different numbers of tokens%s%s", ""); return nullptr; }
   if (hk != c->c.kv_heads || hv != c->c.kv_heads) { PyErr_Format(g_error, "kv: k and v must have %d heads", c->c.kv_heads); return nullptr; }
   if (nk > INT32_MAX) { fail("kv: too many tokens%s%s", ""); return nullptr; }
-  if (!launch(c, [&](void *st) { return (WRITE ? qph_kv_write : qph_kv_read)(&c->c, &k, &v, (int)nk, pos, lens, st); })) return nullptr;
+  bool here;
+  void *st;
+  if (!current(c, &here) || !stream_of(c, &st)) return nullptr;
+  if (!launch(c, here, st, [&](void *st) { return (WRITE ? qph_kv_write : qph_kv_read)(&c->c, &k, &v, (int)nk, pos, lens, st); })) return nullptr;
   Py_RETURN_NONE;
 }
 // attention(q, out, pos, lens, window, sinks, scale)
@@ -162,35 +169,43 @@ PyObject *attention(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   if (n != n2 || h != h2) { fail("kv: out must have q's shape%s%s", ""); return nullptr; }
   if (n > INT32_MAX || h > INT32_MAX) { fail("kv: q is too large%s%s", ""); return nullptr; }
   if (qph_kv_attention_work(&c->c, q.type, (int)h, (int)n, window, sinks, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
+  bool here;
+  void *st, *w = nullptr;
+  if (!current(c, &here) || !stream_of(c, &st)) return nullptr;
   // scratch of this call alone: the allocator gives it to the stream's later work, or to the graph that is being captured
-  Ref work(bytes ? PyObject_CallFunction(g_empty, "LL", (long long)bytes, (long long)c->device) : nullptr);
-  void *w = nullptr;
+  Ref size(bytes ? PyLong_FromLongLong((bytes + c->item - 1) / c->item) : nullptr), work(bytes ? PyObject_CallMethodOneArg(c->data, s_new_empty, size) : nullptr);
   if (bytes && (!work.p || !address(work, &w))) return nullptr;
-  if (!launch(c, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, (float)scale, w, bytes, st); })) return nullptr;
+  if (!launch(c, here, st, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, (float)scale, w, bytes, st); })) return nullptr;
   Py_RETURN_NONE;
 }
 
-int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_heads, head_dim, ctx, k, v, seq, row, device)
+int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_heads, head_dim, ctx, k, v, seq, row, device, data)
   Cache *c = (Cache *)self;
   long long ctx, k, v, seq, row, device;
-  if (!PyArg_ParseTuple(args, "iiiiLLLLLL", &c->c.kind, &c->c.nseq, &c->c.kv_heads, &c->c.head_dim, &ctx, &k, &v, &seq, &row, &device)) return -1;
+  PyObject *data;
+  if (!PyArg_ParseTuple(args, "iiiiLLLLLLO", &c->c.kind, &c->c.nseq, &c->c.kv_heads, &c->c.head_dim, &ctx, &k, &v, &seq, &row, &device, &data)) return -1;
+  Py_INCREF(data);
+  Py_XDECREF(c->data);
+  c->data = data; c->item = c->c.kind == QPH_Q4 ? 1 : 2;
   c->c.ctx = ctx; c->c.k = (void *)k; c->c.v = (void *)v; c->c.seq = seq; c->c.row = row; c->device = device;
   return 0;
 }
-PyObject *pointer(PyObject *self, PyObject *) { return PyLong_FromVoidPtr(&((Cache *)self)->c); }
+void dealloc(PyObject *self) {
+  Py_XDECREF(((Cache *)self)->data);
+  Py_TYPE(self)->tp_free(self);
+}
 
 PyMethodDef cache_methods[] = {
     {"write", (PyCFunction)(void (*)(void))io<true>, METH_FASTCALL, "write(k, v, pos, lens)"},
     {"read", (PyCFunction)(void (*)(void))io<false>, METH_FASTCALL, "read(k, v, pos, lens)"},
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "attention(q, out, pos, lens, window, sinks, scale)"},
-    {"pointer", pointer, METH_NOARGS, "address of the qph_kv"},
     {nullptr, nullptr, 0, nullptr}};
 PyTypeObject cache_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
-// setup(QphError, float32, float16, bfloat16, int32, raw stream of a device, current device, device guard, scratch(bytes, device))
+// setup(QphError, float32, float16, bfloat16, int32, raw stream of a device, current device, device guard)
 PyObject *setup(PyObject *, PyObject *args) {
-  if (!PyArg_ParseTuple(args, "OOOOOOOOO", &g_error, &g_f32, &g_f16, &g_bf16, &g_i32, &g_stream, &g_device, &g_guard, &g_empty)) return nullptr;
-  for (PyObject *p : {g_error, g_f32, g_f16, g_bf16, g_i32, g_stream, g_device, g_guard, g_empty}) Py_INCREF(p);
+  if (!PyArg_ParseTuple(args, "OOOOOOOO", &g_error, &g_f32, &g_f16, &g_bf16, &g_i32, &g_stream, &g_device, &g_guard)) return nullptr;
+  for (PyObject *p : {g_error, g_f32, g_f16, g_bf16, g_i32, g_stream, g_device, g_guard}) Py_INCREF(p);
   Py_RETURN_NONE;
 }
 PyMethodDef module_methods[] = {{"setup", setup, METH_VARARGS, "the names that the module uses of Python's side"}, {nullptr, nullptr, 0, nullptr}};
@@ -200,12 +215,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvbind", nullptr, -1, module_meth
 PyMODINIT_FUNC PyInit__kvbind(void) {
   s_dtype = PyUnicode_InternFromString("dtype"); s_shape = PyUnicode_InternFromString("shape"); s_stride = PyUnicode_InternFromString("stride");
   s_data_ptr = PyUnicode_InternFromString("data_ptr"); s_get_device = PyUnicode_InternFromString("get_device");
-  s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+  s_is_contiguous = PyUnicode_InternFromString("is_contiguous"); s_new_empty = PyUnicode_InternFromString("new_empty");
   cache_type.tp_name = "qpack_amd._kvbind.Cache";
   cache_type.tp_basicsize = sizeof(Cache);
   cache_type.tp_flags = Py_TPFLAGS_DEFAULT;
   cache_type.tp_new = PyType_GenericNew;
   cache_type.tp_init = init;
+  cache_type.tp_dealloc = dealloc;
   cache_type.tp_methods = cache_methods;
   if (PyType_Ready(&cache_type) < 0) return nullptr;
   PyObject *m = PyModule_Create(&module);

@@ -18,7 +18,7 @@ def _binding():
         lib()   # the library, with its message where it has not been built
         from . import _kvbind
         _kvbind.setup(QphError, torch.float32, torch.float16, torch.bfloat16, torch.int32, torch._C._cuda_getCurrentRawStream, torch.cuda.current_device,
-                      torch.cuda.device, lambda n, d: torch.empty(n, dtype=torch.uint8, device=d))
+                      torch.cuda.device)
         _bind = _kvbind
     return _bind
 
@@ -62,7 +62,7 @@ class KvCache:
         if first.device.type != "cuda":
             raise QphError("kv: the cache must be on a GPU")
         self.data, self.device = data, first.device
-        self._c = _binding().Cache(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx, *at, self.device.index)
+        self._c = _binding().Cache(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx, *at, self.device.index, first)
 
     def write(self, k, v, pos, lens=None):
         """round the rows k and v [nseq, n, kv_heads, head_dim] into the cache"""
