@@ -123,6 +123,16 @@ int qph_restore(qph_model *m, const uint8_t *buf, int64_t n);
  * q1) and a q8 or q4 output head.  Takes effect for the next call; the cache contents are kept. */
 int qph_set_order(qph_model *m, int mode);
 
+/* ---- long conversations (no reference counterpart)
+ * qph_set_cache: what the model's key / value cache holds, QPH_F16 (as created) or QPH_Q4: 4-bit records (described at qph_kv below), 9 / 32
+ * of the bytes, rounded as they are written, whatever the length of a prompt's chunks.  At position 0 only.
+ * qph_set_window: with window > 0 a token attends to the last `window` positions, its own among them, and to the first `sinks`; 0: to all of
+ * them.  Takes effect for the next call; every position stays in the cache, so the window can be widened again.
+ * Either needs arithmetic order 0.  prefill_all then takes decode steps; snapshots keep the reference's fp16 layout, which a 4-bit
+ * cache's values fit exactly (restoring one's own snapshot restores the cache; other rows are rounded). */
+int qph_set_cache(qph_model *m, int kind);
+int qph_set_window(qph_model *m, int window, int sinks);
+
 /* ---- measurement (no reference counterpart: qpack-bench times with the host clock, tools/qpack-bench.cpp:40-47) */
 /* Runs n greedy decode steps from token/position as greedy_run does and reports the HIP-event time of the whole run
  * on the model's stream (*ms). */

@@ -79,6 +79,8 @@ SIGNATURES = {
     "qph_snapshot": (_I, [_P, C.c_void_p, C.c_int64]),
     "qph_restore": (_I, [_P, C.c_void_p, C.c_int64]),
     "qph_set_order": (_I, [_P, _I]),
+    "qph_set_cache": (_I, [_P, _I]),
+    "qph_set_window": (_I, [_P, _I, _I]),
     "qph_time_greedy": (_I, [_P, _I, _I, _FP]),
     "qph_time_kernel": (_I, [_P, _I, _I, _FP, C.POINTER(C.c_double)]),
     "qph_verify_batches": (_I, [_P, C.POINTER(C.c_int64)]),

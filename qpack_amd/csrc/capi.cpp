@@ -210,6 +210,14 @@ int qph_snapshot_size(const qph_model *m, int64_t *bytes) { QPH_API_TRY({ need(m
 int qph_snapshot(qph_model *m, uint8_t *buf, int64_t cap) { QPH_API_TRY({ need(m, "model"); need(buf, "buf"); m->m->snapshot(buf, cap); }); }
 int qph_restore(qph_model *m, const uint8_t *buf, int64_t n) { QPH_API_TRY({ need(m, "model"); need(buf, "buf"); m->m->restore(buf, n); }); }
 
+int qph_set_cache(qph_model *m, int kind) {
+  QPH_API_TRY({
+    need(m, "model");
+    if (kind != QPH_F16 && kind != QPH_Q4) throw std::invalid_argument("cache: kind must be QPH_F16 or QPH_Q4");
+    m->m->set_cache(kind == QPH_Q4 ? qph::MK_Q4 : qph::MK_F32);
+  });
+}
+int qph_set_window(qph_model *m, int window, int sinks) { QPH_API_TRY({ need(m, "model"); m->m->set_window(window, sinks); }); }
 int qph_set_order(qph_model *m, int mode) { QPH_API_TRY({ need(m, "model"); m->m->set_order(mode); }); }
 
 int qph_time_greedy(qph_model *m, int token, int n, float *ms) {

@@ -269,6 +269,7 @@ struct PfRopeArgs {
   uint16_t *kc, *vc;
   int p0, nh, nkv, hd;
   int skip_q;   // q is rotated by the attention kernel instead
+  float *kout;     // instead of kc / vc: k rotated, as fp32, into rows like k's (which it may be); v is left alone
   uint16_t *q16;   // optional (with q rotated here): q as fp16 hi [nh * hd] then lo halves per token, as MvArgs::q16
 };
 hipError_t launch_pf_rope(const PfRopeArgs &a, int B, hipStream_t st);

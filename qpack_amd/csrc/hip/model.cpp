@@ -21,6 +21,12 @@ void *HipLlama::dalloc(size_t bytes) {
   return p;
 }
 
+void HipLlama::dfree(void *p) {
+  if (!p) return;
+  allocs_.erase(std::remove(allocs_.begin(), allocs_.end(), p), allocs_.end());
+  (void)hipFree(p);
+}
+
 DMat HipLlama::upload(const qph_tensor &t) {
   DMat m{}; m.rows = (int)t.rows; m.cols = (int)t.cols;
   size_t qb = 0, sb = 0;
@@ -255,12 +261,7 @@ HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int 
 
 HipLlama::~HipLlama() {
   if (st_) (void)hipStreamSynchronize(st_);
-  for (hipGraphExec_t g : {g_state_, g_logits_, g_greedy_, g_ex_state_, g_ex_logits_, g_ex_greedy_, g_lm_state_,
-                           g_lm_logits_, g_lm_greedy_})
-    if (g) (void)hipGraphExecDestroy(g);
-  for (auto &set : g_fs_)
-    for (hipGraphExec_t g : set)
-      if (g) (void)hipGraphExecDestroy(g);
+  drop_graphs();
   for (void *p : allocs_) (void)hipFree(p);
   if (hctl_) (void)hipHostFree(hctl_);
   if (hout_) (void)hipHostFree(hout_);
@@ -272,6 +273,110 @@ HipLlama::~HipLlama() {
   if (htopk_) (void)hipHostFree(htopk_);
   if (hstatus_) (void)hipHostFree(hstatus_);
   if (st_) (void)hipStreamDestroy(st_);
+}
+
+void HipLlama::drop_graphs() {
+  for (hipGraphExec_t *g : {&g_state_, &g_logits_, &g_greedy_, &g_ex_state_, &g_ex_logits_, &g_ex_greedy_, &g_lm_state_,
+                            &g_lm_logits_, &g_lm_greedy_}) {
+    if (*g) (void)hipGraphExecDestroy(*g);
+    *g = nullptr;
+  }
+  for (auto &set : g_fs_)
+    for (hipGraphExec_t &g : set) {
+      if (g) (void)hipGraphExecDestroy(g);
+      g = nullptr;
+    }
+  gst_graphs_.clear();
+  gst_last_ = nullptr;
+}
+
+// ------------------------------------------------------------------ 4-bit cache, sliding window
+KvIoArgs HipLlama::kv_io(int l, float *k, float *v, int n) const {   // k / v: rows [n][kvd_] at ctl_->pos ..
+  KvIoArgs a{};
+  a.cache = kv4_ + (size_t)l * kv4_layer_; a.ctx = ctx_; a.nrec = kv4_records(ctx_);
+  a.nseq = 1; a.nkv = cfg_.kv_heads; a.hd = cfg_.head_dim; a.n = n;
+  a.k = KvRows{k, RT_F32, 0, kvd_, cfg_.head_dim}; a.v = KvRows{v, RT_F32, 0, kvd_, cfg_.head_dim};
+  a.pos = &ctl_->pos;
+  return a;
+}
+KvAttnArgs HipLlama::kv_attn(int l, const float *q, float *out, int n) const {
+  KvAttnArgs a{};
+  if (kv_kind_ == MK_Q4) a.cache = kv4_ + (size_t)l * kv4_layer_;
+  else { a.cache = kc_ + (size_t)l * ctx_ * kvd_; a.cache_v = vc_ + (size_t)l * ctx_ * kvd_; }
+  a.crow = kvd_; a.ctx = ctx_; a.nrec = kv4_records(ctx_);
+  a.nseq = 1; a.nkv = cfg_.kv_heads; a.hd = cfg_.head_dim; a.heads = cfg_.heads; a.rep = cfg_.heads / cfg_.kv_heads; a.n = n;
+  a.q = KvRows{(void *)q, RT_F32, 0, qd_, cfg_.head_dim}; a.out = KvRows{out, RT_F32, 0, qd_, cfg_.head_dim};
+  a.pos = &ctl_->pos; a.window = window_; a.sinks = sinks_;
+  a.scale2 = 1.4426950408889634f / std::sqrt((float)cfg_.head_dim);
+  a.part = kv_part_;
+  return a;
+}
+void HipLlama::kv_append(int l, float *k, float *v, int n) { QPH_CK(launch_kv_write(kv_kind_, kv_io(l, k, v, n), st_)); }
+void HipLlama::kv_attend(int l, const float *q, float *out, int n) {
+  KvAttnArgs a = kv_attn(l, q, out, n);
+  if (kv_attn_plan(a) > kv_part_bytes_) throw std::runtime_error("hip: attention scratch too small");
+  QPH_CK(launch_kv_attn(kv_kind_, a, st_));
+}
+// scratch for every number of tokens that a call can have
+void HipLlama::kv_buffers() {
+  size_t need = 0;
+  for (int n = 1; n <= pf_cap_; n++) { KvAttnArgs a = kv_attn(0, nullptr, nullptr, n); need = std::max(need, kv_attn_plan(a)); }
+  if (need > kv_part_bytes_) {
+    float *p = (float *)dalloc(need);
+    dfree(kv_part_);
+    kv_part_ = p; kv_part_bytes_ = need;
+  }
+}
+void HipLlama::set_cache(int kind) {
+  if (kind == kv_kind_) return;
+  if (pos_ != 0) throw std::runtime_error("cache: the kind can change at position 0 only");
+  if (order_) throw std::runtime_error("cache: the reference order has an fp16 cache");
+  QPH_CK(hipStreamSynchronize(st_));
+  check_status();
+  // the new buffers first: where they do not fit, the model goes on as it was
+  if (kind == MK_Q4) {
+    const size_t layer = (size_t)kv4_bytes(1, cfg_.kv_heads, cfg_.head_dim, ctx_), row = 2ull * ctx_ * kvd_;
+    uint8_t *rec = nullptr;
+    uint16_t *stage = nullptr;
+    int *zero = kv_zero_;
+    try {
+      rec = (uint8_t *)dalloc(layer * cfg_.layers);
+      stage = (uint16_t *)dalloc(2 * row);
+      if (!zero) { zero = (int *)dalloc(sizeof(int)); kv_zero_ = zero; QPH_CK(hipMemset(zero, 0, sizeof(int))); }
+      QPH_CK(hipMemset(rec, 0, layer * cfg_.layers));
+      kv_buffers();
+    } catch (...) { dfree(rec); dfree(stage); throw; }
+    drop_graphs();
+    dfree(kc_); dfree(vc_);
+    kc_ = vc_ = nullptr;
+    kv4_ = rec; kv4_layer_ = layer; kv_stage_ = stage;
+  } else {
+    const size_t bytes = 2ull * cfg_.layers * ctx_ * kvd_;
+    uint16_t *k = nullptr, *v = nullptr;
+    try {
+      k = (uint16_t *)dalloc(bytes); v = (uint16_t *)dalloc(bytes);
+      QPH_CK(hipMemset(k, 0, bytes)); QPH_CK(hipMemset(v, 0, bytes));
+    } catch (...) { dfree(k); dfree(v); throw; }
+    drop_graphs();
+    dfree(kv4_); dfree(kv_stage_);
+    kv4_ = nullptr; kv_stage_ = nullptr;
+    kc_ = k; vc_ = v;
+  }
+  kv_kind_ = kind;
+  build_graphs();
+}
+void HipLlama::set_window(int window, int sinks) {
+  if (window < 0 || sinks < 0) throw std::runtime_error("window: window and sinks must not be negative");
+  if (window > 0 && order_) throw std::runtime_error("window: the reference order attends to every position");
+  if (window == 0) sinks = 0;
+  if (window == window_ && sinks == sinks_) return;
+  QPH_CK(hipStreamSynchronize(st_));
+  check_status();
+  const int w = window_, s = sinks_;
+  window_ = window; sinks_ = sinks;
+  try { if (kv_custom()) kv_buffers(); } catch (...) { window_ = w; sinks_ = s; throw; }
+  drop_graphs();
+  build_graphs();
 }
 
 // the decode q / k / v launch's epilogue: RoPE on q and k at ctl->pos, fp16 k / v rows into this layer's caches
@@ -286,7 +391,8 @@ void HipLlama::enqueue_layer(int l) {
   const Layer &ly = layers_[l];
   const int cap = 1 << 20;
   const float eps = cfg_.rms_eps;
-  uint16_t *kc = kc_ + (size_t)l * ctx_ * kvd_, *vc = vc_ + (size_t)l * ctx_ * kvd_;
+  const size_t at_l = (size_t)l * ctx_ * kvd_;
+  uint16_t *kc = kc_ ? kc_ + at_l : nullptr, *vc = vc_ ? vc_ + at_l : nullptr;   // null: a 4-bit cache
   {  // RMSNorm + q/k/v (+ bias), RoPE on q / k, fp16 k / v rows into the caches
     MvArgs a{}; a.m[0] = ly.wq; a.m[1] = ly.wk; a.m[2] = ly.wv; a.nseg = 3; a.x = x_; a.norm_w = ly.an; a.eps = eps;
     a.out[0] = q_; a.out[1] = k_; a.out[2] = v_; a.bias[0] = ly.bq; a.bias[1] = ly.bk; a.bias[2] = ly.bv;
@@ -299,7 +405,12 @@ void HipLlama::enqueue_layer(int l) {
   at.nh = cfg_.heads; at.nkv = cfg_.kv_heads; at.hd = cfg_.head_dim; at.max_chunks = max_chunks_; at.counters = counters_;
   at.single_max = attn_single_; at.split_pos = attn_split_pos_; at.status = dstatus_; at.spin_limit = attn_spin_;
   at.force_late = attn_force_late_; at.merge_sep = lm_ ? lm_splits_ : 0; at.early = fuse_ ? early_ : 0;
-  if (fuse_ && awo_rows_) {   // every group's attention and whole wo rows + residual in one launch
+  if (kv_custom()) {   // the rows into a 4-bit cache, attention over it or within the window, wo
+    if (kv_kind_ == MK_Q4) kv_append(l, k_, v_, 1);
+    kv_attend(l, q_, att_, 1);
+    MvArgs a{}; a.m[0] = ly.wo; a.nseg = 1; a.x = att_; a.out[0] = x_;
+    mv_plan(a, EPI_RESID); QPH_CK(launch_matvec(PRO_QUANT, EPI_RESID, a, cap, st_));
+  } else if (fuse_ && awo_rows_) {   // every group's attention and whole wo rows + residual in one launch
     AwoArgs w{}; w.wo = ly.wo; w.x = x_;
     QPH_CK(launch_attn_wo_rows(at, w, st_));
   } else if (fuse_ && awo_sum_) {
@@ -425,7 +536,7 @@ void HipLlama::build_graphs() {
   // the first replay) while direct launches of the same kernels profile normally.
   const char *prof = getenv("ROCP_TOOL_LIBRARIES");
   if ((ng && atoi(ng) > 0) || (prof && *prof)) { use_graphs_ = false; return; }
-  if (getenv("QPH_GRAPH_STAMPS")) {   // measurement hook: one step's launches, each its own region
+  if (getenv("QPH_GRAPH_STAMPS") && !gst_) {   // measurement hook: one step's launches, each its own region
     gst_cap_ = (size_t)(4 * cfg_.layers + 2) * 4 * kGstWaves;
     gst_ = (uint64_t *)dalloc(gst_cap_ * 8);
     QPH_CK(hipMemset(gst_, 0, gst_cap_ * 8));
@@ -433,6 +544,7 @@ void HipLlama::build_graphs() {
   g_state_ = capture(0);
   g_logits_ = capture(1);
   g_greedy_ = capture(2);
+  if (kv_custom()) return;
   if (awo_max_ > 0)
     for (int e = 1; e <= kEarlyMax; e++) {
       if (32 * (e - 1) >= awo_max_) break;   // no fused context needs this many early blocks
@@ -446,8 +558,8 @@ void HipLlama::build_graphs() {
 // pos: the position this step writes (its context is pos + 1 positions); contexts up to awo_max_ take the fused
 // attention + wo kernel
 void HipLlama::run_step(int parts, int pos) {
-  const bool fused = !order_ && pos + 1 <= awo_max_;
-  const bool lm = !order_ && !fused && lm_min_ > 0 && pos + 1 >= lm_min_;
+  const bool fused = !order_ && !kv_custom() && pos + 1 <= awo_max_;
+  const bool lm = !order_ && !kv_custom() && !fused && lm_min_ > 0 && pos + 1 >= lm_min_;
   if (use_graphs_) {
     hipGraphExec_t g = order_ ? (parts == 0 ? g_ex_state_ : parts == 1 ? g_ex_logits_ : g_ex_greedy_)
                        : fused ? g_fs_[early_for(pos)][parts]
@@ -608,31 +720,39 @@ void HipLlama::prefill_batched(const int *toks, int n) {
   for (int s0 = 0; s0 < n; s0 += B) {
     B = std::min(pf_cap_, n - s0);
     const int p0 = pos_;
+    if (kv_custom()) write_ctl(toks[s0], p0);   // the kernels read the position there
     QPH_CK(hipMemcpyAsync(pf_tok_, toks + s0, 4ull * B, hipMemcpyHostToDevice, st_));
     QPH_CK(launch_pf_embed(embed_, pf_tok_, B, pf_x_, d, st_));
     for (int l = 0; l < cfg_.layers; l++) {
       const Layer &ly = layers_[l];
-      uint16_t *kc = kc_ + (size_t)l * ctx_ * kvd_, *vc = vc_ + (size_t)l * ctx_ * kvd_;
+      const size_t at_l = (size_t)l * ctx_ * kvd_;
+      uint16_t *kc = kc_ ? kc_ + at_l : nullptr, *vc = vc_ ? vc_ + at_l : nullptr;   // null: a 4-bit cache
       GemmArgs g[3];
       int ng = qkv(ly, B, g);
       products(PRO_NORM, pf_x_, d, ly.an, d, B, g, ng);
       // q's RoPE happens in the attention kernel; at head dim 128 (one head = one quantisation block) that kernel also
       // quantises its output for a q8 wo
       PfRopeArgs r{}; r.q = pf_q_; r.ldq = qd_; r.k = pf_k_; r.v = pf_v_; r.ldk = kvd_; r.cos_t = cos_; r.sin_t = sin_;
-      r.kc = kc; r.vc = vc; r.p0 = p0; r.nh = cfg_.heads; r.nkv = cfg_.kv_heads; r.hd = cfg_.head_dim; r.skip_q = !(unfused & 1);
+      r.kc = kc; r.vc = vc; r.p0 = p0; r.nh = cfg_.heads; r.nkv = cfg_.kv_heads; r.hd = cfg_.head_dim; r.skip_q = !(unfused & 1) && !kv_custom();
+      if (kv_kind_ == MK_Q4) r.kout = pf_k_;
       QPH_CK(launch_pf_rope(r, B, st_));
       PfAttnArgs t{}; t.q = pf_q_; t.ldq = qd_; t.kc = kc; t.vc = vc; t.att = pf_att_; t.lda = qd_;
       t.part = pf_g_; t.part_floats = (size_t)pf_cap_ * ff;   // free until gate / up
       t.ntok = B; t.p0 = p0; t.nh = cfg_.heads; t.nkv = cfg_.kv_heads; t.hd = cfg_.head_dim;
       if (!(unfused & 1)) { t.cos_t = cos_; t.sin_t = sin_; }
-      const bool att_q = !(unfused & 2) && cfg_.head_dim == 128 && ly.wo.kind == MK_Q8;
+      const bool att_q = !(unfused & 2) && !kv_custom() && cfg_.head_dim == 128 && ly.wo.kind == MK_Q8;
       g[0] = product(ly.wo, pf_x_, d, nullptr, true, B);
       Planes pl = plan(g, 1);
       if (att_q) {
         t.tiled = pl.tiles;
         t.oh = pl.tiles ? pf_th_ : pf_xh_; t.ol = pl.tiles ? pf_tl_ : pf_xl_; t.ob = pf_xb_; t.obt = pf_xbt_; t.ldo = pf_ldq_; t.ldb = nb_ld; t.ldbt = pf_ldbt_;
       }
-      QPH_CK(launch_pf_attn(t, st_));
+      if (kv_custom()) {
+        if (kv_kind_ == MK_Q4) kv_append(l, pf_k_, pf_v_, B);
+        kv_attend(l, pf_q_, pf_att_, B);
+      } else {
+        QPH_CK(launch_pf_attn(t, st_));
+      }
       if (!att_q) quant(PRO_QUANT, pf_att_, qd_, nullptr, qd_, B, pl);
       QPH_CK(launch_gemm(g[0], st_));
       // gate and up in one launch, only h = silu(gate) * up stored; fused: quantised by the product's store, straight into
@@ -700,7 +820,7 @@ int HipLlama::greedy_run(int tok, int n, int *out) {
 // 1578 on the 0.5B one), a third one costs 30 us more instead of 590 and 780.
 void HipLlama::prefill_all(const int *toks, int n, float *logits) {
   if (pos_ + n > ctx_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
-  const bool batched = vf_ok_ && !order_ && !getenv("QPH_VERIFY_STEPS");   // test hook: decode steps
+  const bool batched = vf_ok_ && !order_ && !kv_custom() && !getenv("QPH_VERIFY_STEPS");   // test hook: decode steps
   for (int i = 0; i < n;) {
     int m = 0;   // tokens of this batch: valid ids, one regime
     const bool fused = pos_ + 1 <= awo_max_;
@@ -790,25 +910,43 @@ void HipLlama::set_pos(int pos) {
   pos_ = pos; clean_pos_ = std::min(clean_pos_, pos);
 }
 
+// positions 0 .. n - 1 of a 4-bit layer against the fp16 rows in kv_stage_
+KvIoArgs HipLlama::stage_io(int l, int n) const {
+  KvIoArgs a = kv_io(l, nullptr, nullptr, n);
+  a.k = KvRows{kv_stage_, RT_F16, 0, kvd_, cfg_.head_dim}; a.v = KvRows{kv_stage_ + (size_t)ctx_ * kvd_, RT_F16, 0, kvd_, cfg_.head_dim};
+  a.pos = kv_zero_;
+  return a;
+}
+
 void HipLlama::snapshot(uint8_t *buf, int64_t cap) {
   if (cap < snapshot_size()) throw std::runtime_error("snapshot buffer too small");
   { QPH_CK(hipStreamSynchronize(st_)); check_status(); }
   memcpy(buf, &pos_, 4);
   // pieces of the snapshot's body gathered into the pinned slots ahead, copied to the caller's memory in turn
-  const size_t nb = (size_t)pos_ * kvd_ * 2, total = 2 * nb * cfg_.layers, pieces = (total + kSnapSlot - 1) / kSnapSlot;
-  auto gather = [&](size_t i) {
-    const size_t o = i * kSnapSlot;
-    QPH_CK(launch_cache_gather(kc_, vc_, (size_t)ctx_ * kvd_ * 2, nb, o, std::min(total - o, kSnapSlot), snap_host_ + i % kSnapSlots * kSnapSlot, st_));
-    QPH_CK(hipEventRecord(snap_ev_[i % kSnapSlots], st_));
-  };
-  try {
+  const size_t nb = (size_t)pos_ * kvd_ * 2;
+  auto fetch = [&](const uint16_t *kc, const uint16_t *vc, int layers, uint8_t *dst) {
+    const size_t total = 2 * nb * layers, pieces = (total + kSnapSlot - 1) / kSnapSlot;
+    auto gather = [&](size_t i) {
+      const size_t o = i * kSnapSlot;
+      QPH_CK(launch_cache_gather(kc, vc, (size_t)ctx_ * kvd_ * 2, nb, o, std::min(total - o, kSnapSlot), snap_host_ + i % kSnapSlots * kSnapSlot, st_));
+      QPH_CK(hipEventRecord(snap_ev_[i % kSnapSlots], st_));
+    };
     for (size_t i = 0; i < std::min(pieces, kSnapSlots); i++) gather(i);
     for (size_t i = 0; i < pieces; i++) {
       const size_t o = i * kSnapSlot;
       QPH_CK(hipEventSynchronize(snap_ev_[i % kSnapSlots]));
-      memcpy(buf + 4 + o, snap_host_ + i % kSnapSlots * kSnapSlot, std::min(total - o, kSnapSlot));
+      memcpy(dst + o, snap_host_ + i % kSnapSlots * kSnapSlot, std::min(total - o, kSnapSlot));
       if (i + kSnapSlots < pieces) gather(i + kSnapSlots);
     }
+  };
+  if (pos_ == 0) return;
+  try {
+    if (kv_kind_ != MK_Q4) fetch(kc_, vc_, cfg_.layers, buf + 4);
+    else
+      for (int l = 0; l < cfg_.layers; l++) {   // the layer's values as fp16 rows (exact), then as above
+        QPH_CK(launch_kv_read(MK_Q4, stage_io(l, pos_), st_));
+        fetch(kv_stage_, kv_stage_ + (size_t)ctx_ * kvd_, 1, buf + 4 + 2 * nb * l);
+      }
   } catch (...) { (void)hipStreamSynchronize(st_); throw; }
 }
 
@@ -820,6 +958,16 @@ void HipLlama::restore(const uint8_t *buf, int64_t n) {
   if (n < (int64_t)(4 + 2 * nb * cfg_.layers)) throw std::runtime_error("snapshot too short");
   { QPH_CK(hipStreamSynchronize(st_)); check_status(); }
   const uint8_t *p = buf + 4;
+  if (kv_kind_ == MK_Q4) {   // rows that a 4-bit cache gave out go back as they were, others are rounded
+    for (int l = 0; l < cfg_.layers && nb; l++, p += 2 * nb) {
+      QPH_CK(hipMemcpyAsync(kv_stage_, p, nb, hipMemcpyHostToDevice, st_));
+      QPH_CK(hipMemcpyAsync(kv_stage_ + (size_t)ctx_ * kvd_, p + nb, nb, hipMemcpyHostToDevice, st_));
+      QPH_CK(launch_kv_write(MK_Q4, stage_io(l, pos), st_));
+    }
+    QPH_CK(hipStreamSynchronize(st_));
+    pos_ = pos; clean_pos_ = pos;
+    return;
+  }
   for (int l = 0; l < cfg_.layers; l++)
     for (uint16_t *c : {kc_, vc_}) { QPH_CK(hipMemcpy(c + (size_t)l * ctx_ * kvd_, p, nb, hipMemcpyHostToDevice)); p += nb; }
   pos_ = pos; clean_pos_ = pos;
@@ -834,6 +982,7 @@ void HipLlama::restore(const uint8_t *buf, int64_t n) {
 void HipLlama::set_order(int mode) {
   if (mode != 0 && mode != 1) throw std::runtime_error("order: mode must be 0 (default) or 1 (reference order)");
   if (mode == 1) {
+    if (kv_custom()) throw std::runtime_error("order: the reference order has an fp16 cache and no window");
     if (head_.kind != MK_Q8 && head_.kind != MK_Q4) throw std::runtime_error("order: reference order needs a q8 or q4 output head");
     if (!ex_part_) {
       ex_ncmax_ = (ctx_ + 63) / 64;
@@ -998,6 +1147,7 @@ float HipLlama::time_kernel(int which, int iters, double *bytes) {
   const int L = tkl ? std::max(1, std::min(cfg_.layers, atoi(tkl))) : cfg_.layers, d = cfg_.hidden, cap = 1 << 20;
   int li = 0;
   const float eps = cfg_.rms_eps;
+  if (kv_custom() && which >= 6) throw std::runtime_error("time_kernel: the fused attention takes an fp16 cache without a window");
   write_ctl(0, std::min(pos_, ctx_ - 1));
   // QPH_AWO_STAMPS=file (measurement hook): the fused attention + wo kernel's per-workgroup realtime stamps of the
   // last timed launch, written to that file as text
@@ -1050,6 +1200,7 @@ float HipLlama::time_kernel(int which, int iters, double *bytes) {
         a.part = awo_part_; a.nparts = cfg_.kv_heads; a.pstride = (size_t)d; a.xsum = xs_;
         mv_plan(a, EPI_SWIGLU); QPH_CK(launch_matvec(PRO_NORM_SUM, EPI_SWIGLU, a, cap, st_)); break;
       case 5: {
+        if (kv_custom()) { kv_attend((int)(&ly - layers_.data()), q_, att_, 1); break; }
         AttnArgs t{}; t.q = q_; t.q16 = q16_; t.ctx = ctx_; t.kc = kc_; t.vc = vc_; t.ctl = ctl_;
         t.part = part_; t.att = att_; t.nh = cfg_.heads; t.nkv = cfg_.kv_heads; t.hd = cfg_.head_dim;
         t.max_chunks = max_chunks_; t.counters = counters_; t.single_max = attn_single_; t.split_pos = attn_split_pos_;
@@ -1068,7 +1219,10 @@ float HipLlama::time_kernel(int which, int iters, double *bytes) {
       case 2: sum += mat_bytes(ly.wq) + mat_bytes(ly.wk) + mat_bytes(ly.wv) + 4.0 * d; break;
       case 3: sum += mat_bytes(ly.wo); break;
       case 4: sum += mat_bytes(head_) + 4.0 * d + 4.0 * cfg_.vocab; break;
-      case 5: sum += 4.0 * (double)(pos_ + 1) * kvd_; break;
+      case 5: {
+        const double T = window_ > 0 ? std::min<double>(pos_ + 1, (double)window_ + sinks_) : pos_ + 1;
+        sum += (kv_kind_ == MK_Q4 ? 9.0 / 8 : 4.0) * T * kvd_; break;
+      }
       case 6: sum += 4.0 * (double)(pos_ + 1) * kvd_ + mat_bytes(ly.wo); break;
       case 7: sum += mat_bytes(ly.wg) + mat_bytes(ly.wu) + 4.0 * d * (1 + cfg_.kv_heads); break;
       default: throw std::runtime_error("time_kernel: unknown kernel id");

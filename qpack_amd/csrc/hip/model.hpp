@@ -42,6 +42,10 @@ class HipLlama {
     pos_ = pos; clean_pos_ = std::min(clean_pos_, pos); return true;
   }
   void set_pos(int pos);
+  // the cache's storage (MK_F32: fp16, MK_Q4: the records of kvcache.hip); needs position 0
+  void set_cache(int kind);
+  // attention sees the last `window` positions and the first `sinks` (0: all of them)
+  void set_window(int window, int sinks);
   int64_t snapshot_size() const { return 4 + 4ll * cfg_.layers * pos_ * kvd_; }
   void snapshot(uint8_t *buf, int64_t cap);
   void restore(const uint8_t *buf, int64_t n);
@@ -88,6 +92,21 @@ class HipLlama {
   Ctl *ctl_ = nullptr;
   int *out_tok_ = nullptr;
   uint16_t *kc_ = nullptr, *vc_ = nullptr;
+  // A 4-bit cache or a sliding window (kv_custom): decode steps and prompts attend through kvcache.hip's kernels, unfused
+  int kv_kind_ = MK_F32, window_ = 0, sinks_ = 0;
+  bool kv_custom() const { return kv_kind_ == MK_Q4 || window_ > 0; }
+  uint8_t *kv4_ = nullptr;        // [layers] records of all kv heads
+  size_t kv4_layer_ = 0;
+  uint16_t *kv_stage_ = nullptr;  // a 4-bit cache's layer as fp16 rows, K then V: snapshots
+  int *kv_zero_ = nullptr;        // a position 0
+  float *kv_part_ = nullptr;      // the attention's scratch, for the most that a step or a prompt's chunk takes
+  size_t kv_part_bytes_ = 0;
+  KvIoArgs kv_io(int l, float *k, float *v, int n) const;
+  KvIoArgs stage_io(int l, int n) const;
+  KvAttnArgs kv_attn(int l, const float *q, float *out, int n) const;
+  void kv_buffers();
+  void kv_append(int l, float *k, float *v, int n);
+  void kv_attend(int l, const float *q, float *out, int n);
   // pinned host
   Ctl *hctl_ = nullptr;
   float *hout_ = nullptr;
@@ -178,6 +197,8 @@ class HipLlama {
   void qkv_rope(MvArgs &a, uint16_t *kc, uint16_t *vc) const;
   void enqueue_head();
   void build_graphs();
+  void drop_graphs();
+  void dfree(void *p);
   hipGraphExec_t capture(int parts, bool fused = false, bool long_merge = false, int early = 0);
   // the early-load count of a one-split attention at this position (pos + 1 positions)
   static int early_for(int pos) { return std::min(kEarlyMax, (pos + 1 + 31) / 32); }

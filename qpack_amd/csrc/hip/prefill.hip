@@ -843,6 +843,16 @@ __global__ __launch_bounds__(256) void k_pf_rope(PfRopeArgs a) {
     }
   }
   const float *k = a.k + (size_t)t * a.ldk, *v = a.v + (size_t)t * a.ldk;
+  if (a.kout) {
+    float *ko = a.kout + (size_t)t * a.ldk;
+    for (int e = threadIdx.x; e < a.nkv * half; e += blockDim.x) {
+      const int g = e / half, i = e % half;
+      const float x0 = k[g * a.hd + i], x1 = k[g * a.hd + i + half];
+      ko[g * a.hd + i] = __builtin_fmaf(x0, cs[i], -(x1 * sn[i]));
+      ko[g * a.hd + i + half] = __builtin_fmaf(x1, cs[i], x0 * sn[i]);
+    }
+    return;
+  }
   uint16_t *kr = a.kc + (size_t)pos * kvd, *vr = a.vc + (size_t)pos * kvd;
   for (int e = threadIdx.x; e < a.nkv * half; e += blockDim.x) {
     const int g = e / half, i = e % half;

@@ -6,7 +6,7 @@ import mmap
 
 import numpy as np
 
-from ._lib import Config, LoadStatsC, check, lib
+from ._lib import QPH_F16, QPH_Q4, Config, LoadStatsC, check, lib
 
 
 def _fptr(a):
@@ -124,6 +124,15 @@ class HipLlama:
         """0: this library's kernels (default); 1: the reference CPU path's arithmetic order everywhere (bit-identical
         logits and greedy streams; slower)"""
         check(lib().qph_set_order(self._h, int(mode)))
+
+    def set_cache(self, kind):
+        """what the key / value cache holds, "f16" or "q4" (4-bit records, 9 / 32 of the bytes); at position 0 only"""
+        kinds = {"f16": QPH_F16, "q4": QPH_Q4}
+        check(lib().qph_set_cache(self._h, kinds.get(kind, kind)))
+
+    def set_window(self, window, sinks=0):
+        """attend to the last `window` positions and the first `sinks`; window 0: to all of them"""
+        check(lib().qph_set_window(self._h, int(window), int(sinks)))
 
     def rewind(self, pos):
         ok = C.c_int(0)
