@@ -82,7 +82,7 @@ static qph::KvIoArgs kv_io(const qph_kv *c, const qph_rows *k, const qph_rows *v
 static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sinks, qph::KvAttnArgs &a) {
   kv_cache(c, &a.cseq, &a.crow);
   if (heads < 1 || heads % c->kv_heads) throw std::invalid_argument("kv: heads must be a positive multiple of kv_heads");
-  if (n < 0 || n > 1 << 20 || (int64_t)n * heads > 1 << 28 || heads > 65535) throw std::invalid_argument("kv: n must be in [0, 2^20], heads <= 65535 and n * heads <= 2^28");
+  if (n < 0 || n > 1 << 20 || (int64_t)n * (heads / c->kv_heads) > 1 << 23 || heads > 65535) throw std::invalid_argument("kv: n must be in [0, 2^20], heads <= 65535 and n * heads / kv_heads <= 2^23");
   if (window < 0 || sinks < 0) throw std::invalid_argument("kv: window and sinks must not be negative");
   a.cache = c->k; a.cache_v = c->v; a.ctx = c->ctx; a.nrec = qph::kv4_records(c->ctx);
   a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.heads = heads; a.rep = heads / c->kv_heads; a.n = n;

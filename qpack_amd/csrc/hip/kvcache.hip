@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256) void k_kv16_io(KvIoArgs a) {
 }
 
 // ------------------------------------------------------------------ what a workgroup of the attention reads
-// Columns: a kv head's (token, query head) pairs, the head fastest; a workgroup has a.cols of them, c0 .. of sequence b.  The
+// Columns: a kv head's (token, query head) pairs, the head fastest; a workgroup has a.cols of them, a chunk of sequence b.  The
 // records any of its columns may see: the SR first ones (positions below sinks), then from the window's first on; virtual
 // record v is v, or v + skip from SR on.
 struct Span {
@@ -348,39 +348,44 @@ struct Span {
   int PA, PB;       // positions of the workgroup's first and last token
   int ws;           // first position of PA's window
   int SR, skip, NR; // virtual records
-  int nt, S;        // tiles of a.tile positions, splits in use
+  int nt, S;        // tiles, splits in use
   bool any;
 };
 // The columns of a chunk: a.cols from chunk * a.cols on, or, paired (many tokens, no window), half of them from the front and half from
 // the back.  A causal workgroup's time goes with its last position: paired, all take about as long (see k_kv_many)
 __device__ __forceinline__ int chunk_half(const KvAttnArgs &a, int chunk, int h) {   // the first column of half h
-  return (a.paired ? (h ? 2 * a.nchunk - 1 - chunk : chunk) : 2 * chunk + h) * (a.cols / 2);
+  return (a.paired ? (h ? 2 * a.nchunk - 1 - chunk : chunk) : 2 * chunk + h) << a.half_log2;
 }
 __device__ __forceinline__ int chunk_of(const KvAttnArgs &a, int col) {
-  const int u = col / (a.cols / 2);
-  return a.paired ? min(u, 2 * a.nchunk - 1 - u) : u / 2;
+  const int u = col >> a.half_log2;
+  return a.paired ? min(u, 2 * a.nchunk - 1 - u) : u >> 1;
 }
-__device__ __forceinline__ int last_token(const KvAttnArgs &a, int first) { return (first + a.cols / 2 - 1) / a.rep; }   // of a half
+// col / rep (kv_attn_plan's reciprocal): the compiler's divisions, 64-bit ones above all, were a third of a short call's instructions
+__device__ __forceinline__ int token_of(const KvAttnArgs &a, int col) {
+  return a.rep == 1 ? col : (int)(__umulhi((uint32_t)col, a.rep_mul) >> a.rep_shift);
+}
+__device__ __forceinline__ int last_token(const KvAttnArgs &a, int first) { return token_of(a, first + (1 << a.half_log2) - 1); }   // of a half
 __device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int chunk) {
   Span s;
   s.P0 = a.pos[b]; s.cnt = tokens_of(a.lens, b, a.n);
-  const int ta = chunk_half(a, chunk, 0) / a.rep, tb = last_token(a, chunk_half(a, chunk, 1));
+  const int ta = token_of(a, chunk_half(a, chunk, 0)), tb = last_token(a, chunk_half(a, chunk, 1));
   s.any = s.P0 >= 0 && ta < s.cnt && (int64_t)s.P0 + ta < a.ctx;
   s.PA = s.P0 + ta;
   // paired, the back half may lie behind the sequence's tokens while the front half does not reach them
   int te = min(tb, s.cnt - 1);
-  if (a.paired && chunk_half(a, chunk, 1) / a.rep >= s.cnt) te = min(last_token(a, chunk_half(a, chunk, 0)), s.cnt - 1);
+  if (a.paired && token_of(a, chunk_half(a, chunk, 1)) >= s.cnt) te = min(last_token(a, chunk_half(a, chunk, 0)), s.cnt - 1);
   s.PB = (int)min((int64_t)s.P0 + te, a.ctx - 1);
   s.ws = a.window > 0 ? max(0, s.PA - a.window + 1) : 0;
   const int r0 = s.ws / kRec;
-  s.SR = min((int)(((int64_t)a.sinks + kRec - 1) / kRec), r0);
+  s.SR = min((int)(((uint32_t)a.sinks + kRec - 1) / kRec), r0);
   s.skip = r0 - s.SR;
   s.NR = s.PB / kRec + 1 - s.skip;
-  const int rt = a.tile / kRec;
-  s.nt = (s.NR + rt - 1) / rt;
-  s.S = s.nt <= a.one_tiles ? 1 : min(a.nsplit, (s.nt + a.min_tiles - 1) / a.min_tiles);
+  s.nt = (s.NR + (1 << a.tile_log2) - 1) >> a.tile_log2;
+  s.S = s.nt <= a.one_tiles ? 1 : min(a.nsplit, (s.nt + (1 << a.min_log2) - 1) >> a.min_log2);
   return s;
 }
+// the first tile of share i of S (the product fits: nt <= 2^25, i <= 64)
+__device__ __forceinline__ int share(const Span &s, int i) { return s.S == 1 ? i * s.nt : (int)((uint32_t)i * (uint32_t)s.nt / (uint32_t)s.S); }
 __device__ __forceinline__ int record(const Span &s, int v) { return v < s.SR ? v : v + s.skip; }
 // whether the token at P, whose window starts behind lo, sees position p (no short cuts: these are lanes' values)
 __device__ __forceinline__ int behind(const KvAttnArgs &a, int P) { return a.window > 0 ? P - a.window : -1; }
@@ -532,16 +537,16 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   constexpr int kTileBytes = KIND == MK_Q4 ? 0 : NW * kFewTile * HD * 2, kOutBytes = NW * NC * QS * 4;
   __shared__ __align__(16) uint8_t sm[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
   __shared__ float wm[NW][NC], wl[NW][NC];
-  const int b = blockIdx.z, g = blockIdx.y / a.nchunk, chunk = blockIdx.y % a.nchunk, c0 = chunk * NC, split = blockIdx.x;
+  const int b = blockIdx.z, g = a.nchunk == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nchunk, chunk = blockIdx.y - g * a.nchunk, c0 = chunk * NC, split = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-  const int col = c0 + (TWO ? lr & 7 : lr), tok = col / a.rep;
+  const int col = c0 + (TWO ? lr & 7 : lr), tok = token_of(a, col), hr = col - tok * a.rep;
   // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j.  Asked for before
   // the sequence's position is known
   h8 q[KS];
   float x[KS][8];
   {
     const bool there = tok < a.n;
-    const int64_t at = b * a.q.seq + (int64_t)(there ? tok : 0) * a.q.tok + (int64_t)(g * a.rep + col % a.rep) * a.q.head;
+    const int64_t at = b * a.q.seq + (int64_t)(there ? tok : 0) * a.q.tok + (int64_t)(g * a.rep + hr) * a.q.head;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
       const int64_t d = at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg);
@@ -554,7 +559,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
   const int lo = behind(a, P);
-  const int t0 = (int)((int64_t)split * s.nt / s.S), t1 = (int)((int64_t)(split + 1) * s.nt / s.S);
+  const int t0 = share(s, split), t1 = share(s, split + 1);
   const Head h = head_of<HD, KIND>(a, b, g);
   uint16_t *vbuf = (uint16_t *)sm + wave * kFewTile * HD;
   Tile<HD, KIND> cur;
@@ -700,7 +705,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   __syncthreads();
   const int e = threadIdx.x, c = e / (HD / 4), d = 4 * (e % (HD / 4));
   if (c >= NC) return;
-  const int cc = c0 + c, tk = cc / a.rep;
+  const int cc = c0 + c, tk = token_of(a, cc);
   if (tk >= s.cnt || (int64_t)s.P0 + tk >= a.ctx) return;
   float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -713,7 +718,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
     L += wl[w][c] * k;
     y += *(const f32x4 *)(ored + (w * NC + c) * QS + d) * k;
   }
-  const int head = g * a.rep + cc % a.rep;
+  const int head = g * a.rep + cc - tk * a.rep;
   if (s.S == 1) {
     const float inv = 1.f / L;   // a visible position's score is -inf only where the plain softmax gives NaN too: 0 x inf
     float r[4];
@@ -733,7 +738,7 @@ template <int HD, int T>
 __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
   constexpr int CT = HD / 4, SL = 256 / CT;
   __shared__ f32x4 oo[SL][CT];
-  const int head = blockIdx.x, tok = blockIdx.y, b = blockIdx.z, g = head / a.rep;
+  const int head = blockIdx.x, tok = blockIdx.y, b = blockIdx.z, g = token_of(a, head);
   const int col = tok * a.rep + head - g * a.rep;
   const Span s = span_of(a, b, chunk_of(a, col));
   if (!s.any || s.S == 1 || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
@@ -781,24 +786,24 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   __shared__ __align__(16) uint16_t ks[3][kManyBlk * KST];
   __shared__ __align__(16) uint16_t vs[3][VN];
   __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
-  const int b = blockIdx.y, g = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv, split = rest % a.nsplit;
-  const int chunk = a.nchunk - 1 - rest / a.nsplit;   // without pairs: the last columns, with the most to read, first
+  const int b = blockIdx.z, g = blockIdx.x, rest = a.nsplit == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nsplit, split = blockIdx.y - rest * a.nsplit;
+  const int chunk = a.nchunk - 1 - rest;   // without pairs: the last columns, with the most to read, first
   const Span s = span_of(a, b, chunk);
   if (!s.any || split >= s.S) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, ln = lane & 31, hf = lane >> 5;
   // waves w and w + 4 share a SIMD: one of the front half, one of the back half
   const int cw = chunk_half(a, chunk, wave / (kManyWaves / 2)) + 32 * (wave % (kManyWaves / 2));
-  const int col = cw + ln, tok = col / a.rep, head = g * a.rep + col % a.rep;
+  const int col = cw + ln, tok = token_of(a, col), head = g * a.rep + col - tok * a.rep;
   const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
   const int lo = behind(a, P);
   // first and last position of the wave's own columns, and of the halves'
-  const int wa = cw / a.rep;
+  const int wa = token_of(a, cw);
   const bool wlive = wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
   auto position = [&](int t) { return (int)min((int64_t)s.P0 + min(t, s.cnt - 1), a.ctx - 1); };
-  const int PA = s.P0 + wa, PB = position((cw + 31) / a.rep);
-  const int A0 = s.PA, B0 = position(last_token(a, chunk_half(a, chunk, 0))), A1 = s.P0 + chunk_half(a, chunk, 1) / a.rep, B1 = s.PB;
-  const int kb0 = (int)((int64_t)split * s.nt / s.S), kb1 = (int)((int64_t)(split + 1) * s.nt / s.S);
+  const int PA = s.P0 + wa, PB = position(token_of(a, cw + 31));
+  const int A0 = s.PA, B0 = position(last_token(a, chunk_half(a, chunk, 0))), A1 = s.P0 + token_of(a, chunk_half(a, chunk, 1)), B1 = s.PB;
+  const int kb0 = share(s, split), kb1 = share(s, split + 1);
   const Head hd = head_of<HD, KIND>(a, b, g);
 
   // ---- a block's codes (or fp16 pieces): memory -> registers -> LDS
@@ -1115,17 +1120,23 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   const int64_t cols = (int64_t)a.n * a.rep;
   a.many = cols > 64;
   a.cols = a.many ? kManyCols : two ? 8 : 16;
-  a.tile = a.many ? kManyBlk : kFewTile;
-  a.min_tiles = a.many ? 4 : kFewWaves;
+  a.half_log2 = a.many ? 7 : two ? 2 : 3;
+  a.tile_log2 = a.many ? 3 : 2;   // records of a tile
+  a.min_log2 = a.many ? 2 : 3;    // tiles of a split, at least
   a.one_tiles = a.many ? 4 : 4 * kFewWaves;
+  const int tile = kRec << a.tile_log2;
+  // floor(col / rep) = floor(col mul / 2^(32 + shift)) for col < 2^30: mul = ceil(2^(32 + shift) / rep) with 2^shift < rep <= 2^(shift + 1)
+  a.rep_shift = 0;
+  while (2 << a.rep_shift < a.rep) a.rep_shift++;
+  a.rep_mul = a.rep == 1 ? 0 : (uint32_t)(((1ull << (32 + a.rep_shift)) + a.rep - 1) / a.rep);
   a.nchunk = (int)((cols + a.cols - 1) / a.cols);
   a.paired = a.many && a.window == 0;
   // positions that a workgroup can have to read, at most
   const int64_t reach = a.window > 0 ? std::min<int64_t>(a.ctx, (int64_t)a.window + a.sinks + (a.cols + a.rep - 1) / a.rep + 3 * kRec) : a.ctx;
-  const int64_t tiles = (reach + a.tile - 1) / a.tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
+  const int64_t tiles = (reach + tile - 1) / tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
   const int64_t want = (a.many ? 1 : 2) * (int64_t)cus / std::max<int64_t>(groups, 1);
-  a.nsplit = tiles <= a.one_tiles ? 1 : (int)std::max<int64_t>(1, std::min({want, (tiles + a.min_tiles - 1) / a.min_tiles, (int64_t)64}));
-  if (a.n > 65535) a.nsplit = 1;
+  a.nsplit = tiles <= a.one_tiles ? 1 : (int)std::max<int64_t>(1, std::min({want, (tiles >> a.min_log2) + 1, (int64_t)64}));
+  if (a.n > 65535 || a.nchunk * a.nsplit > 65535) a.nsplit = 1;   // grid limits
   return a.nsplit > 1 ? (size_t)a.nseq * a.n * a.heads * a.nsplit * (a.hd + 2) * 4 : 0;
 }
 
@@ -1135,7 +1146,7 @@ template <int HD, int T> static constexpr auto k_many4 = k_kv_many<HD, MK_Q4, T>
 template <int HD, int T> static constexpr auto k_many16 = k_kv_many<HD, MK_F32, T>;
 hipError_t launch_kv_attn(int kind, const KvAttnArgs &a, hipStream_t st) {
   if (a.many) {
-    const dim3 grid((unsigned)(a.nkv * a.nchunk * a.nsplit), a.nseq);
+    const dim3 grid(a.nkv, a.nchunk * a.nsplit, a.nseq);
     if (kind == MK_Q4) QPH_KV(k_many4, a.hd, a.q.type, grid, kManyWaves * 64, a);
     else QPH_KV(k_many16, a.hd, a.q.type, grid, kManyWaves * 64, a);
   } else {

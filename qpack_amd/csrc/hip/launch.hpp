@@ -321,7 +321,8 @@ struct KvAttnArgs {
   float scale2;                 // softmax scale times log2(e), > 0
   float *part;                  // nsplit > 1: partial sums, then (max, sum) pairs, kv_attn_plan's bytes
   // set by kv_attn_plan
-  int many, paired, cols, nchunk, tile, min_tiles, one_tiles, nsplit;
+  int many, paired, cols, half_log2, nchunk, tile_log2, min_log2, one_tiles, nsplit, rep_shift;
+  uint32_t rep_mul;
 };
 // how the call is laid out; the bytes of part
 size_t kv_attn_plan(KvAttnArgs &a);
