@@ -406,10 +406,10 @@ __device__ __forceinline__ float row_power(float mx) {   // 2^-e; 1 for rows tha
   return e == 0 || e >= 254 ? 1.f : __builtin_bit_cast(float, (254u - e) << 23);
 }
 
-// Probabilities are held as 2^(x - m + kPBias) where m follows the running maximum of a column only when that is more than kLag
-// above it: o is rescaled in few tiles rather than in most.  They stay below 2^(kPBias + kLag), fp16's range, and what lies 2^-32
-// below m is still there; the sum they are divided by is scaled alike.
-constexpr float kPBias = 8.f, kLag = 7.f, kRoom = 32768.f;   // kRoom: what a sum of weights may reach before the maximum is looked for
+// Probabilities are held as 2^(x - m + kPBias), where m is a column's maximum as it was when it was last looked for: when there was none,
+// and whenever a lane's weights of a tile add up to more than kRoom.  They stay in fp16's range, what lies 2^-32 below m is
+// still there, and the sum they are divided by is scaled alike.
+constexpr float kPBias = 8.f, kRoom = 32768.f;
 
 // ------------------------------------------------------------------ few tokens
 // Grid (split, kv head and column chunk, sequence), 8 waves, each streaming its own tiles of 32 positions (4 records) with
@@ -446,19 +446,29 @@ __device__ __forceinline__ Head head_of(const KvAttnArgs &a, int b, int g) {
 __device__ __forceinline__ int64_t row_of(const KvAttnArgs &a, const Span &s, int v, int j) {
   return min((int64_t)kRec * record(s, min(v, s.NR - 1)) + j, a.ctx - 1) * a.crow;
 }
+// whether records v .. v + n - 1 are there and follow each other
+__device__ __forceinline__ bool run_of(const Span &s, int v, int n) { return v + n <= s.NR && (s.skip == 0 || v >= s.SR || v + n <= s.SR); }
+// a 4-bit tile's loads: a scalar base and offsets that a lane keeps where its records follow each other (all tiles but a few)
+template <int HD>
+__device__ __forceinline__ const uint8_t *tile_base(const Head &h, const Span &s, int tile, bool run, int r) {   // r: the lane's record of the tile
+  return h.rec + (run ? (int64_t)record(s, 4 * tile) : (int64_t)record(s, min(4 * tile + r, s.NR - 1)) - r) * (9 * HD);
+}
 template <int HD, int KIND>
 __device__ __forceinline__ void load_k(const KvAttnArgs &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t) {
   const int lr = lane & 15, lg = lane >> 4;
   if constexpr (KIND == MK_Q4) {
-    const uint8_t *r = h.rec + (int64_t)record(s, min(4 * tile + (lr >> 2), s.NR - 1)) * (9 * HD);
+    const uint32_t ko = (lr >> 2) * (9 * HD) + (lr & 3) * (HD / 2) + lg * (HD / 8), so = (lr >> 2) * (9 * HD) + 8 * HD + 2 * ((lr & 3) * (HD / 32) + lg * HD / 128);
+    auto get = [&](const uint8_t *r) {
 #pragma unroll
-    for (int mt = 0; mt < 2; mt++) {
-      const int row = 4 * mt + (lr & 3);
-      const uint8_t *kp = r + row * (HD / 2) + lg * (HD / 8);
-      if constexpr (HD == 128) { const u32x4 x = *(const u32x4 *)kp; t.k[mt][0] = x[0]; t.k[mt][1] = x[1]; t.k[mt][2] = x[2]; t.k[mt][3] = x[3]; }
-      else { const u32x2 x = *(const u32x2 *)kp; t.k[mt][0] = x[0]; t.k[mt][1] = x[1]; }
-      t.ks[mt] = *(const uint16_t *)(r + 8 * HD + 2 * (row * (HD / 32) + lg * HD / 128));
-    }
+      for (int mt = 0; mt < 2; mt++) {
+        const uint8_t *kp = r + (ko + mt * 2 * HD);
+        if constexpr (HD == 128) { const u32x4 x = *(const u32x4 *)kp; t.k[mt][0] = x[0]; t.k[mt][1] = x[1]; t.k[mt][2] = x[2]; t.k[mt][3] = x[3]; }
+        else { const u32x2 x = *(const u32x2 *)kp; t.k[mt][0] = x[0]; t.k[mt][1] = x[1]; }
+        t.ks[mt] = *(const uint16_t *)(r + (so + mt * (HD / 4)));
+      }
+    };
+    if (run_of(s, 4 * tile, 4)) get(tile_base<HD>(h, s, tile, true, 0));
+    else get(tile_base<HD>(h, s, tile, false, lr >> 2));
   } else {
 #pragma unroll
     for (int mt = 0; mt < 2; mt++) {
@@ -476,15 +486,19 @@ template <int HD, int KIND>
 __device__ __forceinline__ void load_v(const KvAttnArgs &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t, uint16_t *buf) {
   const int lr = lane & 15, lg = lane >> 4;
   if constexpr (KIND == MK_Q4) {
-    const uint8_t *r = h.rec + (int64_t)record(s, min(4 * tile + lg, s.NR - 1)) * (9 * HD);
+    const uint32_t vo = lg * (9 * HD) + 4 * HD + lr * (HD / 4), so = lg * (9 * HD) + 8 * HD + HD / 2;
+    auto get = [&](const uint8_t *r) {
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-      const u32x4 x = *(const u32x4 *)(r + 4 * HD + lr * (HD / 4) + 16 * i);
+      for (int i = 0; i < HD / 64; i++) {
+        const u32x4 x = *(const u32x4 *)(r + (vo + 16 * i));
 #pragma unroll
-      for (int j = 0; j < 4; j++) t.v[4 * i + j] = x[j];
-    }
+        for (int j = 0; j < 4; j++) t.v[4 * i + j] = x[j];
+      }
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++) t.vs[i] = *(const u32x4 *)(r + 8 * HD + HD / 2 + 16 * i);
+      for (int i = 0; i < HD / 32; i++) t.vs[i] = *(const u32x4 *)(r + (so + 16 * i));
+    };
+    if (run_of(s, 4 * tile, 4)) get(tile_base<HD>(h, s, tile, true, 0));
+    else get(tile_base<HD>(h, s, tile, false, lg));
   } else {
     constexpr int SEG = HD / 8, RPI = 64 / SEG;   // 16-byte segments of a row, rows of a 1 KiB load
 #pragma unroll
@@ -586,7 +600,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   f32x4 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; d++) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, sub = kPBias;
   // the next tile's K is asked for once this one's is used, its V likewise: either is on its way during the other's product
   for (int tile = t0 + wave; tile < t1; tile += NW) {
     const int v = 4 * tile + lg, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
@@ -606,45 +620,51 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       }
     }
     if constexpr (KIND == MK_Q4) { if (tile + NW < t1) load_k<HD, KIND>(a, h, s, tile + NW, lane, cur); }
-    float y[8], bm = -INFINITY;
+    float y[8];
     uint32_t on = 255;   // positions that a column of the workgroup sees
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       y[j] = sc[j >> 2][j & 3];
       if (TWO) y[j] += xchg8_f(y[j]);
-      y[j] *= f;
     }
     if (edge) {
       on = seen_bits(a, s, v, p0);
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] = sees(a, Pin, lo, p0 + j) ? y[j] : -INFINITY;
     }
-#pragma unroll
-    for (int j = 0; j < 8; j++) bm = fmaxf(bm, y[j]);
-    bm = pair_max32(pair_max16(bm));
-    float corr = 1.f;
-    const bool up = __any(bm > m + kLag);
-    if (up) {
-      const float mn = fmaxf(m, bm);
-      corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-    }
-    const float sub = kPBias - (m == -INFINITY ? 0.f : m);
-    float rs = 0.f;
     h8 ph;
+    auto weights = [&]() {   // y -> ph and their sum over the lane's positions
+      float rs = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float pv = __builtin_amdgcn_exp2f(y[j] + sub);
-      rs += pv;
-      const _Float16 hi = (_Float16)pv;
-      ph[j] = TWO && lr >= 8 ? (_Float16)(pv - (float)hi) : hi;
-    }
-    rs = pair_sum32(pair_sum16(rs));
-    l = l * corr + rs;
-    if (up) {
+      for (int j = 0; j < 8; j += 2) {
+        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], f, sub)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j + 1], f, sub));
+        h2 hi = {(_Float16)w0, (_Float16)w1};
+        if constexpr (TWO) {
+          rs += w0; rs += w1;
+          if (lr >= 8) hi = (h2){(_Float16)(w0 - (float)hi[0]), (_Float16)(w1 - (float)hi[1])};
+        } else {
+          rs = __builtin_amdgcn_fdot2(hi, (h2){(_Float16)1.f, (_Float16)1.f}, rs, false);   // the sum of what the product takes
+        }
+        ph[j] = hi[0]; ph[j + 1] = hi[1];
+      }
+      return rs;
+    };
+    float rs = weights();
+    // The maximum is looked for only where the weights say that it has outgrown m, or where there is none yet
+    if (__any(!(rs <= kRoom) | (m == -INFINITY))) {
+      float bm = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; j++) bm = fmaxf(bm, y[j]);
+      bm = pair_max32(pair_max16(bm)) * f;   // f > 0
+      const float mn = fmaxf(m, bm), corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= corr;
 #pragma unroll
       for (int d = 0; d < DT; d++) o[d] *= corr;
+      sub = kPBias - (m == -INFINITY ? 0.f : m);
+      rs = weights();
     }
+    l += rs;
     // what no column sees may hold anything: zeroed (4-bit: its scales), since 0 x NaN is not 0; what only some see, without its
     // NaN and infinite values
     uint32_t bad = 0;
@@ -689,6 +709,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       }
     }
   }
+  l = pair_sum32(pair_sum16(l));
   // the waves' sums meet in LDS
   if (KIND != MK_Q4) __syncthreads();   // no wave's V tile is in use
   float *ored = (float *)sm;
@@ -817,10 +838,13 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   const int krow = tid >> 3, kw = tid & 7, vl = tid >> 6, vr = tid & 15, vt = tid >> 4 & 3;
   const uint32_t ko = krow / kRec * (9 * HD) + krow % kRec * (HD / 2) + 4 * W * kw, kso = krow / kRec * (9 * HD) + 8 * HD + 2 * (krow % kRec * (HD / 32) + W * kw / 4);
   const uint32_t vo = vl * (9 * HD) + 4 * HD + vr * (HD / 4) + 4 * W * vt, vso = vl * (9 * HD) + 8 * HD + HD / 2 + 16 * (W * vt / 2);
+  int64_t po[NP];
+#pragma unroll
+  for (int i = 0; i < NP; i++) po[i] = (int64_t)((tid + NT * i) / (HD / 8)) * a.crow + 8 * ((tid + NT * i) % (HD / 8));
   auto fetch = [&](int kb) {
     const int v0 = BR * kb;
     if constexpr (KIND == MK_Q4) {
-      if (v0 + BR <= s.NR && (s.skip == 0 || v0 >= s.SR || v0 + BR <= s.SR)) {   // records that follow each other
+      if (run_of(s, v0, BR)) {
         const uint8_t *r = hd.rec + (int64_t)record(s, v0) * (9 * HD);
         kq = *(const words *)(r + ko); ksc = *(const uint16_t *)(r + kso);
         vq = *(const words *)(r + vo); vsc = *(const u32x4 *)(r + vso);
@@ -831,12 +855,18 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
         vq = *(const words *)(rv + vo); vsc = *(const u32x4 *)(rv + vso);
       }
     } else {
+      const int64_t p0 = (int64_t)kRec * record(s, v0);
+      const bool run = run_of(s, v0, BR) && p0 + kManyBlk <= a.ctx;
+      const uint16_t *k0 = hd.k + p0 * a.crow, *v00 = hd.v + p0 * a.crow;
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        const int64_t at = row_of(a, s, v0 + x / kRec, x % kRec) + 8 * sg;
-        kp[i] = *(const u32x4 *)(hd.k + at);
-        vp[i] = *(const u32x4 *)(hd.v + at);
+        if (run) { kp[i] = *(const u32x4 *)(k0 + po[i]); vp[i] = *(const u32x4 *)(v00 + po[i]); }
+        else {
+          const int64_t at = row_of(a, s, v0 + x / kRec, x % kRec) + 8 * sg;
+          kp[i] = *(const u32x4 *)(hd.k + at);
+          vp[i] = *(const u32x4 *)(hd.v + at);
+        }
       }
     }
   };
