@@ -804,8 +804,9 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   constexpr int KST = HD + 8;                                   // halves of a K row in LDS: an odd number of 16-byte columns
   constexpr int VST = KIND == MK_Q4 ? kManyBlk + 8 : HD + 32;   // of a V^T row (dims), or a V row (positions): 4 rows of 64 bytes apart
   constexpr int VN = KIND == MK_Q4 ? HD * VST : kManyBlk * VST;
-  __shared__ __align__(16) uint16_t ks[3][kManyBlk * KST];
-  __shared__ __align__(16) uint16_t vs[3][VN];
+  __shared__ __align__(16) uint16_t blocks[3 * (kManyBlk * KST + VN)];
+  auto k_of = [&](int kb) { return blocks + kb % 3 * (kManyBlk * KST); };
+  auto v_of = [&](int kb) { return blocks + 3 * (kManyBlk * KST) + kb % 3 * VN; };
   __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
   const int b = blockIdx.z, g = blockIdx.x, rest = a.nsplit == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nsplit, split = blockIdx.y - rest * a.nsplit;
   const int chunk = a.nchunk - 1 - rest;   // without pairs: the last columns, with the most to read, first
@@ -823,7 +824,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   const bool wlive = wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
   auto position = [&](int t) { return (int)min((int64_t)s.P0 + min(t, s.cnt - 1), a.ctx - 1); };
   const int PA = s.P0 + wa, PB = position(token_of(a, cw + 31));
-  const int A0 = s.PA, B0 = position(last_token(a, chunk_half(a, chunk, 0))), A1 = s.P0 + token_of(a, chunk_half(a, chunk, 1)), B1 = s.PB;
+  const int A0 = s.PA, B0 = position(last_token(a, chunk_half(a, chunk, 0))), A1 = s.P0 + token_of(a, chunk_half(a, chunk, 1));
   const int kb0 = share(s, split), kb1 = share(s, split + 1);
   const Head hd = head_of<HD, KIND>(a, b, g);
 
@@ -832,27 +833,25 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   // group write V^T rows next to each other.  fp16: pieces tid + NT i
   constexpr int W = HD / 64, NP = KIND == MK_Q4 ? 1 : kManyBlk * HD / 8 / NT;
   typedef uint32_t words __attribute__((ext_vector_type(W)));
-  words kq, vq;
-  uint16_t ksc;
-  u32x4 vsc, kp[NP], vp[NP];
+  struct Stage { words kq, vq; uint16_t ksc; u32x4 vsc, kp[NP], vp[NP]; };
   const int krow = tid >> 3, kw = tid & 7, vl = tid >> 6, vr = tid & 15, vt = tid >> 4 & 3;
   const uint32_t ko = krow / kRec * (9 * HD) + krow % kRec * (HD / 2) + 4 * W * kw, kso = krow / kRec * (9 * HD) + 8 * HD + 2 * (krow % kRec * (HD / 32) + W * kw / 4);
   const uint32_t vo = vl * (9 * HD) + 4 * HD + vr * (HD / 4) + 4 * W * vt, vso = vl * (9 * HD) + 8 * HD + HD / 2 + 16 * (W * vt / 2);
   int64_t po[NP];
 #pragma unroll
   for (int i = 0; i < NP; i++) po[i] = (int64_t)((tid + NT * i) / (HD / 8)) * a.crow + 8 * ((tid + NT * i) % (HD / 8));
-  auto fetch = [&](int kb) {
+  auto fetch = [&](int kb, Stage &g) {
     const int v0 = BR * kb;
     if constexpr (KIND == MK_Q4) {
       if (run_of(s, v0, BR)) {
         const uint8_t *r = hd.rec + (int64_t)record(s, v0) * (9 * HD);
-        kq = *(const words *)(r + ko); ksc = *(const uint16_t *)(r + kso);
-        vq = *(const words *)(r + vo); vsc = *(const u32x4 *)(r + vso);
+        g.kq = *(const words *)(r + ko); g.ksc = *(const uint16_t *)(r + kso);
+        g.vq = *(const words *)(r + vo); g.vsc = *(const u32x4 *)(r + vso);
       } else {
         const uint8_t *r = hd.rec + ((int64_t)record(s, min(v0 + krow / kRec, s.NR - 1)) - krow / kRec) * (9 * HD);
         const uint8_t *rv = hd.rec + ((int64_t)record(s, min(v0 + vl, s.NR - 1)) - vl) * (9 * HD);
-        kq = *(const words *)(r + ko); ksc = *(const uint16_t *)(r + kso);
-        vq = *(const words *)(rv + vo); vsc = *(const u32x4 *)(rv + vso);
+        g.kq = *(const words *)(r + ko); g.ksc = *(const uint16_t *)(r + kso);
+        g.vq = *(const words *)(rv + vo); g.vsc = *(const u32x4 *)(rv + vso);
       }
     } else {
       const int64_t p0 = (int64_t)kRec * record(s, v0);
@@ -861,94 +860,110 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        if (run) { kp[i] = *(const u32x4 *)(k0 + po[i]); vp[i] = *(const u32x4 *)(v00 + po[i]); }
+        if (run) { g.kp[i] = *(const u32x4 *)(k0 + po[i]); g.vp[i] = *(const u32x4 *)(v00 + po[i]); }
         else {
           const int64_t at = row_of(a, s, v0 + x / kRec, x % kRec) + 8 * sg;
-          kp[i] = *(const u32x4 *)(hd.k + at);
-          vp[i] = *(const u32x4 *)(hd.v + at);
+          g.kp[i] = *(const u32x4 *)(hd.k + at);
+          g.vp[i] = *(const u32x4 *)(hd.v + at);
         }
       }
     }
   };
-  // first and last position of a block, and whether some columns of tokens A .. B do not see all of it
-  auto first = [&](int kb) { return kRec * record(s, BR * kb); };
-  auto last = [&](int kb) { return kRec * record(s, min(BR * kb + BR - 1, s.NR - 1)) + kRec - 1; };
-  auto partial = [&](int kb, int A, int B) {
-    const int pf = first(kb), pl = last(kb);
-    return BR * kb + BR > s.NR || pl > A || (a.window > 0 && pf <= B - a.window && pl >= a.sinks);
-  };
+  // Blocks by number.  A block from the window's on holds positions 64 kb + 8 skip ..; those before it (the first positions that stay
+  // visible) count as seen in part.  Of tokens A .. B: from whole(A) on A does not see all of a block, before left(B) B does not,
+  // ends(B) is the last that B sees some of.  (Comparisons with these few numbers: worked out anew for every block, they were a
+  // third of the loop's instructions, and a wave issues one in about ten cycles)
+  const int NRb = s.NR / BR, R0 = s.skip ? (s.SR + BR - 1) / BR : 0, off = kRec * s.skip;
+  auto whole = [&](int A) { return min((A + 1 - off) >> 6, NRb); };
+  auto left = [&](int B) { return a.window > 0 ? max((B - a.window - off) >> 6, -1) + 1 : 0; };
+  auto ends = [&](int B) { return (B - off) >> 6; };
+  static_assert(kManyBlk == 64, "the shifts above");
+  const int wK = whole(PA), wY = max(left(PB), R0), wE = wlive ? ends(PB) : -1;          // the wave's
+  const int gK0 = whole(A0), gE0 = ends(B0), gK1 = whole(A1), gY = max(left(s.PB), R0);   // the workgroup's halves'
+  auto partial = [&](int kb) { return (kb >= wK) | (kb < wY); };
   // the same of the waves that take the block: a wave does not take a block behind its last position
-  auto partial_any = [&](int kb) {
-    const int pf = first(kb);
-    return BR * kb + BR > s.NR || (pf <= B0 && partial(kb, A0, B0)) || (pf <= B1 && partial(kb, A1, B1));
-  };
+  auto partial_any = [&](int kb) { return ((kb >= gK0) & (kb <= gE0)) | (kb >= gK1) | (kb < gY); };
   // what no column sees zeroed, and what only some see without its NaN and infinite values (4-bit: by the scales)
-  auto clean = [&](int kb) {
+  auto clean = [&](int kb, Stage &g) {
     if constexpr (KIND == MK_Q4) {
       const int v = BR * kb + vl;
-      const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))), bad = on & not_finite(vsc);
+      const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))), bad = on & not_finite(g.vsc);
       if (bad) atomicOr(&badp[(kb - kb0) % 4][vl / 4], bad << 8 * (vl % 4));
-      vsc = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, vsc), on & ~bad));
+      g.vsc = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, g.vsc), on & ~bad));
     } else {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int x = (tid + NT * i) / (HD / 8), v = BR * kb + x / kRec;
-        const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))) >> x % kRec & 1 ? 255u : 0u, bad = on & not_finite(vp[i]);
+        const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))) >> x % kRec & 1 ? 255u : 0u, bad = on & not_finite(g.vp[i]);
         if (bad) atomicOr(&badp[(kb - kb0) % 4][x / 32], 1u << x % 32);
-        vp[i] = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, vp[i]), on & ~bad));
+        g.vp[i] = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, g.vp[i]), on & ~bad));
       }
     }
   };
-  auto expand = [&](int kb) {
-    uint16_t *kd = ks[kb % 3], *vd = vs[kb % 3];
+  auto expand = [&](int kb, Stage &g) {
+    uint16_t *kd = k_of(kb), *vd = v_of(kb);
     if constexpr (KIND == MK_Q4) {
 #pragma unroll
       for (int i = 0; i < W; i++) {
-        *(h8 *)(kd + krow * KST + 8 * (W * kw + i)) = values(kq[i], ksc);
-        *(h8 *)(vd + (16 * (W * vt + i) + vr) * VST + kRec * vl) = values(vq[i], vsc);
+        *(h8 *)(kd + krow * KST + 8 * (W * kw + i)) = values(g.kq[i], g.ksc);
+        *(h8 *)(vd + (16 * (W * vt + i) + vr) * VST + kRec * vl) = values(g.vq[i], g.vsc);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NP; i++) {
         const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        *(u32x4 *)(kd + x * KST + 8 * sg) = kp[i];
-        *(u32x4 *)(vd + x * VST + 8 * sg) = vp[i];
+        *(u32x4 *)(kd + x * KST + 8 * sg) = g.kp[i];
+        *(u32x4 *)(vd + x * VST + 8 * sg) = g.vp[i];
       }
     }
   };
   if (tid < 8) badp[tid / 2][tid % 2] = 0;
-  fetch(kb0);
-  // ---- queries
   h8 q[KQ], ql[TWO ? KQ : 1];
   float f = a.scale2;
-  {
-    // (columns past the last token are some row's: nothing of them is stored)
-    const int64_t at = b * a.q.seq + (int64_t)min(tok, a.n - 1) * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
-    float x[KQ][8], mx = 0.f;
+  Stage st;
+  {  // the first two blocks, asked for together
+    Stage st1;
+    fetch(kb0, st);
+    if (kb0 + 1 < kb1) fetch(kb0 + 1, st1);
+    // ---- queries
+    {
+      // (columns past the last token are some row's: nothing of them is stored)
+      const int64_t at = b * a.q.seq + (int64_t)min(tok, a.n - 1) * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
+      float x[KQ][8], mx = 0.f;
 #pragma unroll
-    for (int k = 0; k < KQ; k++) {
-      if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
-      else {
-        load_elems<T, 8>(a.q, at + 16 * k, x[k]);
+      for (int k = 0; k < KQ; k++) {
+        if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
+        else {
+          load_elems<T, 8>(a.q, at + 16 * k, x[k]);
 #pragma unroll
-        for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
+          for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
+        }
+      }
+      if constexpr (T != RT_F16) {
+        mx = pair_max32(mx);
+        const float p2 = row_power(mx);
+        f /= p2;
+#pragma unroll
+        for (int k = 0; k < KQ; k++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const float y = x[k][j] * p2;
+            const _Float16 h = (_Float16)y;
+            q[k][j] = h;
+            if constexpr (TWO) ql[k][j] = (_Float16)(y - (float)h);
+          }
       }
     }
-    if constexpr (T != RT_F16) {
-      mx = pair_max32(mx);
-      const float p2 = row_power(mx);
-      f /= p2;
-#pragma unroll
-      for (int k = 0; k < KQ; k++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float y = x[k][j] * p2;
-          const _Float16 h = (_Float16)y;
-          q[k][j] = h;
-          if constexpr (TWO) ql[k][j] = (_Float16)(y - (float)h);
-        }
+    __syncthreads();   // badp
+    if (partial_any(kb0)) clean(kb0, st);
+    expand(kb0, st);
+    if (kb0 + 1 < kb1) {
+      if (partial_any(kb0 + 1)) clean(kb0 + 1, st1);
+      expand(kb0 + 1, st1);
     }
   }
+  if (kb0 + 2 < kb1) fetch(kb0 + 2, st);
+  __syncthreads();
   f32x16 o[OT];
 #pragma unroll
   for (int t = 0; t < OT; t++)
@@ -969,7 +984,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   h8 ph[4], pl[TWO ? 4 : 1];
   f32x16 sc[2];
   auto dots = [&](int kb) {   // K q of a block
-    const uint16_t *kl = ks[kb % 3];
+    const uint16_t *kl = k_of(kb);
 #pragma unroll
     for (int mt = 0; mt < 2; mt++) {
 #pragma unroll
@@ -1003,7 +1018,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     return rs;
   };
   auto product = [&](int kb) {
-    const uint16_t *vb = vs[kb % 3];
+    const uint16_t *vb = v_of(kb);
 #pragma unroll
     for (int u = 0; u < 4; u++)
 #pragma unroll
@@ -1028,28 +1043,18 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
         }
       }
   };
-  auto wanted = [&](int kb) {   // whether one of the wave's columns sees some of a block
-    if (!wlive) return false;
-    const int pf = first(kb), pe = last(kb);
-    return pf <= PB && !(a.window > 0 && pe <= PA - a.window && pf >= a.sinks);
-  };
-  __syncthreads();   // badp
-  if (partial_any(kb0)) clean(kb0);
-  expand(kb0);
-  if (kb0 + 1 < kb1) {
-    fetch(kb0 + 1);
-    if (partial_any(kb0 + 1)) clean(kb0 + 1);
-    expand(kb0 + 1);
-  }
-  if (kb0 + 2 < kb1) fetch(kb0 + 2);
-  __syncthreads();
+  auto first = [&](int kb) { return kRec * record(s, BR * kb); };
+  auto last = [&](int kb) { return kRec * record(s, min(BR * kb + BR - 1, s.NR - 1)) + kRec - 1; };
   // Step kb: K q, the weights, then P V beside the expansion of block kb + 2 (whose codes were asked for a step ago); kb + 3 is asked for.
   // Two blocks ahead, not one: 4 % less time
   for (int kb = kb0; kb < kb1; kb++) {
-    if (kb + 2 < kb1 && partial_any(kb + 2)) clean(kb + 2);
-    if (wanted(kb)) {
+    if (kb + 2 < kb1 && partial_any(kb + 2)) clean(kb + 2, st);
+    // one of the wave's columns sees some of the block?  (Read through the lane: left to itself the compiler splits the loop at wE and
+    // keeps two copies of o, 58 registers more)
+    const int before = (int)(a.window > 0) & (int)(kb < wY) & (int)(last(kb) <= PA - a.window) & (int)(first(kb) >= a.sinks);
+    if (__builtin_amdgcn_readfirstlane((int)(kb <= wE) & (before ^ 1))) {
       dots(kb);
-      if (partial(kb, PA, PB)) {
+      if (partial(kb)) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
           const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
@@ -1076,16 +1081,47 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       }
       l += rs;
       product(kb);
-      expand(kb + 2);   // (past the last block: what the registers hold, to a place that is not read again)
+      expand(kb + 2, st);   // (past the last block: what the registers hold, to a place that is not read again)
       if (partial_any(kb)) fix(kb);   // (also for the columns of a wave that see all of it)
     } else {
-      expand(kb + 2);
+      expand(kb + 2, st);
     }
-    if (kb + 3 < kb1) fetch(kb + 3);
+    if (kb + 3 < kb1) fetch(kb + 3, st);
     if (tid < 2) badp[(kb - kb0 + 3) % 4][tid] = 0;
     __syncthreads();
   }
   l = pair_sum32(l);
+  if constexpr (T != RT_F32) {
+    if (s.S == 1) {
+      // A lane has 4 dims here and there of its column; by way of the wave's own part of LDS the rows leave in 16-byte pieces
+      // next to each other (6800 -> 4000 cycles of a workgroup's end)
+      constexpr int RS = HD + 8;
+      static_assert(kManyWaves * 32 * RS <= 3 * (kManyBlk * KST + VN), "the columns fit where the blocks were");
+      uint16_t *ow = blocks + wave * 32 * RS;
+      const float inv = 1.f / l;
+      const KvRows lds{ow + ln * RS, T, 0, 0, 0};
+#pragma unroll
+      for (int t = 0; t < OT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float r[4] = {o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv};
+          store_elems<T, 4>(lds, 32 * t + 8 * i + 4 * hf, r);
+        }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      constexpr int LR = HD / 8, RI = 64 / LR;   // lanes of a row, rows at a time
+#pragma unroll
+      for (int i = 0; i < 32 / RI; i++) {
+        const int c = RI * i + lane / LR, cc = cw + c, tk = token_of(a, cc);
+        if (tk < s.cnt && (int64_t)s.P0 + tk < a.ctx) {
+          const int64_t at = b * a.out.seq + (int64_t)tk * a.out.tok + (int64_t)(g * a.rep + cc - tk * a.rep) * a.out.head + 8 * (lane % LR);
+          *(u32x4_any *)((uint16_t *)a.out.p + at) = *(const u32x4 *)(ow + c * RS + 8 * (lane % LR));
+        }
+      }
+      return;
+    }
+  }
   if (!live) return;
   if (s.S == 1) {
     const float inv = 1.f / l;
