@@ -1094,7 +1094,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   if constexpr (T != RT_F32) {
     if (s.S == 1) {
       // A lane has 4 dims here and there of its column; by way of the wave's own part of LDS the rows leave in 16-byte pieces
-      // next to each other (6800 -> 4000 cycles of a workgroup's end)
+      // next to each other (4096 tokens with 32 heads: 105 -> 101 us)
       constexpr int RS = HD + 8;
       static_assert(kManyWaves * 32 * RS <= 3 * (kManyBlk * KST + VN), "the columns fit where the blocks were");
       uint16_t *ow = blocks + wave * 32 * RS;
