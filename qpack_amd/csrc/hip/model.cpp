@@ -320,7 +320,7 @@ void HipLlama::kv_attend(int l, const float *q, float *out, int n) {
 // scratch for every number of tokens that a call can have
 void HipLlama::kv_buffers() {
   size_t need = 0;
-  for (int n = 1; n <= pf_cap_; n++) { KvAttnArgs a = kv_attn(0, nullptr, nullptr, n); need = std::max(need, kv_attn_plan(a)); }
+  for (int n = 1; n <= std::max(1, pf_cap_); n++) { KvAttnArgs a = kv_attn(0, nullptr, nullptr, n); need = std::max(need, kv_attn_plan(a)); }
   if (need > kv_part_bytes_) {
     float *p = (float *)dalloc(need);
     dfree(kv_part_);
@@ -342,8 +342,8 @@ void HipLlama::set_cache(int kind) {
     try {
       rec = (uint8_t *)dalloc(layer * cfg_.layers);
       stage = (uint16_t *)dalloc(2 * row);
-      if (!zero) { zero = (int *)dalloc(sizeof(int)); kv_zero_ = zero; QPH_CK(hipMemset(zero, 0, sizeof(int))); }
-      QPH_CK(hipMemset(rec, 0, layer * cfg_.layers));
+      if (!zero) { zero = (int *)dalloc(sizeof(int)); kv_zero_ = zero; QPH_CK(hipMemsetAsync(zero, 0, sizeof(int), st_)); }
+      QPH_CK(hipMemsetAsync(rec, 0, layer * cfg_.layers, st_));
       kv_buffers();
     } catch (...) { dfree(rec); dfree(stage); throw; }
     drop_graphs();
@@ -355,7 +355,7 @@ void HipLlama::set_cache(int kind) {
     uint16_t *k = nullptr, *v = nullptr;
     try {
       k = (uint16_t *)dalloc(bytes); v = (uint16_t *)dalloc(bytes);
-      QPH_CK(hipMemset(k, 0, bytes)); QPH_CK(hipMemset(v, 0, bytes));
+      QPH_CK(hipMemsetAsync(k, 0, bytes, st_)); QPH_CK(hipMemsetAsync(v, 0, bytes, st_));
     } catch (...) { dfree(k); dfree(v); throw; }
     drop_graphs();
     dfree(kv4_); dfree(kv_stage_);
