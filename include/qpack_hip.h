@@ -202,7 +202,8 @@ int qph_pack(const char *src, const char *dst, int threads, int *coded);
  *   K codes  position i at bytes i head_dim / 2; its 32-bit word w holds dims 8 w .. 8 w + 7, dim 8 w + 2 e + o at bits 16 o + 4 e
  *   V codes  at 4 head_dim: dim d in word (d % 16) (head_dim / 16) + d / 16, position 2 e + o at bits 16 o + 4 e
  *   K scales at 8 head_dim: fp16 [8 positions][head_dim / 32];  V scales at 8.5 head_dim: fp16 [head_dim / 32][8 positions]
- * Memory that was never written may hold anything: no position that a token does not see changes its result. */
+ * Memory that was never written may hold anything: no position that a token does not see changes its result.
+ * A word of V codes holds 8 positions: writes to one cache follow each other (one stream, or events), and precede the calls that read them. */
 typedef struct {
   int kind;                            /* QPH_F16 or QPH_Q4 */
   int nseq, kv_heads, head_dim;        /* head_dim 64 or 128; nseq <= 65535, kv_heads <= 4096 */
@@ -220,7 +221,8 @@ typedef struct {
 /* bytes of a QPH_Q4 cache, or of K and V together of a QPH_F16 one without gaps */
 int qph_kv_bytes(int kind, int nseq, int kv_heads, int head_dim, int64_t ctx, int64_t *bytes);
 /* Token t of sequence b, t < min(n, lens[b]) (lens NULL: t < n), is position pos[b] + t; sequences with pos[b] < 0 and
- * positions at or past ctx take no part: nothing of them is written, and what their rows hold does not matter.  n <= 2^20.
+ * positions at or past ctx take no part: nothing of them is written, and what their rows hold does not matter.  n <= 2^20, and
+ * for an fp16 cache n * kv_heads * head_dim <= 2^34.  Rows that a call writes must not overlap.
  * qph_kv_write rounds k and v (one type) into the cache; what else the cache holds stays.  qph_kv_read returns what it holds, rounded to the
  * rows' type (fp16 and fp32: exact). */
 int qph_kv_write(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, const int *pos, const int *lens, void *stream);

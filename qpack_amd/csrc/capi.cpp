@@ -2,11 +2,13 @@
 // and turns it into status -1 plus a thread-local message, so no exception crosses the C boundary.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <memory>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/qpack_hip.h"
@@ -59,13 +61,23 @@ static void kv_cache(const qph_kv *c, int64_t *seq, int64_t *row) {
   *seq = c->seq ? c->seq : c->ctx * *row;
   if ((uintptr_t)c->v % 16 || *row % 8 || *seq % 8) throw std::invalid_argument("kv: an fp16 cache must be 16-byte aligned and its strides multiples of 8");
   if (*row < d || (c->nseq > 1 && *seq < (c->ctx - 1) * *row + d)) throw std::invalid_argument("kv: the cache's rows or sequences overlap");
+  if (c->k == c->v) throw std::invalid_argument("kv: the cache's k and v overlap");
 }
 static qph::KvRows kv_rows(const qph_rows *r, const char *what, bool out, int nseq, int n, int heads, int hd) {
   need(r, what); need(r->p, what);
   if (r->type != QPH_F32 && r->type != QPH_F16 && r->type != QPH_BF16) throw std::invalid_argument(std::string("kv: the type of ") + what + " must be QPH_F32, QPH_F16 or QPH_BF16");
   if ((uintptr_t)r->p % (r->type == QPH_F32 ? 4 : 2)) throw std::invalid_argument(std::string("kv: ") + what + " is not aligned to its type");
   if (r->seq < 0 || r->tok < 0 || r->head < 0) throw std::invalid_argument(std::string("kv: negative strides of ") + what);
-  if (out && ((nseq > 1 && r->seq < hd) || (n > 1 && r->tok < hd) || (heads > 1 && r->head < hd))) throw std::invalid_argument(std::string("kv: the rows of ") + what + " overlap");
+  if (out) {   // rows that are written lie apart: by rising strides, each step is past what the smaller ones cover
+    std::pair<int64_t, int> d[3] = {{r->seq, nseq}, {r->tok, n}, {r->head, heads}};
+    std::sort(d, d + 3);
+    __int128 covered = hd;
+    for (const auto &[stride, count] : d) {
+      if (count <= 1) continue;
+      if (stride < covered) throw std::invalid_argument(std::string("kv: the rows of ") + what + " overlap");
+      covered += (__int128)stride * (count - 1);
+    }
+  }
   return {r->p, r->type == QPH_F32 ? qph::RT_F32 : r->type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16, r->seq, r->tok, r->head};
 }
 static qph::KvIoArgs kv_io(const qph_kv *c, const qph_rows *k, const qph_rows *v, bool out, int n, const int *pos, const int *lens) {
@@ -77,6 +89,9 @@ static qph::KvIoArgs kv_io(const qph_kv *c, const qph_rows *k, const qph_rows *v
   a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.n = n; a.pos = pos; a.lens = lens;
   a.k = kv_rows(k, "k", out, c->nseq, n, c->kv_heads, c->head_dim); a.v = kv_rows(v, "v", out, c->nseq, n, c->kv_heads, c->head_dim);
   if (a.k.type != a.v.type) throw std::invalid_argument("kv: k and v must have the same type");
+  if (out && n && k->p == v->p) throw std::invalid_argument("kv: the rows of k and v overlap");
+  // the launch counts an fp16 cache's threads, 8 dims each, in 32 bits
+  if (c->kind == QPH_F16 && (int64_t)n * c->kv_heads * c->head_dim > (int64_t)1 << 34) throw std::invalid_argument("kv: n * kv_heads * head_dim must not pass 2^34 for an fp16 cache");
   return a;
 }
 static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sinks, qph::KvAttnArgs &a) {
@@ -441,6 +456,7 @@ int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, in
     if (!(scale >= 0.f) || std::isinf(scale)) throw std::invalid_argument("kv: scale must be finite and not negative (0: 1 / sqrt(head_dim))");
     a.pos = pos; a.lens = lens;
     a.scale2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim));
+    if (std::isinf(a.scale2)) throw std::invalid_argument("kv: scale is too large");
     if (n) {
       const int64_t bytes = (int64_t)qph::kv_attn_plan(a);
       if (bytes && (!work || work_bytes < bytes || (uintptr_t)work % 16)) throw std::invalid_argument("kv: work must have the " + std::to_string(bytes) + " bytes that qph_kv_attention_work gives, 16-byte aligned");

@@ -166,6 +166,7 @@ PyObject *attention(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
     return nullptr;
   const double scale = PyFloat_AsDouble(arg[6]);
   if (PyErr_Occurred()) return nullptr;
+  if (scale != 0 && (float)scale == 0.f) { fail("kv: scale is too small%s%s", ""); return nullptr; }   // (0 means the default)
   if (n != n2 || h != h2) { fail("kv: out must have q's shape%s%s", ""); return nullptr; }
   if (n > INT32_MAX || h > INT32_MAX) { fail("kv: q is too large%s%s", ""); return nullptr; }
   if (qph_kv_attention_work(&c->c, q.type, (int)h, (int)n, window, sinks, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }

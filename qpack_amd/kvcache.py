@@ -31,7 +31,10 @@ class KvCache:
     position's rows contiguous.
 
     In all calls token t < n of sequence b, and t < lens[b] where lens is given, is position pos[b] + t; sequences with pos[b] <
-    0 and positions at or past ctx take no part.  pos and lens: int32 tensors [nseq] on the cache's device."""
+    0 and positions at or past ctx take no part.  pos and lens: int32 tensors [nseq] on the cache's device.
+
+    Writes to one cache follow each other: from several streams they need events between them.  Nothing here carries
+    gradients."""
 
     def __init__(self, kind, nseq, kv_heads, head_dim, ctx, data=None, device="cuda"):
         import torch

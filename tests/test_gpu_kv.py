@@ -290,6 +290,18 @@ def test_attention_query_range(type, size):
 
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_attention_vanishing_scores(kind, type):
+    """the scale times a row's power is below fp32's range: the positions weigh alike, the masked ones nothing"""
+    gen = torch.Generator().manual_seed(12)
+    c, K, V = filled(kind, 1, 1, 64, 200, [200], gen)
+    for n in (3, 80):
+        q = (torch.randn(1, n, 4, 64, generator=gen) * 1e-37).to(TYPES[type]).cuda()
+        out = c.attention(q, i32([200 - n]), scale=1e-9)
+        check_rows(out[0], q[0], K[0], V[0], 200 - n, scale=1e-9)
+
+
+@pytest.mark.parametrize("kind", ["q4", "f16"])
 def test_attention_far_smaller_weights_count(kind):
     """one position far above thousands that share the rest of the weight"""
     D, T = 64, 4096
@@ -460,6 +472,10 @@ def test_python_refusals():
             cache.attention(q[:, :, :3], pos)
         with pytest.raises(qa.QphError, match="negative"):
             cache.attention(q, pos, window=-1)
+        with pytest.raises(qa.QphError, match="scale"):
+            cache.attention(q, pos, scale=1e-60)   # 0 as a float, which means the default
+        with pytest.raises(qa.QphError, match="overlap"):
+            cache.read(pos, 3, out=(k, k))
         with pytest.raises(qa.QphError, match="overlap"):
             cache.attention(q, pos, out=torch.zeros(1, 3, 4, 64, device="cuda", dtype=F16).expand(2, 3, 4, 64))
         cache.write(k[:, :0], k[:, :0], pos)

@@ -74,6 +74,23 @@ def test_other_refusals():
     refused(lib().qph_kv_bytes(qa.QPH_Q4, 1, 1, 64, 1, None), "bytes is NULL")
 
 
+def test_rows_that_would_be_written_twice_are_refused():
+    """each stride alone is long enough, two of them together are not; nested in any order they are"""
+    for r in (rows(tok=64, head=64), rows(tok=128, head=64), rows(seq=64 * 11, tok=64 * 4, head=64), rows(seq=64, tok=128, head=320), rows(seq=1 << 62, tok=1 << 62, head=64)):
+        refused(attend(out=r), "overlap")
+    for r in (rows(tok=64, head=192), rows(seq=64, tok=128, head=384), rows(seq=1 << 62, tok=256, head=64)):
+        refused(attend(out=r, scale=-1.0), "scale")   # taken: the next check is what refuses
+    refused(write(cache(), v=rows(p=P), f="qph_kv_read"), "k and v overlap")
+    refused(write(cache(kind=qa.QPH_F16)), "k and v overlap")
+
+
+def test_sizes_past_a_launch_are_refused():
+    wide = cache(kind=qa.QPH_F16, nseq=1, kv_heads=4096, head_dim=128, v=2 * P)
+    far = rows(p=4 * P, seq=0, tok=0, head=0)
+    refused(write(wide, k=far, v=far, n=32769), "2^34")
+    refused(attend(scale=3e38), "scale")
+
+
 def test_no_tokens_is_no_call():
     assert write(cache(), n=0) == 0 and write(cache(), n=0, f="qph_kv_read") == 0 and attend(n=0) == 0
 
