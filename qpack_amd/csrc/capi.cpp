@@ -99,7 +99,7 @@ static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sink
   if (heads < 1 || heads % c->kv_heads) throw std::invalid_argument("kv: heads must be a positive multiple of kv_heads");
   if (n < 0 || n > 1 << 20 || (int64_t)n * (heads / c->kv_heads) > 1 << 23 || heads > 65535) throw std::invalid_argument("kv: n must be in [0, 2^20], heads <= 65535 and n * heads / kv_heads <= 2^23");
   if (window < 0 || sinks < 0) throw std::invalid_argument("kv: window and sinks must not be negative");
-  a.cache = c->k; a.cache_v = c->v; a.ctx = c->ctx; a.nrec = qph::kv4_records(c->ctx);
+  a.kind = kv_kind(c); a.cache = c->k; a.cache_v = c->v; a.ctx = c->ctx; a.nrec = qph::kv4_records(c->ctx);
   a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.heads = heads; a.rep = heads / c->kv_heads; a.n = n;
   a.window = window; a.sinks = sinks;
 }
@@ -461,7 +461,7 @@ int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, in
       const int64_t bytes = (int64_t)qph::kv_attn_plan(a);
       if (bytes && (!work || work_bytes < bytes || (uintptr_t)work % 16)) throw std::invalid_argument("kv: work must have the " + std::to_string(bytes) + " bytes that qph_kv_attention_work gives, 16-byte aligned");
       a.part = (float *)work;
-      hck(qph::launch_kv_attn(kv_kind(c), a, (hipStream_t)stream), "kv attention");
+      hck(qph::launch_kv_attn(a, (hipStream_t)stream), "kv attention");
     }
   });
 }

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "launch.hpp"
 
@@ -131,9 +132,18 @@ __device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits) {
   return float_to_half_bits(bf16_to_f(f_to_bf16(a / 7.f)));
 }
 // clamp(rint(x / s), -7, 7) + 8, ties to even, of the real quotient: the product with 1 / s is off by one step at most, and
-// only next to a border; e = x - r s is exact (r s has 11 bits, e is a multiple of x's last place below 2^24 of them)
+// only next to a border; e = x - r s is exact (r s has 11 bits, e is a multiple of x's last place below 2^24 of them).
+// 16-bit rows: x has 11 bits at most and s 8, so x / s is a border (half an odd number) or 2^-12 away from all of them.  Rounded to a
+// multiple of 2^-16 first (by adding 192), the product, which is off by less than 2^-20, is on the right side or on the border itself; a
+// second sum rounds it to a whole number in the float's low bits.  Four instructions for fifteen: 2048
+// positions of 8 heads of 128 dims 7.1 -> 4.5 us
+template <int T>
 __device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
-  const float y = fminf(fmaxf(x, -7.f * s), 7.f * s);
+  const float y = __builtin_amdgcn_fmed3f(x, -7.f * s, 7.f * s);
+  if constexpr (T != RT_F32) {
+    const float t = __builtin_fmaf(y, inv, 192.f) + (12582912.f + 8.f - 192.f);
+    return __builtin_bit_cast(uint32_t, t) & 15;
+  }
   float r = __builtin_rintf(y * inv);
   const float e = 2.f * __builtin_fmaf(-r, s, y);
   const bool odd = ((int)r & 1) != 0;
@@ -145,7 +155,7 @@ __device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
 // One wave per record's K, one per its V: lane = position lane / 8 of the record, dims EL (lane % 8) ..  Positions outside the
 // call's keep their codes and scales: their K rows and scales are not stored, and the V words, which hold all 8
 // positions, are read and merged where the call covers a part only (no other workgroup of the launch has the record).
-// Bound by memory for prompts and by latency for single tokens.
+// 2048 positions of 8 heads of 128 dims, fp16 rows: 4.5 us for 10.7 MB, of which 2.4 are the launch.
 template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   constexpr int EL = HD / 8, GL = 32 / EL;   // elements of a lane; lanes of a group
@@ -175,7 +185,7 @@ __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   if (s > 0.f) {
     const float inv = 1.f / s;
 #pragma unroll
-    for (int i = 0; i < EL; i++) c[i] = mine ? code_of(x[i], s, inv) : 8;
+    for (int i = 0; i < EL; i++) c[i] = mine ? code_of<T>(x[i], s, inv) : 8;
   } else {
 #pragma unroll
     for (int i = 0; i < EL; i++) c[i] = 8;
@@ -219,7 +229,7 @@ __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
 
 // One token a sequence: a wave has one row of K or V, HD / 64 dims a lane.  Lanes of a K word meet by DPP; a V word is read (as soon as
 // the position is known, beside the row) and its one code replaced.  In k_kv4_write such a row would keep 8 lanes of 64 busy: 4.9 us
-// against 3.4 for 8 heads of 128 dims, of which 2.4 are the launch
+// against 2.9 for 8 heads of 128 dims, of which 2.4 are the launch (bound by latency: position, word, store)
 template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_write1(KvIoArgs a) {
   constexpr int EL = HD / 64;
@@ -261,7 +271,7 @@ __global__ __launch_bounds__(128) void k_kv4_write1(KvIoArgs a) {
   const float s = half_bits_to_float(sb), inv = 1.f / s;
   uint32_t c[EL];
 #pragma unroll
-  for (int i = 0; i < EL; i++) c[i] = s > 0.f ? code_of(x[i], s, inv) : 8;
+  for (int i = 0; i < EL; i++) c[i] = s > 0.f ? code_of<T>(x[i], s, inv) : 8;
   if (vside) {
     const int sh = 16 * (row & 1) + 4 * (row >> 1);
 #pragma unroll
@@ -279,6 +289,8 @@ __global__ __launch_bounds__(128) void k_kv4_write1(KvIoArgs a) {
   if (lane % (32 / EL) == 0) *(uint16_t *)(o + 8 * HD + 2 * (row * (HD / 32) + lane / (32 / EL))) = sb;
 }
 
+// The same lanes as k_kv4_write's.  A lane takes its position's code out of each of its dims' V words, which 8 lanes read from L1: 4.7 us for
+// 2048 positions of 8 heads of 128 dims, 2.4 of them the launch (single tokens 2.8)
 template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
   constexpr int EL = HD / 8, GL = 32 / EL;
@@ -312,7 +324,7 @@ __global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
   store_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x);
 }
 
-// the fp16 cache's: a copy with a conversion, 8 dims of one position's K and V a thread
+// the fp16 cache's: a copy with a conversion, 8 dims of one position's K or V a thread.  Bound by memory, or by the launch
 template <bool WRITE, int T>
 __global__ __launch_bounds__(256) void k_kv16_io(KvIoArgs a) {
   const int b = blockIdx.z, per = a.nkv * a.hd / 8;
@@ -788,6 +800,38 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
   store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, r);
 }
 
+// The same with a row on HD / 4 lanes and 256 / (HD / 4) rows a workgroup, each thread over all splits in order: for many rows, where a
+// workgroup each would come in rounds of 4 us (2048 at a time)
+template <int HD, int T>
+__global__ __launch_bounds__(256) void k_kv_merge_rows(KvAttnArgs a) {
+  constexpr int CT = HD / 4;
+  const int b = blockIdx.z, ct = threadIdx.x % CT, i = blockIdx.x * (256 / CT) + threadIdx.x / CT;
+  if (i >= a.n * a.heads) return;
+  const int tok = i / a.heads, head = i - tok * a.heads, g = token_of(a, head), col = tok * a.rep + head - g * a.rep;
+  const Span s = span_of(a, b, chunk_of(a, col));
+  if (!s.any || s.S == 1 || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
+  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.nsplit * HD) + row * a.nsplit;
+  const float *po = a.part + row * a.nsplit * HD + 4 * ct;
+  float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < s.S; k++) M = fmaxf(M, ml[k].x);
+  const float Mz = M == -INFINITY ? 0.f : M;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int k = 0; k < s.S; k++) {
+    const float2 x = ml[k];
+    const float w = __builtin_amdgcn_exp2f(x.x - Mz);
+    L += x.y * w;
+    y += *(const f32x4 *)(po + (int64_t)k * HD) * w;
+  }
+  const float inv = 1.f / L;
+  float o[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) o[k] = y[k] * inv;
+  store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, o);
+}
+
 // ------------------------------------------------------------------ many tokens
 // 8 waves of 32 columns; the workgroup's 256 columns share blocks of 64 positions (8 records) in LDS, three buffers: while
 // one is computed, the block after next is expanded, and the codes of the one behind that are on their way to registers.
@@ -1186,8 +1230,19 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   const int cus = 256;
   const bool two = a.q.type == RT_F32;
   const int64_t cols = (int64_t)a.n * a.rep;
-  a.many = cols > 64;
-  a.cols = a.many ? kManyCols : two ? 8 : 16;
+  const int few = two ? 8 : 16;
+  // positions that a workgroup of c columns can have to read, at most
+  auto reach = [&](int c) { return a.window > 0 ? std::min<int64_t>(a.ctx, (int64_t)a.window + a.sinks + (c + a.rep - 1) / a.rep + 3 * kRec) : a.ctx; };
+  // k_kv_few's time goes with its chunks of 8 or 16 columns times the positions, each chunk reading them anew; k_kv_many's with the positions
+  // alone up to 256 columns, and it takes some 6 us longer to start.  Chunks up to which the first is faster, from both kernels' times at
+  // 12 to 640 columns, 1 and 8 sequences of 256 to 16384 positions, 8 kv heads of 128 dims (472 calls; the rule's choice is 1 % slower
+  // than the better kernel's in the mean, a limit of 64 columns was 19 %).  4-bit: 64 columns over 8 x 4096 positions 36 us few, 37
+  // many; 128 over 8 x 16384 176 and 112; 128 over 8 x 1024 18 and 35.  fp16: the same 92 and 38, 624 and 133, 44 and 31
+  const int64_t chunks = (cols + few - 1) / few, positions = (int64_t)a.nseq * a.nkv * reach(few);
+  const int64_t most = a.kind == MK_Q4 ? 4 + (384 << 10) / positions : 1 + (192 << 10) / positions;
+  const char *limit = getenv("QPH_KV_FEW");   // test hook: columns up to which k_kv_few is taken
+  a.many = (limit && *limit ? cols > atoi(limit) : chunks > std::min<int64_t>(most, 128)) || chunks * a.nkv > 65535;   // (the last: the grid)
+  a.cols = a.many ? kManyCols : few;
   a.half_log2 = a.many ? 7 : two ? 2 : 3;
   a.tile_log2 = a.many ? 3 : 2;   // records of a tile
   a.min_log2 = a.many ? 2 : 3;    // tiles of a split, at least
@@ -1199,9 +1254,7 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   a.rep_mul = a.rep == 1 ? 0 : (uint32_t)(((1ull << (32 + a.rep_shift)) + a.rep - 1) / a.rep);
   a.nchunk = (int)((cols + a.cols - 1) / a.cols);
   a.paired = a.many && a.window == 0;
-  // positions that a workgroup can have to read, at most
-  const int64_t reach = a.window > 0 ? std::min<int64_t>(a.ctx, (int64_t)a.window + a.sinks + (a.cols + a.rep - 1) / a.rep + 3 * kRec) : a.ctx;
-  const int64_t tiles = (reach + tile - 1) / tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
+  const int64_t tiles = (reach(a.cols) + tile - 1) / tile, groups = (int64_t)a.nkv * a.nchunk * a.nseq;
   const int64_t want = (a.many ? 1 : 2) * (int64_t)cus / std::max<int64_t>(groups, 1);
   a.nsplit = tiles <= a.one_tiles ? 1 : (int)std::max<int64_t>(1, std::min({want, (tiles >> a.min_log2) + 1, (int64_t)64}));
   if (a.n > 65535 || a.nchunk * a.nsplit > 65535) a.nsplit = 1;   // grid limits
@@ -1212,19 +1265,22 @@ template <int HD, int T> static constexpr auto k_few4 = k_kv_few<HD, MK_Q4, T>;
 template <int HD, int T> static constexpr auto k_few16 = k_kv_few<HD, MK_F32, T>;
 template <int HD, int T> static constexpr auto k_many4 = k_kv_many<HD, MK_Q4, T>;
 template <int HD, int T> static constexpr auto k_many16 = k_kv_many<HD, MK_F32, T>;
-hipError_t launch_kv_attn(int kind, const KvAttnArgs &a, hipStream_t st) {
+// rows from which the splits are merged by k_kv_merge_rows: at 2048 the two are even, 6144 rows 44 -> 39 us with the attention, 16384 50 -> 34
+constexpr int kMergeRows = 4096;
+hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st) {
   if (a.many) {
     const dim3 grid(a.nkv, a.nchunk * a.nsplit, a.nseq);
-    if (kind == MK_Q4) QPH_KV(k_many4, a.hd, a.q.type, grid, kManyWaves * 64, a);
+    if (a.kind == MK_Q4) QPH_KV(k_many4, a.hd, a.q.type, grid, kManyWaves * 64, a);
     else QPH_KV(k_many16, a.hd, a.q.type, grid, kManyWaves * 64, a);
   } else {
     const dim3 grid(a.nsplit, a.nkv * a.nchunk, a.nseq);
-    if (kind == MK_Q4) QPH_KV(k_few4, a.hd, a.q.type, grid, kFewWaves * 64, a);
+    if (a.kind == MK_Q4) QPH_KV(k_few4, a.hd, a.q.type, grid, kFewWaves * 64, a);
     else QPH_KV(k_few16, a.hd, a.q.type, grid, kFewWaves * 64, a);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nsplit == 1) return e;
-  QPH_KV(k_kv_merge, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a);
+  if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows) QPH_KV(k_kv_merge_rows, a.hd, a.q.type, dim3((a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd), 1, a.nseq), 256, a);   // (at most 32768 rows a sequence: groups <= 256)
+  else QPH_KV(k_kv_merge, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a);
   return hipGetLastError();
 }
 

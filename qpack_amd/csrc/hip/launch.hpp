@@ -312,6 +312,7 @@ hipError_t launch_kv_read(int kind, const KvIoArgs &a, hipStream_t st);
 // tokens 0 .. of sequence b at positions pos[b] .., whose rows are in the cache, over positions p <= P with p > P - window
 // (window > 0) or p < sinks
 struct KvAttnArgs {
+  int kind;                     // of the cache
   const void *cache, *cache_v;
   int64_t cseq, crow, ctx, nrec;
   int nseq, nkv, hd, heads, rep, n;
@@ -326,7 +327,7 @@ struct KvAttnArgs {
 };
 // how the call is laid out; the bytes of part
 size_t kv_attn_plan(KvAttnArgs &a);
-hipError_t launch_kv_attn(int kind, const KvAttnArgs &a, hipStream_t st);
+hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st);
 
 // ---- reference-order mode (exact.hip): the reference CPU path's float orders, bit-identical results
 // RMSNorm of `rows` vectors [ldx] with the sequential sum of squares, out [ldo]

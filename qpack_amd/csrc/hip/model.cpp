@@ -301,6 +301,7 @@ KvIoArgs HipLlama::kv_io(int l, float *k, float *v, int n) const {   // k / v: r
 }
 KvAttnArgs HipLlama::kv_attn(int l, const float *q, float *out, int n) const {
   KvAttnArgs a{};
+  a.kind = kv_kind_;
   if (kv_kind_ == MK_Q4) a.cache = kv4_ + (size_t)l * kv4_layer_;
   else { a.cache = kc_ + (size_t)l * ctx_ * kvd_; a.cache_v = vc_ + (size_t)l * ctx_ * kvd_; }
   a.crow = kvd_; a.ctx = ctx_; a.nrec = kv4_records(ctx_);
@@ -315,7 +316,7 @@ void HipLlama::kv_append(int l, float *k, float *v, int n) { QPH_CK(launch_kv_wr
 void HipLlama::kv_attend(int l, const float *q, float *out, int n) {
   KvAttnArgs a = kv_attn(l, q, out, n);
   if (kv_attn_plan(a) > kv_part_bytes_) throw std::runtime_error("hip: attention scratch too small");
-  QPH_CK(launch_kv_attn(kv_kind_, a, st_));
+  QPH_CK(launch_kv_attn(a, st_));
 }
 // scratch for every number of tokens that a call can have
 void HipLlama::kv_buffers() {

@@ -31,6 +31,13 @@ def held(x):
     return torch.where(torch.isfinite(a), c * s, math.nan).flatten(-2)
 
 
+@pytest.fixture(params=["", "0", "100000"], ids=["auto", "many", "few"])
+def route(request, monkeypatch):
+    """the call's own choice of kernel, and each of the two"""
+    if request.param:
+        monkeypatch.setenv("QPH_KV_FEW", request.param)
+
+
 def i32(v):
     return torch.tensor(v, dtype=torch.int32, device="cuda")
 
@@ -155,6 +162,34 @@ def test_q4_border_values():
     assert torch.equal(torch.nan_to_num(k2, nan=123.), torch.nan_to_num(k, nan=123.))
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_q4_16_bit_rows_next_to_every_border(type):
+    """every scale of 8 bits at a few sizes, the values of the type on and around the borders (k + 1/2) s, both signs"""
+    t = TYPES[type]
+    rows = []
+    for e in (-22, -14, -7, 0, 5):
+        for j in range(128, 256):
+            s = j * 2.0 ** e
+            edge = torch.tensor([(k + 0.5) * s for k in range(7)]).to(t)
+            bits = edge.view(torch.int16)
+            near = torch.cat([(bits + d).view(t).float() for d in (-1, 0, 1)])   # 21 values and their negatives
+            g = torch.zeros(64)
+            g[0] = g[32] = 7 * s
+            g[1:22], g[33:54] = near, -near
+            rows.append(g)
+    x = torch.stack(rows).to(t).view(1, -1, 1, 64)
+    n = x.shape[1]
+    c = qa.KvCache("q4", 1, 1, 64, n)
+    c.write(x.cuda(), x.flip(-1).contiguous().cuda(), i32([0]))
+    k, v = c.read(i32([0]), n, dtype=F32)
+    assert torch.equal(k.cpu(), held(x).float()) and torch.equal(v.cpu(), held(x.flip(-1)).float())
+    for p in range(0, n, 37):   # the single token's kernel
+        c.write(x[:, p:p + 1].cuda() * 0, x[:, p:p + 1].cuda() * 0, i32([p]))
+        c.write(x[:, p:p + 1].cuda(), x.flip(-1)[:, p:p + 1].contiguous().cuda(), i32([p]))
+    again = c.read(i32([0]), n, dtype=F32)
+    assert torch.equal(again[0], k) and torch.equal(again[1], v)
+
+
 @pytest.mark.parametrize("kind", ["q4", "f16"])
 def test_write_read_strides_limits_and_absent_sequences(kind):
     gen = torch.Generator().manual_seed(9)
@@ -202,7 +237,7 @@ CASES = [   # kind, hd, kv heads, rep, n, pasts, window, sinks
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("kind,hd,G,rep,n,pasts,window,sinks", CASES)
-def test_attention(kind, hd, G, rep, n, pasts, window, sinks, type):
+def test_attention(kind, hd, G, rep, n, pasts, window, sinks, type, route):
     print(f"attention {kind} hd {hd} kv heads {G} rep {rep} n {n} pasts {pasts} window {window} sinks {sinks} {type}", flush=True)
     gen = torch.Generator().manual_seed(n + sum(pasts))
     S, ctx = len(pasts), max(pasts) + n + 5
@@ -215,7 +250,7 @@ def test_attention(kind, hd, G, rep, n, pasts, window, sinks, type):
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
 @pytest.mark.parametrize("n", [1, 3, 40])
-def test_attention_unseen_memory_may_hold_anything(kind, n):
+def test_attention_unseen_memory_may_hold_anything(kind, n, route):
     """NaN and infinities in unwritten positions, behind the last token, and before the window change nothing"""
     gen = torch.Generator().manual_seed(4)
     G, rep, D, past, window, sinks = 2, 4, 128, 150, 60, 3
@@ -233,7 +268,7 @@ def test_attention_unseen_memory_may_hold_anything(kind, n):
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
 @pytest.mark.parametrize("n,rep,where", [(4, 4, 2), (5, 3, 4), (40, 4, 17), (100, 1, 99)])
-def test_attention_nan_rows_stay_with_those_who_see_them(kind, n, rep, where):
+def test_attention_nan_rows_stay_with_those_who_see_them(kind, n, rep, where, route):
     """a NaN in one token's V row, an infinity in another's K: earlier tokens don't see them, the window's later ones no more"""
     gen = torch.Generator().manual_seed(6)
     G, D, past, window = 1, 64, 30, 12
@@ -256,7 +291,7 @@ def test_attention_nan_rows_stay_with_those_who_see_them(kind, n, rep, where):
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
 @pytest.mark.parametrize("n", [1, 33])
-def test_attention_strides_ragged_absent_and_in_place(kind, n):
+def test_attention_strides_ragged_absent_and_in_place(kind, n, route):
     gen = torch.Generator().manual_seed(8)
     S, G, rep, D = 5, 2, 4, 64
     pasts, lens, ctx = [100, 7, -1, 40, 300 - n // 2], [n, max(1, n // 2), n, 0, n], 300
@@ -279,7 +314,7 @@ def test_attention_strides_ragged_absent_and_in_place(kind, n):
 
 
 @pytest.mark.parametrize("type,size", [("f32", 1e-6), ("f32", 3e4), ("bf16", 1e-30), ("bf16", 1e4), ("f16", 6e-8)])
-def test_attention_query_range(type, size):
+def test_attention_query_range(type, size, route):
     """rows far from 1, with the softmax scale that brings the scores back"""
     gen = torch.Generator().manual_seed(2)
     c, K, V = filled("q4", 1, 1, 128, 200, [200], gen)
@@ -291,7 +326,7 @@ def test_attention_query_range(type, size):
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
 @pytest.mark.parametrize("type", ["f32", "bf16"])
-def test_attention_vanishing_scores(kind, type):
+def test_attention_vanishing_scores(kind, type, route):
     """the scale times a row's power is below fp32's range: the positions weigh alike, the masked ones nothing"""
     gen = torch.Generator().manual_seed(12)
     c, K, V = filled(kind, 1, 1, 64, 200, [200], gen)
@@ -302,7 +337,7 @@ def test_attention_vanishing_scores(kind, type):
 
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
-def test_attention_far_smaller_weights_count(kind):
+def test_attention_far_smaller_weights_count(kind, route):
     """one position far above thousands that share the rest of the weight"""
     D, T = 64, 4096
     k = torch.zeros(1, T, 1, D)
@@ -319,7 +354,7 @@ def test_attention_far_smaller_weights_count(kind):
     assert float(out[0, 0, 0, 1]) > 0.05
 
 
-def test_cache_past_32_bit_offsets():
+def test_cache_past_32_bit_offsets(route):
     """17M positions: record and row offsets past 2^31 bytes and elements"""
     G, D = 1, 128
     gen = torch.Generator().manual_seed(1)
@@ -338,7 +373,7 @@ def test_cache_past_32_bit_offsets():
 
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
-def test_captured_steps(kind):
+def test_captured_steps(kind, route):
     """write and attention in a graph, replayed at other positions, eager work between"""
     gen = torch.Generator().manual_seed(3)
     S, G, rep, D, ctx = 2, 2, 4, 128, 2100
@@ -377,7 +412,7 @@ def test_captured_steps(kind):
         assert torch.equal(eager, out)
 
 
-def test_scratch_is_not_read_before_it_is_written_and_results_repeat():
+def test_scratch_is_not_read_before_it_is_written_and_results_repeat(route):
     gen = torch.Generator().manual_seed(12)
     c, K, V = filled("q4", 1, 1, 128, 3000, [3000], gen)
     for n, rep in ((1, 4), (40, 4)):
@@ -400,7 +435,7 @@ def test_scratch_is_not_read_before_it_is_written_and_results_repeat():
         check_rows(outs[0][0], q[0], K[0], V[0], 3000 - n)
 
 
-def test_two_streams_at_once():
+def test_two_streams_at_once(route):
     gen = torch.Generator().manual_seed(13)
     c, K, V = filled("q4", 1, 2, 64, 1500, [1500], gen)
     q = [torch.randn(1, n, 8, 64, generator=gen).half().cuda() for n in (1, 24)]
@@ -419,7 +454,7 @@ def test_two_streams_at_once():
 
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
-def test_conversation(kind):
+def test_conversation(kind, route):
     """a prompt, steps, a turn of several tokens and steps over it, two sequences: as a server runs them"""
     gen = torch.Generator().manual_seed(21)
     S, G, rep, D, ctx, window, sinks = 2, 2, 4, 64, 400, 70, 4

@@ -112,8 +112,10 @@ def test_prompt_steps_and_greedy(cfg, kind, window, sinks, synth):
 
 
 @pytest.mark.parametrize("kind,window,sinks", [("q4", 0, 0), ("f16", 100, 4), ("q4", 150, 5)])
-def test_long_prompt_in_chunks(kind, window, sinks, synth, monkeypatch):
+@pytest.mark.parametrize("few", ["", "0"])
+def test_long_prompt_in_chunks(kind, window, sinks, few, synth, monkeypatch):
     path = synth("mini")
+    monkeypatch.setenv("QPH_KV_FEW", few)   # 0: every call through the many-token kernel
     toks = np.random.default_rng(6).integers(0, 1000, 700).astype(np.int32)
     want = Plain(path).logits(toks, kind, window, sinks)
     for chunk in (0, 97):
