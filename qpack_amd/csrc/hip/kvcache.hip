@@ -432,6 +432,12 @@ constexpr float kTinyF = 0x1p-126f;
 //           position 8 (r / 4) + 4 mt + r % 4, so the C layout leaves lane group lg = lane / 16 the 8 positions of record lg.
 //   values  O^T[d][c] += V^T[d][p] P^T[p][c]: those 8 probabilities are the lane's B fragment as they are, and the A
 //           fragment is dim 16 t + lane % 16 of record lg: one word of V codes.
+// Why 16 columns and, for 4-bit, no LDS: the heads of a kv group leave much of a product's columns empty, but the cache is read once for
+// all of them, and that is what the time goes with: a batch of 32 sequences of up to 8K positions (8 kv heads of 128 dims, 4 heads
+// each) 43 us, 4.85 TB/s where a large copy reaches 4.99.  One sequence of 16K is latency (position, first codes, a tile a wave, the
+// waves' sums): 6.4 us for 1.9 of bytes.  fp16 V goes through LDS, since the product wants it transposed.
+// Splits (kv_attn_plan): up to 1024 positions a sequence is one workgroup's, whose waves meet in LDS, since the merge is a launch of 3.9 us
+// (332 positions: 9.4 -> 5.7 us); above, two workgroups a CU, of at least 256 positions each.  A window makes them fewer alike
 // TWO (fp32 queries): 8 columns, with the queries' hi halves in columns 0 .. 7 and their lo halves in 8 .. 15 of the same
 // product, and P's likewise: 22 bits for the price of 11 where no more than 8 columns are needed.
 constexpr int kFewWaves = 8, kFewTile = 32, kFewOcc = 4;   // waves of a workgroup, positions of a tile, waves of a SIMD
@@ -768,7 +774,8 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
 }
 
 // The splits' sums of one row a workgroup: 256 threads, HD / 4 of them side by side over the dims, the others over the
-// splits.  M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L
+// splits.  M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L.  Bound by latency: 3.9 us for 28 rows of 64 splits, 2.4 of them the
+// launch.  (All loads asked for before M is known: no faster)
 template <int HD, int T>
 __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
   constexpr int CT = HD / 4, SL = 256 / CT;
@@ -841,6 +848,12 @@ __global__ __launch_bounds__(256) void k_kv_merge_rows(KvAttnArgs a) {
 //   values  O^T[d][c] += V^T[d][p] P^T[p][c]: 4-bit: V^T lies in LDS as the words expand, 8 positions of a dim together, one
 //           16-byte read a fragment; fp16: V lies as stored and two transpose reads fetch one.
 // TWO (fp32 queries): hi and lo halves of the queries and probabilities as products of their own.
+// A step of 64 positions takes a wave 32 products (1024 cycles of its SIMD's matrix core, two waves a SIMD), some 130 vector instructions and,
+// for 4-bit, 60 that expand; the 8 waves read 256 KiB of LDS, 2048 cycles at its 128 bytes a cycle.  The three overlap in part only:
+// 2048 tokens of 32 heads over a 4-bit cache 56 to 64 us by box (620 TFLOP/s of the 1149 that a large fp16 product reaches), 4096
+// tokens with a window of 1024 in fp16 95 to 102 us.  256 columns a workgroup, since what a block costs to expand and its LDS writes are
+// shared by them: with 128 columns and two workgroups a CU the 4-bit prompt took 77 us for 64, the fp16 one 97 for 100, and 64
+// tokens each of 32 sequences 6 % more
 constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
 
 template <int HD, int KIND, int T>

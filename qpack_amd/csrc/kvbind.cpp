@@ -1,6 +1,7 @@
 // The Python side of the kv entry points (qpack_amd._kvbind, used by qpack_amd/kvcache.py): reads tensors through their Python
 // attributes, checks them and calls the C ABI.  A step's kernels take 3 to 8 us each; the same checks through ctypes took 10 us a call
-// (15 with scratch), this takes about 3.  CPython's API alone: no torch headers, no torch library.
+// (15 with scratch), this takes 4.5 (8.5 with scratch and a second launch), of which each launch is about 3.  CPython's API alone: no torch
+// headers, no torch library.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
