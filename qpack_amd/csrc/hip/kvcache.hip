@@ -155,7 +155,7 @@ __device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
 // One wave per record's K, one per its V: lane = position lane / 8 of the record, dims EL (lane % 8) ..  Positions outside the
 // call's keep their codes and scales: their K rows and scales are not stored, and the V words, which hold all 8
 // positions, are read and merged where the call covers a part only (no other workgroup of the launch has the record).
-// 2048 positions of 8 heads of 128 dims, fp16 rows: 4.5 us for 10.7 MB, of which 2.4 are the launch.
+// 2048 positions of 8 heads of 128 dims, fp16 rows: 4.5 us, a launch (2.4) and 10.8 MB at the copy rate (2.2).
 template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   constexpr int EL = HD / 8, GL = 32 / EL;   // elements of a lane; lanes of a group
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(128) void k_kv4_write1(KvIoArgs a) {
 }
 
 // The same lanes as k_kv4_write's.  A lane takes its position's code out of each of its dims' V words, which 8 lanes read from L1: 4.7 us for
-// 2048 positions of 8 heads of 128 dims, 2.4 of them the launch (single tokens 2.8)
+// 2048 positions of 8 heads of 128 dims, a launch and 10.8 MB at the copy rate (single tokens 2.8)
 template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
   constexpr int EL = HD / 8, GL = 32 / EL;

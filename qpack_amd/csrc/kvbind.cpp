@@ -1,9 +1,9 @@
-// The Python side of the kv entry points (qpack_amd._kvbind, used by qpack_amd/kvcache.py): reads tensors through their Python
-// attributes, checks them and calls the C ABI.  A step's kernels take 3 to 8 us each; the same checks through ctypes took 10 us a call
-// (15 with scratch), this takes 4.5 (8.5 with scratch and a second launch), of which each launch is about 3.  CPython's API alone: no torch
-// headers, no torch library.
+// The Python side of the kv entry points (qpack_amd._kvbind, used by qpack_amd/kvcache.py): checks tensors and calls the C ABI.  A step's
+// kernels take 3 to 8 us each; the checks through ctypes took 10 us a call (15 with scratch), through the tensors' Python attributes
+// 4.5 (8.5 with scratch and a second launch), from torch's own structures 3.5 (7.7); each launch is about 3 of it.
+// torch is loaded before this module is.
 #define PY_SSIZE_T_CLEAN
-#include <Python.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
 #include <cstring>
@@ -12,8 +12,8 @@
 #include "../../include/qpack_hip.h"
 
 namespace {
-PyObject *g_error, *g_f32, *g_f16, *g_bf16, *g_i32, *g_stream, *g_device, *g_guard;   // QphError, dtypes, functions
-PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_is_contiguous, *s_new_empty;
+PyObject *g_error, *g_stream, *g_device, *g_guard;   // QphError, functions
+PyObject *s_new_empty;
 
 struct Ref {   // owned reference
   PyObject *p;
@@ -35,67 +35,44 @@ bool fail(const char *fmt, const char *a, const char *b = "") {
   PyErr_Format(g_error, fmt, a, b);
   return false;
 }
-bool ints(PyObject *t, int64_t *out, int n) {   // a tuple of n integers
-  if (!t || !PyTuple_Check(t) || PyTuple_GET_SIZE(t) != n) return false;
-  for (int i = 0; i < n; i++) out[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(t, i));
-  return !PyErr_Occurred();
-}
-bool address(PyObject *x, void **p) {
-  Ref v(PyObject_CallMethodNoArgs(x, s_data_ptr));
-  if (!v.p) return false;
-  *p = PyLong_AsVoidPtr(v);
-  return !PyErr_Occurred();
-}
-bool device_of(PyObject *x, int64_t *d) {
-  Ref v(PyObject_CallMethodNoArgs(x, s_get_device));
-  if (!v.p) return false;
-  *d = PyLong_AsLongLong(v);
-  return !PyErr_Occurred();
-}
-bool on_device(const Cache *c, PyObject *x, const char *name) {
-  int64_t d;
-  if (!device_of(x, &d)) return false;
-  return d == c->device || fail("kv: %s is not on the cache's device%s", name);
+bool tensor(const Cache *c, PyObject *x, const char *name, const at::Tensor **t) {   // on the cache's device
+  if (!THPVariable_Check(x)) return fail("kv: %s must be a tensor%s", name);
+  *t = &THPVariable_Unpack(x);
+  if (!(*t)->is_cuda() || (*t)->get_device() != c->device) return fail("kv: %s is not on the cache's device%s", name);
+  return true;
 }
 // a tensor [nseq, n, heads, head_dim] with consecutive dims
-bool rows(const Cache *c, PyObject *x, const char *name, qph_rows *r, int64_t *n, int64_t *heads) {
-  Ref t(PyObject_GetAttr(x, s_dtype));
-  if (!t.p) return false;
-  if (t.p == g_f32) r->type = QPH_F32;
-  else if (t.p == g_f16) r->type = QPH_F16;
-  else if (t.p == g_bf16) r->type = QPH_BF16;
-  else return fail("kv: %s must be float32, float16 or bfloat16%s", name);
-  if (!on_device(c, x, name)) return false;
-  int64_t s[4], st[4];
-  Ref shape(PyObject_GetAttr(x, s_shape)), stride(PyObject_CallMethodNoArgs(x, s_stride));
-  if (!shape.p || !stride.p) return false;
-  if (!ints(shape, s, 4) || !ints(stride, st, 4) || s[0] != c->c.nseq || s[3] != c->c.head_dim) {
-    PyErr_Clear();
+bool rows(const Cache *c, PyObject *x, const char *name, qph_rows *r, int64_t *n, int64_t *heads) try {
+  const at::Tensor *t;
+  if (!tensor(c, x, name, &t)) return false;
+  switch (t->scalar_type()) {
+    case at::kFloat: r->type = QPH_F32; break;
+    case at::kHalf: r->type = QPH_F16; break;
+    case at::kBFloat16: r->type = QPH_BF16; break;
+    default: return fail("kv: %s must be float32, float16 or bfloat16%s", name);
+  }
+  if (t->layout() != at::kStrided || t->dim() != 4 || t->size(0) != c->c.nseq || t->size(3) != c->c.head_dim) {
     PyErr_Format(g_error, "kv: %s must be [%d, n, heads, %d]", name, c->c.nseq, c->c.head_dim);
     return false;
   }
-  if (st[3] != 1) return fail("kv: the last dimension of %s must be contiguous%s", name);
-  *n = s[1]; *heads = s[2];
-  r->seq = st[0]; r->tok = st[1]; r->head = st[2];
-  if (!address(x, &r->p)) return false;
+  if (t->stride(3) != 1) return fail("kv: the last dimension of %s must be contiguous%s", name);
+  *n = t->size(1); *heads = t->size(2);
+  r->seq = t->stride(0); r->tok = t->stride(1); r->head = t->stride(2);
+  r->p = t->data_ptr();
   if (*n == 0 && !r->p) r->p = (void *)16;   // a tensor without elements may have no memory: nothing of it is read
   return true;
-}
-bool index(const Cache *c, PyObject *x, const char *name, const int **p) {   // int32 [nseq]; None: NULL
+} catch (...) { return fail("kv: %s is not a plain tensor%s", name); }   // (nested or fake ones: torch throws)
+bool index(const Cache *c, PyObject *x, const char *name, const int **p) try {   // int32 [nseq]; None: NULL
   if (x == Py_None && !strcmp(name, "lens")) { *p = nullptr; return true; }
-  Ref t(PyObject_GetAttr(x, s_dtype)), shape(PyObject_GetAttr(x, s_shape)), con(PyObject_CallMethodNoArgs(x, s_is_contiguous));
-  if (!t.p || !shape.p || !con.p) return false;
-  int64_t s[1];
-  if (t.p != g_i32 || !ints(shape, s, 1) || s[0] != c->c.nseq || con.p != Py_True) {
-    PyErr_Clear();
+  const at::Tensor *t;
+  if (!tensor(c, x, name, &t)) return false;
+  if (t->scalar_type() != at::kInt || t->layout() != at::kStrided || t->dim() != 1 || t->size(0) != c->c.nseq || !t->is_contiguous()) {
     PyErr_Format(g_error, "kv: %s must be a contiguous int32 tensor [%d]", name, c->c.nseq);
     return false;
   }
-  void *q;
-  if (!on_device(c, x, name) || !address(x, &q)) return false;
-  *p = (const int *)q;
+  *p = (const int *)t->data_ptr();
   return true;
-}
+} catch (...) { return fail("kv: %s is not a plain tensor%s", name); }
 bool stream_of(const Cache *c, void **st) {
   Ref d(PyLong_FromLongLong(c->device));
   Ref v(PyObject_CallOneArg(g_stream, d));
@@ -176,7 +153,8 @@ PyObject *attention(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   if (!current(c, &here) || !stream_of(c, &st)) return nullptr;
   // scratch of this call alone: the allocator gives it to the stream's later work, or to the graph that is being captured
   Ref size(bytes ? PyLong_FromLongLong((bytes + c->item - 1) / c->item) : nullptr), work(bytes ? PyObject_CallMethodOneArg(c->data, s_new_empty, size) : nullptr);
-  if (bytes && (!work.p || !address(work, &w))) return nullptr;
+  if (bytes && !work.p) return nullptr;
+  if (bytes) w = THPVariable_Unpack(work.p).data_ptr();
   if (!launch(c, here, st, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, (float)scale, w, bytes, st); })) return nullptr;
   Py_RETURN_NONE;
 }
@@ -204,10 +182,10 @@ PyMethodDef cache_methods[] = {
     {nullptr, nullptr, 0, nullptr}};
 PyTypeObject cache_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
-// setup(QphError, float32, float16, bfloat16, int32, raw stream of a device, current device, device guard)
+// setup(QphError, raw stream of a device, current device, device guard)
 PyObject *setup(PyObject *, PyObject *args) {
-  if (!PyArg_ParseTuple(args, "OOOOOOOO", &g_error, &g_f32, &g_f16, &g_bf16, &g_i32, &g_stream, &g_device, &g_guard)) return nullptr;
-  for (PyObject *p : {g_error, g_f32, g_f16, g_bf16, g_i32, g_stream, g_device, g_guard}) Py_INCREF(p);
+  if (!PyArg_ParseTuple(args, "OOOO", &g_error, &g_stream, &g_device, &g_guard)) return nullptr;
+  for (PyObject *p : {g_error, g_stream, g_device, g_guard}) Py_INCREF(p);
   Py_RETURN_NONE;
 }
 PyMethodDef module_methods[] = {{"setup", setup, METH_VARARGS, "the names that the module uses of Python's side"}, {nullptr, nullptr, 0, nullptr}};
@@ -215,9 +193,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvbind", nullptr, -1, module_meth
 }  // namespace
 
 PyMODINIT_FUNC PyInit__kvbind(void) {
-  s_dtype = PyUnicode_InternFromString("dtype"); s_shape = PyUnicode_InternFromString("shape"); s_stride = PyUnicode_InternFromString("stride");
-  s_data_ptr = PyUnicode_InternFromString("data_ptr"); s_get_device = PyUnicode_InternFromString("get_device");
-  s_is_contiguous = PyUnicode_InternFromString("is_contiguous"); s_new_empty = PyUnicode_InternFromString("new_empty");
+  s_new_empty = PyUnicode_InternFromString("new_empty");
   cache_type.tp_name = "qpack_amd._kvbind.Cache";
   cache_type.tp_basicsize = sizeof(Cache);
   cache_type.tp_flags = Py_TPFLAGS_DEFAULT;

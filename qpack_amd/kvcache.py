@@ -11,14 +11,13 @@ _bind = None
 
 
 def _binding():
-    """the compiled half of this file (csrc/kvbind.cpp), told what it uses of torch"""
+    """the compiled half of this file (csrc/kvbind.cpp), told what it uses of torch's Python side"""
     global _bind
     if _bind is None:
         import torch
         lib()   # the library, with its message where it has not been built
         from . import _kvbind
-        _kvbind.setup(QphError, torch.float32, torch.float16, torch.bfloat16, torch.int32, torch._C._cuda_getCurrentRawStream, torch.cuda.current_device,
-                      torch.cuda.device)
+        _kvbind.setup(QphError, torch._C._cuda_getCurrentRawStream, torch.cuda.current_device, torch.cuda.device)
         _bind = _kvbind
     return _bind
 
@@ -74,8 +73,8 @@ class KvCache:
     def read(self, pos, n, dtype=None, lens=None, out=None):
         """(k, v) [nseq, n, kv_heads, head_dim]: what the cache holds, in dtype (float16 when None); into out = (k, v) where given.  Rows
         that take no part stay as they are in out, and are zero without it"""
-        import torch
         if out is None:
+            import torch
             shape = (self.nseq, int(n), self.kv_heads, self.head_dim)
             out = tuple(torch.zeros(shape, dtype=dtype or torch.float16, device=self.device) for _ in range(2))
         k, v = out

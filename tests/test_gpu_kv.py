@@ -492,6 +492,11 @@ def test_python_refusals():
             if words != "heads":
                 with pytest.raises(qa.QphError, match=words):
                     cache.attention(bad, pos, out=q)
+        for bad in (None, 3, torch.nested.nested_tensor([k[0], k[1]])):
+            with pytest.raises(qa.QphError, match="must be|plain"):
+                cache.write(bad, k, pos)
+            with pytest.raises(qa.QphError, match="must be|plain"):
+                cache.attention(q, bad)
         for bad in (pos.long(), pos[:1], pos.cpu(), i32([0, 0, 1, 1])[::2]):
             with pytest.raises(qa.QphError, match="pos|device"):
                 cache.attention(q, bad)
