@@ -290,6 +290,25 @@ def test_attention_nan_rows_stay_with_those_who_see_them(kind, n, rep, where, ro
 
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
+@pytest.mark.parametrize("hd,type", [(64, "f32"), (128, "f16"), (128, "bf16")])
+@pytest.mark.parametrize("S,n,G,rep,pasts,lens", [(4, 47, 1, 33, [1400, 30, -1, 1453], [47, 47, 47, 5]), (16, 8, 2, 16, [1100] * 14 + [40, -1], [8] * 12 + [3, 0, 8, 8])])
+def test_attention_many_split_rows(kind, hd, type, S, n, G, rep, pasts, lens, route):
+    """thousands of rows whose splits are merged, beside short and absent sequences; a head of them behind n's end is left alone"""
+    print(f"many split rows {kind} {hd} {type} S {S}", flush=True)
+    gen = torch.Generator().manual_seed(S)
+    ctx = max(pasts) + n
+    c, K, V = filled(kind, S, G, hd, ctx, [p + m if p >= 0 else 0 for p, m in zip(pasts, lens)], gen)
+    q = torch.randn(S, n, G * rep, hd, generator=gen).to(TYPES[type]).cuda()
+    out = torch.full_like(q, 55.)
+    c.attention(q, i32(pasts), lens=i32(lens), out=out)
+    for b in range(S):
+        m = lens[b] if pasts[b] >= 0 else 0
+        if m and (S == 4 or b % 5 == 0 or b > 11):
+            check_rows(out[b, :m], q[b, :m], K[b], V[b], pasts[b])
+        assert bool((out[b, m:] == 55).all())
+
+
+@pytest.mark.parametrize("kind", ["q4", "f16"])
 @pytest.mark.parametrize("n", [1, 33])
 def test_attention_strides_ragged_absent_and_in_place(kind, n, route):
     gen = torch.Generator().manual_seed(8)
@@ -410,6 +429,38 @@ def test_captured_steps(kind, route):
             check_rows(out[b], q[b], K[b], V[b], P)
         eager = c.attention(q, pos - 1)
         assert torch.equal(eager, out)
+
+
+def test_two_graphs_and_an_eager_call_at_once():
+    """each captured call has scratch of its own"""
+    gen = torch.Generator().manual_seed(31)
+    c, K, V = filled("q4", 2, 2, 128, 4000, [4000, 2600], gen)
+    qs = [torch.randn(2, n, 8, 128, generator=gen).half().cuda() for n in (1, 2, 40)]
+    pos = [i32([4000 - q.shape[1], 2600 - q.shape[1]]) for q in qs]
+    want = [c.attention(q, p) for q, p in zip(qs, pos)]
+    for q, p, w in zip(qs, pos, want):
+        for b in range(2):
+            check_rows(w[b], q[b], K[b], V[b], int(p[b]))
+    outs, graphs = [torch.empty_like(q) for q in qs], []
+    torch.cuda.synchronize()
+    for q, p, o in zip(qs, pos, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.attention(q, p, out=o)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        for o in outs:
+            o.fill_(9)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = c.attention(qs[1], pos[1])
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[1])
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
 
 
 def test_scratch_is_not_read_before_it_is_written_and_results_repeat(route):
