@@ -850,7 +850,7 @@ __global__ __launch_bounds__(256) void k_kv_merge_rows(KvAttnArgs a) {
 // TWO (fp32 queries): hi and lo halves of the queries and probabilities as products of their own.
 // A step of 64 positions takes a wave 32 products (1024 cycles of its SIMD's matrix core, two waves a SIMD), some 130 vector instructions and,
 // for 4-bit, 60 that expand; the 8 waves read 256 KiB of LDS, 2048 cycles at its 128 bytes a cycle.  The three overlap in part only:
-// 2048 tokens of 32 heads over a 4-bit cache 56 to 64 us by box (620 TFLOP/s of the 1149 that a large fp16 product reaches), 4096
+// 2048 tokens of 32 heads over a 4-bit cache 56 to 64 us by machine (620 TFLOP/s of the 1149 that a large fp16 product reaches), 4096
 // tokens with a window of 1024 in fp16 95 to 102 us.  256 columns a workgroup, since what a block costs to expand and its LDS writes are
 // shared by them: with 128 columns and two workgroups a CU the 4-bit prompt took 77 us for 64, the fp16 one 97 for 100, and 64
 // tokens each of 32 sequences 6 % more
