@@ -318,10 +318,14 @@ void HipLlama::kv_attend(int l, const float *q, float *out, int n) {
   if (kv_attn_plan(a) > kv_part_bytes_) throw std::runtime_error("hip: attention scratch too small");
   QPH_CK(launch_kv_attn(a, st_));
 }
-// scratch for every number of tokens that a call can have
-void HipLlama::kv_buffers() {
+// scratch for every number of tokens that a call can have, over a cache of this kind
+void HipLlama::kv_buffers(int kind) {
   size_t need = 0;
-  for (int n = 1; n <= std::max(1, pf_cap_); n++) { KvAttnArgs a = kv_attn(0, nullptr, nullptr, n); need = std::max(need, kv_attn_plan(a)); }
+  for (int n = 1; n <= std::max(1, pf_cap_); n++) {
+    KvAttnArgs a = kv_attn(0, nullptr, nullptr, n);
+    a.kind = kind;
+    need = std::max(need, kv_attn_plan(a));
+  }
   if (need > kv_part_bytes_) {
     float *p = (float *)dalloc(need);
     dfree(kv_part_);
@@ -345,7 +349,7 @@ void HipLlama::set_cache(int kind) {
       stage = (uint16_t *)dalloc(2 * row);
       if (!zero) { zero = (int *)dalloc(sizeof(int)); kv_zero_ = zero; QPH_CK(hipMemsetAsync(zero, 0, sizeof(int), st_)); }
       QPH_CK(hipMemsetAsync(rec, 0, layer * cfg_.layers, st_));
-      kv_buffers();
+      kv_buffers(kind);
     } catch (...) { dfree(rec); dfree(stage); throw; }
     drop_graphs();
     dfree(kc_); dfree(vc_);
@@ -357,6 +361,7 @@ void HipLlama::set_cache(int kind) {
     try {
       k = (uint16_t *)dalloc(bytes); v = (uint16_t *)dalloc(bytes);
       QPH_CK(hipMemsetAsync(k, 0, bytes, st_)); QPH_CK(hipMemsetAsync(v, 0, bytes, st_));
+      if (window_ > 0) kv_buffers(kind);
     } catch (...) { dfree(k); dfree(v); throw; }
     drop_graphs();
     dfree(kv4_); dfree(kv_stage_);
@@ -375,7 +380,7 @@ void HipLlama::set_window(int window, int sinks) {
   check_status();
   const int w = window_, s = sinks_;
   window_ = window; sinks_ = sinks;
-  try { if (kv_custom()) kv_buffers(); } catch (...) { window_ = w; sinks_ = s; throw; }
+  try { if (kv_custom()) kv_buffers(kv_kind_); } catch (...) { window_ = w; sinks_ = s; throw; }
   drop_graphs();
   build_graphs();
 }

@@ -104,7 +104,7 @@ class HipLlama {
   KvIoArgs kv_io(int l, float *k, float *v, int n) const;
   KvIoArgs stage_io(int l, int n) const;
   KvAttnArgs kv_attn(int l, const float *q, float *out, int n) const;
-  void kv_buffers();
+  void kv_buffers(int kind);
   void kv_append(int l, float *k, float *v, int n);
   void kv_attend(int l, const float *q, float *out, int n);
   // pinned host

@@ -42,8 +42,10 @@ class Plain:
                 x = np.frombuffer(blob(t["blob"]), np.float32).astype(np.float64)
             self.w[t["name"]] = torch.from_numpy(np.ascontiguousarray(x))
 
-    def logits(self, toks, kind="f16", window=0, sinks=0):
-        """[n, vocab]: every position's"""
+    def logits(self, toks, kind="f16", window=0, sinks=0, cache=None):
+        """[n, vocab]: every position's; cache: the (K, V) [n, kv_heads, head_dim] of each layer that the attention reads instead of the rounded
+        rows, which are to lie within half a step (4-bit; the scale's 2^-9 of 7 steps more) of them, fp16's rounding (2^-11) and 2e-3 for the
+        path's own error before it"""
         c, w, n = self.c, self.w, len(toks)
         H, G, D, eps = c["num_attention_heads"], c["num_key_value_heads"], c["head_dim"], c["rms_norm_eps"]
         norm = lambda x, g: x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * g   # noqa: E731
@@ -63,7 +65,14 @@ class Plain:
             y = norm(x, g("attn_norm"))
             q, k, v = (y @ g("w" + s).T + (g("b" + s) if c["qkv_bias"] else 0) for s in "qkv")
             q, k, v = rope(q.view(n, H, D)), rope(k.view(n, G, D)), v.view(n, G, D)
-            k, v = (held(k), held(v)) if kind == "q4" else (k.half().double(), v.half().double())
+            if cache is not None:
+                for mine, theirs in ((k, cache[i][0]), (v, cache[i][1])):
+                    step = mine.unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True) / 7 if kind == "q4" else torch.zeros(1)
+                    off = (theirs - mine).unflatten(-1, (-1, 32)).abs()
+                    assert bool((off <= step * (0.5 + 2.0 ** -6) + 2e-3).all()), f"layer {i}: a cached row is {float((off - step / 2).max()):.3g} past half a step"
+                k, v = cache[i]
+            else:
+                k, v = (held(k), held(v)) if kind == "q4" else (k.half().double(), v.half().double())
             a = torch.einsum("thd,shd->hts", q, k.repeat_interleave(H // G, 1)) / math.sqrt(D)
             a = torch.softmax(a.masked_fill(~seen, -math.inf), -1)
             x = x + torch.einsum("hts,shd->thd", a, v.repeat_interleave(H // G, 1)).reshape(n, H * D) @ g("wo").T
@@ -72,6 +81,13 @@ class Plain:
             x = x + (u * torch.sigmoid(u) * (y @ g("w_up").T)) @ g("w_down").T
         head = w["embed"] if c["tie_embeddings"] else w["lm_head"]
         return (norm(x, w["final_norm"]) @ head.T).numpy()
+
+
+def cached(m, ref):
+    """the model's cache as its snapshot gives it"""
+    raw, L, G, D = bytes(m.snapshot()), ref.c["num_hidden_layers"], ref.c["num_key_value_heads"], ref.c["head_dim"]
+    x = torch.from_numpy(np.frombuffer(raw[4:], np.float16).astype(np.float64)).view(L, 2, m.pos(), G, D)
+    return [(x[i, 0], x[i, 1]) for i in range(L)]
 
 
 def check(got, want, what):
@@ -196,6 +212,26 @@ def test_switching_back_leaves_the_default_as_it_was(synth):
         for f, words in ((lambda: b.set_window(5), "reference order"), (lambda: (b.reset(), b.set_cache("q4")), "reference order")):
             with pytest.raises(qa.QphError, match=words):
                 f()
+
+
+@pytest.mark.parametrize("chunk,few", [(24, ""), (7, "0"), (90, "100000")])
+def test_modes_one_after_the_other(chunk, few, synth, monkeypatch):
+    """each change finds scratch for its own kernels, whatever the modes before it needed"""
+    monkeypatch.setenv("QPH_PF_CHUNK", str(chunk))
+    monkeypatch.setenv("QPH_KV_FEW", few)
+    path = synth("mini128")
+    ref = Plain(path)
+    toks = np.random.default_rng(13).integers(0, 2048, 100).astype(np.int32)
+    with qa.HipLlama.load(path, max_ctx=3000) as m:
+        for kind, window, sinks in (("q4", 0, 0), ("q4", 40, 3), ("f16", 40, 3), ("f16", 1000, 0), ("q4", 1000, 0), ("f16", 1000, 0), ("q4", 0, 0)):
+            m.reset()
+            m.set_cache(kind)
+            m.set_window(window, sinks)
+            got = m.prefill(toks[:98]), m.step(int(toks[98]))
+            # over the cache's own values: of 100K rounded ones many lie next to a border of their codes, and a narrow window gives each weight
+            want = ref.logits(toks[:99], kind, window, sinks, cached(m, ref))
+            check(got[0], want[97], f"{kind} {window} prompt")
+            check(got[1], want[98], f"{kind} {window} step")
 
 
 def test_window_changes_during_a_conversation(synth):
