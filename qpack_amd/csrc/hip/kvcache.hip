@@ -575,12 +575,12 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int col = c0 + (TWO ? lr & 7 : lr), tok = token_of(a, col), hr = col - tok * a.rep;
   // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j.  Asked for before
-  // the sequence's position is known
-  h8 q[KS];
-  float x[KS][8];
-  {
-    const bool there = tok < a.n;
-    const int64_t at = b * a.q.seq + (int64_t)(there ? tok : 0) * a.q.tok + (int64_t)(g * a.rep + hr) * a.q.head;
+  // the sequence's position is known.  Columns past the call's last token are zeros: any row that is there may be another workgroup's,
+  // whose results may be on their way into it (out may be q)
+  h8 q[KS] = {};
+  float x[KS][8] = {};
+  if (tok < a.n) {
+    const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)(g * a.rep + hr) * a.q.head;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
       const int64_t d = at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg);
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   uint16_t *vbuf = (uint16_t *)sm + wave * kFewTile * HD;
   Tile<HD, KIND> cur;
   if (t0 + wave < t1) { load_v<HD, KIND>(a, h, s, t0 + wave, lane, cur, vbuf); load_k<HD, KIND>(a, h, s, t0 + wave, lane, cur); }
-  float f = a.scale2;   // softmax scale in base 2, times the row's power.  (Columns past the last are some row's: nothing of them is stored)
+  float f = a.scale2;   // softmax scale in base 2, times the row's power
   if constexpr (T != RT_F16) {
     float mx = 0.f;
 #pragma unroll
@@ -670,8 +670,9 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       return rs;
     };
     float rs = weights();
-    // The maximum is looked for only where the weights say that it has outgrown m, or where there is none yet
-    if (__any(!(rs <= kRoom) | (m == -INFINITY))) {
+    // The maximum is looked for only where a token's weights say that it has outgrown m, or where there is none yet.  (What rows that
+    // take no part hold decides nothing: the columns of a wave look for theirs together, which shows in their last bits)
+    if (__any((int)live & (int)(!(rs <= kRoom) | (m == -INFINITY)))) {
       float bm = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; j++) bm = fmaxf(bm, y[j]);
@@ -986,16 +987,20 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (kb0 + 1 < kb1) fetch(kb0 + 1, st1);
     // ---- queries
     {
-      // (columns past the last token are some row's: nothing of them is stored)
-      const int64_t at = b * a.q.seq + (int64_t)min(tok, a.n - 1) * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
-      float x[KQ][8], mx = 0.f;
+      // (columns past the last token are zeros, as in k_kv_few)
+      float x[KQ][8] = {}, mx = 0.f;
 #pragma unroll
-      for (int k = 0; k < KQ; k++) {
-        if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
-        else {
-          load_elems<T, 8>(a.q, at + 16 * k, x[k]);
+      for (int k = 0; k < KQ; k++) q[k] = (h8)(_Float16)0.f;
+      if (tok < a.n) {
+        const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
 #pragma unroll
-          for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
+        for (int k = 0; k < KQ; k++) {
+          if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
+          else {
+            load_elems<T, 8>(a.q, at + 16 * k, x[k]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
+          }
         }
       }
       if constexpr (T != RT_F16) {
@@ -1122,8 +1127,8 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
         }
       }
       float rs = weights();
-      // The maximum is looked for only where the weights say that it has outgrown m, or where there is none yet
-      if (__any(!(rs <= kRoom) | (m == -INFINITY))) {
+      // as in k_kv_few, by the tokens' columns alone
+      if (__any((int)live & (int)(!(rs <= kRoom) | (m == -INFINITY)))) {
         float bm = -INFINITY;
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)

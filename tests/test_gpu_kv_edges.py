@@ -1,0 +1,74 @@
+"""KvCache.attention at its edges: rows that take no part beside rows that do, values at the ends of their types' ranges.  Where a call is
+compared with another one of the same kernel over the same tokens, the two are to agree to the bit."""
+import math
+
+import pytest
+
+import qpack_amd as qa
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_kv import BF16, F16, F32, TYPES, filled, i32, reference, route  # noqa: E402, F401
+
+
+def check_loud(got, q, K, V, P0, **mask):
+    """test_gpu_kv's bound for rows whose softmax picks few positions: where their V is 0 an output is as small as the weights of the
+    others, and fp16's last place is no longer relative.  Below 2^-14 it is 2^-24, so an fp16 output is rounded by up to 2^-25.  A weight is an
+    fp16 operand with 2^8 in the place of the largest, or more: one below 2^-14 is rounded by up to 2^-25, which is 2^-33 of the largest, and
+    the sum of weights that divides it is no smaller than the largest."""
+    reference.two = q.dtype == F32
+    o, A, ds = reference(q.double().cpu(), K, V, P0, **mask)
+    rep = q.shape[1] // V.shape[1]
+    floor = 2.0 ** -33 * V[:P0 + q.shape[0]].abs().sum(0).repeat_interleave(rep, 0)
+    tol = A * ((2.0 ** -21 if q.dtype == F32 else 2.0 ** -11) + 2 * ds) + torch.finfo(q.dtype).eps / 2 * o.abs() + floor + (2.0 ** -25 if q.dtype == F16 else 0)
+    err = (got.double().cpu() - o).abs()
+    assert bool((err <= tol).all()), f"{int((~(err <= tol)).sum())} of {err.numel()} off, worst {float((err / tol).nan_to_num(1e9).max()):.2f} tolerances"
+
+
+# ------------------------------------------------------------------ rows that take no part
+# n * rep a multiple of neither 8, 16 nor 256: the last chunk has columns behind the last token
+@pytest.mark.parametrize("kind", ["q4", "f16"])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,rep,past,window", [(3, 7, 900, 0), (1, 5, 40, 0), (5, 3, 700, 90), (75, 7, 333, 0), (41, 7, 500, 64)])
+def test_over_q_as_beside_it(kind, type, n, rep, past, window, route):
+    """out = q: no workgroup reads another one's rows, whose results may be there already"""
+    print(f"over q: {kind} {type} n {n} rep {rep} past {past} window {window}", flush=True)
+    gen = torch.Generator().manual_seed(n + rep)
+    S, G, D = 3, 2, 64
+    c, K, V = filled(kind, S, G, D, past + n, [past + n] * S, gen)
+    # loud rows: the maxima move often
+    q = (torch.randn(S, n, G * rep, D, generator=gen) * 6).to(TYPES[type]).cuda()
+    pos = i32([past, past // 2, past])
+    want = c.attention(q, pos, window=window)
+    for _ in range(8):
+        x = q.clone()
+        assert c.attention(x, pos, window=window, out=x) is x
+        assert torch.equal(x, want)
+    check_loud(want[0], q[0], K[0], V[0], past, window=window)
+
+
+@pytest.mark.parametrize("kind", ["q4", "f16"])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,lens,rep,past", [(6, [3, 6, 1], 7, 3000), (2, [1, 2, 0], 4, 600), (60, [7, 60, 33], 5, 1500)])
+def test_padding_rows_change_no_bit(kind, type, n, lens, rep, past, route):
+    """what rows at and past lens[b] hold: zeros, values that outgrow every maximum, NaN, infinities"""
+    print(f"padding: {kind} {type} n {n} lens {lens} rep {rep} past {past}", flush=True)
+    gen = torch.Generator().manual_seed(n + past)
+    S, G, D = 3, 1, 128
+    c, K, V = filled(kind, S, G, D, past + n, [past + n] * S, gen)
+    q = (torch.randn(S, n, G * rep, D, generator=gen) * 3).to(TYPES[type]).cuda()
+    outs = []
+    for fill in (0.0, 300 * torch.randn(n, G * rep, D, generator=gen), math.nan, math.inf):
+        x = q.clone()
+        for b, m in enumerate(lens):
+            x[b, m:] = fill if isinstance(fill, float) else fill[m:].to(x)
+        out = torch.full_like(x, 55.)
+        c.attention(x, i32([past] * S), lens=i32(lens), out=out)
+        outs.append(out)
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+    for b, m in enumerate(lens):
+        if m:
+            check_loud(outs[0][b, :m], q[b, :m], K[b], V[b], past)
+        assert bool((outs[0][b, m:] == 55).all())
