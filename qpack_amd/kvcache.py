@@ -22,12 +22,17 @@ def _binding():
     return _bind
 
 
+def _strides(x):
+    """between the sequences and positions of an f16 cache's tensor; 0 (without gaps) for an axis of one, whose stride means nothing"""
+    return tuple(stride if size > 1 else 0 for size, stride in zip(x.shape[:2], x.stride()))
+
+
 class KvCache:
     """nseq sequences of ctx positions, kv_heads heads of head_dim (64 or 128) dims, in fp16 ("f16") or 4 bits ("q4").
 
     data: the memory, new (zeros) when None.  "q4": a contiguous uint8 tensor [nseq, kv_heads, ceil(ctx / 8), 9 * head_dim] of
     the records that include/qpack_hip.h describes; "f16": (K, V), fp16 tensors [nseq, ctx, kv_heads, head_dim] of equal strides, each
-    position's rows contiguous.
+    position's rows contiguous, sequences and positions apart (no expanded tensors).
 
     In all calls token t < n of sequence b, and t < lens[b] where lens is given, is position pos[b] + t; sequences with pos[b] <
     0 and positions at or past ctx take no part.  pos and lens: int32 tensors [nseq] on the cache's device.
@@ -56,11 +61,13 @@ class KvCache:
                 data = tuple(torch.zeros(shape, dtype=torch.float16, device=device) for _ in range(2))
             k, v = data
             for x in (k, v):
-                if x.dtype != torch.float16 or tuple(x.shape) != shape or x.stride()[2:] != (self.head_dim, 1) or x.stride() != k.stride():
+                if x.dtype != torch.float16 or tuple(x.shape) != shape or x.stride(3) != 1 or (self.kv_heads > 1 and x.stride(2) != self.head_dim) or _strides(x) != _strides(k):
                     raise QphError(f"kv: an f16 cache's data must be two fp16 tensors {list(shape)} of equal strides with contiguous rows")
+                if any(size > 1 and stride == 0 for size, stride in zip(x.shape[:2], x.stride())):
+                    raise QphError("kv: an f16 cache's sequences and positions must not share memory (an expanded tensor)")
             if v.device != k.device:
                 raise QphError("kv: K and V on different devices")
-            first, at = k, (k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1))
+            first, at = k, (k.data_ptr(), v.data_ptr(), *_strides(k))
         if first.device.type != "cuda":
             raise QphError("kv: the cache must be on a GPU")
         self.data, self.device = data, first.device
