@@ -207,7 +207,7 @@ int qph_pack(const char *src, const char *dst, int threads, int *coded);
 typedef struct {
   int kind;                            /* QPH_F16 or QPH_Q4 */
   int nseq, kv_heads, head_dim;        /* head_dim 64 or 128; nseq <= 65535, kv_heads <= 4096 */
-  int64_t ctx;                         /* positions of a sequence, <= 2^30 */
+  int64_t ctx;                         /* positions of a sequence, <= 2^30; the cache's bytes are below 2^63 */
   void *k, *v;
   int64_t seq, row;
 } qph_kv;

@@ -41,11 +41,16 @@ static void need(const void *p, const char *what) {
 }
 // ---- the kv entry points' arguments
 static int kv_kind(const qph_kv *c) { return c->kind == QPH_Q4 ? qph::MK_Q4 : qph::MK_F32; }
+static void kv_fits(__int128 bytes) {
+  if (bytes > INT64_MAX) throw std::invalid_argument("kv: the cache's bytes must be below 2^63");
+}
 static void kv_check(int kind, int nseq, int kv_heads, int head_dim, int64_t ctx) {
   if (kind != QPH_F16 && kind != QPH_Q4) throw std::invalid_argument("kv: kind must be QPH_F16 or QPH_Q4");
   if (nseq < 1 || nseq > 65535 || kv_heads < 1 || kv_heads > 4096) throw std::invalid_argument("kv: nseq must be in [1, 65535] and kv_heads in [1, 4096]");
   if (head_dim != 64 && head_dim != 128) throw std::invalid_argument("kv: head_dim must be 64 or 128");
   if (ctx < 1 || ctx > (int64_t)1 << 30) throw std::invalid_argument("kv: ctx must be in [1, 2^30]");
+  // within the limits above the product reaches 2^65
+  kv_fits(kind == QPH_Q4 ? (__int128)nseq * kv_heads * qph::kv4_records(ctx) * 9 * head_dim : (__int128)4 * nseq * ctx * kv_heads * head_dim);
 }
 // the cache's strides
 static void kv_cache(const qph_kv *c, int64_t *seq, int64_t *row) {
@@ -58,9 +63,11 @@ static void kv_cache(const qph_kv *c, int64_t *seq, int64_t *row) {
   need(c->v, "cache v");
   const int64_t d = (int64_t)c->kv_heads * c->head_dim;
   *row = c->row ? c->row : d;
-  *seq = c->seq ? c->seq : c->ctx * *row;
-  if ((uintptr_t)c->v % 16 || *row % 8 || *seq % 8) throw std::invalid_argument("kv: an fp16 cache must be 16-byte aligned and its strides multiples of 8");
-  if (*row < d || (c->nseq > 1 && *seq < (c->ctx - 1) * *row + d)) throw std::invalid_argument("kv: the cache's rows or sequences overlap");
+  const __int128 between = c->seq ? c->seq : (__int128)c->ctx * *row, span = (__int128)(c->ctx - 1) * *row + d;   // of sequences; of one's rows
+  if ((uintptr_t)c->v % 16 || *row % 8 || between % 8) throw std::invalid_argument("kv: an fp16 cache must be 16-byte aligned and its strides multiples of 8");
+  if (*row < d || (c->nseq > 1 && between < span)) throw std::invalid_argument("kv: the cache's rows or sequences overlap");
+  kv_fits(2 * ((c->nseq - 1) * between + span));
+  *seq = (int64_t)between;
   if (c->k == c->v) throw std::invalid_argument("kv: the cache's k and v overlap");
 }
 static qph::KvRows kv_rows(const qph_rows *r, const char *what, bool out, int nseq, int n, int heads, int hd) {
