@@ -464,6 +464,9 @@ int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, in
     a.pos = pos; a.lens = lens;
     a.scale2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim));
     if (std::isinf(a.scale2)) throw std::invalid_argument("kv: scale is too large");
+    // over q: every workgroup stores where it has read, which takes the same rows in the same places
+    if (n && q->p == out->p && ((c->nseq > 1 && q->seq != out->seq) || (n > 1 && q->tok != out->tok) || (heads > 1 && q->head != out->head)))
+      throw std::invalid_argument("kv: out over q must have q's strides");
     if (n) {
       const int64_t bytes = (int64_t)qph::kv_attn_plan(a);
       if (bytes && (!work || work_bytes < bytes || (uintptr_t)work % 16)) throw std::invalid_argument("kv: work must have the " + std::to_string(bytes) + " bytes that qph_kv_attention_work gives, 16-byte aligned");

@@ -92,7 +92,7 @@ class KvCache:
 
     def attention(self, q, pos, lens=None, window=0, sinks=0, scale=0.0, out=None):
         """softmax(scale q K^T) V of the tokens q [nseq, n, heads, head_dim] at pos[b] + t, whose rows are in the cache; scale 0: 1 /
-        sqrt(head_dim).  Position P sees p <= P and, with window > 0, of those p > P - window and p < sinks only.  out may be q; rows that
+        sqrt(head_dim).  Position P sees p <= P and, with window > 0, of those p > P - window and p < sinks only.  out may be q, or apart from it; rows that
         take no part stay as they are in out, and are zero without it"""
         if out is None:
             import torch

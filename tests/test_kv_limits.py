@@ -32,3 +32,13 @@ def test_strides_past_63_bits_are_refused():
     far = rows(p=4 * P, seq=0, tok=0, head=0)
     for c in (f(nseq=1, seq=1 << 62), f(nseq=2, seq=1 << 60), f(nseq=1, ctx=1, row=1 << 62)):   # taken: the next check is what refuses
         refused(write(c, k=far, v=far, n=-1), "n must be")
+
+
+def test_over_q_in_other_places_is_refused():
+    """rows that are stored where other tokens' queries are still to be read"""
+    for r in (rows(seq=3200), rows(tok=320), rows(tok=256), rows(head=128)):
+        refused(attend(q=rows(), out=r), "q's strides")
+    assert attend(q=rows(), out=rows(tok=320), n=0) == 0
+    one = lambda **k: cache(ctx=4096, kv_heads=1, **k)   # noqa: E731
+    for q, out, n, c in ((rows(), rows(), 3, one()), (rows(), rows(tok=7), 1, one()), (rows(), rows(seq=9), 3, one(nseq=1)), (rows(tok=0), rows(p=2 * P), 3, one())):
+        refused(attend(c, q=q, out=out, n=n), "work")   # taken: the next check is what refuses
