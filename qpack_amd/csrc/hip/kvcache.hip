@@ -410,19 +410,18 @@ __device__ __forceinline__ uint32_t seen_bits(const KvAttnArgs &a, const Span &s
   return v < s.NR ? on : 0;
 }
 
-// fp16 queries are the matrix cores' operands as they are.  Others enter as fp16, each row scaled by the power of two that brings its largest magnitude into [1, 2): bf16
-// values keep every bit that is not 2^-25 below that (fp32 ones go in two halves, hi + lo, and keep 22 bits).  The power
+// fp16 queries are the matrix cores' operands as they are.  Others enter as fp16, each row scaled by the power of two that brings its largest magnitude into [1, 2), or [2, 4)
+// from 2^127 on, where that power is no normal number: bf16 values keep every bit that is not 2^-25 below that (fp32 ones go in two halves, hi + lo, and keep 22 bits).  The power
 // returns with the softmax scale, in fp32.
-__device__ __forceinline__ float row_power(float mx) {   // 2^-e; 1 for rows that are zero or not finite
+__device__ __forceinline__ float row_power(float mx) {   // 2^-e, 2^-126 at the least; 1 for rows that are zero or not finite
   const uint32_t e = __builtin_bit_cast(uint32_t, mx) >> 23;
-  return e == 0 || e >= 254 ? 1.f : __builtin_bit_cast(float, (254u - e) << 23);
+  return e == 0 || e == 255 ? 1.f : __builtin_bit_cast(float, (254u - min(e, 253u)) << 23);
 }
-
 // Probabilities are held as 2^(x - m + kPBias), where m is a column's maximum as it was when it was last looked for: when there was none,
 // and whenever a lane's weights of a tile add up to more than kRoom.  They stay in fp16's range, what lies 2^-32 below m is
 // still there, and the sum they are divided by is scaled alike.
 constexpr float kPBias = 8.f, kRoom = 32768.f;
-// The least softmax factor of a row: with 0 a masked score would be -inf x 0.  The scores it takes, up to 2^24, stay below 2^-100
+// The least softmax factor of a row: with 0 a masked score would be -inf x 0.  The scores it takes, up to 2^25, stay below 2^-100
 constexpr float kTinyF = 0x1p-126f;
 
 // ------------------------------------------------------------------ few tokens

@@ -72,3 +72,19 @@ def test_padding_rows_change_no_bit(kind, type, n, lens, rep, past, route):
         if m:
             check_loud(outs[0][b, :m], q[b, :m], K[b], V[b], past)
         assert bool((outs[0][b, m:] == 55).all())
+
+
+# ------------------------------------------------------------------ values at the ends of their ranges
+@pytest.mark.parametrize("kind", ["q4", "f16"])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [2, 70])
+def test_queries_of_the_largest_size(kind, type, n, route):
+    """rows with magnitudes of 2^127 and above, and a softmax scale that brings the scores back"""
+    gen = torch.Generator().manual_seed(17)
+    c, K, V = filled(kind, 1, 1, 64, 200, [200], gen)
+    q = torch.randn(1, n, 4, 64, generator=gen) * 2.0 ** 122
+    q.scatter_(3, torch.randint(0, 64, (1, n, 4, 1), generator=gen), 2.0 ** 127 * (1 + 0.98 * torch.rand(1, n, 4, 1, generator=gen)))
+    q = q.to(TYPES[type]).cuda()
+    assert bool((q.abs().amax(-1) >= 2.0 ** 127).all()) and bool(torch.isfinite(q).all())
+    out = c.attention(q, i32([200 - n]), scale=2.0 ** -125)
+    check_loud(out[0], q[0], K[0], V[0], 200 - n, scale=2.0 ** -125)
