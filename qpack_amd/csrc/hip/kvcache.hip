@@ -421,8 +421,9 @@ __device__ __forceinline__ float row_power(float mx) {   // 2^-e, 2^-126 at the 
 // and whenever a lane's weights of a tile add up to more than kRoom.  They stay in fp16's range, what lies 2^-32 below m is
 // still there, and the sum they are divided by is scaled alike.
 constexpr float kPBias = 8.f, kRoom = 32768.f;
-// The least softmax factor of a row: with 0 a masked score would be -inf x 0.  The scores it takes, up to 2^25, stay below 2^-100
-constexpr float kTinyF = 0x1p-126f;
+// The least and the largest softmax factor of a row: with 0 a masked score would be -inf x 0, with inf a score of 0 would be NaN.  The scores
+// that the least takes, up to 2^25, stay below 2^-100
+constexpr float kTinyF = 0x1p-126f, kMostF = 0x1.fffffep127f;
 
 // ------------------------------------------------------------------ few tokens
 // Grid (split, kv head and column chunk, sequence), 8 waves, each streaming its own tiles of 32 positions (4 records) with
@@ -606,7 +607,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
     mx = pair_max32(pair_max16(mx));
     const float p2 = row_power(mx);
-    f = fmaxf(f / p2, kTinyF);
+    f = fminf(fmaxf(f / p2, kTinyF), kMostF);
 #pragma unroll
     for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -1005,7 +1006,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       if constexpr (T != RT_F16) {
         mx = pair_max32(mx);
         const float p2 = row_power(mx);
-        f = fmaxf(f / p2, kTinyF);
+        f = fminf(fmaxf(f / p2, kTinyF), kMostF);
 #pragma unroll
         for (int k = 0; k < KQ; k++)
 #pragma unroll

@@ -88,3 +88,15 @@ def test_queries_of_the_largest_size(kind, type, n, route):
     assert bool((q.abs().amax(-1) >= 2.0 ** 127).all()) and bool(torch.isfinite(q).all())
     out = c.attention(q, i32([200 - n]), scale=2.0 ** -125)
     check_loud(out[0], q[0], K[0], V[0], 200 - n, scale=2.0 ** -125)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 70])
+def test_scores_of_zero_under_the_largest_factors(type, n, route):
+    """the scale times the rows' magnitude passes fp32, the scores are 0: all positions weigh alike"""
+    gen = torch.Generator().manual_seed(18)
+    c, _, V = filled("f16", 1, 1, 64, 200, [200], gen)
+    c.data[0].zero_()
+    q = (torch.randn(1, n, 4, 64, generator=gen) * 2.0 ** 100).to(TYPES[type]).cuda()
+    out = c.attention(q, i32([200 - n]), scale=1e20)
+    check_loud(out[0], q[0], torch.zeros_like(V[0]), V[0], 200 - n, scale=1e20)
