@@ -673,6 +673,23 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
     // The maximum is looked for only where a token's weights say that it has outgrown m, or where there is none yet.  (What rows that
     // take no part hold decides nothing: the columns of a wave look for theirs together, which shows in their last bits)
     if (__any((int)live & (int)(!(rs <= kRoom) | (m == -INFINITY)))) {
+      if constexpr (TWO && KIND != MK_Q4) {
+        // An infinite K (4-bit scales make it NaN): the score is what the hi half says, whose infinity the lo half's 0 x inf, or infinity of
+        // the other sign, would turn into NaN.  The tile's K is still there (the products again: their results kept would spill)
+        if (__any(!(rs == rs))) {
+#pragma unroll
+          for (int mt = 0; mt < 2; mt++) {
+            f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; k++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, cur.k[mt][k]), q[k], t, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float other = xchg8_f(t[i]), hi = lr < 8 ? t[i] : other;
+              if (y[4 * mt + i] != y[4 * mt + i] && fabsf(hi) == INFINITY) y[4 * mt + i] = hi;   // (masked ones are -inf)
+            }
+          }
+        }
+      }
       float bm = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; j++) bm = fmaxf(bm, y[j]);
@@ -1129,6 +1146,23 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       float rs = weights();
       // as in k_kv_few, by the tokens' columns alone
       if (__any((int)live & (int)(!(rs <= kRoom) | (m == -INFINITY)))) {
+        if constexpr (TWO && KIND != MK_Q4) {
+          // An infinite K, as in k_kv_few: where the sum is NaN (the masked are -inf) and hi's product alone infinite, that is the score
+          if (__any(!(rs == rs))) {
+            const uint16_t *kl = k_of(kb);
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+              f32x16 t;
+#pragma unroll
+              for (int i = 0; i < 16; i++) t[i] = 0.f;
+#pragma unroll
+              for (int k = 0; k < KQ; k++) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8 *)(kl + (32 * mt + kr) * KST + 16 * k + 8 * hf), q[k], t, 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < 16; i++)
+                if (sc[mt][i] != sc[mt][i] && fabsf(t[i]) == INFINITY) sc[mt][i] = t[i];
+            }
+          }
+        }
         float bm = -INFINITY;
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)

@@ -100,3 +100,28 @@ def test_scores_of_zero_under_the_largest_factors(type, n, route):
     q = (torch.randn(1, n, 4, 64, generator=gen) * 2.0 ** 100).to(TYPES[type]).cuda()
     out = c.attention(q, i32([200 - n]), scale=1e20)
     check_loud(out[0], q[0], torch.zeros_like(V[0]), V[0], 200 - n, scale=1e20)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 3, 70])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_infinite_keys(type, n, hd, route):
+    """an fp32 key past fp16's range is infinite in an fp16 cache: where its score is -inf the position has no weight, where it is +inf the
+    row is NaN, as the formula has it"""
+    gen = torch.Generator().manual_seed(19)
+    past, at, rep = 190, 77, 4
+    c, K, V = filled("f16", 1, 1, hd, past + n, [past + n], gen)
+    k, v = c.read(i32([at]), 1, dtype=F32)
+    q = (torch.randn(1, n, rep, hd, generator=gen) * 1.5).to(TYPES[type])
+    # head 0: exact in fp16; the others: halves of either sign, or as the type has them; the last one on the side that is NaN
+    q[:, :, 0, 5], q[:, :, 1, 5], q[:, :, 2, 5] = -1.0, -1.0001, -0.9999
+    q[:, :, 3, 5] = 0.7
+    q = q.cuda()
+    rest = [p for p in range(past + n) if p != at]
+    for key, sign in ((1e5, 1), (-1e5, -1)):
+        k[..., 5] = key
+        c.write(k, v, i32([at]))
+        x = q * sign
+        out = c.attention(x, i32([past]))
+        assert bool(torch.isnan(out[0, :, 3]).all())
+        check_loud(out[0, :, :3], x[0, :, :3], K[0][rest], V[0][rest], past - 1)
