@@ -231,7 +231,8 @@ int qph_kv_read(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, co
  * of those only p > P - window and p < sinks.  heads a multiple of kv_heads (head h reads kv head h / (heads / kv_heads)), at most 65535,
  * n * heads / kv_heads <= 2^23; scale 0: 1 / sqrt(head_dim), else > 0.  out has q's type; its rows are q's own (the same pointer and strides) or lie apart from them.  work: qph_kv_attention_work bytes of scratch
  * (16-byte aligned; NULL if 0) that no other call uses meanwhile - two graphs that may run at once need one each.  fp32 queries are computed to
- * about 22 bits, fp16 and bf16 ones to the 11 of an fp16 operand, all sums in fp32. */
+ * about 22 bits, fp16 and bf16 ones to the 11 of an fp16 operand (the weights too), all sums in fp32.  Infinite keys and values count as the formula
+ * has them; an infinite value whose weight is below 2^-33 of the largest may leave its dim NaN. */
 int qph_kv_attention_work(const qph_kv *c, int type, int heads, int n, int window, int sinks, int64_t *bytes);
 int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, int heads, int n, const int *pos, const int *lens,
                      int window, int sinks, float scale, void *work, int64_t work_bytes, void *stream);

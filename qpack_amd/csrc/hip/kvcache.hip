@@ -756,7 +756,10 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
     f32x4 y = o[d];
     if (TWO) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) y[i] += xchg8_f(y[i]);
+      for (int i = 0; i < 4; i++) {   // an infinite V: as the scores, hi's sum where only lo's makes it NaN
+        const float both = y[i] + xchg8_f(y[i]);
+        y[i] = both != both && fabsf(y[i]) == INFINITY ? y[i] : both;
+      }
     }
     if (lr < NC) *(f32x4 *)(ored + (wave * NC + lr) * QS + 16 * d + 4 * lg) = y;
   }
@@ -1187,6 +1190,31 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (kb + 3 < kb1) fetch(kb + 3, st);
     if (tid < 2) badp[(kb - kb0 + 3) % 4][tid] = 0;
     __syncthreads();
+  }
+  if constexpr (TWO && KIND != MK_Q4) {
+    // An infinite V: the lo halves (0, or of either sign) turn the sum into NaN.  Such sums are what the values say that are not finite and
+    // that the column sees, read again.  (A score that is NaN shows in l)
+    bool nan = false;
+#pragma unroll
+    for (int t = 0; t < OT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) nan |= o[t][i] != o[t][i];
+    if (__any((int)live & (int)nan)) {
+#pragma unroll
+      for (int t = 0; t < OT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[t][i] = o[t][i] != o[t][i] ? 0.f : o[t][i];
+#pragma unroll 1
+      for (int64_t i = (int64_t)kManyBlk * kb0; i < min((int64_t)kManyBlk * kb1, (int64_t)kRec * s.NR); i++) {
+        const int p = kRec * record(s, (int)(i / kRec)) + (int)(i % kRec);
+        const bool sp = sees(a, P, lo, p);
+        if (!__any(sp)) continue;   // (also the positions past ctx)
+#pragma unroll
+        for (int t = 0; t < OT; t++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) add_bad<HD, KIND>(nullptr, hd.v + (int64_t)p * a.crow, p, 32 * t + 8 * j + 4 * hf, sp, o[t], 4 * j);
+      }
+    }
   }
   l = pair_sum32(l);
   if constexpr (T != RT_F32) {

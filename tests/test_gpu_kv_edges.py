@@ -125,3 +125,24 @@ def test_infinite_keys(type, n, hd, route):
         out = c.attention(x, i32([past]))
         assert bool(torch.isnan(out[0, :, 3]).all())
         check_loud(out[0, :, :3], x[0, :, :3], K[0][rest], V[0][rest], past - 1)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,where,window", [(5, 2, 0), (5, 1, 3), (90, 40, 0), (90, 20, 33), (1, 0, 0), (1, -20, 0), (5, -30, 0), (90, -40, 0), (300, -40, 0)])
+def test_infinite_values(type, n, where, window, route):
+    """an infinite V element of a position that some tokens see, or all: theirs is infinite, the others' as it was"""
+    gen = torch.Generator().manual_seed(20)
+    past, rep, D = 45, 4, 64
+    c, K, V = filled("f16", 1, 1, D, past + n, [past + n], gen)
+    k, v = c.read(i32([past + where]), 1, dtype=F32)
+    v[..., 5], v[..., 9] = math.inf, -math.inf
+    c.write(k, v, i32([past + where]))
+    q = torch.randn(1, n, rep, D, generator=gen).to(TYPES[type]).cuda()
+    out = c.attention(q, i32([past]), window=window)
+    for t in range(n):
+        got, W = out[0, t:t + 1].clone(), V[0].clone()
+        if t >= where and (not window or t < where + window):
+            assert bool((got[..., 5] == math.inf).all()) and bool((got[..., 9] == -math.inf).all())
+            got[..., [5, 9]] = 0
+            W[..., [5, 9]] = 0
+        check_loud(got, q[0, t:t + 1], K[0], W, past + t, window=window)
