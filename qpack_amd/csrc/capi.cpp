@@ -108,7 +108,7 @@ static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sink
   if (window < 0 || sinks < 0) throw std::invalid_argument("kv: window and sinks must not be negative");
   a.kind = kv_kind(c); a.cache = c->k; a.cache_v = c->v; a.ctx = c->ctx; a.nrec = qph::kv4_records(c->ctx);
   a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.heads = heads; a.rep = heads / c->kv_heads; a.n = n;
-  a.window = window; a.sinks = sinks;
+  a.window = window; a.sinks = sinks; a.few = qph::kv_few();
 }
 static void hck(hipError_t e, const char *what) {
   if (e != hipSuccess) throw std::runtime_error(std::string("hip: ") + hipGetErrorString(e) + " (" + what + ")");

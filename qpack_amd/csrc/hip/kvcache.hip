@@ -1306,6 +1306,10 @@ hipError_t launch_kv_read(int kind, const KvIoArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
+int kv_few() {
+  const char *e = getenv("QPH_KV_FEW");
+  return e && *e ? std::max(0, atoi(e)) : -1;
+}
 size_t kv_attn_plan(KvAttnArgs &a) {
   const int cus = 256;
   const bool two = a.q.type == RT_F32;
@@ -1320,8 +1324,7 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   // many; 128 over 8 x 16384 176 and 112; 128 over 8 x 1024 18 and 35.  fp16: the same 92 and 38, 624 and 133, 44 and 31
   const int64_t chunks = (cols + few - 1) / few, positions = (int64_t)a.nseq * a.nkv * reach(few);
   const int64_t most = a.kind == MK_Q4 ? 4 + (384 << 10) / positions : 1 + (192 << 10) / positions;
-  const char *limit = getenv("QPH_KV_FEW");   // test hook: columns up to which k_kv_few is taken
-  a.many = (limit && *limit ? cols > atoi(limit) : chunks > std::min<int64_t>(most, 128)) || chunks * a.nkv > 65535;   // (the last: the grid)
+  a.many = (a.few >= 0 ? cols > a.few : chunks > std::min<int64_t>(most, 128)) || chunks * a.nkv > 65535;   // (the last: the grid)
   a.cols = a.many ? kManyCols : few;
   a.half_log2 = a.many ? 7 : two ? 2 : 3;
   a.tile_log2 = a.many ? 3 : 2;   // records of a tile

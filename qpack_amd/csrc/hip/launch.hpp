@@ -321,10 +321,12 @@ struct KvAttnArgs {
   int window, sinks;
   float scale2;                 // softmax scale times log2(e), > 0
   float *part;                  // nsplit > 1: partial sums, then (max, sum) pairs, kv_attn_plan's bytes
+  int few = -1;                 // test hook: columns up to which k_kv_few is taken (-1: by kv_attn_plan's rule)
   // set by kv_attn_plan
   int many, paired, cols, half_log2, nchunk, tile_log2, min_log2, one_tiles, nsplit, rep_shift;
   uint32_t rep_mul;
 };
+int kv_few();   // that hook's value now (QPH_KV_FEW)
 // how the call is laid out; the bytes of part
 size_t kv_attn_plan(KvAttnArgs &a);
 hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st);

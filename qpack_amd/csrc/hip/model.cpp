@@ -122,6 +122,7 @@ HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int 
   if (const char *e = getenv("QPH_ATTN_SPLIT_POS")) attn_split_pos_ = std::max(0, atoi(e));
   // test hook: the bound of a merger's wait for the other splits (the failure path forced from the host)
   if (const char *e = getenv("QPH_ATTN_SPIN")) attn_spin_ = std::max(0, atoi(e));
+  kv_few_ = kv_few();
   attn_force_late_ = getenv("QPH_ATTN_FORCE_LATE") != nullptr;   // test hook: the same failure without the race
   if (const char *e = getenv("QPH_MV_SPLIT")) split_chain_ = atoi(e) != 0;
   {  // long contexts: the splits' merge as a launch of its own from lm_splits_ splits (QPH_ATTN_MERGE_SEP: that
@@ -309,7 +310,7 @@ KvAttnArgs HipLlama::kv_attn(int l, const float *q, float *out, int n) const {
   a.q = KvRows{(void *)q, RT_F32, 0, qd_, cfg_.head_dim}; a.out = KvRows{out, RT_F32, 0, qd_, cfg_.head_dim};
   a.pos = &ctl_->pos; a.window = window_; a.sinks = sinks_;
   a.scale2 = 1.4426950408889634f / std::sqrt((float)cfg_.head_dim);
-  a.part = kv_part_;
+  a.part = kv_part_; a.few = kv_few_;
   return a;
 }
 void HipLlama::kv_append(int l, float *k, float *v, int n) { QPH_CK(launch_kv_write(kv_kind_, kv_io(l, k, v, n), st_)); }

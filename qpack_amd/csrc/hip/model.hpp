@@ -101,6 +101,7 @@ class HipLlama {
   int *kv_zero_ = nullptr;        // a position 0
   float *kv_part_ = nullptr;      // the attention's scratch, for the most that a step or a prompt's chunk takes
   size_t kv_part_bytes_ = 0;
+  int kv_few_ = -1;               // test hook (QPH_KV_FEW at load)
   KvIoArgs kv_io(int l, float *k, float *v, int n) const;
   KvIoArgs stage_io(int l, int n) const;
   KvAttnArgs kv_attn(int l, const float *q, float *out, int n) const;
