@@ -3,6 +3,7 @@
 // 4.5 (8.5 with scratch and a second launch), from torch's own structures 3.5 (7.7); each launch is about 3 of it.
 // torch is loaded before this module is.
 #define PY_SSIZE_T_CLEAN
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -38,6 +39,7 @@ bool fail(const char *fmt, const char *a, const char *b = "") {
 bool tensor(const Cache *c, PyObject *x, const char *name, const at::Tensor **t) {   // on the cache's device
   if (!THPVariable_Check(x)) return fail("kv: %s must be a tensor%s", name);
   *t = &THPVariable_Unpack(x);
+  if ((*t)->requires_grad() && c10::GradMode::is_enabled()) return fail("kv: %s requires a gradient, and no call here passes one on: detach it, or call under torch.no_grad()%s", name);
   if (!(*t)->is_cuda() || (*t)->get_device() != c->device) return fail("kv: %s is not on the cache's device%s", name);
   return true;
 }

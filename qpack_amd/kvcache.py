@@ -38,7 +38,7 @@ class KvCache:
     0 and positions at or past ctx take no part.  pos and lens: int32 tensors [nseq] on the cache's device.
 
     Writes to one cache follow each other: from several streams they need events between them.  Nothing here carries
-    gradients."""
+    gradients: tensors that require one are refused while gradients are recorded."""
 
     def __init__(self, kind, nseq, kv_heads, head_dim, ctx, data=None, device="cuda"):
         import torch
@@ -54,7 +54,7 @@ class KvCache:
                 data = torch.zeros(shape, dtype=torch.uint8, device=device)
             if data.dtype != torch.uint8 or tuple(data.shape) != shape or not data.is_contiguous():
                 raise QphError(f"kv: a q4 cache's data must be a contiguous uint8 tensor {list(shape)}")
-            first, at = data, (data.data_ptr(), 0, 0, 0)
+            tensors, at = (data,), (data.data_ptr(), 0, 0, 0)
         else:
             shape = (self.nseq, self.ctx, self.kv_heads, self.head_dim)
             if data is None:
@@ -67,7 +67,10 @@ class KvCache:
                     raise QphError("kv: an f16 cache's sequences and positions must not share memory (an expanded tensor)")
             if v.device != k.device:
                 raise QphError("kv: K and V on different devices")
-            first, at = k, (k.data_ptr(), v.data_ptr(), *_strides(k))
+            tensors, at = (k, v), (k.data_ptr(), v.data_ptr(), *_strides(k))
+        if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
+            raise QphError("kv: the cache's data requires a gradient, and no call here passes one on")
+        first = tensors[0]
         if first.device.type != "cuda":
             raise QphError("kv: the cache must be on a GPU")
         self.data, self.device = data, first.device

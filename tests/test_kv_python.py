@@ -14,6 +14,30 @@ def f16(*shape):
     return torch.zeros(*shape, dtype=torch.float16)
 
 
+def bound(nseq=2, kv_heads=2, head_dim=64, ctx=40):
+    """the compiled half over an address that is never read: CPU tensors are refused before anything is launched"""
+    from qpack_amd.kvcache import _binding
+    return _binding().Cache(qa.QPH_Q4, nseq, kv_heads, head_dim, ctx, 1 << 20, 0, 0, 0, 0, torch.zeros(1, dtype=torch.uint8))
+
+
+def test_gradients_are_refused():
+    c, x, pos = bound(), torch.zeros(2, 3, 2, 64, dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
+    g = torch.zeros(2, 3, 2, 64, dtype=torch.float16, requires_grad=True)
+    calls = [lambda a: c.write(a, x, pos, None), lambda a: c.attention(a, x, pos, None, 0, 0, 0.0), lambda a: c.read(a, x, pos, None)]
+    for f in calls:
+        for a in (g, g * 2, g[:, :2]):
+            with pytest.raises(qa.QphError, match="requires a gradient"):
+                f(a)
+            with torch.no_grad(), pytest.raises(qa.QphError, match="device"):   # taken as far as that
+                f(a)
+        with pytest.raises(qa.QphError, match="device"):
+            f(g.detach())
+    with pytest.raises(qa.QphError, match="requires a gradient"):
+        cache(f16(3, 40, 2, 64).requires_grad_(), f16(3, 40, 2, 64), 3, 2, 64, 40)
+    with pytest.raises(qa.QphError, match="requires a gradient"):
+        cache(f16(3, 40, 2, 64), f16(3, 40, 2, 64).requires_grad_(), 3, 2, 64, 40)
+
+
 def test_expanded_caches_are_refused():
     """one prefix shared by all sequences, one position by all: the C ABI takes a stride of 0 for a cache without gaps"""
     for x in (f16(1, 40, 2, 64).expand(3, -1, -1, -1), f16(3, 1, 2, 64).expand(-1, 40, -1, -1)):
