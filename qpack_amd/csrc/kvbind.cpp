@@ -29,7 +29,7 @@ struct Cache {
   PyObject_HEAD
   qph_kv c;
   int64_t device, item;
-  PyObject *data;   // a tensor of the cache's memory, item bytes an element: scratch is a new one like it
+  PyObject *data, *data_v;   // tensors of the cache's memory (4-bit: the one of them), item bytes an element: scratch is a new one like data
 };
 
 bool fail(const char *fmt, const char *a, const char *b = "") {
@@ -43,6 +43,8 @@ bool tensor(const Cache *c, PyObject *x, const char *name, const at::Tensor **t)
   if (!(*t)->is_cuda() || (*t)->get_device() != c->device) return fail("kv: %s is not on the cache's device%s", name);
   return true;
 }
+// what a call has written, for autograd's check that nothing saved was changed (inference tensors are not checked)
+void written(const at::Tensor &t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 // a tensor [nseq, n, heads, head_dim] with consecutive dims
 bool rows(const Cache *c, PyObject *x, const char *name, qph_rows *r, int64_t *n, int64_t *heads) try {
   const at::Tensor *t;
@@ -132,6 +134,8 @@ PyObject *io(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   void *st;
   if (!current(c, &here) || !stream_of(c, &st)) return nullptr;
   if (!launch(c, here, st, [&](void *st) { return (WRITE ? qph_kv_write : qph_kv_read)(&c->c, &k, &v, (int)nk, pos, lens, st); })) return nullptr;
+  for (PyObject *t : {WRITE ? c->data : arg[0], WRITE ? c->data_v : arg[1]})
+    if (t) written(THPVariable_Unpack(t));
   Py_RETURN_NONE;
 }
 // attention(q, out, pos, lens, window, sinks, scale)
@@ -158,22 +162,27 @@ PyObject *attention(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   if (bytes && !work.p) return nullptr;
   if (bytes) w = THPVariable_Unpack(work.p).data_ptr();
   if (!launch(c, here, st, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, (float)scale, w, bytes, st); })) return nullptr;
+  written(THPVariable_Unpack(arg[1]));
   Py_RETURN_NONE;
 }
 
-int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_heads, head_dim, ctx, k, v, seq, row, device, data)
+int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_heads, head_dim, ctx, k, v, seq, row, device, data[, the fp16 V's])
   Cache *c = (Cache *)self;
   long long ctx, k, v, seq, row, device;
-  PyObject *data;
-  if (!PyArg_ParseTuple(args, "iiiiLLLLLLO", &c->c.kind, &c->c.nseq, &c->c.kv_heads, &c->c.head_dim, &ctx, &k, &v, &seq, &row, &device, &data)) return -1;
+  PyObject *data, *data_v = nullptr;
+  if (!PyArg_ParseTuple(args, "iiiiLLLLLLO|O", &c->c.kind, &c->c.nseq, &c->c.kv_heads, &c->c.head_dim, &ctx, &k, &v, &seq, &row, &device, &data, &data_v)) return -1;
+  if (!THPVariable_Check(data) || (data_v && !THPVariable_Check(data_v))) { PyErr_SetString(PyExc_TypeError, "data must be tensors"); return -1; }
   Py_INCREF(data);
+  Py_XINCREF(data_v);
   Py_XDECREF(c->data);
-  c->data = data; c->item = c->c.kind == QPH_Q4 ? 1 : 2;
+  Py_XDECREF(c->data_v);
+  c->data = data; c->data_v = data_v; c->item = c->c.kind == QPH_Q4 ? 1 : 2;
   c->c.ctx = ctx; c->c.k = (void *)k; c->c.v = (void *)v; c->c.seq = seq; c->c.row = row; c->device = device;
   return 0;
 }
 void dealloc(PyObject *self) {
   Py_XDECREF(((Cache *)self)->data);
+  Py_XDECREF(((Cache *)self)->data_v);
   Py_TYPE(self)->tp_free(self);
 }
 

@@ -74,7 +74,7 @@ class KvCache:
         if first.device.type != "cuda":
             raise QphError("kv: the cache must be on a GPU")
         self.data, self.device = data, first.device
-        self._c = _binding().Cache(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx, *at, self.device.index, first)
+        self._c = _binding().Cache(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx, *at, self.device.index, *tensors)
 
     def write(self, k, v, pos, lens=None):
         """round the rows k and v [nseq, n, kv_heads, head_dim] into the cache"""
