@@ -16,7 +16,10 @@ def _binding():
     if _bind is None:
         import torch
         lib()   # the library, with its message where it has not been built
-        from . import _kvbind
+        try:
+            from . import _kvbind
+        except ImportError as e:
+            raise QphError(f"kv: the compiled binding (_kvbind.so) was not built, or for another torch than {torch.__version__}: run make in qpack_amd/csrc ({e})") from e
         _kvbind.setup(QphError, torch._C._cuda_getCurrentRawStream, torch.cuda.current_device, torch.cuda.device)
         _bind = _kvbind
     return _bind

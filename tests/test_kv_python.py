@@ -57,3 +57,14 @@ def test_strides_of_single_axes_mean_nothing():
     for shape, a, b in (((2, 20, 1, 64), (1280, 64, 1, 1), (1344, 64, 1, 1)), ((1, 20, 2, 64), (0, 128, 64, 1), (0, 128, 0, 1))):
         with pytest.raises(qa.QphError, match="equal strides"):
             cache(k.as_strided(shape, a), k.as_strided(shape, b), shape[0], shape[2], 64, shape[1])
+
+
+def test_a_binding_that_is_not_built_is_named(monkeypatch):
+    import sys
+
+    from qpack_amd import kvcache
+    monkeypatch.setattr(kvcache, "_bind", None)
+    monkeypatch.setitem(sys.modules, "qpack_amd._kvbind", None)
+    monkeypatch.delattr(qa, "_kvbind", raising=False)
+    with pytest.raises(qa.QphError, match="was not built"):
+        kvcache._binding()
