@@ -125,7 +125,8 @@ int qph_set_order(qph_model *m, int mode);
 
 /* ---- long conversations (no reference counterpart)
  * qph_set_cache: what the model's key / value cache holds, QPH_F16 (as created) or QPH_Q4: 4-bit records (described at qph_kv below), 9 / 32
- * of the bytes, rounded as they are written, whatever the length of a prompt's chunks.  At position 0 only.
+ * of the bytes (and at most 8 MiB for snapshots), rounded as they are written, whatever the length of a prompt's chunks.  At position 0 only; both
+ * caches are in memory while it changes.
  * qph_set_window: with window > 0 a token attends to the last `window` positions, its own among them, and to the first `sinks`; 0: to all of
  * them.  Takes effect for the next call; every position stays in the cache, so the window can be widened again.
  * Either needs arithmetic order 0.  prefill_all then takes decode steps; snapshots keep the reference's fp16 layout, which a 4-bit

@@ -36,7 +36,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
-constexpr int kRec = 8;   // positions of a record
+constexpr int kRec = kKvRec;   // positions of a record
 
 __device__ __forceinline__ float bf16_to_f(uint16_t h) { return __builtin_bit_cast(float, (uint32_t)h << 16); }
 // round to nearest even; NaN stays NaN

@@ -296,7 +296,8 @@ hipError_t launch_pf_attn(const PfAttnArgs &a, hipStream_t st);
 enum RowType : int { RT_F32 = 0, RT_F16 = 1, RT_BF16 = 2 };
 struct KvRows { void *p; int type; int64_t seq, tok, head; };   // strides in elements; a head's dims are consecutive
 // bytes of a sequence's records of one kv head
-inline int64_t kv4_records(int64_t ctx) { return (ctx + 7) / 8; }
+constexpr int kKvRec = 8;   // positions of a record
+inline int64_t kv4_records(int64_t ctx) { return (ctx + kKvRec - 1) / kKvRec; }
 inline int64_t kv4_bytes(int nseq, int nkv, int hd, int64_t ctx) { return (int64_t)nseq * nkv * kv4_records(ctx) * 9 * hd; }
 // rows k / v of tokens 0 .. lens[b] - 1 (n without lens) of sequence b <-> positions pos[b] .. below ctx; pos[b] < 0: none
 struct KvIoArgs {

@@ -341,13 +341,13 @@ void HipLlama::set_cache(int kind) {
   check_status();
   // the new buffers first: where they do not fit, the model goes on as it was
   if (kind == MK_Q4) {
-    const size_t layer = (size_t)kv4_bytes(1, cfg_.kv_heads, cfg_.head_dim, ctx_), row = 2ull * ctx_ * kvd_;
+    const size_t layer = (size_t)kv4_bytes(1, cfg_.kv_heads, cfg_.head_dim, ctx_);
     uint8_t *rec = nullptr;
     uint16_t *stage = nullptr;
     int *zero = kv_zero_;
     try {
       rec = (uint8_t *)dalloc(layer * cfg_.layers);
-      stage = (uint16_t *)dalloc(2 * row);
+      stage = (uint16_t *)dalloc(4ull * stage_rows() * kvd_);
       if (!zero) { zero = (int *)dalloc(sizeof(int)); kv_zero_ = zero; QPH_CK(hipMemsetAsync(zero, 0, sizeof(int), st_)); }
       QPH_CK(hipMemsetAsync(rec, 0, layer * cfg_.layers, st_));
       kv_buffers(kind);
@@ -917,10 +917,16 @@ void HipLlama::set_pos(int pos) {
   pos_ = pos; clean_pos_ = std::min(clean_pos_, pos);
 }
 
-// positions 0 .. n - 1 of a 4-bit layer against the fp16 rows in kv_stage_
-KvIoArgs HipLlama::stage_io(int l, int n) const {
+// positions of a slice of a 4-bit layer that kv_stage_ holds as fp16 rows, K then V: whole records
+int HipLlama::stage_rows() const {
+  const int64_t most = std::max<int64_t>(kKvRec, (int64_t)(kStageBytes / (4 * kvd_)) / kKvRec * kKvRec);
+  return (int)std::min<int64_t>(most, ctx_);
+}
+// positions p0 .. p0 + n - 1 of a layer, p0 a slice's first one, against the rows in kv_stage_
+KvIoArgs HipLlama::stage_io(int l, int p0, int n) const {
   KvIoArgs a = kv_io(l, nullptr, nullptr, n);
-  a.k = KvRows{kv_stage_, RT_F16, 0, kvd_, cfg_.head_dim}; a.v = KvRows{kv_stage_ + (size_t)ctx_ * kvd_, RT_F16, 0, kvd_, cfg_.head_dim};
+  a.cache = (uint8_t *)a.cache + (size_t)(p0 / kKvRec) * 9 * cfg_.head_dim; a.ctx = ctx_ - p0;   // (a head's records are nrec apart as before)
+  a.k = KvRows{kv_stage_, RT_F16, 0, kvd_, cfg_.head_dim}; a.v = KvRows{kv_stage_ + (size_t)stage_rows() * kvd_, RT_F16, 0, kvd_, cfg_.head_dim};
   a.pos = kv_zero_;
   return a;
 }
@@ -929,31 +935,55 @@ void HipLlama::snapshot(uint8_t *buf, int64_t cap) {
   if (cap < snapshot_size()) throw std::runtime_error("snapshot buffer too small");
   { QPH_CK(hipStreamSynchronize(st_)); check_status(); }
   memcpy(buf, &pos_, 4);
-  // pieces of the snapshot's body gathered into the pinned slots ahead, copied to the caller's memory in turn
+  if (pos_ == 0) return;
   const size_t nb = (size_t)pos_ * kvd_ * 2;
-  auto fetch = [&](const uint16_t *kc, const uint16_t *vc, int layers, uint8_t *dst) {
-    const size_t total = 2 * nb * layers, pieces = (total + kSnapSlot - 1) / kSnapSlot;
-    auto gather = [&](size_t i) {
-      const size_t o = i * kSnapSlot;
-      QPH_CK(launch_cache_gather(kc, vc, (size_t)ctx_ * kvd_ * 2, nb, o, std::min(total - o, kSnapSlot), snap_host_ + i % kSnapSlots * kSnapSlot, st_));
+  // pieces of the snapshot's body gathered into the pinned slots ahead, copied to the caller's memory in turn: gather(i, slot) enqueues
+  // piece i, take(i, slot) copies it
+  auto through_slots = [&](size_t pieces, auto gather, auto take) {
+    auto next = [&](size_t i) {
+      gather(i, snap_host_ + i % kSnapSlots * kSnapSlot);
       QPH_CK(hipEventRecord(snap_ev_[i % kSnapSlots], st_));
     };
-    for (size_t i = 0; i < std::min(pieces, kSnapSlots); i++) gather(i);
+    for (size_t i = 0; i < std::min(pieces, kSnapSlots); i++) next(i);
     for (size_t i = 0; i < pieces; i++) {
-      const size_t o = i * kSnapSlot;
       QPH_CK(hipEventSynchronize(snap_ev_[i % kSnapSlots]));
-      memcpy(dst + o, snap_host_ + i % kSnapSlots * kSnapSlot, std::min(total - o, kSnapSlot));
-      if (i + kSnapSlots < pieces) gather(i + kSnapSlots);
+      take(i, snap_host_ + i % kSnapSlots * kSnapSlot);
+      if (i + kSnapSlots < pieces) next(i + kSnapSlots);
     }
   };
-  if (pos_ == 0) return;
   try {
-    if (kv_kind_ != MK_Q4) fetch(kc_, vc_, cfg_.layers, buf + 4);
-    else
-      for (int l = 0; l < cfg_.layers; l++) {   // the layer's values as fp16 rows (exact), then as above
-        QPH_CK(launch_kv_read(MK_Q4, stage_io(l, pos_), st_));
-        fetch(kv_stage_, kv_stage_ + (size_t)ctx_ * kvd_, 1, buf + 4 + 2 * nb * l);
-      }
+    if (kv_kind_ != MK_Q4) {
+      const size_t total = 2 * nb * cfg_.layers;
+      auto len = [&](size_t i) { return std::min(total - i * kSnapSlot, kSnapSlot); };
+      through_slots((total + kSnapSlot - 1) / kSnapSlot,
+                    [&](size_t i, uint8_t *slot) { QPH_CK(launch_cache_gather(kc_, vc_, (size_t)ctx_ * kvd_ * 2, nb, i * kSnapSlot, len(i), slot, st_)); },
+                    [&](size_t i, const uint8_t *slot) { memcpy(buf + 4 + i * kSnapSlot, slot, len(i)); });
+    } else {
+      // slices of a layer's values as fp16 rows (exact), each in `per` pieces (fewer are filled of a layer's last one)
+      const int rows = stage_rows(), slices = (pos_ + rows - 1) / rows;
+      const size_t per = (4ull * rows * kvd_ + kSnapSlot - 1) / kSnapSlot;
+      struct Piece { int l, p0, n; size_t off, len, half; };   // of the slice's K rows, then V rows, `half` bytes each
+      auto piece = [&](size_t i) {
+        Piece q;
+        q.l = (int)(i / per / slices); q.p0 = (int)(i / per % slices) * rows; q.n = std::min(rows, pos_ - q.p0);
+        q.half = 2ull * q.n * kvd_; q.off = i % per * kSnapSlot;
+        q.len = q.off < 2 * q.half ? std::min(2 * q.half - q.off, kSnapSlot) : 0;
+        return q;
+      };
+      through_slots(per * slices * cfg_.layers,
+                    [&](size_t i, uint8_t *slot) {
+                      const Piece q = piece(i);
+                      if (!q.off) QPH_CK(launch_kv_read(MK_Q4, stage_io(q.l, q.p0, q.n), st_));
+                      QPH_CK(launch_cache_gather(kv_stage_, kv_stage_ + (size_t)rows * kvd_, 2ull * rows * kvd_, q.half, q.off, q.len, slot, st_));
+                    },
+                    [&](size_t i, const uint8_t *slot) {
+                      const Piece q = piece(i);
+                      uint8_t *k = buf + 4 + 2 * nb * q.l + 2ull * q.p0 * kvd_, *v = k + nb;
+                      const size_t in_k = q.off < q.half ? std::min(q.len, q.half - q.off) : 0;
+                      memcpy(k + q.off, slot, in_k);
+                      if (q.len > in_k) memcpy(v + (q.off + in_k - q.half), slot + in_k, q.len - in_k);
+                    });
+    }
   } catch (...) { (void)hipStreamSynchronize(st_); throw; }
 }
 
@@ -966,11 +996,14 @@ void HipLlama::restore(const uint8_t *buf, int64_t n) {
   { QPH_CK(hipStreamSynchronize(st_)); check_status(); }
   const uint8_t *p = buf + 4;
   if (kv_kind_ == MK_Q4) {   // rows that a 4-bit cache gave out go back as they were, others are rounded
-    for (int l = 0; l < cfg_.layers && nb; l++, p += 2 * nb) {
-      QPH_CK(hipMemcpyAsync(kv_stage_, p, nb, hipMemcpyHostToDevice, st_));
-      QPH_CK(hipMemcpyAsync(kv_stage_ + (size_t)ctx_ * kvd_, p + nb, nb, hipMemcpyHostToDevice, st_));
-      QPH_CK(launch_kv_write(MK_Q4, stage_io(l, pos), st_));
-    }
+    for (int l = 0; l < cfg_.layers; l++, p += 2 * nb)
+      for (int p0 = 0; p0 < pos; p0 += stage_rows()) {
+        const int m = std::min(stage_rows(), pos - p0);
+        const size_t at = 2ull * p0 * kvd_, bytes = 2ull * m * kvd_;
+        QPH_CK(hipMemcpyAsync(kv_stage_, p + at, bytes, hipMemcpyHostToDevice, st_));
+        QPH_CK(hipMemcpyAsync(kv_stage_ + (size_t)stage_rows() * kvd_, p + nb + at, bytes, hipMemcpyHostToDevice, st_));
+        QPH_CK(launch_kv_write(MK_Q4, stage_io(l, p0, m), st_));
+      }
     QPH_CK(hipStreamSynchronize(st_));
     pos_ = pos; clean_pos_ = pos;
     return;

@@ -97,13 +97,15 @@ class HipLlama {
   bool kv_custom() const { return kv_kind_ == MK_Q4 || window_ > 0; }
   uint8_t *kv4_ = nullptr;        // [layers] records of all kv heads
   size_t kv4_layer_ = 0;
-  uint16_t *kv_stage_ = nullptr;  // a 4-bit cache's layer as fp16 rows, K then V: snapshots
+  uint16_t *kv_stage_ = nullptr;  // positions of a 4-bit cache's layer as fp16 rows, K then V, for snapshots
+  static constexpr size_t kStageBytes = 8 << 20;   // at most (whole records)
   int *kv_zero_ = nullptr;        // a position 0
   float *kv_part_ = nullptr;      // the attention's scratch, for the most that a step or a prompt's chunk takes
   size_t kv_part_bytes_ = 0;
   int kv_few_ = -1;               // test hook (QPH_KV_FEW at load)
   KvIoArgs kv_io(int l, float *k, float *v, int n) const;
-  KvIoArgs stage_io(int l, int n) const;
+  int stage_rows() const;
+  KvIoArgs stage_io(int l, int p0, int n) const;
   KvAttnArgs kv_attn(int l, const float *q, float *out, int n) const;
   void kv_buffers(int kind);
   void kv_append(int l, float *k, float *v, int n);
