@@ -66,6 +66,9 @@ int qph_create(const qph_config *cfg, const qph_tensor *tensors, int n_tensors, 
 /* load_model(path, max_ctx) for arch "llama" (model_llama.cpp:221-235): mmap a QPACK1/QPACK2/QPACK3 file, read
  * config.json and the manifest, upload to HBM; QPACK3's coded blobs are uploaded coded and decoded on the GPU */
 int qph_load(const char *path, int max_ctx, qph_model **out);
+/* the same with a cache of the kind that qph_set_cache takes, QPH_F16 or QPH_Q4: no memory is taken for the other one */
+int qph_create_kv(const qph_config *cfg, const qph_tensor *tensors, int n_tensors, int max_ctx, int cache, qph_model **out);
+int qph_load_kv(const char *path, int max_ctx, int cache, qph_model **out);
 /* the QPACK3 decode of the model's load: coded planes, coded / raw bytes, HIP-event times of the upload (first copy
  * to last), of the decode (first launch to last; the launches run under the upload, one per upload round) and of both,
  * and the number of upload rounds (zeros for a plain file) */
@@ -126,7 +129,7 @@ int qph_set_order(qph_model *m, int mode);
 /* ---- long conversations (no reference counterpart)
  * qph_set_cache: what the model's key / value cache holds, QPH_F16 (as created) or QPH_Q4: 4-bit records (described at qph_kv below), 9 / 32
  * of the bytes (and at most 8 MiB for snapshots), rounded as they are written, whatever the length of a prompt's chunks.  At position 0 only; both
- * caches are in memory while it changes.
+ * caches are in memory while it changes (a context that only fits in 4 bits is loaded by qph_load_kv).
  * qph_set_window: with window > 0 a token attends to the last `window` positions, its own among them, and to the first `sinks`; 0: to all of
  * them.  Takes effect for the next call; every position stays in the cache, so the window can be widened again.
  * Either needs arithmetic order 0.  prefill_all then takes decode steps; snapshots keep the reference's fp16 layout, which a 4-bit

@@ -59,7 +59,9 @@ SIGNATURES = {
     "qph_last_error": (C.c_char_p, []),
     "qph_device_count": (_I, [_IP]),
     "qph_create": (_I, [C.POINTER(Config), C.POINTER(Tensor), _I, _I, C.POINTER(_P)]),
+    "qph_create_kv": (_I, [C.POINTER(Config), C.POINTER(Tensor), _I, _I, _I, C.POINTER(_P)]),
     "qph_load": (_I, [C.c_char_p, _I, C.POINTER(_P)]),
+    "qph_load_kv": (_I, [C.c_char_p, _I, _I, C.POINTER(_P)]),
     "qph_destroy": (None, [_P]),
     "qph_vocab": (_I, [_P]),
     "qph_hidden": (_I, [_P]),

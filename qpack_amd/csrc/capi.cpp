@@ -126,20 +126,31 @@ int qph_device_count(int *n) {
   });
 }
 
+// a model's cache: MK_Q4, or MK_F32 for fp16
+static int cache_kind(int kind) {
+  if (kind != QPH_F16 && kind != QPH_Q4) throw std::invalid_argument("cache: kind must be QPH_F16 or QPH_Q4");
+  return kind == QPH_Q4 ? qph::MK_Q4 : qph::MK_F32;
+}
 int qph_create(const qph_config *cfg, const qph_tensor *tensors, int n_tensors, int max_ctx, qph_model **out) {
+  return qph_create_kv(cfg, tensors, n_tensors, max_ctx, QPH_F16, out);
+}
+int qph_create_kv(const qph_config *cfg, const qph_tensor *tensors, int n_tensors, int max_ctx, int cache, qph_model **out) {
   QPH_API_TRY({
     need(cfg, "cfg"); need(tensors, "tensors"); need(out, "out");
     *out = nullptr;
+    const int kind = cache_kind(cache);
     auto *h = new qph_model;
-    try { h->m.reset(new qph::HipLlama(*cfg, tensors, n_tensors, max_ctx)); } catch (...) { delete h; throw; }
+    try { h->m.reset(new qph::HipLlama(*cfg, tensors, n_tensors, max_ctx, kind)); } catch (...) { delete h; throw; }
     *out = h;
   });
 }
 
-int qph_load(const char *path, int max_ctx, qph_model **out) {
+int qph_load(const char *path, int max_ctx, qph_model **out) { return qph_load_kv(path, max_ctx, QPH_F16, out); }
+int qph_load_kv(const char *path, int max_ctx, int cache, qph_model **out) {
   QPH_API_TRY({
     need(path, "path"); need(out, "out");
     *out = nullptr;
+    const int kind = cache_kind(cache);
     qph::Container c(path);
     const qph::JNode &j = c.config();
     if (j.get("arch").text() != "llama") throw std::runtime_error(std::string(path) + ": arch '" + j.get("arch").text() + "' is not a Llama-family model");
@@ -163,7 +174,7 @@ int qph_load(const char *path, int max_ctx, qph_model **out) {
     }
     cfg.qkv_bias = c.get("layers.0.bq") ? 1 : 0;
     auto *h = new qph_model;
-    try { h->m.reset(new qph::HipLlama(cfg, ts.data(), (int)ts.size(), max_ctx)); } catch (...) { delete h; throw; }
+    try { h->m.reset(new qph::HipLlama(cfg, ts.data(), (int)ts.size(), max_ctx, kind)); } catch (...) { delete h; throw; }
     *out = h;
   });
 }
@@ -232,13 +243,7 @@ int qph_snapshot_size(const qph_model *m, int64_t *bytes) { QPH_API_TRY({ need(m
 int qph_snapshot(qph_model *m, uint8_t *buf, int64_t cap) { QPH_API_TRY({ need(m, "model"); need(buf, "buf"); m->m->snapshot(buf, cap); }); }
 int qph_restore(qph_model *m, const uint8_t *buf, int64_t n) { QPH_API_TRY({ need(m, "model"); need(buf, "buf"); m->m->restore(buf, n); }); }
 
-int qph_set_cache(qph_model *m, int kind) {
-  QPH_API_TRY({
-    need(m, "model");
-    if (kind != QPH_F16 && kind != QPH_Q4) throw std::invalid_argument("cache: kind must be QPH_F16 or QPH_Q4");
-    m->m->set_cache(kind == QPH_Q4 ? qph::MK_Q4 : qph::MK_F32);
-  });
-}
+int qph_set_cache(qph_model *m, int kind) { QPH_API_TRY({ need(m, "model"); m->m->set_cache(cache_kind(kind)); }); }
 int qph_set_window(qph_model *m, int window, int sinks) { QPH_API_TRY({ need(m, "model"); m->m->set_window(window, sinks); }); }
 int qph_set_order(qph_model *m, int mode) { QPH_API_TRY({ need(m, "model"); m->m->set_order(mode); }); }
 

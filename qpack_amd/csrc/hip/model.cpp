@@ -67,7 +67,7 @@ const float *HipLlama::upload_f32(const qph_tensor &t, int64_t n) {
   return (const float *)place(t.data, t.data_coded, 4ull * n, t.name);
 }
 
-HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int max_ctx) : cfg_(cfg) {
+HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int max_ctx, int cache) : cfg_(cfg) {
   const int d = cfg.hidden, nh = cfg.heads, nkv = cfg.kv_heads, hd = cfg.head_dim, ff = cfg.ffn, V = cfg.vocab;
   if (d <= 0 || cfg.layers <= 0 || nh <= 0 || nkv <= 0 || ff <= 0 || V <= 0) throw std::runtime_error("hip: bad model config");
   if (hd != 64 && hd != 128) throw std::runtime_error("hip: head_dim must be 64 or 128");
@@ -134,9 +134,7 @@ HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int 
   }
 
   counters_ = (int *)dalloc(8ull * nkv);
-  const size_t kvn = (size_t)cfg.layers * ctx_ * kvd_;
-  kc_ = (uint16_t *)dalloc(kvn * 2); vc_ = (uint16_t *)dalloc(kvn * 2);
-  QPH_CK(hipMemset(kc_, 0, kvn * 2)); QPH_CK(hipMemset(vc_, 0, kvn * 2));
+  take_cache(cache, new_cache(cache));
   x_ = (float *)dalloc(4ull * d); xn_ = (float *)dalloc(4ull * d); q_ = (float *)dalloc(4ull * qd_);
   k_ = (float *)dalloc(4ull * kvd_); v_ = (float *)dalloc(4ull * kvd_); att_ = (float *)dalloc(4ull * qd_);
   h_ = (float *)dalloc(4ull * ff); logits_ = (float *)dalloc(4ull * V);
@@ -257,6 +255,7 @@ HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int 
   QPH_CK(hipHostGetDevicePointer((void **)&dstatus_, hstatus_, 0));
   memset(hctl_, 0, kRing * sizeof(Ctl));
   QPH_CK(hipMemset(ctl_, 0, sizeof(Ctl)));
+  if (kv_custom()) kv_buffers(kv_kind_);
   build_graphs();
 }
 
@@ -294,7 +293,7 @@ void HipLlama::drop_graphs() {
 // ------------------------------------------------------------------ 4-bit cache, sliding window
 KvIoArgs HipLlama::kv_io(int l, float *k, float *v, int n) const {   // k / v: rows [n][kvd_] at ctl_->pos ..
   KvIoArgs a{};
-  a.cache = kv4_ + (size_t)l * kv4_layer_; a.ctx = ctx_; a.nrec = kv4_records(ctx_);
+  a.cache = kv4_ + (size_t)l * kv4_layer(); a.ctx = ctx_; a.nrec = kv4_records(ctx_);
   a.nseq = 1; a.nkv = cfg_.kv_heads; a.hd = cfg_.head_dim; a.n = n;
   a.k = KvRows{k, RT_F32, 0, kvd_, cfg_.head_dim}; a.v = KvRows{v, RT_F32, 0, kvd_, cfg_.head_dim};
   a.pos = &ctl_->pos;
@@ -303,7 +302,7 @@ KvIoArgs HipLlama::kv_io(int l, float *k, float *v, int n) const {   // k / v: r
 KvAttnArgs HipLlama::kv_attn(int l, const float *q, float *out, int n) const {
   KvAttnArgs a{};
   a.kind = kv_kind_;
-  if (kv_kind_ == MK_Q4) a.cache = kv4_ + (size_t)l * kv4_layer_;
+  if (kv_kind_ == MK_Q4) a.cache = kv4_ + (size_t)l * kv4_layer();
   else { a.cache = kc_ + (size_t)l * ctx_ * kvd_; a.cache_v = vc_ + (size_t)l * ctx_ * kvd_; }
   a.crow = kvd_; a.ctx = ctx_; a.nrec = kv4_records(ctx_);
   a.nseq = 1; a.nkv = cfg_.kv_heads; a.hd = cfg_.head_dim; a.heads = cfg_.heads; a.rep = cfg_.heads / cfg_.kv_heads; a.n = n;
@@ -333,6 +332,25 @@ void HipLlama::kv_buffers(int kind) {
     kv_part_ = p; kv_part_bytes_ = need;
   }
 }
+HipLlama::Cache HipLlama::new_cache(int kind) {   // cleared on the model's stream
+  Cache c;
+  try {
+    if (kind == MK_Q4) {
+      const size_t bytes = kv4_layer() * cfg_.layers;
+      c.rec = (uint8_t *)dalloc(bytes);
+      c.stage = (uint16_t *)dalloc(4ull * stage_rows() * kvd_);
+      QPH_CK(hipMemsetAsync(c.rec, 0, bytes, st_));
+      if (!kv_zero_) { kv_zero_ = (int *)dalloc(sizeof(int)); QPH_CK(hipMemsetAsync(kv_zero_, 0, sizeof(int), st_)); }
+    } else {
+      const size_t bytes = 2ull * cfg_.layers * ctx_ * kvd_;
+      c.k = (uint16_t *)dalloc(bytes); c.v = (uint16_t *)dalloc(bytes);
+      QPH_CK(hipMemsetAsync(c.k, 0, bytes, st_)); QPH_CK(hipMemsetAsync(c.v, 0, bytes, st_));
+    }
+  } catch (...) { free_cache(c); throw; }
+  return c;
+}
+void HipLlama::free_cache(const Cache &c) { dfree(c.k); dfree(c.v); dfree(c.rec); dfree(c.stage); }
+void HipLlama::take_cache(int kind, const Cache &c) { kv_kind_ = kind; kc_ = c.k; vc_ = c.v; kv4_ = c.rec; kv_stage_ = c.stage; }
 void HipLlama::set_cache(int kind) {
   if (kind == kv_kind_) return;
   if (pos_ != 0) throw std::runtime_error("cache: the kind can change at position 0 only");
@@ -340,36 +358,11 @@ void HipLlama::set_cache(int kind) {
   QPH_CK(hipStreamSynchronize(st_));
   check_status();
   // the new buffers first: where they do not fit, the model goes on as it was
-  if (kind == MK_Q4) {
-    const size_t layer = (size_t)kv4_bytes(1, cfg_.kv_heads, cfg_.head_dim, ctx_);
-    uint8_t *rec = nullptr;
-    uint16_t *stage = nullptr;
-    int *zero = kv_zero_;
-    try {
-      rec = (uint8_t *)dalloc(layer * cfg_.layers);
-      stage = (uint16_t *)dalloc(4ull * stage_rows() * kvd_);
-      if (!zero) { zero = (int *)dalloc(sizeof(int)); kv_zero_ = zero; QPH_CK(hipMemsetAsync(zero, 0, sizeof(int), st_)); }
-      QPH_CK(hipMemsetAsync(rec, 0, layer * cfg_.layers, st_));
-      kv_buffers(kind);
-    } catch (...) { dfree(rec); dfree(stage); throw; }
-    drop_graphs();
-    dfree(kc_); dfree(vc_);
-    kc_ = vc_ = nullptr;
-    kv4_ = rec; kv4_layer_ = layer; kv_stage_ = stage;
-  } else {
-    const size_t bytes = 2ull * cfg_.layers * ctx_ * kvd_;
-    uint16_t *k = nullptr, *v = nullptr;
-    try {
-      k = (uint16_t *)dalloc(bytes); v = (uint16_t *)dalloc(bytes);
-      QPH_CK(hipMemsetAsync(k, 0, bytes, st_)); QPH_CK(hipMemsetAsync(v, 0, bytes, st_));
-      if (window_ > 0) kv_buffers(kind);
-    } catch (...) { dfree(k); dfree(v); throw; }
-    drop_graphs();
-    dfree(kv4_); dfree(kv_stage_);
-    kv4_ = nullptr; kv_stage_ = nullptr;
-    kc_ = k; vc_ = v;
-  }
-  kv_kind_ = kind;
+  const Cache c = new_cache(kind);
+  try { if (kind == MK_Q4 || window_ > 0) kv_buffers(kind); } catch (...) { free_cache(c); throw; }
+  drop_graphs();
+  free_cache(Cache{kc_, vc_, kv4_, kv_stage_});
+  take_cache(kind, c);
   build_graphs();
 }
 void HipLlama::set_window(int window, int sinks) {

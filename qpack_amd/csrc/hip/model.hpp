@@ -17,7 +17,7 @@ namespace qph {
 
 class HipLlama {
  public:
-  HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int max_ctx);
+  HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int max_ctx, int cache = MK_F32);   // cache: as set_cache's kind
   ~HipLlama();
   HipLlama(const HipLlama &) = delete;
   HipLlama &operator=(const HipLlama &) = delete;
@@ -96,13 +96,17 @@ class HipLlama {
   int kv_kind_ = MK_F32, window_ = 0, sinks_ = 0;
   bool kv_custom() const { return kv_kind_ == MK_Q4 || window_ > 0; }
   uint8_t *kv4_ = nullptr;        // [layers] records of all kv heads
-  size_t kv4_layer_ = 0;
+  size_t kv4_layer() const { return (size_t)kv4_bytes(1, cfg_.kv_heads, cfg_.head_dim, ctx_); }
   uint16_t *kv_stage_ = nullptr;  // positions of a 4-bit cache's layer as fp16 rows, K then V, for snapshots
   static constexpr size_t kStageBytes = 8 << 20;   // at most (whole records)
   int *kv_zero_ = nullptr;        // a position 0
   float *kv_part_ = nullptr;      // the attention's scratch, for the most that a step or a prompt's chunk takes
   size_t kv_part_bytes_ = 0;
   int kv_few_ = -1;               // test hook (QPH_KV_FEW at load)
+  struct Cache { uint16_t *k = nullptr, *v = nullptr; uint8_t *rec = nullptr; uint16_t *stage = nullptr; };
+  Cache new_cache(int kind);
+  void free_cache(const Cache &c);
+  void take_cache(int kind, const Cache &c);
   KvIoArgs kv_io(int l, float *k, float *v, int n) const;
   int stage_rows() const;
   KvIoArgs stage_io(int l, int p0, int n) const;

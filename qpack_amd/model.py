@@ -26,6 +26,9 @@ _madvise = C.CDLL(None).madvise
 _madvise.restype, _madvise.argtypes = C.c_int, [C.c_void_p, C.c_size_t, C.c_int]
 
 
+_CACHES = {"f16": QPH_F16, "q4": QPH_Q4}
+
+
 class HipLlama:
     def __init__(self, handle):
         self._h = C.c_void_p(handle)
@@ -34,10 +37,10 @@ class HipLlama:
         self.config = cfg
 
     @classmethod
-    def load(cls, path, max_ctx=0):
-        """load_model(path, max_ctx) with QPACK_DEVICE selecting this backend (model_llama.cpp:221-235)"""
+    def load(cls, path, max_ctx=0, cache="f16"):
+        """load_model(path, max_ctx) with QPACK_DEVICE selecting this backend (model_llama.cpp:221-235); cache: as set_cache's kind"""
         h = C.c_void_p()
-        check(lib().qph_load(str(path).encode(), int(max_ctx), C.byref(h)))
+        check(lib().qph_load_kv(str(path).encode(), int(max_ctx), _CACHES.get(cache, cache), C.byref(h)))
         return cls(h.value)
 
     def close(self):
@@ -127,8 +130,7 @@ class HipLlama:
 
     def set_cache(self, kind):
         """what the key / value cache holds, "f16" or "q4" (4-bit records, 9 / 32 of the bytes); at position 0 only"""
-        kinds = {"f16": QPH_F16, "q4": QPH_Q4}
-        check(lib().qph_set_cache(self._h, kinds.get(kind, kind)))
+        check(lib().qph_set_cache(self._h, _CACHES.get(kind, kind)))
 
     def set_window(self, window, sinks=0):
         """attend to the last `window` positions and the first `sinks`; window 0: to all of them"""

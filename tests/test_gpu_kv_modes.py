@@ -55,3 +55,28 @@ def test_a_4_bit_cache_takes_9_of_32_parts(synth):
         assert gained >= f16 * 23 // 32 - 40 * mib, f"{gained / mib:.0f} MiB of {f16 / mib:.0f}"
         m.set_cache("f16")
         assert abs(free() - before) <= 40 * mib
+
+
+def test_loaded_with_a_4_bit_cache(synth):
+    """as set afterwards, without the fp16 cache's memory at any time"""
+    ctx, mib, toks = 1 << 18, 1 << 20, np.random.default_rng(5).integers(0, 2048, 60).astype(np.int32)
+    f16 = 2 * 2 * ctx * 128 * 2
+    used = {}
+    for kind in ("f16", "q4"):
+        before = free()
+        with qa.HipLlama.load(synth("mini128"), max_ctx=ctx, cache=kind) as m:
+            used[kind] = before - free()
+            if kind == "f16":
+                m.set_cache("q4")
+                want = m.prefill(toks), m.step(3), m.greedy_run(4, 9)
+            else:
+                for a, b in zip(want, (m.prefill(toks), m.step(3), m.greedy_run(4, 9))):
+                    np.testing.assert_array_equal(a, b)
+                m.reset()
+                m.set_cache("f16")
+                default = m.prefill(toks), m.step(3)
+                m.set_order(1)
+    assert used["f16"] - used["q4"] >= f16 * 23 // 32 - 40 * mib, {k: v // mib for k, v in used.items()}
+    with qa.HipLlama.load(synth("mini128"), max_ctx=ctx) as m:
+        for a, b in zip(default, (m.prefill(toks), m.step(3))):
+            np.testing.assert_array_equal(a, b)

@@ -42,3 +42,11 @@ def test_over_q_in_other_places_is_refused():
     one = lambda **k: cache(ctx=4096, kv_heads=1, **k)   # noqa: E731
     for q, out, n, c in ((rows(), rows(), 3, one()), (rows(), rows(tok=7), 1, one()), (rows(), rows(seq=9), 3, one(nseq=1)), (rows(tok=0), rows(p=2 * P), 3, one())):
         refused(attend(c, q=q, out=out, n=n), "work")   # taken: the next check is what refuses
+
+
+def test_cache_kinds_of_models_are_checked_first():
+    m = C.c_void_p()
+    for kind in (qa.QPH_F32, qa.QPH_Q8, qa.QPH_BF16, -1):
+        refused(lib().qph_load_kv(b"/nonexistent", 0, kind, C.byref(m)), "cache: kind")
+        assert m.value is None
+    assert lib().qph_load_kv(b"/nonexistent", 0, qa.QPH_Q4, C.byref(m)) == -1 and "kind" not in lib().qph_last_error().decode()
