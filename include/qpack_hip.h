@@ -133,7 +133,8 @@ int qph_set_order(qph_model *m, int mode);
  * qph_set_window: with window > 0 a token attends to the last `window` positions, its own among them, and to the first `sinks`; 0: to all of
  * them.  Takes effect for the next call; every position stays in the cache, so the window can be widened again.
  * Either needs arithmetic order 0.  prefill_all then takes decode steps; snapshots keep the reference's fp16 layout, which a 4-bit
- * cache's values fit exactly (restoring one's own snapshot restores the cache; other rows are rounded). */
+ * cache's values fit exactly (restoring one's own snapshot restores the cache, but for groups whose largest is below 2.4e-6: see qph_kv; other rows
+ * are rounded). */
 int qph_set_cache(qph_model *m, int kind);
 int qph_set_window(qph_model *m, int window, int sinks);
 
@@ -202,7 +203,7 @@ int qph_pack(const char *src, const char *dst, int threads, int *coded);
  * QPH_Q4: k points to qph_kv_bytes bytes (16-byte aligned), v, seq and row unused: per sequence, kv head and 8 positions one record of 9
  * head_dim bytes.  32 dims of one position share a scale: a = max |x| of them, s = fp16(bf16(min(a, 65504) / 7)), code =
  * clamp(rint(x / s), -7, 7) + 8 (8 when s is 0), value = (code - 8) * s, which fp16 holds exactly; a group with a NaN or
- * an infinity has a NaN scale.  In a record:
+ * an infinity has a NaN scale.  Rows read back and written again are the same where s is 7 x 2^-24 or more (a of 2.4e-6); smaller scales are rounded anew.  In a record:
  *   K codes  position i at bytes i head_dim / 2; its 32-bit word w holds dims 8 w .. 8 w + 7, dim 8 w + 2 e + o at bits 16 o + 4 e
  *   V codes  at 4 head_dim: dim d in word (d % 16) (head_dim / 16) + d / 16, position 2 e + o at bits 16 o + 4 e
  *   K scales at 8 head_dim: fp16 [8 positions][head_dim / 32];  V scales at 8.5 head_dim: fp16 [head_dim / 32][8 positions]

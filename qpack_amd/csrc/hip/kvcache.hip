@@ -4,8 +4,10 @@
 // The 4-bit cache.  Each 32 dims of one position's K (V) row share an fp16 scale s: a = max |x|, s = fp16(bf16(min(a, 65504)
 // / 7)), code = clamp(rint(x / s), -7, 7) + 8.  s has 8 significant bits and code - 8 three, so every value (code - 8) s is an
 // fp16 number: the matrix cores' operands, the rows read back and an fp16 snapshot are exact, and a row read back and
-// written again gives the same values.  Rounding s to 8 bits costs at most 2^-9 of it, the codes' step is 2^-3.  A
-// group that holds a NaN or an infinity has a NaN scale and reads back as NaN.
+// written again gives the same values, as long as s is 7 x 2^-24 or more: the largest code is then 7, and 7 s / 7 is s again.  (Groups
+// whose largest is below 2.4e-6 have scales of a few of fp16's least steps; a largest of 10.7 of them gets s = 2 and code 5, which
+// written again is s = 1 and, clamped, 7.)  Rounding s to 8 bits costs at most 2^-9 of it, the codes' step is 2^-3.  A group that holds
+// a NaN or an infinity has a NaN scale and reads back as NaN.
 //
 // One record of 9 HD bytes holds 8 positions of one (sequence, kv head); records follow each other in position order:
 //   [0, 4 HD)         K codes: position i at i HD / 2, a row's 32-bit word w = dims 8 w ..: dim 8 w + 2 e + o at bits 16 o + 4 e

@@ -9,7 +9,7 @@ import qpack_amd as qa
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_kv import BF16, F16, F32, TYPES, filled, i32, reference, route  # noqa: E402, F401
+from test_gpu_kv import BF16, F16, F32, TYPES, filled, held, i32, reference, route  # noqa: E402, F401
 
 
 def check_loud(got, q, K, V, P0, **mask):
@@ -146,3 +146,46 @@ def test_infinite_values(type, n, where, window, route):
             got[..., [5, 9]] = 0
             W[..., [5, 9]] = 0
         check_loud(got, q[0, t:t + 1], K[0], W, past + t, window=window)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+def test_rows_written_again_from_the_smallest_scales_on(type):
+    """scales of a few of fp16's least steps are rounded anew, from 7 of them on rows stay as they are"""
+    step = 2.0 ** -24
+    tops = torch.cat([torch.arange(1, 64 * 60) / 64, torch.arange(60, 4000, 7).float()])   # groups' largest values in steps
+    x = torch.zeros(1, len(tops), 1, 64)
+    x[0, :, 0, 3], x[0, :, 0, 40] = tops * step, -tops * step
+    x[0, :, 0, 9], x[0, :, 0, 50] = tops * step * 0.4, tops * step * 0.7
+    x = x.to(TYPES[type])
+    n, pos = x.shape[1], i32([0])
+    a, b = qa.KvCache("q4", 1, 1, 64, n), qa.KvCache("q4", 1, 1, 64, n)
+    a.write(x.cuda(), x.cuda(), pos)
+    once = a.read(pos, n, dtype=F32)
+    assert all(torch.equal(r.cpu(), held(x).float()) for r in once)
+    b.write(*(r.to(TYPES[type]) if type != "bf16" else r for r in once), pos)
+    again = b.read(pos, n, dtype=F32)
+    assert all(torch.equal(r.cpu(), held(once[0].cpu()).float()) for r in again)
+    s = (x.float().abs().amax(-1) / 7).to(BF16).half().float()[0, :, 0] / step   # both groups' scales
+    same = (once[0] == again[0]).all(-1).cpu()[0, :, 0]
+    assert bool(same[s >= 7].all())
+    assert set(s[~same].tolist()) <= {2.0, 4.0, 5.0, 6.0} and (type == "bf16" or not bool(same.all()))
+    if type == "f32":   # a largest of 10.7 steps: 2 x 5, then 1 x 7
+        x = torch.full((1, 1, 1, 64), 10.7 * step)
+        a.write(x.cuda(), x.cuda(), pos)
+        r = a.read(pos, 1, dtype=F32)
+        assert bool((r[0] == 10 * step).all())
+        a.write(*r, pos)
+        assert bool((a.read(pos, 1, dtype=F32)[0] == 7 * step).all())
+
+
+def test_single_axes_with_strides_of_no_meaning():
+    gen = torch.Generator().manual_seed(23)
+    k = torch.randn(1, 40, 2, 64, generator=gen).half().cuda()
+    data = [x.as_strided((1, 40, 2, 64), st) for x, st in ((k.clone(), (3, 128, 64, 1)), (k.flip(1).contiguous(), (0, 128, 64, 1)))]
+    c = qa.KvCache("f16", 1, 2, 64, 40, data=data)
+    q = torch.randn(1, 5, 4, 64, generator=gen).half().cuda()
+    check_loud(c.attention(q, i32([35]))[0], q[0], data[0][0].cpu().double(), data[1][0].cpu().double(), 35)
+    one = qa.KvCache("f16", 3, 1, 64, 1)
+    x = torch.randn(3, 1, 1, 64, generator=gen).half().cuda()
+    one.write(x, x * 2, i32([0, 0, 0]))
+    assert torch.equal(one.attention(x, i32([0, 0, 0])), x * 2)
