@@ -7,7 +7,7 @@ import qpack_amd as qa
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_kv_model import held  # noqa: E402
+from test_gpu_kv_model import ATOL, Plain, cached, check, held  # noqa: E402
 
 
 @pytest.mark.parametrize("few", ["0", "100000"])
@@ -80,3 +80,68 @@ def test_loaded_with_a_4_bit_cache(synth):
     with qa.HipLlama.load(synth("mini128"), max_ctx=ctx) as m:
         for a, b in zip(default, (m.prefill(toks), m.step(3))):
             np.testing.assert_array_equal(a, b)
+
+
+def forward(ref, toks, seen, kind, cache=None):
+    """every position's logits in 64 bits, where row t of the mask `seen` is what token t attends to: what later tokens find of it in the cache
+    depends on the mask in force when it ran.  cache: the values that the attention reads, each layer's (K, V), in place of the rounded rows: a
+    4-bit code moves by a whole step where the path's fp32 key and the 64-bit one lie on two sides of a border, which a narrow window
+    does not average out.  They are to lie within half a step of the rows (the scale's 2^-9 of 7 steps more) and 2e-3 for the path's own error"""
+    c, w, n = ref.c, ref.w, len(toks)
+    H, G, D = c["num_attention_heads"], c["num_key_value_heads"], c["head_dim"]
+    norm = lambda x, g: x / torch.sqrt((x * x).mean(-1, keepdim=True) + c["rms_norm_eps"]) * g   # noqa: E731
+    ang = torch.arange(n).double()[:, None] / c["rope_theta"] ** (torch.arange(D // 2).double() * 2 / D)
+    cs, sn = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
+    rope = lambda x: torch.cat([x[..., :D // 2] * cs - x[..., D // 2:] * sn, x[..., D // 2:] * cs + x[..., :D // 2] * sn], -1)   # noqa: E731
+    x = w["embed"][torch.from_numpy(np.asarray(toks)).long()]
+    for i in range(c["num_hidden_layers"]):
+        g = lambda s: w[f"layers.{i}.{s}"]   # noqa: E731
+        y = norm(x, g("attn_norm"))
+        q, k, v = (y @ g("w" + s).T + (g("b" + s) if c["qkv_bias"] else 0) for s in "qkv")
+        q, k, v = rope(q.view(n, H, D)), rope(k.view(n, G, D)), v.view(n, G, D)
+        if cache is not None:
+            for mine, theirs in zip((k, v), cache[i]):
+                step = mine.unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True) / 7
+                assert bool(((theirs - mine).unflatten(-1, (-1, 32)).abs() <= step * (0.5 + 2.0 ** -6) + 2e-3).all()), f"layer {i}: a cached row"
+            k, v = cache[i]
+        else:
+            k, v = (held(k), held(v)) if kind == "q4" else (k.half().double(), v.half().double())
+        a = torch.matmul(q.transpose(0, 1), k.repeat_interleave(H // G, 1).permute(1, 2, 0)) / D ** 0.5
+        a = torch.softmax(a.masked_fill(~seen, -torch.inf), -1)
+        x = x + torch.matmul(a, v.repeat_interleave(H // G, 1).transpose(0, 1)).transpose(0, 1).reshape(n, H * D) @ g("wo").T
+        y = norm(x, g("ffn_norm"))
+        u = y @ g("w_gate").T
+        x = x + (u * torch.sigmoid(u) * (y @ g("w_up").T)) @ g("w_down").T
+    return (norm(x, w["final_norm"]) @ (w["embed"] if c["tie_embeddings"] else w["lm_head"]).T).numpy()
+
+
+@pytest.mark.parametrize("cfg,kind", [("mini", "f16"), ("mini128", "f16"), ("mini", "q4")])
+def test_narrowing_and_widening_a_window(cfg, kind, synth):
+    """each change takes effect for the next call, in steps, greedy steps and prompts, and every position stays in the cache"""
+    ref = Plain(synth(cfg))
+    toks = np.random.default_rng(9).integers(0, 1000, 110).astype(np.int32)
+    phases = [(60, 0, 0), (66, 9, 2), (70, 30, 0), (82, 5, 1), (86, 0, 0), (98, 12, 4), (104, 1, 0), (110, 0, 0)]   # up to which token, window, sinks
+    P, p = torch.arange(110)[:, None], torch.arange(110)[None]
+    seen, full = p <= P, p <= P
+    at = 0
+    for upto, window, sinks in phases:
+        if window:
+            seen[at:upto] &= (p > P[at:upto] - window) | (p < sinks)
+        at = upto
+    got, modes = {}, {}
+    with qa.HipLlama.load(synth(cfg), max_ctx=128, cache=kind) as m:
+        at = 0
+        for upto, window, sinks in phases:
+            m.set_window(window, sinks)
+            if upto - at > 8:   # a prompt; the rest by steps
+                got[upto - 1] = m.prefill(toks[at:upto])
+            else:
+                got.update((i, m.step(int(toks[i]))) for i in range(at, upto))
+            modes.update((i, (window, sinks)) for i in range(at, upto))
+            at = upto
+        held_rows = cached(m, ref) if kind == "q4" else None
+    want, plain = forward(ref, toks, seen, kind, held_rows), forward(ref, toks, full, kind)
+    for i, row in got.items():
+        check(row, want[i], f"token {i}, window and sinks {modes[i]}")
+        if modes[i][0]:
+            assert np.abs(want - plain)[i].max() > 3 * ATOL   # the window shows
