@@ -575,13 +575,14 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   __shared__ float wm[NW][NC], wl[NW][NC];
   const int b = blockIdx.z, g = a.nchunk == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nchunk, chunk = blockIdx.y - g * a.nchunk, c0 = chunk * NC, split = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-  const int col = c0 + (TWO ? lr & 7 : lr), tok = token_of(a, col), hr = col - tok * a.rep;
+  // columns past the call's last are that one again: another row may be another workgroup's, whose results may be on their way into it (out may
+  // be q).  (Zeros without a load, or the first column's row: 0.3 us of a short call)
+  const int col = min(c0 + (TWO ? lr & 7 : lr), a.n * a.rep - 1), tok = token_of(a, col), hr = col - tok * a.rep;
   // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j.  Asked for before
-  // the sequence's position is known.  Columns past the call's last token are zeros: any row that is there may be another workgroup's,
-  // whose results may be on their way into it (out may be q)
-  h8 q[KS] = {};
-  float x[KS][8] = {};
-  if (tok < a.n) {
+  // the sequence's position is known
+  h8 q[KS];
+  float x[KS][8];
+  {
     const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)(g * a.rep + hr) * a.q.head;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
@@ -760,7 +761,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
 #pragma unroll
       for (int i = 0; i < 4; i++) {   // an infinite V: as the scores, hi's sum where only lo's makes it NaN
         const float both = y[i] + xchg8_f(y[i]);
-        y[i] = both != both && fabsf(y[i]) == INFINITY ? y[i] : both;
+        y[i] = KIND != MK_Q4 && both != both && fabsf(y[i]) == INFINITY ? y[i] : both;
       }
     }
     if (lr < NC) *(f32x4 *)(ored + (wave * NC + lr) * QS + 16 * d + 4 * lg) = y;
@@ -897,8 +898,9 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, ln = lane & 31, hf = lane >> 5;
   // waves w and w + 4 share a SIMD: one of the front half, one of the back half
   const int cw = chunk_half(a, chunk, wave / (kManyWaves / 2)) + 32 * (wave % (kManyWaves / 2));
-  const int col = cw + ln, tok = token_of(a, col), head = g * a.rep + col - tok * a.rep;
-  const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
+  // (columns past the last read its query, as in k_kv_few; a wave without any other takes no block and uses none of it)
+  const int col = min(cw + ln, a.n * a.rep - 1), tok = token_of(a, col), head = g * a.rep + col - tok * a.rep;
+  const bool live = col == cw + ln && tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? s.P0 + tok : -1;
   const int lo = behind(a, P);
   // first and last position of the wave's own columns, and of the halves'
@@ -1009,20 +1011,15 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (kb0 + 1 < kb1) fetch(kb0 + 1, st1);
     // ---- queries
     {
-      // (columns past the last token are zeros, as in k_kv_few)
-      float x[KQ][8] = {}, mx = 0.f;
+      const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
+      float x[KQ][8], mx = 0.f;
 #pragma unroll
-      for (int k = 0; k < KQ; k++) q[k] = (h8)(_Float16)0.f;
-      if (tok < a.n) {
-        const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
+      for (int k = 0; k < KQ; k++) {
+        if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
+        else {
+          load_elems<T, 8>(a.q, at + 16 * k, x[k]);
 #pragma unroll
-        for (int k = 0; k < KQ; k++) {
-          if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
-          else {
-            load_elems<T, 8>(a.q, at + 16 * k, x[k]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
-          }
+          for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
         }
       }
       if constexpr (T != RT_F16) {
