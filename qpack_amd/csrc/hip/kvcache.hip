@@ -1190,15 +1190,16 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (tid < 2) badp[(kb - kb0 + 3) % 4][tid] = 0;
     __syncthreads();
   }
+  l = pair_sum32(l);
   if constexpr (TWO && KIND != MK_Q4) {
     // An infinite V: the lo halves (0, or of either sign) turn the sum into NaN.  Such sums are what the values say that are not finite and
-    // that the column sees, read again.  (A score that is NaN shows in l)
+    // that the column sees, read again.  (Where l is NaN a score was, and the row is)
     bool nan = false;
 #pragma unroll
     for (int t = 0; t < OT; t++)
 #pragma unroll
       for (int i = 0; i < 16; i++) nan |= o[t][i] != o[t][i];
-    if (__any((int)live & (int)nan)) {
+    if (__any((int)live & (int)nan & (int)(l == l))) {
 #pragma unroll
       for (int t = 0; t < OT; t++)
 #pragma unroll
@@ -1215,7 +1216,6 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       }
     }
   }
-  l = pair_sum32(l);
   if constexpr (T != RT_F32) {
     if (s.S == 1) {
       // A lane has 4 dims here and there of its column; by way of the wave's own part of LDS the rows leave in 16-byte pieces
