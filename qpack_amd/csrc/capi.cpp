@@ -111,7 +111,9 @@ static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sink
   a.window = window; a.sinks = sinks; a.few = qph::kv_few();
 }
 static void hck(hipError_t e, const char *what) {
-  if (e != hipSuccess) throw std::runtime_error(std::string("hip: ") + hipGetErrorString(e) + " (" + what + ")");
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();   // as QPH_CK
+  throw std::runtime_error(std::string("hip: ") + hipGetErrorString(e) + " (" + what + ")");
 }
 
 extern "C" {
@@ -121,7 +123,7 @@ const char *qph_last_error(void) { return g_err.c_str(); }
 int qph_device_count(int *n) {
   QPH_API_TRY({
     need(n, "n"); int c = 0;
-    if (hipGetDeviceCount(&c) != hipSuccess) c = 0;
+    if (hipGetDeviceCount(&c) != hipSuccess) { (void)hipGetLastError(); c = 0; }
     *n = c;
   });
 }

@@ -326,7 +326,8 @@ __global__ __launch_bounds__(128) void k_kv4_read(KvIoArgs a) {
   store_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x);
 }
 
-// the fp16 cache's: a copy with a conversion, 8 dims of one position's K or V a thread.  Bound by memory, or by the launch
+// the fp16 cache's: a copy with a conversion, 8 dims of one position's K or V a thread.  Bound by memory: 16 sequences
+// of 16384 positions, 8 heads of 128 dims, 347 us either way (6.2 TB/s read and written; fp32 rows 5.9); 2048 positions by the launch (4 to 6 us)
 template <bool WRITE, int T>
 __global__ __launch_bounds__(256) void k_kv16_io(KvIoArgs a) {
   const int b = blockIdx.z, per = a.nkv * a.hd / 8;
@@ -366,7 +367,9 @@ struct Span {
   bool any;
 };
 // The columns of a chunk: a.cols from chunk * a.cols on, or, paired (many tokens, no window), half of them from the front and half from
-// the back.  A causal workgroup's time goes with its last position: paired, all take about as long (see k_kv_many)
+// the back.  In a prompt a workgroup's time goes with its last position, and pairs take more alike: 2048 tokens of 32 heads 65 -> 55 us (fp32
+// 105 -> 88).  Behind a long past there is nothing to even out, and pairs change nothing: 77 tokens of 28 heads at 16000 44 us either way, with 4, 5
+// and 8 of a workgroup's waves at work, by the columns that its halves have
 __device__ __forceinline__ int chunk_half(const KvAttnArgs &a, int chunk, int h) {   // the first column of half h
   return (a.paired ? (h ? 2 * a.nchunk - 1 - chunk : chunk) : 2 * chunk + h) << a.half_log2;
 }
@@ -875,7 +878,8 @@ __global__ __launch_bounds__(256) void k_kv_merge_rows(KvAttnArgs a) {
 // A step of 64 positions takes a wave 32 products (1024 cycles of its SIMD's matrix core, two waves a SIMD), some 130 vector instructions and,
 // for 4-bit, 60 that expand; the 8 waves read 256 KiB of LDS, 2048 cycles at its 128 bytes a cycle.  The three overlap in part only:
 // 2048 tokens of 32 heads over a 4-bit cache 56 to 64 us by machine (620 TFLOP/s of the 1149 that a large fp16 product reaches), 4096
-// tokens with a window of 1024 in fp16 95 to 102 us.  256 columns a workgroup, since what a block costs to expand and its LDS writes are
+// tokens with a window of 1024 in fp16 95 to 102 us; fp32 rows, with twice the products, 88 and 150 (over an fp16 cache the 128-dim kernel has all
+// 256 registers and spills 4).  256 columns a workgroup, since what a block costs to expand and its LDS writes are
 // shared by them: with 128 columns and two workgroups a CU the 4-bit prompt took 77 us for 64, the fp16 one 97 for 100, and 64
 // tokens each of 32 sequences 6 % more
 constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
@@ -1320,7 +1324,10 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   // alone up to 256 columns, and it takes some 6 us longer to start.  Chunks up to which the first is faster, from both kernels' times at
   // 12 to 640 columns, 1 and 8 sequences of 256 to 16384 positions, 8 kv heads of 128 dims (472 calls; the rule's choice is 1 % slower
   // than the better kernel's in the mean, a limit of 64 columns was 19 %).  4-bit: 64 columns over 8 x 4096 positions 36 us few, 37
-  // many; 128 over 8 x 16384 176 and 112; 128 over 8 x 1024 18 and 35.  fp16: the same 92 and 38, 624 and 133, 44 and 31
+  // many; 128 over 8 x 16384 176 and 112; 128 over 8 x 1024 18 and 35.  fp16: the same 92 and 38, 624 and 133, 44 and 31.
+  // Other shapes take the same constants.  8 to 512 columns over 512, 4096 and 16384 positions, 1 and 8 sequences, 42 calls each: fp32 rows 0.9 %
+  // (4-bit) and 1.8 % (fp16) slower than the better kernel's in the mean, heads of 64 dims 1.9 and 1.7, two of them with fp32 rows 1.9 and 5.3 (the
+  // worst: 256 columns over 8 x 512 fp16 positions, 22 us many for 11 few)
   const int64_t chunks = (cols + few - 1) / few, positions = (int64_t)a.nseq * a.nkv * reach(few);
   const int64_t most = a.kind == MK_Q4 ? 4 + (384 << 10) / positions : 1 + (192 << 10) / positions;
   a.many = (a.few >= 0 ? cols > a.few : chunks > std::min<int64_t>(most, 128)) || chunks * a.nkv > 65535;   // (the last: the grid)

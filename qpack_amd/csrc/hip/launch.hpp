@@ -10,10 +10,14 @@
 #include "common.hpp"
 
 // host code: throw on a failed HIP call
-#define QPH_CK(x)                                                                                           \
-  do {                                                                                                      \
-    hipError_t e_ = (x);                                                                                    \
-    if (e_ != hipSuccess) throw std::runtime_error(std::string("hip: ") + hipGetErrorString(e_) + " at " + #x); \
+// the error is reported here: left as the thread's last one, the next launch (hipGetLastError) would report it again
+#define QPH_CK(x)                                                                                             \
+  do {                                                                                                        \
+    hipError_t e_ = (x);                                                                                      \
+    if (e_ != hipSuccess) {                                                                                   \
+      (void)hipGetLastError();                                                                                \
+      throw std::runtime_error(std::string("hip: ") + hipGetErrorString(e_) + " at " + #x);                   \
+    }                                                                                                         \
   } while (0)
 
 namespace qph {

@@ -350,7 +350,7 @@ void RansBatch::run(hipStream_t st, RansTiming *tm, uint64_t round_bytes) {
     if (up) (void)hipStreamDestroy(up);
   };
   try {
-    auto ck = [](hipError_t r, const char *what) { if (r != hipSuccess) throw std::runtime_error(std::string("rans: ") + what + ": " + hipGetErrorString(r)); };
+    auto ck = [](hipError_t r, const char *what) { if (r != hipSuccess) { (void)hipGetLastError(); throw std::runtime_error(std::string("rans: ") + what + ": " + hipGetErrorString(r)); } };
     for (hipEvent_t &x : e) ck(hipEventCreate(&x), "event");
     for (hipEvent_t &x : ev) ck(hipEventCreateWithFlags(&x, hipEventDisableTiming), "event");
     ck(hipStreamCreateWithFlags(&up, hipStreamNonBlocking), "copy stream");

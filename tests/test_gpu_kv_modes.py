@@ -145,3 +145,18 @@ def test_narrowing_and_widening_a_window(cfg, kind, synth):
         check(row, want[i], f"token {i}, window and sinks {modes[i]}")
         if modes[i][0]:
             assert np.abs(want - plain)[i].max() > 3 * ATOL   # the window shows
+
+
+def test_an_error_is_not_reported_again(synth):
+    """a context whose cache no card holds (512 GiB): the load fails, and the next one's launches are not told of it"""
+    toks = np.arange(40, dtype=np.int32)
+    with qa.HipLlama.load(synth("mini128"), max_ctx=64) as m:
+        want = m.prefill(toks)
+        with pytest.raises(qa.QphError, match="memory"):
+            qa.HipLlama.load(synth("mini128"), max_ctx=1 << 30)
+        m.reset()
+        np.testing.assert_array_equal(m.prefill(toks), want)
+        with pytest.raises(qa.QphError, match="memory"):
+            qa.HipLlama.load(synth("mini128"), max_ctx=1 << 30)
+    with qa.HipLlama.load(synth("mini128"), max_ctx=64) as m:
+        np.testing.assert_array_equal(m.prefill(toks), want)
