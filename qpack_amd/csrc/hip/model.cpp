@@ -67,7 +67,8 @@ const float *HipLlama::upload_f32(const qph_tensor &t, int64_t n) {
   return (const float *)place(t.data, t.data_coded, 4ull * n, t.name);
 }
 
-HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int max_ctx, int cache) : cfg_(cfg) {
+// (delegating: an exception below runs the destructor, which frees what the load had taken)
+HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int max_ctx, int cache) : HipLlama(cfg) {
   const int d = cfg.hidden, nh = cfg.heads, nkv = cfg.kv_heads, hd = cfg.head_dim, ff = cfg.ffn, V = cfg.vocab;
   if (d <= 0 || cfg.layers <= 0 || nh <= 0 || nkv <= 0 || ff <= 0 || V <= 0) throw std::runtime_error("hip: bad model config");
   if (hd != 64 && hd != 128) throw std::runtime_error("hip: head_dim must be 64 or 128");

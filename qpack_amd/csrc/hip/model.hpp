@@ -59,6 +59,7 @@ class HipLlama {
   float time_kernel(int which, int iters, double *bytes);
 
  private:
+  explicit HipLlama(const qph_config &cfg) : cfg_(cfg) {}
   struct Layer {
     DMat wq, wk, wv, wo, wg, wu, wd;
     const float *an = nullptr, *fn = nullptr, *bq = nullptr, *bk = nullptr, *bv = nullptr;

@@ -160,3 +160,13 @@ def test_an_error_is_not_reported_again(synth):
             qa.HipLlama.load(synth("mini128"), max_ctx=1 << 30)
     with qa.HipLlama.load(synth("mini128"), max_ctx=64) as m:
         np.testing.assert_array_equal(m.prefill(toks), want)
+
+
+def test_a_load_that_fails_gives_its_memory_back(synth):
+    with qa.HipLlama.load(synth("mini128"), max_ctx=64) as m:
+        m.prefill(np.arange(40, dtype=np.int32))
+    before = free()
+    for _ in range(8):
+        with pytest.raises(qa.QphError, match="memory"):
+            qa.HipLlama.load(synth("mini128"), max_ctx=1 << 30)
+    assert before - free() <= 4 << 20
