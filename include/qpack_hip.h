@@ -105,6 +105,13 @@ int qph_prefill_all(qph_model *m, const int *tokens, int n, float *logits);
  * from a logits vector (/root/reference/src/sampler.cpp:12-27, :41-42), here without copying the vocab floats to the
  * host.  1 <= M <= min(512, vocab); a caller wanting more candidates takes the logits (want = 1) instead. */
 int qph_step_topk(qph_model *m, int token, int M, int *idx, float *val);
+/* What Session::nll (/root/reference/src/chat.cpp:278-296) and qpack-perplexity compute from prefill_all's logits, without the vocabulary's floats of
+ * each token crossing to the host: feeds n tokens (like qph_prefill) and gives, behind each, the log probability and the rank of
+ * targets[i] (NULL: the next token; outside the vocabulary, as behind the last one: NaN and -1), the entropy in nats, and the
+ * `top` <= 64 most probable tokens with their log probabilities, [n][top]; as qph_logprobs.  Outputs are host arrays, any of them NULL.  In batched prompt
+ * products with the accuracy of qph_prefill; decode steps for q1 and, without q4 or q1 layers, q4 heads, and in arithmetic order 1.  The first call takes
+ * 4 MiB or so, and for a q8 head 4 bytes per 128 weights, of device memory. */
+int qph_score(qph_model *m, const int *tokens, const int *targets, int n, int top, float *logp, float *entropy, int *rank, int *top_index, float *top_logp);
 int qph_prefill_topk(qph_model *m, const int *tokens, int n, int M, int *idx, float *val);
 /* Model::reset (qpack.h:150) */
 int qph_reset(qph_model *m);
@@ -241,6 +248,47 @@ int qph_kv_read(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, co
 int qph_kv_attention_work(const qph_kv *c, int type, int heads, int n, int window, int sinks, int64_t *bytes);
 int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, int heads, int n, const int *pos, const int *lens,
                      int window, int sinks, float scale, void *work, int64_t work_bytes, void *stream);
+
+/* The same for sequences that all follow one prefix (a system prompt, a document, samples of one prompt), whose positions lie in a cache of their
+ * own: prefix (one sequence; c's kind, kv_heads and head_dim), of which the first *prefix_len (a device pointer, taken as 0 .. ctx; NULL: ctx)
+ * are visible to every token, before the p <= P of the sequence's own cache c.  The prefix is read once for all sequences.  Keys are
+ * as they are in the caches: a rotation of the sequences' own has to count the prefix (qph_turn.at).  nseq * n * heads / kv_heads <= 2^23, nseq * n * heads <= 2^30.
+ * work: qph_kv_attention_prefix_work bytes, as above. */
+int qph_kv_attention_prefix_work(const qph_kv *c, const qph_kv *prefix, int type, int heads, int n, int64_t *bytes);
+int qph_kv_attention_prefix(const qph_kv *c, const qph_kv *prefix, const int *prefix_len, const qph_rows *q, const qph_rows *out, int heads, int n, const int *pos,
+                            const int *lens, float scale, void *work, int64_t work_bytes, void *stream);
+/* From a step's projections to its cache in one pass.  Rows of q and k are first, where a norm is given, x w / sqrt(mean(x^2) + eps), then
+ * turned by their place in the text: dims i and i + half, i < half, by the angle whose cosine and sine stand at [place * half + i] of the tables, dims past 2 half
+ * stay; all in fp32.  q's rows go to out (rounded to their type; q's own rows, or apart from all that is read), k's and v's into the cache as qph_kv_write rounds
+ * them (k from fp32).  Token t of sequence b has place at[b] + t (at NULL: pos[b] + t); tokens whose place is not 0 .. places - 1 take no part either.
+ * n * (heads + 2 kv_heads) <= 2^26, and as for qph_kv_write. */
+typedef struct {
+  const float *cos, *sin;              /* device, [places][half] */
+  int64_t places;
+  int half;                            /* a multiple of head_dim / 8; 0: no rotation */
+  const int *at;                       /* device */
+  const float *q_norm, *k_norm;        /* device, [head_dim]; NULL: no norm */
+  float eps;
+} qph_turn;
+int qph_kv_append(const qph_kv *c, const qph_rows *q, const qph_rows *k, const qph_rows *v, const qph_rows *out, int heads, int n, const int *pos, const int *lens,
+                  const qph_turn *turn, void *stream);
+/* Copies positions, to the bit: position pos[b] + t of dst's sequence b (t and lens as above) becomes position index[b * index_seq + t] of src's sequence seqs[b]
+ * (seqs NULL: b).  dst and src may be the same or share memory: all is read before anything is written, by way of work, qph_kv_copy_work bytes (0 where
+ * the caches lie apart).  apart = 1 is the caller's word that no position that the call writes is read by it: then neither scratch nor a second pass.
+ * Sequences and positions outside src take no part. */
+int qph_kv_copy_work(const qph_kv *dst, const qph_kv *src, int n, int apart, int64_t *bytes);
+int qph_kv_copy(const qph_kv *dst, const qph_kv *src, const int *index, int64_t index_seq, int n, const int *pos, const int *lens, const int *seqs, int apart, void *work,
+                int64_t work_bytes, void *stream);
+
+/* ---- what a sampled or given token was worth (no counterpart in the reference, whose sampler works on host logits).  Device pointers, a stream, no allocation, as above.
+ * Row r of logits: vocab elements of type (QPH_F32, QPH_F16, QPH_BF16) at x + r * ld, at any alignment of the type.  logp[r] = x[tokens[r]] - ln sum e^x; rank[r] = the number
+ * of logits ahead of that token's (larger, or equal with a lower index); a token outside the vocabulary has NaN and -1.  entropy[r] = -sum p ln p in
+ * nats.  top_index / top_logp [rows][top]: the first top <= min(64, vocab) in the order of the ranks.  logp, entropy and rank may be NULL, tokens then too.
+ * Logits of -inf have probability 0; a row with a NaN or +inf, or of -inf alone, has NaN results, and its top_index entries are indices or -1.
+ * work: qph_logprobs_work bytes (16-byte aligned, NULL if 0) that no other call uses meanwhile. */
+int qph_logprobs_work(int type, int64_t rows, int vocab, int top, int64_t *bytes);
+int qph_logprobs(const void *x, int type, int64_t rows, int vocab, int64_t ld, const int *tokens, int top, float *logp, float *entropy, int *rank, int *top_index,
+                 float *top_logp, void *work, int64_t work_bytes, void *stream);
 
 /* ---- synthetic models (no reference counterpart: the reference's files come from convert_llama.py / qpack-quantize).
  * Writes a seeded random-init Llama-family QPACK2 file; see qpack_amd/csrc/host/synth.cpp for the exact rules. */

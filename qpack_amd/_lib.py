@@ -49,6 +49,11 @@ class RowsC(C.Structure):
     _fields_ = [("p", C.c_void_p), ("type", C.c_int), ("seq", C.c_int64), ("tok", C.c_int64), ("head", C.c_int64)]
 
 
+class TurnC(C.Structure):
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("places", C.c_int64), ("half", C.c_int), ("at", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("eps", C.c_float)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _FP = C.POINTER(C.c_float)
@@ -99,6 +104,14 @@ SIGNATURES = {
     "qph_kv_read": (_I, [_P, _P, _P, _I, _P, _P, _P]),
     "qph_kv_attention_work": (_I, [_P, _I, _I, _I, _I, _I, C.POINTER(C.c_int64)]),
     "qph_kv_attention": (_I, [_P, _P, _P, _I, _I, _P, _P, _I, _I, C.c_float, _P, C.c_int64, _P]),
+    "qph_kv_attention_prefix_work": (_I, [_P, _P, _I, _I, _I, C.POINTER(C.c_int64)]),
+    "qph_kv_attention_prefix": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P, C.c_float, _P, C.c_int64, _P]),
+    "qph_kv_append": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P]),
+    "qph_kv_copy_work": (_I, [_P, _P, _I, _I, C.POINTER(C.c_int64)]),
+    "qph_kv_copy": (_I, [_P, _P, _P, C.c_int64, _I, _P, _P, _P, _I, _P, C.c_int64, _P]),
+    "qph_logprobs_work": (_I, [_I, C.c_int64, _I, _I, C.POINTER(C.c_int64)]),
+    "qph_logprobs": (_I, [_P, _I, C.c_int64, _I, C.c_int64, _P, _I, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "qph_score": (_I, [_P, _IP, _P, _I, _I, _P, _P, _P, _P, _P]),
     "qph_kernel_rans_decode": (_I, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.POINTER(C.c_int64), _FP]),
     "qph_pack": (_I, [C.c_char_p, C.c_char_p, _I, _IP]),
 }

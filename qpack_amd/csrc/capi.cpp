@@ -110,6 +110,72 @@ static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sink
   a.nseq = c->nseq; a.nkv = c->kv_heads; a.hd = c->head_dim; a.heads = heads; a.rep = heads / c->kv_heads; a.n = n;
   a.window = window; a.sinks = sinks; a.few = qph::kv_few();
 }
+// attention over a common prefix and the sequences' own caches: both passes' arguments without their rows
+static void kv_prefix_args(const qph_kv *c, const qph_kv *prefix, const int *prefix_len, int heads, int n, qph::KvAttnArgs &a, qph::KvAttnArgs &p) {
+  kv_attn_args(c, heads, n, 0, 0, a);
+  int64_t seq, row;
+  kv_cache(prefix, &seq, &row);
+  if (prefix->kind != c->kind || prefix->kv_heads != c->kv_heads || prefix->head_dim != c->head_dim || prefix->nseq != 1)
+    throw std::invalid_argument("kv: the prefix must be a cache of one sequence, with the kind, kv_heads and head_dim of the sequences' own");
+  const int64_t tokens = (int64_t)c->nseq * n;
+  if (tokens * a.rep > 1 << 23 || tokens * heads > 1 << 30) throw std::invalid_argument("kv: with a prefix nseq * n * heads / kv_heads must be <= 2^23 and nseq * n * heads <= 2^30");
+  kv_attn_args(prefix, heads, 0, 0, 0, p);
+  p.n = (int)tokens;
+  p.prefix = {prefix_len, prefix->ctx, c->ctx, std::max(n, 1)};
+}
+// over q: every workgroup stores where it has read, which takes the same rows in the same places
+static void kv_over(const qph_rows *q, const qph_rows *out, int nseq, int n, int heads) {
+  if (n && q->p == out->p && ((nseq > 1 && q->seq != out->seq) || (n > 1 && q->tok != out->tok) || (heads > 1 && q->head != out->head)))
+    throw std::invalid_argument("kv: out over q must have q's strides");
+}
+// what both attention calls check and set besides their caches
+static void kv_attn_rows(const qph_kv *c, const qph_rows *q, const qph_rows *out, int heads, int n, const int *pos, const int *lens, float scale, qph::KvAttnArgs &a) {
+  need(pos, "pos");
+  a.q = kv_rows(q, "q", false, c->nseq, n, heads, c->head_dim); a.out = kv_rows(out, "out", true, c->nseq, n, heads, c->head_dim);
+  if (a.q.type != a.out.type) throw std::invalid_argument("kv: q and out must have the same type");
+  if (!(scale >= 0.f) || std::isinf(scale)) throw std::invalid_argument("kv: scale must be finite and not negative (0: 1 / sqrt(head_dim))");
+  a.pos = pos; a.lens = lens;
+  a.scale2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim));
+  if (std::isinf(a.scale2)) throw std::invalid_argument("kv: scale is too large");
+  kv_over(q, out, c->nseq, n, heads);
+}
+static int kv_row_type(int type) {
+  if (type != QPH_F32 && type != QPH_F16 && type != QPH_BF16) throw std::invalid_argument("kv: the type of q must be QPH_F32, QPH_F16 or QPH_BF16");
+  return type == QPH_F32 ? qph::RT_F32 : type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16;
+}
+// what two caches' memory covers, K and V
+static bool kv_overlap(const qph_kv *x, const qph_kv *y) {
+  auto span = [](const qph_kv *c, bool v) {
+    int64_t seq, row;
+    kv_cache(c, &seq, &row);
+    const uintptr_t p = (uintptr_t)(v ? c->v : c->k), d = (uintptr_t)c->kv_heads * c->head_dim;
+    const uintptr_t n = c->kind == QPH_Q4 ? (uintptr_t)qph::kv4_bytes(c->nseq, c->kv_heads, c->head_dim, c->ctx) : 2 * ((c->nseq - 1) * (uintptr_t)seq + (c->ctx - 1) * (uintptr_t)row + d);
+    return std::pair<uintptr_t, uintptr_t>(p, p + n);
+  };
+  for (int i = 0; i < (x->kind == QPH_Q4 ? 1 : 4); i++) {
+    const auto a = span(x, i & 1), b = span(y, i >> 1);
+    if (a.first < b.second && b.first < a.second) return true;
+  }
+  return false;
+}
+static void kv_copy_args(const qph_kv *dst, const qph_kv *src, int n, qph::KvCopyArgs &a) {
+  kv_cache(dst, &a.cseq, &a.crow);
+  kv_cache(src, &a.src_cseq, &a.src_crow);
+  if (dst->kind != src->kind || dst->kv_heads != src->kv_heads || dst->head_dim != src->head_dim) throw std::invalid_argument("kv: caches that are copied between must have the same kind, kv_heads and head_dim");
+  if (n < 0 || n > 1 << 20) throw std::invalid_argument("kv: n must be in [0, 2^20]");
+  a.cache = dst->k; a.cache_v = dst->v; a.ctx = dst->ctx; a.nrec = qph::kv4_records(dst->ctx);
+  a.src = src->k; a.src_v = src->v; a.src_ctx = src->ctx; a.src_nrec = qph::kv4_records(src->ctx);
+  a.nseq = dst->nseq; a.src_nseq = src->nseq; a.nkv = dst->kv_heads; a.hd = dst->head_dim; a.n = n;
+}
+static int64_t kv_copy_bytes(const qph_kv *dst, const qph_kv *src, int n, int apart) {
+  if (!n || apart || !kv_overlap(dst, src)) return 0;
+  const __int128 bytes = (__int128)dst->nseq * dst->kv_heads * dst->head_dim * (dst->kind == QPH_Q4 ? 9 * qph::kv4_records(n) : 4 * (int64_t)n);
+  kv_fits(bytes);
+  return (int64_t)bytes;
+}
+static void kv_work(const void *work, int64_t have, int64_t bytes, const char *call) {
+  if (bytes && (!work || have < bytes || (uintptr_t)work % 16)) throw std::invalid_argument("kv: work must have the " + std::to_string(bytes) + " bytes that " + call + " gives, 16-byte aligned");
+}
 static void hck(hipError_t e, const char *what) {
   if (e == hipSuccess) return;
   (void)hipGetLastError();   // as QPH_CK
@@ -226,6 +292,12 @@ int qph_verify_batches(const qph_model *m, int64_t *n) {
 }
 int qph_prefill_all(qph_model *m, const int *tokens, int n, float *logits) {
   QPH_API_TRY({ need(m, "model"); need(tokens, "tokens"); need(logits, "logits"); m->m->prefill_all(tokens, n, logits); });
+}
+int qph_score(qph_model *m, const int *tokens, const int *targets, int n, int top, float *logp, float *entropy, int *rank, int *top_index, float *top_logp) {
+  QPH_API_TRY({
+    need(m, "model"); need(tokens, "tokens");
+    m->m->score(tokens, targets, n, top, {logp, entropy, rank, top_index, top_logp});
+  });
 }
 int qph_step_topk(qph_model *m, int token, int M, int *idx, float *val) {
   QPH_API_TRY({ need(m, "model"); need(idx, "idx"); need(val, "val"); m->m->step_topk(token, M, idx, val); });
@@ -349,6 +421,41 @@ int qph_topk_noalloc(const float *x, int n, int M, int *idx, float *val, void *s
     hck(qph::launch_topk_noalloc(x, n, M, idx, val, (hipStream_t)stream), "launch topk");
   });
 }
+static void logprob_args(int type, int64_t rows, int vocab, int top, qph::LogprobArgs &a) {
+  if (type != QPH_F32 && type != QPH_F16 && type != QPH_BF16) throw std::invalid_argument("logprobs: the type must be QPH_F32, QPH_F16 or QPH_BF16");
+  if (rows < 0 || rows > 1 << 24) throw std::invalid_argument("logprobs: rows must be in [0, 2^24]");
+  if (vocab < 1 || vocab > 1 << 28) throw std::invalid_argument("logprobs: vocab must be in [1, 2^28]");
+  if (top < 0 || top > std::min(qph::kLpTop, vocab)) throw std::invalid_argument("logprobs: top must be in [0, min(64, vocab)]");
+  a.type = type == QPH_F32 ? qph::RT_F32 : type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16;
+  a.rows = rows; a.vocab = vocab; a.top = top;
+}
+int qph_logprobs_work(int type, int64_t rows, int vocab, int top, int64_t *bytes) {
+  QPH_API_TRY({
+    need(bytes, "bytes");
+    qph::LogprobArgs a{};
+    logprob_args(type, rows, vocab, top, a);
+    *bytes = rows ? (int64_t)qph::logprobs_plan(a) : 0;
+  });
+}
+int qph_logprobs(const void *x, int type, int64_t rows, int vocab, int64_t ld, const int *tokens, int top, float *logp, float *entropy, int *rank, int *top_index,
+                 float *top_logp, void *work, int64_t work_bytes, void *stream) {
+  QPH_API_TRY({
+    qph::LogprobArgs a{};
+    logprob_args(type, rows, vocab, top, a);
+    if (rows) {
+      need(x, "x");
+      if ((uintptr_t)x % (type == QPH_F32 ? 4 : 2)) throw std::invalid_argument("logprobs: x is not aligned to its type");
+      if (ld < 0) throw std::invalid_argument("logprobs: negative stride");
+      if (!tokens && (logp || rank)) throw std::invalid_argument("logprobs: logp and rank need tokens");
+      if (top) { need(top_index, "top_index"); need(top_logp, "top_logp"); }
+      a.x = x; a.ld = ld; a.tokens = tokens; a.logp = logp; a.entropy = entropy; a.rank = rank; a.top_index = top_index; a.top_logp = top_logp;
+      const int64_t bytes = (int64_t)qph::logprobs_plan(a);
+      if (bytes && (!work || work_bytes < bytes || (uintptr_t)work % 16)) throw std::invalid_argument("logprobs: work must have the " + std::to_string(bytes) + " bytes that qph_logprobs_work gives, 16-byte aligned");
+      a.work = work;
+      hck(qph::launch_logprobs(a, (hipStream_t)stream), "logprobs");
+    }
+  });
+}
 int qph_kernel_matmul(int kind, const void *q, const void *scale, int rows, int cols, const float *X, int B, float *Y) {
   QPH_API_TRY({
     need(q, "q"); need(scale, "scale"); need(X, "X"); need(Y, "Y");
@@ -449,13 +556,55 @@ int qph_kv_read(const qph_kv *c, const qph_rows *k, const qph_rows *v, int n, co
     if (n) hck(qph::launch_kv_read(kv_kind(c), a, (hipStream_t)stream), "kv read");
   });
 }
+int qph_kv_append(const qph_kv *c, const qph_rows *q, const qph_rows *k, const qph_rows *v, const qph_rows *out, int heads, int n, const int *pos, const int *lens,
+                  const qph_turn *turn, void *stream) {
+  QPH_API_TRY({
+    qph::KvAppendArgs a{};
+    a.io = kv_io(c, k, v, false, n, pos, lens);
+    need(turn, "turn");
+    if (heads < 1 || heads % c->kv_heads || heads > 65535) throw std::invalid_argument("kv: heads must be a positive multiple of kv_heads, at most 65535");
+    if ((int64_t)n * (heads + 2 * c->kv_heads) > 1 << 26) throw std::invalid_argument("kv: n * (heads + 2 * kv_heads) must not pass 2^26");
+    a.q = kv_rows(q, "q", false, c->nseq, n, heads, c->head_dim); a.out = kv_rows(out, "out", true, c->nseq, n, heads, c->head_dim);
+    if (a.q.type != a.out.type || a.q.type != a.io.k.type) throw std::invalid_argument("kv: q, k, v and out must have the same type");
+    kv_over(q, out, c->nseq, n, heads);
+    if (turn->half < 0 || 2 * turn->half > c->head_dim || turn->half % (c->head_dim / 8)) throw std::invalid_argument("kv: half the rotated dims must be a multiple of head_dim / 8, and at most head_dim / 2");
+    if (turn->places < 1 || turn->places > (int64_t)1 << 31) throw std::invalid_argument("kv: places must be in [1, 2^31]");
+    if (turn->half) { need(turn->cos, "cos"); need(turn->sin, "sin"); }
+    if (!(turn->eps >= 0.f) || std::isinf(turn->eps)) throw std::invalid_argument("kv: eps must be finite and not negative");
+    for (const float *p : {turn->cos, turn->sin, turn->q_norm, turn->k_norm}) if ((uintptr_t)p % 4) throw std::invalid_argument("kv: cos, sin and the norms' weights must be aligned to 4 bytes");
+    a.heads = heads; a.half = turn->half; a.cos_t = turn->cos; a.sin_t = turn->sin; a.places = turn->places;
+    a.qw = turn->q_norm; a.kw = turn->k_norm; a.eps = turn->eps; a.at = turn->at;
+    if (n) hck(qph::launch_kv_append(kv_kind(c), a, (hipStream_t)stream), "kv append");
+  });
+}
+int qph_kv_copy_work(const qph_kv *dst, const qph_kv *src, int n, int apart, int64_t *bytes) {
+  QPH_API_TRY({
+    need(bytes, "bytes");
+    qph::KvCopyArgs a{};
+    kv_copy_args(dst, src, n, a);
+    *bytes = kv_copy_bytes(dst, src, n, apart);
+  });
+}
+int qph_kv_copy(const qph_kv *dst, const qph_kv *src, const int *index, int64_t index_seq, int n, const int *pos, const int *lens, const int *seqs, int apart, void *work,
+                int64_t work_bytes, void *stream) {
+  QPH_API_TRY({
+    qph::KvCopyArgs a{};
+    kv_copy_args(dst, src, n, a);
+    need(index, "index"); need(pos, "pos");
+    if (index_seq < 0) throw std::invalid_argument("kv: negative stride of index");
+    a.index = index; a.index_seq = index_seq; a.pos = pos; a.lens = lens; a.seqs = seqs;
+    const int64_t bytes = kv_copy_bytes(dst, src, n, apart);
+    kv_work(work, work_bytes, bytes, "qph_kv_copy_work");
+    a.work = bytes ? work : nullptr;
+    if (n) hck(qph::launch_kv_copy(kv_kind(dst), a, (hipStream_t)stream), "kv copy");
+  });
+}
 int qph_kv_attention_work(const qph_kv *c, int type, int heads, int n, int window, int sinks, int64_t *bytes) {
   QPH_API_TRY({
     need(bytes, "bytes");
-    if (type != QPH_F32 && type != QPH_F16 && type != QPH_BF16) throw std::invalid_argument("kv: the type of q must be QPH_F32, QPH_F16 or QPH_BF16");
     qph::KvAttnArgs a{};
+    a.q.type = kv_row_type(type);
     kv_attn_args(c, heads, n, window, sinks, a);
-    a.q.type = type == QPH_F32 ? qph::RT_F32 : type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16;
     *bytes = n ? (int64_t)qph::kv_attn_plan(a) : 0;
   });
 }
@@ -464,21 +613,38 @@ int qph_kv_attention(const qph_kv *c, const qph_rows *q, const qph_rows *out, in
   QPH_API_TRY({
     qph::KvAttnArgs a{};
     kv_attn_args(c, heads, n, window, sinks, a);
-    need(pos, "pos");
-    a.q = kv_rows(q, "q", false, c->nseq, n, heads, c->head_dim); a.out = kv_rows(out, "out", true, c->nseq, n, heads, c->head_dim);
-    if (a.q.type != a.out.type) throw std::invalid_argument("kv: q and out must have the same type");
-    if (!(scale >= 0.f) || std::isinf(scale)) throw std::invalid_argument("kv: scale must be finite and not negative (0: 1 / sqrt(head_dim))");
-    a.pos = pos; a.lens = lens;
-    a.scale2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim));
-    if (std::isinf(a.scale2)) throw std::invalid_argument("kv: scale is too large");
-    // over q: every workgroup stores where it has read, which takes the same rows in the same places
-    if (n && q->p == out->p && ((c->nseq > 1 && q->seq != out->seq) || (n > 1 && q->tok != out->tok) || (heads > 1 && q->head != out->head)))
-      throw std::invalid_argument("kv: out over q must have q's strides");
+    kv_attn_rows(c, q, out, heads, n, pos, lens, scale, a);
     if (n) {
       const int64_t bytes = (int64_t)qph::kv_attn_plan(a);
-      if (bytes && (!work || work_bytes < bytes || (uintptr_t)work % 16)) throw std::invalid_argument("kv: work must have the " + std::to_string(bytes) + " bytes that qph_kv_attention_work gives, 16-byte aligned");
+      kv_work(work, work_bytes, bytes, "qph_kv_attention_work");
       a.part = (float *)work;
       hck(qph::launch_kv_attn(a, (hipStream_t)stream), "kv attention");
+    }
+  });
+}
+int qph_kv_attention_prefix_work(const qph_kv *c, const qph_kv *prefix, int type, int heads, int n, int64_t *bytes) {
+  QPH_API_TRY({
+    need(bytes, "bytes");
+    qph::KvAttnArgs a{};
+    qph::KvAttnArgs p{};
+    a.q.type = p.q.type = kv_row_type(type);
+    kv_prefix_args(c, prefix, nullptr, heads, n, a, p);
+    *bytes = n ? (int64_t)qph::kv_prefix_plan(a, p) : 0;
+  });
+}
+int qph_kv_attention_prefix(const qph_kv *c, const qph_kv *prefix, const int *prefix_len, const qph_rows *q, const qph_rows *out, int heads, int n, const int *pos,
+                            const int *lens, float scale, void *work, int64_t work_bytes, void *stream) {
+  QPH_API_TRY({
+    qph::KvAttnArgs a{};
+    qph::KvAttnArgs p{};
+    kv_prefix_args(c, prefix, prefix_len, heads, n, a, p);
+    kv_attn_rows(c, q, out, heads, n, pos, lens, scale, a);
+    if (n) {
+      p.q = a.q; p.out = a.out; p.pos = pos; p.lens = lens; p.scale2 = a.scale2;
+      const int64_t bytes = (int64_t)qph::kv_prefix_plan(a, p);
+      kv_work(work, work_bytes, bytes, "qph_kv_attention_prefix_work");
+      a.part = p.part = (float *)work;
+      hck(qph::launch_kv_prefix(a, p, (hipStream_t)stream), "kv attention");
     }
   });
 }

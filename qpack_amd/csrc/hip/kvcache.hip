@@ -23,144 +23,20 @@
 #include <cmath>
 #include <cstdlib>
 
+#include "kvrec.hpp"
 #include "launch.hpp"
 
 namespace qph {
 
 namespace {
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef short s8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) s4 lds_s4;
-
-constexpr int kRec = kKvRec;   // positions of a record
-
-__device__ __forceinline__ float bf16_to_f(uint16_t h) { return __builtin_bit_cast(float, (uint32_t)h << 16); }
-// round to nearest even; NaN stays NaN
-__device__ __forceinline__ uint16_t f_to_bf16(float f) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)(u >> 16 | 0x40);
-  return (uint16_t)((u + 0x7fff + (u >> 16 & 1)) >> 16);
-}
-
-// N (a multiple of 8) consecutive elements of type T (RowType) from element `at` of rows.  The loads and stores are 16 (8) bytes at any alignment of
-// the type, which the memory pipeline takes as they are: a second, element by element, path made the kernels twice as
-// long, and their first pass through the instruction cache is what a short call waits for
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
-typedef u32x2 u32x2_any __attribute__((aligned(2)));
-template <int T, int N>
-__device__ __forceinline__ void load_elems(const KvRows &r, int64_t at, float *x) {
-  if constexpr (T == RT_F32) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const u32x4 v = *(const u32x4_any *)((const float *)r.p + at + i);
-#pragma unroll
-      for (int j = 0; j < 4; j++) { const uint32_t w = v[j]; x[i + j] = __builtin_bit_cast(float, w); }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 8) {
-      const u32x4 v = *(const u32x4_any *)((const uint16_t *)r.p + at + i);
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const uint16_t h = (uint16_t)(v[j / 2] >> 16 * (j & 1));
-        x[i + j] = T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h);
-      }
-    }
-  }
-}
-// N a multiple of 4
-template <int T, int N>
-__device__ __forceinline__ void store_elems(const KvRows &r, int64_t at, const float *x) {
-  auto e = [](float f) { return (uint32_t)(T == RT_F16 ? float_to_half_bits(f) : f_to_bf16(f)); };
-#pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    if constexpr (T == RT_F32) {
-      *(u32x4_any *)((float *)r.p + at + i) = (u32x4){__builtin_bit_cast(uint32_t, x[i]), __builtin_bit_cast(uint32_t, x[i + 1]), __builtin_bit_cast(uint32_t, x[i + 2]),
-                                                      __builtin_bit_cast(uint32_t, x[i + 3])};
-    } else {
-      *(u32x2_any *)((uint16_t *)r.p + at + i) = (u32x2){e(x[i]) | e(x[i + 1]) << 16, e(x[i + 2]) | e(x[i + 3]) << 16};
-    }
-  }
-}
-
-// 8 fp16 elements as the matrix cores take them
-__device__ __forceinline__ h8 load_halves(const KvRows &r, int64_t at) {
-  const u32x4 v = *(const u32x4_any *)((const uint16_t *)r.p + at);
-  return __builtin_bit_cast(h8, v);
-}
-
-// bit position of element i (0 .. 7) of a word of codes
-__host__ __device__ constexpr int nib(int i) { return 16 * (i & 1) + 4 * (i >> 1); }
-
-// a word's 8 values in element order.  Codes 0 .. 15 in the low mantissa bits of fp16 1024 (or, four bits higher, 16 times
-// them, brought back by an exact fma): c - 8 exact, times the elements' scales exact
-__device__ __forceinline__ uint32_t vreg(uint32_t c) { asm("" : "+v"(c)); return c; }   // an instruction reads one scalar: v_and_or_b32 wants the other constant in a vector register
-__device__ __forceinline__ h2 code_pair(uint32_t w, int e) {
-  const h2 k1032 = {(_Float16)1032.f, (_Float16)1032.f}, k16 = {(_Float16)0.0625f, (_Float16)0.0625f}, k72 = {(_Float16)-72.f, (_Float16)-72.f};
-  if (e & 1) {
-    const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x00f000f0u) | vreg(0x64006400u));
-    return __builtin_elementwise_fma(x, k16, k72);
-  }
-  const h2 x = __builtin_bit_cast(h2, ((e > 1 ? w >> 8 : w) & 0x000f000fu) | vreg(0x64006400u));
-  return x - k1032;
-}
-// scales of the four element pairs: one for all (K: a group of dims), or the positions' own (V)
-__device__ __forceinline__ h8 values(uint32_t w, h2 s0, h2 s1, h2 s2, h2 s3) {
-  const h2 a = code_pair(w, 0) * s0, b = code_pair(w, 1) * s1, c = code_pair(w, 2) * s2, d = code_pair(w, 3) * s3;
-  return (h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-__device__ __forceinline__ h8 values(uint32_t w, uint16_t s) {
-  const h2 x = __builtin_bit_cast(h2, (uint32_t)s * 0x10001u);
-  return values(w, x, x, x, x);
-}
-__device__ __forceinline__ h8 values(uint32_t w, u32x4 s) {
-  const uint32_t s0 = s[0], s1 = s[1], s2 = s[2], s3 = s[3];   // (a bit cast of a vector's element takes the first one)
-  return values(w, __builtin_bit_cast(h2, s0), __builtin_bit_cast(h2, s1), __builtin_bit_cast(h2, s2), __builtin_bit_cast(h2, s3));
-}
-
-__device__ __forceinline__ int tokens_of(const int *lens, int b, int n) { return lens ? min(max(lens[b], 0), n) : n; }
-
 // ------------------------------------------------------------------ writing and reading
-// the scale of a group from the bits of its largest magnitude
-__device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return 0x7e00;
-  const float a = fminf(__builtin_bit_cast(float, amax_bits), 65504.f);
-  return float_to_half_bits(bf16_to_f(f_to_bf16(a / 7.f)));
-}
-// clamp(rint(x / s), -7, 7) + 8, ties to even, of the real quotient: the product with 1 / s is off by one step at most, and
-// only next to a border; e = x - r s is exact (r s has 11 bits, e is a multiple of x's last place below 2^24 of them).
-// 16-bit rows: x has 11 bits at most and s 8, so x / s is a border (half an odd number) or 2^-12 away from all of them.  Rounded to a
-// multiple of 2^-16 first (by adding 192), the product, which is off by less than 2^-20, is on the right side or on the border itself; a
-// second sum rounds it to a whole number in the float's low bits.  Four instructions for fifteen: 2048
-// positions of 8 heads of 128 dims 7.1 -> 4.5 us
-template <int T>
-__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
-  const float y = __builtin_amdgcn_fmed3f(x, -7.f * s, 7.f * s);
-  if constexpr (T != RT_F32) {
-    const float t = __builtin_fmaf(y, inv, 192.f) + (12582912.f + 8.f - 192.f);
-    return __builtin_bit_cast(uint32_t, t) & 15;
-  }
-  float r = __builtin_rintf(y * inv);
-  const float e = 2.f * __builtin_fmaf(-r, s, y);
-  const bool odd = ((int)r & 1) != 0;
-  if (e > s || (e == s && odd)) r += 1.f;
-  else if (e < -s || (e == -s && odd)) r -= 1.f;
-  return (uint32_t)((int)r + 8);
-}
-
 // One wave per record's K, one per its V: lane = position lane / 8 of the record, dims EL (lane % 8) ..  Positions outside the
 // call's keep their codes and scales: their K rows and scales are not stored, and the V words, which hold all 8
 // positions, are read and merged where the call covers a part only (no other workgroup of the launch has the record).
 // 2048 positions of 8 heads of 128 dims, fp16 rows: 4.5 us, a launch (2.4) and 10.8 MB at the copy rate (2.2).
 template <int HD, int T>
 __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
-  constexpr int EL = HD / 8, GL = 32 / EL;   // elements of a lane; lanes of a group
+  constexpr int EL = HD / 8;   // elements of a lane
   __shared__ __align__(16) uint8_t codes[kRec][HD];
   const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 63, vside = threadIdx.x >> 6;
   const int P0 = a.pos[b], cnt = tokens_of(a.lens, b, a.n);
@@ -173,60 +49,8 @@ __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   const bool mine = p >= P0 && p < last;
   const KvRows &r = vside ? a.v : a.k;
   float x[EL];
-  uint32_t mx = 0;
-  if (mine) {
-    load_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x);
-#pragma unroll
-    for (int i = 0; i < EL; i++) mx = max(mx, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
-  }
-  mx = max(mx, (uint32_t)dpp_i<kDppQuadXor1>((int)mx));
-  if (GL == 4) mx = max(mx, (uint32_t)dpp_i<kDppQuadXor2>((int)mx));
-  const uint16_t sb = group_scale(mx);
-  const float s = half_bits_to_float(sb);
-  uint32_t c[EL];
-  if (s > 0.f) {
-    const float inv = 1.f / s;
-#pragma unroll
-    for (int i = 0; i < EL; i++) c[i] = mine ? code_of<T>(x[i], s, inv) : 8;
-  } else {
-#pragma unroll
-    for (int i = 0; i < EL; i++) c[i] = 8;
-  }
-  uint8_t *o = (uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD);
-  if (!vside) {
-    if (!mine) return;
-    uint32_t w[EL / 8];
-#pragma unroll
-    for (int i = 0; i < EL / 8; i++) {
-      w[i] = 0;
-#pragma unroll
-      for (int j = 0; j < 8; j++) w[i] |= c[8 * i + j] << nib(j);
-      *(uint32_t *)(o + row * (HD / 2) + part * (EL / 2) + 4 * i) = w[i];
-    }
-    if (part % GL == 0) *(uint16_t *)(o + 8 * HD + 2 * (row * (HD / 32) + part / GL)) = sb;
-    return;
-  }
-  if (mine && part % GL == 0) *(uint16_t *)(o + 8 * HD + HD / 2 + 2 * (part / GL * kRec + row)) = sb;
-#pragma unroll
-  for (int i = 0; i < EL; i += 4) *(uint32_t *)&codes[row][EL * part + i] = c[i] | c[i + 1] << 8 | c[i + 2] << 16 | c[i + 3] << 24;
-  // the V wave alone reads what it wrote
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  uint32_t keep = 0;   // bits of the positions that the call does not write
-#pragma unroll
-  for (int i = 0; i < kRec; i++)
-    if (!(rec * kRec + i >= P0 && rec * kRec + i < last)) keep |= 15u << nib(i);
-#pragma unroll
-  for (int k = 0; k < HD / 64; k++) {
-    const int idx = lane * (HD / 64) + k, d = idx % (HD / 16) * 16 + idx / (HD / 16);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < kRec; i++) w |= (uint32_t)codes[i][d] << nib(i);
-    uint32_t *dst = (uint32_t *)(o + 4 * HD) + idx;
-    if (keep) w = (w & ~keep) | (*dst & keep);
-    *dst = w;
-  }
+  if (mine) load_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x);
+  store_record<HD, T>((uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD), x, mine, vside, row, part, kept_bits(rec * kRec, P0, last), codes);
 }
 
 // One token a sequence: a wave has one row of K or V, HD / 64 dims a lane.  Lanes of a K word meet by DPP; a V word is read (as soon as
@@ -247,48 +71,7 @@ __global__ __launch_bounds__(128) void k_kv4_write1(KvIoArgs a) {
   const int p = a.pos[b];
   if (p < 0 || p >= a.ctx || tokens_of(a.lens, b, a.n) <= 0) return;
   uint8_t *o = (uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + p / kRec) * (9 * HD);
-  const int row = p % kRec;
-  uint32_t *vw[EL], old[EL];
-  if (vside) {
-#pragma unroll
-    for (int i = 0; i < EL; i++) {
-      const int d = EL * lane + i;
-      vw[i] = (uint32_t *)(o + 4 * HD) + d % 16 * (HD / 16) + d / 16;
-      old[i] = *vw[i];
-    }
-  }
-  uint32_t mx = 0;
-#pragma unroll
-  for (int i = 0; i < EL; i++) mx = max(mx, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
-  mx = max(mx, (uint32_t)dpp_i<kDppQuadXor1>((int)mx));
-  mx = max(mx, (uint32_t)dpp_i<kDppQuadXor2>((int)mx));
-  mx = max(mx, (uint32_t)dpp_i<kDppHalfMirror>((int)mx));
-  mx = max(mx, (uint32_t)dpp_i<kDppMirror>((int)mx));
-  if (EL == 1) {   // 32 dims are 32 lanes (a maximum of the bits: NaN's are the largest)
-    float u, v;
-    swap16(__builtin_bit_cast(float, mx), u, v);
-    mx = max(__builtin_bit_cast(uint32_t, u), __builtin_bit_cast(uint32_t, v));
-  }
-  const uint16_t sb = group_scale(mx);
-  const float s = half_bits_to_float(sb), inv = 1.f / s;
-  uint32_t c[EL];
-#pragma unroll
-  for (int i = 0; i < EL; i++) c[i] = s > 0.f ? code_of<T>(x[i], s, inv) : 8;
-  if (vside) {
-    const int sh = 16 * (row & 1) + 4 * (row >> 1);
-#pragma unroll
-    for (int i = 0; i < EL; i++) *vw[i] = (old[i] & ~(15u << sh)) | c[i] << sh;
-    if (lane % (32 / EL) == 0) *(uint16_t *)(o + 8 * HD + HD / 2 + 2 * (lane / (32 / EL) * kRec + row)) = sb;
-    return;
-  }
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < EL; i++) { const int j = (EL * lane + i) & 7; w |= c[i] << (16 * (j & 1) + 4 * (j >> 1)); }
-  w |= (uint32_t)dpp_i<kDppQuadXor1>((int)w);
-  w |= (uint32_t)dpp_i<kDppQuadXor2>((int)w);
-  if (EL == 1) w |= (uint32_t)dpp_i<kDppHalfMirror>((int)w);
-  if (lane % (8 / EL) == 0) *(uint32_t *)(o + row * (HD / 2) + EL * lane / 2) = w;
-  if (lane % (32 / EL) == 0) *(uint16_t *)(o + 8 * HD + 2 * (row * (HD / 32) + lane / (32 / EL))) = sb;
+  store_one<HD, T>(o, p % kRec, x, vside, lane);
 }
 
 // The same lanes as k_kv4_write's.  A lane takes its position's code out of each of its dims' V words, which 8 lanes read from L1: 4.7 us for
@@ -400,6 +183,35 @@ __device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int chunk) {
   s.nt = (s.NR + (1 << a.tile_log2) - 1) >> a.tile_log2;
   s.S = s.nt <= a.one_tiles ? 1 : min(a.nsplit, (s.nt + (1 << a.min_log2) - 1) >> a.min_log2);
   return s;
+}
+// The span of a pass over a common prefix: every column sees all of its positions.  Its columns are (sequence, token, query head), the tokens of all
+// sequences counted through, and b is 0
+__device__ __forceinline__ int prefix_length(const KvPrefix &p) { return p.len ? (int)min((int64_t)max(*p.len, 0), p.ctx) : (int)p.ctx; }
+__device__ __forceinline__ int splits_of(int nt, int one_tiles, int nsplit, int min_log2) { return nt <= one_tiles ? (int)(nt > 0) : min(nsplit, (nt + (1 << min_log2) - 1) >> min_log2); }
+__device__ __forceinline__ Span prefix_span_of(const KvAttnArgs &a) {
+  Span s;
+  const int L = prefix_length(a.prefix);
+  s.P0 = 0; s.cnt = a.n; s.any = L > 0;
+  s.PA = s.PB = L - 1;
+  s.ws = s.SR = s.skip = 0;
+  s.NR = (L + kRec - 1) / kRec;
+  s.nt = (s.NR + (1 << a.tile_log2) - 1) >> a.tile_log2;
+  s.S = splits_of(s.nt, a.one_tiles, a.nsplit, a.min_log2);
+  return s;
+}
+__device__ __forceinline__ int prefix_splits(const KvJoin &p) {
+  const int nr = (prefix_length(p.prefix) + kRec - 1) / kRec;
+  return splits_of((nr + (1 << p.tile_log2) - 1) >> p.tile_log2, p.one_tiles, p.nsplit, p.min_log2);
+}
+// a token counted through all sequences, as its sequence's
+struct SeqTok { int b, t; };
+__device__ __forceinline__ SeqTok seq_tok(const KvAttnArgs &a, int tok) {
+  const int b = a.prefix.n == 1 ? tok : tok / a.prefix.n;
+  return {b, tok - b * a.prefix.n};
+}
+__device__ __forceinline__ bool takes_part(const KvAttnArgs &a, SeqTok x) {
+  const int P0 = a.pos[x.b];
+  return (P0 >= 0) & (x.t < tokens_of(a.lens, x.b, a.prefix.n)) & ((int64_t)P0 + x.t < a.prefix.own_ctx);
 }
 // the first tile of share i of S (the product fits: nt <= 2^25, i <= 64)
 __device__ __forceinline__ int share(const Span &s, int i) { return s.S == 1 ? i * s.nt : (int)((uint32_t)i * (uint32_t)s.nt / (uint32_t)s.S); }
@@ -569,7 +381,7 @@ __device__ __forceinline__ void add_bad(const uint8_t *rec, const uint16_t *row,
   }
 }
 
-template <int HD, int KIND, int T>
+template <int HD, int KIND, int T, bool PRE = false>
 __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a) {
   constexpr bool TWO = T == RT_F32;
   constexpr int NW = kFewWaves, KS = HD / 32, DT = HD / 16, NC = TWO ? 8 : 16, QS = HD + 4;
@@ -585,8 +397,9 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   // the sequence's position is known
   h8 q[KS];
   float x[KS][8];
+  const SeqTok st = PRE ? seq_tok(a, tok) : SeqTok{b, tok};
   {
-    const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)(g * a.rep + hr) * a.q.head;
+    const int64_t at = st.b * a.q.seq + (int64_t)st.t * a.q.tok + (int64_t)(g * a.rep + hr) * a.q.head;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
       const int64_t d = at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg);
@@ -594,10 +407,10 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
       else load_elems<T, 8>(a.q, d, x[k]);
     }
   }
-  const Span s = span_of(a, b, chunk);
+  const Span s = PRE ? prefix_span_of(a) : span_of(a, b, chunk);
   if (!s.any || split >= s.S) return;
-  const bool live = tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
-  const int P = live ? s.P0 + tok : -1;
+  const bool live = PRE ? takes_part(a, st) : tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
+  const int P = live ? PRE ? s.PB : s.P0 + tok : -1;
   const int lo = behind(a, P);
   const int t0 = share(s, split), t1 = share(s, split + 1);
   const Head h = head_of<HD, KIND>(a, b, g);
@@ -774,7 +587,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
   const int e = threadIdx.x, c = e / (HD / 4), d = 4 * (e % (HD / 4));
   if (c >= NC) return;
   const int cc = c0 + c, tk = token_of(a, cc);
-  if (tk >= s.cnt || (int64_t)s.P0 + tk >= a.ctx) return;
+  if (tk >= s.cnt || (!PRE && (int64_t)s.P0 + tk >= a.ctx)) return;   // (a prefix's pass leaves zeros for tokens that take no part: not read)
   float M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][c]);
@@ -787,7 +600,7 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
     y += *(const f32x4 *)(ored + (w * NC + c) * QS + d) * k;
   }
   const int head = g * a.rep + cc - tk * a.rep;
-  if (s.S == 1) {
+  if (!PRE && s.S == 1 && !a.joined) {
     const float inv = 1.f / L;   // a visible position's score is -inf only where the plain softmax gives NaN too: 0 x inf
     float r[4];
 #pragma unroll
@@ -795,9 +608,9 @@ __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a
     store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tk * a.out.tok + (int64_t)head * a.out.head + d, r);
     return;
   }
-  const int64_t row = ((int64_t)b * a.n + tk) * a.heads + head, at = row * a.nsplit + split;
+  const int64_t row = ((int64_t)b * a.n + tk) * a.heads + head, at = row * a.slots + a.slot0 + split;
   *(f32x4 *)(a.part + at * HD + d) = y;
-  if (d == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.nsplit * HD + 2 * at) = make_float2(M, L);
+  if (d == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD + 2 * at) = make_float2(M, L);
 }
 
 // The splits' sums of one row a workgroup: 256 threads, HD / 4 of them side by side over the dims, the others over the
@@ -866,6 +679,73 @@ __global__ __launch_bounds__(256) void k_kv_merge_rows(KvAttnArgs a) {
   store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, o);
 }
 
+// A sequence's own splits and the common prefix's.  As the two above; every token that takes part has a row of partial sums, and the own part holds at
+// least its own position
+template <int HD, int T>
+__global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a, KvJoin p) {
+  constexpr int CT = HD / 4, SL = 256 / CT;
+  __shared__ f32x4 oo[SL][CT];
+  const int head = blockIdx.x, tok = blockIdx.y, b = blockIdx.z, g = token_of(a, head);
+  const int col = tok * a.rep + head - g * a.rep;
+  const Span s = span_of(a, b, chunk_of(a, col));
+  if (!s.any || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
+  const int S0 = prefix_splits(p);
+  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD) + row * a.slots;
+  const float *po = a.part + row * a.slots * HD;
+  const int ct = threadIdx.x % CT, sl = threadIdx.x / CT, lane = threadIdx.x & 63;
+  const float2 none = make_float2(-INFINITY, 0.f), x = lane < s.S ? ml[lane] : none, x0 = lane < S0 ? ml[a.nsplit + lane] : none;
+  const float M = wave_max(fmaxf(x.x, x0.x)), Mz = M == -INFINITY ? 0.f : M;
+  const float L = wave_sum(x.y * __builtin_amdgcn_exp2f(x.x - Mz) + x0.y * __builtin_amdgcn_exp2f(x0.x - Mz));
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = sl; i < s.S + S0; i += SL) {
+    const int k = i < s.S ? i : a.nsplit + i - s.S;
+    y += *(const f32x4 *)(po + (int64_t)k * HD + 4 * ct) * __builtin_amdgcn_exp2f(ml[k].x - Mz);
+  }
+  oo[sl][ct] = y;
+  __syncthreads();
+  if (sl) return;
+#pragma unroll
+  for (int i = 1; i < SL; i++) y += oo[i][ct];
+  const float inv = 1.f / L;
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) r[i] = y[i] * inv;
+  store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, r);
+}
+template <int HD, int T>
+__global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a, KvJoin p) {
+  constexpr int CT = HD / 4;
+  const int b = blockIdx.z, ct = threadIdx.x % CT, i = blockIdx.x * (256 / CT) + threadIdx.x / CT;
+  if (i >= a.n * a.heads) return;
+  const int tok = i / a.heads, head = i - tok * a.heads, g = token_of(a, head), col = tok * a.rep + head - g * a.rep;
+  const Span s = span_of(a, b, chunk_of(a, col));
+  if (!s.any || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
+  const int S0 = prefix_splits(p);
+  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD) + row * a.slots;
+  const float *po = a.part + row * a.slots * HD + 4 * ct;
+  float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < s.S + S0; k++) M = fmaxf(M, ml[k < s.S ? k : a.nsplit + k - s.S].x);
+  const float Mz = M == -INFINITY ? 0.f : M;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int j = 0; j < s.S + S0; j++) {
+    const int k = j < s.S ? j : a.nsplit + j - s.S;
+    const float2 x = ml[k];
+    const float w = __builtin_amdgcn_exp2f(x.x - Mz);
+    L += x.y * w;
+    y += *(const f32x4 *)(po + (int64_t)k * HD) * w;
+  }
+  const float inv = 1.f / L;
+  float o[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) o[k] = y[k] * inv;
+  store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head + 4 * ct, o);
+}
+
 // ------------------------------------------------------------------ many tokens
 // 8 waves of 32 columns; the workgroup's 256 columns share blocks of 64 positions (8 records) in LDS, three buffers: while
 // one is computed, the block after next is expanded, and the codes of the one behind that are on their way to registers.
@@ -884,7 +764,7 @@ __global__ __launch_bounds__(256) void k_kv_merge_rows(KvAttnArgs a) {
 // tokens each of 32 sequences 6 % more
 constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
 
-template <int HD, int KIND, int T>
+template <int HD, int KIND, int T, bool PRE = false>
 __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   constexpr bool TWO = T == RT_F32;
   constexpr int NT = kManyWaves * 64, KQ = HD / 16, OT = HD / 32, BR = kManyBlk / kRec;
@@ -897,22 +777,23 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
   const int b = blockIdx.z, g = blockIdx.x, rest = a.nsplit == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nsplit, split = blockIdx.y - rest * a.nsplit;
   const int chunk = a.nchunk - 1 - rest;   // without pairs: the last columns, with the most to read, first
-  const Span s = span_of(a, b, chunk);
+  const Span s = PRE ? prefix_span_of(a) : span_of(a, b, chunk);
   if (!s.any || split >= s.S) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, ln = lane & 31, hf = lane >> 5;
   // waves w and w + 4 share a SIMD: one of the front half, one of the back half
   const int cw = chunk_half(a, chunk, wave / (kManyWaves / 2)) + 32 * (wave % (kManyWaves / 2));
   // (columns past the last read its query, as in k_kv_few; a wave without any other takes no block and uses none of it)
   const int col = min(cw + ln, a.n * a.rep - 1), tok = token_of(a, col), head = g * a.rep + col - tok * a.rep;
-  const bool live = col == cw + ln && tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
-  const int P = live ? s.P0 + tok : -1;
+  const SeqTok sq = PRE ? seq_tok(a, tok) : SeqTok{b, tok};
+  const bool live = col == cw + ln && (PRE ? takes_part(a, sq) : tok < s.cnt && (int64_t)s.P0 + tok < a.ctx);
+  const int P = live ? PRE ? s.PB : s.P0 + tok : -1;
   const int lo = behind(a, P);
   // first and last position of the wave's own columns, and of the halves'
   const int wa = token_of(a, cw);
-  const bool wlive = wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
+  const bool wlive = wa < s.cnt && (PRE || (int64_t)s.P0 + wa < a.ctx);
   auto position = [&](int t) { return (int)min((int64_t)s.P0 + min(t, s.cnt - 1), a.ctx - 1); };
-  const int PA = s.P0 + wa, PB = position(token_of(a, cw + 31));
-  const int A0 = s.PA, B0 = position(last_token(a, chunk_half(a, chunk, 0))), A1 = s.P0 + token_of(a, chunk_half(a, chunk, 1));
+  const int PA = PRE ? s.PA : s.P0 + wa, PB = PRE ? s.PB : position(token_of(a, cw + 31));
+  const int A0 = s.PA, B0 = PRE ? s.PB : position(last_token(a, chunk_half(a, chunk, 0))), A1 = PRE ? s.PA : s.P0 + token_of(a, chunk_half(a, chunk, 1));
   const int kb0 = share(s, split), kb1 = share(s, split + 1);
   const Head hd = head_of<HD, KIND>(a, b, g);
 
@@ -1015,7 +896,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     if (kb0 + 1 < kb1) fetch(kb0 + 1, st1);
     // ---- queries
     {
-      const int64_t at = b * a.q.seq + (int64_t)tok * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
+      const int64_t at = sq.b * a.q.seq + (int64_t)sq.t * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
       float x[KQ][8], mx = 0.f;
 #pragma unroll
       for (int k = 0; k < KQ; k++) {
@@ -1220,8 +1101,8 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       }
     }
   }
-  if constexpr (T != RT_F32) {
-    if (s.S == 1) {
+  if constexpr (T != RT_F32 && !PRE) {
+    if (s.S == 1 && !a.joined) {
       // A lane has 4 dims here and there of its column; by way of the wave's own part of LDS the rows leave in 16-byte pieces
       // next to each other (4096 tokens with 32 heads: 105 -> 101 us)
       constexpr int RS = HD + 8;
@@ -1252,7 +1133,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     }
   }
   if (!live) return;
-  if (s.S == 1) {
+  if (!PRE && s.S == 1 && !a.joined) {
     const float inv = 1.f / l;
     const int64_t at = b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head;
 #pragma unroll
@@ -1264,13 +1145,13 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       }
     return;
   }
-  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head, at = row * a.nsplit + split;
+  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head, at = row * a.slots + a.slot0 + split;
 #pragma unroll
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int i = 0; i < 4; i++)
       *(f32x4 *)(a.part + at * HD + 32 * t + 8 * i + 4 * hf) = (f32x4){o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
-  if (hf == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.nsplit * HD + 2 * at) = make_float2(m, l);
+  if (hf == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD + 2 * at) = make_float2(m, l);
 }
 
 // ------------------------------------------------------------------ launches
@@ -1347,6 +1228,7 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   const int64_t want = (a.many ? 1 : 2) * (int64_t)cus / std::max<int64_t>(groups, 1);
   a.nsplit = tiles <= a.one_tiles ? 1 : (int)std::max<int64_t>(1, std::min({want, (tiles >> a.min_log2) + 1, (int64_t)64}));
   if (a.n > 65535 || a.nchunk * a.nsplit > 65535) a.nsplit = 1;   // grid limits
+  a.slots = a.nsplit; a.slot0 = 0; a.joined = 0;
   return a.nsplit > 1 ? (size_t)a.nseq * a.n * a.heads * a.nsplit * (a.hd + 2) * 4 : 0;
 }
 
@@ -1367,9 +1249,55 @@ hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st) {
     else QPH_KV(k_few16, a.hd, a.q.type, grid, kFewWaves * 64, a);
   }
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.nsplit == 1) return e;
+  if (e != hipSuccess || a.nsplit == 1 || a.joined) return e;
   if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows) QPH_KV(k_kv_merge_rows, a.hd, a.q.type, dim3((a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd), 1, a.nseq), 256, a);   // (at most 32768 rows a sequence: groups <= 256)
   else QPH_KV(k_kv_merge, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ a common prefix
+// Three launches: the sequences' own positions as above, the prefix as if all sequences' tokens were one sequence's, and what joins their sums.
+// `a` is the own part's, planned; the prefix's plan goes by the columns of all sequences
+size_t kv_prefix_plan(KvAttnArgs &a, KvAttnArgs &p) {
+  kv_attn_plan(a);
+  kv_attn_plan(p);
+  p.paired = 0;   // (every column sees all: nothing to even out)
+  a.slots = p.slots = a.nsplit + p.nsplit;
+  p.slot0 = a.nsplit;
+  a.joined = p.joined = 1;
+  return (size_t)a.nseq * a.n * a.heads * a.slots * (a.hd + 2) * 4;
+}
+template <int HD, int T> static constexpr auto k_pre_few4 = k_kv_few<HD, MK_Q4, T, true>;
+template <int HD, int T> static constexpr auto k_pre_few16 = k_kv_few<HD, MK_F32, T, true>;
+template <int HD, int T> static constexpr auto k_pre_many4 = k_kv_many<HD, MK_Q4, T, true>;
+template <int HD, int T> static constexpr auto k_pre_many16 = k_kv_many<HD, MK_F32, T, true>;
+hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvAttnArgs &p, hipStream_t st) {
+  hipError_t e = launch_kv_attn(a, st);
+  if (e != hipSuccess) return e;
+  if (p.many) {
+    const dim3 grid(p.nkv, p.nchunk * p.nsplit, 1);
+    if (p.kind == MK_Q4) QPH_KV(k_pre_many4, p.hd, p.q.type, grid, kManyWaves * 64, p);
+    else QPH_KV(k_pre_many16, p.hd, p.q.type, grid, kManyWaves * 64, p);
+  } else {
+    const dim3 grid(p.nsplit, p.nkv * p.nchunk, 1);
+    if (p.kind == MK_Q4) QPH_KV(k_pre_few4, p.hd, p.q.type, grid, kFewWaves * 64, p);
+    else QPH_KV(k_pre_few16, p.hd, p.q.type, grid, kFewWaves * 64, p);
+  }
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  const KvJoin j{p.prefix, p.tile_log2, p.min_log2, p.one_tiles, p.nsplit};
+#define QPH_JOIN(KERNEL, grid)                                                                                                                  \
+  do {                                                                                                                                          \
+    const dim3 g_ = (grid);                                                                                                                     \
+    if (a.hd == 128 && a.q.type == RT_F32) hipLaunchKernelGGL((KERNEL<128, RT_F32>), g_, dim3(256), 0, st, a, j);                               \
+    else if (a.hd == 128 && a.q.type == RT_F16) hipLaunchKernelGGL((KERNEL<128, RT_F16>), g_, dim3(256), 0, st, a, j);                          \
+    else if (a.hd == 128) hipLaunchKernelGGL((KERNEL<128, RT_BF16>), g_, dim3(256), 0, st, a, j);                                               \
+    else if (a.q.type == RT_F32) hipLaunchKernelGGL((KERNEL<64, RT_F32>), g_, dim3(256), 0, st, a, j);                                          \
+    else if (a.q.type == RT_F16) hipLaunchKernelGGL((KERNEL<64, RT_F16>), g_, dim3(256), 0, st, a, j);                                          \
+    else hipLaunchKernelGGL((KERNEL<64, RT_BF16>), g_, dim3(256), 0, st, a, j);                                                                 \
+  } while (0)
+  if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows || a.n > 65535) QPH_JOIN(k_kv_join_rows, dim3((unsigned)(((int64_t)a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd)), 1, a.nseq));
+  else QPH_JOIN(k_kv_join, dim3(a.heads, a.n, a.nseq));
+#undef QPH_JOIN
   return hipGetLastError();
 }
 

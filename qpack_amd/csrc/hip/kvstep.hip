@@ -1,0 +1,268 @@
+// What a server does to its caches besides kvcache.hip's write, read and attention: append (norms of queries and keys for each head, the position
+// rotation, keys and values into the cache, in one pass) and copy (positions from places of one cache to places of another, or of the same).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kvrec.hpp"
+#include "launch.hpp"
+
+namespace qph {
+
+namespace {
+// ------------------------------------------------------------------ append
+// Rows x of head_dim values, w the norm's weights (or none), c and s the cosines and sines of the token's place:
+//   y = x w / sqrt(mean(x^2) + eps);  y[i], y[i + half] = y[i] c[i] - y[i + half] s[i], y[i + half] c[i] + y[i] s[i], i < half
+// All in fp32, rounded once: queries to their type, keys and values as the cache holds them.
+//
+// EL consecutive dims, from d0 on, of a row on HD / EL consecutive lanes.  The pair's other dims lie in another lane: they are loaded as well (from
+// L1), which keeps the lanes' order free; half is a multiple of EL, so they too follow each other
+template <int HD, int EL>
+__device__ __forceinline__ float row_sum(float v) {   // over the HD / EL lanes of a row
+  static_assert(HD / EL == 8 || HD / EL == 16 || HD / EL == 64, "lanes of a row");
+  if constexpr (HD / EL == 64) return wave_sum(v);
+  v += dpp_f<kDppQuadXor1>(v);
+  v += dpp_f<kDppQuadXor2>(v);
+  v += dpp_f<kDppHalfMirror>(v);
+  if constexpr (HD / EL == 16) v += dpp_f<kDppMirror>(v);
+  return v;
+}
+template <int T, int N>
+__device__ __forceinline__ void load_some(const KvRows &r, int64_t at, float *x) {   // as load_elems, any N
+  if constexpr (N % 8 == 0) load_elems<T, N>(r, at, x);
+  else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if constexpr (T == RT_F32) x[i] = ((const float *)r.p)[at + i];
+      else { const uint16_t h = ((const uint16_t *)r.p)[at + i]; x[i] = T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h); }
+    }
+  }
+}
+// `mine`: the lane's row takes part (all its lanes alike); others leave zeros
+template <int HD, int EL, int T>
+__device__ __forceinline__ void turned(const KvAppendArgs &a, const KvRows &r, int64_t row, const float *w, int64_t place, int d0, bool mine, float *y) {
+  float x[EL], o[EL], c[EL], s[EL];
+  const bool pair = mine && d0 < 2 * a.half, low = d0 < a.half;
+  const int d1 = low ? d0 + a.half : d0 - a.half, i0 = low ? d0 : d1;   // the other dims; the pair's number
+#pragma unroll
+  for (int i = 0; i < EL; i++) x[i] = o[i] = s[i] = 0.f, c[i] = 1.f;
+  if (mine) load_some<T, EL>(r, row + d0, x);
+  if (pair) {
+    load_some<T, EL>(r, row + d1, o);
+#pragma unroll
+    for (int i = 0; i < EL; i++) { c[i] = a.cos_t[place * a.half + i0 + i]; s[i] = a.sin_t[place * a.half + i0 + i]; }
+  }
+  if (w) {
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < EL; i++) q = __builtin_fmaf(x[i], x[i], q);
+    const float f = 1.f / sqrtf(row_sum<HD, EL>(q) * (1.f / HD) + a.eps);
+#pragma unroll
+    for (int i = 0; i < EL; i++) x[i] = x[i] * f * w[d0 + i];
+    if (pair) {
+#pragma unroll
+      for (int i = 0; i < EL; i++) o[i] = o[i] * f * w[d1 + i];
+    }
+  }
+  // (a dim that has no pair is x itself, whatever it is: 0 x NaN and -0 + 0 would change it)
+#pragma unroll
+  for (int i = 0; i < EL; i++) y[i] = pair ? __builtin_fmaf(x[i], c[i], low ? -(o[i] * s[i]) : o[i] * s[i]) : x[i];
+}
+// a sequence's first position and place, and its tokens that take part
+struct Seq { int P0, at; int64_t cnt; };
+__device__ __forceinline__ Seq seq_of(const KvAppendArgs &a, int b) {
+  Seq s;
+  s.P0 = a.io.pos[b];
+  s.at = a.at ? a.at[b] : s.P0;
+  s.cnt = s.P0 < 0 || s.at < 0 ? 0 : min(min((int64_t)tokens_of(a.io.lens, b, a.io.n), a.io.ctx - s.P0), a.places - s.at);
+  return s;
+}
+// the query rows i = token x heads + head, a row on HD / 8 lanes
+template <int HD, int T>
+__device__ __forceinline__ void query(const KvAppendArgs &a, const Seq &s, int b, int i, int lane) {
+  const int t = i / a.heads, h = i - t * a.heads;
+  const bool mine = t < s.cnt;
+  const int d0 = 8 * (lane % (HD / 8));
+  float y[8];
+  turned<HD, 8, T>(a, a.q, b * a.q.seq + (int64_t)t * a.q.tok + (int64_t)h * a.q.head, a.qw, (int64_t)s.at + t, d0, mine, y);
+  if (mine) store_elems<T, 8>(a.out, b * a.out.seq + (int64_t)t * a.out.tok + (int64_t)h * a.out.head + d0, y);
+}
+
+// an fp16 cache: the rows of a token - queries, keys, values - one after the other, 8 dims a thread
+template <int HD, int T>
+__global__ __launch_bounds__(256) void k_append16(KvAppendArgs a) {
+  const int b = blockIdx.z, per = a.heads + 2 * a.io.nkv, lane = threadIdx.x & 63;
+  const Seq s = seq_of(a, b);
+  const int i = blockIdx.x * (256 * 8 / HD) + threadIdx.x / (HD / 8), t = i / per, h = i - t * per;
+  if (t >= s.cnt) return;   // (whole rows)
+  if (h < a.heads) {
+    query<HD, T>(a, s, b, t * a.heads + h, lane);
+    return;
+  }
+  const bool v = h >= a.heads + a.io.nkv;
+  const int g = h - a.heads - (v ? a.io.nkv : 0), d0 = 8 * (lane % (HD / 8));
+  float y[8];
+  if (v) load_elems<T, 8>(a.io.v, b * a.io.v.seq + (int64_t)t * a.io.v.tok + (int64_t)g * a.io.v.head + d0, y);
+  else turned<HD, 8, T>(a, a.io.k, b * a.io.k.seq + (int64_t)t * a.io.k.tok + (int64_t)g * a.io.k.head, a.kw, (int64_t)s.at + t, d0, true, y);
+  u32x4 w;
+#pragma unroll
+  for (int j = 0; j < 4; j++) w[j] = float_to_half_bits(y[2 * j]) | (uint32_t)float_to_half_bits(y[2 * j + 1]) << 16;
+  *(u32x4 *)((uint16_t *)(v ? a.io.cache_v : a.io.cache) + b * a.io.cseq + ((int64_t)s.P0 + t) * a.io.crow + g * HD + d0) = w;
+}
+
+// a 4-bit cache: the first workgroups have a record each (ONE: one token a sequence, a position), waves K and V as k_kv4_write's and k_kv4_write1's; the
+// others query rows
+template <int HD, int T, bool ONE>
+__global__ __launch_bounds__(128) void k_append4(KvAppendArgs a, int records) {
+  __shared__ __align__(16) uint8_t codes[kRec][HD];
+  const int b = blockIdx.z, lane = threadIdx.x & 63, vside = threadIdx.x >> 6;
+  const Seq s = seq_of(a, b);
+  if (s.cnt <= 0) return;
+  if ((int)blockIdx.x >= records) {
+    const int i = (blockIdx.x - records) * (128 * 8 / HD) + threadIdx.x / (HD / 8);
+    if (i / a.heads < s.cnt) query<HD, T>(a, s, b, i, lane);
+    return;
+  }
+  const int g = blockIdx.x % (uint32_t)a.io.nkv;
+  const int64_t rec = s.P0 / kRec + (int64_t)(blockIdx.x / (uint32_t)a.io.nkv), last = s.P0 + s.cnt;
+  if (rec * kRec >= last) return;
+  uint8_t *o = (uint8_t *)a.io.cache + (((int64_t)b * a.io.nkv + g) * a.io.nrec + rec) * (9 * HD);
+  const KvRows &r = vside ? a.io.v : a.io.k;
+  if constexpr (ONE) {
+    constexpr int EL = HD / 64;
+    const int64_t row = b * r.seq + g * r.head;
+    float x[EL];
+    if (vside) { load_some<T, EL>(r, row + EL * lane, x); store_one<HD, T>(o, s.P0 % kRec, x, true, lane); }
+    else { turned<HD, EL, T>(a, r, row, a.kw, s.at, EL * lane, true, x); store_one<HD, RT_F32>(o, s.P0 % kRec, x, false, lane); }
+  } else {
+    constexpr int EL = HD / 8;
+    const int row = lane >> 3, part = lane & 7;
+    const int64_t p = rec * kRec + row, t = p - s.P0, at = b * r.seq + t * r.tok + g * r.head;
+    const bool mine = p >= s.P0 && p < last;
+    const uint32_t keep = kept_bits(rec * kRec, s.P0, last);
+    float x[EL];
+    if (vside) {
+      if (mine) load_elems<T, EL>(r, at + EL * part, x);
+      store_record<HD, T>(o, x, mine, true, row, part, keep, codes);
+    } else {
+      turned<HD, EL, T>(a, r, at, a.kw, s.at + t, EL * part, mine, x);
+      store_record<HD, RT_F32>(o, x, mine, false, row, part, keep, codes);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ copy
+// Position pos[b] + t of sequence b becomes position index[b][t] of the source's sequence seqs[b].  What lies outside either cache takes no part
+struct Place { int seq, p; };   // the source's; p < 0: none
+__device__ __forceinline__ Place place_of(const KvCopyArgs &a, int b, int t) {
+  Place s{a.seqs ? a.seqs[b] : b, a.index[b * a.index_seq + t]};
+  const int P0 = a.pos[b];
+  if (P0 < 0 || t >= tokens_of(a.lens, b, a.n) || (int64_t)P0 + t >= a.ctx || s.seq < 0 || s.seq >= a.src_nseq || s.p >= a.src_ctx) s.p = -1;
+  return s;
+}
+// By way of scratch (what is read and what is written may be the same memory): STAGE 1 gathers the rows into scratch, position t of sequence b, 2 brings
+// them from there; 0 does both at once
+template <int STAGE>
+__global__ __launch_bounds__(256) void k_copy16(KvCopyArgs a) {
+  const int b = blockIdx.z, per = a.nkv * a.hd / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / per;
+  if (t >= a.n) return;
+  const int d = 8 * (int)(i - t * per);
+  const Place s = place_of(a, b, (int)t);
+  if (s.p < 0) return;
+  const int64_t staged = (((int64_t)blockIdx.y * a.nseq + b) * a.n + t) * (8 * per) + d;
+  const uint16_t *src = STAGE == 2 ? (const uint16_t *)a.work + staged : (const uint16_t *)(blockIdx.y ? a.src_v : a.src) + s.seq * a.src_cseq + (int64_t)s.p * a.src_crow + d;
+  uint16_t *dst = STAGE == 1 ? (uint16_t *)a.work + staged : (uint16_t *)(blockIdx.y ? a.cache_v : a.cache) + b * a.cseq + ((int64_t)a.pos[b] + t) * a.crow + d;
+  *(u32x4 *)dst = *(const u32x4 *)src;
+}
+// A workgroup has a record of one kv head: 8 positions whose codes come from up to 8 records.  A thread has a word of K, which stays whole, and one
+// of V, whose 8 codes are one dim's of 8 positions and come from a word each; V words that hold positions outside the call are merged
+template <int HD, int STAGE>
+__global__ __launch_bounds__(HD) void k_copy4(KvCopyArgs a) {
+  const int b = blockIdx.z, g = blockIdx.y, tid = threadIdx.x;
+  const int P0 = a.pos[b];
+  if (P0 < 0) return;
+  const int64_t rec = (STAGE == 1 ? 0 : P0 / kRec) + (int64_t)blockIdx.x;   // in scratch tokens lie from position 0 on
+  const int64_t t0 = rec * kRec - (STAGE == 1 ? 0 : P0), wrec = (a.n + kRec - 1) / kRec;
+  uint8_t *o = STAGE == 1 ? (uint8_t *)a.work + (((int64_t)b * a.nkv + g) * wrec + rec) * (9 * HD) : (uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD);
+  const uint8_t *from[kRec];   // of each position of the record: the source's record, and the place there
+  int at[kRec];
+  uint32_t keep = 0;
+#pragma unroll
+  for (int j = 0; j < kRec; j++) {
+    const int64_t t = t0 + j;
+    const Place s = t >= 0 && t < a.n ? place_of(a, b, (int)t) : Place{0, -1};
+    const int p = STAGE == 2 ? (int)t : s.p;
+    at[j] = s.p < 0 ? -1 : p % kRec;
+    from[j] = STAGE == 2 ? (const uint8_t *)a.work + (((int64_t)b * a.nkv + g) * wrec + p / kRec) * (9 * HD)
+                         : (const uint8_t *)a.src + (((int64_t)s.seq * a.nkv + g) * a.src_nrec + p / kRec) * (9 * HD);
+    if (s.p < 0) keep |= 15u << nib(j);
+  }
+  if (keep == ~0u) return;
+  const int row = tid / (HD / 8);
+  uint32_t v = 0;
+#pragma unroll
+  for (int j = 0; j < kRec; j++) {
+    if (at[j] < 0) continue;
+    v |= (((const uint32_t *)(from[j] + 4 * HD))[tid] >> (16 * (at[j] & 1) + 4 * (at[j] >> 1)) & 15) << nib(j);
+    if (j == row) ((uint32_t *)o)[tid] = ((const uint32_t *)from[j])[at[j] * (HD / 8) + tid % (HD / 8)];
+    // scales: K's of the position follow each other, V's lie 8 positions apart
+    if (tid < HD / 32) ((uint16_t *)(o + 8 * HD))[j * (HD / 32) + tid] = ((const uint16_t *)(from[j] + 8 * HD))[at[j] * (HD / 32) + tid];
+    else if (tid < HD / 16) ((uint16_t *)(o + 8 * HD + HD / 2))[(tid - HD / 32) * kRec + j] = ((const uint16_t *)(from[j] + 8 * HD + HD / 2))[(tid - HD / 32) * kRec + at[j]];
+  }
+  uint32_t *vd = (uint32_t *)(o + 4 * HD) + tid;
+  if (keep) v |= *vd & keep;
+  *vd = v;
+}
+}  // namespace
+
+hipError_t launch_kv_append(int kind, const KvAppendArgs &a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.io.n * (kind == MK_Q4 ? a.heads : a.heads + 2 * a.io.nkv), threads = kind == MK_Q4 ? 128 : 256;
+  const int64_t blocks = (rows * (a.io.hd / 8) + threads - 1) / threads;
+  const int records = kind != MK_Q4 ? 0 : a.io.n == 1 ? a.io.nkv : ((a.io.n + kRec - 1) / kRec + 1) * a.io.nkv;
+  const dim3 grid((unsigned)(records + blocks), 1, a.io.nseq), thr((unsigned)threads);
+#define QPH_APPEND(HD, T)                                                                                  \
+  do {                                                                                                     \
+    if (kind != MK_Q4) hipLaunchKernelGGL((k_append16<HD, T>), grid, thr, 0, st, a);                       \
+    else if (a.io.n == 1) hipLaunchKernelGGL((k_append4<HD, T, true>), grid, thr, 0, st, a, records);      \
+    else hipLaunchKernelGGL((k_append4<HD, T, false>), grid, thr, 0, st, a, records);                      \
+  } while (0)
+  if (a.io.hd == 128) {
+    if (a.q.type == RT_F32) QPH_APPEND(128, RT_F32);
+    else if (a.q.type == RT_F16) QPH_APPEND(128, RT_F16);
+    else QPH_APPEND(128, RT_BF16);
+  } else {
+    if (a.q.type == RT_F32) QPH_APPEND(64, RT_F32);
+    else if (a.q.type == RT_F16) QPH_APPEND(64, RT_F16);
+    else QPH_APPEND(64, RT_BF16);
+  }
+#undef QPH_APPEND
+  return hipGetLastError();
+}
+
+size_t kv_copy_bytes(int kind, int nseq, int nkv, int hd, int n) {
+  return kind == MK_Q4 ? (size_t)kv4_bytes(nseq, nkv, hd, n) : (size_t)4 * nseq * n * nkv * hd;
+}
+template <int STAGE>
+static void launch_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
+  if (kind == MK_Q4) {
+    const dim3 grid((unsigned)((a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1)), a.nkv, a.nseq);
+    if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE>), grid, dim3(128), 0, st, a);
+    else hipLaunchKernelGGL((k_copy4<64, STAGE>), grid, dim3(64), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((k_copy16<STAGE>), dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
+  }
+}
+hipError_t launch_kv_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
+  if (!a.work) {
+    launch_copy<0>(kind, a, st);
+    return hipGetLastError();
+  }
+  launch_copy<1>(kind, a, st);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  launch_copy<2>(kind, a, st);
+  return hipGetLastError();
+}
+
+}  // namespace qph

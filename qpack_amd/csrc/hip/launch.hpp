@@ -314,6 +314,17 @@ struct KvIoArgs {
 };
 hipError_t launch_kv_write(int kind, const KvIoArgs &a, hipStream_t st);
 hipError_t launch_kv_read(int kind, const KvIoArgs &a, hipStream_t st);
+// the pass over a prefix that all sequences follow (launch_kv_prefix): its length (device; null: all of ctx), its cache's positions, the
+// tokens of a sequence and the positions of the sequences' own cache
+struct KvPrefix {
+  const int *len;
+  int64_t ctx, own_ctx;
+  int n;
+};
+struct KvJoin {   // how that pass is laid out
+  KvPrefix prefix;
+  int tile_log2, min_log2, one_tiles, nsplit;
+};
 // tokens 0 .. of sequence b at positions pos[b] .., whose rows are in the cache, over positions p <= P with p > P - window
 // (window > 0) or p < sinks
 struct KvAttnArgs {
@@ -330,11 +341,65 @@ struct KvAttnArgs {
   // set by kv_attn_plan
   int many, paired, cols, half_log2, nchunk, tile_log2, min_log2, one_tiles, nsplit, rep_shift;
   uint32_t rep_mul;
+  // partial sums of a row: `slots` of them, this pass's from slot0 on; joined: they are left there also by a single split
+  int slots, slot0, joined;
+  KvPrefix prefix;              // of a prefix's pass alone
 };
 int kv_few();   // that hook's value now (QPH_KV_FEW)
 // how the call is laid out; the bytes of part
 size_t kv_attn_plan(KvAttnArgs &a);
 hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st);
+// Attention whose sequences follow one prefix: a over their own cache, p over the prefix's with nseq 1 and the tokens of all sequences (prefix.n of each), both with
+// the same q, out, pos, lens and part
+size_t kv_prefix_plan(KvAttnArgs &a, KvAttnArgs &p);
+hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvAttnArgs &p, hipStream_t st);
+
+// ---- kvstep.hip
+// rows q -> out and k, both with their norms (weights qw, kw; null: none) and turned by the angles of places at[b] + t (null: pos[b] + t) of the
+// tables, and v, into the cache; tokens whose place is not in the tables take no part
+struct KvAppendArgs {
+  KvIoArgs io;
+  KvRows q, out;
+  int heads, half;              // half the rotated dims
+  const float *cos_t, *sin_t;   // [places][half]
+  int64_t places;
+  const float *qw, *kw;
+  float eps;
+  const int *at;
+};
+hipError_t launch_kv_append(int kind, const KvAppendArgs &a, hipStream_t st);
+// position pos[b] + t := position index[b index_seq + t] of sequence seqs[b] (null: b) of the source; by way of work where that is given
+struct KvCopyArgs {
+  void *cache, *cache_v;        // as KvIoArgs
+  int64_t cseq, crow, ctx, nrec;
+  const void *src, *src_v;
+  int64_t src_cseq, src_crow, src_ctx, src_nrec;
+  int nseq, src_nseq, nkv, hd, n;
+  const int *index, *pos, *lens, *seqs;
+  int64_t index_seq;
+  void *work;
+};
+size_t kv_copy_bytes(int kind, int nseq, int nkv, int hd, int n);   // of work
+hipError_t launch_kv_copy(int kind, const KvCopyArgs &a, hipStream_t st);
+
+// ---- logprobs.hip: of rows of logits the given tokens' log probabilities, ranks, the entropies and the first `top` alternatives; outputs may be null
+constexpr int kLpTop = 64, kLpSplits = 64;   // alternatives, shares of a row, at most
+struct LogprobArgs {
+  const void *x;
+  int type;                     // RowType
+  int64_t rows, ld;
+  int vocab, top;
+  const int *tokens;            // null, or outside the vocabulary: none
+  float *logp, *entropy;
+  int *rank;
+  int *top_index;
+  float *top_logp;
+  void *work;                   // splits > 1: logprobs_plan's bytes
+  // set by logprobs_plan
+  int splits, share;
+};
+size_t logprobs_plan(LogprobArgs &a);
+hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t st);
 
 // ---- reference-order mode (exact.hip): the reference CPU path's float orders, bit-identical results
 // RMSNorm of `rows` vectors [ldx] with the sequential sum of squares, out [ldo]

@@ -206,7 +206,8 @@ HipLlama::HipLlama(const qph_config &cfg, const qph_tensor *tensors, int n, int 
     vf_ok_ = !half_mats && head_.kind == MK_Q8 && (awo_max_ <= 0 || awo_rows_ || awo_sum_);
     const size_t vn = vf_ok_ ? std::min<size_t>(kVerify, B) : 0;   // tokens of a batch
     // its attention partials and logits are left in the gate / up output's buffer, whatever the context window
-    pf_g_ = (float *)dalloc(4 * std::max(B * ff, vn * std::max<size_t>(V, (size_t)nh * max_chunks_ * (hd + 2))));
+    pf_g_floats_ = std::max(B * ff, vn * std::max<size_t>(V, (size_t)nh * max_chunks_ * (hd + 2)));
+    pf_g_ = (float *)dalloc(4 * pf_g_floats_);
     pf_xh_ = (int8_t *)dalloc(B * pf_ldq_); pf_xl_ = (int8_t *)dalloc(B * pf_ldq_);
     const size_t B16 = (B + 15) / 16 * 16;
     if (q8_mats) {
@@ -648,11 +649,16 @@ void HipLlama::prefill(const int *toks, int n, int want, float *out) {
   if (want && out) memcpy(out, hout_, 4ull * (want == 1 ? cfg_.vocab : cfg_.hidden));
 }
 
+struct HipLlama::Scoring {
+  const int *targets;   // host
+  int top, slice;
+  ScoreOut out;         // host
+};
 // The prompt in chunks of up to pf_cap_ tokens, each layer as matrix products (model_llama.cpp:66-130): per chunk the
 // embeddings, then per layer RMSNorm + quantise -> q / k / v products (+ bias) -> RoPE and the fp16 cache rows ->
 // causal attention -> quantise -> wo product into the residual -> RMSNorm + quantise -> gate product, up product
 // with SwiGLU in its store -> quantise -> down product into the residual.  Leaves the last token's hidden state in x_.
-void HipLlama::prefill_batched(const int *toks, int n) {
+void HipLlama::prefill_batched(const int *toks, int n, const Scoring *sc) {
   // QPH_PF_UNFUSED=bits (test hook): 1 q's RoPE, 2 the attention output's quantisation, 4 the SwiGLU output's
   // quantisation as launches of their own, for bit-for-bit comparisons with the fused kernels
   const int unfused = getenv("QPH_PF_UNFUSED") ? atoi(getenv("QPH_PF_UNFUSED")) : 0;
@@ -775,6 +781,14 @@ void HipLlama::prefill_batched(const int *toks, int n) {
       }
       QPH_CK(launch_gemm(g[0], st_));
     }
+    if (sc) {   // the head over the chunk's tokens, as many at a time as their logits fit where gate / up were
+      for (int r = 0; r < B; r += sc->slice) {
+        const int rows = std::min(sc->slice, B - r);
+        GemmArgs g = product(sc_head_, pf_g_, cfg_.vocab, nullptr, false, rows);
+        products(PRO_NORM, pf_x_ + (size_t)r * d, d, fnorm_, d, rows, &g, 1);
+        score_rows(pf_g_, s0 + r, rows, *sc);
+      }
+    }
     pos_ += B;
   }
   QPH_CK(hipMemcpyAsync(x_, pf_x_ + (size_t)(B - 1) * d, 4ull * d, hipMemcpyDeviceToDevice, st_));
@@ -798,6 +812,73 @@ void HipLlama::prefill_topk(const int *toks, int n, int M, int *idx, float *val)
   if (n <= 0) throw std::runtime_error("prefill: no tokens");
   prefill(toks, n, 3, nullptr);
   topk_to_host(M, idx, val);
+}
+
+// the logits of tokens at .. at + rows - 1 (at most pf_cap_) of a call
+void HipLlama::score_rows(const float *logits, int at, int rows, const Scoring &sc) {
+  QPH_CK(hipMemcpyAsync(sc_tok_, sc.targets + at, 4ull * rows, hipMemcpyHostToDevice, st_));
+  LogprobArgs a{}; a.x = logits; a.type = RT_F32; a.rows = rows; a.ld = cfg_.vocab; a.vocab = cfg_.vocab; a.top = sc.out.top_index || sc.out.top_logp ? sc.top : 0;
+  a.tokens = sc_tok_; a.logp = sc_out_; a.entropy = sc_out_ + pf_cap_; a.rank = (int *)sc_out_ + 2 * pf_cap_;
+  a.top_index = (int *)sc_out_ + 3 * pf_cap_; a.top_logp = sc_out_ + (3 + kLpTop) * (size_t)pf_cap_;
+  const size_t bytes = logprobs_plan(a);
+  if (bytes > sc_work_bytes_) {   // (more rows need fewer shares of each: a few calls settle it)
+    QPH_CK(hipStreamSynchronize(st_));
+    dfree(sc_work_);
+    sc_work_ = nullptr; sc_work_bytes_ = 0;
+    sc_work_ = dalloc(bytes);
+    sc_work_bytes_ = bytes;
+  }
+  a.work = sc_work_;
+  QPH_CK(launch_logprobs(a, st_));
+  auto back = [&](void *to, const void *from, int per) {
+    if (to) QPH_CK(hipMemcpyAsync((uint8_t *)to + 4ull * at * per, from, 4ull * rows * per, hipMemcpyDeviceToHost, st_));
+  };
+  back(sc.out.logp, a.logp, 1); back(sc.out.entropy, a.entropy, 1); back(sc.out.rank, a.rank, 1);
+  if (a.top) { back(sc.out.top_index, a.top_index, a.top); back(sc.out.top_logp, a.top_logp, a.top); }
+}
+void HipLlama::score(const int *toks, const int *targets, int n, int top, const ScoreOut &out) {
+  if (top < 0 || top > std::min(kLpTop, cfg_.vocab)) throw std::runtime_error("score: top must be in [0, min(64, vocab)]");
+  if (n <= 0) return;
+  if (pos_ + n > ctx_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
+  for (int i = 0; i < n; i++) if (toks[i] < 0 || toks[i] >= cfg_.vocab) throw std::runtime_error("token id out of range");
+  std::vector<int> next;
+  if (!targets) {
+    next.assign(toks + 1, toks + n);
+    next.push_back(-1);
+    targets = next.data();
+  }
+  if (!sc_out_) {
+    sc_tok_ = (int *)dalloc(4ull * pf_cap_);
+    sc_out_ = (float *)dalloc(4ull * pf_cap_ * (3 + 2 * kLpTop));
+  }
+  Scoring sc{targets, top, (int)std::min<size_t>(pf_g_floats_ / cfg_.vocab, pf_cap_), out};
+  // the prompt's products take the head too where its kind's activation planes are there; else, and in the reference order, decode steps
+  const bool batched = !order_ && n > 1 && sc.slice > 0 && (head_.kind == MK_Q8 || (head_.kind == MK_Q4 && pf_fp_)) && !getenv("QPH_PREFILL_STEPS");
+  if (batched) {
+    if (!sc_head_.q) {
+      DMat m = head_;
+      if (m.kind == MK_Q8 && !pf_th_) {   // no layer is q8
+        const size_t planes = (size_t)(pf_cap_ + 15) / 16 * 16 * pf_ldq_;
+        pf_tl_ = (int8_t *)dalloc(planes);
+        pf_th_ = (int8_t *)dalloc(planes);
+      }
+      if (m.kind == MK_Q8 && !m.rs) {
+        int *rs = (int *)dalloc(4ull * ws_pitch(m.rows) * (m.cols / 128));
+        QPH_CK(launch_rowsum_q8((const int8_t *)m.q, m.rows, m.cols, rs, st_));
+        m.rs = rs;
+      } else if (m.kind == MK_Q4 && !m.st) {
+        uint16_t *t = (uint16_t *)dalloc(2ull * m.rows * (m.cols / 32));
+        QPH_CK(launch_scale_blocks(m.kind, (const uint16_t *)m.s, m.rows, m.cols, t, st_));
+        m.st = t;
+      }
+      sc_head_ = m;
+    }
+    prefill_batched(toks, n, &sc);
+  } else {
+    for (int i = 0; i < n; i++) { step(toks[i], 3, nullptr); score_rows(logits_, i, 1, sc); }
+  }
+  QPH_CK(hipStreamSynchronize(st_));
+  check_status();
 }
 
 int HipLlama::greedy_run(int tok, int n, int *out) {

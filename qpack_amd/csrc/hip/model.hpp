@@ -36,6 +36,10 @@ class HipLlama {
   // sampler's order (1 <= M <= min(kTopkMax, vocab))
   void step_topk(int tok, int M, int *idx, float *val);
   void prefill_topk(const int *toks, int n, int M, int *idx, float *val);
+  // feeds n tokens and gives, for each, the log probability and rank of targets[i] (null: the next token; outside the vocabulary: none) behind it, the
+  // entropy and the `top` (<= kLpTop) most probable tokens; outputs [n] and [n][top], any null
+  struct ScoreOut { float *logp, *entropy; int *rank, *top_index; float *top_logp; };
+  void score(const int *toks, const int *targets, int n, int top, const ScoreOut &out);
   void reset() { pos_ = 0; clean_pos_ = 0; }
   bool rewind(int pos) {
     if (pos < 0 || pos > pos_) return false;
@@ -186,7 +190,15 @@ class HipLlama {
   float *pf_xb2_ = nullptr, *pf_xbt2_ = nullptr;
   uint16_t *pf_fp_ = nullptr;   // the q4 / q1 products' planes (PfQuantArgs::fp), for models with such layers
   int *pf_tok_ = nullptr;
-  void prefill_batched(const int *toks, int n);
+  struct Scoring;   // what prefill_batched does with each chunk's hidden states, for score
+  void prefill_batched(const int *toks, int n, const Scoring *sc = nullptr);
+  // device memory of score, taken by its first call: the head as a prompt product's matrix, targets and results of a chunk
+  DMat sc_head_{};
+  int *sc_tok_ = nullptr;
+  float *sc_out_ = nullptr;
+  void *sc_work_ = nullptr;
+  size_t sc_work_bytes_ = 0, pf_g_floats_ = 0;
+  void score_rows(const float *logits, int at, int rows, const Scoring &sc);
   // prefill_all in batches of up to kVerify tokens whose every logit equals its decode step's bit for bit (q8 models)
   static constexpr int kVerify = 16;
   bool vf_ok_ = false;

@@ -1,8 +1,9 @@
-// The Python side of the kv entry points (qpack_amd._kvbind, used by qpack_amd/kvcache.py): checks tensors and calls the C ABI.  A step's
+// The Python side of the kv entry points and of qph_logprobs (qpack_amd._kvbind, used by qpack_amd/kvcache.py and tokenprobs.py): checks tensors and calls the C ABI.  A step's
 // kernels take 3 to 8 us each; the checks through ctypes took 10 us a call (15 with scratch), through the tensors' Python attributes
 // 4.5 (8.5 with scratch and a second launch), from torch's own structures 3.5 (7.7); each launch is about 3 of it.
 // torch is loaded before this module is.
 #define PY_SSIZE_T_CLEAN
+#include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -36,10 +37,14 @@ bool fail(const char *fmt, const char *a, const char *b = "") {
   PyErr_Format(g_error, fmt, a, b);
   return false;
 }
-bool tensor(const Cache *c, PyObject *x, const char *name, const at::Tensor **t) {   // on the cache's device
-  if (!THPVariable_Check(x)) return fail("kv: %s must be a tensor%s", name);
+bool tensor(PyObject *x, const char *name, const at::Tensor **t, const char *call = "kv") {
+  if (!THPVariable_Check(x)) return fail("%s: %s must be a tensor", call, name);
   *t = &THPVariable_Unpack(x);
-  if ((*t)->requires_grad() && c10::GradMode::is_enabled()) return fail("kv: %s requires a gradient, and no call here passes one on: detach it, or call under torch.no_grad()%s", name);
+  if ((*t)->requires_grad() && c10::GradMode::is_enabled()) return fail("%s: %s requires a gradient, and no call here passes one on: detach it, or call under torch.no_grad()", call, name);
+  return true;
+}
+bool tensor(const Cache *c, PyObject *x, const char *name, const at::Tensor **t) {   // on the cache's device
+  if (!tensor(x, name, t)) return false;
   if (!(*t)->is_cuda() || (*t)->get_device() != c->device) return fail("kv: %s is not on the cache's device%s", name);
   return true;
 }
@@ -66,37 +71,50 @@ bool rows(const Cache *c, PyObject *x, const char *name, qph_rows *r, int64_t *n
   if (*n == 0 && !r->p) r->p = (void *)16;   // a tensor without elements may have no memory: nothing of it is read
   return true;
 } catch (...) { return fail("kv: %s is not a plain tensor%s", name); }   // (nested or fake ones: torch throws)
-bool index(const Cache *c, PyObject *x, const char *name, const int **p) try {   // int32 [nseq]; None: NULL
-  if (x == Py_None && !strcmp(name, "lens")) { *p = nullptr; return true; }
+bool index(const Cache *c, PyObject *x, const char *name, const int **p, bool may_lack = false, int64_t n = -1) try {   // int32 [n], or [nseq]; None: NULL
+  if (n < 0) n = c->c.nseq;
+  if (x == Py_None && may_lack) { *p = nullptr; return true; }
   const at::Tensor *t;
   if (!tensor(c, x, name, &t)) return false;
-  if (t->scalar_type() != at::kInt || t->layout() != at::kStrided || t->dim() != 1 || t->size(0) != c->c.nseq || !t->is_contiguous()) {
-    PyErr_Format(g_error, "kv: %s must be a contiguous int32 tensor [%d]", name, c->c.nseq);
+  if (t->scalar_type() != at::kInt || t->layout() != at::kStrided || t->dim() != 1 || t->size(0) != n || !t->is_contiguous()) {
+    PyErr_Format(g_error, "kv: %s must be a contiguous int32 tensor [%lld]", name, (long long)n);
     return false;
   }
   *p = (const int *)t->data_ptr();
   return true;
 } catch (...) { return fail("kv: %s is not a plain tensor%s", name); }
-bool stream_of(const Cache *c, void **st) {
-  Ref d(PyLong_FromLongLong(c->device));
+// float32, contiguous, of these sizes (last < 0: any); None: NULL
+bool floats(const Cache *c, PyObject *x, const char *name, int64_t dims, int64_t last, const float **p, const at::Tensor **t) try {
+  if (x == Py_None && dims == 1) { *p = nullptr; return true; }
+  if (!tensor(c, x, name, t)) return false;
+  if ((*t)->scalar_type() != at::kFloat || (*t)->layout() != at::kStrided || (*t)->dim() != dims || (last >= 0 && (*t)->size(dims - 1) != last) || !(*t)->is_contiguous())
+    return fail("kv: %s must be a contiguous float32 tensor %s", name, dims == 1 ? "[head_dim]" : "[places, half the rotated dims], cos and sin alike");
+  *p = (const float *)(*t)->data_ptr();
+  return true;
+} catch (...) { return fail("kv: %s is not a plain tensor%s", name); }
+bool stream_of(int64_t device, void **st) {
+  Ref d(PyLong_FromLongLong(device));
   Ref v(PyObject_CallOneArg(g_stream, d));
   if (!v.p) return false;
   *st = PyLong_AsVoidPtr(v);
   return !PyErr_Occurred();
 }
-// runs f on the cache's device; a switch only where another one is current
-bool current(const Cache *c, bool *yes) {
+// runs f on the tensors' device; a switch only where another one is current
+bool current(int64_t device, bool *yes) {
   Ref now(PyObject_CallNoArgs(g_device));
   if (!now.p) return false;
-  *yes = PyLong_AsLongLong(now) == c->device;
+  *yes = PyLong_AsLongLong(now) == device;
   return !PyErr_Occurred();
 }
 template <typename F>
-bool launch(const Cache *c, bool here, void *st, const F &f) {
+bool launch(int64_t device, const F &f) {
+  bool here;
+  void *st;
+  if (!current(device, &here) || !stream_of(device, &st)) return false;
   int rc;
   if (here) rc = f(st);
   else {
-    Ref d(PyLong_FromLongLong(c->device));
+    Ref d(PyLong_FromLongLong(device));
     Ref guard(PyObject_CallOneArg(g_guard, d));
     Ref in(guard.p ? PyObject_CallMethod(guard, "__enter__", nullptr) : nullptr);
     if (!in.p) return false;
@@ -125,46 +143,175 @@ PyObject *io(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   qph_rows k, v;
   int64_t nk, nv, hk, hv;
   const int *pos, *lens;
-  if (!nargs(na, 4) || !rows(c, arg[0], "k", &k, &nk, &hk) || !rows(c, arg[1], "v", &v, &nv, &hv) || !index(c, arg[2], "pos", &pos) || !index(c, arg[3], "lens", &lens))
+  if (!nargs(na, 4) || !rows(c, arg[0], "k", &k, &nk, &hk) || !rows(c, arg[1], "v", &v, &nv, &hv) || !index(c, arg[2], "pos", &pos) || !index(c, arg[3], "lens", &lens, true))
     return nullptr;
   if (nk != nv) { fail("kv: k and v have different numbers of tokens%s%s", ""); return nullptr; }
   if (hk != c->c.kv_heads || hv != c->c.kv_heads) { PyErr_Format(g_error, "kv: k and v must have %d heads", c->c.kv_heads); return nullptr; }
   if (nk > INT32_MAX) { fail("kv: too many tokens%s%s", ""); return nullptr; }
-  bool here;
-  void *st;
-  if (!current(c, &here) || !stream_of(c, &st)) return nullptr;
-  if (!launch(c, here, st, [&](void *st) { return (WRITE ? qph_kv_write : qph_kv_read)(&c->c, &k, &v, (int)nk, pos, lens, st); })) return nullptr;
+  if (!launch(c->device, [&](void *st) { return (WRITE ? qph_kv_write : qph_kv_read)(&c->c, &k, &v, (int)nk, pos, lens, st); })) return nullptr;
   for (PyObject *t : {WRITE ? c->data : arg[0], WRITE ? c->data_v : arg[1]})
     if (t) written(THPVariable_Unpack(t));
   Py_RETURN_NONE;
+}
+// scratch of this call alone: the allocator gives it to the stream's later work, or to the graph that is being captured
+bool scratch(const Cache *c, int64_t bytes, PyObject **work, void **p) {
+  *work = nullptr; *p = nullptr;
+  if (!bytes) return true;
+  Ref size(PyLong_FromLongLong((bytes + c->item - 1) / c->item));
+  *work = PyObject_CallMethodOneArg(c->data, s_new_empty, size);
+  if (!*work) return false;
+  *p = THPVariable_Unpack(*work).data_ptr();
+  return true;
+}
+bool scale_of(PyObject *x, float *scale) {
+  const double y = PyFloat_AsDouble(x);
+  if (PyErr_Occurred()) return false;
+  *scale = (float)y;
+  return y == 0 || *scale != 0.f || fail("kv: scale is too small%s%s", "");   // (0 means the default)
+}
+bool attend_rows(const Cache *c, PyObject *const *arg, qph_rows *q, qph_rows *o, int64_t *n, int64_t *h, const int **pos, const int **lens) {   // (q, out, pos, lens)
+  int64_t n2, h2;
+  if (!rows(c, arg[0], "q", q, n, h) || !rows(c, arg[1], "out", o, &n2, &h2) || !index(c, arg[2], "pos", pos) || !index(c, arg[3], "lens", lens, true)) return false;
+  if (*n != n2 || *h != h2) return fail("kv: out must have q's shape%s%s", "");
+  return (*n <= INT32_MAX && *h <= INT32_MAX) || fail("kv: q is too large%s%s", "");
 }
 // attention(q, out, pos, lens, window, sinks, scale)
 PyObject *attention(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   const Cache *c = (const Cache *)self;
   qph_rows q, o;
-  int64_t n, n2, h, h2, bytes = 0;
+  int64_t n, h, bytes = 0;
   const int *pos, *lens;
   int window, sinks;
-  if (!nargs(na, 7) || !rows(c, arg[0], "q", &q, &n, &h) || !rows(c, arg[1], "out", &o, &n2, &h2) || !index(c, arg[2], "pos", &pos) || !index(c, arg[3], "lens", &lens) ||
-      !integer(arg[4], "window", &window) || !integer(arg[5], "sinks", &sinks))
-    return nullptr;
-  const double scale = PyFloat_AsDouble(arg[6]);
-  if (PyErr_Occurred()) return nullptr;
-  if (scale != 0 && (float)scale == 0.f) { fail("kv: scale is too small%s%s", ""); return nullptr; }   // (0 means the default)
-  if (n != n2 || h != h2) { fail("kv: out must have q's shape%s%s", ""); return nullptr; }
-  if (n > INT32_MAX || h > INT32_MAX) { fail("kv: q is too large%s%s", ""); return nullptr; }
+  float scale;
+  if (!nargs(na, 7) || !attend_rows(c, arg, &q, &o, &n, &h, &pos, &lens) || !integer(arg[4], "window", &window) || !integer(arg[5], "sinks", &sinks) || !scale_of(arg[6], &scale)) return nullptr;
   if (qph_kv_attention_work(&c->c, q.type, (int)h, (int)n, window, sinks, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
-  bool here;
-  void *st, *w = nullptr;
-  if (!current(c, &here) || !stream_of(c, &st)) return nullptr;
-  // scratch of this call alone: the allocator gives it to the stream's later work, or to the graph that is being captured
-  Ref size(bytes ? PyLong_FromLongLong((bytes + c->item - 1) / c->item) : nullptr), work(bytes ? PyObject_CallMethodOneArg(c->data, s_new_empty, size) : nullptr);
-  if (bytes && !work.p) return nullptr;
-  if (bytes) w = THPVariable_Unpack(work.p).data_ptr();
-  if (!launch(c, here, st, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, (float)scale, w, bytes, st); })) return nullptr;
+  PyObject *keep;
+  void *w;
+  if (!scratch(c, bytes, &keep, &w)) return nullptr;
+  Ref work(keep);
+  if (!launch(c->device, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, scale, w, bytes, st); })) return nullptr;
   written(THPVariable_Unpack(arg[1]));
   Py_RETURN_NONE;
 }
+PyTypeObject cache_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+bool cache_of(const Cache *c, PyObject *x, const char *name, const Cache **y) {
+  if (!PyObject_TypeCheck(x, &cache_type)) { PyErr_Format(PyExc_TypeError, "%s must be a cache", name); return false; }
+  *y = (const Cache *)x;
+  return (*y)->device == c->device || fail("kv: %s is not on the cache's device%s", name);
+}
+// attention_prefix(q, out, pos, lens, scale, prefix, prefix_len)
+PyObject *attention_prefix(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
+  const Cache *c = (const Cache *)self, *p;
+  qph_rows q, o;
+  int64_t n, h, bytes = 0;
+  const int *pos, *lens, *plen;
+  float scale;
+  if (!nargs(na, 7) || !attend_rows(c, arg, &q, &o, &n, &h, &pos, &lens) || !scale_of(arg[4], &scale) || !cache_of(c, arg[5], "prefix", &p) || !index(c, arg[6], "prefix_len", &plen, true, 1)) return nullptr;
+  if (qph_kv_attention_prefix_work(&c->c, &p->c, q.type, (int)h, (int)n, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
+  PyObject *keep;
+  void *w;
+  if (!scratch(c, bytes, &keep, &w)) return nullptr;
+  Ref work(keep);
+  if (!launch(c->device, [&](void *st) { return qph_kv_attention_prefix(&c->c, &p->c, plen, &q, &o, (int)h, (int)n, pos, lens, scale, w, bytes, st); })) return nullptr;
+  written(THPVariable_Unpack(arg[1]));
+  Py_RETURN_NONE;
+}
+// append(q, k, v, out, pos, lens, cos, sin, at, q_weight, k_weight, eps)
+PyObject *append(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
+  const Cache *c = (const Cache *)self;
+  qph_rows r[4];
+  int64_t n[4], h[4];
+  const char *names[4] = {"q", "k", "v", "out"};
+  const int *pos, *lens;
+  qph_turn t{};
+  const at::Tensor *cos, *sin, *w;
+  if (!nargs(na, 12)) return nullptr;
+  for (int i = 0; i < 4; i++)
+    if (!rows(c, arg[i], names[i], &r[i], &n[i], &h[i])) return nullptr;
+  if (!index(c, arg[4], "pos", &pos) || !index(c, arg[5], "lens", &lens, true) || !floats(c, arg[6], "cos", 2, -1, &t.cos, &cos) || !floats(c, arg[7], "sin", 2, cos->size(1), &t.sin, &sin) ||
+      !index(c, arg[8], "at", &t.at, true) || !floats(c, arg[9], "q_weight", 1, c->c.head_dim, &t.q_norm, &w) || !floats(c, arg[10], "k_weight", 1, c->c.head_dim, &t.k_norm, &w)) return nullptr;
+  const double eps = PyFloat_AsDouble(arg[11]);
+  if (PyErr_Occurred()) return nullptr;
+  if (n[1] != n[0] || n[2] != n[0]) { fail("kv: q, k and v have different numbers of tokens%s%s", ""); return nullptr; }
+  if (n[3] != n[0] || h[3] != h[0]) { fail("kv: out must have q's shape%s%s", ""); return nullptr; }
+  if (h[1] != c->c.kv_heads || h[2] != c->c.kv_heads) { PyErr_Format(g_error, "kv: k and v must have %d heads", c->c.kv_heads); return nullptr; }
+  if (sin->size(0) != cos->size(0)) { fail("kv: cos and sin must have the same shape%s%s", ""); return nullptr; }
+  if (n[0] > INT32_MAX || h[0] > INT32_MAX || cos->size(1) > INT32_MAX) { fail("kv: q or cos is too large%s%s", ""); return nullptr; }
+  t.places = cos->size(0); t.half = (int)cos->size(1); t.eps = (float)eps;
+  if (!launch(c->device, [&](void *st) { return qph_kv_append(&c->c, &r[0], &r[1], &r[2], &r[3], (int)h[0], (int)n[0], pos, lens, &t, st); })) return nullptr;
+  for (PyObject *x : {c->data, c->data_v, (PyObject *)arg[3]})
+    if (x) written(THPVariable_Unpack(x));
+  Py_RETURN_NONE;
+}
+// copy(source, index, pos, lens, seqs, apart)
+PyObject *copy(PyObject *self, PyObject *const *arg, Py_ssize_t na) try {
+  const Cache *c = (const Cache *)self, *src;
+  const at::Tensor *x;
+  const int *pos, *lens, *seqs;
+  int64_t bytes = 0;
+  if (!nargs(na, 6) || !cache_of(c, arg[0], "source", &src) || !tensor(c, arg[1], "index", &x) || !index(c, arg[2], "pos", &pos) || !index(c, arg[3], "lens", &lens, true) ||
+      !index(c, arg[4], "seqs", &seqs, true)) return nullptr;
+  const int apart = PyObject_IsTrue(arg[5]);
+  if (apart < 0) return nullptr;
+  if (x->scalar_type() != at::kInt || x->layout() != at::kStrided || x->dim() != 2 || x->size(0) != c->c.nseq || (x->size(1) > 1 && x->stride(1) != 1)) {
+    PyErr_Format(g_error, "kv: index must be an int32 tensor [%d, n] with contiguous rows", c->c.nseq);
+    return nullptr;
+  }
+  const int64_t n = x->size(1);
+  if (n > INT32_MAX) { fail("kv: too many tokens%s%s", ""); return nullptr; }
+  const int *at = n ? (const int *)x->data_ptr() : (const int *)16;
+  if (qph_kv_copy_work(&c->c, &src->c, (int)n, apart, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
+  PyObject *keep;
+  void *w;
+  if (!scratch(c, bytes, &keep, &w)) return nullptr;
+  Ref work(keep);
+  if (!launch(c->device, [&](void *st) { return qph_kv_copy(&c->c, &src->c, at, x->stride(0), (int)n, pos, lens, seqs, apart, w, bytes, st); })) return nullptr;
+  for (PyObject *y : {c->data, c->data_v})
+    if (y) written(THPVariable_Unpack(y));
+  Py_RETURN_NONE;
+} catch (...) { fail("kv: index is not a plain tensor%s%s", ""); return nullptr; }
+
+// logprobs(logits, tokens, top) -> (logp, entropy, rank, top_index, top_logp)
+PyObject *logprobs(PyObject *, PyObject *const *arg, Py_ssize_t na) try {
+  const at::Tensor *x, *tok = nullptr;
+  int top, type;
+  if (!nargs(na, 3) || !tensor(arg[0], "logits", &x, "logprobs") || (arg[1] != Py_None && !tensor(arg[1], "tokens", &tok, "logprobs")) || !integer(arg[2], "top", &top)) return nullptr;
+  switch (x->scalar_type()) {
+    case at::kFloat: type = QPH_F32; break;
+    case at::kHalf: type = QPH_F16; break;
+    case at::kBFloat16: type = QPH_BF16; break;
+    default: fail("logprobs: logits must be float32, float16 or bfloat16%s%s", ""); return nullptr;
+  }
+  if (x->layout() != at::kStrided || x->dim() != 2 || (x->size(1) > 1 && x->stride(1) != 1) || x->size(1) > INT32_MAX) { fail("logprobs: logits must be [rows, vocab] with contiguous rows%s%s", ""); return nullptr; }
+  if (!x->is_cuda()) { fail("logprobs: logits must be on a GPU%s%s", ""); return nullptr; }
+  const int64_t rows = x->size(0), device = x->get_device();
+  if (tok && (tok->scalar_type() != at::kInt || tok->layout() != at::kStrided || tok->dim() != 1 || tok->size(0) != rows || !tok->is_contiguous())) {
+    PyErr_Format(g_error, "logprobs: tokens must be a contiguous int32 tensor [%lld]", (long long)rows);
+    return nullptr;
+  }
+  if (tok && (!tok->is_cuda() || tok->get_device() != device)) { fail("logprobs: tokens are not on the logits' device%s%s", ""); return nullptr; }
+  int64_t bytes = 0;
+  if (qph_logprobs_work(type, rows, (int)x->size(1), top, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
+  const auto f32 = at::TensorOptions().device(x->device()).dtype(at::kFloat), i32 = f32.dtype(at::kInt);
+  at::Tensor logp, rank, work, entropy = at::empty({rows}, f32), ti = at::empty({rows, top}, i32), tl = at::empty({rows, top}, f32);
+  if (tok) { logp = at::empty({rows}, f32); rank = at::empty({rows}, i32); }
+  if (bytes) work = at::empty({(bytes + 3) / 4}, f32);
+  auto at = [](at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+  if (!launch(device, [&](void *st) {
+        return qph_logprobs(x->data_ptr(), type, rows, (int)x->size(1), x->stride(0), tok ? (const int *)tok->data_ptr() : nullptr, top, (float *)at(logp), (float *)at(entropy), (int *)at(rank),
+                            (int *)at(ti), (float *)at(tl), at(work), bytes, st);
+      }))
+    return nullptr;
+  PyObject *out = PyTuple_New(5);
+  if (!out) return nullptr;
+  int i = 0;
+  for (at::Tensor *t : {&logp, &entropy, &rank, &ti, &tl}) {
+    PyObject *y = t->defined() ? THPVariable_Wrap(*t) : Py_NewRef(Py_None);
+    if (!y) { Py_DECREF(out); return nullptr; }
+    PyTuple_SET_ITEM(out, i++, y);
+  }
+  return out;
+} catch (const std::exception &e) { if (!PyErr_Occurred()) fail("logprobs: %s%s", e.what()); return nullptr; }
 
 int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_heads, head_dim, ctx, k, v, seq, row, device, data[, the fp16 V's])
   Cache *c = (Cache *)self;
@@ -190,8 +337,10 @@ PyMethodDef cache_methods[] = {
     {"write", (PyCFunction)(void (*)(void))io<true>, METH_FASTCALL, "write(k, v, pos, lens)"},
     {"read", (PyCFunction)(void (*)(void))io<false>, METH_FASTCALL, "read(k, v, pos, lens)"},
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "attention(q, out, pos, lens, window, sinks, scale)"},
+    {"attention_prefix", (PyCFunction)(void (*)(void))attention_prefix, METH_FASTCALL, "attention_prefix(q, out, pos, lens, scale, prefix, prefix_len)"},
+    {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, "append(q, k, v, out, pos, lens, cos, sin, at, q_weight, k_weight, eps)"},
+    {"copy", (PyCFunction)(void (*)(void))copy, METH_FASTCALL, "copy(source, index, pos, lens, seqs, apart)"},
     {nullptr, nullptr, 0, nullptr}};
-PyTypeObject cache_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
 // setup(QphError, raw stream of a device, current device, device guard)
 PyObject *setup(PyObject *, PyObject *args) {
@@ -199,7 +348,8 @@ PyObject *setup(PyObject *, PyObject *args) {
   for (PyObject *p : {g_error, g_stream, g_device, g_guard}) Py_INCREF(p);
   Py_RETURN_NONE;
 }
-PyMethodDef module_methods[] = {{"setup", setup, METH_VARARGS, "the names that the module uses of Python's side"}, {nullptr, nullptr, 0, nullptr}};
+PyMethodDef module_methods[] = {{"setup", setup, METH_VARARGS, "the names that the module uses of Python's side"},
+                                {"logprobs", (PyCFunction)(void (*)(void))logprobs, METH_FASTCALL, "logprobs(logits, tokens, top)"}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvbind", nullptr, -1, module_methods};
 }  // namespace
 

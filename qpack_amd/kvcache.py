@@ -79,6 +79,27 @@ class KvCache:
         self.data, self.device = data, first.device
         self._c = _binding().Cache(self.kind, self.nseq, self.kv_heads, self.head_dim, self.ctx, *at, self.device.index, *tensors)
 
+    def append(self, q, k, v, pos, cos, sin, q_weight=None, k_weight=None, eps=1e-6, at=None, lens=None, out=None):
+        """a step's projections to its cache: norms (where q_weight, k_weight, float32 [head_dim], are given) of the rows q [nseq, n, heads, head_dim] and k, v
+        [nseq, n, kv_heads, head_dim] of one type, the rotation, and k and v into the cache.  Returns the queries, rounded to their type (in out where given, which
+        may be q; rows that take no part stay as they are in out, and are zero without it).
+
+        cos, sin: float32 [places, r]: dims i and i + r of a row are turned by the angle of the token's place, at[b] + t (at None: pos[b] + t; int32 [nseq]), i < r, others
+        stay; r a multiple of head_dim / 8.  Tokens whose place is outside the tables take no part.  All in fp32, rounded once"""
+        if out is None:
+            import torch
+            out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        self._c.append(q, k, v, out, pos, lens, cos, sin, at, q_weight, k_weight, eps)
+        return out
+
+    def copy(self, index, pos, lens=None, seqs=None, source=None, apart=False):
+        """position pos[b] + t becomes position index[b, t] of sequence seqs[b] (None: b) of source (None: this cache), to the bit.  index: int32 [nseq, n], rows contiguous (they may
+        be one row, expanded); seqs: int32 [nseq].  Sequences and positions outside the source take no part.
+
+        All is read before anything is written (a second pass by way of scratch, where the caches share memory).  apart=True promises that no position that the call
+        writes is read by it, as when one sequence is forked into others: one pass"""
+        self._c.copy((source or self)._c, index, pos, lens, seqs, apart)
+
     def write(self, k, v, pos, lens=None):
         """round the rows k and v [nseq, n, kv_heads, head_dim] into the cache"""
         self._c.write(k, v, pos, lens)
@@ -96,12 +117,22 @@ class KvCache:
         self._c.read(k, v, pos, lens)
         return out
 
-    def attention(self, q, pos, lens=None, window=0, sinks=0, scale=0.0, out=None):
+    def attention(self, q, pos, lens=None, window=0, sinks=0, scale=0.0, out=None, prefix=None, prefix_len=None):
         """softmax(scale q K^T) V of the tokens q [nseq, n, heads, head_dim] at pos[b] + t, whose rows are in the cache; scale 0: 1 /
         sqrt(head_dim).  Position P sees p <= P and, with window > 0, of those p > P - window and p < sinks only.  out may be q, or apart from it; rows that
-        take no part stay as they are in out, and are zero without it"""
+        take no part stay as they are in out, and are zero without it.
+
+        prefix: a cache of one sequence (of this one's kind, kv_heads and head_dim) whose first prefix_len positions (int32 [1], None: all) every token sees before its own
+        sequence's; it is read once for all sequences.  A window and a prefix exclude each other"""
         if out is None:
             import torch
             out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        if prefix is not None:
+            if window or sinks:
+                raise QphError("kv: a window and a prefix exclude each other")
+            self._c.attention_prefix(q, out, pos, lens, scale, prefix._c, prefix_len)
+            return out
+        if prefix_len is not None:
+            raise QphError("kv: prefix_len without a prefix")
         self._c.attention(q, out, pos, lens, window, sinks, scale)
         return out

@@ -6,7 +6,8 @@ import mmap
 
 import numpy as np
 
-from ._lib import QPH_F16, QPH_Q4, Config, LoadStatsC, check, lib
+from ._lib import QPH_F16, QPH_Q4, Config, LoadStatsC, QphError, check, lib
+from .tokenprobs import LogProbs
 
 
 def _fptr(a):
@@ -119,6 +120,19 @@ class HipLlama:
         idx = np.empty(M, np.int32); val = np.empty(M, np.float32)
         check(lib().qph_prefill_topk(self._h, _iptr(toks), len(toks), int(M), _iptr(idx), _fptr(val)))
         return idx, val
+
+    def score(self, tokens, targets=None, top=0):
+        """feeds tokens and returns, behind each, LogProbs(logp, entropy, rank, top_index, top_logp) as numpy arrays: of targets[i] (None: the next token;
+        outside the vocabulary, as behind the last one, NaN and -1), and the `top` most probable tokens [n][top].  The logits stay on the GPU"""
+        toks = np.ascontiguousarray(tokens, dtype=np.int32)
+        n = len(toks)
+        if targets is not None:
+            targets = np.ascontiguousarray(targets, dtype=np.int32)
+            if targets.shape != toks.shape:
+                raise QphError("score: targets must be as many as tokens")
+        r = LogProbs(np.empty(n, np.float32), np.empty(n, np.float32), np.empty(n, np.int32), np.empty((n, max(int(top), 0)), np.int32), np.empty((n, max(int(top), 0)), np.float32))
+        check(lib().qph_score(self._h, _iptr(toks), targets.ctypes.data if targets is not None else None, n, int(top), *(x.ctypes.data for x in r)))
+        return r
 
     def reset(self):
         check(lib().qph_reset(self._h))
