@@ -6,9 +6,11 @@
 // every step.  x - m is one rounding off and e^(x - m) its own size times 2^-24 and two of the exponential's last places; sums are fp32, a thread's own,
 // then added as a tree.
 //
-// The alternatives: a wave keeps the K <= 64 first of what it has seen in order, one a lane, and inserts what precedes the last of them.  Its indices
-// rise, so that among equal values the list's own come first and a comparison of values decides.  Of a random row few logits pass: K ln(V / 512) a wave
-// or so; the first 64 lanes' worth is cut down first, to what reaches the K-th largest of the lanes' maxima.
+// The alternatives: a wave keeps in LDS what of its logits may be among the K <= 64 first, and a bound that K of them reach.  Indices rise, so that only a
+// logit above the bound can get past those that are there; all lanes that have one leave it by a ballot and a count of the lanes before them.  Past
+// kLpKeep entries the bound is raised, by bisection over the values' order with a ballot and a count for each entry of a lane, until it leaves K to 2 K + 16; of a
+// wave's first load before anything is kept.  Where more than that are equal, the lower indices stay.  (Kept in order in registers and inserted one by one, a chain of some
+// hundred dependent instructions each, 20 alternatives of one row took 24 us, and of 1024 rows in bf16 129.)
 //
 // A workgroup of 4 waves has a row, or a share of one where there are few; shares leave sums and lists that k_logprobs_merge joins.
 #include <hip/hip_runtime.h>
@@ -32,7 +34,11 @@ __device__ __forceinline__ int order_of(float x) {
   return b ^ (b >> 31 & 0x7fffffff);
 }
 __device__ __forceinline__ float value_of(int o) { return __builtin_bit_cast(float, o ^ (o >> 31 & 0x7fffffff)); }
-__device__ __forceinline__ bool before(int o, int i, int o2, int i2) { return o > o2 || (o == o2 && i < i2); }
+// a logit's place among the others as one number: what is ahead is larger
+__device__ __forceinline__ int64_t key_of(int o, int i) { return (int64_t)o << 32 | (uint32_t)~i; }
+__device__ __forceinline__ int order_in(int64_t k) { return (int)(k >> 32); }
+__device__ __forceinline__ int index_in(int64_t k) { return ~(int)k; }
+constexpr int64_t kNoKey = INT64_MIN;   // kNone's
 
 template <int T>
 constexpr int lp_elems() { return T == RT_F32 ? 4 : 8; }   // of 16 bytes
@@ -49,6 +55,16 @@ template <int T>
 __device__ __forceinline__ float lp_load(const void *p, int64_t i) {
   if constexpr (T == RT_F32) return ((const float *)p)[i];
   else { const uint16_t h = ((const uint16_t *)p)[i]; return T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h); }
+}
+// an element by a scalar load (16 bits: of the 4 bytes that it lies in)
+typedef const int __attribute__((address_space(4))) scalar_int;
+template <int T>
+__device__ __forceinline__ float lp_scalar(const void *p, int64_t i) {
+  const uintptr_t at = (uintptr_t)p + i * (T == RT_F32 ? 4 : 2);
+  const uint32_t w = *(const scalar_int *)(at & ~(uintptr_t)3);
+  if constexpr (T == RT_F32) return __builtin_bit_cast(float, w);
+  const uint16_t h = (uint16_t)(w >> (at & 2 ? 16 : 0));
+  return T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h);
 }
 // what a share of a row comes to
 struct LpSum { float m, s, t; int ahead; };
@@ -67,8 +83,9 @@ __device__ __forceinline__ void join(LpSum &a, const LpSum &b) {
   a.ahead += b.ahead;
 }
 // a list's entry into the outputs
-__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t row, int k, int o, int i, float m, float ls) {
-  a.top_index[row * a.top + k] = o == kNone ? -1 : i;
+__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t row, int k, int64_t key, float m, float ls) {
+  const int o = order_in(key);
+  a.top_index[row * a.top + k] = o == kNone ? -1 : index_in(key);
   a.top_logp[row * a.top + k] = o == kNone ? __builtin_nanf("") : value_of(o) - ref(m) - ls;
 }
 __device__ __forceinline__ void put(const LogprobArgs &a, int64_t row, const LpSum &s, float ls, float xt, bool has) {
@@ -77,54 +94,149 @@ __device__ __forceinline__ void put(const LogprobArgs &a, int64_t row, const LpS
   if (a.entropy) a.entropy[row] = ls - s.t / s.s;
 }
 
-// a wave's list: lane i < K has the i-th
-struct LpList { int o = kNone, i = 0; };
-__device__ __forceinline__ void insert(LpList &l, int lane, int o, int i) {
-  const int p = __popcll(__ballot(l.o >= o));   // (kNone below all)
-  const int so = __builtin_amdgcn_update_dpp(0, l.o, 0x138, 0xf, 0xf, false), si = __builtin_amdgcn_update_dpp(0, l.i, 0x138, 0xf, 0xf, false);   // wave_shr:1
-  l.o = lane < p ? l.o : lane == p ? o : so;
-  l.i = lane < p ? l.i : lane == p ? i : si;
+constexpr int kLpKeep = 128;   // entries that a wave goes on with, at most
+__device__ __forceinline__ void wave_sync() {   // what lanes left in LDS is there for the others of the wave
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ int lanes_before(uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)); }
+// The lanes' M values each.  lo is raised towards hi as long as more than `most` of them, n, reach it and K do; K reach it at the start
+template <int M>
+__device__ __forceinline__ int raised(const int (&o)[M], int lo, int hi, int K, int most, int &n) {
+  lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi);   // (the wave's: scalar arithmetic)
+  int mid = hi;   // (what a single alternative needs)
+  while (n > most && lo < hi) {
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < M; k++) c += __popcll(__ballot(o[k] >= mid));
+    if (c >= K) { lo = mid; n = c; }
+    else hi = mid - 1;
+    mid = lo + (int)(((uint32_t)hi - (uint32_t)lo + 1) >> 1);   // above lo, up to hi
+  }
+  return lo;
+}
+// the key that K to `most` (at least K) of the entries reach, kNoKey: none; their orders lie between lo, which K reach, and hi
+template <int M>
+__device__ __forceinline__ int64_t bound_of(const int64_t (&x)[M], int lo, int hi, int K, int most) {
+  int n = 0, o[M];
+#pragma unroll
+  for (int k = 0; k < M; k++) { o[k] = order_in(x[k]); n += __popcll(__ballot(o[k] >= lo)); }
+  lo = raised<M>(o, lo, hi, K, most, n);
+  int low = 0;   // (of the key: every index)
+  if (n > most) {   // too many are equal: their indices, without the sign that the order has
+    int above = 0, t[M];
+#pragma unroll
+    for (int k = 0; k < M; k++) { above += __popcll(__ballot(o[k] > lo)); t[k] = o[k] == lo ? (int)x[k] : kNone; }
+    n -= above;
+    low = raised<M>(t, kNone + 1, -1, K - above, K - above, n);
+  }
+  return (int64_t)lo << 32 | (uint32_t)low;
+}
+// a wave's n <= 64 M entries cut down to K .. most; the order of the last, which was `lo`
+template <int M>
+__device__ __forceinline__ int cut(int64_t *buf, int &n, int lo, int K, int most, int lane) {
+  int64_t x[M];
+  int hi = kNone;
+#pragma unroll
+  for (int k = 0; k < M; k++) {
+    x[k] = 64 * k + lane < n ? buf[64 * k + lane] : kNoKey;
+    hi = max(hi, order_in(x[k]));
+  }
+  hi = order_of(wave_max(value_of(hi)));   // (NaN, which lanes without an entry have here, is no maximum)
+  const int64_t b = bound_of<M>(x, max(lo, kNone + 1), hi, K, most);
+  int left = 0;
+#pragma unroll
+  for (int k = 0; k < M; k++) {
+    const bool here = x[k] >= b;   // (above kNoKey)
+    const uint64_t m = __ballot(here);
+    if (here) buf[left + lanes_before(m)] = x[k];
+    left += __popcll(m);
+  }
+  n = left;
+  wave_sync();
+  return order_in(b);
+}
+// the number of n entries ahead of x
+__device__ __forceinline__ int ahead_of(int64_t x, const int64_t *all, int n) {
+  int k = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; j++) k += all[j] > x;
+  return k;
+}
+// the wave's lanes that have an x to add leave it among the workgroup's
+__device__ __forceinline__ void add_to(int64_t *all, int *count, bool has, int64_t x, int lane) {
+  const uint64_t m = __ballot(has);
+  int at = 0;
+  if (lane == 0 && m) at = atomicAdd(count, __popcll(m));
+  at = __builtin_amdgcn_readfirstlane(at);
+  if (has) all[at + lanes_before(m)] = x;
 }
 
-template <int T, bool TOP>
+// TINY: vocabularies of less than a lane's load
+template <int T, bool TOP, bool TINY = false>
 __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
-  constexpr int VE = lp_elems<T>(), GE = 64 * VE, U = 4;   // elements of a lane's load, of a wave's; loads on their way
+  constexpr int VE = lp_elems<T>(), GE = 64 * VE, U = 2;   // elements of a lane's load, of a wave's; loads on their way (3 and 4: no faster, and longer code)
   __shared__ LpSum sums[kLpWaves];
-  __shared__ int lo[kLpWaves * kLpTop], li[kLpWaves * kLpTop];
+  constexpr int CAP = kLpKeep + GE;
+  __shared__ int64_t entries[TOP ? kLpWaves : 1][TOP ? CAP : 1], joint[TOP ? kLpWaves * kLpKeep : 1];
+  __shared__ int count, bounds[kLpWaves];
   const int64_t row = blockIdx.x / (uint32_t)a.splits;
   const int split = blockIdx.x - (int)row * a.splits;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int from = split * a.share, to = min(a.vocab, from + a.share);
   const int esize = T == RT_F32 ? 4 : 2;
   const uint8_t *x0 = (const uint8_t *)a.x + row * a.ld * esize;
-  const int token = a.tokens ? a.tokens[row] : -1;
-  const bool has = token >= 0 && token < a.vocab;
-  const float xt = has ? lp_load<T>(x0, token) : INFINITY;
   LpSum s{-INFINITY, 0.f, 0.f, 0};
-  LpList list;
-  float last = 0.f;   // value of the list's K-th
+  int64_t *buf = entries[TOP ? wave : 0];
+  int held = 0, bound = kNone;   // entries, what the K-th of them reaches
+  float last = 0.f;              // that, as a value
   bool first = true;
-  auto load = [&](int at) -> u32x4 {   // a lane's elements from at on
-    if (at + VE <= to) return *(const u32x4_any *)(x0 + (int64_t)at * esize);
-    u32x4 w;
+  // what a cut leaves, and from how many entries on there is one: a bound near the K-th lets few logits pass, a cut costs as much as some of them
+  const int most = a.top + a.top / 4 + 2, full = min(most + 32, kLpKeep);
+  if (threadIdx.x == 0) count = 0;
+  // A lane's elements from `at` on: where the share ends before, the last ones of it, of which those before `at` don't count.  Every load is made, so that the
+  // compiler can count those on their way
+  auto start = [&](int at) { return TINY ? at : min(at, to - VE); };
+  auto load = [&](int at) -> u32x4 {
+    if constexpr (!TINY) return __builtin_nontemporal_load((const u32x4_any *)(x0 + (int64_t)start(at) * esize));   // (read once: 1023 x 128256 fp32 95 -> 85 us)
+    u32x4 w = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if constexpr (T == RT_F32) w[i] = at + i < to ? ((const uint32_t *)x0)[at + i] : 0xff800000u;
-      else {
-        const uint32_t none = T == RT_F16 ? 0xfc00u : 0xff80u;
-        const uint32_t u0 = at + 2 * i < to ? ((const uint16_t *)x0)[at + 2 * i] : none, u1 = at + 2 * i + 1 < to ? ((const uint16_t *)x0)[at + 2 * i + 1] : none;
-        w[i] = u0 | u1 << 16;
-      }
+    for (int i = 0; i < VE; i++) {
+      if (at + i >= to) continue;
+      if constexpr (T == RT_F32) w[i] = ((const uint32_t *)x0)[at + i];
+      else w[i / 2] |= (uint32_t)((const uint16_t *)x0)[at + i] << 16 * (i & 1);
     }
     return w;
   };
-  auto take = [&](u32x4 w, int base) {   // a wave's elements base .., those past `to` -inf
-    const int at = base + VE * lane;
+  u32x4 w[U];
+  constexpr int STEP = GE * kLpWaves;
+  const int steps = (to - from + STEP - 1) / STEP, base = from + GE * wave;
+#pragma unroll
+  for (int u = 0; u < U; u++) w[u] = load(base + u * STEP + VE * lane);
+  // the token and its logit through the scalar cache: in the vector loads' order they would be waited for one after the other
+  const int token = a.tokens ? __builtin_amdgcn_readfirstlane(*(const scalar_int *)(uintptr_t)(a.tokens + row)) : -1;
+  const bool has = token >= 0 && token < a.vocab;
+  const float xt = has ? lp_scalar<T>(x0, token) : INFINITY;
+  auto take = [&](u32x4 w, int base) {   // a wave's elements base ..
+    const int from0 = base + VE * lane, at = start(from0);
     float x[VE], bm = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < VE; i++) { x[i] = lp_elem<T>(w, i); bm = fmaxf(bm, x[i]); }
+    for (int i = 0; i < VE; i++) x[i] = lp_elem<T>(w, i);
+    uint32_t counts = ~0u;
+    if (base + GE > to) {
+      counts = 0;
+#pragma unroll
+      for (int i = 0; i < VE; i++) {
+        const bool c = (at + i >= from0) & (at + i < to);
+        counts |= (uint32_t)c << i;
+        x[i] = c ? x[i] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VE; i++) bm = fmaxf(bm, x[i]);
     if (__any(bm > s.m + kLpRoom)) {   // (always while there is none)
-      const float m = wave_max(bm);
+      const float m = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, wave_max(bm))));
       if (m > s.m) {
         const float d = s.m == -INFINITY ? 0.f : near(s.m - m), c = __builtin_amdgcn_exp2f(d * kLog2e);
         s.t = (s.t + s.s * d) * c;
@@ -141,78 +253,65 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
     }
     if (base + GE <= token) {
 #pragma unroll
-      for (int i = 0; i < VE; i++) s.ahead += x[i] >= xt;
+      for (int i = 0; i < VE; i++) s.ahead += __popcll(__ballot(x[i] >= xt));
     } else if (base > token) {
 #pragma unroll
-      for (int i = 0; i < VE; i++) s.ahead += x[i] > xt;
+      for (int i = 0; i < VE; i++) s.ahead += __popcll(__ballot(x[i] > xt));
     } else {
 #pragma unroll
-      for (int i = 0; i < VE; i++) s.ahead += (x[i] > xt) | ((x[i] == xt) & (at + i < token));
+      for (int i = 0; i < VE; i++) s.ahead += __popcll(__ballot((x[i] > xt) | ((x[i] == xt) & (at + i < token) & (int)(counts >> i & 1))));
     }
     if constexpr (TOP) {
       if (first) {
-        // the K-th largest of the lanes' first ones bounds the K-th largest of all from below
         first = false;
-        int o[VE], mo = kNone;
+        int64_t k[VE], b = kNoKey + 1;
 #pragma unroll
-        for (int i = 0; i < VE; i++) { o[i] = at + i < to ? order_of(x[i]) : kNone; mo = max(mo, o[i]); }
-        int n = 0;
-#pragma unroll 8
-        for (int l = 0; l < 64; l++) {
-          const int other = __builtin_amdgcn_readlane(mo, l);
-          n += other > mo || (other == mo && l < lane);
+        for (int i = 0; i < VE; i++) k[i] = counts >> i & 1 ? key_of(order_of(x[i]), at + i) : kNoKey;
+        if (to - base > full) {   // the least of the lanes' maxima is reached by one of each lane
+          b = bound_of<VE>(k, order_of(-wave_max(-bm)), order_of(wave_max(bm)), a.top, most);
+          bound = order_in(b);
         }
-        const int bound = __builtin_amdgcn_readlane(mo, __builtin_ctzll(__ballot(n == a.top - 1)));
-        uint64_t lanes = __ballot(mo >= bound && mo != kNone);
-        while (lanes) {
-          const int l = __builtin_ctzll(lanes);
-          lanes &= lanes - 1;
 #pragma unroll
-          for (int i = 0; i < VE; i++) {
-            const int v = __builtin_amdgcn_readlane(o[i], l);
-            if (v >= bound && v != kNone) insert(list, lane, v, base + VE * l + i);
-          }
+        for (int i = 0; i < VE; i++) {
+          const bool here = k[i] >= b;
+          const uint64_t m = __ballot(here);
+          if (here) buf[held + lanes_before(m)] = k[i];
+          held += __popcll(m);
         }
+        last = value_of(bound);
       } else {
-        uint64_t lanes = __ballot(bm > last);
-        if (!lanes) return;
-        while (lanes) {
-          const int l = __builtin_ctzll(lanes);
-          lanes &= lanes - 1;
-          int lo = __builtin_amdgcn_readlane(list.o, a.top - 1);
+        if (!__any(bm > last)) return;
 #pragma unroll
-          for (int i = 0; i < VE; i++) {
-            const int v = order_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[i]), l)));
-            if (v > lo) { insert(list, lane, v, base + VE * l + i); lo = __builtin_amdgcn_readlane(list.o, a.top - 1); }
+        for (int i = 0; i < VE; i++) {
+          const uint64_t m = __ballot(x[i] > last);
+          if (m) {
+            if (x[i] > last) buf[held + lanes_before(m)] = key_of(order_of(x[i]), at + i);
+            held += __popcll(m);
           }
+        }
+        wave_sync();
+        if (held > full) {
+          bound = held > kLpKeep ? cut<CAP / 64>(buf, held, bound, a.top, most, lane) : cut<kLpKeep / 64>(buf, held, bound, a.top, most, lane);
+          last = value_of(bound);
         }
       }
-      last = value_of(__builtin_amdgcn_readlane(list.o, a.top - 1));
     }
   };
-  u32x4 w[U];
-  int base = from + GE * wave;
-  constexpr int STEP = GE * kLpWaves;
-#pragma unroll
-  for (int u = 0; u < U; u++) if (base + u * STEP < to) w[u] = load(base + u * STEP + VE * lane);
-  while (base < to) {
+  for (int k = 0; k < steps; k += U) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if (base < to) {
-        const u32x4 now = w[u];
-        if (base + U * STEP < to) w[u] = load(base + U * STEP + VE * lane);
-        take(now, base);
-      }
-      base += STEP;
+      const u32x4 now = w[u];
+      w[u] = load(base + (k + u + U) * STEP + VE * lane);
+      if (k + u < steps) take(now, base + (k + u) * STEP);
     }
   }
   // lanes share the reference; then the waves
   s.s = wave_sum(s.s); s.t = wave_sum(s.t);
-  s.ahead = sum32_i(s.ahead);
-  s.ahead += __shfl_xor(s.ahead, 32);
   if (lane == 0) sums[wave] = s;
   if constexpr (TOP) {
-    if (lane < a.top) { lo[wave * a.top + lane] = list.o; li[wave * a.top + lane] = list.i; }
+    wave_sync();
+    if (held > most) bound = cut<kLpKeep / 64>(buf, held, bound, a.top, most, lane);
+    if (lane == 0) bounds[wave] = bound;
   }
   __syncthreads();
   LpSum all = sums[0];
@@ -225,19 +324,33 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
     else ((LpSum *)a.work)[part] = all;
   }
   if constexpr (TOP) {
-    // an entry's place among all is the number before it (those of kNone are alike, in the lists' order)
-    const int e = threadIdx.x;
-    if (e < kLpWaves * a.top) {
-      const int o = lo[e], i = o == kNone ? INT_MAX : li[e];
-      int n = 0;
-      for (int j = 0; j < kLpWaves * a.top; j++) {
-        const int oj = lo[j], ij = oj == kNone ? INT_MAX : li[j];
-        n += before(oj, ij, o, i) || (oj == kNone && o == kNone && j < e);
+    // what reaches every wave's bound is put together; an entry's place is the number of those before it
+    int most = bounds[0];
+#pragma unroll
+    for (int i = 1; i < kLpWaves; i++) most = max(most, bounds[i]);
+    for (int e = lane; e - lane < held; e += 64) {
+      const int64_t x = e < held ? buf[e] : kNoKey;
+      add_to(joint, &count, e < held && order_in(x) >= most, x, lane);
+    }
+    __syncthreads();
+    if (count > 2 * kLpTop) {   // (where four lists of many are left)
+      if (wave == 0) {
+        int n = count;
+        cut<kLpWaves * kLpKeep / 64>(joint, n, most, a.top, kLpTop + 16, lane);
+        if (lane == 0) count = n;
       }
-      if (n < a.top) {
-        if (a.splits == 1) put_top(a, row, n, o, i, all.m, ls);
-        else ((int2 *)((LpSum *)a.work + a.rows * a.splits))[part * a.top + n] = make_int2(o, i);
-      }
+      __syncthreads();
+    }
+    const int n = count;
+    auto put_at = [&](int k, int64_t x) {
+      if (a.splits == 1) put_top(a, row, k, x, all.m, ls);
+      else ((int64_t *)((LpSum *)a.work + a.rows * a.splits))[part * a.top + k] = x;
+    };
+    for (int e = threadIdx.x; e < max(n, a.top); e += kLpWaves * 64) {
+      if (e >= n) { put_at(e, kNoKey); continue; }   // fewer than K (a share of a few logits)
+      const int64_t x = joint[e];
+      const int k = ahead_of(x, joint, n);
+      if (k < a.top) put_at(k, x);
     }
   }
 }
@@ -247,14 +360,16 @@ template <int T>
 __global__ __launch_bounds__(256) void k_logprobs_merge(LogprobArgs a) {
   constexpr int kMost = kLpSplits * kLpTop;
   __shared__ LpSum all;
-  __shared__ int heads[kLpSplits], bound, count;
-  __shared__ int co[kMost], ci[kMost];
+  __shared__ int64_t firsts[kLpSplits + kLpTop], bound, joint[kMost];
+  __shared__ int count;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, S = a.splits;
+  const int tid = threadIdx.x, S = a.splits, K = a.top;
   const LpSum *sums = (const LpSum *)a.work + row * S;
-  const int2 *lists = (const int2 *)((const LpSum *)a.work + a.rows * S) + row * S * a.top;
-  if (tid < S && a.top) heads[tid] = lists[tid * a.top].x;
-  if (tid == 0) { count = 0; bound = kNone; }
+  const int64_t *lists = (const int64_t *)((const LpSum *)a.work + a.rows * S) + row * S * K;
+  // the first d of each list are K at least; what the K-th of them precedes is not among the first K
+  const int d = K ? (K + S - 1) / S : 0, F = S * d;
+  if (tid < F) firsts[tid] = lists[tid / d * K + tid % d];
+  if (tid == 0) { count = 0; bound = kNoKey + 1; }
   if (tid < 64) {
     LpSum s = tid < S ? sums[tid] : LpSum{-INFINITY, 0.f, 0.f, 0};
 #pragma unroll
@@ -268,24 +383,23 @@ __global__ __launch_bounds__(256) void k_logprobs_merge(LogprobArgs a) {
     const bool has = token >= 0 && token < a.vocab;
     put(a, row, all, ls, has ? lp_load<T>((const uint8_t *)a.x + row * a.ld * (T == RT_F32 ? 4 : 2), token) : 0.f, has);
   }
-  if (!a.top) return;
-  // what lies behind the K-th of the lists' first entries is not among the first K
-  if (tid < S && S >= a.top) {
-    int n = 0;
-    for (int j = 0; j < S; j++) n += heads[j] > heads[tid] || (heads[j] == heads[tid] && j < tid);
-    if (n == a.top - 1) bound = heads[tid];
+  if (!K) return;
+  if (tid < F && order_in(firsts[tid]) != kNone) {
+    const int64_t x = firsts[tid];
+    if (ahead_of(x, firsts, F) == K - 1) bound = x;
   }
   __syncthreads();
-  for (int e = tid; e < S * a.top; e += 256) {
-    const int2 x = lists[e];
-    if (x.x >= bound && x.x != kNone) { const int c = atomicAdd(&count, 1); co[c] = x.x; ci[c] = x.y; }
+  for (int e = tid; e - tid < S * K; e += 256) {
+    const int64_t x = e < S * K ? lists[e] : kNoKey;
+    add_to(joint, &count, order_in(x) != kNone && x >= bound, x, tid & 63);
   }
   __syncthreads();
-  for (int e = tid; e < max(count, a.top); e += 256) {
-    if (e >= count) { put_top(a, row, e, kNone, 0, all.m, ls); continue; }   // fewer than K (a vocabulary of NaN)
-    int n = 0;
-    for (int j = 0; j < count; j++) n += before(co[j], ci[j], co[e], ci[e]);
-    if (n < a.top) put_top(a, row, n, co[e], ci[e], all.m, ls);
+  const int n = count;
+  for (int e = tid; e < max(n, K); e += 256) {
+    if (e >= n) { put_top(a, row, e, kNoKey, all.m, ls); continue; }   // fewer than K (a vocabulary of NaN)
+    const int64_t x = joint[e];
+    const int k = ahead_of(x, joint, n);
+    if (k < K) put_top(a, row, k, x, all.m, ls);
   }
 }
 }  // namespace
@@ -305,7 +419,8 @@ hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t st) {
   const dim3 grid((unsigned)(a.rows * a.splits)), thr(kLpWaves * 64);
 #define QPH_LP(T)                                                                          \
   do {                                                                                     \
-    if (a.top) hipLaunchKernelGGL((k_logprobs<T, true>), grid, thr, 0, st, a);             \
+    if (a.vocab < lp_elems<T>()) hipLaunchKernelGGL((k_logprobs<T, true, true>), grid, thr, 0, st, a); \
+    else if (a.top) hipLaunchKernelGGL((k_logprobs<T, true>), grid, thr, 0, st, a);             \
     else hipLaunchKernelGGL((k_logprobs<T, false>), grid, thr, 0, st, a);                  \
     const hipError_t e = hipGetLastError();                                                \
     if (e != hipSuccess || a.splits == 1) return e;                                        \
