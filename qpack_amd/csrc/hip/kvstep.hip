@@ -175,44 +175,89 @@ __global__ __launch_bounds__(256) void k_copy16(KvCopyArgs a) {
   uint16_t *dst = STAGE == 1 ? (uint16_t *)a.work + staged : (uint16_t *)(blockIdx.y ? a.cache_v : a.cache) + b * a.cseq + ((int64_t)a.pos[b] + t) * a.crow + d;
   *(u32x4 *)dst = *(const u32x4 *)src;
 }
-// A workgroup has a record of one kv head: 8 positions whose codes come from up to 8 records.  A thread has a word of K, which stays whole, and one
-// of V, whose 8 codes are one dim's of 8 positions and come from a word each; V words that hold positions outside the call are merged
+// A workgroup has 32 records of one kv head, 256 positions, one a thread to look up.  Records that come from one whole record, as all but the last of a fork do, are
+// copied as they are, 16 bytes a thread.  Of others a wave has one: lanes 0 .. have 16 bytes of a position's K, lanes 32 .. four words of V, whose
+// 8 codes come from a word each of up to 8 records; V words that hold positions outside the call are merged.
+// 6001 positions of 8 heads of 128 dims forked into 8 sequences: 62 MB
+constexpr int kCopyRecs = 32;
 template <int HD, int STAGE>
-__global__ __launch_bounds__(HD) void k_copy4(KvCopyArgs a) {
-  const int b = blockIdx.z, g = blockIdx.y, tid = threadIdx.x;
+__global__ __launch_bounds__(256) void k_copy4(KvCopyArgs a) {
+  constexpr int P = 9 * HD / 16, NP = (kCopyRecs * P + 255) / 256;   // 16-byte pieces of a record, of a thread
+  __shared__ int place[kCopyRecs * kRec], whole[kCopyRecs];   // where positions come from; whole records' first, -1: of several, -2: none
+  const int b = blockIdx.z, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int P0 = a.pos[b];
   if (P0 < 0) return;
-  const int64_t rec = (STAGE == 1 ? 0 : P0 / kRec) + (int64_t)blockIdx.x;   // in scratch tokens lie from position 0 on
+  const int64_t rec = (STAGE == 1 ? 0 : P0 / kRec) + (int64_t)blockIdx.x * kCopyRecs;   // in scratch tokens lie from position 0 on
   const int64_t t0 = rec * kRec - (STAGE == 1 ? 0 : P0), wrec = (a.n + kRec - 1) / kRec;
-  uint8_t *o = STAGE == 1 ? (uint8_t *)a.work + (((int64_t)b * a.nkv + g) * wrec + rec) * (9 * HD) : (uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD);
-  const uint8_t *from[kRec];   // of each position of the record: the source's record, and the place there
-  int at[kRec];
-  uint32_t keep = 0;
-#pragma unroll
-  for (int j = 0; j < kRec; j++) {
-    const int64_t t = t0 + j;
+  const int64_t head = (int64_t)b * a.nkv + g;
+  uint8_t *dst = STAGE == 1 ? (uint8_t *)a.work + (head * wrec + rec) * (9 * HD) : (uint8_t *)a.cache + (head * a.nrec + rec) * (9 * HD);
+  const uint8_t *src;
+  {
+    const int64_t t = t0 + tid;
     const Place s = t >= 0 && t < a.n ? place_of(a, b, (int)t) : Place{0, -1};
-    const int p = STAGE == 2 ? (int)t : s.p;
-    at[j] = s.p < 0 ? -1 : p % kRec;
-    from[j] = STAGE == 2 ? (const uint8_t *)a.work + (((int64_t)b * a.nkv + g) * wrec + p / kRec) * (9 * HD)
-                         : (const uint8_t *)a.src + (((int64_t)s.seq * a.nkv + g) * a.src_nrec + p / kRec) * (9 * HD);
-    if (s.p < 0) keep |= 15u << nib(j);
+    const int p = s.p < 0 ? -1 : STAGE == 2 ? (int)t : s.p, p0 = __shfl(p, lane & ~7);
+    place[tid] = p;
+    const uint32_t there = (uint32_t)(__ballot(p >= 0) >> (lane & ~7)) & 255, run = (uint32_t)(__ballot(p >= 0 && p == p0 + (lane & 7) && p0 % kRec == 0) >> (lane & ~7)) & 255;
+    if ((lane & 7) == 0) whole[tid / kRec] = run == 255 ? p0 : there ? -1 : -2;
+    const int seq = a.seqs ? a.seqs[b] : b;   // (outside the source: no position is there)
+    src = STAGE == 2 ? (const uint8_t *)a.work + head * wrec * (9 * HD) : (const uint8_t *)a.src + ((int64_t)seq * a.nkv + g) * a.src_nrec * (9 * HD);
   }
-  if (keep == ~0u) return;
-  const int row = tid / (HD / 8);
-  uint32_t v = 0;
+  __syncthreads();
+  u32x4 piece[NP];
 #pragma unroll
-  for (int j = 0; j < kRec; j++) {
-    if (at[j] < 0) continue;
-    v |= (((const uint32_t *)(from[j] + 4 * HD))[tid] >> (16 * (at[j] & 1) + 4 * (at[j] >> 1)) & 15) << nib(j);
-    if (j == row) ((uint32_t *)o)[tid] = ((const uint32_t *)from[j])[at[j] * (HD / 8) + tid % (HD / 8)];
-    // scales: K's of the position follow each other, V's lie 8 positions apart
-    if (tid < HD / 32) ((uint16_t *)(o + 8 * HD))[j * (HD / 32) + tid] = ((const uint16_t *)(from[j] + 8 * HD))[at[j] * (HD / 32) + tid];
-    else if (tid < HD / 16) ((uint16_t *)(o + 8 * HD + HD / 2))[(tid - HD / 32) * kRec + j] = ((const uint16_t *)(from[j] + 8 * HD + HD / 2))[(tid - HD / 32) * kRec + at[j]];
+  for (int i = 0; i < NP; i++) {
+    const int id = tid + 256 * i, r = id / P;
+    const int from = r < kCopyRecs ? whole[r] : -1;
+    if (from >= 0) piece[i] = *(const u32x4 *)(src + (int64_t)(from / kRec) * (9 * HD) + id % P * 16);
   }
-  uint32_t *vd = (uint32_t *)(o + 4 * HD) + tid;
-  if (keep) v |= *vd & keep;
-  *vd = v;
+#pragma unroll
+  for (int i = 0; i < NP; i++) {
+    const int id = tid + 256 * i, r = id / P;
+    if (r < kCopyRecs && whole[r] >= 0) *(u32x4 *)(dst + id * 16) = piece[i];
+  }
+  for (int r = tid / 64; r < kCopyRecs; r += 4) {
+    if (whole[r] != -1) continue;
+    const int *at = place + kRec * r;
+    uint8_t *o = dst + r * (9 * HD);
+    const bool v = lane >= 32;
+    const int l = lane & 31, j = l / (HD / 32);   // (K: the position; the piece of its row is l % (HD / 32))
+    u32x4 w = {0, 0, 0, 0};
+    uint32_t keep = 0;
+    uint16_t sc[2] = {0, 0};
+    auto record = [&](int p) { return src + (int64_t)(p / kRec) * (9 * HD); };
+    if (l < HD / 4) {
+      if (v) {
+        u32x4 x[kRec], old = *(const u32x4 *)(o + 4 * HD + 16 * l);
+#pragma unroll
+        for (int k = 0; k < kRec; k++) x[k] = at[k] >= 0 ? *(const u32x4 *)(record(at[k]) + 4 * HD + 16 * l) : (u32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < kRec; k++) {
+          const int q = at[k] & 7;
+          if (at[k] < 0) keep |= 15u << nib(k);
+          w |= (x[k] >> (uint32_t)(16 * (q & 1) + 4 * (q >> 1)) & 15u) << (uint32_t)nib(k);
+        }
+        w = (w & ~keep) | (old & keep);
+      } else if (at[j] >= 0) {
+        w = *(const u32x4 *)(record(at[j]) + at[j] % kRec * (HD / 2) + l % (HD / 32) * 16);
+      }
+    }
+    // the scales: of position lane % 8 and group lane / 8 of K, then of V
+    const int k = lane & 7, q = lane >> 3;
+    const bool scale = q < HD / 32 && at[k] >= 0;
+    if (scale) {
+      const uint8_t *x = record(at[k]) + 8 * HD;
+      sc[0] = *(const uint16_t *)(x + 2 * (at[k] % kRec * (HD / 32) + q));
+      sc[1] = *(const uint16_t *)(x + HD / 2 + 2 * (q * kRec + at[k] % kRec));
+    }
+    if (l < HD / 4) {
+      if (v) *(u32x4 *)(o + 4 * HD + 16 * l) = w;
+      else if (at[j] >= 0) *(u32x4 *)(o + 16 * l) = w;
+    }
+    if (scale) {
+      *(uint16_t *)(o + 8 * HD + 2 * (k * (HD / 32) + q)) = sc[0];
+      *(uint16_t *)(o + 8 * HD + HD / 2 + 2 * (q * kRec + k)) = sc[1];
+    }
+  }
 }
 }  // namespace
 
@@ -246,9 +291,9 @@ size_t kv_copy_bytes(int kind, int nseq, int nkv, int hd, int n) {
 template <int STAGE>
 static void launch_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
   if (kind == MK_Q4) {
-    const dim3 grid((unsigned)((a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1)), a.nkv, a.nseq);
-    if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE>), grid, dim3(128), 0, st, a);
-    else hipLaunchKernelGGL((k_copy4<64, STAGE>), grid, dim3(64), 0, st, a);
+    const dim3 grid((unsigned)(((a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1) + kCopyRecs - 1) / kCopyRecs), a.nkv, a.nseq);
+    if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_copy4<64, STAGE>), grid, dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL((k_copy16<STAGE>), dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
   }
