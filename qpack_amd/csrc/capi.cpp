@@ -111,7 +111,7 @@ static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sink
   a.window = window; a.sinks = sinks; a.few = qph::kv_few();
 }
 // attention over a common prefix and the sequences' own caches: both passes' arguments without their rows
-static void kv_prefix_args(const qph_kv *c, const qph_kv *prefix, const int *prefix_len, int heads, int n, qph::KvAttnArgs &a, qph::KvAttnArgs &p) {
+static void kv_prefix_args(const qph_kv *c, const qph_kv *prefix, const int *prefix_len, int heads, int n, qph::KvAttnArgs &a, qph::KvPreArgs &p) {
   kv_attn_args(c, heads, n, 0, 0, a);
   int64_t seq, row;
   kv_cache(prefix, &seq, &row);
@@ -626,7 +626,7 @@ int qph_kv_attention_prefix_work(const qph_kv *c, const qph_kv *prefix, int type
   QPH_API_TRY({
     need(bytes, "bytes");
     qph::KvAttnArgs a{};
-    qph::KvAttnArgs p{};
+    qph::KvPreArgs p{};
     a.q.type = p.q.type = kv_row_type(type);
     kv_prefix_args(c, prefix, nullptr, heads, n, a, p);
     *bytes = n ? (int64_t)qph::kv_prefix_plan(a, p) : 0;
@@ -636,7 +636,7 @@ int qph_kv_attention_prefix(const qph_kv *c, const qph_kv *prefix, const int *pr
                             const int *lens, float scale, void *work, int64_t work_bytes, void *stream) {
   QPH_API_TRY({
     qph::KvAttnArgs a{};
-    qph::KvAttnArgs p{};
+    qph::KvPreArgs p{};
     kv_prefix_args(c, prefix, prefix_len, heads, n, a, p);
     kv_attn_rows(c, q, out, heads, n, pos, lens, scale, a);
     if (n) {

@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 #include "kvrec.hpp"
 #include "launch.hpp"
@@ -48,9 +49,8 @@ __global__ __launch_bounds__(128) void k_kv4_write(KvIoArgs a) {
   const int64_t p = rec * kRec + row;
   const bool mine = p >= P0 && p < last;
   const KvRows &r = vside ? a.v : a.k;
-  float x[EL];
-  if (mine) load_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x);
-  store_record<HD, T>((uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD), x, mine, vside, row, part, kept_bits(rec * kRec, P0, last), codes);
+  store_record<HD, T>([&](float *x) { load_elems<T, EL>(r, b * r.seq + (p - P0) * r.tok + g * r.head + EL * part, x); },
+                      [&]() { return (uint8_t *)a.cache + (((int64_t)b * a.nkv + g) * a.nrec + rec) * (9 * HD); }, mine, vside, row, part, rec * kRec, P0, last, codes);
 }
 
 // One token a sequence: a wave has one row of K or V, HD / 64 dims a lane.  Lanes of a K word meet by DPP; a V word is read (as soon as
@@ -188,7 +188,7 @@ __device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int chunk) {
 // sequences counted through, and b is 0
 __device__ __forceinline__ int prefix_length(const KvPrefix &p) { return p.len ? (int)min((int64_t)max(*p.len, 0), p.ctx) : (int)p.ctx; }
 __device__ __forceinline__ int splits_of(int nt, int one_tiles, int nsplit, int min_log2) { return nt <= one_tiles ? (int)(nt > 0) : min(nsplit, (nt + (1 << min_log2) - 1) >> min_log2); }
-__device__ __forceinline__ Span prefix_span_of(const KvAttnArgs &a) {
+__device__ __forceinline__ Span prefix_span_of(const KvPreArgs &a) {
   Span s;
   const int L = prefix_length(a.prefix);
   s.P0 = 0; s.cnt = a.n; s.any = L > 0;
@@ -205,14 +205,19 @@ __device__ __forceinline__ int prefix_splits(const KvJoin &p) {
 }
 // a token counted through all sequences, as its sequence's
 struct SeqTok { int b, t; };
-__device__ __forceinline__ SeqTok seq_tok(const KvAttnArgs &a, int tok) {
+__device__ __forceinline__ SeqTok seq_tok(const KvPreArgs &a, int tok) {
   const int b = a.prefix.n == 1 ? tok : tok / a.prefix.n;
   return {b, tok - b * a.prefix.n};
 }
-__device__ __forceinline__ bool takes_part(const KvAttnArgs &a, SeqTok x) {
+template <bool PRE> using Args = std::conditional_t<PRE, KvPreArgs, KvAttnArgs>;   // of the kernels below
+__device__ __forceinline__ bool takes_part(const KvPreArgs &a, SeqTok x) {
   const int P0 = a.pos[x.b];
   return (P0 >= 0) & (x.t < tokens_of(a.lens, x.b, a.prefix.n)) & ((int64_t)P0 + x.t < a.prefix.own_ctx);
 }
+// whether a pass leaves its sums, one split's too, to be joined with another pass's
+__host__ __device__ __forceinline__ bool joined(const KvAttnArgs &a) { return a.one_tiles < 0; }
+// the partial sums of a row: the own positions' first, a prefix's last
+__host__ __device__ __forceinline__ int slots_of(const KvAttnArgs &a) { return joined(a) ? -a.one_tiles : a.nsplit; }
 // the first tile of share i of S (the product fits: nt <= 2^25, i <= 64)
 __device__ __forceinline__ int share(const Span &s, int i) { return s.S == 1 ? i * s.nt : (int)((uint32_t)i * (uint32_t)s.nt / (uint32_t)s.S); }
 __device__ __forceinline__ int record(const Span &s, int v) { return v < s.SR ? v : v + s.skip; }
@@ -381,236 +386,46 @@ __device__ __forceinline__ void add_bad(const uint8_t *rec, const uint16_t *row,
   }
 }
 
-template <int HD, int KIND, int T, bool PRE = false>
-__global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(KvAttnArgs a) {
-  constexpr bool TWO = T == RT_F32;
-  constexpr int NW = kFewWaves, KS = HD / 32, DT = HD / 16, NC = TWO ? 8 : 16, QS = HD + 4;
-  constexpr int kTileBytes = KIND == MK_Q4 ? 0 : NW * kFewTile * HD * 2, kOutBytes = NW * NC * QS * 4;
-  __shared__ __align__(16) uint8_t sm[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
-  __shared__ float wm[NW][NC], wl[NW][NC];
-  const int b = blockIdx.z, g = a.nchunk == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nchunk, chunk = blockIdx.y - g * a.nchunk, c0 = chunk * NC, split = blockIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-  // columns past the call's last are that one again: another row may be another workgroup's, whose results may be on their way into it (out may
-  // be q).  (Zeros without a load, or the first column's row: 0.3 us of a short call)
-  const int col = min(c0 + (TWO ? lr & 7 : lr), a.n * a.rep - 1), tok = token_of(a, col), hr = col - tok * a.rep;
-  // the column's query: dims HD / 4 lg + 8 k + j (4-bit: a lane's words are consecutive) or 32 k + 8 lg + j.  Asked for before
-  // the sequence's position is known
-  h8 q[KS];
-  float x[KS][8];
-  const SeqTok st = PRE ? seq_tok(a, tok) : SeqTok{b, tok};
-  {
-    const int64_t at = st.b * a.q.seq + (int64_t)st.t * a.q.tok + (int64_t)(g * a.rep + hr) * a.q.head;
-#pragma unroll
-    for (int k = 0; k < KS; k++) {
-      const int64_t d = at + (KIND == MK_Q4 ? HD / 4 * lg + 8 * k : 32 * k + 8 * lg);
-      if constexpr (T == RT_F16) q[k] = load_halves(a.q, d);
-      else load_elems<T, 8>(a.q, d, x[k]);
-    }
+template <int HD, int KIND, int T>
+constexpr int few_lds() {   // bytes: V's tiles, then the waves' sums
+  constexpr int tiles = KIND == MK_Q4 ? 0 : kFewWaves * kFewTile * HD * 2, out = kFewWaves * (T == RT_F32 ? 8 : 16) * (HD + 4) * 4;
+  return tiles > out ? tiles : out;
+}
+template <int HD, int KIND, int T>
+__device__ __forceinline__ uint8_t (&few_sm())[few_lds<HD, KIND, T>()] {
+  __shared__ __align__(16) uint8_t sm[few_lds<HD, KIND, T>()];
+  return sm;
+}
+template <int T, int I>
+__device__ __forceinline__ float (&few_wm())[kFewWaves][T == RT_F32 ? 8 : 16] {
+  __shared__ float wm[kFewWaves][T == RT_F32 ? 8 : 16];
+  return wm;
+}
+template <int HD, int KIND, int T, bool PRE = false>   // (PRE: below)
+__global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(Args<PRE> a) {
+  __shared__ __align__(16) uint8_t sm[few_lds<HD, KIND, T>()];
+  __shared__ float wm[kFewWaves][T == RT_F32 ? 8 : 16], wl[kFewWaves][T == RT_F32 ? 8 : 16];
+  const int split = blockIdx.x, gc = blockIdx.y, b = blockIdx.z;
+#include "kv_few.inc"
+}
+template <int HD, int KIND, int T, bool PRE, typename A>
+__device__ __forceinline__ void few_tokens(A a, int split, int gc, int b) {   // (the arguments by value: by reference the kernel below spills)
+  auto &sm = few_sm<HD, KIND, T>();
+  auto &wm = few_wm<T, 0>();
+  auto &wl = few_wm<T, 1>();
+#include "kv_few.inc"
+}
+// a common prefix's workgroups and then the sequences' own, in one launch (a launch and the first kernel's last workgroups: 4 samples behind 700 positions 17.2 -> TODO us)
+template <int HD, int KIND, int T>
+__global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few_both(KvAttnArgs a, KvPreArgs p) {
+  const uint32_t pre = (uint32_t)p.nsplit * p.nkv * p.nchunk;
+  if (blockIdx.x < pre) {
+    const uint32_t gc = blockIdx.x / (uint32_t)p.nsplit;
+    few_tokens<HD, KIND, T, true, KvPreArgs>(p, blockIdx.x - gc * p.nsplit, gc, 0);
+  } else {
+    const uint32_t i = blockIdx.x - pre, r = i / (uint32_t)a.nsplit, per = (uint32_t)a.nkv * a.nchunk, b = r / per;
+    few_tokens<HD, KIND, T, false, KvAttnArgs>(a, i - r * a.nsplit, r - b * per, b);
   }
-  const Span s = PRE ? prefix_span_of(a) : span_of(a, b, chunk);
-  if (!s.any || split >= s.S) return;
-  const bool live = PRE ? takes_part(a, st) : tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
-  const int P = live ? PRE ? s.PB : s.P0 + tok : -1;
-  const int lo = behind(a, P);
-  const int t0 = share(s, split), t1 = share(s, split + 1);
-  const Head h = head_of<HD, KIND>(a, b, g);
-  uint16_t *vbuf = (uint16_t *)sm + wave * kFewTile * HD;
-  Tile<HD, KIND> cur;
-  if (t0 + wave < t1) { load_v<HD, KIND>(a, h, s, t0 + wave, lane, cur, vbuf); load_k<HD, KIND>(a, h, s, t0 + wave, lane, cur); }
-  float f = a.scale2;   // softmax scale in base 2, times the row's power
-  if constexpr (T != RT_F16) {
-    float mx = 0.f;
-#pragma unroll
-    for (int k = 0; k < KS; k++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
-    mx = pair_max32(pair_max16(mx));
-    const float p2 = row_power(mx);
-    f = fminf(fmaxf(f / p2, kTinyF), kMostF);
-#pragma unroll
-    for (int k = 0; k < KS; k++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float y = x[k][j] * p2;
-        const _Float16 hi = (_Float16)y;
-        q[k][j] = TWO && lr >= 8 ? (_Float16)(y - (float)hi) : hi;
-      }
-  }
-  f32x4 o[DT];
-#pragma unroll
-  for (int d = 0; d < DT; d++) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f, sub = kPBias;
-  // the next tile's K is asked for once this one's is used, its V likewise: either is on its way during the other's product
-  for (int tile = t0 + wave; tile < t1; tile += NW) {
-    const int v = 4 * tile + lg, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
-    // whether some column does not see all of the tile: its first and last position bound the others
-    const int pf = kRec * record(s, 4 * tile), pl = kRec * record(s, min(4 * tile + 3, s.NR - 1)) + kRec - 1;
-    const bool edge = 4 * tile + 4 > s.NR || pl > s.PA || (a.window > 0 && pf <= s.PB - a.window && pl >= a.sinks);
-    f32x4 sc[2];
-#pragma unroll
-    for (int mt = 0; mt < 2; mt++) {
-      sc[mt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KS; k++) {
-        h8 kf;
-        if constexpr (KIND == MK_Q4) kf = values(cur.k[mt][k], cur.ks[mt]);
-        else kf = __builtin_bit_cast(h8, cur.k[mt][k]);
-        sc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[k], sc[mt], 0, 0, 0);
-      }
-    }
-    if constexpr (KIND == MK_Q4) { if (tile + NW < t1) load_k<HD, KIND>(a, h, s, tile + NW, lane, cur); }
-    float y[8];
-    uint32_t on = 255;   // positions that a column of the workgroup sees
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      y[j] = sc[j >> 2][j & 3];
-      if (TWO) y[j] += xchg8_f(y[j]);
-    }
-    if (edge) {
-      on = seen_bits(a, s, v, p0);
-#pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = sees(a, Pin, lo, p0 + j) ? y[j] : -INFINITY;
-    }
-    h8 ph;
-    auto weights = [&]() {   // y -> ph and their sum over the lane's positions
-      float rs = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], f, sub)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j + 1], f, sub));
-        h2 hi = {(_Float16)w0, (_Float16)w1};
-        if constexpr (TWO) {
-          rs += w0; rs += w1;
-          if (lr >= 8) hi = (h2){(_Float16)(w0 - (float)hi[0]), (_Float16)(w1 - (float)hi[1])};
-        } else {
-          rs = __builtin_amdgcn_fdot2(hi, (h2){(_Float16)1.f, (_Float16)1.f}, rs, false);   // the sum of what the product takes
-        }
-        ph[j] = hi[0]; ph[j + 1] = hi[1];
-      }
-      return rs;
-    };
-    float rs = weights();
-    // The maximum is looked for only where a token's weights say that it has outgrown m, or where there is none yet.  (What rows that
-    // take no part hold decides nothing: the columns of a wave look for theirs together, which shows in their last bits)
-    if (__any((int)live & (int)(!(rs <= kRoom) | (m == -INFINITY)))) {
-      if constexpr (TWO && KIND != MK_Q4) {
-        // An infinite K (4-bit scales make it NaN): the score is what the hi half says, whose infinity the lo half's 0 x inf, or infinity of
-        // the other sign, would turn into NaN.  The tile's K is still there (the products again: their results kept would spill)
-        if (__any(!(rs == rs))) {
-#pragma unroll
-          for (int mt = 0; mt < 2; mt++) {
-            f32x4 t = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KS; k++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, cur.k[mt][k]), q[k], t, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const float other = xchg8_f(t[i]), hi = lr < 8 ? t[i] : other;
-              if (y[4 * mt + i] != y[4 * mt + i] && fabsf(hi) == INFINITY) y[4 * mt + i] = hi;   // (masked ones are -inf)
-            }
-          }
-        }
-      }
-      float bm = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; j++) bm = fmaxf(bm, y[j]);
-      bm = pair_max32(pair_max16(bm)) * f;   // f > 0
-      const float mn = fmaxf(m, bm), corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= corr;
-#pragma unroll
-      for (int d = 0; d < DT; d++) o[d] *= corr;
-      sub = kPBias - (m == -INFINITY ? 0.f : m);
-      rs = weights();
-    }
-    l += rs;
-    // what no column sees may hold anything: zeroed (4-bit: its scales), since 0 x NaN is not 0; what only some see, without its
-    // NaN and infinite values
-    uint32_t bad = 0;
-    auto clean = [&](u32x4 w) {
-      uint32_t keep = on;
-      if (s.PA != s.PB) { const uint32_t n = not_finite(w) & on; bad |= n; keep &= ~n; }
-      return __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, w), keep));
-    };
-    if constexpr (KIND == MK_Q4) {
-      if (edge) {
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) cur.vs[i] = clean(cur.vs[i]);
-      }
-#pragma unroll
-      for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values(cur.v[d], cur.vs[d / 2]), ph, o[d], 0, 0, 0);
-    } else {
-      // V's tile in LDS (a wait written out, since the compiler does not see what the loads write)
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (tile + NW < t1) load_k<HD, KIND>(a, h, s, tile + NW, lane, cur);
-      // ds_read_b64_tr_b16 hands lane i of 16 the element i % 4 of what lanes 4 j + i / 4 address, as its element j
-      const int xr = 8 * lg + (lr >> 2), dq = 4 * (lr & 3);
-#pragma unroll
-      for (int d = 0; d < DT; d++) {
-        const int seg = (16 * d + dq) >> 3, in8 = dq & 4;
-        const s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + xr * HD + 8 * (seg ^ vsw<HD>(xr)) + in8));
-        const s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(vbuf + (xr + 4) * HD + 8 * (seg ^ vsw<HD>(xr + 4)) + in8));
-        u32x4 w = __builtin_bit_cast(u32x4, (s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-        if (edge) w = clean(w);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, w), ph, o[d], 0, 0, 0);
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile is read before the next one's loads write it
-    }
-    if (tile + NW < t1) load_v<HD, KIND>(a, h, s, tile + NW, lane, cur, vbuf);
-    if (__any(bad != 0)) {
-#pragma unroll 1
-      for (int i = 0; i < kFewTile; i++) {   // record i / 8 is lane group i / 8's
-        if (!(__ballot(bad >> (i % kRec) & 1) >> 16 * (i / kRec) & 0xffff)) continue;
-        const int r = record(s, 4 * tile + i / kRec), p = kRec * r + i % kRec;
-        const bool sp = sees(a, P, lo, p) & (!TWO | (lr < 8));
-#pragma unroll
-        for (int d = 0; d < DT; d++) add_bad<HD, KIND>(h.rec + (int64_t)r * (9 * HD), h.v + (int64_t)p * a.crow, p, 16 * d + 4 * lg, sp, o[d], 0);
-      }
-    }
-  }
-  l = pair_sum32(pair_sum16(l));
-  // the waves' sums meet in LDS
-  if (KIND != MK_Q4) __syncthreads();   // no wave's V tile is in use
-  float *ored = (float *)sm;
-#pragma unroll
-  for (int d = 0; d < DT; d++) {
-    f32x4 y = o[d];
-    if (TWO) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {   // an infinite V: as the scores, hi's sum where only lo's makes it NaN
-        const float both = y[i] + xchg8_f(y[i]);
-        y[i] = KIND != MK_Q4 && both != both && fabsf(y[i]) == INFINITY ? y[i] : both;
-      }
-    }
-    if (lr < NC) *(f32x4 *)(ored + (wave * NC + lr) * QS + 16 * d + 4 * lg) = y;
-  }
-  if (lg == 0 && lr < NC) { wm[wave][lr] = m; wl[wave][lr] = l; }
-  __syncthreads();
-  const int e = threadIdx.x, c = e / (HD / 4), d = 4 * (e % (HD / 4));
-  if (c >= NC) return;
-  const int cc = c0 + c, tk = token_of(a, cc);
-  if (tk >= s.cnt || (!PRE && (int64_t)s.P0 + tk >= a.ctx)) return;   // (a prefix's pass leaves zeros for tokens that take no part: not read)
-  float M = -INFINITY, L = 0.f;
-#pragma unroll
-  for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][c]);
-  f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  const float Mz = M == -INFINITY ? 0.f : M;
-#pragma unroll
-  for (int w = 0; w < NW; w++) {
-    const float k = __builtin_amdgcn_exp2f(wm[w][c] - Mz);
-    L += wl[w][c] * k;
-    y += *(const f32x4 *)(ored + (w * NC + c) * QS + d) * k;
-  }
-  const int head = g * a.rep + cc - tk * a.rep;
-  if (!PRE && s.S == 1 && !a.joined) {
-    const float inv = 1.f / L;   // a visible position's score is -inf only where the plain softmax gives NaN too: 0 x inf
-    float r[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = y[i] * inv;
-    store_elems<T, 4>(a.out, b * a.out.seq + (int64_t)tk * a.out.tok + (int64_t)head * a.out.head + d, r);
-    return;
-  }
-  const int64_t row = ((int64_t)b * a.n + tk) * a.heads + head, at = row * a.slots + a.slot0 + split;
-  *(f32x4 *)(a.part + at * HD + d) = y;
-  if (d == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD + 2 * at) = make_float2(M, L);
 }
 
 // The splits' sums of one row a workgroup: 256 threads, HD / 4 of them side by side over the dims, the others over the
@@ -691,8 +506,8 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a, KvJoin p) {
   if (!s.any || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
   const int S0 = prefix_splits(p);
   const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
-  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD) + row * a.slots;
-  const float *po = a.part + row * a.slots * HD;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of(a) * HD) + row * slots_of(a);
+  const float *po = a.part + row * slots_of(a) * HD;
   const int ct = threadIdx.x % CT, sl = threadIdx.x / CT, lane = threadIdx.x & 63;
   const float2 none = make_float2(-INFINITY, 0.f), x = lane < s.S ? ml[lane] : none, x0 = lane < S0 ? ml[a.nsplit + lane] : none;
   const float M = wave_max(fmaxf(x.x, x0.x)), Mz = M == -INFINITY ? 0.f : M;
@@ -724,8 +539,8 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a, KvJoin p) {
   if (!s.any || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
   const int S0 = prefix_splits(p);
   const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
-  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD) + row * a.slots;
-  const float *po = a.part + row * a.slots * HD + 4 * ct;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of(a) * HD) + row * slots_of(a);
+  const float *po = a.part + row * slots_of(a) * HD + 4 * ct;
   float M = -INFINITY, L = 0.f;
 #pragma unroll 8
   for (int k = 0; k < s.S + S0; k++) M = fmaxf(M, ml[k < s.S ? k : a.nsplit + k - s.S].x);
@@ -765,7 +580,7 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a, KvJoin p) {
 constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
 
 template <int HD, int KIND, int T, bool PRE = false>
-__global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
+__global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
   constexpr bool TWO = T == RT_F32;
   constexpr int NT = kManyWaves * 64, KQ = HD / 16, OT = HD / 32, BR = kManyBlk / kRec;
   constexpr int KST = HD + 8;                                   // halves of a K row in LDS: an odd number of 16-byte columns
@@ -777,20 +592,24 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
   __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
   const int b = blockIdx.z, g = blockIdx.x, rest = a.nsplit == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nsplit, split = blockIdx.y - rest * a.nsplit;
   const int chunk = a.nchunk - 1 - rest;   // without pairs: the last columns, with the most to read, first
-  const Span s = PRE ? prefix_span_of(a) : span_of(a, b, chunk);
+  Span s;
+  if constexpr (PRE) s = prefix_span_of(a);
+  else s = span_of(a, b, chunk);
   if (!s.any || split >= s.S) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, ln = lane & 31, hf = lane >> 5;
   // waves w and w + 4 share a SIMD: one of the front half, one of the back half
   const int cw = chunk_half(a, chunk, wave / (kManyWaves / 2)) + 32 * (wave % (kManyWaves / 2));
   // (columns past the last read its query, as in k_kv_few; a wave without any other takes no block and uses none of it)
   const int col = min(cw + ln, a.n * a.rep - 1), tok = token_of(a, col), head = g * a.rep + col - tok * a.rep;
-  const SeqTok sq = PRE ? seq_tok(a, tok) : SeqTok{b, tok};
-  const bool live = col == cw + ln && (PRE ? takes_part(a, sq) : tok < s.cnt && (int64_t)s.P0 + tok < a.ctx);
+  SeqTok sq{b, tok};
+  bool live = col == cw + ln;
+  if constexpr (PRE) { sq = seq_tok(a, tok); live = live && takes_part(a, sq); }
+  else live = live && tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
   const int P = live ? PRE ? s.PB : s.P0 + tok : -1;
   const int lo = behind(a, P);
   // first and last position of the wave's own columns, and of the halves'
   const int wa = token_of(a, cw);
-  const bool wlive = wa < s.cnt && (PRE || (int64_t)s.P0 + wa < a.ctx);
+  const bool wlive = PRE ? __any((int)live) : wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
   auto position = [&](int t) { return (int)min((int64_t)s.P0 + min(t, s.cnt - 1), a.ctx - 1); };
   const int PA = PRE ? s.PA : s.P0 + wa, PB = PRE ? s.PB : position(token_of(a, cw + 31));
   const int A0 = s.PA, B0 = PRE ? s.PB : position(last_token(a, chunk_half(a, chunk, 0))), A1 = PRE ? s.PA : s.P0 + token_of(a, chunk_half(a, chunk, 1));
@@ -887,6 +706,12 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     }
   };
   if (tid < 8) badp[tid / 2][tid % 2] = 0;
+  __shared__ int some;   // (PRE: whether some column takes part)
+  if constexpr (PRE) {
+    if (tid == 0) some = 0;
+    __syncthreads();
+    if (wlive) some = 1;
+  }
   h8 q[KQ], ql[TWO ? KQ : 1];
   float f = a.scale2;
   Stage st;
@@ -922,7 +747,8 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
           }
       }
     }
-    __syncthreads();   // badp
+    __syncthreads();   // badp, some
+    if constexpr (PRE) { if (!some) return; }
     if (partial_any(kb0)) clean(kb0, st);
     expand(kb0, st);
     if (kb0 + 1 < kb1) {
@@ -1102,7 +928,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
     }
   }
   if constexpr (T != RT_F32 && !PRE) {
-    if (s.S == 1 && !a.joined) {
+    if (s.S == 1 && !joined(a)) {
       // A lane has 4 dims here and there of its column; by way of the wave's own part of LDS the rows leave in 16-byte pieces
       // next to each other (4096 tokens with 32 heads: 105 -> 101 us)
       constexpr int RS = HD + 8;
@@ -1132,8 +958,8 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       return;
     }
   }
-  if (!live) return;
-  if (!PRE && s.S == 1 && !a.joined) {
+  if (!PRE && s.S == 1 && !joined(a)) {
+    if (!live) return;
     const float inv = 1.f / l;
     const int64_t at = b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head;
 #pragma unroll
@@ -1145,30 +971,48 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(KvAttnArgs a) {
       }
     return;
   }
-  const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head, at = row * a.slots + a.slot0 + split;
+  // partial sums, by way of the wave's own part of LDS like the rows above, 64 dims at a time: 256 bytes of a column next to each other instead of 16 here and there
+  constexpr int RS = 64 + 4;
+  static_assert(kManyWaves * 32 * RS * 2 <= 3 * (kManyBlk * KST + VN), "the columns fit where the blocks were");
+  float *ow = (float *)blocks + wave * 32 * RS;
+  const uint64_t lives = __ballot(live);
+  auto place = [&](int tok, int head) { return (((int64_t)b * a.n + tok) * a.heads + head) * slots_of(a) + (PRE ? slots_of(a) - a.nsplit : 0) + split; };
 #pragma unroll
-  for (int t = 0; t < OT; t++)
+  for (int h = 0; h < HD / 64; h++) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      *(f32x4 *)(a.part + at * HD + 32 * t + 8 * i + 4 * hf) = (f32x4){o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
-  if (hf == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * a.slots * HD + 2 * at) = make_float2(m, l);
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *(f32x4 *)(ow + ln * RS + 32 * t + 8 * i + 4 * hf) = (f32x4){o[2 * h + t][4 * i], o[2 * h + t][4 * i + 1], o[2 * h + t][4 * i + 2], o[2 * h + t][4 * i + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int c = 4 * i + lane / 16, cc = cw + c, tk = token_of(a, cc);
+      if (lives >> c & 1) *(f32x4 *)(a.part + place(tk, g * a.rep + cc - tk * a.rep) * HD + 64 * h + 4 * (lane % 16)) = *(const f32x4 *)(ow + c * RS + 4 * (lane % 16));
+    }
+  }
+  if (live && hf == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of(a) * HD + 2 * place(tok, head)) = make_float2(m, l);
 }
 
 // ------------------------------------------------------------------ launches
 // KERNEL<HD, T> by head dim and rows' type
-#define QPH_KV(KERNEL, hd, type, grid, threads, a)                                                                      \
+#define QPH_KVN(KERNEL, hd, type, grid, threads, ...)                                                                   \
   do {                                                                                                                  \
     const dim3 g_ = (grid), t_(threads);                                                                                \
     if ((hd) == 128) {                                                                                                  \
-      if ((type) == RT_F32) hipLaunchKernelGGL((KERNEL<128, RT_F32>), g_, t_, 0, st, a);                                \
-      else if ((type) == RT_F16) hipLaunchKernelGGL((KERNEL<128, RT_F16>), g_, t_, 0, st, a);                           \
-      else hipLaunchKernelGGL((KERNEL<128, RT_BF16>), g_, t_, 0, st, a);                                                \
+      if ((type) == RT_F32) hipLaunchKernelGGL((KERNEL<128, RT_F32>), g_, t_, 0, st, __VA_ARGS__);                      \
+      else if ((type) == RT_F16) hipLaunchKernelGGL((KERNEL<128, RT_F16>), g_, t_, 0, st, __VA_ARGS__);                 \
+      else hipLaunchKernelGGL((KERNEL<128, RT_BF16>), g_, t_, 0, st, __VA_ARGS__);                                      \
     } else {                                                                                                            \
-      if ((type) == RT_F32) hipLaunchKernelGGL((KERNEL<64, RT_F32>), g_, t_, 0, st, a);                                 \
-      else if ((type) == RT_F16) hipLaunchKernelGGL((KERNEL<64, RT_F16>), g_, t_, 0, st, a);                            \
-      else hipLaunchKernelGGL((KERNEL<64, RT_BF16>), g_, t_, 0, st, a);                                                 \
+      if ((type) == RT_F32) hipLaunchKernelGGL((KERNEL<64, RT_F32>), g_, t_, 0, st, __VA_ARGS__);                       \
+      else if ((type) == RT_F16) hipLaunchKernelGGL((KERNEL<64, RT_F16>), g_, t_, 0, st, __VA_ARGS__);                  \
+      else hipLaunchKernelGGL((KERNEL<64, RT_BF16>), g_, t_, 0, st, __VA_ARGS__);                                       \
     }                                                                                                                   \
   } while (0)
+#define QPH_KV(KERNEL, hd, type, grid, threads, a) QPH_KVN(KERNEL, hd, type, grid, threads, a)
 template <bool WRITE>
 void launch_io16(const KvIoArgs &a, hipStream_t st) {
   const dim3 grid((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), thr(256);
@@ -1194,7 +1038,8 @@ int kv_few() {
   const char *e = getenv("QPH_KV_FEW");
   return e && *e ? std::max(0, atoi(e)) : -1;
 }
-size_t kv_attn_plan(KvAttnArgs &a) {
+// parted: the sums are joined with others' in any case
+size_t kv_attn_plan(KvAttnArgs &a, bool parted) {
   const int cus = 256;
   const bool two = a.q.type == RT_F32;
   const int64_t cols = (int64_t)a.n * a.rep;
@@ -1216,7 +1061,7 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   a.half_log2 = a.many ? 7 : two ? 2 : 3;
   a.tile_log2 = a.many ? 3 : 2;   // records of a tile
   a.min_log2 = a.many ? 2 : 3;    // tiles of a split, at least
-  a.one_tiles = a.many ? 4 : 4 * kFewWaves;
+  a.one_tiles = parted ? -1 : a.many ? 4 : 4 * kFewWaves;
   const int tile = kRec << a.tile_log2;
   // floor(col / rep) = floor(col mul / 2^(32 + shift)) for col < 2^30: mul = ceil(2^(32 + shift) / rep) with 2^shift < rep <= 2^(shift + 1)
   a.rep_shift = 0;
@@ -1228,7 +1073,6 @@ size_t kv_attn_plan(KvAttnArgs &a) {
   const int64_t want = (a.many ? 1 : 2) * (int64_t)cus / std::max<int64_t>(groups, 1);
   a.nsplit = tiles <= a.one_tiles ? 1 : (int)std::max<int64_t>(1, std::min({want, (tiles >> a.min_log2) + 1, (int64_t)64}));
   if (a.n > 65535 || a.nchunk * a.nsplit > 65535) a.nsplit = 1;   // grid limits
-  a.slots = a.nsplit; a.slot0 = 0; a.joined = 0;
   return a.nsplit > 1 ? (size_t)a.nseq * a.n * a.heads * a.nsplit * (a.hd + 2) * 4 : 0;
 }
 
@@ -1249,7 +1093,7 @@ hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st) {
     else QPH_KV(k_few16, a.hd, a.q.type, grid, kFewWaves * 64, a);
   }
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.nsplit == 1 || a.joined) return e;
+  if (e != hipSuccess || a.nsplit == 1 || joined(a)) return e;
   if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows) QPH_KV(k_kv_merge_rows, a.hd, a.q.type, dim3((a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd), 1, a.nseq), 256, a);   // (at most 32768 rows a sequence: groups <= 256)
   else QPH_KV(k_kv_merge, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a);
   return hipGetLastError();
@@ -1258,46 +1102,34 @@ hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st) {
 // ------------------------------------------------------------------ a common prefix
 // Three launches: the sequences' own positions as above, the prefix as if all sequences' tokens were one sequence's, and what joins their sums.
 // `a` is the own part's, planned; the prefix's plan goes by the columns of all sequences
-size_t kv_prefix_plan(KvAttnArgs &a, KvAttnArgs &p) {
-  kv_attn_plan(a);
-  kv_attn_plan(p);
+size_t kv_prefix_plan(KvAttnArgs &a, KvPreArgs &p) {
+  kv_attn_plan(a, true);
+  kv_attn_plan(p, true);
+  if (a.many && !p.many) { p.few = 0; kv_attn_plan(p, true); }   // one launch where both are of few tokens
   p.paired = 0;   // (every column sees all: nothing to even out)
-  a.slots = p.slots = a.nsplit + p.nsplit;
-  p.slot0 = a.nsplit;
-  a.joined = p.joined = 1;
-  return (size_t)a.nseq * a.n * a.heads * a.slots * (a.hd + 2) * 4;
+  a.one_tiles = p.one_tiles = -(a.nsplit + p.nsplit);
+  return (size_t)a.nseq * a.n * a.heads * slots_of(a) * (a.hd + 2) * 4;
 }
-template <int HD, int T> static constexpr auto k_pre_few4 = k_kv_few<HD, MK_Q4, T, true>;
-template <int HD, int T> static constexpr auto k_pre_few16 = k_kv_few<HD, MK_F32, T, true>;
+template <int HD, int T> static constexpr auto k_both4 = k_kv_few_both<HD, MK_Q4, T>;
+template <int HD, int T> static constexpr auto k_both16 = k_kv_few_both<HD, MK_F32, T>;
 template <int HD, int T> static constexpr auto k_pre_many4 = k_kv_many<HD, MK_Q4, T, true>;
 template <int HD, int T> static constexpr auto k_pre_many16 = k_kv_many<HD, MK_F32, T, true>;
-hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvAttnArgs &p, hipStream_t st) {
-  hipError_t e = launch_kv_attn(a, st);
-  if (e != hipSuccess) return e;
+hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvPreArgs &p, hipStream_t st) {
+  hipError_t e;
   if (p.many) {
+    if ((e = launch_kv_attn(a, st)) != hipSuccess) return e;
     const dim3 grid(p.nkv, p.nchunk * p.nsplit, 1);
     if (p.kind == MK_Q4) QPH_KV(k_pre_many4, p.hd, p.q.type, grid, kManyWaves * 64, p);
     else QPH_KV(k_pre_many16, p.hd, p.q.type, grid, kManyWaves * 64, p);
   } else {
-    const dim3 grid(p.nsplit, p.nkv * p.nchunk, 1);
-    if (p.kind == MK_Q4) QPH_KV(k_pre_few4, p.hd, p.q.type, grid, kFewWaves * 64, p);
-    else QPH_KV(k_pre_few16, p.hd, p.q.type, grid, kFewWaves * 64, p);
+    const int64_t blocks = (int64_t)p.nsplit * p.nkv * p.nchunk + (int64_t)a.nsplit * a.nkv * a.nchunk * a.nseq;
+    if (p.kind == MK_Q4) QPH_KVN(k_both4, p.hd, p.q.type, dim3((unsigned)blocks), kFewWaves * 64, a, p);
+    else QPH_KVN(k_both16, p.hd, p.q.type, dim3((unsigned)blocks), kFewWaves * 64, a, p);
   }
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const KvJoin j{p.prefix, p.tile_log2, p.min_log2, p.one_tiles, p.nsplit};
-#define QPH_JOIN(KERNEL, grid)                                                                                                                  \
-  do {                                                                                                                                          \
-    const dim3 g_ = (grid);                                                                                                                     \
-    if (a.hd == 128 && a.q.type == RT_F32) hipLaunchKernelGGL((KERNEL<128, RT_F32>), g_, dim3(256), 0, st, a, j);                               \
-    else if (a.hd == 128 && a.q.type == RT_F16) hipLaunchKernelGGL((KERNEL<128, RT_F16>), g_, dim3(256), 0, st, a, j);                          \
-    else if (a.hd == 128) hipLaunchKernelGGL((KERNEL<128, RT_BF16>), g_, dim3(256), 0, st, a, j);                                               \
-    else if (a.q.type == RT_F32) hipLaunchKernelGGL((KERNEL<64, RT_F32>), g_, dim3(256), 0, st, a, j);                                          \
-    else if (a.q.type == RT_F16) hipLaunchKernelGGL((KERNEL<64, RT_F16>), g_, dim3(256), 0, st, a, j);                                          \
-    else hipLaunchKernelGGL((KERNEL<64, RT_BF16>), g_, dim3(256), 0, st, a, j);                                                                 \
-  } while (0)
-  if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows || a.n > 65535) QPH_JOIN(k_kv_join_rows, dim3((unsigned)(((int64_t)a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd)), 1, a.nseq));
-  else QPH_JOIN(k_kv_join, dim3(a.heads, a.n, a.nseq));
-#undef QPH_JOIN
+  if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows || a.n > 65535) QPH_KVN(k_kv_join_rows, a.hd, a.q.type, dim3((unsigned)(((int64_t)a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd)), 1, a.nseq), 256, a, j);
+  else QPH_KVN(k_kv_join, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a, j);
   return hipGetLastError();
 }
 

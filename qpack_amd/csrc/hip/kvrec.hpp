@@ -140,13 +140,16 @@ __device__ __forceinline__ uint32_t kept_bits(int64_t p0, int64_t from, int64_t 
     if (!(p0 + i >= from && p0 + i < to)) keep |= 15u << nib(i);
   return keep;
 }
-// A wave's K (V) rows of the record at o: lane = position row = lane / 8, dims HD / 8 part .. in x, part = lane % 8.  Positions that are not `mine` keep their codes
-// and scales: their K rows and scales are not stored, and V words, which hold all 8 positions, are merged by `keep`.  codes: LDS, the V wave's
-template <int HD, int T>
-__device__ __forceinline__ void store_record(uint8_t *o, const float *x, bool mine, bool vside, int row, int part, uint32_t keep, uint8_t (*codes)[HD]) {
+// A wave's K (V) rows of a record: lane = position row = lane / 8, dims HD / 8 part .. by load(x), part = lane % 8, where the position is `mine`.  Others keep their codes
+// and scales: their K rows and scales are not stored, and V words, which hold all 8 positions, are merged: the record's positions are p0 .., the call's
+// from .. to - 1.  codes: LDS, the V wave's
+template <int HD, int T, typename Load, typename Record>
+__device__ __forceinline__ void store_record(Load load, Record record, bool mine, bool vside, int row, int part, int64_t p0, int64_t from, int64_t to, uint8_t (*codes)[HD]) {
   constexpr int EL = HD / 8, GL = 32 / EL;   // elements of a lane; lanes of a group
+  float x[EL];
   uint32_t mx = 0;
   if (mine) {
+    load(x);
 #pragma unroll
     for (int i = 0; i < EL; i++) mx = max(mx, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
   }
@@ -163,6 +166,7 @@ __device__ __forceinline__ void store_record(uint8_t *o, const float *x, bool mi
 #pragma unroll
     for (int i = 0; i < EL; i++) c[i] = 8;
   }
+  uint8_t *o = record();
   if (!vside) {
     if (!mine) return;
     uint32_t w[EL / 8];
@@ -184,6 +188,7 @@ __device__ __forceinline__ void store_record(uint8_t *o, const float *x, bool mi
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   const int lane = 8 * row + part;
+  const uint32_t keep = kept_bits(p0, from, to);
 #pragma unroll
   for (int k = 0; k < HD / 64; k++) {
     const int idx = lane * (HD / 64) + k, d = idx % (HD / 16) * 16 + idx / (HD / 16);

@@ -139,15 +139,9 @@ __global__ __launch_bounds__(128) void k_append4(KvAppendArgs a, int records) {
     const int row = lane >> 3, part = lane & 7;
     const int64_t p = rec * kRec + row, t = p - s.P0, at = b * r.seq + t * r.tok + g * r.head;
     const bool mine = p >= s.P0 && p < last;
-    const uint32_t keep = kept_bits(rec * kRec, s.P0, last);
-    float x[EL];
-    if (vside) {
-      if (mine) load_elems<T, EL>(r, at + EL * part, x);
-      store_record<HD, T>(o, x, mine, true, row, part, keep, codes);
-    } else {
-      turned<HD, EL, T>(a, r, at, a.kw, s.at + t, EL * part, mine, x);
-      store_record<HD, RT_F32>(o, x, mine, false, row, part, keep, codes);
-    }
+    auto record = [&]() { return o; };
+    if (vside) store_record<HD, T>([&](float *x) { load_elems<T, EL>(r, at + EL * part, x); }, record, mine, true, row, part, rec * kRec, s.P0, last, codes);
+    else store_record<HD, RT_F32>([&](float *x) { turned<HD, EL, T>(a, r, at, a.kw, s.at + t, EL * part, true, x); }, record, mine, false, row, part, rec * kRec, s.P0, last, codes);
   }
 }
 

@@ -338,21 +338,19 @@ struct KvAttnArgs {
   float scale2;                 // softmax scale times log2(e), > 0
   float *part;                  // nsplit > 1: partial sums, then (max, sum) pairs, kv_attn_plan's bytes
   int few = -1;                 // test hook: columns up to which k_kv_few is taken (-1: by kv_attn_plan's rule)
-  // set by kv_attn_plan
+  // set by kv_attn_plan (one_tiles: tiles that one split takes; below 0: sums that are joined with another pass's, so many of a row together)
   int many, paired, cols, half_log2, nchunk, tile_log2, min_log2, one_tiles, nsplit, rep_shift;
   uint32_t rep_mul;
-  // partial sums of a row: `slots` of them, this pass's from slot0 on; joined: they are left there also by a single split
-  int slots, slot0, joined;
-  KvPrefix prefix;              // of a prefix's pass alone
 };
+struct KvPreArgs : KvAttnArgs { KvPrefix prefix; };   // a prefix's pass
 int kv_few();   // that hook's value now (QPH_KV_FEW)
 // how the call is laid out; the bytes of part
-size_t kv_attn_plan(KvAttnArgs &a);
+size_t kv_attn_plan(KvAttnArgs &a, bool parted = false);
 hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st);
 // Attention whose sequences follow one prefix: a over their own cache, p over the prefix's with nseq 1 and the tokens of all sequences (prefix.n of each), both with
 // the same q, out, pos, lens and part
-size_t kv_prefix_plan(KvAttnArgs &a, KvAttnArgs &p);
-hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvAttnArgs &p, hipStream_t st);
+size_t kv_prefix_plan(KvAttnArgs &a, KvPreArgs &p);
+hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvPreArgs &p, hipStream_t st);
 
 // ---- kvstep.hip
 // rows q -> out and k, both with their norms (weights qw, kw; null: none) and turned by the angles of places at[b] + t (null: pos[b] + t) of the
