@@ -971,27 +971,29 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
       }
     return;
   }
-  // partial sums, by way of the wave's own part of LDS like the rows above, 64 dims at a time: 256 bytes of a column next to each other instead of 16 here and there
-  constexpr int RS = 64 + 4;
+  // partial sums, by way of the wave's own part of LDS like the rows above, half the dims at a time: a column's next to each other instead of 16 bytes here and there
+  constexpr int HW = HD / 2, RS = HW + 4, LR = HW / 4, RI = 64 / LR;   // dims, floats of a column in LDS, lanes of one, columns at a time
   static_assert(kManyWaves * 32 * RS * 2 <= 3 * (kManyBlk * KST + VN), "the columns fit where the blocks were");
   float *ow = (float *)blocks + wave * 32 * RS;
   const uint64_t lives = __ballot(live);
   auto place = [&](int tok, int head) { return (((int64_t)b * a.n + tok) * a.heads + head) * slots_of(a) + (PRE ? slots_of(a) - a.nsplit : 0) + split; };
 #pragma unroll
-  for (int h = 0; h < HD / 64; h++) {
+  for (int h = 0; h < 2; h++) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int t = 0; t < 2; t++)
+    for (int t = 0; t < OT / 2; t++)
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        *(f32x4 *)(ow + ln * RS + 32 * t + 8 * i + 4 * hf) = (f32x4){o[2 * h + t][4 * i], o[2 * h + t][4 * i + 1], o[2 * h + t][4 * i + 2], o[2 * h + t][4 * i + 3]};
+      for (int i = 0; i < 4; i++) {
+        const f32x16 &x = o[OT / 2 * h + t];
+        *(f32x4 *)(ow + ln * RS + 32 * t + 8 * i + 4 * hf) = (f32x4){x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+      }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int c = 4 * i + lane / 16, cc = cw + c, tk = token_of(a, cc);
-      if (lives >> c & 1) *(f32x4 *)(a.part + place(tk, g * a.rep + cc - tk * a.rep) * HD + 64 * h + 4 * (lane % 16)) = *(const f32x4 *)(ow + c * RS + 4 * (lane % 16));
+    for (int i = 0; i < 32 / RI; i++) {
+      const int c = RI * i + lane / LR, cc = cw + c, tk = token_of(a, cc);
+      if (lives >> c & 1) *(f32x4 *)(a.part + place(tk, g * a.rep + cc - tk * a.rep) * HD + HW * h + 4 * (lane % LR)) = *(const f32x4 *)(ow + c * RS + 4 * (lane % LR));
     }
   }
   if (live && hf == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of(a) * HD + 2 * place(tok, head)) = make_float2(m, l);
