@@ -186,7 +186,9 @@ __device__ __forceinline__ Span span_of(const KvAttnArgs &a, int b, int chunk) {
 }
 // The span of a pass over a common prefix: every column sees all of its positions.  Its columns are (sequence, token, query head), the tokens of all
 // sequences counted through, and b is 0
-__device__ __forceinline__ int prefix_length(const KvPrefix &p) { return p.len ? (int)min((int64_t)max(*p.len, 0), p.ctx) : (int)p.ctx; }
+// (through the scalar cache: a vector load of it would be waited for together with those before it)
+typedef const int __attribute__((address_space(4))) scalar_int;
+__device__ __forceinline__ int prefix_length(const KvPrefix &p) { return p.len ? (int)min((int64_t)max(*(const scalar_int *)(uintptr_t)p.len, 0), p.ctx) : (int)p.ctx; }
 __device__ __forceinline__ int splits_of(int nt, int one_tiles, int nsplit, int min_log2) { return nt <= one_tiles ? (int)(nt > 0) : min(nsplit, (nt + (1 << min_log2) - 1) >> min_log2); }
 __device__ __forceinline__ Span prefix_span_of(const KvPreArgs &a) {
   Span s;
@@ -592,6 +594,21 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
   __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
   const int b = blockIdx.z, g = blockIdx.x, rest = a.nsplit == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nsplit, split = blockIdx.y - rest * a.nsplit;
   const int chunk = a.nchunk - 1 - rest;   // without pairs: the last columns, with the most to read, first
+  // a prefix's queries are asked for before its length is known (behind it, with the sequences' positions, the first block came 1.5 us later TODO)
+  h8 q[KQ], ql[TWO ? KQ : 1];
+  float x[KQ][8];
+  auto queries = [&](SeqTok t, int head, int half) {
+    const int64_t at = t.b * a.q.seq + (int64_t)t.t * a.q.tok + (int64_t)head * a.q.head + 8 * half;
+#pragma unroll
+    for (int k = 0; k < KQ; k++) {
+      if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
+      else load_elems<T, 8>(a.q, at + 16 * k, x[k]);
+    }
+  };
+  if constexpr (PRE) {
+    const int w = threadIdx.x >> 6, c = min(chunk_half(a, chunk, w / (kManyWaves / 2)) + 32 * (w % (kManyWaves / 2)) + (int)(threadIdx.x & 31), a.n * a.rep - 1), t = token_of(a, c);
+    queries(seq_tok(a, t), g * a.rep + c - t * a.rep, threadIdx.x >> 5 & 1);
+  }
   Span s;
   if constexpr (PRE) s = prefix_span_of(a);
   else s = span_of(a, b, chunk);
@@ -706,13 +723,6 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
     }
   };
   if (tid < 8) badp[tid / 2][tid % 2] = 0;
-  __shared__ int some;   // (PRE: whether some column takes part)
-  if constexpr (PRE) {
-    if (tid == 0) some = 0;
-    __syncthreads();
-    if (wlive) some = 1;
-  }
-  h8 q[KQ], ql[TWO ? KQ : 1];
   float f = a.scale2;
   Stage st;
   {  // the first two blocks, asked for together
@@ -721,18 +731,13 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
     if (kb0 + 1 < kb1) fetch(kb0 + 1, st1);
     // ---- queries
     {
-      const int64_t at = sq.b * a.q.seq + (int64_t)sq.t * a.q.tok + (int64_t)head * a.q.head + 8 * hf;
-      float x[KQ][8], mx = 0.f;
+      if constexpr (!PRE) queries(sq, head, hf);
+      if constexpr (T != RT_F16) {
+        float mx = 0.f;
 #pragma unroll
-      for (int k = 0; k < KQ; k++) {
-        if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
-        else {
-          load_elems<T, 8>(a.q, at + 16 * k, x[k]);
+        for (int k = 0; k < KQ; k++)
 #pragma unroll
           for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
-        }
-      }
-      if constexpr (T != RT_F16) {
         mx = pair_max32(mx);
         const float p2 = row_power(mx);
         f = fminf(fmaxf(f / p2, kTinyF), kMostF);
@@ -747,8 +752,8 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
           }
       }
     }
-    __syncthreads();   // badp, some
-    if constexpr (PRE) { if (!some) return; }
+    if constexpr (PRE) { if (!__syncthreads_or(wlive)) return; }   // (no column takes part)
+    else __syncthreads();   // badp
     if (partial_any(kb0)) clean(kb0, st);
     expand(kb0, st);
     if (kb0 + 1 < kb1) {
