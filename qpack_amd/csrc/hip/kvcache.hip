@@ -417,7 +417,7 @@ __device__ __forceinline__ void few_tokens(A a, int split, int gc, int b) {   //
   auto &wl = few_wm<T, 1>();
 #include "kv_few.inc"
 }
-// a common prefix's workgroups and then the sequences' own, in one launch (a launch and the first kernel's last workgroups: 4 samples behind 700 positions 17.2 -> TODO us)
+// a common prefix's workgroups and then the sequences' own, in one launch (a launch and the first kernel's last workgroups: 4 samples behind 700 positions 17.2 -> 10.2 us with the joining)
 template <int HD, int KIND, int T>
 __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few_both(KvAttnArgs a, KvPreArgs p) {
   const uint32_t pre = (uint32_t)p.nsplit * p.nkv * p.nchunk;
@@ -594,7 +594,7 @@ __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
   __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
   const int b = blockIdx.z, g = blockIdx.x, rest = a.nsplit == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nsplit, split = blockIdx.y - rest * a.nsplit;
   const int chunk = a.nchunk - 1 - rest;   // without pairs: the last columns, with the most to read, first
-  // a prefix's queries are asked for before its length is known (behind it, with the sequences' positions, the first block came 1.5 us later TODO)
+  // a prefix's queries are asked for before its length is known (behind it, with the sequences' positions: 32 sequences behind 8190 positions 18.9 us for 17.8)
   h8 q[KQ], ql[TWO ? KQ : 1];
   float x[KQ][8];
   auto queries = [&](SeqTok t, int head, int half) {
@@ -1067,7 +1067,8 @@ size_t kv_attn_plan(KvAttnArgs &a, bool parted) {
   a.cols = a.many ? kManyCols : few;
   a.half_log2 = a.many ? 7 : two ? 2 : 3;
   a.tile_log2 = a.many ? 3 : 2;   // records of a tile
-  a.min_log2 = a.many ? 2 : 3;    // tiles of a split, at least
+  // tiles of a split, at least (parted, where the sums are joined in any case: with 8, 4 samples behind 700 positions 7.2 us for 6.4)
+  a.min_log2 = a.many || parted ? 2 : 3;
   a.one_tiles = parted ? -1 : a.many ? 4 : 4 * kFewWaves;
   const int tile = kRec << a.tile_log2;
   // floor(col / rep) = floor(col mul / 2^(32 + shift)) for col < 2^30: mul = ceil(2^(32 + shift) / rep) with 2^shift < rep <= 2^(shift + 1)
