@@ -7,10 +7,11 @@
 // then added as a tree.
 //
 // The alternatives: a wave keeps in LDS what of its logits may be among the K <= 64 first, and a bound that K of them reach.  Indices rise, so that only a
-// logit above the bound can get past those that are there; all lanes that have one leave it by a ballot and a count of the lanes before them.  Past
-// kLpKeep entries the bound is raised, by bisection over the values' order with a ballot and a count for each entry of a lane, until it leaves K to 2 K + 16; of a
-// wave's first load before anything is kept.  Where more than that are equal, the lower indices stay.  (Kept in order in registers and inserted one by one, a chain of some
-// hundred dependent instructions each, 20 alternatives of one row took 24 us, and of 1024 rows in bf16 129.)
+// logit above the bound can get past those that are there; all lanes that have one leave it by a ballot and a count of the lanes before them.  The first
+// bound is what K of the lanes' maxima of a load reach; past some 32 entries more than needed it is raised, by bisection over the values' order with a ballot and
+// a count for each entry of a lane.  Where too many are equal, the lower indices stay.  (Kept in order in registers and inserted one by one, a chain of some
+// hundred dependent instructions each, 20 alternatives of one row took 24 us, and of 1024 rows in bf16 129.  The first bound from all values of the load, 8 ballots and
+// counts a step: 64 rows of 151936 14.1 us for 13.0)
 //
 // A workgroup of 4 waves has a row, or a share of one where there are few; shares leave sums and lists that k_logprobs_merge joins.
 #include <hip/hip_runtime.h>
@@ -263,37 +264,39 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
     }
     if constexpr (TOP) {
       if (first) {
+        // K of the maxima of the lanes' halves reach the first bound, and few of the others: 20 of 128 maxima of 4 each some 22 of the 512
         first = false;
-        int64_t k[VE], b = kNoKey + 1;
+        float h[2] = {x[0], x[VE / 2]};
 #pragma unroll
-        for (int i = 0; i < VE; i++) k[i] = counts >> i & 1 ? key_of(order_of(x[i]), at + i) : kNoKey;
-        if (to - base > full) {   // the least of the lanes' maxima is reached by one of each lane
-          b = bound_of<VE>(k, order_of(-wave_max(-bm)), order_of(wave_max(bm)), a.top, most);
-          bound = order_in(b);
-        }
+        for (int i = 1; i < VE / 2; i++) { h[0] = fmaxf(h[0], x[i]); h[1] = fmaxf(h[1], x[VE / 2 + i]); }
+        const int o[2] = {order_of(fmaxf(h[0], -INFINITY)), order_of(fmaxf(h[1], -INFINITY))};   // (of NaN alone)
+        int n = 128;
+        bound = raised<2>(o, order_of(-wave_max(-fminf(value_of(o[0]), value_of(o[1])))), order_of(wave_max(bm)), a.top, most, n);
+        if (bound == order_of(-INFINITY)) {   // what a mask leaves, or a load with few elements: these too, but NaN, which no bound holds back
 #pragma unroll
-        for (int i = 0; i < VE; i++) {
-          const bool here = k[i] >= b;
-          const uint64_t m = __ballot(here);
-          if (here) buf[held + lanes_before(m)] = k[i];
-          held += __popcll(m);
-        }
-        last = value_of(bound);
-      } else {
-        if (!__any(bm > last)) return;
-#pragma unroll
-        for (int i = 0; i < VE; i++) {
-          const uint64_t m = __ballot(x[i] > last);
-          if (m) {
-            if (x[i] > last) buf[held + lanes_before(m)] = key_of(order_of(x[i]), at + i);
+          for (int i = 0; i < VE; i++) {
+            const bool here = (int)(x[i] == -INFINITY) & (int)(counts >> i & 1);
+            const uint64_t m = __ballot(here);
+            if (here) buf[held + lanes_before(m)] = key_of(order_of(x[i]), at + i);
             held += __popcll(m);
           }
         }
-        wave_sync();
-        if (held > full) {
-          bound = held > kLpKeep ? cut<CAP / 64>(buf, held, bound, a.top, most, lane) : cut<kLpKeep / 64>(buf, held, bound, a.top, most, lane);
-          last = value_of(bound);
+        last = value_of(max(bound - 2, order_of(-INFINITY)));   // (what passes is at the bound too, and at 0 both zeros)
+      }
+      if ((held <= full) & !__any(bm > last)) return;
+#pragma unroll
+      for (int i = 0; i < VE; i++) {
+        const uint64_t m = __ballot(x[i] > last);
+        if (m) {
+          if (x[i] > last) buf[held + lanes_before(m)] = key_of(order_of(x[i]), at + i);
+          held += __popcll(m);
         }
+      }
+      wave_sync();
+      last = value_of(bound);
+      if (held > full) {
+        bound = held > kLpKeep ? cut<CAP / 64>(buf, held, bound, a.top, most, lane) : cut<kLpKeep / 64>(buf, held, bound, a.top, most, lane);
+        last = value_of(bound);
       }
     }
   };

@@ -118,6 +118,23 @@ def test_not_finite_rows():
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("top", [1, 64])
+def test_nan_before_what_rises(type, top):
+    # each wave's first load is NaN and every later one passes its bound: what it keeps stays within its room, and the row beside it is right
+    V = 40000
+    x = torch.linspace(-20, 20, V).repeat(3, 1)
+    x[0, :4096] = math.nan
+    x[1, torch.randperm(V, generator=torch.Generator().manual_seed(top))[: V // 2]] = math.nan
+    x = x.to(dict(f32=torch.float32, f16=torch.float16, bf16=torch.bfloat16)[type]).cuda()
+    r = qa.logprobs(x.repeat(400, 1), torch.zeros(1200, dtype=torch.int32, device="cuda"), top)
+    nan = torch.arange(1200, device="cuda") % 3 < 2
+    assert bool(torch.isnan(r.logp[nan]).all()) and bool(torch.isnan(r.entropy[nan]).all()) and bool(torch.isnan(r.top_logp[nan]).all())
+    assert bool(((r.top_index >= -1) & (r.top_index < V)).all())
+    one = qa.logprobs(x[2:], torch.zeros(1, dtype=torch.int32, device="cuda"), top)
+    assert bool((r.top_index[~nan] == one.top_index).all()) and bool((r.rank[~nan] == one.rank).all())
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 def test_strides_alignment_and_no_tokens(type):
     gen = torch.Generator().manual_seed(4)
     base = (torch.randn(9, 4003, generator=gen) * 2).to(TYPES[type]).cuda()
