@@ -275,7 +275,7 @@ int qph_kv_append(const qph_kv *c, const qph_rows *q, const qph_rows *k, const q
 /* Copies positions, to the bit: position pos[b] + t of dst's sequence b (t and lens as above) becomes position index[b * index_seq + t] of src's sequence seqs[b]
  * (seqs NULL: b).  dst and src may be the same or share memory: all is read before anything is written, by way of work, qph_kv_copy_work bytes (0 where
  * the caches lie apart).  apart = 1 is the caller's word that no position that the call writes is read by it: then neither scratch nor a second pass.
- * Sequences and positions outside src take no part. */
+ * Sequences and positions outside src take no part.  n as for qph_kv_write. */
 int qph_kv_copy_work(const qph_kv *dst, const qph_kv *src, int n, int apart, int64_t *bytes);
 int qph_kv_copy(const qph_kv *dst, const qph_kv *src, const int *index, int64_t index_seq, int n, const int *pos, const int *lens, const int *seqs, int apart, void *work,
                 int64_t work_bytes, void *stream);
@@ -285,7 +285,7 @@ int qph_kv_copy(const qph_kv *dst, const qph_kv *src, const int *index, int64_t 
  * of logits ahead of that token's (larger, or equal with a lower index); a token outside the vocabulary has NaN and -1.  entropy[r] = -sum p ln p in
  * nats.  top_index / top_logp [rows][top]: the first top <= min(64, vocab) in the order of the ranks.  logp, entropy and rank may be NULL, tokens then too.
  * Logits of -inf have probability 0; a row with a NaN or +inf, or of -inf alone, has NaN results, and its top_index entries are indices or -1.
- * work: qph_logprobs_work bytes (16-byte aligned, NULL if 0) that no other call uses meanwhile. */
+ * rows <= 2^23, vocab <= 2^28.  work: qph_logprobs_work bytes (16-byte aligned, NULL if 0) that no other call uses meanwhile. */
 int qph_logprobs_work(int type, int64_t rows, int vocab, int top, int64_t *bytes);
 int qph_logprobs(const void *x, int type, int64_t rows, int vocab, int64_t ld, const int *tokens, int top, float *logp, float *entropy, int *rank, int *top_index,
                  float *top_logp, void *work, int64_t work_bytes, void *stream);

@@ -70,6 +70,10 @@ static void kv_cache(const qph_kv *c, int64_t *seq, int64_t *row) {
   *seq = (int64_t)between;
   if (c->k == c->v) throw std::invalid_argument("kv: the cache's k and v overlap");
 }
+// the launches count an fp16 cache's threads, 8 dims each, in 32 bits
+static void kv_threads(const qph_kv *c, int n) {
+  if (c->kind == QPH_F16 && (int64_t)n * c->kv_heads * c->head_dim > (int64_t)1 << 34) throw std::invalid_argument("kv: n * kv_heads * head_dim must not pass 2^34 for an fp16 cache");
+}
 static qph::KvRows kv_rows(const qph_rows *r, const char *what, bool out, int nseq, int n, int heads, int hd) {
   need(r, what); need(r->p, what);
   if (r->type != QPH_F32 && r->type != QPH_F16 && r->type != QPH_BF16) throw std::invalid_argument(std::string("kv: the type of ") + what + " must be QPH_F32, QPH_F16 or QPH_BF16");
@@ -97,8 +101,7 @@ static qph::KvIoArgs kv_io(const qph_kv *c, const qph_rows *k, const qph_rows *v
   a.k = kv_rows(k, "k", out, c->nseq, n, c->kv_heads, c->head_dim); a.v = kv_rows(v, "v", out, c->nseq, n, c->kv_heads, c->head_dim);
   if (a.k.type != a.v.type) throw std::invalid_argument("kv: k and v must have the same type");
   if (out && n && k->p == v->p) throw std::invalid_argument("kv: the rows of k and v overlap");
-  // the launch counts an fp16 cache's threads, 8 dims each, in 32 bits
-  if (c->kind == QPH_F16 && (int64_t)n * c->kv_heads * c->head_dim > (int64_t)1 << 34) throw std::invalid_argument("kv: n * kv_heads * head_dim must not pass 2^34 for an fp16 cache");
+  kv_threads(c, n);
   return a;
 }
 static void kv_attn_args(const qph_kv *c, int heads, int n, int window, int sinks, qph::KvAttnArgs &a) {
@@ -163,6 +166,7 @@ static void kv_copy_args(const qph_kv *dst, const qph_kv *src, int n, qph::KvCop
   kv_cache(src, &a.src_cseq, &a.src_crow);
   if (dst->kind != src->kind || dst->kv_heads != src->kv_heads || dst->head_dim != src->head_dim) throw std::invalid_argument("kv: caches that are copied between must have the same kind, kv_heads and head_dim");
   if (n < 0 || n > 1 << 20) throw std::invalid_argument("kv: n must be in [0, 2^20]");
+  kv_threads(dst, n);
   a.cache = dst->k; a.cache_v = dst->v; a.ctx = dst->ctx; a.nrec = qph::kv4_records(dst->ctx);
   a.src = src->k; a.src_v = src->v; a.src_ctx = src->ctx; a.src_nrec = qph::kv4_records(src->ctx);
   a.nseq = dst->nseq; a.src_nseq = src->nseq; a.nkv = dst->kv_heads; a.hd = dst->head_dim; a.n = n;
@@ -423,7 +427,7 @@ int qph_topk_noalloc(const float *x, int n, int M, int *idx, float *val, void *s
 }
 static void logprob_args(int type, int64_t rows, int vocab, int top, qph::LogprobArgs &a) {
   if (type != QPH_F32 && type != QPH_F16 && type != QPH_BF16) throw std::invalid_argument("logprobs: the type must be QPH_F32, QPH_F16 or QPH_BF16");
-  if (rows < 0 || rows > 1 << 24) throw std::invalid_argument("logprobs: rows must be in [0, 2^24]");
+  if (rows < 0 || rows > 1 << 23) throw std::invalid_argument("logprobs: rows must be in [0, 2^23]");   // (256 threads each, counted in 32 bits)
   if (vocab < 1 || vocab > 1 << 28) throw std::invalid_argument("logprobs: vocab must be in [1, 2^28]");
   if (top < 0 || top > std::min(qph::kLpTop, vocab)) throw std::invalid_argument("logprobs: top must be in [0, min(64, vocab)]");
   a.type = type == QPH_F32 ? qph::RT_F32 : type == QPH_F16 ? qph::RT_F16 : qph::RT_BF16;

@@ -534,7 +534,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a, KvJoin p) {
 template <int HD, int T>
 __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a, KvJoin p) {
   constexpr int CT = HD / 4;
-  const int b = blockIdx.z, ct = threadIdx.x % CT, i = blockIdx.x * (256 / CT) + threadIdx.x / CT;
+  const int b = blockIdx.z, ct = threadIdx.x % CT, i = (blockIdx.y * gridDim.x + blockIdx.x) * (256 / CT) + threadIdx.x / CT;   // (at most 2^30 rows)
   if (i >= a.n * a.heads) return;
   const int tok = i / a.heads, head = i - tok * a.heads, g = token_of(a, head), col = tok * a.rep + head - g * a.rep;
   const Span s = span_of(a, b, chunk_of(a, col));
@@ -1136,7 +1136,8 @@ hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvPreArgs &p, hipStream_t
   }
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const KvJoin j{p.prefix, p.tile_log2, p.min_log2, p.one_tiles, p.nsplit};
-  if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows || a.n > 65535) QPH_KVN(k_kv_join_rows, a.hd, a.q.type, dim3((unsigned)(((int64_t)a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd)), 1, a.nseq), 256, a, j);
+  const unsigned blocks = (unsigned)(((int64_t)a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd)), wide = std::min(blocks, 65536u);   // (a grid's threads are counted in 32 bits for each dimension)
+  if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows || a.n > 65535) QPH_KVN(k_kv_join_rows, a.hd, a.q.type, dim3(wide, (blocks + wide - 1) / wide, a.nseq), 256, a, j);
   else QPH_KVN(k_kv_join, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a, j);
   return hipGetLastError();
 }

@@ -93,6 +93,8 @@ def test_copy():
         refused(copy(src=src), "same kind")
     refused(copy(n=-1), "n must be")
     refused(copy(n=(1 << 20) + 1), "n must be")
+    wide = dict(kind=qa.QPH_F16, nseq=1, kv_heads=4096, head_dim=128, ctx=8, v=P << 5)
+    refused(copy(cache(**wide), cache(**{**wide, "k": P << 4}), n=1 << 20), "2^34")   # more threads than a launch counts
     refused(copy(index=None), "index is NULL")
     refused(copy(pos=None), "pos is NULL")
     refused(copy(stride=-1), "negative stride")
@@ -139,7 +141,7 @@ def test_logprobs():
     refused(logprobs(x=None), "NULL")
     refused(logprobs(type=qa.QPH_Q4), "type")
     refused(logprobs(x=P + 2), "aligned")
-    for n in (-1, (1 << 24) + 1):
+    for n in (-1, (1 << 23) + 1, 1 << 24, (1 << 24) + 1):
         refused(logprobs(n=n), "rows")
     for vocab in (0, (1 << 28) + 1):
         refused(logprobs(vocab=vocab), "vocab")

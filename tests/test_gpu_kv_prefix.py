@@ -217,3 +217,14 @@ def test_refusals():
     with pytest.raises(qa.QphError, match="same type"):
         c.attention(q, pos, prefix=p, out=q.float())
     assert c.attention(q[:, :0], pos, prefix=p).shape == (2, 0, 4, 64)
+
+
+def test_more_rows_than_a_grid_is_wide():
+    gen = torch.Generator().manual_seed(6)
+    n, rep, D, L = 8200, 65, 128, 30   # 8 rows a workgroup, 65536 workgroups side by side
+    p, K0, V0 = filled("f16", 1, 1, D, L, [L], gen)
+    c, K, V = filled("f16", 1, 1, D, n, [n], gen)
+    q = torch.randn(1, n, rep, D, generator=gen).half().cuda()
+    out = c.attention(q, i32([0]), prefix=p)
+    for t in (0, 4000, 8065, 8066, n - 1):
+        check_rows(out[0, t:t + 1], q[0, t:t + 1], both(K0, K, L, 0)[:L + t + 1], both(V0, V, L, 0)[:L + t + 1], L + t)

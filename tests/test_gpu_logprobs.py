@@ -211,3 +211,14 @@ def test_refusals():
         qa.logprobs(g, t)
     with torch.no_grad():
         assert qa.logprobs(g, t).logp.shape == (2,)
+
+
+def test_the_most_rows():
+    R = 1 << 23
+    x = (torch.arange(2 * R, device="cuda", dtype=torch.int32) % 777).half().view(R, 2)
+    r = qa.logprobs(x, (torch.arange(R, device="cuda") % 2).int(), 1)
+    d = (x[:, 1] - x[:, 0]).float()
+    assert torch.equal(r.top_index[:, 0].bool(), d > 0)
+    # differences of whole numbers are exact; the sum 1 + e^-d is off by 2^-24 (2 d e^-d + 6) or less, its logarithm by another 2^-23, the result's rounding is 2^-24 of it
+    want = -torch.nn.functional.softplus(torch.where(torch.arange(R, device="cuda") % 2 == 0, d, -d).double())
+    assert bool(((r.logp - want).abs() <= 2.0 ** -20 * (1 + want.abs())).all())
