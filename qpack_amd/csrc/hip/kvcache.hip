@@ -216,10 +216,9 @@ __device__ __forceinline__ bool takes_part(const KvPreArgs &a, SeqTok x) {
   const int P0 = a.pos[x.b];
   return (P0 >= 0) & (x.t < tokens_of(a.lens, x.b, a.prefix.n)) & ((int64_t)P0 + x.t < a.prefix.own_ctx);
 }
-// whether a pass leaves its sums, one split's too, to be joined with another pass's
-__host__ __device__ __forceinline__ bool joined(const KvAttnArgs &a) { return a.one_tiles < 0; }
-// the partial sums of a row: the own positions' first, a prefix's last
-__host__ __device__ __forceinline__ int slots_of(const KvAttnArgs &a) { return joined(a) ? -a.one_tiles : a.nsplit; }
+// the partial sums of a row: the own positions' first, a prefix's last.  JOIN: of a pass whose sums, one split's too, are joined with another pass's
+template <bool JOIN>
+__host__ __device__ __forceinline__ int slots_of(const KvAttnArgs &a) { return JOIN ? -a.one_tiles : a.nsplit; }
 // the first tile of share i of S (the product fits: nt <= 2^25, i <= 64)
 __device__ __forceinline__ int share(const Span &s, int i) { return s.S == 1 ? i * s.nt : (int)((uint32_t)i * (uint32_t)s.nt / (uint32_t)s.S); }
 __device__ __forceinline__ int record(const Span &s, int v) { return v < s.SR ? v : v + s.skip; }
@@ -393,41 +392,27 @@ constexpr int few_lds() {   // bytes: V's tiles, then the waves' sums
   constexpr int tiles = KIND == MK_Q4 ? 0 : kFewWaves * kFewTile * HD * 2, out = kFewWaves * (T == RT_F32 ? 8 : 16) * (HD + 4) * 4;
   return tiles > out ? tiles : out;
 }
-template <int HD, int KIND, int T>
-__device__ __forceinline__ uint8_t (&few_sm())[few_lds<HD, KIND, T>()] {
-  __shared__ __align__(16) uint8_t sm[few_lds<HD, KIND, T>()];
-  return sm;
-}
-template <int T, int I>
-__device__ __forceinline__ float (&few_wm())[kFewWaves][T == RT_F32 ? 8 : 16] {
-  __shared__ float wm[kFewWaves][T == RT_F32 ? 8 : 16];
-  return wm;
-}
-template <int HD, int KIND, int T, bool PRE = false>   // (PRE: below)
+template <int T> using few_cols = float[kFewWaves][T == RT_F32 ? 8 : 16];   // the waves' maxima, sums
+template <int HD, int KIND, int T, bool PRE = false, bool JOIN = false>   // (of the body)
 __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(Args<PRE> a) {
   __shared__ __align__(16) uint8_t sm[few_lds<HD, KIND, T>()];
-  __shared__ float wm[kFewWaves][T == RT_F32 ? 8 : 16], wl[kFewWaves][T == RT_F32 ? 8 : 16];
+  __shared__ few_cols<T> wm, wl;
   const int split = blockIdx.x, gc = blockIdx.y, b = blockIdx.z;
 #include "kv_few.inc"
 }
-template <int HD, int KIND, int T, bool PRE, typename A>
-__device__ __forceinline__ void few_tokens(A a, int split, int gc, int b) {   // (the arguments by value: by reference the kernel below spills)
-  auto &sm = few_sm<HD, KIND, T>();
-  auto &wm = few_wm<T, 0>();
-  auto &wl = few_wm<T, 1>();
-#include "kv_few.inc"
+// LDS of functions within one kernel: the same for the same arguments
+template <typename X, int I = 0>
+__device__ __forceinline__ X &lds() {
+  __shared__ __align__(16) X x;
+  return x;
 }
-// a common prefix's workgroups and then the sequences' own, in one launch (a launch and the first kernel's last workgroups: 4 samples behind 700 positions 17.2 -> 10.2 us with the joining)
-template <int HD, int KIND, int T>
-__global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few_both(KvAttnArgs a, KvPreArgs p) {
-  const uint32_t pre = (uint32_t)p.nsplit * p.nkv * p.nchunk;
-  if (blockIdx.x < pre) {
-    const uint32_t gc = blockIdx.x / (uint32_t)p.nsplit;
-    few_tokens<HD, KIND, T, true, KvPreArgs>(p, blockIdx.x - gc * p.nsplit, gc, 0);
-  } else {
-    const uint32_t i = blockIdx.x - pre, r = i / (uint32_t)a.nsplit, per = (uint32_t)a.nkv * a.nchunk, b = r / per;
-    few_tokens<HD, KIND, T, false, KvAttnArgs>(a, i - r * a.nsplit, r - b * per, b);
-  }
+// the same within a kernel that has other work beside it (PRE: over a common prefix; below) and LDS bytes for either.  (The arguments by value and LDS by its
+// name: by reference that kernel spills)
+template <int HD, int KIND, int T, bool PRE, int LDS, bool JOIN = true>
+__device__ __forceinline__ void few_tokens(Args<PRE> a, int split, int gc, int b) {
+  auto &sm = lds<uint8_t[LDS]>();
+  auto &wm = lds<few_cols<T>, 0>(), &wl = lds<few_cols<T>, 1>();
+#include "kv_few.inc"
 }
 
 // The splits' sums of one row a workgroup: 256 threads, HD / 4 of them side by side over the dims, the others over the
@@ -508,8 +493,8 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a, KvJoin p) {
   if (!s.any || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
   const int S0 = prefix_splits(p);
   const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
-  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of(a) * HD) + row * slots_of(a);
-  const float *po = a.part + row * slots_of(a) * HD;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of<true>(a) * HD) + row * slots_of<true>(a);
+  const float *po = a.part + row * slots_of<true>(a) * HD;
   const int ct = threadIdx.x % CT, sl = threadIdx.x / CT, lane = threadIdx.x & 63;
   const float2 none = make_float2(-INFINITY, 0.f), x = lane < s.S ? ml[lane] : none, x0 = lane < S0 ? ml[a.nsplit + lane] : none;
   const float M = wave_max(fmaxf(x.x, x0.x)), Mz = M == -INFINITY ? 0.f : M;
@@ -541,8 +526,8 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a, KvJoin p) {
   if (!s.any || tok >= s.cnt || (int64_t)s.P0 + tok >= a.ctx) return;
   const int S0 = prefix_splits(p);
   const int64_t row = ((int64_t)b * a.n + tok) * a.heads + head;
-  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of(a) * HD) + row * slots_of(a);
-  const float *po = a.part + row * slots_of(a) * HD + 4 * ct;
+  const float2 *ml = (const float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of<true>(a) * HD) + row * slots_of<true>(a);
+  const float *po = a.part + row * slots_of<true>(a) * HD + 4 * ct;
   float M = -INFINITY, L = 0.f;
 #pragma unroll 8
   for (int k = 0; k < s.S + S0; k++) M = fmaxf(M, ml[k < s.S ? k : a.nsplit + k - s.S].x);
@@ -581,427 +566,65 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a, KvJoin p) {
 // tokens each of 32 sequences 6 % more
 constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
 
-template <int HD, int KIND, int T, bool PRE = false>
+template <int HD>
+constexpr int many_kst() { return HD + 8; }   // halves of a K row in LDS: an odd number of 16-byte columns
+template <int HD, int KIND>
+constexpr int many_vst() { return KIND == MK_Q4 ? kManyBlk + 8 : HD + 32; }   // of a V^T row (dims), or a V row (positions): 4 rows of 64 bytes apart
+template <int HD, int KIND>
+constexpr int many_vn() { return (KIND == MK_Q4 ? HD : kManyBlk) * many_vst<HD, KIND>(); }
+template <int HD, int KIND>
+constexpr int many_lds() { return 3 * (kManyBlk * many_kst<HD>() + many_vn<HD, KIND>()); }
+using many_bad = uint32_t[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
+template <int HD, int KIND, int T, bool PRE = false, bool JOIN = false>   // (of the body)
 __global__ __launch_bounds__(kManyWaves * 64) void k_kv_many(Args<PRE> a) {
-  constexpr bool TWO = T == RT_F32;
-  constexpr int NT = kManyWaves * 64, KQ = HD / 16, OT = HD / 32, BR = kManyBlk / kRec;
-  constexpr int KST = HD + 8;                                   // halves of a K row in LDS: an odd number of 16-byte columns
-  constexpr int VST = KIND == MK_Q4 ? kManyBlk + 8 : HD + 32;   // of a V^T row (dims), or a V row (positions): 4 rows of 64 bytes apart
-  constexpr int VN = KIND == MK_Q4 ? HD * VST : kManyBlk * VST;
-  __shared__ __align__(16) uint16_t blocks[3 * (kManyBlk * KST + VN)];
-  auto k_of = [&](int kb) { return blocks + kb % 3 * (kManyBlk * KST); };
-  auto v_of = [&](int kb) { return blocks + 3 * (kManyBlk * KST) + kb % 3 * VN; };
-  __shared__ uint32_t badp[4][2];   // positions of block kb left to add_bad, at (kb - kb0) % 4: set in step kb - 2 or before the first, read in kb, cleared in kb + 1
-  const int b = blockIdx.z, g = blockIdx.x, rest = a.nsplit == 1 ? blockIdx.y : blockIdx.y / (uint32_t)a.nsplit, split = blockIdx.y - rest * a.nsplit;
-  const int chunk = a.nchunk - 1 - rest;   // without pairs: the last columns, with the most to read, first
-  // a prefix's queries are asked for before its length is known (behind it, with the sequences' positions: 32 sequences behind 8190 positions 18.9 us for 17.8)
-  h8 q[KQ], ql[TWO ? KQ : 1];
-  float x[KQ][8];
-  auto queries = [&](SeqTok t, int head, int half) {
-    const int64_t at = t.b * a.q.seq + (int64_t)t.t * a.q.tok + (int64_t)head * a.q.head + 8 * half;
-#pragma unroll
-    for (int k = 0; k < KQ; k++) {
-      if constexpr (T == RT_F16) q[k] = load_halves(a.q, at + 16 * k);
-      else load_elems<T, 8>(a.q, at + 16 * k, x[k]);
-    }
-  };
-  if constexpr (PRE) {
-    const int w = threadIdx.x >> 6, c = min(chunk_half(a, chunk, w / (kManyWaves / 2)) + 32 * (w % (kManyWaves / 2)) + (int)(threadIdx.x & 31), a.n * a.rep - 1), t = token_of(a, c);
-    queries(seq_tok(a, t), g * a.rep + c - t * a.rep, threadIdx.x >> 5 & 1);
-  }
-  Span s;
-  if constexpr (PRE) s = prefix_span_of(a);
-  else s = span_of(a, b, chunk);
-  if (!s.any || split >= s.S) return;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, ln = lane & 31, hf = lane >> 5;
-  // waves w and w + 4 share a SIMD: one of the front half, one of the back half
-  const int cw = chunk_half(a, chunk, wave / (kManyWaves / 2)) + 32 * (wave % (kManyWaves / 2));
-  // (columns past the last read its query, as in k_kv_few; a wave without any other takes no block and uses none of it)
-  const int col = min(cw + ln, a.n * a.rep - 1), tok = token_of(a, col), head = g * a.rep + col - tok * a.rep;
-  SeqTok sq{b, tok};
-  bool live = col == cw + ln;
-  if constexpr (PRE) { sq = seq_tok(a, tok); live = live && takes_part(a, sq); }
-  else live = live && tok < s.cnt && (int64_t)s.P0 + tok < a.ctx;
-  const int P = live ? PRE ? s.PB : s.P0 + tok : -1;
-  const int lo = behind(a, P);
-  // first and last position of the wave's own columns, and of the halves'
-  const int wa = token_of(a, cw);
-  const bool wlive = PRE ? __any((int)live) : wa < s.cnt && (int64_t)s.P0 + wa < a.ctx;
-  auto position = [&](int t) { return (int)min((int64_t)s.P0 + min(t, s.cnt - 1), a.ctx - 1); };
-  const int PA = PRE ? s.PA : s.P0 + wa, PB = PRE ? s.PB : position(token_of(a, cw + 31));
-  const int A0 = s.PA, B0 = PRE ? s.PB : position(last_token(a, chunk_half(a, chunk, 0))), A1 = PRE ? s.PA : s.P0 + token_of(a, chunk_half(a, chunk, 1));
-  const int kb0 = share(s, split), kb1 = share(s, split + 1);
-  const Head hd = head_of<HD, KIND>(a, b, g);
+  __shared__ __align__(16) uint16_t blocks[many_lds<HD, KIND>()];
+  __shared__ many_bad badp;
+  const int b = blockIdx.z, g = blockIdx.x, cs = blockIdx.y;
+#include "kv_many.inc"
+}
+template <int HD, int KIND, int T, bool PRE, int LDS, bool JOIN = true>
+__device__ __forceinline__ void many_tokens(Args<PRE> a, int g, int cs, int b) {
+  uint16_t *blocks = (uint16_t *)lds<uint8_t[LDS]>();
+  auto &badp = lds<many_bad>();
+#include "kv_many.inc"
+}
 
-  // ---- a block's codes (or fp16 pieces): memory -> registers -> LDS
-  // 4-bit: a thread has W words of a K row, and W of a record's V: dims 16 (W vt + i) + vr of record vl, so that the 16 lanes of a
-  // group write V^T rows next to each other.  fp16: pieces tid + NT i
-  constexpr int W = HD / 64, NP = KIND == MK_Q4 ? 1 : kManyBlk * HD / 8 / NT;
-  typedef uint32_t words __attribute__((ext_vector_type(W)));
-  struct Stage { words kq, vq; uint16_t ksc; u32x4 vsc, kp[NP], vp[NP]; };
-  const int krow = tid >> 3, kw = tid & 7, vl = tid >> 6, vr = tid & 15, vt = tid >> 4 & 3;
-  const uint32_t ko = krow / kRec * (9 * HD) + krow % kRec * (HD / 2) + 4 * W * kw, kso = krow / kRec * (9 * HD) + 8 * HD + 2 * (krow % kRec * (HD / 32) + W * kw / 4);
-  const uint32_t vo = vl * (9 * HD) + 4 * HD + vr * (HD / 4) + 4 * W * vt, vso = vl * (9 * HD) + 8 * HD + HD / 2 + 16 * (W * vt / 2);
-  int64_t po[NP];
-#pragma unroll
-  for (int i = 0; i < NP; i++) po[i] = (int64_t)((tid + NT * i) / (HD / 8)) * a.crow + 8 * ((tid + NT * i) % (HD / 8));
-  auto fetch = [&](int kb, Stage &g) {
-    const int v0 = BR * kb;
-    if constexpr (KIND == MK_Q4) {
-      if (run_of(s, v0, BR)) {
-        const uint8_t *r = hd.rec + (int64_t)record(s, v0) * (9 * HD);
-        g.kq = *(const words *)(r + ko); g.ksc = *(const uint16_t *)(r + kso);
-        g.vq = *(const words *)(r + vo); g.vsc = *(const u32x4 *)(r + vso);
-      } else {
-        const uint8_t *r = hd.rec + ((int64_t)record(s, min(v0 + krow / kRec, s.NR - 1)) - krow / kRec) * (9 * HD);
-        const uint8_t *rv = hd.rec + ((int64_t)record(s, min(v0 + vl, s.NR - 1)) - vl) * (9 * HD);
-        g.kq = *(const words *)(r + ko); g.ksc = *(const uint16_t *)(r + kso);
-        g.vq = *(const words *)(rv + vo); g.vsc = *(const u32x4 *)(rv + vso);
-      }
-    } else {
-      const int64_t p0 = (int64_t)kRec * record(s, v0);
-      const bool run = run_of(s, v0, BR) && p0 + kManyBlk <= a.ctx;
-      const uint16_t *k0 = hd.k + p0 * a.crow, *v00 = hd.v + p0 * a.crow;
-#pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        if (run) { g.kp[i] = *(const u32x4 *)(k0 + po[i]); g.vp[i] = *(const u32x4 *)(v00 + po[i]); }
-        else {
-          const int64_t at = row_of(a, s, v0 + x / kRec, x % kRec) + 8 * sg;
-          g.kp[i] = *(const u32x4 *)(hd.k + at);
-          g.vp[i] = *(const u32x4 *)(hd.v + at);
-        }
-      }
-    }
-  };
-  // Blocks by number.  A block from the window's on holds positions 64 kb + 8 skip ..; those before it (the first positions that stay
-  // visible) count as seen in part.  Of tokens A .. B: from whole(A) on A does not see all of a block, before left(B) B does not,
-  // ends(B) is the last that B sees some of.  (Comparisons with these few numbers: worked out anew for every block, they were a
-  // third of the loop's instructions, and a wave issues one in about ten cycles)
-  const int NRb = s.NR / BR, R0 = s.skip ? (s.SR + BR - 1) / BR : 0, off = kRec * s.skip;
-  auto whole = [&](int A) { return min((A + 1 - off) >> 6, NRb); };
-  auto left = [&](int B) { return a.window > 0 ? max((B - a.window - off) >> 6, -1) + 1 : 0; };
-  auto ends = [&](int B) { return (B - off) >> 6; };
-  static_assert(kManyBlk == 64, "the shifts above");
-  const int wK = whole(PA), wY = max(left(PB), R0), wE = wlive ? ends(PB) : -1;          // the wave's
-  const int gK0 = whole(A0), gE0 = ends(B0), gK1 = whole(A1), gY = max(left(s.PB), R0);   // the workgroup's halves'
-  auto partial = [&](int kb) { return (kb >= wK) | (kb < wY); };
-  // the same of the waves that take the block: a wave does not take a block behind its last position
-  auto partial_any = [&](int kb) { return ((kb >= gK0) & (kb <= gE0)) | (kb >= gK1) | (kb < gY); };
-  // what no column sees zeroed, and what only some see without its NaN and infinite values (4-bit: by the scales)
-  auto clean = [&](int kb, Stage &g) {
-    if constexpr (KIND == MK_Q4) {
-      const int v = BR * kb + vl;
-      const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))), bad = on & not_finite(g.vsc);
-      if (bad) atomicOr(&badp[(kb - kb0) % 4][vl / 4], bad << 8 * (vl % 4));
-      g.vsc = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, g.vsc), on & ~bad));
-    } else {
-#pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const int x = (tid + NT * i) / (HD / 8), v = BR * kb + x / kRec;
-        const uint32_t on = seen_bits(a, s, v, kRec * record(s, min(v, s.NR - 1))) >> x % kRec & 1 ? 255u : 0u, bad = on & not_finite(g.vp[i]);
-        if (bad) atomicOr(&badp[(kb - kb0) % 4][x / 32], 1u << x % 32);
-        g.vp[i] = __builtin_bit_cast(u32x4, only(__builtin_bit_cast(h8, g.vp[i]), on & ~bad));
-      }
-    }
-  };
-  auto expand = [&](int kb, Stage &g) {
-    uint16_t *kd = k_of(kb), *vd = v_of(kb);
-    if constexpr (KIND == MK_Q4) {
-#pragma unroll
-      for (int i = 0; i < W; i++) {
-        *(h8 *)(kd + krow * KST + 8 * (W * kw + i)) = values(g.kq[i], g.ksc);
-        *(h8 *)(vd + (16 * (W * vt + i) + vr) * VST + kRec * vl) = values(g.vq[i], g.vsc);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const int c = tid + NT * i, x = c / (HD / 8), sg = c % (HD / 8);
-        *(u32x4 *)(kd + x * KST + 8 * sg) = g.kp[i];
-        *(u32x4 *)(vd + x * VST + 8 * sg) = g.vp[i];
-      }
-    }
-  };
-  if (tid < 8) badp[tid / 2][tid % 2] = 0;
-  float f = a.scale2;
-  Stage st;
-  {  // the first two blocks, asked for together
-    Stage st1;
-    fetch(kb0, st);
-    if (kb0 + 1 < kb1) fetch(kb0 + 1, st1);
-    // ---- queries
-    {
-      if constexpr (!PRE) queries(sq, head, hf);
-      if constexpr (T != RT_F16) {
-        float mx = 0.f;
-#pragma unroll
-        for (int k = 0; k < KQ; k++)
-#pragma unroll
-          for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[k][j]));
-        mx = pair_max32(mx);
-        const float p2 = row_power(mx);
-        f = fminf(fmaxf(f / p2, kTinyF), kMostF);
-#pragma unroll
-        for (int k = 0; k < KQ; k++)
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float y = x[k][j] * p2;
-            const _Float16 h = (_Float16)y;
-            q[k][j] = h;
-            if constexpr (TWO) ql[k][j] = (_Float16)(y - (float)h);
-          }
-      }
-    }
-    if constexpr (PRE) { if (!__syncthreads_or(wlive)) return; }   // (no column takes part)
-    else __syncthreads();   // badp
-    if (partial_any(kb0)) clean(kb0, st);
-    expand(kb0, st);
-    if (kb0 + 1 < kb1) {
-      if (partial_any(kb0 + 1)) clean(kb0 + 1, st1);
-      expand(kb0 + 1, st1);
-    }
+// ------------------------------------------------------------------ a common prefix
+// The sequences' own positions, the prefix as if all sequences' tokens were one sequence's, and what joins their sums (k_kv_join, k_kv_join_rows).  The prefix's
+// workgroups come first and the own ones after them in one launch: they fill what the prefix's leave idle, and a launch and the first kernel's last
+// workgroups are saved.  4 samples behind 700 positions 17.2 -> 10.2 us with the joining, 83 sequences behind 4380 33 -> 25, 681 tokens of 2 behind 105 45 -> 35, 8 x up to 128 behind
+// 12001 211 -> 208.5
+template <int HD, int KIND, int T>
+__global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_both_few(KvAttnArgs a, KvPreArgs p) {
+  constexpr int LDS = few_lds<HD, KIND, T>();
+  const uint32_t pre = (uint32_t)p.nsplit * p.nkv * p.nchunk;
+  if (blockIdx.x < pre) {
+    const uint32_t gc = blockIdx.x / (uint32_t)p.nsplit;
+    few_tokens<HD, KIND, T, true, LDS>(p, blockIdx.x - gc * p.nsplit, gc, 0);
+  } else {
+    const uint32_t i = blockIdx.x - pre, r = i / (uint32_t)a.nsplit, per = (uint32_t)a.nkv * a.nchunk, b = r / per;
+    few_tokens<HD, KIND, T, false, LDS>(a, i - r * a.nsplit, r - b * per, b);
   }
-  if (kb0 + 2 < kb1) fetch(kb0 + 2, st);
-  __syncthreads();
-  f32x16 o[OT];
-#pragma unroll
-  for (int t = 0; t < OT; t++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) o[t][i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  // LDS row of the lane's K row
-  const int kr = (ln & 16) | (ln & 4) << 1 | (ln & 8) >> 1 | (ln & 3);
-  auto vfrag = [&](const uint16_t *v, int t, int u) {
-    if constexpr (KIND == MK_Q4) return *(const h8 *)(v + (32 * t + ln) * VST + 16 * u + 8 * hf);
-    else {
-      const int r = lane & 15, x = 16 * u + 8 * hf + (r >> 2), d = 32 * t + (ln & 16) + 4 * (r & 3);
-      const s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v + x * VST + d));
-      const s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(v + (x + 4) * VST + d));
-      return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-  };
-  h8 ph[4], pl[TWO ? 4 : 1];
-  f32x16 sc[2];
-  auto dots = [&](int kb) {   // K q of a block
-    const uint16_t *kl = k_of(kb);
-#pragma unroll
-    for (int mt = 0; mt < 2; mt++) {
-#pragma unroll
-      for (int i = 0; i < 16; i++) sc[mt][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KQ; k++) {
-        const h8 kf = *(const h8 *)(kl + (32 * mt + kr) * KST + 16 * k + 8 * hf);
-        sc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[k], sc[mt], 0, 0, 0);
-        if constexpr (TWO) sc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc[mt], 0, 0, 0);
-      }
-    }
-  };
-  float sub = kPBias;
-  auto weights = [&]() {   // sc -> ph, pl and their sum over the lane's positions
-    float rs = 0.f;
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][8 * (u & 1) + j], f, sub));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][8 * (u & 1) + j + 1], f, sub));
-        const h2 h = {(_Float16)p0, (_Float16)p1};
-        ph[u][j] = h[0]; ph[u][j + 1] = h[1];
-        if constexpr (TWO) {
-          rs += p0; rs += p1;
-          pl[u][j] = (_Float16)(p0 - (float)h[0]); pl[u][j + 1] = (_Float16)(p1 - (float)h[1]);
-        } else {
-          rs = __builtin_amdgcn_fdot2(h, (h2){(_Float16)1.f, (_Float16)1.f}, rs, false);   // the sum of what the product takes
-        }
-      }
-    return rs;
-  };
-  auto product = [&](int kb) {
-    const uint16_t *vb = v_of(kb);
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-#pragma unroll
-      for (int t = 0; t < OT; t++) {
-        const h8 x = vfrag(vb, t, u);
-        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[u], o[t], 0, 0, 0);
-        if constexpr (TWO) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[u], o[t], 0, 0, 0);
-      }
-  };
-  auto fix = [&](int kb) {
-#pragma unroll 1
-      for (int w = 0; w < 2; w++) {
-        uint32_t bad = __builtin_amdgcn_readfirstlane(badp[(kb - kb0) % 4][w]);
-        while (bad) {
-          const int x = 32 * w + __builtin_ctz(bad), r = record(s, BR * kb + x / kRec), p = kRec * r + x % kRec;
-          const bool sp = sees(a, P, lo, p);
-          bad &= bad - 1;
-#pragma unroll
-          for (int t = 0; t < OT; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) add_bad<HD, KIND>(hd.rec + (int64_t)r * (9 * HD), hd.v + (int64_t)p * a.crow, p, 32 * t + 8 * i + 4 * hf, sp, o[t], 4 * i);
-        }
-      }
-  };
-  auto first = [&](int kb) { return kRec * record(s, BR * kb); };
-  auto last = [&](int kb) { return kRec * record(s, min(BR * kb + BR - 1, s.NR - 1)) + kRec - 1; };
-  // Step kb: K q, the weights, then P V beside the expansion of block kb + 2 (whose codes were asked for a step ago); kb + 3 is asked for.
-  // Two blocks ahead, not one: 4 % less time
-  for (int kb = kb0; kb < kb1; kb++) {
-    if (kb + 2 < kb1 && partial_any(kb + 2)) clean(kb + 2, st);
-    // one of the wave's columns sees some of the block?  (Read through the lane: left to itself the compiler splits the loop at wE and
-    // keeps two copies of o, 58 registers more)
-    const int before = (int)(a.window > 0) & (int)(kb < wY) & (int)(last(kb) <= PA - a.window) & (int)(first(kb) >= a.sinks);
-    if (__builtin_amdgcn_readfirstlane((int)(kb <= wE) & (before ^ 1))) {
-      dots(kb);
-      if (partial(kb)) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const int v = BR * kb + 2 * u + hf, p0 = kRec * record(s, min(v, s.NR - 1)), Pin = v < s.NR ? P : -1;
-#pragma unroll
-          for (int j = 0; j < 8; j++) sc[u >> 1][8 * (u & 1) + j] = sees(a, Pin, lo, p0 + j) ? sc[u >> 1][8 * (u & 1) + j] : -INFINITY;
-        }
-      }
-      float rs = weights();
-      // as in k_kv_few, by the tokens' columns alone
-      if (__any((int)live & (int)(!(rs <= kRoom) | (m == -INFINITY)))) {
-        if constexpr (TWO && KIND != MK_Q4) {
-          // An infinite K, as in k_kv_few: where the sum is NaN (the masked are -inf) and hi's product alone infinite, that is the score
-          if (__any(!(rs == rs))) {
-            const uint16_t *kl = k_of(kb);
-#pragma unroll
-            for (int mt = 0; mt < 2; mt++) {
-              f32x16 t;
-#pragma unroll
-              for (int i = 0; i < 16; i++) t[i] = 0.f;
-#pragma unroll
-              for (int k = 0; k < KQ; k++) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8 *)(kl + (32 * mt + kr) * KST + 16 * k + 8 * hf), q[k], t, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 16; i++)
-                if (sc[mt][i] != sc[mt][i] && fabsf(t[i]) == INFINITY) sc[mt][i] = t[i];
-            }
-          }
-        }
-        float bm = -INFINITY;
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[mt][i]);
-        bm = pair_max32(bm) * f;   // f > 0
-        const float mn = fmaxf(m, bm), corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= corr;
-#pragma unroll
-        for (int t = 0; t < OT; t++) o[t] *= corr;
-        sub = kPBias - (m == -INFINITY ? 0.f : m);
-        rs = weights();
-      }
-      l += rs;
-      product(kb);
-      expand(kb + 2, st);   // (past the last block: what the registers hold, to a place that is not read again)
-      if (partial_any(kb)) fix(kb);   // (also for the columns of a wave that see all of it)
-    } else {
-      expand(kb + 2, st);
-    }
-    if (kb + 3 < kb1) fetch(kb + 3, st);
-    if (tid < 2) badp[(kb - kb0 + 3) % 4][tid] = 0;
-    __syncthreads();
+}
+// many columns behind the prefix; OWN: of the sequences themselves too
+constexpr int kWideLog2 = 20;   // workgroups side by side: past them the grid has rows (a dimension's threads are counted in 32 bits)
+template <int HD, int KIND, int T, bool OWN>
+__global__ __launch_bounds__(kManyWaves * 64) void k_kv_both_many(KvAttnArgs a, KvPreArgs p) {
+  static_assert(kManyWaves == kFewWaves, "one launch of both");
+  constexpr int LDS = OWN || 2 * many_lds<HD, KIND>() > few_lds<HD, KIND, T>() ? 2 * many_lds<HD, KIND>() : few_lds<HD, KIND, T>();
+  const uint32_t id = blockIdx.y << kWideLog2 | blockIdx.x, pre = (uint32_t)p.nkv * p.nchunk * p.nsplit, i = id - pre;
+  if (id < pre) {
+    const uint32_t cs = id / (uint32_t)p.nkv;
+    many_tokens<HD, KIND, T, true, LDS>(p, id - cs * p.nkv, cs, 0);
+  } else if constexpr (OWN) {
+    const uint32_t r = i / (uint32_t)a.nkv, per = (uint32_t)a.nchunk * a.nsplit, b = r / per;
+    if (b >= (uint32_t)a.nseq) return;
+    many_tokens<HD, KIND, T, false, LDS>(a, i - r * a.nkv, r - b * per, b);
+  } else {
+    const uint32_t r = i / (uint32_t)a.nsplit, per = (uint32_t)a.nkv * a.nchunk, b = r / per;
+    if (b >= (uint32_t)a.nseq) return;
+    few_tokens<HD, KIND, T, false, LDS>(a, i - r * a.nsplit, r - b * per, b);
   }
-  l = pair_sum32(l);
-  if constexpr (TWO && KIND != MK_Q4) {
-    // An infinite V: the lo halves (0, or of either sign) turn the sum into NaN.  Such sums are what the values say that are not finite and
-    // that the column sees, read again.  (Where l is NaN a score was, and the row is)
-    bool nan = false;
-#pragma unroll
-    for (int t = 0; t < OT; t++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) nan |= o[t][i] != o[t][i];
-    if (__any((int)live & (int)nan & (int)(l == l))) {
-#pragma unroll
-      for (int t = 0; t < OT; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[t][i] = o[t][i] != o[t][i] ? 0.f : o[t][i];
-#pragma unroll 1
-      for (int64_t i = (int64_t)kManyBlk * kb0; i < min((int64_t)kManyBlk * kb1, (int64_t)kRec * s.NR); i++) {
-        const int p = kRec * record(s, (int)(i / kRec)) + (int)(i % kRec);
-        const bool sp = sees(a, P, lo, p);
-        if (!__any(sp)) continue;   // (also the positions past ctx)
-#pragma unroll
-        for (int t = 0; t < OT; t++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) add_bad<HD, KIND>(nullptr, hd.v + (int64_t)p * a.crow, p, 32 * t + 8 * j + 4 * hf, sp, o[t], 4 * j);
-      }
-    }
-  }
-  if constexpr (T != RT_F32 && !PRE) {
-    if (s.S == 1 && !joined(a)) {
-      // A lane has 4 dims here and there of its column; by way of the wave's own part of LDS the rows leave in 16-byte pieces
-      // next to each other (4096 tokens with 32 heads: 105 -> 101 us)
-      constexpr int RS = HD + 8;
-      static_assert(kManyWaves * 32 * RS <= 3 * (kManyBlk * KST + VN), "the columns fit where the blocks were");
-      uint16_t *ow = blocks + wave * 32 * RS;
-      const float inv = 1.f / l;
-      const KvRows lds{ow + ln * RS, T, 0, 0, 0};
-#pragma unroll
-      for (int t = 0; t < OT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float r[4] = {o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv};
-          store_elems<T, 4>(lds, 32 * t + 8 * i + 4 * hf, r);
-        }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      constexpr int LR = HD / 8, RI = 64 / LR;   // lanes of a row, rows at a time
-#pragma unroll
-      for (int i = 0; i < 32 / RI; i++) {
-        const int c = RI * i + lane / LR, cc = cw + c, tk = token_of(a, cc);
-        if (tk < s.cnt && (int64_t)s.P0 + tk < a.ctx) {
-          const int64_t at = b * a.out.seq + (int64_t)tk * a.out.tok + (int64_t)(g * a.rep + cc - tk * a.rep) * a.out.head + 8 * (lane % LR);
-          *(u32x4_any *)((uint16_t *)a.out.p + at) = *(const u32x4 *)(ow + c * RS + 8 * (lane % LR));
-        }
-      }
-      return;
-    }
-  }
-  if (!PRE && s.S == 1 && !joined(a)) {
-    if (!live) return;
-    const float inv = 1.f / l;
-    const int64_t at = b * a.out.seq + (int64_t)tok * a.out.tok + (int64_t)head * a.out.head;
-#pragma unroll
-    for (int t = 0; t < OT; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float r[4] = {o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv};
-        store_elems<T, 4>(a.out, at + 32 * t + 8 * i + 4 * hf, r);
-      }
-    return;
-  }
-  // partial sums, by way of the wave's own part of LDS like the rows above, half the dims at a time: a column's next to each other instead of 16 bytes here and there
-  constexpr int HW = HD / 2, RS = HW + 4, LR = HW / 4, RI = 64 / LR;   // dims, floats of a column in LDS, lanes of one, columns at a time
-  static_assert(kManyWaves * 32 * RS * 2 <= 3 * (kManyBlk * KST + VN), "the columns fit where the blocks were");
-  float *ow = (float *)blocks + wave * 32 * RS;
-  const uint64_t lives = __ballot(live);
-  auto place = [&](int tok, int head) { return (((int64_t)b * a.n + tok) * a.heads + head) * slots_of(a) + (PRE ? slots_of(a) - a.nsplit : 0) + split; };
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int t = 0; t < OT / 2; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const f32x16 &x = o[OT / 2 * h + t];
-        *(f32x4 *)(ow + ln * RS + 32 * t + 8 * i + 4 * hf) = (f32x4){x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int i = 0; i < 32 / RI; i++) {
-      const int c = RI * i + lane / LR, cc = cw + c, tk = token_of(a, cc);
-      if (lives >> c & 1) *(f32x4 *)(a.part + place(tk, g * a.rep + cc - tk * a.rep) * HD + HW * h + 4 * (lane % LR)) = *(const f32x4 *)(ow + c * RS + 4 * (lane % LR));
-    }
-  }
-  if (live && hf == 0) *(float2 *)(a.part + (int64_t)a.nseq * a.n * a.heads * slots_of(a) * HD + 2 * place(tok, head)) = make_float2(m, l);
 }
 
 // ------------------------------------------------------------------ launches
@@ -1101,38 +724,57 @@ hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st) {
     else QPH_KV(k_few16, a.hd, a.q.type, grid, kFewWaves * 64, a);
   }
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.nsplit == 1 || joined(a)) return e;
+  if (e != hipSuccess || a.nsplit == 1) return e;
   if ((int64_t)a.nseq * a.n * a.heads >= kMergeRows) QPH_KV(k_kv_merge_rows, a.hd, a.q.type, dim3((a.n * a.heads + 1024 / a.hd - 1) / (1024 / a.hd), 1, a.nseq), 256, a);   // (at most 32768 rows a sequence: groups <= 256)
   else QPH_KV(k_kv_merge, a.hd, a.q.type, dim3(a.heads, a.n, a.nseq), 256, a);
   return hipGetLastError();
 }
 
 // ------------------------------------------------------------------ a common prefix
-// Three launches: the sequences' own positions as above, the prefix as if all sequences' tokens were one sequence's, and what joins their sums.
 // `a` is the own part's, planned; the prefix's plan goes by the columns of all sequences
+// Own tokens of few columns beside many behind the prefix: k_kv_few has two workgroups a CU in a launch of its own, one in that of both.  Up to the former's one round a launch of both
+// takes less time (410 workgroups 28.0 -> 21.4 us, 424 59.6 -> 51.2), past it more (992 49.5 -> 53.0, 2436 96 -> 107, 6832 138 -> 183)
+static int64_t few_blocks(const KvAttnArgs &a) { return (int64_t)a.nsplit * a.nkv * a.nchunk * a.nseq; }
+static bool few_apart(const KvAttnArgs &a) { return few_blocks(a) > 512; }
 size_t kv_prefix_plan(KvAttnArgs &a, KvPreArgs &p) {
   kv_attn_plan(a, true);
   kv_attn_plan(p, true);
   if (a.many && !p.many) { p.few = 0; kv_attn_plan(p, true); }   // one launch where both are of few tokens
   p.paired = 0;   // (every column sees all: nothing to even out)
+  if (p.many && !a.many && !few_apart(a)) a.nsplit = std::max(1, a.nsplit / 2);   // (one workgroup a CU beside the others: 32 sequences behind 8190 positions 38.4 us for 35.2)
   a.one_tiles = p.one_tiles = -(a.nsplit + p.nsplit);
-  return (size_t)a.nseq * a.n * a.heads * slots_of(a) * (a.hd + 2) * 4;
+  return (size_t)a.nseq * a.n * a.heads * slots_of<true>(a) * (a.hd + 2) * 4;
 }
-template <int HD, int T> static constexpr auto k_both4 = k_kv_few_both<HD, MK_Q4, T>;
-template <int HD, int T> static constexpr auto k_both16 = k_kv_few_both<HD, MK_F32, T>;
-template <int HD, int T> static constexpr auto k_pre_many4 = k_kv_many<HD, MK_Q4, T, true>;
-template <int HD, int T> static constexpr auto k_pre_many16 = k_kv_many<HD, MK_F32, T, true>;
+template <int HD, int T> static constexpr auto k_own4 = k_kv_few<HD, MK_Q4, T, false, true>;
+template <int HD, int T> static constexpr auto k_own16 = k_kv_few<HD, MK_F32, T, false, true>;
+template <int HD, int T> static constexpr auto k_few_few4 = k_kv_both_few<HD, MK_Q4, T>;
+template <int HD, int T> static constexpr auto k_few_few16 = k_kv_both_few<HD, MK_F32, T>;
+template <int HD, int T> static constexpr auto k_many_few4 = k_kv_both_many<HD, MK_Q4, T, false>;
+template <int HD, int T> static constexpr auto k_many_few16 = k_kv_both_many<HD, MK_F32, T, false>;
+template <int HD, int T> static constexpr auto k_many_many4 = k_kv_both_many<HD, MK_Q4, T, true>;
+template <int HD, int T> static constexpr auto k_many_many16 = k_kv_both_many<HD, MK_F32, T, true>;
 hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvPreArgs &p, hipStream_t st) {
   hipError_t e;
-  if (p.many) {
-    if ((e = launch_kv_attn(a, st)) != hipSuccess) return e;
-    const dim3 grid(p.nkv, p.nchunk * p.nsplit, 1);
-    if (p.kind == MK_Q4) QPH_KV(k_pre_many4, p.hd, p.q.type, grid, kManyWaves * 64, p);
-    else QPH_KV(k_pre_many16, p.hd, p.q.type, grid, kManyWaves * 64, p);
+  const bool q4 = p.kind == MK_Q4, apart = p.many && !a.many && few_apart(a);
+  const int64_t all = (int64_t)p.nsplit * p.nkv * p.nchunk + (apart ? 0 : few_blocks(a)), width = std::min(all, (int64_t)1 << kWideLog2);
+  KvAttnArgs own = a;
+  if (apart) {
+    own.nseq = 0;   // (none in the launch below)
+    const dim3 grid(a.nsplit, a.nkv * a.nchunk, a.nseq);
+    if (q4) QPH_KV(k_own4, a.hd, a.q.type, grid, kFewWaves * 64, a);
+    else QPH_KV(k_own16, a.hd, a.q.type, grid, kFewWaves * 64, a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  const dim3 both((unsigned)width, (unsigned)((all + width - 1) / width));
+  if (!p.many) {   // (at most 65535 workgroups of the prefix, whose chunks have 8 columns at least: 2^21 of all)
+    if (q4) QPH_KVN(k_few_few4, p.hd, p.q.type, dim3((unsigned)all), kFewWaves * 64, a, p);
+    else QPH_KVN(k_few_few16, p.hd, p.q.type, dim3((unsigned)all), kFewWaves * 64, a, p);
+  } else if (!a.many) {
+    if (q4) QPH_KVN(k_many_few4, p.hd, p.q.type, both, kManyWaves * 64, own, p);
+    else QPH_KVN(k_many_few16, p.hd, p.q.type, both, kManyWaves * 64, own, p);
   } else {
-    const int64_t blocks = (int64_t)p.nsplit * p.nkv * p.nchunk + (int64_t)a.nsplit * a.nkv * a.nchunk * a.nseq;
-    if (p.kind == MK_Q4) QPH_KVN(k_both4, p.hd, p.q.type, dim3((unsigned)blocks), kFewWaves * 64, a, p);
-    else QPH_KVN(k_both16, p.hd, p.q.type, dim3((unsigned)blocks), kFewWaves * 64, a, p);
+    if (q4) QPH_KVN(k_many_many4, p.hd, p.q.type, both, kManyWaves * 64, own, p);
+    else QPH_KVN(k_many_many16, p.hd, p.q.type, both, kManyWaves * 64, own, p);
   }
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const KvJoin j{p.prefix, p.tile_log2, p.min_log2, p.one_tiles, p.nsplit};

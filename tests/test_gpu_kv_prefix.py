@@ -228,3 +228,40 @@ def test_more_rows_than_a_grid_is_wide():
     out = c.attention(q, i32([0]), prefix=p)
     for t in (0, 4000, 8065, 8066, n - 1):
         check_rows(out[0, t:t + 1], q[0, t:t + 1], both(K0, K, L, 0)[:L + t + 1], both(V0, V, L, 0)[:L + t + 1], L + t)
+
+
+@pytest.mark.parametrize("kind", ["q4", "f16"])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+def test_many_sequences_of_one_token(kind, type):
+    """more workgroups of few own columns than the launch with the prefix's many columns takes"""
+    gen = torch.Generator().manual_seed(12)
+    S, G, rep, D, L = 200, 4, 2, 64, 333
+    pasts = [i % 37 for i in range(S)]
+    p, K0, V0 = filled(kind, 1, G, D, L, [L], gen)
+    c, K, V = filled(kind, S, G, D, 40, [a + 1 for a in pasts], gen)
+    q = torch.randn(S, 1, G * rep, D, generator=gen).to(TYPES[type]).cuda()
+    out = c.attention(q, i32(pasts), prefix=p)
+    for b in range(0, S, 7):
+        check_rows(out[b], q[b], both(K0, K, L, b), both(V0, V, L, b), L + pasts[b])
+
+
+def test_more_workgroups_than_a_grid_is_wide(monkeypatch):
+    monkeypatch.setenv("QPH_KV_FEW", "0")   # (of the kernel for many columns, whose workgroups are one for each sequence and kv head)
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    S, G, D, L, ctx = 65535, 17, 64, 50, 2
+    c, p = qa.KvCache("f16", S, G, D, ctx), qa.KvCache("f16", 1, G, D, L)
+    k, v = (torch.randn(S, ctx, G, D, generator=gen, device="cuda").half() for _ in range(2))
+    k0, v0 = (torch.randn(1, L, G, D, generator=gen, device="cuda").half() for _ in range(2))
+    c.write(k, v, torch.zeros(S, dtype=torch.int32, device="cuda"))
+    p.write(k0, v0, i32([0]))
+    some = [0, 1, 61679, 61680, 61681, 61682, 65534]   # (2^20 / 17 = 61680.9)
+    pos = torch.full((S,), -1, dtype=torch.int32, device="cuda")
+    pos[some] = i32([1, 0, 1, 1, 0, 1, 1])
+    q = torch.randn(S, 1, G, D, generator=gen, device="cuda").half()
+    out = torch.full_like(q, 55.)
+    c.attention(q, pos, prefix=p, out=out)
+    for b in some:
+        check_rows(out[b], q[b], torch.cat([k0[0], k[b]]).double().cpu(), torch.cat([v0[0], v[b]]).double().cpu(), L + int(pos[b]))
+    others = torch.ones(S, dtype=torch.bool, device="cuda")
+    others[some] = False
+    assert bool((out[others] == 55).all())
