@@ -23,6 +23,8 @@ CASES = [
     # many columns: 256 a workgroup, the last one ragged, tokens of several sequences in one
     ("f16", 128, 1, 4, 1, 900, [5] * 70, None), ("q4", 128, 2, 3, 1, 300, list(range(90)), None), ("f16", 64, 1, 5, 40, 130, [0, 300, 9], [40, 11, 25]), ("q4", 64, 1, 8, 66, 64, [513], None),
     ("f16", 128, 1, 2, 150, 1000, [0, 64], [150, 3]), ("q4", 128, 1, 7, 13, 63, [0] * 7, [13, 1, 2, 0, 13, 6, 7]),
+    # own columns in several chunks of k_kv_few for each of many sequences
+    ("q4", 64, 5, 2, 20, 200, list(range(40)), None), ("f16", 128, 3, 3, 17, 70, [11] * 64, [1 + i % 17 for i in range(64)]),
 ]
 
 
@@ -235,7 +237,7 @@ def test_more_rows_than_a_grid_is_wide():
 def test_many_sequences_of_one_token(kind, type):
     """more workgroups of few own columns than the launch with the prefix's many columns takes"""
     gen = torch.Generator().manual_seed(12)
-    S, G, rep, D, L = 200, 4, 2, 64, 333
+    S, G, rep, D, L = 270, 4, 2, 64, 333
     pasts = [i % 37 for i in range(S)]
     p, K0, V0 = filled(kind, 1, G, D, L, [L], gen)
     c, K, V = filled(kind, S, G, D, 40, [a + 1 for a in pasts], gen)
