@@ -169,30 +169,30 @@ __global__ __launch_bounds__(256) void k_copy16(KvCopyArgs a) {
   uint16_t *dst = STAGE == 1 ? (uint16_t *)a.work + staged : (uint16_t *)(blockIdx.y ? a.cache_v : a.cache) + b * a.cseq + ((int64_t)a.pos[b] + t) * a.crow + d;
   *(u32x4 *)dst = *(const u32x4 *)src;
 }
-// A workgroup has 32 records of one kv head, 256 positions, one a thread to look up.  Records that come from one whole record, as all but the last of a fork do, are
+// A workgroup has RECS records of one kv head, and a thread a position to look up.  Records that come from one whole record, as all but the last of a fork do, are
 // copied as they are, 16 bytes a thread.  Of others a wave has one: lanes 0 .. have 16 bytes of a position's K, lanes 32 .. four words of V, whose
-// 8 codes come from a word each of up to 8 records; V words that hold positions outside the call are merged.
-// 6001 positions of 8 heads of 128 dims forked into 8 sequences: 62 MB
-constexpr int kCopyRecs = 32;
-template <int HD, int STAGE>
+// 8 codes come from a word each of up to 8 records; V words that hold positions outside the call are merged.  Bound by HBM: 6001 positions of 8 heads of 128 dims
+// forked into 8 sequences, 62 MB, 12.3 us, 5.1 TB/s; where positions are picked, by the loads and shifts of up to 8 words a word: 4000 of 16384 of 16 sequences, 147 MB, 58.8 us
+template <int HD, int STAGE, int RECS>
 __global__ __launch_bounds__(256) void k_copy4(KvCopyArgs a) {
-  constexpr int P = 9 * HD / 16, NP = (kCopyRecs * P + 255) / 256;   // 16-byte pieces of a record, of a thread
-  __shared__ int place[kCopyRecs * kRec], whole[kCopyRecs];   // where positions come from; whole records' first, -1: of several, -2: none
+  constexpr int P = 9 * HD / 16, NP = (RECS * P + 255) / 256;   // 16-byte pieces of a record, of a thread
+  __shared__ int place[RECS * kRec], whole[RECS];   // where positions come from; whole records' first, -1: of several, -2: none
   const int b = blockIdx.z, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int P0 = a.pos[b];
   if (P0 < 0) return;
-  const int64_t rec = (STAGE == 1 ? 0 : P0 / kRec) + (int64_t)blockIdx.x * kCopyRecs;   // in scratch tokens lie from position 0 on
+  const int64_t rec = (STAGE == 1 ? 0 : P0 / kRec) + (int64_t)blockIdx.x * RECS;   // in scratch tokens lie from position 0 on
   const int64_t t0 = rec * kRec - (STAGE == 1 ? 0 : P0), wrec = (a.n + kRec - 1) / kRec;
   const int64_t head = (int64_t)b * a.nkv + g;
   uint8_t *dst = STAGE == 1 ? (uint8_t *)a.work + (head * wrec + rec) * (9 * HD) : (uint8_t *)a.cache + (head * a.nrec + rec) * (9 * HD);
   const uint8_t *src;
   {
     const int64_t t = t0 + tid;
-    const Place s = t >= 0 && t < a.n ? place_of(a, b, (int)t) : Place{0, -1};
+    const bool mine = tid < RECS * kRec;
+    const Place s = mine && t >= 0 && t < a.n ? place_of(a, b, (int)t) : Place{0, -1};
     const int p = s.p < 0 ? -1 : STAGE == 2 ? (int)t : s.p, p0 = __shfl(p, lane & ~7);
-    place[tid] = p;
+    if (mine) place[tid] = p;
     const uint32_t there = (uint32_t)(__ballot(p >= 0) >> (lane & ~7)) & 255, run = (uint32_t)(__ballot(p >= 0 && p == p0 + (lane & 7) && p0 % kRec == 0) >> (lane & ~7)) & 255;
-    if ((lane & 7) == 0) whole[tid / kRec] = run == 255 ? p0 : there ? -1 : -2;
+    if (mine && (lane & 7) == 0) whole[tid / kRec] = run == 255 ? p0 : there ? -1 : -2;
     const int seq = a.seqs ? a.seqs[b] : b;   // (outside the source: no position is there)
     src = STAGE == 2 ? (const uint8_t *)a.work + head * wrec * (9 * HD) : (const uint8_t *)a.src + ((int64_t)seq * a.nkv + g) * a.src_nrec * (9 * HD);
   }
@@ -201,15 +201,15 @@ __global__ __launch_bounds__(256) void k_copy4(KvCopyArgs a) {
 #pragma unroll
   for (int i = 0; i < NP; i++) {
     const int id = tid + 256 * i, r = id / P;
-    const int from = r < kCopyRecs ? whole[r] : -1;
+    const int from = r < RECS ? whole[r] : -1;
     if (from >= 0) piece[i] = *(const u32x4 *)(src + (int64_t)(from / kRec) * (9 * HD) + id % P * 16);
   }
 #pragma unroll
   for (int i = 0; i < NP; i++) {
     const int id = tid + 256 * i, r = id / P;
-    if (r < kCopyRecs && whole[r] >= 0) *(u32x4 *)(dst + id * 16) = piece[i];
+    if (r < RECS && whole[r] >= 0) *(u32x4 *)(dst + id * 16) = piece[i];
   }
-  for (int r = tid / 64; r < kCopyRecs; r += 4) {
+  for (int r = tid / 64; r < RECS; r += 4) {
     if (whole[r] != -1) continue;
     const int *at = place + kRec * r;
     uint8_t *o = dst + r * (9 * HD);
@@ -285,9 +285,17 @@ size_t kv_copy_bytes(int kind, int nseq, int nkv, int hd, int n) {
 template <int STAGE>
 static void launch_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
   if (kind == MK_Q4) {
-    const dim3 grid((unsigned)(((a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1) + kCopyRecs - 1) / kCopyRecs), a.nkv, a.nseq);
-    if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_copy4<64, STAGE>), grid, dim3(256), 0, st, a);
+    const int recs = (a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1);
+    // a record a wave up to eight such workgroups a CU, two past them: of 4 sequences' 1000 positions picked from 4000 (8 heads of 128 dims) 5.6 us with one, 6.6 with two; 250 positions forked
+    // into 32 6.0 and 5.7, 6001 into 8 14.0 and 12.3; 4000 picked for each of 16 57.4 and 58.7.  (Eight: 14.2, 7.6, 12.1, 71.6)
+    auto grid = [&](int each) { return dim3((unsigned)((recs + each - 1) / each), a.nkv, a.nseq); };
+    if ((int64_t)((recs + 7) / 8) * a.nkv * a.nseq <= 2048) {
+      if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE, 4>), grid(4), dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((k_copy4<64, STAGE, 4>), grid(4), dim3(256), 0, st, a);
+    } else {
+      if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE, 8>), grid(8), dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((k_copy4<64, STAGE, 8>), grid(8), dim3(256), 0, st, a);
+    }
   } else {
     hipLaunchKernelGGL((k_copy16<STAGE>), dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
   }

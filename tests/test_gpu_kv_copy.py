@@ -157,3 +157,21 @@ def test_refusals():
                 c.copy(index, pos, seqs=bad)
             with pytest.raises(qa.QphError, match="lens"):
                 c.copy(index, pos, lens=bad)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_records_of_many_sequences(D):
+    """more records than a wave each: in order, picked, shifted, and back by way of scratch"""
+    gen = torch.Generator().manual_seed(D + 1)
+    S, G, ctx, n = 90, 8, 270, 250   # 90 x 8 x 32 records
+    src, dst = cache("q4", S, G, D, ctx, gen), cache("q4", S, G, D, ctx, gen)
+    was, new = values(src), values(dst)
+    b = torch.arange(S)[:, None]
+    for index, pos in ((torch.arange(n).repeat(S, 1), b[:, 0] % 9), (torch.randint(0, ctx, (S, n), generator=gen), b[:, 0] % 5), (torch.arange(n).repeat(S, 1) + b % 3, b[:, 0] % 2 * 8)):
+        at = (pos[:, None] + torch.arange(n)).cuda()
+        new[:, b.cuda(), at] = was[:, b.cuda(), index.cuda()]
+        dst.copy(index.int().cuda(), pos.int().cuda(), source=src)
+        assert torch.equal(values(dst), new)
+    new[:, b.cuda(), torch.arange(n, device="cuda") + 7] = new[:, b.cuda(), torch.arange(n, device="cuda")]
+    dst.copy(torch.arange(n, dtype=torch.int32, device="cuda").expand(S, n), torch.full((S,), 7, dtype=torch.int32, device="cuda"))
+    assert torch.equal(values(dst), new)
