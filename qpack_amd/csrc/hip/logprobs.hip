@@ -364,14 +364,15 @@ template <int T>
 __global__ __launch_bounds__(256) void k_logprobs_merge(LogprobArgs a) {
   constexpr int kMost = kLpSplits * kLpTop, N = 8;   // (63 shares' 20 entries are 5 a thread; past 2048 entries they are loaded in their turn)
   __shared__ LpSum all;
-  __shared__ int64_t firsts[kLpSplits + kLpTop], bound, joint[kMost];
+  __shared__ int64_t firsts[kLpSplits + 2 * kLpTop], bound, joint[kMost];
   __shared__ int count;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, S = a.splits, K = a.top;
   const LpSum *sums = (const LpSum *)a.work + row * S;
   const int64_t *lists = (const int64_t *)((const LpSum *)a.work + a.rows * S) + row * S * K;
-  // the first d of each list are K at least; what the K-th of them precedes is not among the first K
-  const int d = K ? (K + S - 1) / S : 0, F = S * d;
+  // the first d of each list are K at least; what the K-th of them precedes is not among the first K.  (Of no more than K the last is some list's least, which many precede:
+  // 64 of 16 x 32000 39 us for 17)
+  const int d = K ? min((K + K / 2 + S - 1) / S, K) : 0, F = S * d;
   const int64_t mine = tid < F ? lists[tid / d * K + tid % d] : kNoKey;
   LpSum s = tid < S ? sums[tid] : LpSum{-INFINITY, 0.f, 0.f, 0};
   int64_t x[N];
@@ -410,11 +411,13 @@ __global__ __launch_bounds__(256) void k_logprobs_merge(LogprobArgs a) {
 }  // namespace
 
 size_t logprobs_plan(LogprobArgs &a) {
-  // A workgroup's pass over its share is a chain of loads: rows are shared out until there are four workgroups a CU, in
-  // pieces of a wave's load for each of its waves
+  // A workgroup's pass over its share is a chain of loads, of its waves' loads side by side (a unit) after one another: rows are shared out until there are four workgroups a CU.  Not
+  // rows of few units, since the shares' joining costs as much as some of them (a row of 2000 to 5000 fp32 logits 8.8 us in shares, 5.6 to 7.1 without; 256 rows of 16000
+  // 14.3 and 13.2, 64 of them 11.5 and 12.8), and not into shares of one unit where there are more than two a CU then (16 rows of 64000 12.4 us for 11.2)
   const int unit = kLpWaves * 64 * (a.type == RT_F32 ? 4 : 8);
   const int units = (a.vocab + unit - 1) / unit;
-  const int want = (int)std::min<int64_t>(std::max<int64_t>(1024 / a.rows, 1), std::min(units, kLpSplits));
+  const int least = a.rows * std::min(units, kLpSplits) > 512 ? 2 : 1;
+  const int want = units <= 6 + a.rows / 24 ? 1 : (int)std::min<int64_t>(std::max<int64_t>(1024 / a.rows, 1), std::min((units + least - 1) / least, kLpSplits));
   const int each = (units + want - 1) / want;
   a.share = (int)std::min<int64_t>((int64_t)each * unit, INT_MAX);
   a.splits = (units + each - 1) / each;
