@@ -286,16 +286,19 @@ template <int STAGE>
 static void launch_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
   if (kind == MK_Q4) {
     const int recs = (a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1);
-    // a record a wave up to eight such workgroups a CU, two past them: of 4 sequences' 1000 positions picked from 4000 (8 heads of 128 dims) 5.6 us with one, 6.6 with two; 250 positions forked
-    // into 32 6.0 and 5.7, 6001 into 8 14.0 and 12.3; 4000 picked for each of 16 57.4 and 58.7.  (Eight: 14.2, 7.6, 12.1, 71.6)
+    // A record a wave up to eight workgroups of two a wave a CU: of 4 sequences' 1000 positions picked from 4000 (8 heads of 128 dims) 5.6 us with one, 6.6 with two, 14.2 with eight; 250
+    // forked into 32 6.0, 5.7 and 7.6.  Past them two, 4000 picked for each of 16 57.4, 58.7 and 71.6, but eight where the call names source sequences: they are forked or change
+    // places, in whole records as a rule, 6001 positions into 8 14.0, 12.3 and 12.1 (15.3 and 12.2 with other memory read between the calls)
     auto grid = [&](int each) { return dim3((unsigned)((recs + each - 1) / each), a.nkv, a.nseq); };
-    if ((int64_t)((recs + 7) / 8) * a.nkv * a.nseq <= 2048) {
-      if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE, 4>), grid(4), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((k_copy4<64, STAGE, 4>), grid(4), dim3(256), 0, st, a);
-    } else {
-      if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE, 8>), grid(8), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((k_copy4<64, STAGE, 8>), grid(8), dim3(256), 0, st, a);
-    }
+#define QPH_COPY(RECS)                                                                                          \
+  do {                                                                                                          \
+    if (a.hd == 128) hipLaunchKernelGGL((k_copy4<128, STAGE, RECS>), grid(RECS), dim3(256), 0, st, a);          \
+    else hipLaunchKernelGGL((k_copy4<64, STAGE, RECS>), grid(RECS), dim3(256), 0, st, a);                       \
+  } while (0)
+    if ((int64_t)((recs + 7) / 8) * a.nkv * a.nseq <= 2048) QPH_COPY(4);
+    else if (!a.seqs) QPH_COPY(8);
+    else QPH_COPY(32);
+#undef QPH_COPY
   } else {
     hipLaunchKernelGGL((k_copy16<STAGE>), dim3((unsigned)(((int64_t)a.n * a.nkv * a.hd / 8 + 255) / 256), 2, a.nseq), dim3(256), 0, st, a);
   }

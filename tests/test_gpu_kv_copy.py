@@ -172,6 +172,10 @@ def test_records_of_many_sequences(D):
         new[:, b.cuda(), at] = was[:, b.cuda(), index.cuda()]
         dst.copy(index.int().cuda(), pos.int().cuda(), source=src)
         assert torch.equal(values(dst), new)
+        seqs = torch.randint(0, S, (S,), generator=gen)
+        new[:, b.cuda(), at] = was[:, seqs[:, None].cuda(), index.cuda()]
+        dst.copy(index.int().cuda(), pos.int().cuda(), seqs=seqs.int().cuda(), source=src)
+        assert torch.equal(values(dst), new)
     new[:, b.cuda(), torch.arange(n, device="cuda") + 7] = new[:, b.cuda(), torch.arange(n, device="cuda")]
     dst.copy(torch.arange(n, dtype=torch.int32, device="cuda").expand(S, n), torch.full((S,), 7, dtype=torch.int32, device="cuda"))
     assert torch.equal(values(dst), new)
