@@ -15,8 +15,10 @@ namespace {
 //   y = x w / sqrt(mean(x^2) + eps);  y[i], y[i + half] = y[i] c[i] - y[i + half] s[i], y[i + half] c[i] + y[i] s[i], i < half
 // All in fp32, rounded once: queries to their type, keys and values as the cache holds them.
 //
-// EL consecutive dims, from d0 on, of a row on HD / EL consecutive lanes.  The pair's other dims lie in another lane: they are loaded as well (from
-// L1), which keeps the lanes' order free; half is a multiple of EL, so they too follow each other
+// Rows that are stored as they are lie on HD / 8 lanes, 4 dims and those that they are turned with each (pairs_of); what a 4-bit cache takes has the dims of a lane consecutive, as its
+// scales and codes want them (turned).  Bound by a launch for a step (a token each of 64 sequences 3.5 us), by HBM for prompts: 4001 tokens of 28 and 2 x 4 heads of 128 dims into an
+// fp16 cache, 75 MB, 14.8 us, 5.05 TB/s (8 consecutive dims a lane and their partners loaded too, by twice the instructions 16.7); 2048 of 32 and 2 x 8 into 4 bits 14.9 us, of which some
+// 5 are the codes of 2056 records, bound by issue
 template <int HD, int EL>
 __device__ __forceinline__ float row_sum(float v) {   // over the HD / EL lanes of a row
   static_assert(HD / EL == 8 || HD / EL == 16 || HD / EL == 64, "lanes of a row");
@@ -38,15 +40,16 @@ __device__ __forceinline__ void load_some(const KvRows &r, int64_t at, float *x)
     }
   }
 }
-// `mine`: the lane's row takes part (all its lanes alike); others leave zeros
+// EL consecutive dims, from d0 on, of a row on HD / EL consecutive lanes.  The pair's other dims lie in another lane: they are loaded as well (from
+// L1), which keeps the lanes' order free; half is a multiple of EL, so they too follow each other
 template <int HD, int EL, int T>
-__device__ __forceinline__ void turned(const KvAppendArgs &a, const KvRows &r, int64_t row, const float *w, int64_t place, int d0, bool mine, float *y) {
+__device__ __forceinline__ void turned(const KvAppendArgs &a, const KvRows &r, int64_t row, const float *w, int64_t place, int d0, float *y) {
   float x[EL], o[EL], c[EL], s[EL];
-  const bool pair = mine && d0 < 2 * a.half, low = d0 < a.half;
+  const bool pair = d0 < 2 * a.half, low = d0 < a.half;
   const int d1 = low ? d0 + a.half : d0 - a.half, i0 = low ? d0 : d1;   // the other dims; the pair's number
 #pragma unroll
-  for (int i = 0; i < EL; i++) x[i] = o[i] = s[i] = 0.f, c[i] = 1.f;
-  if (mine) load_some<T, EL>(r, row + d0, x);
+  for (int i = 0; i < EL; i++) o[i] = s[i] = 0.f, c[i] = 1.f;
+  load_some<T, EL>(r, row + d0, x);
   if (pair) {
     load_some<T, EL>(r, row + d1, o);
 #pragma unroll
@@ -68,6 +71,60 @@ __device__ __forceinline__ void turned(const KvAppendArgs &a, const KvRows &r, i
 #pragma unroll
   for (int i = 0; i < EL; i++) y[i] = pair ? __builtin_fmaf(x[i], c[i], low ? -(o[i] * s[i]) : o[i] * s[i]) : x[i];
 }
+// Lane j of a row's HD / 8 has dims d .. d + 3 and e .. e + 3: a pair's, d + half = e, or 8 consecutive ones behind the pairs.  `mine`: the row takes part (all
+// its lanes alike)
+struct Pairs { int d, e; float x[4], y[4]; };
+template <int T>
+__device__ __forceinline__ void load_four(const KvRows &r, int64_t at, float *x) {
+  if constexpr (T == RT_F32) load_elems<T, 4>(r, at, x);
+  else {
+    const u32x2 v = *(const u32x2_any *)((const uint16_t *)r.p + at);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint16_t h = (uint16_t)(v[i / 2] >> 16 * (i & 1));
+      x[i] = T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h);
+    }
+  }
+}
+template <int HD, int T>
+__device__ __forceinline__ Pairs pairs_of(const KvAppendArgs &a, const KvRows &r, int64_t row, const float *w, int64_t place, int j, bool mine) {
+  Pairs p;
+  const bool pair = 4 * j < a.half;
+  p.d = pair ? 4 * j : 8 * j;   // (behind the pairs: 2 half + 8 (j - half / 4))
+  p.e = pair ? 4 * j + a.half : 8 * j + 4;
+  float c[4], s[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) p.x[i] = p.y[i] = s[i] = 0.f, c[i] = 1.f;
+  if (mine) {
+    load_four<T>(r, row + p.d, p.x);
+    load_four<T>(r, row + p.e, p.y);
+    if (pair) {
+      const KvRows ct{(void *)a.cos_t, RT_F32, 0, 0, 0}, st{(void *)a.sin_t, RT_F32, 0, 0, 0};
+      load_four<RT_F32>(ct, place * a.half + p.d, c);
+      load_four<RT_F32>(st, place * a.half + p.d, s);
+    }
+  }
+  if (w) {
+    float q = 0.f, u[4], v[4];
+    const KvRows wt{(void *)w, RT_F32, 0, 0, 0};
+    load_four<RT_F32>(wt, p.d, u);
+    load_four<RT_F32>(wt, p.e, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) q = __builtin_fmaf(p.y[i], p.y[i], __builtin_fmaf(p.x[i], p.x[i], q));
+    const float f = 1.f / sqrtf(row_sum<HD, 8>(q) * (1.f / HD) + a.eps);
+#pragma unroll
+    for (int i = 0; i < 4; i++) { p.x[i] = p.x[i] * f * u[i]; p.y[i] = p.y[i] * f * v[i]; }
+  }
+  if (pair) {   // (others are themselves, whatever they are: 0 x NaN and -0 + 0 would change them)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float x = p.x[i], y = p.y[i];
+      p.x[i] = __builtin_fmaf(x, c[i], -(y * s[i]));
+      p.y[i] = __builtin_fmaf(y, c[i], x * s[i]);
+    }
+  }
+  return p;
+}
 // a sequence's first position and place, and its tokens that take part
 struct Seq { int P0, at; int64_t cnt; };
 __device__ __forceinline__ Seq seq_of(const KvAppendArgs &a, int b) {
@@ -82,10 +139,11 @@ template <int HD, int T>
 __device__ __forceinline__ void query(const KvAppendArgs &a, const Seq &s, int b, int i, int lane) {
   const int t = i / a.heads, h = i - t * a.heads;
   const bool mine = t < s.cnt;
-  const int d0 = 8 * (lane % (HD / 8));
-  float y[8];
-  turned<HD, 8, T>(a, a.q, b * a.q.seq + (int64_t)t * a.q.tok + (int64_t)h * a.q.head, a.qw, (int64_t)s.at + t, d0, mine, y);
-  if (mine) store_elems<T, 8>(a.out, b * a.out.seq + (int64_t)t * a.out.tok + (int64_t)h * a.out.head + d0, y);
+  const Pairs p = pairs_of<HD, T>(a, a.q, b * a.q.seq + (int64_t)t * a.q.tok + (int64_t)h * a.q.head, a.qw, (int64_t)s.at + t, lane % (HD / 8), mine);
+  if (!mine) return;
+  const int64_t o = b * a.out.seq + (int64_t)t * a.out.tok + (int64_t)h * a.out.head;
+  store_elems<T, 4>(a.out, o + p.d, p.x);
+  store_elems<T, 4>(a.out, o + p.e, p.y);
 }
 
 // an fp16 cache: the rows of a token - queries, keys, values - one after the other, 8 dims a thread
@@ -100,14 +158,19 @@ __global__ __launch_bounds__(256) void k_append16(KvAppendArgs a) {
     return;
   }
   const bool v = h >= a.heads + a.io.nkv;
-  const int g = h - a.heads - (v ? a.io.nkv : 0), d0 = 8 * (lane % (HD / 8));
-  float y[8];
-  if (v) load_elems<T, 8>(a.io.v, b * a.io.v.seq + (int64_t)t * a.io.v.tok + (int64_t)g * a.io.v.head + d0, y);
-  else turned<HD, 8, T>(a, a.io.k, b * a.io.k.seq + (int64_t)t * a.io.k.tok + (int64_t)g * a.io.k.head, a.kw, (int64_t)s.at + t, d0, true, y);
-  u32x4 w;
-#pragma unroll
-  for (int j = 0; j < 4; j++) w[j] = float_to_half_bits(y[2 * j]) | (uint32_t)float_to_half_bits(y[2 * j + 1]) << 16;
-  *(u32x4 *)((uint16_t *)(v ? a.io.cache_v : a.io.cache) + b * a.io.cseq + ((int64_t)s.P0 + t) * a.io.crow + g * HD + d0) = w;
+  const int g = h - a.heads - (v ? a.io.nkv : 0);
+  uint16_t *o = (uint16_t *)(v ? a.io.cache_v : a.io.cache) + b * a.io.cseq + ((int64_t)s.P0 + t) * a.io.crow + g * HD;
+  auto halves = [](float x, float y) { return float_to_half_bits(x) | (uint32_t)float_to_half_bits(y) << 16; };
+  if (v) {
+    const int d0 = 8 * (lane % (HD / 8));
+    float y[8];
+    load_elems<T, 8>(a.io.v, b * a.io.v.seq + (int64_t)t * a.io.v.tok + (int64_t)g * a.io.v.head + d0, y);
+    *(u32x4 *)(o + d0) = (u32x4){halves(y[0], y[1]), halves(y[2], y[3]), halves(y[4], y[5]), halves(y[6], y[7])};
+  } else {
+    const Pairs p = pairs_of<HD, T>(a, a.io.k, b * a.io.k.seq + (int64_t)t * a.io.k.tok + (int64_t)g * a.io.k.head, a.kw, (int64_t)s.at + t, lane % (HD / 8), true);
+    *(u32x2 *)(o + p.d) = (u32x2){halves(p.x[0], p.x[1]), halves(p.x[2], p.x[3])};
+    *(u32x2 *)(o + p.e) = (u32x2){halves(p.y[0], p.y[1]), halves(p.y[2], p.y[3])};
+  }
 }
 
 // a 4-bit cache: the first workgroups have a record each (ONE: one token a sequence, a position), waves K and V as k_kv4_write's and k_kv4_write1's; the
@@ -133,7 +196,7 @@ __global__ __launch_bounds__(128) void k_append4(KvAppendArgs a, int records) {
     const int64_t row = b * r.seq + g * r.head;
     float x[EL];
     if (vside) { load_some<T, EL>(r, row + EL * lane, x); store_one<HD, T>(o, s.P0 % kRec, x, true, lane); }
-    else { turned<HD, EL, T>(a, r, row, a.kw, s.at, EL * lane, true, x); store_one<HD, RT_F32>(o, s.P0 % kRec, x, false, lane); }
+    else { turned<HD, EL, T>(a, r, row, a.kw, s.at, EL * lane, x); store_one<HD, RT_F32>(o, s.P0 % kRec, x, false, lane); }
   } else {
     constexpr int EL = HD / 8;
     const int row = lane >> 3, part = lane & 7;
@@ -141,7 +204,7 @@ __global__ __launch_bounds__(128) void k_append4(KvAppendArgs a, int records) {
     const bool mine = p >= s.P0 && p < last;
     auto record = [&]() { return o; };
     if (vside) store_record<HD, T>([&](float *x) { load_elems<T, EL>(r, at + EL * part, x); }, record, mine, true, row, part, rec * kRec, s.P0, last, codes);
-    else store_record<HD, RT_F32>([&](float *x) { turned<HD, EL, T>(a, r, at, a.kw, s.at + t, EL * part, true, x); }, record, mine, false, row, part, rec * kRec, s.P0, last, codes);
+    else store_record<HD, RT_F32>([&](float *x) { turned<HD, EL, T>(a, r, at, a.kw, s.at + t, EL * part, x); }, record, mine, false, row, part, rec * kRec, s.P0, last, codes);
   }
 }
 
@@ -279,9 +342,6 @@ hipError_t launch_kv_append(int kind, const KvAppendArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
-size_t kv_copy_bytes(int kind, int nseq, int nkv, int hd, int n) {
-  return kind == MK_Q4 ? (size_t)kv4_bytes(nseq, nkv, hd, n) : (size_t)4 * nseq * n * nkv * hd;
-}
 template <int STAGE>
 static void launch_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
   if (kind == MK_Q4) {

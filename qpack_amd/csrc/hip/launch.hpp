@@ -377,7 +377,6 @@ struct KvCopyArgs {
   int64_t index_seq;
   void *work;
 };
-size_t kv_copy_bytes(int kind, int nseq, int nkv, int hd, int n);   // of work
 hipError_t launch_kv_copy(int kind, const KvCopyArgs &a, hipStream_t st);
 
 // ---- logprobs.hip: of rows of logits the given tokens' log probabilities, ranks, the entropies and the first `top` alternatives; outputs may be null
