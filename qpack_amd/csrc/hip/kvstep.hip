@@ -348,7 +348,7 @@ static void launch_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
     const int recs = (a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1);
     // A record a wave up to eight workgroups of two a wave a CU: of 4 sequences' 1000 positions picked from 4000 (8 heads of 128 dims) 5.6 us with one, 6.6 with two, 14.2 with eight; 250
     // forked into 32 6.0, 5.7 and 7.6.  Past them two, 4000 picked for each of 16 57.4, 58.7 and 71.6, but eight where the call names source sequences: they are forked or change
-    // places, in whole records as a rule, 6001 positions into 8 14.0, 12.3 and 12.1 (15.3 and 12.2 with other memory read between the calls)
+    // places, in whole records as a rule, 6001 positions into 8 14.0, 12.3 and 12.1 (62.8 and 60.8 with the caches read back each time)
     auto grid = [&](int each) { return dim3((unsigned)((recs + each - 1) / each), a.nkv, a.nseq); };
 #define QPH_COPY(RECS)                                                                                          \
   do {                                                                                                          \
