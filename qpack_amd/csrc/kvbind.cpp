@@ -292,9 +292,21 @@ PyObject *logprobs(PyObject *, PyObject *const *arg, Py_ssize_t na) try {
   if (tok && (!tok->is_cuda() || tok->get_device() != device)) { fail("logprobs: tokens are not on the logits' device%s%s", ""); return nullptr; }
   int64_t bytes = 0;
   if (qph_logprobs_work(type, rows, (int)x->size(1), top, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
-  const auto f32 = at::TensorOptions().device(x->device()).dtype(at::kFloat), i32 = f32.dtype(at::kInt);
-  at::Tensor logp, rank, work, entropy = at::empty({rows}, f32), ti = at::empty({rows, top}, i32), tl = at::empty({rows, top}, f32);
-  if (tok) { logp = at::empty({rows}, f32); rank = at::empty({rows}, i32); }
+  // the results side by side in one allocation, each from a multiple of 64 bytes on (an allocation each takes as long as the rest of the call)
+  const auto f32 = at::TensorOptions().device(x->device()).dtype(at::kFloat);
+  const int64_t one = (rows + 15) / 16 * 16, list = (rows * top + 15) / 16 * 16;
+  const at::Tensor all = at::empty({(tok ? 3 : 1) * one + 2 * list}, f32);
+  int64_t used = 0;
+  auto part = [&](at::ScalarType t, at::IntArrayRef sizes, int64_t room) {
+    at::Tensor y = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(t));
+    y.unsafeGetTensorImpl()->set_storage_offset(used);
+    y.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    used += room;
+    return y;
+  };
+  at::Tensor logp, rank, work, entropy = part(at::kFloat, {rows}, one);
+  if (tok) { logp = part(at::kFloat, {rows}, one); rank = part(at::kInt, {rows}, one); }
+  at::Tensor ti = part(at::kInt, {rows, top}, list), tl = part(at::kFloat, {rows, top}, list);
   if (bytes) work = at::empty({(bytes + 3) / 4}, f32);
   auto at = [](at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
   if (!launch(device, [&](void *st) {

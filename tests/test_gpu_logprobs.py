@@ -222,3 +222,23 @@ def test_the_most_rows():
     # differences of whole numbers are exact; the sum 1 + e^-d is off by 2^-24 (2 d e^-d + 6) or less, its logarithm by another 2^-23, the result's rounding is 2^-24 of it
     want = -torch.nn.functional.softplus(torch.where(torch.arange(R, device="cuda") % 2 == 0, d, -d).double())
     assert bool(((r.logp - want).abs() <= 2.0 ** -20 * (1 + want.abs())).all())
+
+
+def test_results_are_tensors_of_their_own():
+    x, tokens = torch.randn(5, 900, device="cuda"), torch.arange(5, dtype=torch.int32, device="cuda")
+    r, again = qa.logprobs(x, tokens, 3), qa.logprobs(x, tokens, 3)
+    with torch.inference_mode():
+        inside = qa.logprobs(x, tokens, 3)
+    for i, y in enumerate(r):   # one changed, the others stay
+        assert torch.equal(y, inside[i])
+        assert y.is_contiguous() and y.device == x.device and not y.requires_grad and y.data_ptr() % 64 == 0
+        y.fill_(7)
+        for j in range(i + 1, 5):
+            assert torch.equal(r[j], again[j])
+    w = torch.ones(5, device="cuda", requires_grad=True)
+    (again.logp * w).sum().backward()   # (as constants of a graph)
+    assert torch.equal(w.grad, again.logp)
+    none = qa.logprobs(x[:0], tokens[:0], 3)
+    assert none.logp.shape == (0,) and none.top_index.shape == (0, 3)
+    only = qa.logprobs(x)
+    assert only.logp is None and only.rank is None and only.top_index.shape == (5, 0) and torch.equal(only.entropy, inside.entropy)
