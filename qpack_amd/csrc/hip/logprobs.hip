@@ -8,7 +8,7 @@
 //
 // The alternatives: a wave keeps in LDS what of its logits may be among the K <= 64 first, and a bound that K of them reach.  Indices rise, so that only a
 // logit above the bound can get past those that are there; all lanes that have one leave it by a ballot and a count of the lanes before them.  The first
-// bound is what K of the lanes' maxima of a load reach; past some 32 entries more than needed it is raised, by bisection over the values' order with a ballot and
+// bound is what K of the lanes' maxima of two loads reach; past some 32 entries more than needed it is raised, by bisection over the values' order with a ballot and
 // a count for each entry of a lane.  Where too many are equal, the lower indices stay.  (Kept in order in registers and inserted one by one, a chain of some
 // hundred dependent instructions each, 20 alternatives of one row took 24 us, and of 1024 rows in bf16 129.  The first bound from all values of the load, 8 ballots and
 // counts a step: 64 rows of 151936 14.1 us for 13.0)
@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "kvrec.hpp"
 #include "launch.hpp"
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
   int64_t *buf = entries[TOP ? wave : 0];
   int held = 0, bound = kNone;   // entries, what the K-th of them reaches
   float last = 0.f;              // that, as a value
-  bool first = true;
+  bool first = true, soft = false;   // soft: the next load holds some that reach the bound
   // what a cut leaves, and from how many entries on there is one: a bound near the K-th lets few logits pass, a cut costs as much as some of them
   const int most = a.top + a.top / 4 + 2, full = min(most + 32, kLpKeep);
   if (threadIdx.x == 0) count = 0;
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
   const int token = a.tokens ? __builtin_amdgcn_readfirstlane(*(const scalar_int *)(uintptr_t)(a.tokens + row)) : -1;
   const bool has = token >= 0 && token < a.vocab;
   const float xt = has ? lp_scalar<T>(x0, token) : INFINITY;
-  auto take = [&](u32x4 w, int base) {   // a wave's elements base ..
+  auto take = [&](u32x4 w, int base, auto may_be_first, u32x4 next) {   // a wave's elements base ..; next: those STEP further on, of the first
     const int from0 = base + VE * lane, at = start(from0);
     float x[VE], bm = -INFINITY;
 #pragma unroll
@@ -263,15 +264,24 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
       for (int i = 0; i < VE; i++) s.ahead += __popcll(__ballot((x[i] > xt) | ((x[i] == xt) & (at + i < token) & (int)(counts >> i & 1))));
     }
     if constexpr (TOP) {
-      if (first) {
-        // K of the maxima of the lanes' halves reach the first bound, and few of the others: 20 of 128 maxima of 4 each some 22 of the 512
+      if (decltype(may_be_first)::value && first) {
+        // K of 128 maxima reach the first bound, and few of the other logits: the lanes' of this load and the next one, or of the halves of a last load; 20 of 128 maxima of 8 some 22 of
+        // 1024.  (Of the halves always: 5 of 64 x 151936 17.7 us for 17.0, 64 of them 27.6 for 26.0)
         first = false;
         float h[2] = {x[0], x[VE / 2]};
+        if (base + STEP + GE <= to) {
+          h[0] = bm;
+          h[1] = lp_elem<T>(next, 0);
 #pragma unroll
-        for (int i = 1; i < VE / 2; i++) { h[0] = fmaxf(h[0], x[i]); h[1] = fmaxf(h[1], x[VE / 2 + i]); }
+          for (int i = 1; i < VE; i++) h[1] = fmaxf(h[1], lp_elem<T>(next, i));
+          soft = true;
+        } else {
+#pragma unroll
+          for (int i = 1; i < VE / 2; i++) { h[0] = fmaxf(h[0], x[i]); h[1] = fmaxf(h[1], x[VE / 2 + i]); }
+        }
         const int o[2] = {order_of(fmaxf(h[0], -INFINITY)), order_of(fmaxf(h[1], -INFINITY))};   // (of NaN alone)
         int n = 128;
-        bound = raised<2>(o, order_of(-wave_max(-fminf(value_of(o[0]), value_of(o[1])))), order_of(wave_max(bm)), a.top, most, n);
+        bound = raised<2>(o, order_of(-wave_max(-fminf(value_of(o[0]), value_of(o[1])))), order_of(wave_max(fmaxf(value_of(o[0]), value_of(o[1])))), a.top, most, n);
         if (bound == order_of(-INFINITY)) {   // what a mask leaves, or a load with few elements: these too, but NaN, which no bound holds back
 #pragma unroll
           for (int i = 0; i < VE; i++) {
@@ -293,20 +303,22 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
         }
       }
       wave_sync();
-      last = value_of(bound);
+      if (decltype(may_be_first)::value && soft) soft = false;   // (the next load's that are at the bound have to pass too)
+      else last = value_of(bound);
       if (held > full) {
         bound = held > kLpKeep ? cut<CAP / 64>(buf, held, bound, a.top, most, lane) : cut<kLpKeep / 64>(buf, held, bound, a.top, most, lane);
         last = value_of(bound);
       }
     }
   };
+  static_assert(U == 2, "the loop below");
   for (int k = 0; k < steps; k += U) {
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const u32x4 now = w[u];
-      w[u] = load(base + (k + u + U) * STEP + VE * lane);
-      if (k + u < steps) take(now, base + (k + u) * STEP);
-    }
+    const u32x4 x0 = w[0];
+    w[0] = load(base + (k + U) * STEP + VE * lane);
+    take(x0, base + k * STEP, std::true_type(), w[1]);
+    const u32x4 x1 = w[1];
+    w[1] = load(base + (k + U + 1) * STEP + VE * lane);
+    if (k + 1 < steps) take(x1, base + (k + 1) * STEP, std::false_type(), x1);
   }
   // lanes share the reference; then the waves
   s.s = wave_sum(s.s); s.t = wave_sum(s.t);

@@ -242,3 +242,25 @@ def test_results_are_tensors_of_their_own():
     assert none.logp.shape == (0,) and none.top_index.shape == (0, 3)
     only = qa.logprobs(x)
     assert only.logp is None and only.rank is None and only.top_index.shape == (5, 0) and torch.equal(only.entropy, inside.entropy)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("top", [1, 5, 64])
+def test_what_reaches_the_first_bound_lies_in_the_second_load(type, top):
+    # a wave's loads are 256 or 512 logits, 1024 or 2048 apart
+    V = 24000
+    gen = torch.Generator().manual_seed(top)
+    x = torch.randn(6, V, generator=gen)
+    i = torch.arange(V)
+    x[0] = torch.where(i % 4096 >= 1024, x[0], -math.inf)
+    x[1] = torch.where((i >= 1024) & (i < 1024 + top // 2 + 1), x[1], -math.inf)
+    x[2] = torch.where(i >= 2048, x[2] + 9, x[2] - 9)
+    x[3] = torch.where(i % 2048 < 1024, 3., 2.)
+    x[4] = 3.
+    x[5] = torch.where((i >= 2048) & (i < 4096), 5., x[5].clamp(max=4))
+    x = x.to(TYPES[type])
+    tokens = torch.tensor([1024, 0, 3000, 23999, 17, 2048])
+    r = qa.logprobs(x.repeat(100, 1).cuda(), tokens.repeat(100).int().cuda(), top)   # (whole rows and shares of them)
+    few = qa.logprobs(x.cuda(), tokens.int().cuda(), top)
+    for y in (qa.LogProbs(*(z[:6] for z in r)), qa.LogProbs(*(z[594:] for z in r)), few):
+        check(y, x, tokens, top)
