@@ -732,6 +732,7 @@ hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t st) {
 
 // ------------------------------------------------------------------ a common prefix
 // `a` is the own part's, planned; the prefix's plan goes by the columns of all sequences
+// The prefix's columns are few up to one round of k_kv_few's workgroups (480 of them and 504 own ones 16.1 us, 17.7 by k_kv_many; 632 and 672 19.2 and 14.7, 872 and 888 33.8 and 26.0).
 // Own tokens of few columns beside many behind the prefix.  k_kv_few has two workgroups a CU in a launch of its own, one in that of both, which it starts with the prefix's.  From
 // several rounds on either way is slow: where a sequence's columns are several of k_kv_few's chunks, k_kv_many takes them past 512 workgroups (1014 of them 54 us for 36, 2584 43 for 20,
 // 10848 229 for 103; 444 18.0 for 20.0, 475 22.7 for 26.0).  A single chunk would leave it 16 columns of 256: those have a launch of their own
@@ -741,7 +742,7 @@ static bool few_apart(const KvAttnArgs &a) { return few_blocks(a) > 1024; }
 size_t kv_prefix_plan(KvAttnArgs &a, KvPreArgs &p) {
   kv_attn_plan(a, true);
   kv_attn_plan(p, true);
-  if (a.many && !p.many) { p.few = 0; kv_attn_plan(p, true); }   // one launch where both are of few tokens
+  if (!p.many && (a.many || few_blocks(p) > 512)) { p.few = 0; kv_attn_plan(p, true); }   // (few columns of either: one launch of k_kv_few's workgroups, two a CU)
   if (p.many && !a.many && a.nchunk > 1 && few_blocks(a) > 512) { a.few = 0; kv_attn_plan(a, true); }
   p.paired = 0;   // (every column sees all: nothing to even out)
   if (p.many && !a.many && !few_apart(a)) a.nsplit = std::max(1, a.nsplit / 2);   // (one workgroup a CU beside the others: 32 sequences behind 8190 positions 38.4 us for 35.2)
