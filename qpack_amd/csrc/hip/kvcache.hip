@@ -412,6 +412,7 @@ template <int HD, int KIND, int T, bool PRE, int LDS, bool JOIN = true>
 __device__ __forceinline__ void few_tokens(Args<PRE> a, int split, int gc, int b) {
   auto &sm = lds<uint8_t[LDS]>();
   auto &wm = lds<few_cols<T>, 0>(), &wl = lds<few_cols<T>, 1>();
+  if constexpr (PRE) a.window = a.sinks = a.paired = 0;
 #include "kv_few.inc"
 }
 
@@ -586,6 +587,7 @@ template <int HD, int KIND, int T, bool PRE, int LDS, bool JOIN = true>
 __device__ __forceinline__ void many_tokens(Args<PRE> a, int g, int cs, int b) {
   uint16_t *blocks = (uint16_t *)lds<uint8_t[LDS]>();
   auto &badp = lds<many_bad>();
+  if constexpr (PRE) a.window = a.sinks = a.paired = 0;
 #include "kv_many.inc"
 }
 
