@@ -1,10 +1,11 @@
 // The Python side of the kv entry points and of qph_logprobs (qpack_amd._kvbind, used by qpack_amd/kvcache.py and tokenprobs.py): checks tensors and calls the C ABI.  A step's
 // kernels take 3 to 8 us each; the checks through ctypes took 10 us a call (15 with scratch), through the tensors' Python attributes
-// 4.5 (8.5 with scratch and a second launch), from torch's own structures 3.5 (7.7); each launch is about 3 of it.
+// 4.5 (8.5 with scratch and a second launch), from torch's own structures 3.3 (6.5, 7.8 with scratch by way of a Python call); each launch is about 3 of it.
 // torch is loaded before this module is.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -15,7 +16,6 @@
 
 namespace {
 PyObject *g_error, *g_stream, *g_device, *g_guard;   // QphError, functions
-PyObject *s_new_empty;
 
 struct Ref {   // owned reference
   PyObject *p;
@@ -29,8 +29,8 @@ struct Ref {   // owned reference
 struct Cache {
   PyObject_HEAD
   qph_kv c;
-  int64_t device, item;
-  PyObject *data, *data_v;   // tensors of the cache's memory (4-bit: the one of them), item bytes an element: scratch is a new one like data
+  int64_t device;
+  PyObject *data, *data_v;   // tensors of the cache's memory (4-bit: the one of them)
 };
 
 bool fail(const char *fmt, const char *a, const char *b = "") {
@@ -154,15 +154,13 @@ PyObject *io(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   Py_RETURN_NONE;
 }
 // scratch of this call alone: the allocator gives it to the stream's later work, or to the graph that is being captured
-bool scratch(const Cache *c, int64_t bytes, PyObject **work, void **p) {
-  *work = nullptr; *p = nullptr;
+bool scratch(const Cache *c, int64_t bytes, at::Tensor *work, void **p) try {
+  *p = nullptr;
   if (!bytes) return true;
-  Ref size(PyLong_FromLongLong((bytes + c->item - 1) / c->item));
-  *work = PyObject_CallMethodOneArg(c->data, s_new_empty, size);
-  if (!*work) return false;
-  *p = THPVariable_Unpack(*work).data_ptr();
+  *work = at::empty({bytes}, at::TensorOptions().device(THPVariable_Unpack(c->data).device()).dtype(at::kByte));
+  *p = work->data_ptr();
   return true;
-}
+} catch (...) { torch::translate_exception_to_python(std::current_exception()); return false; }
 bool scale_of(PyObject *x, float *scale) {
   const double y = PyFloat_AsDouble(x);
   if (PyErr_Occurred()) return false;
@@ -185,10 +183,9 @@ PyObject *attention(PyObject *self, PyObject *const *arg, Py_ssize_t na) {
   float scale;
   if (!nargs(na, 7) || !attend_rows(c, arg, &q, &o, &n, &h, &pos, &lens) || !integer(arg[4], "window", &window) || !integer(arg[5], "sinks", &sinks) || !scale_of(arg[6], &scale)) return nullptr;
   if (qph_kv_attention_work(&c->c, q.type, (int)h, (int)n, window, sinks, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
-  PyObject *keep;
+  at::Tensor work;
   void *w;
-  if (!scratch(c, bytes, &keep, &w)) return nullptr;
-  Ref work(keep);
+  if (!scratch(c, bytes, &work, &w)) return nullptr;
   if (!launch(c->device, [&](void *st) { return qph_kv_attention(&c->c, &q, &o, (int)h, (int)n, pos, lens, window, sinks, scale, w, bytes, st); })) return nullptr;
   written(THPVariable_Unpack(arg[1]));
   Py_RETURN_NONE;
@@ -208,10 +205,9 @@ PyObject *attention_prefix(PyObject *self, PyObject *const *arg, Py_ssize_t na) 
   float scale;
   if (!nargs(na, 7) || !attend_rows(c, arg, &q, &o, &n, &h, &pos, &lens) || !scale_of(arg[4], &scale) || !cache_of(c, arg[5], "prefix", &p) || !index(c, arg[6], "prefix_len", &plen, true, 1)) return nullptr;
   if (qph_kv_attention_prefix_work(&c->c, &p->c, q.type, (int)h, (int)n, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
-  PyObject *keep;
+  at::Tensor work;
   void *w;
-  if (!scratch(c, bytes, &keep, &w)) return nullptr;
-  Ref work(keep);
+  if (!scratch(c, bytes, &work, &w)) return nullptr;
   if (!launch(c->device, [&](void *st) { return qph_kv_attention_prefix(&c->c, &p->c, plen, &q, &o, (int)h, (int)n, pos, lens, scale, w, bytes, st); })) return nullptr;
   written(THPVariable_Unpack(arg[1]));
   Py_RETURN_NONE;
@@ -261,10 +257,9 @@ PyObject *copy(PyObject *self, PyObject *const *arg, Py_ssize_t na) try {
   if (n > INT32_MAX) { fail("kv: too many tokens%s%s", ""); return nullptr; }
   const int *at = n ? (const int *)x->data_ptr() : (const int *)16;
   if (qph_kv_copy_work(&c->c, &src->c, (int)n, apart, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
-  PyObject *keep;
+  at::Tensor work;
   void *w;
-  if (!scratch(c, bytes, &keep, &w)) return nullptr;
-  Ref work(keep);
+  if (!scratch(c, bytes, &work, &w)) return nullptr;
   if (!launch(c->device, [&](void *st) { return qph_kv_copy(&c->c, &src->c, at, x->stride(0), (int)n, pos, lens, seqs, apart, w, bytes, st); })) return nullptr;
   for (PyObject *y : {c->data, c->data_v})
     if (y) written(THPVariable_Unpack(y));
@@ -323,7 +318,7 @@ PyObject *logprobs(PyObject *, PyObject *const *arg, Py_ssize_t na) try {
     PyTuple_SET_ITEM(out, i++, y);
   }
   return out;
-} catch (const std::exception &e) { if (!PyErr_Occurred()) fail("logprobs: %s%s", e.what()); return nullptr; }
+} catch (...) { if (!PyErr_Occurred()) torch::translate_exception_to_python(std::current_exception()); return nullptr; }
 
 int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_heads, head_dim, ctx, k, v, seq, row, device, data[, the fp16 V's])
   Cache *c = (Cache *)self;
@@ -335,7 +330,7 @@ int init(PyObject *self, PyObject *args, PyObject *) {   // (kind, nseq, kv_head
   Py_XINCREF(data_v);
   Py_XDECREF(c->data);
   Py_XDECREF(c->data_v);
-  c->data = data; c->data_v = data_v; c->item = c->c.kind == QPH_Q4 ? 1 : 2;
+  c->data = data; c->data_v = data_v;
   c->c.ctx = ctx; c->c.k = (void *)k; c->c.v = (void *)v; c->c.seq = seq; c->c.row = row; c->device = device;
   return 0;
 }
@@ -366,7 +361,6 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvbind", nullptr, -1, module_meth
 }  // namespace
 
 PyMODINIT_FUNC PyInit__kvbind(void) {
-  s_new_empty = PyUnicode_InternFromString("new_empty");
   cache_type.tp_name = "qpack_amd._kvbind.Cache";
   cache_type.tp_basicsize = sizeof(Cache);
   cache_type.tp_flags = Py_TPFLAGS_DEFAULT;
