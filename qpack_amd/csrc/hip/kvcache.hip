@@ -286,7 +286,8 @@ __device__ __forceinline__ Head head_of(const KvAttnArgs &a, int b, int g) {
   return h;
 }
 // records and positions past the span's are the last one's (masked, and in the allocation)
-__device__ __forceinline__ int64_t row_of(const KvAttnArgs &a, const Span &s, int v, int j) {
+template <typename A>   // (A: ctx, crow)
+__device__ __forceinline__ int64_t row_of(const A &a, const Span &s, int v, int j) {
   return min((int64_t)kRec * record(s, min(v, s.NR - 1)) + j, a.ctx - 1) * a.crow;
 }
 // whether records v .. v + n - 1 are there and follow each other
@@ -296,8 +297,8 @@ template <int HD>
 __device__ __forceinline__ const uint8_t *tile_base(const Head &h, const Span &s, int tile, bool run, int r) {   // r: the lane's record of the tile
   return h.rec + (run ? (int64_t)record(s, 4 * tile) : (int64_t)record(s, min(4 * tile + r, s.NR - 1)) - r) * (9 * HD);
 }
-template <int HD, int KIND>
-__device__ __forceinline__ void load_k(const KvAttnArgs &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t) {
+template <int HD, int KIND, typename A>
+__device__ __forceinline__ void load_k(const A &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t) {
   const int lr = lane & 15, lg = lane >> 4;
   if constexpr (KIND == MK_Q4) {
     const uint32_t ko = (lr >> 2) * (9 * HD) + (lr & 3) * (HD / 2) + lg * (HD / 8), so = (lr >> 2) * (9 * HD) + 8 * HD + 2 * ((lr & 3) * (HD / 32) + lg * HD / 128);
@@ -325,8 +326,8 @@ __device__ __forceinline__ void load_k(const KvAttnArgs &a, const Head &h, const
 // records) cover all banks
 template <int HD>
 __device__ __forceinline__ int vsw(int x) { return HD == 128 ? 2 * ((x & 3) | (x >> 1 & 4)) : 2 * ((x >> 1 & 1) | (x >> 2 & 2)); }
-template <int HD, int KIND>
-__device__ __forceinline__ void load_v(const KvAttnArgs &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t, uint16_t *buf) {
+template <int HD, int KIND, typename A>
+__device__ __forceinline__ void load_v(const A &a, const Head &h, const Span &s, int tile, int lane, Tile<HD, KIND> &t, uint16_t *buf) {
   const int lr = lane & 15, lg = lane >> 4;
   if constexpr (KIND == MK_Q4) {
     const uint32_t vo = lg * (9 * HD) + 4 * HD + lr * (HD / 4), so = lg * (9 * HD) + 8 * HD + HD / 2;
@@ -393,7 +394,13 @@ constexpr int few_lds() {   // bytes: V's tiles, then the waves' sums
   return tiles > out ? tiles : out;
 }
 template <int T> using few_cols = float[kFewWaves][T == RT_F32 ? 8 : 16];   // the waves' maxima, sums
-template <int HD, int KIND, int T, bool PRE = false, bool JOIN = false>   // (of the body)
+#define KV_OWN 0
+#define KV_SPAN(t) s
+#define KV_HEAD(t) h
+#define KV_MEM(t) a
+#define KV_TILE(t) (t)
+#define KV_P(t) P
+template <int HD, int KIND, int T, bool PRE = false, bool JOIN = false, bool ALL = false>   // (of the body)
 __global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few(Args<PRE> a) {
   __shared__ __align__(16) uint8_t sm[few_lds<HD, KIND, T>()];
   __shared__ few_cols<T> wm, wl;
@@ -408,13 +415,47 @@ __device__ __forceinline__ X &lds() {
 }
 // the same within a kernel that has other work beside it (PRE: over a common prefix; below) and LDS bytes for either.  (The arguments by value and LDS by its
 // name: by reference that kernel spills)
-template <int HD, int KIND, int T, bool PRE, int LDS, bool JOIN = true>
+template <int HD, int KIND, int T, bool PRE, int LDS, bool JOIN = true, bool ALL = false>
 __device__ __forceinline__ void few_tokens(Args<PRE> a, int split, int gc, int b) {
   auto &sm = lds<uint8_t[LDS]>();
   auto &wm = lds<few_cols<T>, 0>(), &wl = lds<few_cols<T>, 1>();
   if constexpr (PRE) a.window = a.sinks = a.paired = 0;
 #include "kv_few.inc"
 }
+
+#undef KV_OWN
+#undef KV_SPAN
+#undef KV_HEAD
+#undef KV_MEM
+#undef KV_TILE
+#undef KV_P
+// A sequence's columns over a common prefix's tiles and then its own, without sums to be joined: a launch and their way through memory are saved, and the prefix is read for each
+// sequence anew (kv_prefix_plan).  4 samples behind 700 positions 9.5 -> 8.9 us, 53 sequences of 3 tokens behind 37 13.2 -> 5.6
+#define KV_OWN own
+#define KV_SPAN(t) ((t) < own ? pspan : s)
+#define KV_HEAD(t) ((t) < own ? phead : h)
+#define KV_MEM(t) ((t) < own ? mp : mo)
+#define KV_TILE(t) ((t) < own ? (t) : (t) - own)
+#define KV_P(t) ((t) < own ? live ? pspan.PB : -1 : P)
+struct KvMem { int64_t ctx, crow; };
+template <int HD, int KIND, int T, bool PRE = false, bool JOIN = false, bool ALL = true>
+__global__ __launch_bounds__(kFewWaves * 64, kFewOcc) void k_kv_few_all(Args<PRE> a, KvPreArgs pre) {
+  __shared__ __align__(16) uint8_t sm[few_lds<HD, KIND, T>()];
+  __shared__ few_cols<T> wm, wl;
+  a.window = a.sinks = a.paired = 0;
+  const Span pspan = prefix_span_of(pre);
+  const int own = pspan.nt;   // the first of the own tiles
+  const KvMem mp{pre.ctx, pre.crow}, mo{a.ctx, a.crow};
+  const int split = 0, gc = blockIdx.y, b = blockIdx.z;
+  const Head phead = head_of<HD, KIND>(pre, 0, a.nchunk == 1 ? gc : gc / (uint32_t)a.nchunk);
+#include "kv_few.inc"
+}
+#undef KV_OWN
+#undef KV_SPAN
+#undef KV_HEAD
+#undef KV_MEM
+#undef KV_TILE
+#undef KV_P
 
 // The splits' sums of one row a workgroup: 256 threads, HD / 4 of them side by side over the dims, the others over the
 // splits.  M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L.  Bound by latency: 3.9 us for 28 rows of 64 splits, 2.4 of them the
@@ -746,11 +787,20 @@ size_t kv_prefix_plan(KvAttnArgs &a, KvPreArgs &p) {
   kv_attn_plan(p, true);
   if (!p.many && (a.many || few_blocks(p) > 512)) { p.few = 0; kv_attn_plan(p, true); }   // (few columns of either: one launch of k_kv_few's workgroups, two a CU)
   if (p.many && !a.many && a.nchunk > 1 && few_blocks(a) > 512) { a.few = 0; kv_attn_plan(a, true); }
+  // Few positions of both: each workgroup takes all that its columns see, and nothing is left to be joined.  24 tiles of both 22.5 us for 19.0, 11 10.5 for 7.9, 4 8.1 for 4.5; with 128 dims
+  // 27 9.9 for 12.9 and 30 9.5 for 10.6, with 64 30 8.5 for 7.9 and 43 9.2 for 11.7
+  const int64_t tiles = (p.ctx + kFewTile - 1) / kFewTile + (a.ctx + kFewTile - 1) / kFewTile;
+  if (!p.many && tiles <= (a.hd == 64 ? 4 : 3) * kFewWaves && few_blocks(a) / a.nsplit <= 512) {
+    p.nsplit = 0;   // (says so to the launch)
+    return 0;
+  }
   p.paired = 0;   // (every column sees all: nothing to even out)
   if (p.many && !a.many && !few_apart(a)) a.nsplit = std::max(1, a.nsplit / 2);   // (one workgroup a CU beside the others: 32 sequences behind 8190 positions 38.4 us for 35.2)
   a.one_tiles = p.one_tiles = -(a.nsplit + p.nsplit);
   return (size_t)a.nseq * a.n * a.heads * slots_of<true>(a) * (a.hd + 2) * 4;
 }
+template <int HD, int T> static constexpr auto k_all4 = k_kv_few_all<HD, MK_Q4, T>;
+template <int HD, int T> static constexpr auto k_all16 = k_kv_few_all<HD, MK_F32, T>;
 template <int HD, int T> static constexpr auto k_own4 = k_kv_few<HD, MK_Q4, T, false, true>;
 template <int HD, int T> static constexpr auto k_own16 = k_kv_few<HD, MK_F32, T, false, true>;
 template <int HD, int T> static constexpr auto k_few_few4 = k_kv_both_few<HD, MK_Q4, T>;
@@ -761,6 +811,12 @@ template <int HD, int T> static constexpr auto k_many_many4 = k_kv_both_many<HD,
 template <int HD, int T> static constexpr auto k_many_many16 = k_kv_both_many<HD, MK_F32, T, true>;
 hipError_t launch_kv_prefix(const KvAttnArgs &a, const KvPreArgs &p, hipStream_t st) {
   hipError_t e;
+  if (p.nsplit == 0) {
+    const dim3 grid(1, a.nkv * a.nchunk, a.nseq);
+    if (p.kind == MK_Q4) QPH_KVN(k_all4, p.hd, p.q.type, grid, kFewWaves * 64, a, p);
+    else QPH_KVN(k_all16, p.hd, p.q.type, grid, kFewWaves * 64, a, p);
+    return hipGetLastError();
+  }
   const bool q4 = p.kind == MK_Q4, apart = p.many && !a.many && few_apart(a);
   const int64_t all = (int64_t)p.nsplit * p.nkv * p.nchunk + (apart ? 0 : few_blocks(a)), width = std::min(all, (int64_t)1 << kWideLog2);
   KvAttnArgs own = a;

@@ -128,11 +128,13 @@ def test_attention_prefix():
     for scale in (-1.0, float("inf"), float("nan"), 3e38):
         refused(attend(scale=scale), "scale")
     c, p = cache(), cache(nseq=1)
+    assert size(lib().qph_kv_attention_prefix_work, C.byref(c), C.byref(p), qa.QPH_F16, 4, 3) == 0   # few positions: nothing to be joined
+    p = cache(nseq=1, ctx=5000)
     need = size(lib().qph_kv_attention_prefix_work, C.byref(c), C.byref(p), qa.QPH_F16, 4, 3)
     assert need >= 2 * 3 * 4 * 2 * 66 * 4   # two sums of a row at least
-    refused(attend(size=need - 1), "qph_kv_attention_prefix_work")
-    refused(attend(work=None), "qph_kv_attention_prefix_work")
-    refused(attend(work=P + 4), "qph_kv_attention_prefix_work")
+    refused(attend(p=p, size=need - 1), "qph_kv_attention_prefix_work")
+    refused(attend(p=p, work=None), "qph_kv_attention_prefix_work")
+    refused(attend(p=p, work=P + 4), "qph_kv_attention_prefix_work")
     assert attend(n=0) == 0 and size(lib().qph_kv_attention_prefix_work, C.byref(c), C.byref(p), qa.QPH_F16, 4, 0) == 0
     refused(lib().qph_kv_attention_prefix_work(C.byref(c), C.byref(p), qa.QPH_Q8, 4, 3, C.byref(C.c_int64())), "type of q")
 

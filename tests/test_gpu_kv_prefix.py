@@ -47,10 +47,11 @@ def test_prefix(kind, hd, G, rep, n, L, pasts, lens, type, route):
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
 @pytest.mark.parametrize("n", [1, 30])
-def test_lengths_of_the_prefix(kind, n, route):
+@pytest.mark.parametrize("ctx", [300, 1500])   # (of few positions a workgroup takes all, of more their sums are joined: here and below)
+def test_lengths_of_the_prefix(kind, n, ctx, route):
     """none, negative (none), past the cache's end (all of it), not given (all of it); a length that changes between replays"""
     gen = torch.Generator().manual_seed(3)
-    G, rep, D, ctx = 2, 4, 64, 300
+    G, rep, D = 2, 4, 64
     p, K0, V0 = filled(kind, 1, G, D, ctx, [ctx], gen)
     c, K, V = filled(kind, 2, G, D, 100, [70, 70], gen)
     q, pos = torch.randn(2, n, G * rep, D, generator=gen).half().cuda(), i32([70 - n, 12])
@@ -77,9 +78,10 @@ def test_lengths_of_the_prefix(kind, n, route):
 @pytest.mark.parametrize("kind", ["q4", "f16"])
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n", [1, 21])
-def test_strides_absent_sequences_over_q_and_padding(kind, type, n, route):
+@pytest.mark.parametrize("L", [400, 1100])
+def test_strides_absent_sequences_over_q_and_padding(kind, type, n, L, route):
     gen = torch.Generator().manual_seed(8)
-    S, G, rep, D, L = 6, 2, 4, 64, 400
+    S, G, rep, D = 6, 2, 4, 64
     ctx = 120
     pasts, lens = [100 - n, 7, -1, 40, ctx - n // 2, ctx], [n, max(1, n // 2), n, 0, n, n]
     T = [min(ctx, max(0, a) + m) if a >= 0 else 0 for a, m in zip(pasts, lens)]
@@ -110,13 +112,14 @@ def test_strides_absent_sequences_over_q_and_padding(kind, type, n, route):
 
 
 @pytest.mark.parametrize("kind", ["q4", "f16"])
-def test_unseen_memory_and_not_finite_values(kind, route):
+@pytest.mark.parametrize("room", [200, 1300])
+def test_unseen_memory_and_not_finite_values(kind, room, route):
     """NaN behind the prefix and behind the tokens changes nothing; one in the prefix reaches every sequence"""
     gen = torch.Generator().manual_seed(4)
     G, rep, D, L = 1, 4, 128, 77
-    p, K0, V0 = filled(kind, 1, G, D, 200, [L], gen)
+    p, K0, V0 = filled(kind, 1, G, D, room, [L], gen)
     c, K, V = filled(kind, 3, G, D, 64, [20, 20, 20], gen)
-    bad = torch.full((1, 200 - L, G, D), math.nan, device="cuda")
+    bad = torch.full((1, room - L, G, D), math.nan, device="cuda")
     p.write(bad, bad, i32([L]))
     bad = torch.full((3, 44, G, D), math.inf, device="cuda")
     c.write(bad, bad, i32([20] * 3))
@@ -134,18 +137,19 @@ def test_unseen_memory_and_not_finite_values(kind, route):
     assert bool(torch.isnan(out[..., dims]).all()) and bool(torch.isfinite(out[..., ~dims]).all())
 
 
-def test_loud_prefix_and_loud_own_positions():
+@pytest.mark.parametrize("room", [50, 1100])
+def test_loud_prefix_and_loud_own_positions(room):
     """one part's scores far above the other's: its weights are all there is, and nothing overflows"""
     gen = torch.Generator().manual_seed(5)
     D, L = 64, 50
     for mine, theirs in ((40., 0.1), (0.1, 40.)):
-        p, c = qa.KvCache("f16", 1, 1, D, L), qa.KvCache("f16", 1, 1, D, 10)
+        p, c = qa.KvCache("f16", 1, 1, D, room), qa.KvCache("f16", 1, 1, D, 10)
         k0, v0, k, v = (torch.randn(1, m, 1, D, generator=gen).half() for m in (L, L, 10, 10))
         k0, k = k0 * theirs, k * mine
         p.write(k0.cuda(), v0.cuda(), i32([0]))
         c.write(k.cuda(), v.cuda(), i32([0]))
         q = torch.randn(1, 1, 4, D, generator=gen).float().cuda()
-        out = c.attention(q, i32([9]), prefix=p)
+        out = c.attention(q, i32([9]), prefix=p, prefix_len=i32([L]))
         check_rows(out[0], q[0], torch.cat([k0[0], k[0]]).double(), torch.cat([v0[0], v[0]]).double(), L + 9)
 
 
@@ -267,3 +271,23 @@ def test_more_workgroups_than_a_grid_is_wide(monkeypatch):
     others = torch.ones(S, dtype=torch.bool, device="cuda")
     others[some] = False
     assert bool((out[others] == 55).all())
+
+
+@pytest.mark.parametrize("kind", ["q4", "f16"])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_few_positions_of_both(kind, type, hd):
+    """up to and past the positions that a workgroup takes by itself: 32 tiles of 32 with 64 dims, 24 with 128"""
+    gen = torch.Generator().manual_seed(hd)
+    G, rep, n = 2, 3, 7
+    most = (32 if hd == 64 else 24) * 32
+    for L, ctx in ((1, 8), (31, 32), (33, 100), (most - 64, 33), (most - 33, 33), (most - 32, 33), (most - 200, 200)):
+        pasts, lens = [ctx - n, 0, 3], [n, 2, min(5, ctx - 3)]
+        p, K0, V0 = filled(kind, 1, G, hd, L, [L], gen)
+        c, K, V = filled(kind, 3, G, hd, ctx, [a + m for a, m in zip(pasts, lens)], gen)
+        q = torch.randn(3, n, G * rep, hd, generator=gen).to(TYPES[type]).cuda()
+        out = torch.full_like(q, 55.)
+        c.attention(q, i32(pasts), lens=i32(lens), prefix=p, out=out)
+        for b, m in enumerate(lens):
+            check_rows(out[b, :m], q[b, :m], both(K0, K, L, b), both(V0, V, L, b), L + pasts[b])
+            assert bool((out[b, m:] == 55).all())
