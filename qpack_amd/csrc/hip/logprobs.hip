@@ -182,7 +182,7 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
   __shared__ LpSum sums[kLpWaves];
   constexpr int CAP = kLpKeep + GE;
   __shared__ int64_t entries[TOP ? kLpWaves : 1][TOP ? CAP : 1], joint[TOP ? kLpWaves * kLpKeep : 1];
-  __shared__ int count, bounds[kLpWaves];
+  __shared__ int count, kept, bounds[kLpWaves];
   const int64_t row = blockIdx.x / (uint32_t)a.splits;
   const int split = blockIdx.x - (int)row * a.splits;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -348,15 +348,15 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
       add_to(joint, &count, e < held && order_in(x) >= most, x, lane);
     }
     __syncthreads();
-    if (count > 2 * kLpTop) {   // (where four lists of many are left)
+    int n = count;
+    if (n > 2 * kLpTop) {   // (where four lists of many are left; count stays, so that all waves come here)
       if (wave == 0) {
-        int n = count;
         cut<kLpWaves * kLpKeep / 64>(joint, n, most, a.top, kLpTop + 16, lane);
-        if (lane == 0) count = n;
+        if (lane == 0) kept = n;
       }
       __syncthreads();
+      n = kept;
     }
-    const int n = count;
     auto put_at = [&](int k, int64_t x) {
       if (a.splits == 1) put_top(a, row, k, x, all.m, ls);
       else ((int64_t *)((LpSum *)a.work + a.rows * a.splits))[part * a.top + k] = x;

@@ -264,3 +264,15 @@ def test_what_reaches_the_first_bound_lies_in_the_second_load(type, top):
     few = qa.logprobs(x.cuda(), tokens.int().cuda(), top)
     for y in (qa.LogProbs(*(z[:6] for z in r)), qa.LogProbs(*(z[594:] for z in r)), few):
         check(y, x, tokens, top)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,top", [(1, 64), (9, 40), (1100, 64)])
+def test_four_lists_of_many(type, rows, top):
+    # every wave of a workgroup has more than a quarter of 128 of what reaches the common bound: all logits equal, or two values by turns of 1, 8 and 512
+    V = 9001
+    i = torch.arange(V)
+    x = torch.stack([torch.zeros(V), (i % 2).float(), (i // 8 % 2).float(), (i // 512 % 2).float(), torch.where(i > 4000, 2., 1.)]).repeat((rows + 4) // 5, 1)[:rows].to(TYPES[type])
+    tokens = torch.arange(rows) * 977 % V
+    for _ in range(3):
+        check(qa.logprobs(x.cuda(), tokens.int().cuda(), top), x, tokens, top)
