@@ -291,7 +291,9 @@ __global__ __launch_bounds__(kLpWaves * 64) void k_logprobs(LogprobArgs a) {
             held += __popcll(m);
           }
         }
-        last = value_of(max(bound - 2, order_of(-INFINITY)));   // (what passes is at the bound too, and at 0 both zeros)
+        // The value just below the bound: what passes reaches it (-0 has 0's place: below 0 is the largest negative one).  Not any lower, since a cut keeps what reaches the bound: of a
+        // load full of logits one step below it none would be left, and the next load's at the bound would not pass
+        last = value_of(max(bound - (bound ? 1 : 2), order_of(-INFINITY)));
       }
       if ((held <= full) & !__any(bm > last)) return;
 #pragma unroll

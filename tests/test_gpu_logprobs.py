@@ -276,3 +276,38 @@ def test_four_lists_of_many(type, rows, top):
     tokens = torch.arange(rows) * 977 % V
     for _ in range(3):
         check(qa.logprobs(x.cuda(), tokens.int().cuda(), top), x, tokens, top)
+
+
+@pytest.mark.parametrize("below", [1.0, -1.0, 0.0, -2.0 ** -149, 2.0 ** -149, 12345.678])
+@pytest.mark.parametrize("top", [1, 5, 20, 64])
+def test_plateaus_one_step_below_the_first(below, top):
+    # a wave's loads are 256 logits, 1024 apart; its first bound is what `top` of the lanes' largest of two loads reach.  Much of every row is one step of fp32 below those
+    below = torch.tensor(below)
+    up = torch.nextafter(below, torch.tensor(math.inf))
+    V = 6144
+    i = torch.arange(V)
+    gen = torch.Generator().manual_seed(top)
+    x = below.repeat(10, V)
+    x[0, 1029] = up                                               # the only one, in the second load
+    x[1, 1024:1024 + 4 * (top + 3):4] = up                        # a lane each, all of them in the second load
+    x[2, :4 * (top // 2):4] = up                                  # fewer than top in the first load, the others in the second
+    x[2, 1024:1024 + 4 * (top - top // 2 + 1):4] = up
+    x[3] = torch.where(i < 40, below, torch.nextafter(below, torch.tensor(-math.inf)))   # 40 one step below, the others two
+    x[3, 1024] = up
+    x[4] = torch.where(torch.rand(V, generator=gen) < 0.002, up, below)
+    x[5] = torch.where(torch.rand(V, generator=gen) < 0.5, up, below)
+    x[6, 5000:] = up                                              # past both loads
+    x[7] = torch.where(i % 2 == 0, below, -below)
+    x[7, 1300] = torch.nextafter(below.abs(), torch.tensor(math.inf))
+    x[8] = torch.where(i < 1024, below, torch.nextafter(up, torch.tensor(math.inf)))
+    x[8, 2048:] = -math.inf
+    x[9] = torch.where(i < 2048, below, up)
+    tokens = torch.tensor([1029, 0, 1024, 1024, 7, 8, 6143, 1300, 1024, 2048])
+    wide = torch.cat([below.repeat(10, 128256 - V - 2100), x, below.repeat(10, 2100)], -1)   # shares of several units, what matters in the last ones
+    whole = below.repeat(10, 40000)
+    whole[:, :V] = x
+    for y, t in ((x[:, :4096], tokens.clamp(max=4095)), (x, tokens), (whole, tokens), (wide, tokens + 128256 - V - 2100)):
+        for some in (slice(0, 1), slice(2, 3), slice(0, 10)):   # (rows alone, too: other shares)
+            check(qa.logprobs(y[some].cuda(), t[some].int().cuda(), top), y[some], t[some], top)
+    r = qa.logprobs(x.repeat(103, 1).cuda(), tokens.repeat(103).int().cuda(), top)   # (as many rows as take no shares)
+    check(qa.LogProbs(*(z[1020:] for z in r)), x, tokens, top)
