@@ -99,7 +99,8 @@ bool stream_of(int64_t device, void **st) {
   *st = PyLong_AsVoidPtr(v);
   return !PyErr_Occurred();
 }
-// runs f on the tensors' device; a switch only where another one is current
+// runs f on the tensors' device; a switch only where another one is current.  f does not throw, which would leave the switch in place: tensors say where their
+// memory is (functorch's, without storage, throw) before
 bool current(int64_t device, bool *yes) {
   Ref now(PyObject_CallNoArgs(g_device));
   if (!now.p) return false;
@@ -256,11 +257,12 @@ PyObject *copy(PyObject *self, PyObject *const *arg, Py_ssize_t na) try {
   const int64_t n = x->size(1);
   if (n > INT32_MAX) { fail("kv: too many tokens%s%s", ""); return nullptr; }
   const int *at = n ? (const int *)x->data_ptr() : (const int *)16;
+  const int64_t stride = x->stride(0);
   if (qph_kv_copy_work(&c->c, &src->c, (int)n, apart, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
   at::Tensor work;
   void *w;
   if (!scratch(c, bytes, &work, &w)) return nullptr;
-  if (!launch(c->device, [&](void *st) { return qph_kv_copy(&c->c, &src->c, at, x->stride(0), (int)n, pos, lens, seqs, apart, w, bytes, st); })) return nullptr;
+  if (!launch(c->device, [&](void *st) { return qph_kv_copy(&c->c, &src->c, at, stride, (int)n, pos, lens, seqs, apart, w, bytes, st); })) return nullptr;
   for (PyObject *y : {c->data, c->data_v})
     if (y) written(THPVariable_Unpack(y));
   Py_RETURN_NONE;
@@ -285,6 +287,9 @@ PyObject *logprobs(PyObject *, PyObject *const *arg, Py_ssize_t na) try {
     return nullptr;
   }
   if (tok && (!tok->is_cuda() || tok->get_device() != device)) { fail("logprobs: tokens are not on the logits' device%s%s", ""); return nullptr; }
+  const void *from, *ids;
+  try { from = x->data_ptr(); ids = tok ? tok->data_ptr() : nullptr; }
+  catch (...) { fail("logprobs: logits and tokens must be plain tensors%s%s", ""); return nullptr; }
   int64_t bytes = 0;
   if (qph_logprobs_work(type, rows, (int)x->size(1), top, &bytes) != 0) { fail("%s%s", qph_last_error()); return nullptr; }
   // the results side by side in one allocation, each from a multiple of 64 bytes on (an allocation each takes as long as the rest of the call)
@@ -303,10 +308,12 @@ PyObject *logprobs(PyObject *, PyObject *const *arg, Py_ssize_t na) try {
   if (tok) { logp = part(at::kFloat, {rows}, one); rank = part(at::kInt, {rows}, one); }
   at::Tensor ti = part(at::kInt, {rows, top}, list), tl = part(at::kFloat, {rows, top}, list);
   if (bytes) work = at::empty({(bytes + 3) / 4}, f32);
-  auto at = [](at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+  void *to[6], **next = to;
+  for (const at::Tensor *t : {&logp, &entropy, &rank, &ti, &tl, &work}) *next++ = t->defined() ? t->data_ptr() : nullptr;
+  const int vocab = (int)x->size(1);
+  const int64_t ld = x->stride(0);
   if (!launch(device, [&](void *st) {
-        return qph_logprobs(x->data_ptr(), type, rows, (int)x->size(1), x->stride(0), tok ? (const int *)tok->data_ptr() : nullptr, top, (float *)at(logp), (float *)at(entropy), (int *)at(rank),
-                            (int *)at(ti), (float *)at(tl), at(work), bytes, st);
+        return qph_logprobs(from, type, rows, vocab, ld, (const int *)ids, top, (float *)to[0], (float *)to[1], (int *)to[2], (int *)to[3], (float *)to[4], to[5], bytes, st);
       }))
     return nullptr;
   PyObject *out = PyTuple_New(5);

@@ -311,3 +311,35 @@ def test_plateaus_one_step_below_the_first(below, top):
             check(qa.logprobs(y[some].cuda(), t[some].int().cuda(), top), y[some], t[some], top)
     r = qa.logprobs(x.repeat(103, 1).cuda(), tokens.repeat(103).int().cuda(), top)   # (as many rows as take no shares)
     check(qa.LogProbs(*(z[1020:] for z in r)), x, tokens, top)
+
+
+def test_refused_where_another_device_is_current():
+    """tensors without memory of their own (functorch's) while another device is current: refused, and that device stays current"""
+    from qpack_amd import kvcache
+
+    class Guard:   # as torch.cuda.device of the tensors' device, entered from another one
+        inside = entered = 0
+
+        def __init__(self, device):
+            assert device == 0
+
+        def __enter__(self):
+            Guard.inside += 1
+            Guard.entered += 1
+
+        def __exit__(self, *error):
+            Guard.inside -= 1
+
+    x, t = torch.randn(3, 2, 700, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    kvcache._binding().setup(qa.QphError, torch._C._cuda_getCurrentRawStream, lambda: 1, Guard)
+    try:
+        there = qa.logprobs(x[0], t[0], 3)
+        assert Guard.entered == 1 and Guard.inside == 0
+        for call in (lambda: torch.func.vmap(lambda y: qa.logprobs(y))(x), lambda: torch.func.vmap(lambda u: qa.logprobs(x[0], u))(t)):
+            with pytest.raises(qa.QphError, match="plain tensors"):
+                call()
+            assert Guard.inside == 0
+    finally:
+        kvcache._bind = None
+        kvcache._binding()
+    check(there, x[0], t[0], 3)
