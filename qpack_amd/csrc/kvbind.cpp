@@ -37,10 +37,20 @@ bool fail(const char *fmt, const char *a, const char *b = "") {
   PyErr_Format(g_error, fmt, a, b);
   return false;
 }
+// whether t, whose autograd data m is, has a forward-mode tangent.  Its own question takes a lock and, of a view, its base's: asked only where one of them had a tangent
+// (three views a call: 0.1 us of 3.7)
+bool tangent(const at::Tensor &t, const torch::autograd::AutogradMeta *m) {
+  const auto may_have = [](const torch::autograd::AutogradMeta *x) { return x && x->fw_grad_; };
+  const auto *v = m->is_view_ ? static_cast<const torch::autograd::DifferentiableViewMeta *>(m) : nullptr;
+  return (may_have(m) || (v && v->has_fw_view() && may_have(torch::autograd::impl::get_autograd_meta(v->get_forward_view().base_)))) && t._fw_grad(0).defined();
+}
 bool tensor(PyObject *x, const char *name, const at::Tensor **t, const char *call = "kv") {
   if (!THPVariable_Check(x)) return fail("%s: %s must be a tensor", call, name);
   *t = &THPVariable_Unpack(x);
-  if ((*t)->requires_grad() && c10::GradMode::is_enabled()) return fail("%s: %s requires a gradient, and no call here passes one on: detach it, or call under torch.no_grad()", call, name);
+  const torch::autograd::AutogradMeta *m = torch::autograd::impl::get_autograd_meta(**t);   // (plain tensors have none)
+  if (!m) return true;
+  if (m->requires_grad() && c10::GradMode::is_enabled()) return fail("%s: %s requires a gradient, and no call here passes one on: detach it, or call under torch.no_grad()", call, name);
+  if (tangent(**t, m)) return fail("%s: %s has a forward-mode tangent, and no call here passes one on: take unpack_dual's primal", call, name);
   return true;
 }
 bool tensor(const Cache *c, PyObject *x, const char *name, const at::Tensor **t) {   // on the cache's device

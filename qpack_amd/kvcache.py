@@ -41,7 +41,7 @@ class KvCache:
     0 and positions at or past ctx take no part.  pos and lens: int32 tensors [nseq] on the cache's device.
 
     Writes to one cache follow each other: from several streams they need events between them.  Nothing here carries
-    gradients: tensors that require one are refused while gradients are recorded."""
+    gradients: tensors that require one are refused while gradients are recorded, and those with a forward-mode tangent."""
 
     def __init__(self, kind, nseq, kv_heads, head_dim, ctx, data=None, device="cuda"):
         import torch
@@ -73,6 +73,8 @@ class KvCache:
             tensors, at = (k, v), (k.data_ptr(), v.data_ptr(), *_strides(k))
         if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
             raise QphError("kv: the cache's data requires a gradient, and no call here passes one on")
+        if any(torch.autograd.forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+            raise QphError("kv: the cache's data has a forward-mode tangent, and no call here passes one on")
         first = tensors[0]
         if first.device.type != "cuda":
             raise QphError("kv: the cache must be on a GPU")

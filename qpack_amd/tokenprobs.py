@@ -11,6 +11,6 @@ def logprobs(logits, tokens=None, top=0):
 
     A token outside the vocabulary has logp NaN and rank -1; without tokens logp and rank are None.  top <= 64.  Of equal logits the lower index
     comes first.  Logits of -inf have probability 0; a row with a NaN or +inf, or of -inf alone, has NaN results.  Nothing here carries gradients: logits that
-    require one are refused while gradients are recorded.  The results lie side by side in one allocation."""
+    require one are refused while gradients are recorded, and those with a forward-mode tangent.  The results lie side by side in one allocation."""
     from .kvcache import _binding
     return LogProbs(*_binding().logprobs(logits, tokens, top))

@@ -68,3 +68,28 @@ def test_a_binding_that_is_not_built_is_named(monkeypatch):
     monkeypatch.delattr(qa, "_kvbind", raising=False)
     with pytest.raises(qa.QphError, match="was not built"):
         kvcache._binding()
+
+
+def test_tangents_are_refused():
+    """forward mode: of what is read, of what is written and of the cache's own memory; also where no gradients are recorded, which leaves forward mode on"""
+    from qpack_amd.kvcache import _binding
+    from torch.autograd import forward_ad
+    c, x, pos, t = bound(), torch.zeros(2, 3, 2, 64), torch.zeros(2, dtype=torch.int32), torch.zeros(9, 32)
+    calls = [lambda a: c.write(a, x, pos, None), lambda a: c.read(a, x, pos, None), lambda a: c.attention(a, x, pos, None, 0, 0, 0.0), lambda a: c.attention(a, a, pos, None, 0, 0, 0.0),
+             lambda a: c.append(a, x, x, x, pos, None, t, t, None, None, None, 1e-6), lambda a: c.attention_prefix(a, x, pos, None, 0.0, c, None), lambda a: _binding().logprobs(a[0, 0], None, 0)]
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in calls:
+            for a in (d, d * 2, d[:, :2]):
+                with pytest.raises(qa.QphError, match="tangent"):
+                    f(a)
+                with torch.no_grad(), pytest.raises(qa.QphError, match="tangent"):
+                    f(a)
+            with pytest.raises(qa.QphError, match="device|GPU"):   # taken as far as that
+                f(forward_ad.unpack_dual(d).primal)
+        memory = forward_ad.make_dual(f16(3, 40, 2, 64), f16(3, 40, 2, 64))
+        for k, v in ((f16(3, 40, 2, 64), memory), (memory, f16(3, 40, 2, 64))):
+            with pytest.raises(qa.QphError, match="tangent"):
+                cache(k, v, 3, 2, 64, 40)
+    with pytest.raises(qa.QphError, match="device|GPU"):
+        calls[0](d)
