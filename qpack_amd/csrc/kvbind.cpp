@@ -81,6 +81,8 @@ bool rows(const Cache *c, PyObject *x, const char *name, qph_rows *r, int64_t *n
   if (*n == 0 && !r->p) r->p = (void *)16;   // a tensor without elements may have no memory: nothing of it is read
   return true;
 } catch (...) { return fail("kv: %s is not a plain tensor%s", name); }   // (nested or fake ones: torch throws)
+// a tensor whose memory was given back would be NULL, and so taken as not given
+bool there(const at::Tensor &t, const void *p, const char *name) { return p || !t.numel() || fail("kv: %s has no memory%s", name); }
 bool index(const Cache *c, PyObject *x, const char *name, const int **p, bool may_lack = false, int64_t n = -1) try {   // int32 [n], or [nseq]; None: NULL
   if (n < 0) n = c->c.nseq;
   if (x == Py_None && may_lack) { *p = nullptr; return true; }
@@ -91,7 +93,7 @@ bool index(const Cache *c, PyObject *x, const char *name, const int **p, bool ma
     return false;
   }
   *p = (const int *)t->data_ptr();
-  return true;
+  return there(*t, *p, name);
 } catch (...) { return fail("kv: %s is not a plain tensor%s", name); }
 // float32, contiguous, of these sizes (last < 0: any); None: NULL
 bool floats(const Cache *c, PyObject *x, const char *name, int64_t dims, int64_t last, const float **p, const at::Tensor **t) try {
@@ -100,7 +102,7 @@ bool floats(const Cache *c, PyObject *x, const char *name, int64_t dims, int64_t
   if ((*t)->scalar_type() != at::kFloat || (*t)->layout() != at::kStrided || (*t)->dim() != dims || (last >= 0 && (*t)->size(dims - 1) != last) || !(*t)->is_contiguous())
     return fail("kv: %s must be a contiguous float32 tensor %s", name, dims == 1 ? "[head_dim]" : "[places, half the rotated dims], cos and sin alike");
   *p = (const float *)(*t)->data_ptr();
-  return true;
+  return there(**t, *p, name);
 } catch (...) { return fail("kv: %s is not a plain tensor%s", name); }
 bool stream_of(int64_t device, void **st) {
   Ref d(PyLong_FromLongLong(device));

@@ -257,3 +257,26 @@ def test_refusals():
     refused("eps", eps=math.inf)
     refused("eps", eps=math.nan)
     assert c.append(**{**ok, "q": q[:, :0], "k": k[:, :0], "v": k[:, :0]}).shape == (2, 0, 4, 64)
+
+
+def test_optional_tensors_without_memory_are_refused():
+    """what may be left out and was given back (its storage resized to nothing) is not taken as left out: lens, at, norms' weights, a prefix's length, a copy's sequences"""
+    def gone(x):
+        x.untyped_storage().resize_(0)
+        return x
+
+    one, ones = lambda *s: torch.ones(*s, device="cuda"), lambda: gone(torch.ones(2, dtype=torch.int32, device="cuda"))   # noqa: E731
+    c, prefix = qa.KvCache("f16", 2, 1, 64, 40), qa.KvCache("f16", 1, 1, 64, 8)
+    x, pos, t = one(2, 1, 1, 64), i32([3, 4]), one(50, 32)
+    index = i32([[0], [0]])
+    for name, call in (("q_weight", lambda: c.append(x, x, x, pos, t, t, q_weight=gone(one(64)))), ("k_weight", lambda: c.append(x, x, x, pos, t, t, k_weight=gone(one(64)))),
+                       ("at", lambda: c.append(x, x, x, pos, t, t, at=ones())), ("lens", lambda: c.append(x, x, x, pos, t, t, lens=ones())), ("pos", lambda: c.append(x, x, x, ones(), t, t)),
+                       ("cos", lambda: c.append(x, x, x, pos, gone(one(50, 32)), t)), ("lens", lambda: c.attention(x, pos, lens=ones())), ("lens", lambda: c.write(x, x, pos, lens=ones())),
+                       ("prefix_len", lambda: c.attention(x, pos, prefix=prefix, prefix_len=gone(torch.ones(1, dtype=torch.int32, device="cuda")))),
+                       ("seqs", lambda: c.copy(index, pos, seqs=ones()))):
+        with pytest.raises(qa.QphError, match=f"{name} has no memory"):
+            call()
+    assert not bool(c.data[0].any())
+    empty = one(50, 0)
+    assert torch.equal(c.append(x, x, x, pos, empty, empty), x)   # (nothing to turn: tables without elements are as good as any)
+    assert torch.equal(c.data[0][0, 3, 0].float(), x[0, 0, 0])
