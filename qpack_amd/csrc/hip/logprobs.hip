@@ -53,11 +53,6 @@ __device__ __forceinline__ float lp_elem(u32x4 w, int i) {
     return __builtin_bit_cast(float, i & 1 ? u & 0xffff0000u : u << 16);
   }
 }
-template <int T>
-__device__ __forceinline__ float lp_load(const void *p, int64_t i) {
-  if constexpr (T == RT_F32) return ((const float *)p)[i];
-  else { const uint16_t h = ((const uint16_t *)p)[i]; return T == RT_F16 ? half_bits_to_float(h) : bf16_to_f(h); }
-}
 // an element by a scalar load (16 bits: of the 4 bytes that it lies in)
 typedef const int __attribute__((address_space(4))) scalar_int;
 template <int T>
