@@ -625,7 +625,7 @@ void HipLlama::step(int tok, int want, float *out) {
 
 void HipLlama::prefill(const int *toks, int n, int want, float *out) {
   if (n <= 0) return;
-  if (pos_ + n > ctx_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
+  if (n > ctx_ - pos_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
   for (int i = 0; i < n; i++) if (toks[i] < 0 || toks[i] >= cfg_.vocab) throw std::runtime_error("token id out of range");
   const bool force_steps = getenv("QPH_PREFILL_STEPS") != nullptr;   // test hook: the decode-step path
   if (n == 1 || force_steps) {   // one token: the reference's n == 1 case
@@ -839,7 +839,7 @@ void HipLlama::score_rows(const float *logits, int at, int rows, const Scoring &
 void HipLlama::score(const int *toks, const int *targets, int n, int top, const ScoreOut &out) {
   if (top < 0 || top > std::min(kLpTop, cfg_.vocab)) throw std::runtime_error("score: top must be in [0, min(64, vocab)]");
   if (n <= 0) return;
-  if (pos_ + n > ctx_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
+  if (n > ctx_ - pos_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
   for (int i = 0; i < n; i++) if (toks[i] < 0 || toks[i] >= cfg_.vocab) throw std::runtime_error("token id out of range");
   std::vector<int> next;
   if (!targets) {
@@ -901,7 +901,7 @@ int HipLlama::greedy_run(int tok, int n, int *out) {
 // already take less than two steps (behind 600 positions 1103 against 1184 us on eight layers of the 8B shape, 1431 against
 // 1578 on the 0.5B one), a third one costs 30 us more instead of 590 and 780.
 void HipLlama::prefill_all(const int *toks, int n, float *logits) {
-  if (pos_ + n > ctx_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
+  if (n > ctx_ - pos_) throw std::runtime_error("context window full (" + std::to_string(ctx_) + " tokens)");
   const bool batched = vf_ok_ && !order_ && !kv_custom() && !getenv("QPH_VERIFY_STEPS");   // test hook: decode steps
   for (int i = 0; i < n;) {
     int m = 0;   // tokens of this batch: valid ids, one regime

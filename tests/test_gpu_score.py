@@ -116,3 +116,18 @@ def test_refusals(synth):
         assert m.pos() == 0 and m.score([]).logp.shape == (0,)
         m.score([1] * 16)
         assert m.pos() == 16
+
+
+def test_a_text_of_2_31_tokens_does_not_fit(synth):
+    """its last position passes 32 bits: refused before any of its tokens is read"""
+    import ctypes as C
+
+    from qpack_amd._lib import lib
+    with qa.HipLlama.load(synth("mini"), max_ctx=16) as m:
+        m.prefill([1, 2, 3], 0)
+        tokens, out = (C.c_int * 4)(1, 2, 3, 4), (C.c_float * 1)()
+        at = C.cast(tokens, C.POINTER(C.c_int))
+        for call in (lambda n: lib().qph_score(m._h, at, None, n, 0, None, None, None, None, None), lambda n: lib().qph_prefill(m._h, at, n, 0, None), lambda n: lib().qph_prefill_all(m._h, at, n, out)):
+            for n in (2 ** 31 - 1, 2 ** 31 - 3, 14):
+                assert call(n) == -1 and b"context window full" in lib().qph_last_error()
+        assert m.pos() == 3
