@@ -603,7 +603,7 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a, KvJoin p) {
 // for 4-bit, 60 that expand; the 8 waves read 256 KiB of LDS, 2048 cycles at its 128 bytes a cycle.  The three overlap in part only:
 // 2048 tokens of 32 heads over a 4-bit cache 56 to 64 us by machine (620 TFLOP/s of the 1149 that a large fp16 product reaches), 4096
 // tokens with a window of 1024 in fp16 95 to 102 us; fp32 rows, with twice the products, 88 and 150 (over an fp16 cache the 128-dim kernel has all
-// 256 registers and spills 4).  256 columns a workgroup, since what a block costs to expand and its LDS writes are
+// 256 registers and spills 6).  256 columns a workgroup, since what a block costs to expand and its LDS writes are
 // shared by them: with 128 columns and two workgroups a CU the 4-bit prompt took 77 us for 64, the fp16 one 97 for 100, and 64
 // tokens each of 32 sequences 6 % more
 constexpr int kManyWaves = 8, kManyBlk = 64, kManyCols = 32 * kManyWaves;
@@ -788,7 +788,8 @@ size_t kv_prefix_plan(KvAttnArgs &a, KvPreArgs &p) {
   if (!p.many && (a.many || few_blocks(p) > 512)) { p.few = 0; kv_attn_plan(p, true); }   // (few columns of either: one launch of k_kv_few's workgroups, two a CU)
   if (p.many && !a.many && a.nchunk > 1 && few_blocks(a) > 512) { a.few = 0; kv_attn_plan(a, true); }
   // Few positions of both: each workgroup takes all that its columns see, and nothing is left to be joined.  24 tiles of both 22.5 us for 19.0, 11 10.5 for 7.9, 4 8.1 for 4.5; with 128 dims
-  // 27 9.9 for 12.9 and 30 9.5 for 10.6, with 64 30 8.5 for 7.9 and 43 9.2 for 11.7
+  // 27 9.9 for 12.9 and 30 9.5 for 10.6, with 64 30 8.5 for 7.9 and 43 9.2 for 11.7.  Like all of the plan it goes by the caches' room, since the host does not know what they hold: 53 sequences of 3 tokens
+  // at 50 behind 37 5.6 us with caches as long as that, 11.1 where the own ones have room for 4096 positions
   const int64_t tiles = (p.ctx + kFewTile - 1) / kFewTile + (a.ctx + kFewTile - 1) / kFewTile;
   if (!p.many && tiles <= (a.hd == 64 ? 4 : 3) * kFewWaves && few_blocks(a) / a.nsplit <= 512) {
     p.nsplit = 0;   // (says so to the launch)

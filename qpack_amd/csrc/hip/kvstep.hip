@@ -237,7 +237,8 @@ __global__ __launch_bounds__(256) void k_copy16(KvCopyArgs a) {
 // A workgroup has RECS records of one kv head, and a thread a position to look up.  Records that come from one whole record, as all but the last of a fork do, are
 // copied as they are, 16 bytes a thread.  Of others a wave has one: lanes 0 .. have 16 bytes of a position's K, lanes 32 .. four words of V, whose
 // 8 codes come from a word each of up to 8 records; V words that hold positions outside the call are merged.  Bound by HBM: 6001 positions of 8 heads of 128 dims
-// forked into 8 sequences, 62 MB, 12.3 us, 5.1 TB/s; where positions are picked, by the loads and shifts of up to 8 words a word: 4000 of 16384 of 16 sequences, 147 MB, 58.8 us
+// forked into 8 sequences, 62 MB, 12.3 us, 5.1 TB/s.  Where positions are picked too: a V word holds 8 positions, so nine tenths of the source's V are read for a quarter of its positions, 4000 of 16384 of 16 sequences some
+// 250 MB for 147 of what is picked and written, 48 of 58.8 us
 template <int HD, int STAGE, int RECS>
 __global__ __launch_bounds__(256) void k_copy4(KvCopyArgs a) {
   constexpr int P = 9 * HD / 16, NP = (RECS * P + 255) / 256;   // 16-byte pieces of a record, of a thread
@@ -350,7 +351,8 @@ static void launch_copy(int kind, const KvCopyArgs &a, hipStream_t st) {
     const int recs = (a.n + kRec - 1) / kRec + (STAGE == 1 ? 0 : 1);
     // A record a wave up to eight workgroups of two a wave a CU: of 4 sequences' 1000 positions picked from 4000 (8 heads of 128 dims) 5.6 us with one, 6.6 with two, 14.2 with eight; 250
     // forked into 32 6.0, 5.7 and 7.6.  Past them two, 4000 picked for each of 16 57.4, 58.7 and 71.6, but eight where the call names source sequences: they are forked or change
-    // places, in whole records as a rule, 6001 positions into 8 14.0, 12.3 and 12.1 (62.8 and 60.8 with the caches read back each time)
+    // places, in whole records as a rule, 6001 positions into 8 14.0, 12.3 and 12.1 (62.8 and 60.8 with the caches read back each time).  Positions
+    // that are picked from named sources lose by it: those 4000 70.7 for 58.0 (and 97 for 76 in fp16, whose loads past the caches go by the same)
     auto grid = [&](int each) { return dim3((unsigned)((recs + each - 1) / each), a.nkv, a.nseq); };
 #define QPH_COPY(RECS)                                                                                          \
   do {                                                                                                          \
